@@ -15,6 +15,10 @@
  * device memory; decode / GEMV / GEMM are enqueued on a caller stream
  * without host synchronisation, and errors are collected in a device status
  * word read back by xksv_plan_status().
+ *
+ * Parts 7 and 8 serve a model whose weights stay compressed (no counterpart
+ * in the reference): a linear layer on a plan's weights with its epilogue,
+ * and a paged key/value cache with the attention that reads it.
  */
 #ifndef XKSV_CUDA_H
 #define XKSV_CUDA_H
@@ -305,6 +309,161 @@ void xksv_tp_comm_destroy(void* comm);
 int xksv_tp_gemm(const xksv_plan* plan, const void* d_payload, size_t payload_size, const float* d_x,
                  size_t x_rows, float* d_y_shard, size_t rows_shard, float* d_y_full, size_t batch, void* comm,
                  void* stream);
+
+/* ---------------- Part 7: linear layer on compressed weights ------------ */
+/* No reference counterpart (the reference's GEMV takes one FP32 column and
+ * leaves bias, activation and residual to the caller, python/runtime.py:
+ * 264-284).  Element types of activations and caches: */
+enum { XKSV_BF16 = 1, XKSV_FP16 = 2, XKSV_FP32 = 3, XKSV_E4M3 = 4 };
+enum { XKSV_ACT_NONE = 0, XKSV_ACT_RELU = 1, XKSV_ACT_SILU = 2, XKSV_ACT_GELU = 3, XKSV_ACT_GELU_TANH = 4 };
+
+/* For every token b and every row r of Y that a slab covers:
+ *   z = sum_c W[r, c] x[b, x_offset + c] + bias[r]
+ *   y[b, r] = act(z) * mul[b, r] + residual[b, r]
+ * Rows of Y are y's columns (dst_offset + r of the slab, below y_cols);
+ * columns of Y that no slab covers are left as they were.  x is BF16
+ * [batch, x_cols], y BF16 or FP32 [batch, y_cols]; consecutive tokens are
+ * x_stride, y_stride, mul_stride and residual_stride elements apart (at
+ * least the columns; 2- or 4-byte aligned rows will do).  bias [y_cols], mul and
+ * residual [batch, y_cols] are BF16 or FP32, NULL when absent.  residual and
+ * mul may be y itself (same type and stride); no other buffers overlap y.
+ * GELU is z Phi(z); GELU_TANH its tanh form; SILU z / (1 + exp(-z)).  Sums,
+ * bias, activation, product and residual are FP32, rounded once into y. */
+typedef struct xksv_linear_args {
+  const void* x;
+  uint64_t x_cols, x_stride;
+  void* y;
+  uint64_t y_cols, y_stride;
+  uint64_t batch;
+  const void* bias;
+  const void* mul;
+  uint64_t mul_stride;
+  const void* residual;
+  uint64_t residual_stride;
+  uint32_t y_type, bias_type, mul_type, residual_type; /* XKSV_BF16 or XKSV_FP32; ignored for NULL */
+  uint32_t act;                                        /* XKSV_ACT_* */
+  uint32_t flags;                                      /* must be 0 */
+} xksv_linear_args;
+
+/* Enqueues the layer on `stream`, on the device the plan was created on.
+ * d_workspace is caller-owned device memory of at least
+ * xksv_plan_linear_workspace(plan, batch) bytes, 256-byte aligned, its
+ * contents free before and after; calls that may overlap need their own (and
+ * their own plan: one call in flight per plan).  Allocates nothing, so it can
+ * be captured into a graph.  A tile index (xksv_plan_index) speeds it up as
+ * it does xksv_plan_gemm.  Returns 1 without launching for a slab outside the
+ * payload, x or y, two slabs covering the same row of Y, a raw slab that is
+ * not rows x cols, unknown types or activations, or a workspace too small;
+ * batch 0 does nothing.  Slab errors are read with xksv_plan_status.  As in
+ * xksv_plan_gemm, batches that share a row between several CTAs add in an
+ * order that may differ between runs (the last bits of the FP32 sums). */
+size_t xksv_plan_linear_workspace(const xksv_plan* plan, size_t batch);
+int xksv_plan_linear(const xksv_plan* plan, const void* d_payload, size_t payload_size,
+                     const xksv_linear_args* args, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------- Part 8: paged key/value cache ------------------------- */
+/* No reference counterpart.  The cache is two caller-owned device buffers of
+ * pages; a page holds page_size tokens of every KV head.  Element (page p,
+ * token t, head h, dim d) of k is k[p * k_stride[0] + t * k_stride[1] +
+ * h * k_stride[2] + d], likewise v: strides in elements, so pages may be
+ * [page_size, heads, dim] or [heads, page_size, dim] or slices of a larger
+ * buffer.  type is XKSV_BF16, XKSV_FP16 or XKSV_E4M3; an E4M3 element stands
+ * for its value times k_scale[h] / v_scale[h] (device FP32 [kv_heads]; NULL:
+ * 1).  A sequence's tokens live in the pages its row of the page table lists:
+ * token j in page table[j / page_size] at place j % page_size. */
+typedef struct xksv_kv_desc {
+  void* k;
+  void* v;
+  uint64_t k_bytes, v_bytes; /* buffer sizes */
+  uint64_t pages, page_size;
+  uint64_t k_stride[3], v_stride[3]; /* page, token, head */
+  const float* k_scale;
+  const float* v_scale;
+  uint32_t kv_heads, head_dim, type, flags; /* flags must be 0 */
+} xksv_kv_desc;
+typedef struct xksv_kv xksv_kv;
+
+/* Describes a cache on the current device.  Returns 1 for null or
+ * misaligned buffers (16 bytes), strides that are no multiple of 16 bytes,
+ * that leave the buffer or let two elements overlap, a head_dim above 256 or
+ * whose row is no multiple of 16 bytes, and scales with a 16-bit type.
+ * Every call below runs on this device, whichever is current. */
+int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** kv);
+void xksv_kv_destroy(xksv_kv* kv);
+/* Synchronises `stream`; 0 when no call reported an error since the last one
+ * (then clears the word), else 1: a page outside the cache, a sequence or a
+ * place outside the page table, a length above the table's. */
+int xksv_kv_status(const xksv_kv* kv, void* stream);
+
+/* New tokens into the cache.  Token t is token index[t] of sequence seq[t]
+ * (NULL: sequence t) and its rotation position is positions[t] (NULL:
+ * index[t]).  Keys and queries are rotated: for the pairs (a, b) of the first
+ * rot_dim dims -- (i, i + rot_dim / 2), or (2i, 2i + 1) with
+ * XKSV_KV_INTERLEAVED -- and the angle positions[t] * inv_freq[i],
+ *   (a, b) -> rot_scale * (a cos - b sin, b cos + a sin),
+ * angles exact to FP32 after reduction at any position; rot_dim 0 rotates
+ * nothing.  Values are stored as they are.  A stored element is rounded once
+ * (E4M3: divided by the head's scale, saturated at 448, NaN kept).  q [tokens,
+ * q_heads, head_dim] rotated goes to q_out (may be q itself with the same strides);
+ * both NULL when there is none.  Strides in elements: [0] token, [1] head;
+ * the last dimension is contiguous; any alignment of the type will do.
+ * A token whose seq or index is negative is padding: nothing of it is read or
+ * written.  A token outside the table or whose page is outside the cache is
+ * skipped too and reported by xksv_kv_status.  Two tokens of one call with
+ * the same place leave either one's elements there. */
+#define XKSV_KV_INTERLEAVED 1u
+typedef struct xksv_kv_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  uint64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2];
+  uint64_t tokens;
+  const int32_t* table; /* [table_rows, table_cols], rows table_stride apart */
+  uint64_t table_rows, table_cols, table_stride;
+  const int32_t* seq;
+  const int32_t* index;
+  const int32_t* positions;
+  const float* inv_freq; /* device FP32 [rot_dim / 2] */
+  float rot_scale;
+  uint32_t rot_dim, q_heads;
+  uint32_t type;  /* of q, k, v and q_out: XKSV_BF16, XKSV_FP16 or XKSV_FP32 */
+  uint32_t flags; /* XKSV_KV_INTERLEAVED or 0 */
+} xksv_kv_append_args;
+int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* stream);
+
+/* Attention of one new token per sequence: with L = lens[s] cached tokens
+ * (the new one included, its key appended first), query head h of KV head
+ * g = h / (q_heads / kv_heads), and j over the last `window` of the L tokens
+ * (0: all of them),
+ *   t_j = scale * q[s, h] . K[j, g]   (softcap c > 0: c * tanh(t_j / c))
+ *   out[s, h] = sum_j softmax(t)_j V[j, g],   lse[s, h] = log sum_j exp(t_j).
+ * No score above -infinity (L = 0 among them): zeros and -infinity.  Tokens
+ * behind L, and the rest of their pages, are not read.  q and out are [seqs, q_heads, head_dim] of `type`, strides
+ * in elements ([0] sequence, [1] head), the last dimension contiguous; type
+ * is the cache's, or BF16 or FP16 over an E4M3 cache.  lse is FP32 [seqs,
+ * q_heads] contiguous, or NULL.  Scores, softmax statistics and sums are
+ * FP32.  A length that is negative or above table_cols * page_size gives
+ * zeros and -infinity, a page outside the cache counts as masked; both are
+ * reported by xksv_kv_status.  d_workspace: as for xksv_plan_linear, of at
+ * least xksv_kv_attend_workspace(kv, seqs, q_heads, table_cols) bytes; NULL
+ * when that is 0. */
+typedef struct xksv_kv_attend_args {
+  const void* q;
+  void* out;
+  float* lse;
+  uint64_t q_stride[2], out_stride[2];
+  uint64_t seqs;
+  const int32_t* table; /* [seqs, table_cols], rows table_stride apart */
+  uint64_t table_cols, table_stride;
+  const int32_t* lens;
+  float scale, softcap;
+  uint64_t window;
+  uint32_t q_heads, type;
+} xksv_kv_attend_args;
+size_t xksv_kv_attend_workspace(const xksv_kv* kv, size_t seqs, size_t q_heads, size_t table_cols);
+int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* args, void* d_workspace, size_t workspace_bytes,
+                   void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,97 @@
+"""CPU: the paged cache's index arithmetic (csrc/kv_index.h) as plain C++ on
+the host -- pages outside the cache, tokens outside the table, lengths and
+windows at their edges -- and the binding's argument checks."""
+import subprocess
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+CSRC = ROOT / "xks-vectorforge_b200" / "csrc"
+
+
+def run_cpp(tmp_path, body):
+    src = tmp_path / "t.cpp"
+    src.write_text('#include "kv_index.h"\n#include <cassert>\n#include <cstdio>\n#include <vector>\n'
+                   "using namespace xksv;\nint main() {\n" + body + "\n return 0;\n}\n")
+    exe = tmp_path / "t"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=address,undefined", "-I", str(CSRC), str(src), "-o",
+                    str(exe)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_page_lookup_stays_inside_the_table(tmp_path):
+    run_cpp(tmp_path, """
+  // 3 sequences by 4 pages, rows 5 apart; the last row holds 4 entries only
+  std::vector<int32_t> t(2 * 5 + 4, 0);
+  t[0] = 7; t[3] = 9; t[5] = -1; t[10 + 3] = 8; t[10] = 2147483647;
+  auto at = [&](int64_t s, int64_t i) { return kv_page(t.data(), 3, 4, 5, 9, 16, s, i); };
+  assert(at(0, 0) == 7 && at(0, 15) == 7 && at(0, 16) == 0);
+  assert(at(0, 63) == -1);            // page 9 of a cache of 9 pages
+  assert(at(1, 3) == -1);             // page -1
+  assert(at(2, 63) == 8);             // the table's last entry
+  assert(at(2, 64) == -1);            // behind it
+  assert(at(2, 0) == -1);             // a page number of 2^31 - 1
+  assert(at(3, 0) == -1 && at(-1, 0) == -1 && at(0, -1) == -1);
+  assert(at(0, 2147483647) == -1 && at(int64_t(1) << 40, 0) == -1);
+""")
+
+
+def test_span_of_lengths_and_windows(tmp_path):
+    run_cpp(tmp_path, """
+  auto is = [](KvSpan s, int64_t f, int64_t l, bool ok) { return s.first == f && s.length == l && s.ok == ok; };
+  assert(is(kv_span(0, 4, 16, 0), 0, 0, true));
+  assert(is(kv_span(64, 4, 16, 0), 0, 64, true));
+  assert(is(kv_span(65, 4, 16, 0), 0, 0, false));
+  assert(is(kv_span(-1, 4, 16, 0), 0, 0, false));
+  assert(is(kv_span(64, 4, 16, 1), 63, 64, true));
+  assert(is(kv_span(64, 4, 16, 64), 0, 64, true));
+  assert(is(kv_span(64, 4, 16, 63), 1, 64, true));
+  assert(is(kv_span(64, 4, 16, ~uint64_t(0)), 0, 64, true));
+  assert(is(kv_span(0, 4, 16, 1), 0, 0, true));
+""")
+
+
+def test_binding_refuses_before_the_library():
+    torch = pytest.importorskip("torch")
+    import xksv_gpu as xg
+    k = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA tensors"):
+        xg.KVCache(k, k.clone())
+    with pytest.raises(ValueError, match="layout"):
+        xg.KVCache(k, k.clone(), layout="dhn")
+    dev = torch.device("cpu")
+    x = torch.zeros(4, 8)
+    assert xg._matrix(x, 4, 8, "x", dev) == (x.data_ptr(), 8)
+    assert xg._matrix(x[:, :6], 4, 6, "x", dev) == (x.data_ptr(), 8)
+    for bad in (x.t(), x[0], x[:, ::2], x[:3]):
+        with pytest.raises(ValueError):
+            xg._matrix(bad, 4, 8, "x", dev)
+    with pytest.raises(ValueError, match="dtype"):
+        xg._type(x.double(), (xg.BF16,), "x")
+    h = torch.zeros(3, 2, 64)
+    assert xg._heads(h.transpose(0, 1), 2, 3, 64, "h", dev)[1] == (64, 128)
+    with pytest.raises(ValueError, match="contiguous"):
+        xg._heads(h[..., ::2], 3, 2, 32, "h", dev)
+    with pytest.raises(ValueError):
+        xg._ints(torch.zeros(4, dtype=torch.int64), 4, "index", dev)
+    with pytest.raises(ValueError):
+        xg._ints(torch.zeros(8, dtype=torch.int32)[::2], 4, "index", dev)
+    with pytest.raises(ValueError):
+        xg._table(torch.zeros(4, 4, dtype=torch.int32).t(), dev)
+
+
+def test_null_arguments_are_refused():
+    import build as b
+    b.build()
+    import xksv_gpu as xg
+    lib = xg.load()
+    assert lib.xksv_kv_create(None, None) == 1
+    assert lib.xksv_kv_append(None, None, None) == 1
+    assert lib.xksv_kv_attend(None, None, None, 0, None) == 1
+    assert lib.xksv_kv_status(None, None) == 1
+    assert lib.xksv_kv_attend_workspace(None, 1, 1, 1) == 0
+    assert lib.xksv_plan_linear(None, None, 0, None, None, 0, None) == 1
+    assert lib.xksv_plan_linear_workspace(None, 4) == 0
+    lib.xksv_kv_destroy(None)

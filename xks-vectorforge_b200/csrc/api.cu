@@ -221,6 +221,12 @@ struct xksv_plan {
   uint32_t* d_fmembers = nullptr;
   void* d_ftabs = nullptr;  // per group: its lane tables, built with the index
   uint64_t* d_hash_ranges = nullptr;  // per slab in creation order: {dst, decoded bytes}
+  // linear layer (xksv_plan_linear): the runs of Y rows the slabs cover; off
+  // when two slabs cover one row or a slab has no rows and columns
+  bool linear_ok = false;
+  uint32_t n_runs = 0;
+  uint64_t max_run = 0;
+  xksv::RowRun* d_runs = nullptr;
   // xksv_plan_decode_host: copy stream and per-chunk events (created on first use)
   cudaStream_t copy_st = nullptr;
   cudaEvent_t chunk_ev[9] = {};
@@ -308,6 +314,26 @@ bool build_tc_groups(const std::vector<xksv::Slab>& all, std::vector<xksv::TcGro
   groups.push_back(cur);
   return true;
 }
+// The runs of consecutive Y rows that the slabs cover, in order; false when a
+// row is covered twice or a slab has no shape.
+bool row_runs(const std::vector<xksv::Slab>& all, std::vector<xksv::RowRun>& runs) {
+  std::vector<xksv::RowRun> v;
+  v.reserve(all.size());
+  for (const xksv::Slab& s : all) {
+    if (!s.rows || !s.cols) return false;
+    v.push_back(xksv::RowRun{s.dst, s.rows});
+  }
+  std::sort(v.begin(), v.end(), [](const xksv::RowRun& a, const xksv::RowRun& b) { return a.row0 < b.row0; });
+  for (const xksv::RowRun& r : v) {
+    if (!runs.empty() && r.row0 < runs.back().row0 + runs.back().rows) return false;
+    if (!runs.empty() && r.row0 == runs.back().row0 + runs.back().rows)
+      runs.back().rows += r.rows;
+    else
+      runs.push_back(r);
+  }
+  return true;
+}
+
 // Fused-GEMM groups and CTA work: slabs reading the same X columns
 // (x_offset, cols) in groups of up to 32 (one slab per lane).  The work unit
 // is a half tile of a group (8 rows x 16 columns of all its slabs; the same
@@ -582,6 +608,18 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
                      cudaSuccess;
     }
   }
+  // runs of covered Y rows (linear layer)
+  if (ok && raw_gemm_ok) {
+    std::vector<RowRun> runs;
+    // X and Y below 2^40 rows: the workspace's byte counts fit 64 bits
+    p->linear_ok = need_x < (1ull << 40) && need_y < (1ull << 40) && row_runs(all, runs);
+    if (p->linear_ok && !runs.empty()) {
+      p->n_runs = uint32_t(runs.size());
+      for (const RowRun& r : runs) p->max_run = std::max(p->max_run, r.rows);
+      ok = cudaMalloc(&p->d_runs, runs.size() * sizeof(RowRun)) == cudaSuccess &&
+           cudaMemcpy(p->d_runs, runs.data(), runs.size() * sizeof(RowRun), cudaMemcpyHostToDevice) == cudaSuccess;
+    }
+  }
   // the copies above ran on the legacy default stream, which callers' non-blocking
   // streams do not wait for: finish them before the plan is used anywhere
   ok = ok && cudaStreamSynchronize(nullptr) == cudaSuccess;
@@ -602,6 +640,7 @@ void xksv_plan_destroy(xksv_plan* p) {
   if (p->d_scratch && p->scratch_owned) cudaFree(p->d_scratch);
   if (p->d_xt) cudaFree(p->d_xt);
   if (p->d_hash_ranges) cudaFree(p->d_hash_ranges);
+  if (p->d_runs) cudaFree(p->d_runs);
   if (p->d_slabs) cudaFree(p->d_slabs);
   if (p->d_status) cudaFree(p->d_status);
   if (p->h_status) cudaFreeHost(p->h_status);
@@ -752,16 +791,19 @@ int xksv_plan_decode_host(const xksv_plan* pc, const void* h_payload, size_t pay
   return e == cudaSuccess ? 0 : 1;
 }
 
-int xksv_plan_gemm(const xksv_plan* pc, const void* d_payload, size_t payload_size, const float* d_x,
-                   size_t x_rows, float* d_y, size_t y_rows, size_t batch, void* stream) {
-  auto* p = const_cast<xksv_plan*>(pc);
-  if (!p || !d_payload || !d_x || !d_y || !batch || batch > std::numeric_limits<uint32_t>::max() ||
-      misaligned(d_x, 4) || misaligned(d_y, 4))
-    return 1;
-  if (p->need_payload > payload_size || p->need_x_rows > x_rows || p->need_y_rows > y_rows) return 1;
-  if (p->n_raw && !p->raw_gemm_ok) return 1;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const uint8_t* pay = static_cast<const uint8_t*>(d_payload);
+namespace {
+// Which tensor-core buffers a product of `batch` columns uses: X^T in BF16
+// (and the fused route), or that and the decoded scratch.
+bool gemm_fused(const xksv_plan* p, const void* d_payload, size_t batch) {
+  return p->fused_ok && p->d_tidx && d_payload == p->indexed_payload && batch >= 4 && batch <= 128 &&
+         p->gemm_route != XKSV_GEMM_SCRATCH;
+}
+
+// Enqueues Y = W X (xksv_plan_gemm after its checks) with the given buffers
+// for X^T in BF16 [256][x_cols] and the decoded weights, which only the
+// tensor-core routes touch.
+int gemm_run(xksv_plan* p, const uint8_t* pay, const float* d_x, float* d_y, size_t batch, void* xt,
+             uint8_t* scratch, cudaStream_t st) {
   p->launches = 0;
   cudaError_t e = cudaSuccess;
   const uint32_t ld = uint32_t(batch);
@@ -770,12 +812,11 @@ int xksv_plan_gemm(const xksv_plan* pc, const void* d_payload, size_t payload_si
   // 182 / 190 us at 2 / 3); from batch 4, decode + tensor-core GEMM with X
   // rounded to BF16 (200 us for any batch <= 256, against 230 us for batch 4
   // on the CUDA cores; the 70B linears: 164 ms against 226 ms at batch 4)
-  const bool indexed = p->d_tidx && d_payload == p->indexed_payload;
-  const bool fused = p->fused_ok && indexed && batch >= 4 && batch <= 128 && p->gemm_route != XKSV_GEMM_SCRATCH;
+  const bool indexed = p->d_tidx && pay == p->indexed_payload;
+  const bool fused = gemm_fused(p, pay, batch);
   if (fused) {
     // one kernel decodes every tile row into tensor-core operand stages,
     // after a prep kernel (X^T in BF16, zeroed Y rows) that it overlaps
-    if (!p->d_xt && cudaMalloc(&p->d_xt, 256 * p->x_cols * 2) != cudaSuccess) return 1;
     FusedArgs f{};
     f.seg0 = p->d_fseg0;
     f.tasks = p->d_ftasks;
@@ -787,7 +828,7 @@ int xksv_plan_gemm(const xksv_plan* pc, const void* d_payload, size_t payload_si
     f.tmid = p->d_tmid;
     f.tabs = p->d_ftabs;
     f.payload = pay;
-    f.xt = p->d_xt;
+    f.xt = xt;
     f.xt_ld = p->x_cols;
     f.y = d_y;
     f.ld = ld;
@@ -801,34 +842,31 @@ int xksv_plan_gemm(const xksv_plan* pc, const void* d_payload, size_t payload_si
   if (p->tc_ok && batch >= 4) {
     // decode every slab into its BF16 row group, then the tensor-core GEMM,
     // up to 256 batch columns per pass over the same decoded scratch
-    if (!p->d_scratch && cudaMalloc(&p->d_scratch, std::max<uint64_t>(16, p->scratch_bytes)) != cudaSuccess)
-      return 1;
-    if (!p->d_xt && cudaMalloc(&p->d_xt, 256 * p->x_cols * 2) != cudaSuccess) return 1;
     const uint32_t tser0 = indexed && p->n_items ? p->n_ser_idx : 0;
     if (tser0) {
-      e = tile_decode(p, p->d_tc_slabs, pay, p->d_scratch, st);
+      e = tile_decode(p, p->d_tc_slabs, pay, scratch, st);
       ++p->launches;
     }
     if (e == cudaSuccess && p->n_ser > tser0) {
-      e = launch_serial_decode(p->d_tc_slabs + tser0, p->n_ser - tser0, pay, p->d_scratch, p->d_status,
+      e = launch_serial_decode(p->d_tc_slabs + tser0, p->n_ser - tser0, pay, scratch, p->d_status,
                                p->grid_ser, st);
       ++p->launches;
     }
     if (e == cudaSuccess && p->n_par) {
-      e = launch_parallel_decode(p->d_tc_slabs + p->n_ser, p->n_par, pay, p->d_scratch, p->d_status,
+      e = launch_parallel_decode(p->d_tc_slabs + p->n_ser, p->n_par, pay, scratch, p->d_status,
                                  p->grid_par, st);
       ++p->launches;
     }
     if (e == cudaSuccess && p->n_raw) {
-      e = launch_raw_decode(p->d_tc_slabs + p->n_ser + p->n_par, p->n_raw, pay, p->d_scratch,
+      e = launch_raw_decode(p->d_tc_slabs + p->n_ser + p->n_par, p->n_raw, pay, scratch,
                             p->grid_raw, st);
       ++p->launches;
     }
     for (size_t b0 = 0; b0 < batch && e == cudaSuccess; b0 += 256) {
       TcGemmArgs g{};
       g.groups = p->d_groups;
-      g.scratch = p->d_scratch;
-      g.xt = p->d_xt;
+      g.scratch = scratch;
+      g.xt = xt;
       g.xt_ld = p->x_cols;
       g.y = d_y + b0;
       g.ld = ld;
@@ -886,6 +924,120 @@ int xksv_plan_gemm(const xksv_plan* pc, const void* d_payload, size_t payload_si
     }
   }
   return e == cudaSuccess ? 0 : 1;
+}
+}  // namespace
+
+int xksv_plan_gemm(const xksv_plan* pc, const void* d_payload, size_t payload_size, const float* d_x,
+                   size_t x_rows, float* d_y, size_t y_rows, size_t batch, void* stream) {
+  auto* p = const_cast<xksv_plan*>(pc);
+  if (!p || !d_payload || !d_x || !d_y || !batch || batch > std::numeric_limits<uint32_t>::max() ||
+      misaligned(d_x, 4) || misaligned(d_y, 4))
+    return 1;
+  if (p->need_payload > payload_size || p->need_x_rows > x_rows || p->need_y_rows > y_rows) return 1;
+  if (p->n_raw && !p->raw_gemm_ok) return 1;
+  // the plan's own tensor-core buffers, allocated on first use and kept
+  if (p->tc_ok && batch >= 4) {
+    if (!gemm_fused(p, d_payload, batch) && !p->d_scratch &&
+        cudaMalloc(&p->d_scratch, std::max<uint64_t>(16, p->scratch_bytes)) != cudaSuccess)
+      return 1;
+    if (!p->d_xt && cudaMalloc(&p->d_xt, 256 * p->x_cols * 2) != cudaSuccess) return 1;
+  }
+  return gemm_run(p, static_cast<const uint8_t*>(d_payload), d_x, d_y, batch, p->d_xt, p->d_scratch,
+                  static_cast<cudaStream_t>(stream));
+}
+
+// ---------------------------------------------------------- linear layer
+namespace {
+// Carves a workspace: every part 256-byte aligned.
+struct Carve {
+  uint64_t pos = 0;
+  uint64_t take(uint64_t bytes) {
+    const uint64_t at = pos;
+    pos += (bytes + 255) & ~uint64_t(255);
+    return at;
+  }
+};
+struct LinearSpace {
+  uint64_t x, z, xt, scratch, total;
+};
+LinearSpace linear_space(const xksv_plan* p, uint64_t batch) {
+  Carve c;
+  LinearSpace s{};
+  s.x = c.take(p->need_x_rows * batch * sizeof(float));
+  s.z = c.take(p->need_y_rows * batch * sizeof(float));
+  if (p->tc_ok && batch >= 4) {
+    s.xt = c.take(256 * p->x_cols * 2);
+    s.scratch = c.take(p->scratch_bytes);
+  }
+  s.total = c.pos;
+  return s;
+}
+constexpr uint64_t kMaxBatch = 1ull << 20;
+bool elem_ok(const void* ptr, uint32_t type) {
+  return !ptr || ((type == XKSV_BF16 || type == XKSV_FP32) && !misaligned(ptr, type == XKSV_FP32 ? 4 : 2));
+}
+// Runs a call on a plan's device, whichever is current.
+struct OnDevice {
+  int before = -1;
+  bool ok = false;
+  explicit OnDevice(int dev) {
+    if (cudaGetDevice(&before) != cudaSuccess) return;
+    ok = before == dev || cudaSetDevice(dev) == cudaSuccess;
+    if (before == dev) before = -1;
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+}  // namespace
+
+size_t xksv_plan_linear_workspace(const xksv_plan* p, size_t batch) {
+  if (!p || !p->linear_ok || !batch || batch >= kMaxBatch) return 0;
+  return size_t(linear_space(p, batch).total);
+}
+
+int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_size, const xksv_linear_args* a,
+                     void* d_workspace, size_t workspace_bytes, void* stream) {
+  auto* p = const_cast<xksv_plan*>(pc);
+  if (!p || !a || a->flags || !p->linear_ok || a->act > XKSV_ACT_GELU_TANH || a->batch >= kMaxBatch) return 1;
+  if ((a->y_type != XKSV_BF16 && a->y_type != XKSV_FP32) || !elem_ok(a->y, a->y_type) ||
+      !elem_ok(a->bias, a->bias_type) || !elem_ok(a->mul, a->mul_type) || !elem_ok(a->residual, a->residual_type) ||
+      misaligned(a->x, 2))
+    return 1;
+  if (p->need_payload > payload_size || p->need_x_rows > a->x_cols || p->need_y_rows > a->y_cols) return 1;
+  // a single token's stride is never used
+  if (a->batch > 1 && (a->x_stride < a->x_cols || a->y_stride < a->y_cols || (a->mul && a->mul_stride < a->y_cols) ||
+                       (a->residual && a->residual_stride < a->y_cols)))
+    return 1;
+  p->launches = 0;
+  if (!a->batch || !p->n_runs) return 0;
+  if (!d_payload || !a->x || !a->y) return 1;
+  const LinearSpace sp = linear_space(p, a->batch);
+  if (!d_workspace || workspace_bytes < sp.total || misaligned(d_workspace, 256)) return 1;
+  OnDevice dev(p->device);
+  if (!dev.ok) return 1;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto* ws = static_cast<uint8_t*>(d_workspace);
+  auto* x = reinterpret_cast<float*>(ws + sp.x);
+  auto* z = reinterpret_cast<float*>(ws + sp.z);
+  Epilogue ep{};
+  ep.y = a->y;
+  ep.bias = a->bias;
+  ep.mul = a->mul;
+  ep.residual = a->residual;
+  ep.y_stride = a->y_stride;
+  ep.mul_stride = a->mul_stride;
+  ep.residual_stride = a->residual_stride;
+  ep.act = a->act;
+  ep.y_f32 = a->y_type == XKSV_FP32;
+  ep.bias_f32 = a->bias_type == XKSV_FP32;
+  ep.mul_f32 = a->mul_type == XKSV_FP32;
+  ep.residual_f32 = a->residual_type == XKSV_FP32;
+  if (launch_linear_x(a->x, a->x_stride, a->batch, p->need_x_rows, x, st) != cudaSuccess) return 1;
+  if (gemm_run(p, static_cast<const uint8_t*>(d_payload), x, z, a->batch, ws + sp.xt, ws + sp.scratch, st)) return 1;
+  if (launch_linear_y(z, a->batch, p->d_runs, p->n_runs, p->max_run, ep, st) != cudaSuccess) return 1;
+  p->launches += 2;
+  return 0;
 }
 
 int xksv_plan_set_gemm_route(xksv_plan* p, int route) {

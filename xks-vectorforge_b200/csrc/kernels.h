@@ -170,6 +170,28 @@ cudaError_t launch_fused_check(const Slab* slabs, uint32_t n, const uint8_t* pay
 cudaError_t launch_fused_gemm(const FusedArgs& args, uint32_t nctas, const float* x, uint64_t x_cols,
                               const TcGroup* groups, uint32_t ngroups, cudaStream_t st);
 
+// A run of consecutive rows of Y that a plan's slabs cover.
+struct RowRun {
+  uint64_t row0, rows;
+};
+// What a linear layer does with z[b, row] on its way into y (mirrors
+// xksv_linear_args; null pointers are absent).
+struct Epilogue {
+  void* y;
+  const void* bias;
+  const void* mul;
+  const void* residual;
+  uint64_t y_stride, mul_stride, residual_stride;
+  uint32_t act;
+  bool y_f32, bias_f32, mul_f32, residual_f32;
+};
+// x BF16 [batch, cols] (rows `stride` elements apart) to FP32 [cols, batch].
+cudaError_t launch_linear_x(const void* x, uint64_t stride, uint64_t batch, uint64_t cols, float* xt, cudaStream_t st);
+// z FP32 [Y rows, batch] through the epilogue into y, for the rows of `runs`
+// (nruns of them, `rows` the longest).
+cudaError_t launch_linear_y(const float* z, uint64_t batch, const RowRun* runs, uint32_t nruns, uint64_t rows,
+                            const Epilogue& e, cudaStream_t st);
+
 // SHA-256 (FIPS 180-4) of n ranges {offset, length} (device array of 2n u64)
 // of d_base; 32-byte big-endian digests to d_digests.
 cudaError_t launch_sha256(const uint64_t* d_ranges, uint32_t n, const uint8_t* d_base, uint8_t* d_digests,

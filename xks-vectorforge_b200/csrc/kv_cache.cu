@@ -1,0 +1,391 @@
+// Paged key/value cache (include/xksv_cuda.h, part 8): the append of new
+// tokens with their position rotation, and the attention of one new token per
+// sequence over the cached ones.
+//
+// This file holds the kernels and their C entries; the cache itself is the
+// caller's memory, the handle its geometry and a device status word.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <new>
+#include <utility>
+
+#include "kernels.h"
+#include "kv_index.h"
+#include "xksv_cuda.h"
+
+struct xksv_kv {
+  int device = 0;
+  xksv_kv_desc d{};
+  int* d_status = nullptr;
+  int* h_status = nullptr;
+};
+
+namespace xksv {
+namespace {
+
+// Runs a call on the handle's device, whichever is current.
+struct DeviceGuard {
+  int before = -1;
+  bool ok = false;
+  explicit DeviceGuard(int dev) {
+    if (cudaGetDevice(&before) != cudaSuccess) return;
+    ok = before == dev || cudaSetDevice(dev) == cudaSuccess;
+    if (before == dev) before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+// ------------------------------------------------------------- elements ---
+struct E4m3 {
+  __nv_fp8_storage_t b;
+};
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(E4m3 x) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(x.b, __NV_E4M3)));
+}
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) {
+  return __float2half_rn(x);
+}
+template <>
+__device__ __forceinline__ float from_float<float>(float x) {
+  return x;
+}
+template <>
+__device__ __forceinline__ E4m3 from_float<E4m3>(float x) {
+  return E4m3{__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3)};
+}
+
+// --------------------------------------------------------------- append ---
+constexpr int AT = 256;         // threads per token
+constexpr int kMaxPairs = 128;  // head_dim <= 256
+
+struct AppendArgs {
+  xksv_kv_append_args a;
+  xksv_kv_desc c;
+  int* status;
+};
+
+// One CTA per token: its angles once in shared memory, then its heads.
+template <class TI, class TC>
+__global__ void __launch_bounds__(AT) kv_append_kernel(const AppendArgs p) {
+  __shared__ float cs[kMaxPairs], sn[kMaxPairs];
+  const uint64_t t = blockIdx.x;
+  const int64_t s = p.a.seq ? int64_t(p.a.seq[t]) : int64_t(t);
+  const int64_t idx = p.a.index[t];
+  if (s < 0 || idx < 0) return;
+  const uint64_t place = uint64_t(idx) % p.c.page_size;
+  const int64_t page = kv_page(p.a.table, p.a.table_rows, p.a.table_cols, p.a.table_stride, p.c.pages, p.c.page_size, s, idx);
+  if (page < 0) {
+    if (threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
+    return;
+  }
+  const uint32_t D = p.c.head_dim, half = p.a.rot_dim / 2;
+  const int32_t pos = p.a.positions ? p.a.positions[t] : int32_t(idx);
+  for (uint32_t i = threadIdx.x; i < half; i += AT) {
+    // the angle in 64 bits, less its whole turns: an FP32 product would be
+    // wrong by radians at far positions
+    constexpr double kTurn = 6.283185307179586476925286766559;
+    const double angle = double(pos) * double(p.a.inv_freq[i]);
+    const float r = float(fma(-rint(angle / kTurn), kTurn, angle));
+    float sv, cv;
+    sincosf(r, &sv, &cv);
+    cs[i] = cv * p.a.rot_scale;
+    sn[i] = sv * p.a.rot_scale;
+  }
+  __syncthreads();
+  const bool inter = p.a.flags & XKSV_KV_INTERLEAVED;
+  const uint32_t rest = D - 2 * half, items = half + rest;  // pairs, then single elements
+  const TI* q = static_cast<const TI*>(p.a.q) + t * p.a.q_stride[0];
+  TI* qo = static_cast<TI*>(p.a.q_out) + t * p.a.q_out_stride[0];
+  const TI* k = static_cast<const TI*>(p.a.k) + t * p.a.k_stride[0];
+  const TI* v = static_cast<const TI*>(p.a.v) + t * p.a.v_stride[0];
+  TC* ck = static_cast<TC*>(p.c.k) + uint64_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1];
+  TC* cv = static_cast<TC*>(p.c.v) + uint64_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1];
+  const uint32_t nq = p.a.q ? p.a.q_heads : 0;
+  for (uint32_t w = threadIdx.x; w < (nq + p.c.kv_heads) * items; w += AT) {
+    const uint32_t hh = w / items, i = w - hh * items;
+    const bool is_q = hh < nq;
+    const uint32_t h = is_q ? hh : hh - nq;
+    const TI* src = is_q ? q + h * p.a.q_stride[1] : k + h * p.a.k_stride[1];
+    const float inv = !is_q && p.c.k_scale ? p.c.k_scale[h] : 1.f;
+    auto put = [&](uint32_t d, float x) {
+      if (is_q)
+        qo[h * p.a.q_out_stride[1] + d] = from_float<TI>(x);
+      else
+        ck[h * p.c.k_stride[2] + d] = from_float<TC>(p.c.k_scale ? x / inv : x);
+    };
+    if (i < half) {
+      const uint32_t da = inter ? 2 * i : i, db = inter ? 2 * i + 1 : i + half;
+      const float a = to_float(src[da]), b = to_float(src[db]);
+      put(da, a * cs[i] - b * sn[i]);
+      put(db, b * cs[i] + a * sn[i]);
+    } else {
+      const uint32_t d = i + half;
+      put(d, to_float(src[d]));
+    }
+  }
+  for (uint32_t w = threadIdx.x; w < p.c.kv_heads * D; w += AT) {
+    const uint32_t h = w / D, d = w - h * D;
+    const float x = to_float(v[h * p.a.v_stride[1] + d]);
+    cv[h * p.c.v_stride[2] + d] = from_float<TC>(p.c.v_scale ? x / p.c.v_scale[h] : x);
+  }
+}
+
+template <class TI>
+cudaError_t append_cache(const AppendArgs& p, cudaStream_t st) {
+  const dim3 g(uint32_t(p.a.tokens));
+  switch (p.c.type) {
+    case XKSV_BF16: kv_append_kernel<TI, __nv_bfloat16><<<g, AT, 0, st>>>(p); break;
+    case XKSV_FP16: kv_append_kernel<TI, __half><<<g, AT, 0, st>>>(p); break;
+    default: kv_append_kernel<TI, E4m3><<<g, AT, 0, st>>>(p); break;
+  }
+  return cudaGetLastError();
+}
+
+// --------------------------------------------------------------- attend ---
+constexpr int DT = 128;  // threads per (sequence, query head)
+
+struct AttendArgs {
+  xksv_kv_attend_args a;
+  xksv_kv_desc c;
+  int* status;
+};
+
+// One CTA per (sequence, query head); a warp takes every fourth token, its
+// lanes the dims, with a running maximum and sum; the warps join at the end.
+template <class TQ, class TC>
+__global__ void __launch_bounds__(DT) kv_attend_kernel(const AttendArgs p) {
+  __shared__ float sm[DT / 32], sl[DT / 32], so[DT / 32][256];
+  const uint64_t s = blockIdx.y;
+  const uint32_t h = blockIdx.x, g = h / (p.a.q_heads / p.c.kv_heads), D = p.c.head_dim;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const TQ* q = static_cast<const TQ*>(p.a.q) + s * p.a.q_stride[0] + h * p.a.q_stride[1];
+  TQ* out = static_cast<TQ*>(p.a.out) + s * p.a.out_stride[0] + h * p.a.out_stride[1];
+  const KvSpan span = kv_span(p.a.lens[s], p.a.table_cols, p.c.page_size, p.a.window);
+  if (!span.ok && threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
+  const int64_t L = span.length, j0 = span.first;
+  const float ks = (p.c.k_scale ? p.c.k_scale[g] : 1.f) * p.a.scale;
+  const float vs = p.c.v_scale ? p.c.v_scale[g] : 1.f;
+  float qr[8], o[8], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t d = i * 32 + lane;
+    qr[i] = d < D ? to_float(q[d]) : 0.f;
+    o[i] = 0.f;
+  }
+  for (int64_t j = j0 + warp; j < L; j += DT / 32) {
+    const int64_t page = kv_page(p.a.table, p.a.seqs, p.a.table_cols, p.a.table_stride, p.c.pages, p.c.page_size, s, j);
+    if (page < 0) {
+      if (lane == 0) atomicOr(p.status, kStatusHeader);
+      continue;
+    }
+    const uint64_t place = uint64_t(j) % p.c.page_size;
+    const TC* k = static_cast<const TC*>(p.c.k) + uint64_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2];
+    const TC* v = static_cast<const TC*>(p.c.v) + uint64_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2];
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i * 32 + lane < D) dot = fmaf(qr[i], to_float(k[i * 32 + lane]), dot);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+    float t = dot * ks;
+    if (p.a.softcap > 0.f) t = p.a.softcap * tanhf(t / p.a.softcap);
+    const float mn = fmaxf(m, t), base = mn == -INFINITY ? 0.f : mn;
+    const float f = expf(m - base), w = expf(t - base);
+    l = l * f + w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i * 32 + lane < D) o[i] = o[i] * f + w * to_float(v[i * 32 + lane]);
+    m = mn;
+  }
+  if (lane == 0) {
+    sm[warp] = m;
+    sl[warp] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) so[warp][i * 32 + lane] = o[i];
+  __syncthreads();
+  float mt = -INFINITY, lt = 0.f;
+  for (int w = 0; w < DT / 32; ++w) mt = fmaxf(mt, sm[w]);
+  const float base = mt == -INFINITY ? 0.f : mt;
+  for (int w = 0; w < DT / 32; ++w) lt += sl[w] * expf(sm[w] - base);
+  for (uint32_t d = threadIdx.x; d < D; d += DT) {
+    float x = 0.f;
+    for (int w = 0; w < DT / 32; ++w) x += so[w][d] * expf(sm[w] - base);
+    out[d] = from_float<TQ>(lt > 0.f || lt != lt ? x * vs / lt : 0.f);
+  }
+  if (threadIdx.x == 0 && p.a.lse) p.a.lse[s * p.a.q_heads + h] = base + logf(lt);
+}
+
+template <class TQ, class TC>
+cudaError_t attend_launch(const AttendArgs& p, cudaStream_t st) {
+  kv_attend_kernel<TQ, TC><<<dim3(p.a.q_heads, uint32_t(p.a.seqs)), DT, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+// ---------------------------------------------------------- C entry checks
+uint64_t elem_bytes(uint32_t type) { return type == XKSV_E4M3 ? 1 : type == XKSV_FP32 ? 4 : 2; }
+bool off_align(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0; }
+
+// The elements of a cache buffer lie inside it, on 16-byte rows, and no two
+// (page, token, head) rows overlap: ordered by stride, each dimension steps
+// past the whole extent of the smaller ones.
+bool strides_ok(const xksv_kv_desc& d, const void* base, uint64_t bytes, const uint64_t* stride) {
+  const uint64_t e = elem_bytes(d.type), total = bytes / e;
+  if (!base || off_align(base, 16)) return false;
+  struct Dim {
+    uint64_t n, stride;
+  } dim[3] = {{d.pages, stride[0]}, {d.page_size, stride[1]}, {d.kv_heads, stride[2]}};
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 3; ++j)
+      if (dim[j].stride < dim[i].stride) std::swap(dim[i], dim[j]);
+  uint64_t extent = d.head_dim;
+  if (extent > total) return false;
+  for (const Dim& x : dim) {
+    if (x.n == 1) continue;
+    if (x.stride * e % 16 || x.stride < extent) return false;
+    if (x.stride > (total - extent) / (x.n - 1)) return false;
+    extent += x.stride * (x.n - 1);
+  }
+  return true;
+}
+
+// No two rows of an output [n, heads, dim] overlap.
+bool rows_distinct(uint64_t n, uint64_t heads, uint64_t dim, const uint64_t* stride) {
+  const bool token_major = stride[0] >= stride[1];
+  const uint64_t n0 = token_major ? heads : n, s0 = token_major ? stride[1] : stride[0];
+  const uint64_t n1 = token_major ? n : heads, s1 = token_major ? stride[0] : stride[1];
+  if (n0 > 1 && s0 < dim) return false;
+  const uint64_t extent = n0 > 1 ? s0 * (n0 - 1) + dim : dim;
+  return n1 <= 1 || s1 >= extent;
+}
+bool strides_small(const uint64_t* stride) { return stride[0] < (1ull << 40) && stride[1] < (1ull << 40); }
+
+}  // namespace
+}  // namespace xksv
+
+using namespace xksv;
+
+extern "C" {
+
+int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** out) {
+  if (!out) return 1;
+  *out = nullptr;
+  if (!desc || desc->flags || (desc->type != XKSV_BF16 && desc->type != XKSV_FP16 && desc->type != XKSV_E4M3)) return 1;
+  const xksv_kv_desc& d = *desc;
+  constexpr uint64_t kDim = 1ull << 31;
+  if (!d.pages || !d.page_size || !d.kv_heads || !d.head_dim || d.head_dim > 256 || d.pages >= kDim ||
+      d.page_size >= kDim || d.kv_heads > 65535 || d.head_dim * elem_bytes(d.type) % 16)
+    return 1;
+  if (d.type != XKSV_E4M3 && (d.k_scale || d.v_scale)) return 1;
+  if (off_align(d.k_scale, 4) || off_align(d.v_scale, 4)) return 1;
+  for (int i = 0; i < 3; ++i)
+    if (d.k_stride[i] >= (1ull << 48) || d.v_stride[i] >= (1ull << 48)) return 1;
+  if (!strides_ok(d, d.k, d.k_bytes, d.k_stride) || !strides_ok(d, d.v, d.v_bytes, d.v_stride)) return 1;
+  auto* kv = new (std::nothrow) xksv_kv();
+  if (!kv) return 1;
+  kv->d = d;
+  const bool ok = cudaGetDevice(&kv->device) == cudaSuccess && cudaMalloc(&kv->d_status, sizeof(int)) == cudaSuccess &&
+                  cudaMallocHost(&kv->h_status, sizeof(int)) == cudaSuccess &&
+                  cudaMemset(kv->d_status, 0, sizeof(int)) == cudaSuccess && cudaStreamSynchronize(nullptr) == cudaSuccess;
+  if (!ok) {
+    xksv_kv_destroy(kv);
+    return 1;
+  }
+  *out = kv;
+  return 0;
+}
+
+void xksv_kv_destroy(xksv_kv* kv) {
+  if (!kv) return;
+  if (kv->d_status) cudaFree(kv->d_status);
+  if (kv->h_status) cudaFreeHost(kv->h_status);
+  delete kv;
+}
+
+int xksv_kv_status(const xksv_kv* kv, void* stream) {
+  if (!kv) return 1;
+  DeviceGuard guard(kv->device);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (!guard.ok || cudaMemcpyAsync(kv->h_status, kv->d_status, sizeof(int), cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+      cudaStreamSynchronize(st) != cudaSuccess)
+    return 1;
+  const int v = *kv->h_status;
+  if (v && (cudaMemsetAsync(kv->d_status, 0, sizeof(int), st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess))
+    return 1;
+  return v == 0 ? 0 : 1;
+}
+
+int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* a, void* stream) {
+  if (!kv || !a || (a->flags & ~XKSV_KV_INTERLEAVED)) return 1;
+  if (a->type != XKSV_BF16 && a->type != XKSV_FP16 && a->type != XKSV_FP32) return 1;
+  if (a->rot_dim % 2 || a->rot_dim > kv->d.head_dim || (a->rot_dim && !a->inv_freq) || off_align(a->inv_freq, 4)) return 1;
+  if (!a->q != !a->q_out || (a->q && (!a->q_heads || a->q_heads > 65535))) return 1;
+  if (!a->tokens) return 0;
+  const uintptr_t e = elem_bytes(a->type);
+  if (!a->k || !a->v || !a->table || !a->index || a->tokens >= (1ull << 31) || !a->table_rows || !a->table_cols ||
+      (a->table_rows > 1 && a->table_stride < a->table_cols) || off_align(a->table, 4) || off_align(a->seq, 4) ||
+      off_align(a->index, 4) || off_align(a->positions, 4) || off_align(a->q, e) || off_align(a->k, e) ||
+      off_align(a->v, e) || off_align(a->q_out, e))
+    return 1;
+  if (!strides_small(a->k_stride) || !strides_small(a->v_stride) ||
+      (a->q && (!strides_small(a->q_stride) || !strides_small(a->q_out_stride) ||
+                !rows_distinct(a->tokens, a->q_heads, kv->d.head_dim, a->q_out_stride))))
+    return 1;
+  DeviceGuard guard(kv->device);
+  if (!guard.ok) return 1;
+  const AppendArgs p{*a, kv->d, kv->d_status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t err = a->type == XKSV_BF16   ? append_cache<__nv_bfloat16>(p, st)
+                          : a->type == XKSV_FP16 ? append_cache<__half>(p, st)
+                                                 : append_cache<float>(p, st);
+  return err == cudaSuccess ? 0 : 1;
+}
+
+size_t xksv_kv_attend_workspace(const xksv_kv* kv, size_t, size_t, size_t) {
+  (void)kv;
+  return 0;
+}
+
+int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* a, void* d_workspace, size_t workspace_bytes,
+                   void* stream) {
+  if (!kv || !a || !a->q_heads || a->q_heads % kv->d.kv_heads || a->q_heads > 65535) return 1;
+  if (a->type != XKSV_BF16 && a->type != XKSV_FP16) return 1;
+  if (kv->d.type != XKSV_E4M3 && kv->d.type != a->type) return 1;
+  if (!(a->softcap >= 0.f) || a->seqs > 65535) return 1;
+  if (!a->seqs) return 0;
+  if (!a->q || !a->out || !a->table || !a->lens || !a->table_cols || a->table_cols >= (1ull << 31) ||
+      (a->seqs > 1 && a->table_stride < a->table_cols) || off_align(a->q, 2) || off_align(a->out, 2) ||
+      off_align(a->lse, 4) || off_align(a->table, 4) || off_align(a->lens, 4))
+    return 1;
+  if (!strides_small(a->q_stride) || !strides_small(a->out_stride) ||
+      !rows_distinct(a->seqs, a->q_heads, kv->d.head_dim, a->out_stride))
+    return 1;
+  if (workspace_bytes < xksv_kv_attend_workspace(kv, a->seqs, a->q_heads, a->table_cols) || off_align(d_workspace, 256))
+    return 1;
+  DeviceGuard guard(kv->device);
+  if (!guard.ok) return 1;
+  const AttendArgs p{*a, kv->d, kv->d_status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool e4 = kv->d.type == XKSV_E4M3;
+  const cudaError_t err = a->type == XKSV_BF16 ? (e4 ? attend_launch<__nv_bfloat16, E4m3>(p, st)
+                                                     : attend_launch<__nv_bfloat16, __nv_bfloat16>(p, st))
+                                               : (e4 ? attend_launch<__half, E4m3>(p, st)
+                                                     : attend_launch<__half, __half>(p, st));
+  return err == cudaSuccess ? 0 : 1;
+}
+
+}  // extern "C"

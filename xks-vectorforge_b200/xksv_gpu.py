@@ -25,6 +25,47 @@ class Slab(ctypes.Structure):
                 ("codec", ctypes.c_uint32), ("flags", ctypes.c_uint32)]
 
 
+class LinearArgs(ctypes.Structure):
+    """xksv_linear_args."""
+    _fields_ = [("x", ctypes.c_void_p), ("x_cols", ctypes.c_uint64), ("x_stride", ctypes.c_uint64),
+                ("y", ctypes.c_void_p), ("y_cols", ctypes.c_uint64), ("y_stride", ctypes.c_uint64),
+                ("batch", ctypes.c_uint64), ("bias", ctypes.c_void_p), ("mul", ctypes.c_void_p),
+                ("mul_stride", ctypes.c_uint64), ("residual", ctypes.c_void_p),
+                ("residual_stride", ctypes.c_uint64), ("y_type", ctypes.c_uint32), ("bias_type", ctypes.c_uint32),
+                ("mul_type", ctypes.c_uint32), ("residual_type", ctypes.c_uint32), ("act", ctypes.c_uint32),
+                ("flags", ctypes.c_uint32)]
+
+
+class KvDesc(ctypes.Structure):
+    """xksv_kv_desc."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_bytes", ctypes.c_uint64),
+                ("v_bytes", ctypes.c_uint64), ("pages", ctypes.c_uint64), ("page_size", ctypes.c_uint64),
+                ("k_stride", ctypes.c_uint64 * 3), ("v_stride", ctypes.c_uint64 * 3), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("type", ctypes.c_uint32), ("flags", ctypes.c_uint32)]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """xksv_kv_append_args."""
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+                ("q_stride", ctypes.c_uint64 * 2), ("k_stride", ctypes.c_uint64 * 2),
+                ("v_stride", ctypes.c_uint64 * 2), ("q_out_stride", ctypes.c_uint64 * 2),
+                ("tokens", ctypes.c_uint64), ("table", ctypes.c_void_p), ("table_rows", ctypes.c_uint64),
+                ("table_cols", ctypes.c_uint64), ("table_stride", ctypes.c_uint64), ("seq", ctypes.c_void_p),
+                ("index", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+                ("rot_scale", ctypes.c_float), ("rot_dim", ctypes.c_uint32), ("q_heads", ctypes.c_uint32),
+                ("type", ctypes.c_uint32), ("flags", ctypes.c_uint32)]
+
+
+class KvAttendArgs(ctypes.Structure):
+    """xksv_kv_attend_args."""
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("q_stride", ctypes.c_uint64 * 2), ("out_stride", ctypes.c_uint64 * 2), ("seqs", ctypes.c_uint64),
+                ("table", ctypes.c_void_p), ("table_cols", ctypes.c_uint64), ("table_stride", ctypes.c_uint64),
+                ("lens", ctypes.c_void_p), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("window", ctypes.c_uint64), ("q_heads", ctypes.c_uint32), ("type", ctypes.c_uint32)]
+
+
 _SIGS = {
     "xksv_cuda_decode": ([ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t,
                           ctypes.c_void_p], ctypes.c_int),
@@ -88,7 +129,24 @@ _SIGS = {
     "xksv_cuda_decode_noalloc": ([ctypes.POINTER(Slab), ctypes.c_size_t, ctypes.c_void_p,
                                   ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t,
                                   ctypes.c_void_p], ctypes.c_int),
+    "xksv_plan_linear_workspace": ([ctypes.c_void_p, ctypes.c_size_t], ctypes.c_size_t),
+    "xksv_plan_linear": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.POINTER(LinearArgs),
+                          ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
+    "xksv_kv_create": ([ctypes.POINTER(KvDesc), ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
+    "xksv_kv_destroy": ([ctypes.c_void_p], None),
+    "xksv_kv_status": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
+    "xksv_kv_append": ([ctypes.c_void_p, ctypes.POINTER(KvAppendArgs), ctypes.c_void_p], ctypes.c_int),
+    "xksv_kv_attend_workspace": ([ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t],
+                                 ctypes.c_size_t),
+    "xksv_kv_attend": ([ctypes.c_void_p, ctypes.POINTER(KvAttendArgs), ctypes.c_void_p, ctypes.c_size_t,
+                        ctypes.c_void_p], ctypes.c_int),
 }
+
+# element types and activations of the linear layer and the key/value cache
+BF16, FP16, FP32, E4M3 = 1, 2, 3, 4
+TYPE_BY_NAME = {"torch.bfloat16": BF16, "torch.float16": FP16, "torch.float32": FP32, "torch.float8_e4m3fn": E4M3}
+ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+KV_INTERLEAVED = 1
 
 NOALLOC_MAX_SLABS = 4096
 # xksv_plan_set_gemm_route
@@ -236,6 +294,75 @@ def _rows(buf, nrows, batch, what):
     return int(buf), int(nrows)
 
 
+def _type(t, allowed, what):
+    """The element type code of tensor t, one of `allowed`."""
+    code = TYPE_BY_NAME.get(str(t.dtype))
+    if code not in allowed:
+        raise ValueError(f"{what}: dtype {t.dtype} is not supported")
+    return code
+
+
+def _matrix(t, rows, cols, what, device, least=False):
+    """(address, row stride) of a [rows, cols] tensor whose rows are contiguous
+    (with `least`, cols or more columns)."""
+    if t.dim() != 2 or t.shape[0] != rows or (t.shape[1] < cols if least else t.shape[1] != cols):
+        raise ValueError(f"{what}: shape {tuple(t.shape)} is not [{rows}, {cols}]")
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        raise ValueError(f"{what}: rows must be contiguous")
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    return t.data_ptr(), max(t.stride(0), 0)
+
+
+def _heads(t, rows, heads, dim, what, device):
+    """(address, (row, head) strides) of a [rows, heads, dim] tensor whose
+    last dimension is contiguous."""
+    if tuple(t.shape) != (rows, heads, dim):
+        raise ValueError(f"{what}: shape {tuple(t.shape)} is not [{rows}, {heads}, {dim}]")
+    if t.stride(2) != 1 and dim > 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    return t.data_ptr(), (t.stride(0), t.stride(1))
+
+
+def _ints(t, n, what, device):
+    """Address of a contiguous int32 [n] tensor."""
+    if str(t.dtype) != "torch.int32" or tuple(t.shape) != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: a contiguous int32 [{n}] tensor is needed")
+    if t.device != device:
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    return t.data_ptr()
+
+
+def _table(t, device):
+    """(address, rows, columns, row stride) of an int32 page table."""
+    if str(t.dtype) != "torch.int32" or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError("table: an int32 [sequences, pages] tensor with contiguous rows is needed")
+    if t.device != device:
+        raise ValueError(f"table: on {t.device}, expected {device}")
+    return t.data_ptr(), t.shape[0], t.shape[1], t.stride(0)
+
+
+def _workspace(given, nbytes, device, stream):
+    """(tensor, address, bytes) of a call's workspace: the caller's uint8 tensor, or a
+    new one from torch's allocator of the call's stream, so that neither two
+    calls nor two captured graphs share one."""
+    import torch
+    if given is not None:
+        if given.device != device or not given.is_contiguous():
+            raise ValueError("workspace: a contiguous tensor on the call's device is needed")
+        return given, given.data_ptr(), given.numel() * given.element_size()
+    if not nbytes:
+        return None, None, 0
+    if stream == torch.cuda.current_stream(device).cuda_stream:
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    else:
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return buf, buf.data_ptr(), nbytes
+
+
 class Plan:
     """A device-resident plan over one payload buffer (see include/xksv_cuda.h).
     Device buffers are torch tensors (their sizes bound the call) or integer
@@ -272,6 +399,45 @@ class Plan:
         y, ny = _rows(d_y, y_rows, batch, "y")
         if self.lib.xksv_plan_gemm(self.handle, pay, npay, x, nx, y, ny, batch, stream):
             raise RuntimeError("xksv_plan_gemm refused the call or failed to launch")
+
+    def linear(self, d_payload, x, y, bias=None, act="none", mul=None, residual=None, stream=0, payload_bytes=None,
+               workspace=None):
+        """y = act(x W^T + bias) * mul + residual (xksv_plan_linear): x BF16
+        [batch, x columns], y BF16 or FP32 [batch, Y rows]; bias [Y rows], mul and
+        residual [batch, Y rows] are BF16 or FP32; act is a key of ACTS.  Rows may
+        be strided; residual or mul may be y.  `workspace` (uint8, at least
+        linear_workspace(batch) bytes) defaults to a new buffer per call."""
+        if act not in ACTS:
+            raise ValueError(f"unknown activation {act}")
+        device = x.device
+        pay, npay = dev_buffer(d_payload, payload_bytes, "payload")
+        if x.dim() != 2 or y.dim() != 2:
+            raise ValueError("x and y are [batch, columns]")
+        batch, rows = x.shape[0], y.shape[1]
+        _type(x, (BF16,), "x")
+        xp, xs = _matrix(x, batch, x.shape[1], "x", device)
+        yp, ys = _matrix(y, batch, rows, "y", device)
+        a = LinearArgs(xp, x.shape[1], xs, yp, rows, ys, batch)
+        a.y_type = _type(y, (BF16, FP32), "y")
+        if bias is not None:
+            a.bias_type = _type(bias, (BF16, FP32), "bias")
+            if tuple(bias.shape) != (rows,) or (rows > 1 and bias.stride(0) != 1) or bias.device != device:
+                raise ValueError(f"bias: a contiguous [{rows}] tensor on {device} is needed")
+            a.bias = bias.data_ptr()
+        if mul is not None:
+            a.mul_type = _type(mul, (BF16, FP32), "mul")
+            a.mul, a.mul_stride = _matrix(mul, batch, rows, "mul", device)
+        if residual is not None:
+            a.residual_type = _type(residual, (BF16, FP32), "residual")
+            a.residual, a.residual_stride = _matrix(residual, batch, rows, "residual", device)
+        a.act = ACTS[act]
+        ws, wp, wn = _workspace(workspace, self.linear_workspace(batch), device, stream)
+        if self.lib.xksv_plan_linear(self.handle, pay, npay, ctypes.byref(a), wp, wn, stream):
+            raise RuntimeError("xksv_plan_linear refused the call or failed to launch")
+
+    def linear_workspace(self, batch):
+        """Bytes of workspace a linear call of `batch` tokens needs."""
+        return self.lib.xksv_plan_linear_workspace(self.handle, batch)
 
     def index(self, d_payload, stream=0, payload_bytes=None):
         """Builds the tile index (xksv_plan_index); returns 0, or 1 on a bad slab."""
@@ -315,6 +481,141 @@ class Plan:
     def close(self):
         if self.handle:
             self.lib.xksv_plan_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KVCache:
+    """A paged key/value cache over two torch tensors (xksv_kv_*): k and v are
+    [pages, page_size, heads, dim] (layout "nhd") or [pages, heads, page_size,
+    dim] ("hnd") of BF16, FP16 or float8_e4m3fn, any strides that are
+    multiples of 16 bytes; k_scale and v_scale are FP32 [heads] for float8.
+    A page table is an int32 [sequences, pages] tensor of page numbers."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, layout="nhd", lib=None):
+        import torch
+        if layout not in ("nhd", "hnd"):
+            raise ValueError(f"unknown layout {layout}")
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.device.type != "cuda":
+            raise ValueError("k and v are CUDA tensors of one shape [pages, page_size, heads, dim] and dtype")
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("the last dimension of k and v must be contiguous")
+        self.lib = lib or load()
+        self.handle = None
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device, self.type = k.device, _type(k, (BF16, FP16, E4M3), "k")
+        order = (0, 1, 2) if layout == "nhd" else (0, 2, 1)  # page, token, head
+        self.pages, self.page_size, self.kv_heads = (k.shape[i] for i in order)
+        self.head_dim = k.shape[3]
+        for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (self.kv_heads,)
+                                  or not s.is_contiguous() or s.device != self.device):
+                raise ValueError(f"{name}: a contiguous FP32 [{self.kv_heads}] tensor on {self.device} is needed")
+        nbytes = [(t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()) for t in (k, v)]
+        d = KvDesc(k.data_ptr(), v.data_ptr(), nbytes[0], nbytes[1], self.pages, self.page_size)
+        d.k_stride[:] = [k.stride(i) for i in order]
+        d.v_stride[:] = [v.stride(i) for i in order]
+        d.k_scale = k_scale.data_ptr() if k_scale is not None else None
+        d.v_scale = v_scale.data_ptr() if v_scale is not None else None
+        d.kv_heads, d.head_dim, d.type = self.kv_heads, self.head_dim, self.type
+        h = ctypes.c_void_p()
+        with torch.cuda.device(self.device):
+            if self.lib.xksv_kv_create(ctypes.byref(d), ctypes.byref(h)):
+                raise ValueError("xksv_kv_create rejected the cache")
+        self.handle = h
+
+    def append(self, k, v, table, index, seq=None, positions=None, inv_freq=None, rot_scale=1.0, interleaved=False,
+               q=None, q_out=None, stream=0):
+        """Rotates new keys (and queries) and writes keys and values to their
+        places (xksv_kv_append): k, v [tokens, heads, dim] and q, q_out [tokens,
+        query heads, dim] of one dtype; token t is token index[t] of sequence
+        seq[t] (default t; negative: padding, skipped), rotated by positions[t]
+        (default index[t]) and inv_freq FP32 [rotated dims / 2] (None: no
+        rotation).  q_out defaults to q, in place."""
+        n, dev = k.shape[0], self.device
+        a = KvAppendArgs()
+        a.type = _type(k, (BF16, FP16, FP32), "k")
+        a.k, a.k_stride[:] = _heads(k, n, self.kv_heads, self.head_dim, "k", dev)
+        a.v, a.v_stride[:] = _heads(v, n, self.kv_heads, self.head_dim, "v", dev)
+        if v.dtype != k.dtype:
+            raise ValueError("k and v are of one dtype")
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            if q.dtype != k.dtype or q_out.dtype != k.dtype or q.dim() != 3:
+                raise ValueError("q and q_out are [tokens, heads, dim] of k's dtype")
+            a.q_heads = q.shape[1]
+            a.q, a.q_stride[:] = _heads(q, n, q.shape[1], self.head_dim, "q", dev)
+            a.q_out, a.q_out_stride[:] = _heads(q_out, n, q.shape[1], self.head_dim, "q_out", dev)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        a.tokens = n
+        a.table, a.table_rows, a.table_cols, a.table_stride = _table(table, dev)
+        a.index = _ints(index, n, "index", dev)
+        if seq is not None:
+            a.seq = _ints(seq, n, "seq", dev)
+        if positions is not None:
+            a.positions = _ints(positions, n, "positions", dev)
+        if inv_freq is not None:
+            if str(inv_freq.dtype) != "torch.float32" or inv_freq.dim() != 1 or inv_freq.device != dev \
+                    or (inv_freq.numel() > 1 and inv_freq.stride(0) != 1):
+                raise ValueError(f"inv_freq: a contiguous FP32 vector on {dev} is needed")
+            a.inv_freq, a.rot_dim = inv_freq.data_ptr(), 2 * inv_freq.numel()
+        a.rot_scale = rot_scale
+        a.flags = KV_INTERLEAVED if interleaved else 0
+        if self.lib.xksv_kv_append(self.handle, ctypes.byref(a), stream):
+            raise RuntimeError("xksv_kv_append refused the call or failed to launch")
+
+    def attend(self, q, table, lens, out, lse=None, scale=None, window=0, softcap=0.0, stream=0, workspace=None):
+        """Attention of one new token per sequence over its lens[s] cached
+        tokens (xksv_kv_attend): q and out [sequences, query heads, dim] of the
+        cache's dtype (BF16 or FP16 over float8), lse FP32 [sequences, query
+        heads] or None; scale defaults to dim ** -0.5; window 0 sees the whole
+        sequence; softcap 0 is off.  `workspace` (uint8, at least
+        attend_workspace(...) bytes) defaults to a new buffer per call."""
+        dev, n = self.device, lens.shape[0]
+        if q.dim() != 3 or out.dtype != q.dtype:
+            raise ValueError("q and out are [sequences, heads, dim] of one dtype")
+        heads = q.shape[1]
+        a = KvAttendArgs()
+        a.type = _type(q, (BF16, FP16), "q")
+        a.q, a.q_stride[:] = _heads(q, n, heads, self.head_dim, "q", dev)
+        a.out, a.out_stride[:] = _heads(out, n, heads, self.head_dim, "out", dev)
+        if lse is not None:
+            if str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (n, heads) or not lse.is_contiguous() \
+                    or lse.device != dev:
+                raise ValueError(f"lse: a contiguous FP32 [{n}, {heads}] tensor on {dev} is needed")
+            a.lse = lse.data_ptr()
+        a.table, rows, a.table_cols, a.table_stride = _table(table, dev)
+        if rows < n:
+            raise ValueError(f"table: {rows} rows for {n} sequences")
+        a.seqs, a.q_heads = n, heads
+        a.lens = _ints(lens, n, "lens", dev)
+        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        if window < 0:
+            raise ValueError("window is not negative")
+        a.window, a.softcap = window, softcap
+        need = self.lib.xksv_kv_attend_workspace(self.handle, n, heads, a.table_cols)
+        ws, wp, wn = _workspace(workspace, need, dev, stream)
+        if self.lib.xksv_kv_attend(self.handle, ctypes.byref(a), wp, wn, stream):
+            raise RuntimeError("xksv_kv_attend refused the call or failed to launch")
+
+    def attend_workspace(self, seqs, q_heads, table_cols):
+        """Bytes of workspace an attend call needs."""
+        return self.lib.xksv_kv_attend_workspace(self.handle, seqs, q_heads, table_cols)
+
+    def status(self, stream=0):
+        """0 when no call met a page, place or length outside the cache since
+        the last call, else 1."""
+        return self.lib.xksv_kv_status(self.handle, stream)
+
+    def close(self):
+        if self.handle:
+            self.lib.xksv_kv_destroy(self.handle)
             self.handle = None
 
     def __del__(self):
