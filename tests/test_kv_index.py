@@ -53,6 +53,51 @@ def test_span_of_lengths_and_windows(tmp_path):
 """)
 
 
+def test_split_covers_every_block_once(tmp_path):
+    """Workers' block ranges tile all blocks; every unit is either written by
+    one worker or joined from exactly the slots its workers left."""
+    run_cpp(tmp_path, """
+  uint64_t seed = 1;
+  auto rnd = [&](uint64_t n) { seed = seed * 6364136223846793005ull + 1442695040888963407ull; return (seed >> 33) % n; };
+  for (int round = 0; round < 300; ++round) {
+    const uint64_t units = 1 + rnd(round % 3 ? 9 : 300), warps = 1 + rnd(round % 2 ? 1184 : 40);
+    std::vector<uint64_t> u0{0};
+    for (uint64_t u = 0; u < units; ++u) u0.push_back(u0.back() + 1 + rnd(rnd(4) ? 5 : 900));
+    const uint64_t total = u0.back(), workers = warps < total ? warps : total;
+    std::vector<int> seen(2 * workers, 0), done(units, 0);
+    struct Join { uint64_t u, i; uint32_t parts; };
+    std::vector<Join> joins;
+    std::vector<uint64_t> slot_unit(2 * workers, ~0ull);
+    for (uint64_t i = 0, u = 0; i < workers; ++i) {
+      const uint64_t a = kv_start(i, workers, total), b = kv_start(i + 1, workers, total);
+      assert(a < b && (i + 1 < workers || b == total) && (i || a == 0));
+      for (uint64_t t = a; t < b; ++t) assert(kv_owner(t, workers, total) == i);
+      while (u0[u + 1] <= a) ++u;
+      for (uint64_t v = u; v < units && u0[v] < b; ++v) {
+        const KvPiece p = kv_piece(i, a, b, u0[v], u0[v + 1], workers, total);
+        if (p.slot < 0) { assert(!done[v]); done[v] = 1; continue; }
+        assert(uint64_t(p.slot) < 2 * workers && !seen[p.slot]);
+        seen[p.slot] = 1; slot_unit[p.slot] = v;
+        if (p.parts) { assert(p.parts >= 2 && p.slot == int64_t(2 * i + 1)); joins.push_back({v, i, p.parts}); }
+      }
+    }
+    for (auto& j : joins) {
+      assert(!done[j.u]);
+      done[j.u] = 1;
+      for (uint32_t k = 0; k < j.parts; ++k) {
+        const uint64_t slot = k ? 2 * (j.i + k) : 2 * j.i + 1;
+        assert(slot < 2 * workers && slot_unit[slot] == j.u);
+        slot_unit[slot] = ~0ull;
+      }
+    }
+    for (uint64_t u = 0; u < units; ++u) assert(done[u]);
+    for (uint64_t x : slot_unit) assert(x == ~0ull);
+  }
+  assert(kv_blocks(kv_span(0, 4, 16, 0), 16) == 1 && kv_blocks(kv_span(17, 4, 16, 0), 16) == 2);
+  assert(kv_blocks(kv_span(64, 4, 16, 1), 16) == 1 && kv_blocks(kv_span(-3, 4, 16, 1), 16) == 1);
+""")
+
+
 def test_binding_refuses_before_the_library():
     torch = pytest.importorskip("torch")
     import xksv_gpu as xg

@@ -11,12 +11,12 @@
 #include <new>
 #include <utility>
 
-#include "kernels.h"
+#include "kv_cache.h"
 #include "kv_index.h"
-#include "xksv_cuda.h"
+#include "xksv_types.h"
 
 struct xksv_kv {
-  int device = 0;
+  int device = 0, sms = 148;
   xksv_kv_desc d{};
   int* d_status = nullptr;
   int* h_status = nullptr;
@@ -71,12 +71,6 @@ __device__ __forceinline__ E4m3 from_float<E4m3>(float x) {
 // --------------------------------------------------------------- append ---
 constexpr int AT = 256;         // threads per token
 constexpr int kMaxPairs = 128;  // head_dim <= 256
-
-struct AppendArgs {
-  xksv_kv_append_args a;
-  xksv_kv_desc c;
-  int* status;
-};
 
 // One CTA per token: its angles once in shared memory, then its heads.
 template <class TI, class TC>
@@ -155,87 +149,6 @@ cudaError_t append_cache(const AppendArgs& p, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-// --------------------------------------------------------------- attend ---
-constexpr int DT = 128;  // threads per (sequence, query head)
-
-struct AttendArgs {
-  xksv_kv_attend_args a;
-  xksv_kv_desc c;
-  int* status;
-};
-
-// One CTA per (sequence, query head); a warp takes every fourth token, its
-// lanes the dims, with a running maximum and sum; the warps join at the end.
-template <class TQ, class TC>
-__global__ void __launch_bounds__(DT) kv_attend_kernel(const AttendArgs p) {
-  __shared__ float sm[DT / 32], sl[DT / 32], so[DT / 32][256];
-  const uint64_t s = blockIdx.y;
-  const uint32_t h = blockIdx.x, g = h / (p.a.q_heads / p.c.kv_heads), D = p.c.head_dim;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const TQ* q = static_cast<const TQ*>(p.a.q) + s * p.a.q_stride[0] + h * p.a.q_stride[1];
-  TQ* out = static_cast<TQ*>(p.a.out) + s * p.a.out_stride[0] + h * p.a.out_stride[1];
-  const KvSpan span = kv_span(p.a.lens[s], p.a.table_cols, p.c.page_size, p.a.window);
-  if (!span.ok && threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
-  const int64_t L = span.length, j0 = span.first;
-  const float ks = (p.c.k_scale ? p.c.k_scale[g] : 1.f) * p.a.scale;
-  const float vs = p.c.v_scale ? p.c.v_scale[g] : 1.f;
-  float qr[8], o[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t d = i * 32 + lane;
-    qr[i] = d < D ? to_float(q[d]) : 0.f;
-    o[i] = 0.f;
-  }
-  for (int64_t j = j0 + warp; j < L; j += DT / 32) {
-    const int64_t page = kv_page(p.a.table, p.a.seqs, p.a.table_cols, p.a.table_stride, p.c.pages, p.c.page_size, s, j);
-    if (page < 0) {
-      if (lane == 0) atomicOr(p.status, kStatusHeader);
-      continue;
-    }
-    const uint64_t place = uint64_t(j) % p.c.page_size;
-    const TC* k = static_cast<const TC*>(p.c.k) + uint64_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2];
-    const TC* v = static_cast<const TC*>(p.c.v) + uint64_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2];
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 32 + lane < D) dot = fmaf(qr[i], to_float(k[i * 32 + lane]), dot);
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    float t = dot * ks;
-    if (p.a.softcap > 0.f) t = p.a.softcap * tanhf(t / p.a.softcap);
-    const float mn = fmaxf(m, t), base = mn == -INFINITY ? 0.f : mn;
-    const float f = expf(m - base), w = expf(t - base);
-    l = l * f + w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 32 + lane < D) o[i] = o[i] * f + w * to_float(v[i * 32 + lane]);
-    m = mn;
-  }
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) so[warp][i * 32 + lane] = o[i];
-  __syncthreads();
-  float mt = -INFINITY, lt = 0.f;
-  for (int w = 0; w < DT / 32; ++w) mt = fmaxf(mt, sm[w]);
-  const float base = mt == -INFINITY ? 0.f : mt;
-  for (int w = 0; w < DT / 32; ++w) lt += sl[w] * expf(sm[w] - base);
-  for (uint32_t d = threadIdx.x; d < D; d += DT) {
-    float x = 0.f;
-    for (int w = 0; w < DT / 32; ++w) x += so[w][d] * expf(sm[w] - base);
-    out[d] = from_float<TQ>(lt > 0.f || lt != lt ? x * vs / lt : 0.f);
-  }
-  if (threadIdx.x == 0 && p.a.lse) p.a.lse[s * p.a.q_heads + h] = base + logf(lt);
-}
-
-template <class TQ, class TC>
-cudaError_t attend_launch(const AttendArgs& p, cudaStream_t st) {
-  kv_attend_kernel<TQ, TC><<<dim3(p.a.q_heads, uint32_t(p.a.seqs)), DT, 0, st>>>(p);
-  return cudaGetLastError();
-}
-
 // ---------------------------------------------------------- C entry checks
 uint64_t elem_bytes(uint32_t type) { return type == XKSV_E4M3 ? 1 : type == XKSV_FP32 ? 4 : 2; }
 bool off_align(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0; }
@@ -275,6 +188,15 @@ bool rows_distinct(uint64_t n, uint64_t heads, uint64_t dim, const uint64_t* str
 bool strides_small(const uint64_t* stride) { return stride[0] < (1ull << 40) && stride[1] < (1ull << 40); }
 
 }  // namespace
+
+cudaError_t launch_kv_append(const AppendArgs& p, cudaStream_t st) {
+  switch (p.a.type) {
+    case XKSV_BF16: return append_cache<__nv_bfloat16>(p, st);
+    case XKSV_FP16: return append_cache<__half>(p, st);
+    default: return append_cache<float>(p, st);
+  }
+}
+
 }  // namespace xksv
 
 using namespace xksv;
@@ -298,7 +220,9 @@ int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** out) {
   auto* kv = new (std::nothrow) xksv_kv();
   if (!kv) return 1;
   kv->d = d;
-  const bool ok = cudaGetDevice(&kv->device) == cudaSuccess && cudaMalloc(&kv->d_status, sizeof(int)) == cudaSuccess &&
+  const bool ok = cudaGetDevice(&kv->device) == cudaSuccess &&
+                  cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, kv->device) == cudaSuccess &&
+                  cudaMalloc(&kv->d_status, sizeof(int)) == cudaSuccess &&
                   cudaMallocHost(&kv->h_status, sizeof(int)) == cudaSuccess &&
                   cudaMemset(kv->d_status, 0, sizeof(int)) == cudaSuccess && cudaStreamSynchronize(nullptr) == cudaSuccess;
   if (!ok) {
@@ -349,15 +273,13 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* a, void* stream
   if (!guard.ok) return 1;
   const AppendArgs p{*a, kv->d, kv->d_status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t err = a->type == XKSV_BF16   ? append_cache<__nv_bfloat16>(p, st)
-                          : a->type == XKSV_FP16 ? append_cache<__half>(p, st)
-                                                 : append_cache<float>(p, st);
-  return err == cudaSuccess ? 0 : 1;
+  return launch_kv_append(p, st) == cudaSuccess ? 0 : 1;
 }
 
-size_t xksv_kv_attend_workspace(const xksv_kv* kv, size_t, size_t, size_t) {
-  (void)kv;
-  return 0;
+size_t xksv_kv_attend_workspace(const xksv_kv* kv, size_t seqs, size_t q_heads, size_t table_cols) {
+  if (!kv || !seqs || !q_heads || q_heads % kv->d.kv_heads || q_heads > 65535 || !table_cols || table_cols >= (1ull << 31))
+    return 0;
+  return size_t(kv_attend_plan(kv->d, seqs, uint32_t(q_heads), table_cols, kv->sms).bytes);
 }
 
 int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* a, void* d_workspace, size_t workspace_bytes,
@@ -365,7 +287,7 @@ int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* a, void* d_work
   if (!kv || !a || !a->q_heads || a->q_heads % kv->d.kv_heads || a->q_heads > 65535) return 1;
   if (a->type != XKSV_BF16 && a->type != XKSV_FP16) return 1;
   if (kv->d.type != XKSV_E4M3 && kv->d.type != a->type) return 1;
-  if (!(a->softcap >= 0.f) || a->seqs > 65535) return 1;
+  if (!(a->softcap >= 0.f) || a->seqs >= (1ull << 31)) return 1;
   if (!a->seqs) return 0;
   if (!a->q || !a->out || !a->table || !a->lens || !a->table_cols || a->table_cols >= (1ull << 31) ||
       (a->seqs > 1 && a->table_stride < a->table_cols) || off_align(a->q, 2) || off_align(a->out, 2) ||
@@ -374,18 +296,13 @@ int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* a, void* d_work
   if (!strides_small(a->q_stride) || !strides_small(a->out_stride) ||
       !rows_distinct(a->seqs, a->q_heads, kv->d.head_dim, a->out_stride))
     return 1;
-  if (workspace_bytes < xksv_kv_attend_workspace(kv, a->seqs, a->q_heads, a->table_cols) || off_align(d_workspace, 256))
-    return 1;
+  const AttendPlan pl = kv_attend_plan(kv->d, a->seqs, a->q_heads, a->table_cols, kv->sms);
+  if (!d_workspace || workspace_bytes < pl.bytes || off_align(d_workspace, 256)) return 1;
   DeviceGuard guard(kv->device);
   if (!guard.ok) return 1;
-  const AttendArgs p{*a, kv->d, kv->d_status};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool e4 = kv->d.type == XKSV_E4M3;
-  const cudaError_t err = a->type == XKSV_BF16 ? (e4 ? attend_launch<__nv_bfloat16, E4m3>(p, st)
-                                                     : attend_launch<__nv_bfloat16, __nv_bfloat16>(p, st))
-                                               : (e4 ? attend_launch<__half, E4m3>(p, st)
-                                                     : attend_launch<__half, __half>(p, st));
-  return err == cudaSuccess ? 0 : 1;
+  auto* ws = static_cast<uint8_t*>(d_workspace);
+  const AttendArgs p{*a, kv->d, kv->d_status, reinterpret_cast<float*>(ws), reinterpret_cast<int4*>(ws + pl.joins_off)};
+  return launch_kv_attend(p, pl, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0 : 1;
 }
 
 }  // extern "C"
