@@ -59,28 +59,34 @@ def test_split_covers_every_block_once(tmp_path):
     run_cpp(tmp_path, """
   uint64_t seed = 1;
   auto rnd = [&](uint64_t n) { seed = seed * 6364136223846793005ull + 1442695040888963407ull; return (seed >> 33) % n; };
-  for (int round = 0; round < 300; ++round) {
+  for (int round = 0; round < 60; ++round) {
     const uint64_t units = 1 + rnd(round % 3 ? 9 : 300), warps = 1 + rnd(round % 2 ? 1184 : 40);
     std::vector<uint64_t> u0{0};
     for (uint64_t u = 0; u < units; ++u) u0.push_back(u0.back() + 1 + rnd(rnd(4) ? 5 : 900));
-    const uint64_t total = u0.back(), workers = warps < total ? warps : total;
+    const uint64_t total = u0.back();
+    const KvShare sh = kv_share(total, uint32_t(warps));
+    const uint64_t workers = sh.workers;
+    assert(workers == (warps < total ? warps : total));
     std::vector<int> seen(2 * workers, 0), done(units, 0);
     struct Join { uint64_t u, i; uint32_t parts; };
     std::vector<Join> joins;
     std::vector<uint64_t> slot_unit(2 * workers, ~0ull);
     for (uint64_t i = 0, u = 0; i < workers; ++i) {
-      const uint64_t a = kv_start(i, workers, total), b = kv_start(i + 1, workers, total);
+      const uint64_t a = kv_start(sh, i), b = kv_start(sh, i + 1);
       assert(a < b && (i + 1 < workers || b == total) && (i || a == 0));
-      for (uint64_t t = a; t < b; ++t) assert(kv_owner(t, workers, total) == i);
+      for (uint64_t t = a; t < b; ++t) assert(kv_owner(sh, t) == i);
       while (u0[u + 1] <= a) ++u;
       for (uint64_t v = u; v < units && u0[v] < b; ++v) {
-        const KvPiece p = kv_piece(i, a, b, u0[v], u0[v + 1], workers, total);
+        const KvPiece p = kv_piece(sh, i, a, b, u0[v], u0[v + 1]);
         if (p.slot < 0) { assert(!done[v]); done[v] = 1; continue; }
         assert(uint64_t(p.slot) < 2 * workers && !seen[p.slot]);
         seen[p.slot] = 1; slot_unit[p.slot] = v;
         if (p.parts) { assert(p.parts >= 2 && p.slot == int64_t(2 * i + 1)); joins.push_back({v, i, p.parts}); }
       }
     }
+    for (size_t x = 0; x < joins.size(); ++x)
+      for (size_t y = x + 1; y < joins.size() && joins[y].i / 8 == joins[x].i / 8; ++y)
+        assert(joins[x].parts <= 8 || joins[y].parts <= 8);
     for (auto& j : joins) {
       assert(!done[j.u]);
       done[j.u] = 1;
@@ -95,6 +101,7 @@ def test_split_covers_every_block_once(tmp_path):
   }
   assert(kv_blocks(kv_span(0, 4, 16, 0), 16) == 1 && kv_blocks(kv_span(17, 4, 16, 0), 16) == 2);
   assert(kv_blocks(kv_span(64, 4, 16, 1), 16) == 1 && kv_blocks(kv_span(-3, 4, 16, 1), 16) == 1);
+  assert(kv_blocks(kv_span(49, 4, 16, 2), 16) == 2 && kv_blocks(kv_span(49, 4, 16, 49), 32) == 2);
 """)
 
 

@@ -48,7 +48,7 @@ template <bool E8, int DP>
 struct Shape {
   static constexpr int ES = E8 ? 1 : 2;
   static constexpr int RB = DP * ES;              // bytes of a staged row
-  static constexpr int CH = RB / 16;              // 16-byte pieces of a row
+  static constexpr int CH = RB / 16;              // 16-byte pieces of a row (4 .. 32)
   static constexpr int BT = RB >= 256 ? 16 : 32;  // tokens of a block
   static constexpr int KV = BT * RB;              // bytes of a block's keys (or values)
   static constexpr bool QS = DP > 128;            // query fragments in shared memory, not registers
@@ -64,6 +64,9 @@ __device__ __forceinline__ uint32_t swz(uint32_t r, uint32_t c) {
   return CH >= 8 ? (c ^ (r & 7)) : (c ^ ((r >> 1) & 3));
 }
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -120,11 +123,11 @@ __device__ __forceinline__ void store16(uint16_t* p, float x) {
     *reinterpret_cast<__half*>(p) = __float2half_rn(x);
 }
 
-// Position in the list of blocks: sequence, unit of the sequence, block of the unit.
+// Position in the list of blocks: sequence, unit of the sequence, block of
+// the unit; the sequence's attended tokens [first, length) (below 2^31).
 struct Cursor {
-  uint32_t seq, unit;
-  uint64_t block, blocks;
-  KvSpan span;
+  uint32_t seq, unit, block, blocks;
+  int32_t first, length;
 };
 
 // Every warp's first block and the end of its range, found from the lengths.
@@ -134,7 +137,8 @@ struct Ranges {
   uint64_t before[kWarps];  // blocks ahead of that sequence
 };
 
-template <bool BF, bool E8, int DP>
+// FULL: head_dim is DP.
+template <bool BF, bool E8, int DP, bool FULL>
 __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_kernel(const AttendArgs p, const AttendPlan pl) {
   using Sh = Shape<E8, DP>;
   constexpr int CH = Sh::CH, BT = Sh::BT, RB = Sh::RB;
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
   __shared__ Ranges R;
   __shared__ uint64_t wsum[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t D = p.c.head_dim;
+  const uint32_t D = FULL ? DP : p.c.head_dim;
   const uint32_t U = p.c.kv_heads * pl.chunks;  // units of a sequence
   // the join may start launching; it waits for this grid's end
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
@@ -174,11 +178,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     if (w < warp) ahead += wsum[w];
     total += wsum[w];
   }
-  const uint64_t workers = min(uint64_t(pl.warps), total);
+  const KvShare share = kv_share(total, pl.warps);
   for (int w = 0; w < kWarps; ++w) {
-    const uint64_t i = uint64_t(blockIdx.x) * kWarps + w;
-    if (i >= workers) break;
-    const uint64_t a = kv_start(i, workers, total);
+    const uint32_t i = blockIdx.x * kWarps + w;
+    if (i >= share.workers) break;
+    const uint64_t a = kv_start(share, i);
     if (a >= ahead && a < ahead + mine) {
       uint64_t at = ahead, s = s0;
       for (uint64_t n; at + (n = blocks_of(s)) <= a; ++s) at += n;
@@ -187,11 +191,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     }
   }
   __syncthreads();
-  const uint64_t me = uint64_t(blockIdx.x) * kWarps + warp;
+  const uint32_t me = blockIdx.x * kWarps + warp;
   if (me >= pl.warps) return;
   if (lane == 0) p.joins[me] = make_int4(0, 0, 0, 0);
-  if (me >= workers) return;
-  const uint64_t a = kv_start(me, workers, total), b = kv_start(me + 1, workers, total);
+  if (me >= share.workers) return;
+  const uint64_t a = kv_start(share, me), b = kv_start(share, me + 1);
 
   uint8_t* ws = smem + warp * Sh::WARP;
   const uint32_t ring = smem_addr(ws), qsm = ring + kStages * 2 * Sh::KV;
@@ -203,73 +207,101 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     __syncwarp();
   }
 
-  auto start = [&](uint64_t t) {
-    Cursor c;
-    c.seq = R.seq[warp];
-    c.span = span_of(c.seq);
-    c.blocks = kv_blocks(c.span, BT);
-    const uint64_t in = t - R.before[warp];
-    c.unit = uint32_t(in / c.blocks);
-    c.block = in - c.unit * c.blocks;
-    return c;
+  auto enter = [&](Cursor& c) {
+    const KvSpan sp = span_of(c.seq);
+    c.first = int32_t(sp.first);
+    c.length = int32_t(sp.length);
+    c.blocks = uint32_t(kv_blocks(sp, BT));
   };
   auto step = [&](Cursor& c) {
     if (++c.block < c.blocks) return;
     c.block = 0;
     if (++c.unit < U) return;
     c.unit = 0;
-    if (++c.seq >= S) return;
-    c.span = span_of(c.seq);
-    c.blocks = kv_blocks(c.span, BT);
+    if (++c.seq < S) enter(c);
   };
 
   // ---- copies: a block's rows, each lane one token's place ----
   const uint32_t row_ch = D * Sh::ES / 16;  // 16-byte pieces that a row really has
-  const bool same = p.c.k_stride[0] == p.c.v_stride[0] && p.c.k_stride[1] == p.c.v_stride[1] && p.c.k_stride[2] == p.c.v_stride[2];
-  Cursor ld = start(a);
-  int64_t ld_page = -1;  // this lane's token of the next block to copy: its page
+  const bool run = p.c.page_size % 16 == 0;  // a block's sixteen tokens lie in one page
+  Cursor ld;  // of the next block to copy
+  ld.seq = R.seq[warp];
+  enter(ld);
+  {
+    const uint64_t in = a - R.before[warp];
+    ld.unit = uint32_t(in / ld.blocks);
+    ld.block = uint32_t(in - uint64_t(ld.unit) * ld.blocks);
+  }
+  Cursor cu = ld;  // of the block being worked on
+  // this lane's token of the next block to copy: its rows' offsets in bytes
+  bool ld_ok = false;
+  uint64_t ld_k = 0, ld_v = 0;
+  const uint32_t psize = uint32_t(p.c.page_size);
   auto look_up = [&]() {
-    const int64_t j = ld.span.first + int64_t(ld.block) * BT + lane;
-    ld_page = -1;
-    if (lane < BT && j < ld.span.length)
-      ld_page = kv_page(p.a.table, S, p.a.table_cols, p.a.table_stride, p.c.pages, p.c.page_size, ld.seq, j);
+    const uint32_t j = (uint32_t(ld.first) / BT + ld.block) * BT + lane;
+    ld_ok = false;
+    ld_k = ld_v = 0;
+    if (lane < BT && j >= uint32_t(ld.first) && j < uint32_t(ld.length)) {
+      const uint32_t col = pl.page_shift >= 0 ? j >> pl.page_shift : j / psize, place = j - col * psize;
+      const int32_t page = p.a.table[ld.seq * p.a.table_stride + col];  // kv_span keeps the length inside the table
+      if (uint32_t(page) < p.c.pages) {
+        const uint32_t g = ld.unit / pl.chunks;
+        ld_ok = true;
+        ld_k = (uint32_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2]) * Sh::ES;
+        ld_v = (uint32_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2]) * Sh::ES;
+      } else {
+        atomicOr(p.status, kStatusHeader);  // a page outside the cache
+      }
+    }
   };
-  auto issue = [&](uint64_t t) {  // copies block t (ld's position) into its stage, and steps on
-    const uint32_t stage = uint32_t((t - a) % kStages);
-    const int64_t j = ld.span.first + int64_t(ld.block) * BT + lane;
-    const uint32_t g = ld.unit / pl.chunks;
-    const bool ok = ld_page >= 0;
-    const uint64_t place = ok ? uint64_t(j) % p.c.page_size : 0, page = ok ? uint64_t(ld_page) : 0;
-    const uint64_t ko = (page * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2]) * Sh::ES;
-    const uint64_t vo = (page * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2]) * Sh::ES;
-    const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+  const uint8_t* const kb = static_cast<const uint8_t*>(p.c.k);
+  const uint8_t* const vb = static_cast<const uint8_t*>(p.c.v);
+  // a lane copies the same 16-byte piece of every 32 / CH-th row
+  const uint32_t lr = lane / CH, lc = lane % CH;
+  const uint64_t kstep = p.c.k_stride[1] * Sh::ES, vstep = p.c.v_stride[1] * Sh::ES;
+  auto issue = [&](uint32_t stage) {  // copies the looked-up block into a stage, and steps on
+    const uint32_t mask = __ballot_sync(0xffffffffu, ld_ok);
     if (lane == 0) masks[stage] = mask;
-    if (lane < BT && !ok && j < ld.span.length) atomicOr(p.status, kStatusHeader);  // a page outside the cache
     const uint32_t kd = ring + stage * 2 * Sh::KV, vd = kd + Sh::KV;
-    const uint8_t* kb = static_cast<const uint8_t*>(p.c.k);
-    const uint8_t* vb = static_cast<const uint8_t*>(p.c.v);
+    if (FULL && run && mask == (BT == 32 ? 0xffffffffu : 0xffffu)) {
+      // sixteen tokens of a page lie one token's stride apart
 #pragma unroll
-    for (int i = 0; i < BT * CH / 32; ++i) {
-      const uint32_t idx = i * 32 + lane, r = idx / CH, c = idx % CH;
-      const uint64_t kr = __shfl_sync(0xffffffffu, ko, r);
-      const uint64_t vr = same ? kr : __shfl_sync(0xffffffffu, vo, r);
-      // masked tokens are zeros: no garbage (NaN) meets their zero weight
-      const uint32_t n = (mask >> r) & 1 ? 16u : 0u;
-      if (c < row_ch) {
-        const uint32_t off = r * RB + swz<CH>(r, c) * 16;
-        cp_async16_zfill(kd + off, kb + kr + c * 16, n);
-        cp_async16_zfill(vd + off, vb + vr + c * 16, n);
+      for (int h = 0; h < BT / 16; ++h) {
+        const uint8_t* kp = kb + __shfl_sync(0xffffffffu, ld_k, 16 * h) + lr * kstep + lc * 16;
+        const uint8_t* vp = vb + __shfl_sync(0xffffffffu, ld_v, 16 * h) + lr * vstep + lc * 16;
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) {
+          const uint32_t r = 16 * h + i * (32 / CH) + lr, off = r * RB + swz<CH>(r, lc) * 16;
+          copy16(kd + off, kp);
+          copy16(vd + off, vp);
+          kp += (32 / CH) * kstep;
+          vp += (32 / CH) * vstep;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < BT * CH / 32; ++i) {
+        const uint32_t r = i * (32 / CH) + lr;
+        const uint64_t kr = __shfl_sync(0xffffffffu, ld_k, r), vr = __shfl_sync(0xffffffffu, ld_v, r);
+        // masked tokens are zeros: no garbage (NaN) meets their zero weight
+        const uint32_t n = (mask >> r) & 1 ? 16u : 0u;
+        if (FULL || lc < row_ch) {
+          const uint32_t off = r * RB + swz<CH>(r, lc) * 16;
+          cp_async16_zfill(kd + off, kb + kr + lc * 16, n);
+          cp_async16_zfill(vd + off, vb + vr + lc * 16, n);
+        }
       }
     }
     step(ld);
   };
 
   // ---- the unit being worked on ----
+  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+  constexpr float kUp = MB ? 0.f : 15.f;  // weights are scaled by 2^kUp
   const int r0 = lane >> 2, qc = lane & 3;
   constexpr int QK = Sh::QS ? 1 : KS;
   uint32_t qf[QK][4];
   float o[2 * KS][4], m[2], l[2], qs[2];  // rows r0 and r0 + 8
-  Cursor cu = start(a);
   uint32_t head0 = 0, heads = 0;  // the unit's query heads
   auto begin = [&]() {
     const uint32_t group = p.a.q_heads / p.c.kv_heads, g = cu.unit / pl.chunks, ch = cu.unit % pl.chunks;
@@ -298,8 +330,10 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
         }
       }
     }
-    qs[0] = scale[0];
-    qs[1] = scale[1];
+    // scores in powers of two (a softcap acts on the natural ones first)
+    const float pw = p.a.softcap > 0.f ? 1.f : kLog2e;
+    qs[0] = scale[0] * pw;
+    qs[1] = scale[1] * pw;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       uint32_t f[4] = {0, 0, 0, 0};
@@ -336,8 +370,6 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     m[0] = m[1] = -INFINITY;
     l[0] = l[1] = 0.f;
   };
-  constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
-  constexpr float kUp = MB ? 0.f : 15.f;  // weights are scaled by 2^kUp
 
   // dims of accumulator column i, element x (0, 1: row r0; 2, 3: row r0 + 8)
   auto dim_of = [&](int i, int x) -> uint32_t {
@@ -350,7 +382,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
     const uint64_t u0 = t - cu.block, u1 = u0 + cu.blocks;
-    const KvPiece piece = kv_piece(me, a, b, u0, u1, workers, total);
+    const KvPiece piece = kv_piece(share, me, a, b, u0, u1);
     if (piece.slot < 0) {
       const float vs = E8 && p.c.v_scale ? p.c.v_scale[cu.unit / pl.chunks] : 1.f;
 #pragma unroll
@@ -392,25 +424,28 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
   };
 
   look_up();
-  for (uint64_t t = a; t < a + kStages - 1; ++t) {
-    if (t < b) {
-      issue(t);
-      if (t + 1 < b) look_up();
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (a + i < b) {
+      issue(i);
+      if (a + i + 1 < b) look_up();
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   }
   begin();
+  uint32_t stage = 0, put = kStages - 1;  // stages to read and to fill next
   for (uint64_t t = a; t < b; ++t) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
     __syncwarp();
-    const uint32_t stage = uint32_t((t - a) % kStages);
     const uint32_t kd = ring + stage * 2 * Sh::KV, vd = kd + Sh::KV;
     const uint32_t mask = masks[stage];
     // the stage before this one is free: every lane has passed the barrier
     if (t + kStages - 1 < b) {
-      issue(t + kStages - 1);
+      issue(put);
       if (t + kStages < b) look_up();
     }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    put = put + 1 == kStages ? 0 : put + 1;
     asm volatile("cp.async.commit_group;\n" ::: "memory");
 
     // ---- S = Q K^T ----
@@ -421,7 +456,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
       for (int x = 0; x < 4; ++x) sc[n][x] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ks += E8 ? 2 : 1) {
-      if (uint32_t(ks * 16) >= D) break;
+      if (!FULL && uint32_t(ks * 16) >= D) break;
       uint32_t qa[2][4];
 #pragma unroll
       for (int y = 0; y < (E8 ? 2 : 1); ++y) {
@@ -453,17 +488,28 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     }
     // ---- softmax step, in powers of two ----
     float mx[2] = {m[0], m[1]};
+    if (p.a.softcap > 0.f) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[n][x] = kLog2e * p.a.softcap * tanhf(sc[n][x] * qs[x >> 1] / p.a.softcap);
+    } else {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[n][x] *= qs[x >> 1];
+    }
+    if (mask != (BT == 32 ? 0xffffffffu : 0xffffu)) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (!((mask >> (n * 8 + 2 * qc + (x & 1))) & 1)) sc[n][x] = -INFINITY;
+    }
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float s = sc[n][x] * qs[x >> 1];
-        if (p.a.softcap > 0.f) s = p.a.softcap * tanhf(s / p.a.softcap);
-        s *= kLog2e;
-        if (!((mask >> (n * 8 + 2 * qc + (x & 1))) & 1)) s = -INFINITY;
-        sc[n][x] = s;
-        mx[x >> 1] = fmaxf(mx[x >> 1], s);
-      }
+      for (int x = 0; x < 4; ++x) mx[x >> 1] = fmaxf(mx[x >> 1], sc[n][x]);
     float base[2];
     bool grew = false;
 #pragma unroll
@@ -520,7 +566,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
       const uint32_t row = tb * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
 #pragma unroll
       for (int dc = 0; dc < CH; dc += 2) {  // two 16-byte pieces of every row
-        if (uint32_t(dc) >= row_ch) break;
+        if (!FULL && uint32_t(dc) >= row_ch) break;
         uint32_t r[4];
         ldsm4t(vd + row * RB + swz<CH>(row, dc + (lane >> 4)) * 16, r);
         if (E8) {
@@ -549,71 +595,168 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 }
 
-constexpr int JT = 128;  // threads of a join
+constexpr int JT = 256;                // threads of a join
+constexpr uint32_t kJoin = JT / 32;    // workers whose units a CTA joins, and parts that a warp joins alone
 
-// Joins the pieces of the units whose first piece this CTA's workers hold:
-// CTA (x, y) the workers 4 x .. 4 x + 3 and head y of their chunk.  Each warp
-// takes every fourth piece, lanes the dims; then the four sums in order.
+// Joins the pieces of the units that workers 8 x .. 8 x + 7 begin, for query
+// head y of their chunk.  A unit of few parts takes one warp, all its loads in
+// flight at once; of the eight at most one has more than eight (its parts are
+// successive workers), and that one takes the whole CTA: the parts' weights
+// once in shared memory, then each warp every eighth part, lanes the dims;
+// last the warps' sums in order.
 template <bool BF>
 __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const AttendPlan pl, float up) {
-  __shared__ float so[JT / 32][256];
-  __shared__ float sl[JT / 32];
+  extern __shared__ float weight[];  // [workers]
+  __shared__ __align__(16) float so[JT / 32][256];
+  __shared__ float red[2][JT / 32];
+  __shared__ int4 big;
+  __shared__ uint32_t big_at;
+  constexpr float kLn2 = 0.69314718055994531f;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t head = blockIdx.y, DP = pl.pad_dim, D = p.c.head_dim;
+  const uint32_t group = p.a.q_heads / p.c.kv_heads, st = pl.heads * DP + 2 * head;
+  if (threadIdx.x == 0) big_at = ~0u;
+  __syncthreads();
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  for (uint32_t w = 0; w < kWarps; ++w) {
-    const uint64_t i = uint64_t(blockIdx.x) * kWarps + w;
-    if (i >= pl.warps) break;
-    const int4 j = p.joins[i];
-    if (!j.z) continue;
-    const uint32_t group = p.a.q_heads / p.c.kv_heads, g = uint32_t(j.y) / pl.chunks, ch = uint32_t(j.y) % pl.chunks;
-    if (head >= min(pl.heads, group - ch * pl.heads)) continue;
-    const uint32_t h = g * group + ch * pl.heads + head;
-    auto slot = [&](int k) { return p.slots + uint64_t(k ? 2 * (i + k) : 2 * i + 1) * pl.slot_floats; };
-    const uint32_t st = pl.heads * DP + 2 * head;
-    float mt = -INFINITY;
-    for (int k = lane; k < j.z; k += 32) mt = fmaxf(mt, slot(k)[st]);
+  auto slot = [&](uint32_t i, uint32_t k) { return p.slots + uint64_t(k ? 2 * (i + k) : 2 * i + 1) * pl.slot_floats; };
+  struct Unit {
+    uint32_t head, kv_head;
+    bool mine;
+  };
+  auto unit_of = [&](int4 j) {
+    const uint32_t g = uint32_t(j.y) / pl.chunks, ch = uint32_t(j.y) % pl.chunks;
+    return Unit{g * group + ch * pl.heads + head, g, head < min(pl.heads, group - ch * pl.heads)};
+  };
+  auto out_of = [&](int4 j, const Unit& u) {
+    return static_cast<uint16_t*>(p.a.out) + uint64_t(j.x) * p.a.out_stride[0] + u.head * p.a.out_stride[1];
+  };
+  auto scale_of = [&](const Unit& u, float l) {  // no weight at all: zeros
+    return l > 0.f || l != l ? (p.c.v_scale ? p.c.v_scale[u.kv_head] : 1.f) / l : 0.f;
+  };
+  auto put_lse = [&](int4 j, const Unit& u, float base, float l) {
+    if (p.a.lse)
+      p.a.lse[uint64_t(j.x) * p.a.q_heads + u.head] = l > 0.f || l != l ? (base + log2f(l) - up) * kLn2 : -INFINITY;
+  };
+  const uint32_t i = blockIdx.x * kJoin + warp;
+  const int4 j = i < pl.warps ? p.joins[i] : make_int4(0, 0, 0, 0);
+  if (uint32_t(j.z) > kJoin) {
+    if (lane == 0) {
+      big = j;
+      big_at = i;
+    }
+  } else if (j.z) {
+    const Unit u = unit_of(j);
+    if (u.mine) {
+      float m[kJoin], w[kJoin], l = 0.f, base = -INFINITY;
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
-    const float base = mt == -INFINITY ? 0.f : mt;
-    float acc[8], lt = 0.f;
+      for (uint32_t k = 0; k < kJoin; ++k) {
+        m[k] = k < uint32_t(j.z) ? slot(i, k)[st] : -INFINITY;
+        w[k] = k < uint32_t(j.z) ? slot(i, k)[st + 1] : 0.f;
+      }
+      float acc[8] = {};
+      float v[kJoin][4];  // 128 dims of every part at a time
+      auto fetch = [&](uint32_t d0) {
 #pragma unroll
-    for (int x = 0; x < 8; ++x) acc[x] = 0.f;
-#pragma unroll 4
-    for (int k = warp; k < j.z; k += JT / 32) {
-      const float* s = slot(k);
-      const float f = exp2f(s[st] - base);
-      lt += s[st + 1] * f;
+        for (uint32_t k = 0; k < kJoin; ++k)
+#pragma unroll
+          for (uint32_t x = 0; x < 4; ++x) {
+            const uint32_t d = d0 + x * 32 + lane;
+            v[k][x] = k < uint32_t(j.z) && d < D ? slot(i, k)[head * DP + d] : 0.f;
+          }
+      };
+      fetch(0);
+#pragma unroll
+      for (uint32_t k = 0; k < kJoin; ++k) base = fmaxf(base, m[k]);
+      base = base == -INFINITY ? 0.f : base;
+#pragma unroll
+      for (uint32_t k = 0; k < kJoin; ++k) {
+        m[k] = k < uint32_t(j.z) ? exp2f(m[k] - base) : 0.f;
+        l += w[k] * m[k];
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < kJoin; ++k)
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) acc[x] += k < uint32_t(j.z) ? v[k][x] * m[k] : 0.f;
+      if (D > 128) {
+        fetch(128);
+#pragma unroll
+        for (uint32_t k = 0; k < kJoin; ++k)
+#pragma unroll
+          for (uint32_t x = 0; x < 4; ++x) acc[4 + x] += k < uint32_t(j.z) ? v[k][x] * m[k] : 0.f;
+      }
+      const float f = scale_of(u, l);
+      const bool some = l > 0.f || l != l;
+      uint16_t* out = out_of(j, u);
 #pragma unroll
       for (int x = 0; x < 8; ++x)
-        if (x * 32 + lane < D) acc[x] += s[head * DP + x * 32 + lane] * f;
+        if (x * 32 + lane < D) store16<BF>(out + x * 32 + lane, some ? acc[x] * f : 0.f);
+      if (lane == 0) put_lse(j, u, base, l);
     }
-#pragma unroll
-    for (int x = 0; x < 8; ++x) so[warp][x * 32 + lane] = acc[x];
-    if (lane == 0) sl[warp] = lt;
-    __syncthreads();
-    float l = 0.f;
-    for (int k = 0; k < JT / 32; ++k) l += sl[k];
-    const bool some = l > 0.f || l != l;
-    const float f = some ? (p.c.v_scale ? p.c.v_scale[g] : 1.f) / l : 0.f;
-    uint16_t* out = static_cast<uint16_t*>(p.a.out) + uint64_t(j.x) * p.a.out_stride[0] + h * p.a.out_stride[1];
-    for (uint32_t d = threadIdx.x; d < D; d += JT) {
-      float x = 0.f;
-      for (int k = 0; k < JT / 32; ++k) x += so[k][d];
-      store16<BF>(out + d, some ? x * f : 0.f);
-    }
-    if (threadIdx.x == 0 && p.a.lse)
-      p.a.lse[uint64_t(j.x) * p.a.q_heads + h] = some ? (base + log2f(l) - up) * 0.69314718055994531f : -INFINITY;
-    __syncthreads();
   }
+  __syncthreads();
+  const uint32_t many = big_at;
+  const int4 jm = big;
+  if (many == ~0u) return;
+  const Unit u = unit_of(jm);
+  if (!u.mine) return;
+  const uint32_t parts = uint32_t(jm.z);
+  float mt = -INFINITY;
+  for (uint32_t k = threadIdx.x; k < parts; k += JT) {
+    weight[k] = slot(many, k)[st];
+    mt = fmaxf(mt, weight[k]);
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+  if (lane == 0) red[0][warp] = mt;
+  __syncthreads();
+  for (int w = 0; w < JT / 32; ++w) mt = fmaxf(mt, red[0][w]);
+  const float base = mt == -INFINITY ? 0.f : mt;
+  float l = 0.f;
+  for (uint32_t k = threadIdx.x; k < parts; k += JT) {
+    weight[k] = exp2f(weight[k] - base);
+    l += slot(many, k)[st + 1] * weight[k];
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = 0.f;
+  for (int w = 0; w < JT / 32; ++w) l += red[1][w];
+  // four dims a lane, two such rows for more than 128 dims
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const uint32_t d = (y * 32 + lane) * 4;
+    if (d >= D) break;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (uint32_t k = warp; k < parts; k += JT / 32) {
+      const float4 v = *reinterpret_cast<const float4*>(slot(many, k) + head * DP + d);
+      const float f = weight[k];
+      acc.x += v.x * f;
+      acc.y += v.y * f;
+      acc.z += v.z * f;
+      acc.w += v.w * f;
+    }
+    *reinterpret_cast<float4*>(&so[warp][d]) = acc;
+  }
+  __syncthreads();
+  const float f = scale_of(u, l);
+  const bool some = l > 0.f || l != l;
+  uint16_t* out = out_of(jm, u);
+  for (uint32_t d = threadIdx.x; d < D; d += JT) {
+    float x = 0.f;
+    for (int w = 0; w < JT / 32; ++w) x += so[w][d];
+    store16<BF>(out + d, some ? x * f : 0.f);
+  }
+  if (threadIdx.x == 0) put_lse(jm, u, base, l);
 }
 
 int pad_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-template <bool BF, bool E8, int DP>
+template <bool BF, bool E8, int DP, bool FULL>
 cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
   using Sh = Shape<E8, DP>;
-  const cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<BF, E8, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::CTA);
+  const cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<BF, E8, DP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::CTA);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((pl.warps + kWarps - 1) / kWarps);
@@ -625,20 +768,21 @@ cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t f = cudaLaunchKernelEx(&cfg, kv_attend_kernel<BF, E8, DP>, p, pl);
+  const cudaError_t f = cudaLaunchKernelEx(&cfg, kv_attend_kernel<BF, E8, DP, FULL>, p, pl);
   if (f != cudaSuccess) return f;
-  cfg.gridDim = dim3((pl.warps + kWarps - 1) / kWarps, pl.heads);
+  cfg.gridDim = dim3((pl.warps + kJoin - 1) / kJoin, pl.heads);
   cfg.blockDim = dim3(JT);
-  cfg.dynamicSmemBytes = 0;
+  cfg.dynamicSmemBytes = pl.warps * sizeof(float);
   return cudaLaunchKernelEx(&cfg, kv_join_kernel<BF>, p, pl, BF && !E8 ? 0.f : 15.f);
 }
 
 template <bool BF, bool E8>
 cudaError_t launch_dim(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
+  const bool full = p.c.head_dim == pl.pad_dim;
   switch (pl.pad_dim) {
-    case 64: return launch_attend<BF, E8, 64>(p, pl, st);
-    case 128: return launch_attend<BF, E8, 128>(p, pl, st);
-    default: return launch_attend<BF, E8, 256>(p, pl, st);
+    case 64: return full ? launch_attend<BF, E8, 64, true>(p, pl, st) : launch_attend<BF, E8, 64, false>(p, pl, st);
+    case 128: return full ? launch_attend<BF, E8, 128, true>(p, pl, st) : launch_attend<BF, E8, 128, false>(p, pl, st);
+    default: return full ? launch_attend<BF, E8, 256, true>(p, pl, st) : launch_attend<BF, E8, 256, false>(p, pl, st);
   }
 }
 
@@ -656,6 +800,9 @@ AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads
   pl.chunks = (group + 15) / 16;
   pl.heads = (group + pl.chunks - 1) / pl.chunks;
   pl.pad_dim = uint32_t(pad_dim(c.head_dim));
+  pl.page_shift = -1;
+  for (int k = 0; k < 31; ++k)
+    if (c.page_size == 1ull << k) pl.page_shift = k;
   uint32_t block = 16, per_sm = 1;
   if (c.type == XKSV_E4M3)
     shape_of<true>(int(pl.pad_dim), &block, &per_sm);

@@ -26,6 +26,7 @@ struct AttendArgs {
 // Warps that share the work of a call, and the workspace they need.
 struct AttendPlan {
   uint32_t warps, chunks, heads, pad_dim;  // query-head chunks per KV head, heads per chunk, padded head_dim
+  int page_shift;  // log2 page_size, -1 when that is no power of two
   uint64_t slot_floats, joins_off, bytes;
 };
 AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads, uint64_t table_cols, int sms);

@@ -38,31 +38,46 @@ XKSV_HD KvSpan kv_span(int64_t length, uint64_t cols, uint64_t page_size, uint64
 
 // ------------------------------------------------------ the attention's split
 // A unit is one (sequence, KV head, chunk of query heads); its cached tokens
-// are cut into blocks, an empty unit counting one.  All units' blocks in order,
-// `total` of them, are shared evenly among workers = min(warps, total): worker
-// i takes blocks [kv_start(i), kv_start(i + 1)), at least one.
+// are cut into blocks at multiples of the block's size (so that a block lies
+// in as few pages as it can), an empty unit counting one.
 XKSV_HD uint64_t kv_blocks(KvSpan s, uint32_t tokens) {
-  return s.length > s.first ? uint64_t(s.length - s.first + tokens - 1) / tokens : 1;
+  return s.length > s.first ? uint64_t(s.length + tokens - 1) / tokens - uint64_t(s.first) / tokens : 1;
 }
-XKSV_HD uint64_t kv_start(uint64_t worker, uint64_t workers, uint64_t total) { return worker * total / workers; }
-// The worker that holds a block: the largest i with kv_start(i) <= block.
-XKSV_HD uint64_t kv_owner(uint64_t block, uint64_t workers, uint64_t total) {
-  return ((block + 1) * workers - 1) / total;
+// All units' blocks in order, `total` > 0 of them, are shared evenly among
+// workers = min(warps, total): worker i takes blocks [start(i), start(i + 1)),
+// quot or quot + 1 of them.
+struct KvShare {
+  uint64_t total, quot;
+  uint32_t workers, more;  // the first `more` workers take quot + 1
+};
+XKSV_HD KvShare kv_share(uint64_t total, uint32_t warps) {
+  const uint32_t w = total < warps ? uint32_t(total) : warps;
+  const uint64_t q = total / w;
+  return KvShare{total, q, w, uint32_t(total - q * w)};
+}
+XKSV_HD uint64_t kv_start(const KvShare& s, uint32_t worker) {
+  return worker * s.quot + (worker < s.more ? worker : s.more);
+}
+// The worker that holds a block.
+XKSV_HD uint32_t kv_owner(const KvShare& s, uint64_t block) {
+  const uint64_t head = s.more * (s.quot + 1);
+  return block < head ? uint32_t(block / (s.quot + 1)) : s.more + uint32_t((block - head) / s.quot);
 }
 // What worker `i`, holding blocks [a, b), does with its piece of the unit of
 // blocks [u0, u1): writes the output (slot -1) or leaves the piece in a slot
 // for the join.  A worker leaves at most two pieces: one of a unit begun
 // before its blocks (slot 2 i), one of a unit that goes on behind them (slot
 // 2 i + 1).  parts > 0 on the unit's first piece: the join reads that one and
-// the slots 2 (i + 1), .. , 2 (i + parts - 1).
+// the slots 2 (i + 1), .. , 2 (i + parts - 1).  Among n workers in a row
+// one at most begins a unit of more than n parts.
 struct KvPiece {
   int64_t slot;
   uint32_t parts;
 };
-XKSV_HD KvPiece kv_piece(uint64_t i, uint64_t a, uint64_t b, uint64_t u0, uint64_t u1, uint64_t workers, uint64_t total) {
+XKSV_HD KvPiece kv_piece(const KvShare& s, uint32_t i, uint64_t a, uint64_t b, uint64_t u0, uint64_t u1) {
   if (u0 >= a && u1 <= b) return KvPiece{-1, 0};
-  if (u0 < a) return KvPiece{int64_t(2 * i), 0};
-  return KvPiece{int64_t(2 * i + 1), uint32_t(kv_owner(u1 - 1, workers, total) - i + 1)};
+  if (u0 < a) return KvPiece{2 * int64_t(i), 0};
+  return KvPiece{2 * int64_t(i) + 1, kv_owner(s, u1 - 1) - i + 1};
 }
 
 }  // namespace xksv
