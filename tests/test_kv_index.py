@@ -99,8 +99,8 @@ def test_split_covers_every_block_once(tmp_path):
     for (uint64_t u = 0; u < units; ++u) assert(done[u]);
     for (uint64_t x : slot_unit) assert(x == ~0ull);
   }
-  assert(kv_blocks(kv_span(0, 4, 16, 0), 16) == 1 && kv_blocks(kv_span(17, 4, 16, 0), 16) == 2);
-  assert(kv_blocks(kv_span(64, 4, 16, 1), 16) == 1 && kv_blocks(kv_span(-3, 4, 16, 1), 16) == 1);
+  assert(kv_blocks(kv_span(0, 4, 16, 0), 16) == 0 && kv_blocks(kv_span(17, 4, 16, 0), 16) == 2);
+  assert(kv_blocks(kv_span(64, 4, 16, 1), 16) == 1 && kv_blocks(kv_span(-3, 4, 16, 1), 16) == 0);
   assert(kv_blocks(kv_span(49, 4, 16, 2), 16) == 2 && kv_blocks(kv_span(49, 4, 16, 49), 32) == 2);
 """)
 

@@ -30,7 +30,7 @@ def build(verbose=False, force=False):
     deps = srcs + list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + [ROOT / "include" / "xksv_cuda.h"]
     if LIB.exists() and not force and all(LIB.stat().st_mtime >= d.stat().st_mtime for d in deps):
         return LIB
-    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "-Xcompiler", "-fPIC,-pthread",
+    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "--threads", "0", "-Xcompiler", "-fPIC,-pthread",
            "-I", str(ROOT / "include"), "-o", str(LIB) + ".tmp", *map(str, srcs), "-ldl"]
     if verbose:
         cmd[1:1] = ["-Xptxas", "-v"]

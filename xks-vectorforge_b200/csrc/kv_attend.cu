@@ -11,11 +11,13 @@
 //     kStages stages of shared memory by cp.async (16-byte pieces, XOR-swizzled
 //     rows), across units' borders, so the next unit's keys are on their way
 //     while one is finished.
-//   * Scores and sums run on mma.sync m16n8k16, the query heads as the 16 rows
-//     (the product needs 1 - 2 % of the tensor cores' rate; the wide tcgen05
-//     forms need 128 rows): S = Q K^T gives each lane the weights in the very
-//     layout that the second product reads them in.  Softmax statistics and
-//     sums are FP32 registers.
+//   * Scores and sums run on mma.sync m16n8k16 with the tokens, then the dims,
+//     as its 16 rows and eight query heads as its columns: S^T = K Q^T, O^T =
+//     V^T P^T (the product needs about 1 % of the tensor cores' rate; the wide
+//     tcgen05 forms need 128 rows).  Up to eight heads of a KV head cost one
+//     such product, and their softmax no padded rows; the weights pass from
+//     the first product's layout to the second's by movmatrix.  Softmax
+//     statistics and sums are FP32 registers.
 //   * Weights reach the second product as 16-bit numbers.  BF16: as a pair
 //     hi + lo of two products (2^-17 relative; one BF16 rounding, 2^-9, would
 //     be as coarse as the output's own).  FP16 and E4M3: as FP16 scaled by 2^15,
@@ -43,16 +45,17 @@ namespace {
 constexpr int kWarps = 4;   // per CTA
 constexpr int kStages = 3;  // blocks in a warp's ring
 
-// Shape of a kernel: the cache's elements (E8: E4M3), rows padded to DP dims.
-template <bool E8, int DP>
+// Shape of a kernel: the cache's elements (E8: E4M3), rows padded to DP dims,
+// NG groups of eight query heads.
+template <bool E8, int DP, int NG>
 struct Shape {
   static constexpr int ES = E8 ? 1 : 2;
   static constexpr int RB = DP * ES;              // bytes of a staged row
   static constexpr int CH = RB / 16;              // 16-byte pieces of a row (4 .. 32)
   static constexpr int BT = RB >= 256 ? 16 : 32;  // tokens of a block
   static constexpr int KV = BT * RB;              // bytes of a block's keys (or values)
-  static constexpr bool QS = DP > 128;            // query fragments in shared memory, not registers
-  static constexpr int QB = QS ? DP / 16 * 32 * 16 : 0;
+  static constexpr bool QS = DP * NG > 256;       // query fragments in shared memory, not registers
+  static constexpr int QB = QS ? DP / 16 * 32 * 8 * NG : 0;
   static constexpr int WARP = kStages * 2 * KV + QB + 16;  // + the stages' token masks
   static constexpr int CTA = kWarps * WARP;
   static constexpr int PER_SM = 2 * CTA <= 225 * 1024 ? 2 : 1;
@@ -92,10 +95,16 @@ __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, ui
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two E4M3 values (the low 16 bits of x) as FP16.
-__device__ __forceinline__ uint32_t e4m3x2(uint32_t x) {
+// Four E4M3 values as two pairs of FP16.
+__device__ __forceinline__ void e4m3x4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(x));
+}
+// The 8 x 8 matrix of 16-bit elements that the warp holds, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t r;
-  asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(r) : "r"(x));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -111,13 +120,11 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-template <bool BF>
-__device__ __forceinline__ float load16(const uint16_t* p) {
-  return BF ? __uint_as_float(uint32_t(*p) << 16) : __half2float(*reinterpret_cast<const __half*>(p));
+__device__ __forceinline__ float unpack16(bool bf, uint32_t x) {  // the low 16 bits
+  return bf ? __uint_as_float(x << 16) : __half2float(__ushort_as_half(uint16_t(x)));
 }
-template <bool BF>
-__device__ __forceinline__ void store16(uint16_t* p, float x) {
-  if (BF)
+__device__ __forceinline__ void store16(bool bf, uint16_t* p, float x) {
+  if (bf)
     *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(x);
   else
     *reinterpret_cast<__half*>(p) = __float2half_rn(x);
@@ -137,14 +144,14 @@ struct Ranges {
   uint64_t before[kWarps];  // blocks ahead of that sequence
 };
 
-// FULL: head_dim is DP.
-template <bool BF, bool E8, int DP, bool FULL>
-__global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_kernel(const AttendArgs p, const AttendPlan pl) {
-  using Sh = Shape<E8, DP>;
+// MB: BF16 products (else FP16); FULL: head_dim is DP.
+template <bool MB, bool E8, int DP, int NG, bool FULL>
+__global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_attend_kernel(const AttendArgs p, const AttendPlan pl) {
+  using Sh = Shape<E8, DP, NG>;
   constexpr int CH = Sh::CH, BT = Sh::BT, RB = Sh::RB;
-  constexpr bool MB = BF && !E8;       // BF16 products (else FP16)
-  constexpr int KS = DP / 16;          // 16-dim steps
-  constexpr int NB = BT / 8;           // 8-token columns of S
+  constexpr int KS = DP / 16;  // 16-dim steps
+  constexpr int TB = BT / 16;  // 16-token steps
+  const bool bf = E8 ? p.a.type == XKSV_BF16 : MB;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ Ranges R;
   __shared__ uint64_t wsum[kWarps];
@@ -178,6 +185,13 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     if (w < warp) ahead += wsum[w];
     total += wsum[w];
   }
+  // sequences without a token to attend to: zeros, by the CTAs in turn
+  for (uint64_t s = blockIdx.x; s < S; s += gridDim.x) {
+    if (blocks_of(s)) continue;
+    uint16_t* out = static_cast<uint16_t*>(p.a.out) + s * p.a.out_stride[0];
+    for (uint32_t x = threadIdx.x; x < p.a.q_heads * D; x += kWarps * 32) out[x / D * p.a.out_stride[1] + x % D] = 0;
+    for (uint32_t h = threadIdx.x; p.a.lse && h < p.a.q_heads; h += kWarps * 32) p.a.lse[s * p.a.q_heads + h] = -INFINITY;
+  }
   const KvShare share = kv_share(total, pl.warps);
   for (int w = 0; w < kWarps; ++w) {
     const uint32_t i = blockIdx.x * kWarps + w;
@@ -194,7 +208,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
   const uint32_t me = blockIdx.x * kWarps + warp;
   if (me >= pl.warps) return;
   if (lane == 0) p.joins[me] = make_int4(0, 0, 0, 0);
-  if (me >= share.workers) return;
+  if (me >= share.workers) return;  // all of them when there is no block
   const uint64_t a = kv_start(share, me), b = kv_start(share, me + 1);
 
   uint8_t* ws = smem + warp * Sh::WARP;
@@ -218,7 +232,16 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     c.block = 0;
     if (++c.unit < U) return;
     c.unit = 0;
-    if (++c.seq < S) enter(c);
+    // the next sequence that has tokens, 32 looked at a time (there is one:
+    // a range's last block is not stepped past)
+    for (uint64_t s = c.seq + 1; s < S; s += 32) {
+      const uint32_t some = __ballot_sync(0xffffffffu, s + lane < S && blocks_of(s + lane) != 0);
+      if (some) {
+        c.seq = uint32_t(s) + __ffs(some) - 1;
+        break;
+      }
+    }
+    enter(c);
   };
 
   // ---- copies: a block's rows, each lane one token's place ----
@@ -259,7 +282,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
   // a lane copies the same 16-byte piece of every 32 / CH-th row
   const uint32_t lr = lane / CH, lc = lane % CH;
   const uint64_t kstep = p.c.k_stride[1] * Sh::ES, vstep = p.c.v_stride[1] * Sh::ES;
-  auto issue = [&](uint32_t stage) {  // copies the looked-up block into a stage, and steps on
+  auto issue = [&](uint32_t stage) {  // copies the looked-up block into a stage
     const uint32_t mask = __ballot_sync(0xffffffffu, ld_ok);
     if (lane == 0) masks[stage] = mask;
     const uint32_t kd = ring + stage * 2 * Sh::KV, vd = kd + Sh::KV;
@@ -292,133 +315,133 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
         }
       }
     }
-    step(ld);
   };
 
   // ---- the unit being worked on ----
   constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
   constexpr float kUp = MB ? 0.f : 15.f;  // weights are scaled by 2^kUp
-  const int r0 = lane >> 2, qc = lane & 3;
-  constexpr int QK = Sh::QS ? 1 : KS;
-  uint32_t qf[QK][4];
-  float o[2 * KS][4], m[2], l[2], qs[2];  // rows r0 and r0 + 8
+  // A lane's elements of a product's 16 x 8 result: rows hr and hr + 8
+  // (elements 0, 1 and 2, 3), columns (query heads) 2 qc and 2 qc + 1.
+  const int hr = lane >> 2, qc = lane & 3;
+  uint32_t qf[Sh::QS ? 1 : KS][NG][2];
+  float o[NG][KS][4], m[NG][2], l[NG][2], qs[NG][2];
   uint32_t head0 = 0, heads = 0;  // the unit's query heads
+  const bool q_pairs = ((reinterpret_cast<uintptr_t>(p.a.q) / 2 | p.a.q_stride[0] | p.a.q_stride[1]) & 1) == 0;
   auto begin = [&]() {
     const uint32_t group = p.a.q_heads / p.c.kv_heads, g = cu.unit / pl.chunks, ch = cu.unit % pl.chunks;
     head0 = g * group + ch * pl.heads;
     heads = min(pl.heads, group - ch * pl.heads);
     const uint16_t* q = static_cast<const uint16_t*>(p.a.q) + cu.seq * p.a.q_stride[0];
-    float scale[2] = {p.a.scale, p.a.scale};
-    if (E8 && p.c.k_scale) scale[0] = scale[1] = p.a.scale * p.c.k_scale[g];
-    float up[2] = {1.f, 1.f};
-    if (E8) {
-      // the rows' powers of two
+    // scores in powers of two (a softcap acts on the natural ones first)
+    float scale = p.a.scale * (p.a.softcap > 0.f ? 1.f : kLog2e);
+    if (E8 && p.c.k_scale) scale *= p.c.k_scale[g];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float mx = 0.f;
-        if (uint32_t(r0 + 8 * h) < heads) {
-          const uint16_t* qr = q + (head0 + r0 + 8 * h) * p.a.q_stride[1];
-          for (uint32_t d = qc; d < D; d += 4) mx = fmaxf(mx, fabsf(load16<BF>(qr + d)));
+    for (int n = 0; n < NG; ++n) {
+      const uint32_t head = 8 * n + hr;  // the head whose query this lane holds parts of
+      const uint16_t* qr = q + (head0 + head) * p.a.q_stride[1];
+      uint32_t f[KS][2];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          // dims of this lane's element pairs: E4M3 rows give a lane four
+          // dims in a row (both pairs), 16-bit rows two and two
+          const uint32_t d = ks * 16 + (E8 ? 4 * qc + 2 * x : 2 * qc + 8 * x);
+          f[ks][x] = 0;
+          if (head < heads && (FULL || d < D))
+            f[ks][x] = q_pairs ? *reinterpret_cast<const uint32_t*>(qr + d) : uint32_t(qr[d]) | (uint32_t(qr[d + 1]) << 16);
         }
+      float mine = scale;
+      if (E8) {
+        float mx = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) mx = fmaxf(mx, fmaxf(fabsf(unpack16(bf, f[ks][x])), fabsf(unpack16(bf, f[ks][x] >> 16))));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        float up = 1.f;
         if (mx > 0.f && mx < INFINITY) {
           // an exponent whose inverse is a normal number too
           const int e = max(-110, min(126, 14 - ilogbf(mx)));
-          up[h] = ldexpf(1.f, e);
-          scale[h] = ldexpf(scale[h], -e);
+          up = __int_as_float((e + 127) << 23);
+          mine = ldexpf(scale, -e);
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) f[ks][x] = pack_f16(unpack16(bf, f[ks][x]) * up, unpack16(bf, f[ks][x] >> 16) * up);
+      }
+      qs[n][0] = __shfl_sync(0xffffffffu, mine, 8 * qc);
+      qs[n][1] = __shfl_sync(0xffffffffu, mine, 8 * qc + 4);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        if (Sh::QS) {
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};\n" ::"r"(qsm + ((ks * NG + n) * 32 + lane) * 8), "r"(f[ks][0]),
+                       "r"(f[ks][1])
+                       : "memory");
+        } else {
+          qf[Sh::QS ? 0 : ks][n][0] = f[ks][0];
+          qf[Sh::QS ? 0 : ks][n][1] = f[ks][1];
         }
       }
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[n][i][x] = 0.f;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
     }
-    // scores in powers of two (a softcap acts on the natural ones first)
-    const float pw = p.a.softcap > 0.f ? 1.f : kLog2e;
-    qs[0] = scale[0] * pw;
-    qs[1] = scale[1] * pw;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      uint32_t f[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (uint32_t(r0 + 8 * h) < heads) {
-          const uint16_t* qr = q + (head0 + r0 + 8 * h) * p.a.q_stride[1];
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            // dims of this lane's element pairs: E4M3 rows give a lane four
-            // dims in a row (both pairs), 16-bit rows two and two
-            const uint32_t d = ks * 16 + (E8 ? 4 * qc + 2 * x : 2 * qc + 8 * x);
-            if (d < D) {
-              if (E8)
-                f[h + 2 * x] = pack_f16(load16<BF>(qr + d) * up[h], load16<BF>(qr + d + 1) * up[h]);
-              else
-                f[h + 2 * x] = uint32_t(qr[d]) | (uint32_t(qr[d + 1]) << 16);
-            }
-          }
-        }
-      if (Sh::QS) {
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(qsm + (ks * 32 + lane) * 16), "r"(f[0]),
-                     "r"(f[1]), "r"(f[2]), "r"(f[3])
-                     : "memory");
-      } else {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) qf[Sh::QS ? 0 : ks][x] = f[x];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * KS; ++i)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
   };
-
-  // dims of accumulator column i, element x (0, 1: row r0; 2, 3: row r0 + 8)
-  auto dim_of = [&](int i, int x) -> uint32_t {
-    return E8 ? (i >> 1) * 16 + 4 * qc + 2 * (x & 1) + (i & 1) : i * 8 + 2 * qc + (x & 1);
-  };
+  // dim of row hr + 8 y of accumulator i
+  auto dim_of = [&](int i, int y) -> uint32_t { return i * 16 + (E8 ? 2 * hr + y : hr + 8 * y); };
   auto finish = [&](uint64_t t) {  // block t was the unit's last in this warp's range
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-    }
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], d);
     const uint64_t u0 = t - cu.block, u1 = u0 + cu.blocks;
     const KvPiece piece = kv_piece(share, me, a, b, u0, u1);
     if (piece.slot < 0) {
       const float vs = E8 && p.c.v_scale ? p.c.v_scale[cu.unit / pl.chunks] : 1.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t head = r0 + 8 * h;
-        if (head >= heads) continue;
-        const bool some = l[h] > 0.f || l[h] != l[h];
-        const float f = some ? vs / l[h] : 0.f;
-        uint16_t* out = static_cast<uint16_t*>(p.a.out) + cu.seq * p.a.out_stride[0] + (head0 + head) * p.a.out_stride[1];
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int i = 0; i < 2 * KS; ++i)
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t head = 8 * n + 2 * qc + h;
+          if (head >= heads) continue;
+          const bool some = l[n][h] > 0.f || l[n][h] != l[n][h];
+          const float f = some ? vs / l[n][h] : 0.f;
+          uint16_t* out = static_cast<uint16_t*>(p.a.out) + cu.seq * p.a.out_stride[0] + (head0 + head) * p.a.out_stride[1];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t d = dim_of(i, x);
-            if (d < D) store16<BF>(out + d, some ? o[i][2 * h + x] * f : 0.f);
-          }
-        if (qc == 0 && p.a.lse)
-          p.a.lse[uint64_t(cu.seq) * p.a.q_heads + head0 + head] =
-              some ? (m[h] == -INFINITY ? 0.f : m[h] + log2f(l[h]) - kUp) * kLn2 : -INFINITY;
-      }
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              if (FULL || dim_of(i, y) < D) store16(bf, out + dim_of(i, y), some ? o[n][i][2 * y + h] * f : 0.f);
+          if (hr == 0 && p.a.lse)
+            p.a.lse[uint64_t(cu.seq) * p.a.q_heads + head0 + head] =
+                some ? (m[n][h] == -INFINITY ? 0.f : m[n][h] + log2f(l[n][h]) - kUp) * kLn2 : -INFINITY;
+        }
     } else {
       float* slot = p.slots + uint64_t(piece.slot) * pl.slot_floats;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t head = r0 + 8 * h;
-        if (head >= heads) continue;
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int i = 0; i < 2 * KS; ++i)
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t head = 8 * n + 2 * qc + h;
+          if (head >= heads) continue;
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            if (dim_of(i, x) < D) slot[head * DP + dim_of(i, x)] = o[i][2 * h + x];
-        if (qc == 0) {
-          slot[pl.heads * DP + 2 * head] = m[h];
-          slot[pl.heads * DP + 2 * head + 1] = l[h];
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              if (FULL || dim_of(i, y) < D) slot[head * DP + dim_of(i, y)] = o[n][i][2 * y + h];
+          if (hr == 0) {
+            slot[pl.heads * DP + 2 * head] = m[n][h];
+            slot[pl.heads * DP + 2 * head + 1] = l[n][h];
+          }
         }
-      }
       if (piece.parts && lane == 0) p.joins[me] = make_int4(int(cu.seq), int(cu.unit), int(piece.parts), 0);
     }
   };
@@ -428,7 +451,10 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
   for (int i = 0; i < kStages - 1; ++i) {
     if (a + i < b) {
       issue(i);
-      if (a + i + 1 < b) look_up();
+      if (a + i + 1 < b) {
+        step(ld);
+        look_up();
+      }
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   }
@@ -442,155 +468,176 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP>::PER_SM) kv_attend_
     // the stage before this one is free: every lane has passed the barrier
     if (t + kStages - 1 < b) {
       issue(put);
-      if (t + kStages < b) look_up();
+      if (t + kStages < b) {
+        step(ld);
+        look_up();
+      }
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
     put = put + 1 == kStages ? 0 : put + 1;
     asm volatile("cp.async.commit_group;\n" ::: "memory");
 
-    // ---- S = Q K^T ----
-    float sc[NB][4];
+    // ---- S^T = K Q^T ----
+    float sc[TB][NG][4];
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) sc[n][x] = 0.f;
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sc[tb][n][x] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ks += E8 ? 2 : 1) {
       if (!FULL && uint32_t(ks * 16) >= D) break;
-      uint32_t qa[2][4];
+      constexpr int Y = E8 ? 2 : 1;
+      uint32_t qb[Y][NG][2];
 #pragma unroll
-      for (int y = 0; y < (E8 ? 2 : 1); ++y) {
-        if (Sh::QS)
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
-                       : "=r"(qa[y][0]), "=r"(qa[y][1]), "=r"(qa[y][2]), "=r"(qa[y][3])
-                       : "r"(qsm + ((ks + y) * 32 + lane) * 16)
-                       : "memory");
-        else
+      for (int y = 0; y < Y; ++y)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) qa[y][x] = qf[Sh::QS ? 0 : ks + y][x];
-      }
+        for (int n = 0; n < NG; ++n) {
+          if (Sh::QS) {
+            asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];\n"
+                         : "=r"(qb[y][n][0]), "=r"(qb[y][n][1])
+                         : "r"(qsm + (((ks + y) * NG + n) * 32 + lane) * 8)
+                         : "memory");
+          } else {
+            qb[y][n][0] = qf[Sh::QS ? 0 : ks + y][n][0];
+            qb[y][n][1] = qf[Sh::QS ? 0 : ks + y][n][1];
+          }
+        }
 #pragma unroll
-      for (int tb = 0; tb < BT / 16; ++tb) {
-        const uint32_t row = tb * 16 + (lane >> 4) * 8 + (lane & 7);
-        const uint32_t c = (E8 ? ks : 2 * ks) + ((lane >> 3) & 1);
+      for (int tb = 0; tb < TB; ++tb) {
+        // tokens 0 .. 7 and 8 .. 15 of one 16-byte piece, then of the next
+        const uint32_t row = tb * 16 + (lane & 15), c = (E8 ? ks : 2 * ks) + (lane >> 4);
         uint32_t r[4];
         ldsm4(kd + row * RB + swz<CH>(row, c) * 16, r);
         if (E8) {
-          mma<false>(sc[2 * tb], qa[0], e4m3x2(r[0]), e4m3x2(r[0] >> 16));
-          mma<false>(sc[2 * tb], qa[1], e4m3x2(r[1]), e4m3x2(r[1] >> 16));
-          mma<false>(sc[2 * tb + 1], qa[0], e4m3x2(r[2]), e4m3x2(r[2] >> 16));
-          mma<false>(sc[2 * tb + 1], qa[1], e4m3x2(r[3]), e4m3x2(r[3] >> 16));
+#pragma unroll
+          for (int y = 0; y < Y; ++y) {
+            uint32_t ka[4];
+            e4m3x4(r[2 * y], ka[0], ka[2]);
+            e4m3x4(r[2 * y + 1], ka[1], ka[3]);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) mma<false>(sc[tb][n], ka, qb[y][n][0], qb[y][n][1]);
+          }
         } else {
-          mma<MB>(sc[2 * tb], qa[0], r[0], r[1]);
-          mma<MB>(sc[2 * tb + 1], qa[0], r[2], r[3]);
+#pragma unroll
+          for (int n = 0; n < NG; ++n) mma<MB>(sc[tb][n], r, qb[0][n][0], qb[0][n][1]);
         }
       }
     }
     // ---- softmax step, in powers of two ----
-    float mx[2] = {m[0], m[1]};
     if (p.a.softcap > 0.f) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sc[n][x] = kLog2e * p.a.softcap * tanhf(sc[n][x] * qs[x >> 1] / p.a.softcap);
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            sc[tb][n][x] = kLog2e * p.a.softcap * tanhf(sc[tb][n][x] * qs[n][x & 1] / p.a.softcap);
     } else {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sc[n][x] *= qs[x >> 1];
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[tb][n][x] *= qs[n][x & 1];
     }
     if (mask != (BT == 32 ? 0xffffffffu : 0xffffu)) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
-          if (!((mask >> (n * 8 + 2 * qc + (x & 1))) & 1)) sc[n][x] = -INFINITY;
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (!((mask >> (tb * 16 + hr + 8 * (x >> 1))) & 1)) sc[tb][n][x] = -INFINITY;
     }
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) mx[x >> 1] = fmaxf(mx[x >> 1], sc[n][x]);
-    float base[2];
+    float mx[NG][2], base[NG][2];
     bool grew = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-      base[h] = mx[h] == -INFINITY ? 0.f : mx[h] - kUp;
-      grew |= mx[h] != m[h];
-    }
-    if (__any_sync(0xffffffffu, grew)) {
+    for (int n = 0; n < NG; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float f = exp2_fast(m[h] - (mx[h] == -INFINITY ? 0.f : mx[h]));
-        l[h] *= f;
+        float v = m[n][h];
 #pragma unroll
-        for (int i = 0; i < 2 * KS; ++i) {
-          o[i][2 * h] *= f;
-          o[i][2 * h + 1] *= f;
-        }
-        m[h] = mx[h];
+        for (int tb = 0; tb < TB; ++tb) v = fmaxf(v, fmaxf(sc[tb][n][h], sc[tb][n][2 + h]));
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, d));
+        mx[n][h] = v;
+        base[n][h] = v == -INFINITY ? 0.f : v - kUp;
+        grew |= v != m[n][h];
       }
+    if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float f = exp2_fast(m[n][h] - (mx[n][h] == -INFINITY ? 0.f : mx[n][h]));
+          l[n][h] *= f;
+#pragma unroll
+          for (int i = 0; i < KS; ++i) {
+            o[n][i][h] *= f;
+            o[n][i][2 + h] *= f;
+          }
+          m[n][h] = mx[n][h];
+        }
     }
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+    for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        sc[n][x] = exp2_fast(sc[n][x] - base[x >> 1]);
-        l[x >> 1] += sc[n][x];
-      }
-    // ---- O += P V ----
+      for (int n = 0; n < NG; ++n)
 #pragma unroll
-    for (int tb = 0; tb < BT / 16; ++tb) {
-      const float* s0 = sc[2 * tb];
-      const float* s1 = sc[2 * tb + 1];
-      uint32_t hi[4], lo[4];
-      if (MB) {
-        hi[0] = pack_bf16(s0[0], s0[1]);
-        hi[1] = pack_bf16(s0[2], s0[3]);
-        hi[2] = pack_bf16(s1[0], s1[1]);
-        hi[3] = pack_bf16(s1[2], s1[3]);
-        auto rest = [](uint32_t h, float x, float y) {
-          return pack_bf16(x - __uint_as_float(h << 16), y - __uint_as_float(h & 0xffff0000u));
-        };
-        lo[0] = rest(hi[0], s0[0], s0[1]);
-        lo[1] = rest(hi[1], s0[2], s0[3]);
-        lo[2] = rest(hi[2], s1[0], s1[1]);
-        lo[3] = rest(hi[3], s1[2], s1[3]);
-      } else {
-        hi[0] = pack_f16(s0[0], s0[1]);
-        hi[1] = pack_f16(s0[2], s0[3]);
-        hi[2] = pack_f16(s1[0], s1[1]);
-        hi[3] = pack_f16(s1[2], s1[3]);
-      }
-      const uint32_t row = tb * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+        for (int x = 0; x < 4; ++x) {
+          sc[tb][n][x] = exp2_fast(sc[tb][n][x] - base[n][x & 1]);
+          l[n][x & 1] += sc[tb][n][x];
+        }
+    // ---- O^T += V^T P^T ----
 #pragma unroll
-      for (int dc = 0; dc < CH; dc += 2) {  // two 16-byte pieces of every row
-        if (!FULL && uint32_t(dc) >= row_ch) break;
+    for (int tb = 0; tb < TB; ++tb) {
+      uint32_t hi[NG][2], lo[NG][2];
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float s0 = sc[tb][n][2 * y], s1 = sc[tb][n][2 * y + 1];
+          const uint32_t w = MB ? pack_bf16(s0, s1) : pack_f16(s0, s1);
+          hi[n][y] = transpose8(w);
+          if (MB) lo[n][y] = transpose8(pack_bf16(s0 - __uint_as_float(w << 16), s1 - __uint_as_float(w & 0xffff0000u)));
+        }
+#pragma unroll
+      for (int i = 0; i < KS; i += E8 ? 2 : 1) {  // 16 dims a product
+        if (!FULL && uint32_t(i * 16) >= D) break;
         uint32_t r[4];
-        ldsm4t(vd + row * RB + swz<CH>(row, dc + (lane >> 4)) * 16, r);
         if (E8) {
+          // tokens 0 .. 7 and 8 .. 15 of one 16-byte piece, then of the next
+          const uint32_t row = tb * 16 + (lane & 15);
+          ldsm4t(vd + row * RB + swz<CH>(row, i + (lane >> 4)) * 16, r);
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             // bytes (dim 2n, 2n + 1) of two tokens -> dim 2n of both, dim 2n + 1 of both
-            const uint32_t t0 = __byte_perm(r[2 * y], 0, 0x3120), t1 = __byte_perm(r[2 * y + 1], 0, 0x3120);
-            mma<false>(o[2 * (dc + y)], hi, e4m3x2(t0), e4m3x2(t1));
-            mma<false>(o[2 * (dc + y) + 1], hi, e4m3x2(t0 >> 16), e4m3x2(t1 >> 16));
+            uint32_t va[4];
+            e4m3x4(__byte_perm(r[2 * y], 0, 0x3120), va[0], va[1]);
+            e4m3x4(__byte_perm(r[2 * y + 1], 0, 0x3120), va[2], va[3]);
+#pragma unroll
+            for (int n = 0; n < NG; ++n) mma<false>(o[n][i + y], va, hi[n][0], hi[n][1]);
           }
         } else {
-          mma<MB>(o[dc], hi, r[0], r[1]);
-          mma<MB>(o[dc + 1], hi, r[2], r[3]);
-          if (MB) {
-            mma<MB>(o[dc], lo, r[0], r[1]);
-            mma<MB>(o[dc + 1], lo, r[2], r[3]);
+          // dims 0 .. 7 and 8 .. 15 of tokens 0 .. 7, then of tokens 8 .. 15
+          const uint32_t row = tb * 16 + (lane >> 4) * 8 + (lane & 7);
+          ldsm4t(vd + row * RB + swz<CH>(row, 2 * i + ((lane >> 3) & 1)) * 16, r);
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            mma<MB>(o[n][i], r, hi[n][0], hi[n][1]);
+            if (MB) mma<MB>(o[n][i], r, lo[n][0], lo[n][1]);
           }
         }
       }
     }
     const bool last = cu.block + 1 == cu.blocks;
     if (last || t + 1 == b) finish(t);
-    step(cu);
-    if (last && t + 1 < b) begin();
+    if (t + 1 < b) {
+      step(cu);
+      if (last) begin();
+    }
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
 }
@@ -604,7 +651,6 @@ constexpr uint32_t kJoin = JT / 32;    // workers whose units a CTA joins, and p
 // successive workers), and that one takes the whole CTA: the parts' weights
 // once in shared memory, then each warp every eighth part, lanes the dims;
 // last the warps' sums in order.
-template <bool BF>
 __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const AttendPlan pl, float up) {
   extern __shared__ float weight[];  // [workers]
   __shared__ __align__(16) float so[JT / 32][256];
@@ -614,6 +660,7 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
   constexpr float kLn2 = 0.69314718055994531f;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t head = blockIdx.y, DP = pl.pad_dim, D = p.c.head_dim;
+  const bool bf = p.a.type == XKSV_BF16;
   const uint32_t group = p.a.q_heads / p.c.kv_heads, st = pl.heads * DP + 2 * head;
   if (threadIdx.x == 0) big_at = ~0u;
   __syncthreads();
@@ -689,7 +736,7 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
       uint16_t* out = out_of(j, u);
 #pragma unroll
       for (int x = 0; x < 8; ++x)
-        if (x * 32 + lane < D) store16<BF>(out + x * 32 + lane, some ? acc[x] * f : 0.f);
+        if (x * 32 + lane < D) store16(bf, out + x * 32 + lane, some ? acc[x] * f : 0.f);
       if (lane == 0) put_lse(j, u, base, l);
     }
   }
@@ -746,17 +793,18 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
   for (uint32_t d = threadIdx.x; d < D; d += JT) {
     float x = 0.f;
     for (int w = 0; w < JT / 32; ++w) x += so[w][d];
-    store16<BF>(out + d, some ? x * f : 0.f);
+    store16(bf, out + d, some ? x * f : 0.f);
   }
   if (threadIdx.x == 0) put_lse(jm, u, base, l);
 }
 
 int pad_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-template <bool BF, bool E8, int DP, bool FULL>
+template <bool MB, bool E8, int DP, int NG, bool FULL>
 cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
-  using Sh = Shape<E8, DP>;
-  const cudaError_t e = cudaFuncSetAttribute(kv_attend_kernel<BF, E8, DP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::CTA);
+  using Sh = Shape<E8, DP, NG>;
+  auto kernel = kv_attend_kernel<MB, E8, DP, NG, FULL>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::CTA);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((pl.warps + kWarps - 1) / kWarps);
@@ -768,28 +816,39 @@ cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t f = cudaLaunchKernelEx(&cfg, kv_attend_kernel<BF, E8, DP, FULL>, p, pl);
+  const cudaError_t f = cudaLaunchKernelEx(&cfg, kernel, p, pl);
   if (f != cudaSuccess) return f;
   cfg.gridDim = dim3((pl.warps + kJoin - 1) / kJoin, pl.heads);
   cfg.blockDim = dim3(JT);
   cfg.dynamicSmemBytes = pl.warps * sizeof(float);
-  return cudaLaunchKernelEx(&cfg, kv_join_kernel<BF>, p, pl, BF && !E8 ? 0.f : 15.f);
+  return cudaLaunchKernelEx(&cfg, kv_join_kernel, p, pl, MB ? 0.f : 15.f);
 }
 
-template <bool BF, bool E8>
+template <bool MB, bool E8, int DP, int NG>
+cudaError_t launch_full(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
+  return p.c.head_dim == DP ? launch_attend<MB, E8, DP, NG, true>(p, pl, st)
+                            : launch_attend<MB, E8, DP, NG, false>(p, pl, st);
+}
+template <bool MB, bool E8, int DP>
+cudaError_t launch_heads(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
+  return pl.heads <= 8 ? launch_full<MB, E8, DP, 1>(p, pl, st) : launch_full<MB, E8, DP, 2>(p, pl, st);
+}
+template <bool MB, bool E8>
 cudaError_t launch_dim(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
-  const bool full = p.c.head_dim == pl.pad_dim;
   switch (pl.pad_dim) {
-    case 64: return full ? launch_attend<BF, E8, 64, true>(p, pl, st) : launch_attend<BF, E8, 64, false>(p, pl, st);
-    case 128: return full ? launch_attend<BF, E8, 128, true>(p, pl, st) : launch_attend<BF, E8, 128, false>(p, pl, st);
-    default: return full ? launch_attend<BF, E8, 256, true>(p, pl, st) : launch_attend<BF, E8, 256, false>(p, pl, st);
+    case 64: return launch_heads<MB, E8, 64>(p, pl, st);
+    case 128: return launch_heads<MB, E8, 128>(p, pl, st);
+    default: return launch_heads<MB, E8, 256>(p, pl, st);
   }
 }
 
-template <bool E8>
-void shape_of(int dp, uint32_t* block, uint32_t* per_sm) {
-  *block = dp == 64 ? Shape<E8, 64>::BT : dp == 128 ? Shape<E8, 128>::BT : Shape<E8, 256>::BT;
-  *per_sm = dp == 64 ? Shape<E8, 64>::PER_SM : dp == 128 ? Shape<E8, 128>::PER_SM : Shape<E8, 256>::PER_SM;
+template <bool E8, int NG>
+void shape_of(uint32_t dp, uint32_t* block, uint32_t* per_sm) {
+  using A = Shape<E8, 64, NG>;
+  using B = Shape<E8, 128, NG>;
+  using C = Shape<E8, 256, NG>;
+  *block = dp == 64 ? A::BT : dp == 128 ? B::BT : C::BT;
+  *per_sm = dp == 64 ? A::PER_SM : dp == 128 ? B::PER_SM : C::PER_SM;
 }
 
 }  // namespace
@@ -804,10 +863,11 @@ AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads
   for (int k = 0; k < 31; ++k)
     if (c.page_size == 1ull << k) pl.page_shift = k;
   uint32_t block = 16, per_sm = 1;
-  if (c.type == XKSV_E4M3)
-    shape_of<true>(int(pl.pad_dim), &block, &per_sm);
+  const bool e8 = c.type == XKSV_E4M3;
+  if (pl.heads <= 8)
+    e8 ? shape_of<true, 1>(pl.pad_dim, &block, &per_sm) : shape_of<false, 1>(pl.pad_dim, &block, &per_sm);
   else
-    shape_of<false>(int(pl.pad_dim), &block, &per_sm);
+    e8 ? shape_of<true, 2>(pl.pad_dim, &block, &per_sm) : shape_of<false, 2>(pl.pad_dim, &block, &per_sm);
   // no more workers than blocks of the longest sequences the table can hold
   const uint64_t longest = table_cols * c.page_size / block + 1;
   const uint64_t blocks = seqs * c.kv_heads * pl.chunks;
@@ -820,9 +880,8 @@ AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads
 }
 
 cudaError_t launch_kv_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
-  const bool bf = p.a.type == XKSV_BF16, e8 = p.c.type == XKSV_E4M3;
-  if (bf) return e8 ? launch_dim<true, true>(p, pl, st) : launch_dim<true, false>(p, pl, st);
-  return e8 ? launch_dim<false, true>(p, pl, st) : launch_dim<false, false>(p, pl, st);
+  if (p.c.type == XKSV_E4M3) return launch_dim<false, true>(p, pl, st);
+  return p.c.type == XKSV_BF16 ? launch_dim<true, false>(p, pl, st) : launch_dim<false, false>(p, pl, st);
 }
 
 }  // namespace xksv

@@ -39,11 +39,11 @@ XKSV_HD KvSpan kv_span(int64_t length, uint64_t cols, uint64_t page_size, uint64
 // ------------------------------------------------------ the attention's split
 // A unit is one (sequence, KV head, chunk of query heads); its cached tokens
 // are cut into blocks at multiples of the block's size (so that a block lies
-// in as few pages as it can), an empty unit counting one.
+// in as few pages as it can); an empty unit has none.
 XKSV_HD uint64_t kv_blocks(KvSpan s, uint32_t tokens) {
-  return s.length > s.first ? uint64_t(s.length + tokens - 1) / tokens - uint64_t(s.first) / tokens : 1;
+  return s.length > s.first ? uint64_t(s.length + tokens - 1) / tokens - uint64_t(s.first) / tokens : 0;
 }
-// All units' blocks in order, `total` > 0 of them, are shared evenly among
+// All units' blocks in order, `total` of them, are shared evenly among
 // workers = min(warps, total): worker i takes blocks [start(i), start(i + 1)),
 // quot or quot + 1 of them.
 struct KvShare {
@@ -52,7 +52,7 @@ struct KvShare {
 };
 XKSV_HD KvShare kv_share(uint64_t total, uint32_t warps) {
   const uint32_t w = total < warps ? uint32_t(total) : warps;
-  const uint64_t q = total / w;
+  const uint64_t q = w ? total / w : 0;
   return KvShare{total, q, w, uint32_t(total - q * w)};
 }
 XKSV_HD uint64_t kv_start(const KvShare& s, uint32_t worker) {
