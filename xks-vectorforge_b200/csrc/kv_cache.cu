@@ -46,9 +46,6 @@ struct E4m3 {
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(E4m3 x) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(x.b, __NV_E4M3)));
-}
 template <class T>
 __device__ __forceinline__ T from_float(float x);
 template <>
@@ -69,57 +66,193 @@ __device__ __forceinline__ E4m3 from_float<E4m3>(float x) {
 }
 
 // --------------------------------------------------------------- append ---
+// Bound: memory (every element is read once and written once) for prompts,
+// the chain of dependent loads (place -> page -> store) for a few tokens.  One
+// CTA per token: its page is looked up and its angles are computed while the
+// first rows are already being read; a thread moves 8 elements (and, rotated
+// in halves, their 8 partners) at a time.
 constexpr int AT = 256;         // threads per token
 constexpr int kMaxPairs = 128;  // head_dim <= 256
 
-// One CTA per token: its angles once in shared memory, then its heads.
+// cos and sin of a token's angles into shared memory.  The angle is formed in
+// 64 bits, less its whole turns: an FP32 product would be wrong by radians at
+// far positions.
+__device__ __forceinline__ void angles(const xksv_kv_append_args& a, int32_t pos, float* cs, float* sn) {
+  constexpr double kTurn = 6.283185307179586476925286766559, kTurns = 1.0 / kTurn, kHalfTurns = 2.0 / kTurn;
+  for (uint32_t i = threadIdx.x; i < a.rot_dim / 2; i += AT) {
+    const double angle = double(pos) * double(a.inv_freq[i]);
+    float sv, cv;
+    sincospif(float(fma(-rint(angle * kTurns), kTurn, angle) * kHalfTurns), &sv, &cv);
+    cs[i] = cv * a.rot_scale;
+    sn[i] = sv * a.rot_scale;
+  }
+}
+
+// A token's place in the cache; page -1: nothing of it is stored.
+struct Place {
+  int64_t page;
+  uint64_t place;
+};
+__device__ __forceinline__ Place token_place(const AppendArgs& p, uint64_t t, int64_t idx) {
+  const int64_t s = p.a.seq ? int64_t(p.a.seq[t]) : int64_t(t);
+  if (s < 0 || idx < 0) return Place{-1, 0};  // padding
+  const int64_t page = kv_page(p.a.table, p.a.table_rows, p.a.table_cols, p.a.table_stride, p.c.pages, p.c.page_size, s, idx);
+  if (page < 0 && threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
+  return Place{page, uint64_t(idx) % p.c.page_size};
+}
+
+template <class T>
+struct alignas(sizeof(T) * 8 >= 16 ? 16 : 8) Eight {
+  T x[8];
+};
+
+// Rows of 16-byte pieces (alignment, and rotated pairs that fill them).  An
+// item is 8 elements of a row, in a row rotated by halves with their partners
+// half a rotation further on.
 template <class TI, class TC>
 __global__ void __launch_bounds__(AT) kv_append_kernel(const AppendArgs p) {
-  __shared__ float cs[kMaxPairs], sn[kMaxPairs];
+  __shared__ __align__(16) float cs[kMaxPairs], sn[kMaxPairs];
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const uint64_t t = blockIdx.x;
-  const int64_t s = p.a.seq ? int64_t(p.a.seq[t]) : int64_t(t);
+  const uint32_t D = p.c.head_dim, rot = p.a.rot_dim, H = p.c.kv_heads, nq = p.a.q ? p.a.q_heads : 0;
+  const bool inter = p.a.flags & XKSV_KV_INTERLEAVED;
+  const uint32_t pairs = inter ? 0 : rot / 16;  // items that hold two pieces
+  const uint32_t per = D / 8 - pairs, vper = D / 8;
+  const uint32_t turned = (nq + H) * per, items = turned + H * vper;
+  // item w: its row in the inputs, first piece, and the partner's distance (0: none)
+  struct Item {
+    const TI* src;
+    uint32_t head, d, partner;
+    int kind;  // 0 query, 1 key, 2 value
+  };
+  auto item = [&](uint32_t w) {
+    Item it;
+    if (w < turned) {
+      const uint32_t row = w / per, c = w - row * per;
+      it.kind = row < nq ? 0 : 1;
+      it.head = row < nq ? row : row - nq;
+      it.d = c < pairs ? 8 * c : 8 * (c + pairs);
+      it.partner = c < pairs ? rot / 2 : 0;
+      it.src = it.kind == 0 ? static_cast<const TI*>(p.a.q) + t * p.a.q_stride[0] + it.head * p.a.q_stride[1]
+                            : static_cast<const TI*>(p.a.k) + t * p.a.k_stride[0] + it.head * p.a.k_stride[1];
+    } else {
+      it.kind = 2;
+      it.head = (w - turned) / vper;
+      it.d = 8 * (w - turned - it.head * vper);
+      it.partner = 0;
+      it.src = static_cast<const TI*>(p.a.v) + t * p.a.v_stride[0] + it.head * p.a.v_stride[1];
+    }
+    return it;
+  };
+  using In = Eight<TI>;
+  auto fetch = [&](const Item& it, In& a, In& b) {
+    a = *reinterpret_cast<const In*>(it.src + it.d);
+    if (it.partner) b = *reinterpret_cast<const In*>(it.src + it.d + it.partner);
+  };
+  // the first items are on their way while the page and the angles are found
+  // (a padding token's rows are not read)
   const int64_t idx = p.a.index[t];
-  if (s < 0 || idx < 0) return;
-  const uint64_t place = uint64_t(idx) % p.c.page_size;
-  const int64_t page = kv_page(p.a.table, p.a.table_rows, p.a.table_cols, p.a.table_stride, p.c.pages, p.c.page_size, s, idx);
-  if (page < 0) {
-    if (threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
-    return;
-  }
-  const uint32_t D = p.c.head_dim, half = p.a.rot_dim / 2;
   const int32_t pos = p.a.positions ? p.a.positions[t] : int32_t(idx);
-  for (uint32_t i = threadIdx.x; i < half; i += AT) {
-    // the angle in 64 bits, less its whole turns: an FP32 product would be
-    // wrong by radians at far positions
-    constexpr double kTurn = 6.283185307179586476925286766559;
-    const double angle = double(pos) * double(p.a.inv_freq[i]);
-    const float r = float(fma(-rint(angle / kTurn), kTurn, angle));
-    float sv, cv;
-    sincosf(r, &sv, &cv);
-    cs[i] = cv * p.a.rot_scale;
-    sn[i] = sv * p.a.rot_scale;
+  if (idx < 0 || (p.a.seq && p.a.seq[t] < 0)) return;
+  constexpr int kAhead = 2;
+  Item it[kAhead];
+  In a[kAhead], b[kAhead];
+#pragma unroll
+  for (int x = 0; x < kAhead; ++x)
+    if (threadIdx.x + x * AT < items) {
+      it[x] = item(threadIdx.x + x * AT);
+      fetch(it[x], a[x], b[x]);
+    }
+  const Place at = token_place(p, t, idx);
+  angles(p.a, pos, cs, sn);
+  if (at.page < 0) return;  // the whole CTA
+  __syncthreads();
+  TC* ck = static_cast<TC*>(p.c.k) + uint64_t(at.page) * p.c.k_stride[0] + at.place * p.c.k_stride[1];
+  TC* cv = static_cast<TC*>(p.c.v) + uint64_t(at.page) * p.c.v_stride[0] + at.place * p.c.v_stride[1];
+  TI* qo = static_cast<TI*>(p.a.q_out) + t * p.a.q_out_stride[0];
+  auto put = [&](const Item& i, uint32_t d, const float* x) {
+    if (i.kind == 0) {
+      In y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y.x[e] = from_float<TI>(x[e]);
+      *reinterpret_cast<In*>(qo + i.head * p.a.q_out_stride[1] + d) = y;
+    } else {
+      const float* sc = i.kind == 1 ? p.c.k_scale : p.c.v_scale;
+      const float f = sc ? sc[i.head] : 1.f;
+      Eight<TC> y;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y.x[e] = from_float<TC>(sc ? x[e] / f : x[e]);
+      TC* dst = i.kind == 1 ? ck + i.head * p.c.k_stride[2] : cv + i.head * p.c.v_stride[2];
+      *reinterpret_cast<Eight<TC>*>(dst + d) = y;
+    }
+  };
+  auto work = [&](const Item& i, const In& a, const In& b) {
+    float x[8], y[8];
+    if (i.partner) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float u = to_float(a.x[e]), v = to_float(b.x[e]), c = cs[i.d + e], s = sn[i.d + e];
+        x[e] = u * c - v * s;
+        y[e] = v * c + u * s;
+      }
+      put(i, i.d + i.partner, y);
+    } else if (inter && i.kind != 2 && i.d < rot) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float u = to_float(a.x[e]), v = to_float(a.x[e + 1]), c = cs[(i.d + e) / 2], s = sn[(i.d + e) / 2];
+        x[e] = u * c - v * s;
+        x[e + 1] = v * c + u * s;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = to_float(a.x[e]);
+    }
+    put(i, i.d, x);
+  };
+#pragma unroll
+  for (int x = 0; x < kAhead; ++x)
+    if (threadIdx.x + x * AT < items) work(it[x], a[x], b[x]);
+  for (uint32_t w = threadIdx.x + kAhead * AT; w < items; w += AT) {
+    it[0] = item(w);
+    fetch(it[0], a[0], b[0]);
+    work(it[0], a[0], b[0]);
   }
+}
+
+// Any strides, alignment and rotation: element by element, a thread per pair.
+template <class TI, class TC>
+__global__ void __launch_bounds__(AT) kv_append_any_kernel(const AppendArgs p) {
+  __shared__ float cs[kMaxPairs], sn[kMaxPairs];
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const uint64_t t = blockIdx.x;
+  const int64_t idx = p.a.index[t];
+  const Place at = token_place(p, t, idx);
+  if (at.page < 0) return;
+  const uint32_t D = p.c.head_dim, half = p.a.rot_dim / 2;
+  angles(p.a, p.a.positions ? p.a.positions[t] : int32_t(idx), cs, sn);
   __syncthreads();
   const bool inter = p.a.flags & XKSV_KV_INTERLEAVED;
-  const uint32_t rest = D - 2 * half, items = half + rest;  // pairs, then single elements
+  const uint32_t items = D - half;  // pairs, then single elements
   const TI* q = static_cast<const TI*>(p.a.q) + t * p.a.q_stride[0];
   TI* qo = static_cast<TI*>(p.a.q_out) + t * p.a.q_out_stride[0];
   const TI* k = static_cast<const TI*>(p.a.k) + t * p.a.k_stride[0];
   const TI* v = static_cast<const TI*>(p.a.v) + t * p.a.v_stride[0];
-  TC* ck = static_cast<TC*>(p.c.k) + uint64_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1];
-  TC* cv = static_cast<TC*>(p.c.v) + uint64_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1];
+  TC* ck = static_cast<TC*>(p.c.k) + uint64_t(at.page) * p.c.k_stride[0] + at.place * p.c.k_stride[1];
+  TC* cv = static_cast<TC*>(p.c.v) + uint64_t(at.page) * p.c.v_stride[0] + at.place * p.c.v_stride[1];
   const uint32_t nq = p.a.q ? p.a.q_heads : 0;
   for (uint32_t w = threadIdx.x; w < (nq + p.c.kv_heads) * items; w += AT) {
     const uint32_t hh = w / items, i = w - hh * items;
     const bool is_q = hh < nq;
     const uint32_t h = is_q ? hh : hh - nq;
     const TI* src = is_q ? q + h * p.a.q_stride[1] : k + h * p.a.k_stride[1];
-    const float inv = !is_q && p.c.k_scale ? p.c.k_scale[h] : 1.f;
+    const float f = !is_q && p.c.k_scale ? p.c.k_scale[h] : 1.f;
     auto put = [&](uint32_t d, float x) {
       if (is_q)
         qo[h * p.a.q_out_stride[1] + d] = from_float<TI>(x);
       else
-        ck[h * p.c.k_stride[2] + d] = from_float<TC>(p.c.k_scale ? x / inv : x);
+        ck[h * p.c.k_stride[2] + d] = from_float<TC>(p.c.k_scale ? x / f : x);
     };
     if (i < half) {
       const uint32_t da = inter ? 2 * i : i, db = inter ? 2 * i + 1 : i + half;
@@ -138,15 +271,33 @@ __global__ void __launch_bounds__(AT) kv_append_kernel(const AppendArgs p) {
   }
 }
 
+template <class TI, class TC>
+cudaError_t append_launch(const AppendArgs& p, cudaStream_t st) {
+  auto whole = [](const void* ptr, const uint64_t* stride) {  // rows of 16-byte pieces
+    return (reinterpret_cast<uintptr_t>(ptr) | stride[0] * sizeof(TI) | stride[1] * sizeof(TI)) % 16 == 0;
+  };
+  const bool pieces = p.a.rot_dim % (p.a.flags & XKSV_KV_INTERLEAVED ? 8 : 16) == 0 && whole(p.a.k, p.a.k_stride) &&
+                      whole(p.a.v, p.a.v_stride) &&
+                      (!p.a.q || (whole(p.a.q, p.a.q_stride) && whole(p.a.q_out, p.a.q_out_stride)));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(uint32_t(p.a.tokens));
+  cfg.blockDim = dim3(AT);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, pieces ? kv_append_kernel<TI, TC> : kv_append_any_kernel<TI, TC>, p);
+}
+
 template <class TI>
 cudaError_t append_cache(const AppendArgs& p, cudaStream_t st) {
-  const dim3 g(uint32_t(p.a.tokens));
   switch (p.c.type) {
-    case XKSV_BF16: kv_append_kernel<TI, __nv_bfloat16><<<g, AT, 0, st>>>(p); break;
-    case XKSV_FP16: kv_append_kernel<TI, __half><<<g, AT, 0, st>>>(p); break;
-    default: kv_append_kernel<TI, E4m3><<<g, AT, 0, st>>>(p); break;
+    case XKSV_BF16: return append_launch<TI, __nv_bfloat16>(p, st);
+    case XKSV_FP16: return append_launch<TI, __half>(p, st);
+    default: return append_launch<TI, E4m3>(p, st);
   }
-  return cudaGetLastError();
 }
 
 // ---------------------------------------------------------- C entry checks
