@@ -26,7 +26,11 @@ def test_page_lookup_stays_inside_the_table(tmp_path):
   // 3 sequences by 4 pages, rows 5 apart; the last row holds 4 entries only
   std::vector<int32_t> t(2 * 5 + 4, 0);
   t[0] = 7; t[3] = 9; t[5] = -1; t[10 + 3] = 8; t[10] = 2147483647;
-  auto at = [&](int64_t s, int64_t i) { return kv_page(t.data(), 3, 4, 5, 9, 16, s, i); };
+  auto at = [&](int64_t s, int32_t i) {
+    const KvPlace p = kv_place(t.data(), 3, 4, 5, 9, 16, s, i);
+    assert(p.place == (p.page < 0 ? 0u : uint32_t(i) % 16));
+    return p.page;
+  };
   assert(at(0, 0) == 7 && at(0, 15) == 7 && at(0, 16) == 0);
   assert(at(0, 63) == -1);            // page 9 of a cache of 9 pages
   assert(at(1, 3) == -1);             // page -1

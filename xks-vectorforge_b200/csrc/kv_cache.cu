@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <new>
 #include <utility>
 
@@ -67,12 +68,15 @@ __device__ __forceinline__ E4m3 from_float<E4m3>(float x) {
 
 // --------------------------------------------------------------- append ---
 // Bound: memory (every element is read once and written once) for prompts,
-// the chain of dependent loads (place -> page -> store) for a few tokens.  One
-// CTA per token: its page is looked up and its angles are computed while the
-// first rows are already being read; a thread moves 8 elements (and, rotated
-// in halves, their 8 partners) at a time.
-constexpr int AT = 256;         // threads per token
+// the chain of dependent loads (place -> page -> store) for a few tokens.  A
+// CTA takes tokens in turn: a token's page is looked up and its angles are
+// computed while its first rows are already being read.  A thread moves 8
+// elements (and, rotated in halves, their 8 partners) at a time and keeps its
+// place in the row, so that it reads its angles once a token and divides no
+// index in the loop.
+constexpr int AT = 128;         // threads per token
 constexpr int kMaxPairs = 128;  // head_dim <= 256
+constexpr int kPerSm = 6;       // CTAs an SM holds (16384 tokens: 71 us; three of 256 threads 83 us)
 
 // cos and sin of a token's angles into shared memory.  The angle is formed in
 // 64 bits, less its whole turns: an FP32 product would be wrong by radians at
@@ -88,135 +92,201 @@ __device__ __forceinline__ void angles(const xksv_kv_append_args& a, int32_t pos
   }
 }
 
-// A token's place in the cache; page -1: nothing of it is stored.
-struct Place {
-  int64_t page;
-  uint64_t place;
-};
-__device__ __forceinline__ Place token_place(const AppendArgs& p, uint64_t t, int64_t idx) {
-  const int64_t s = p.a.seq ? int64_t(p.a.seq[t]) : int64_t(t);
-  if (s < 0 || idx < 0) return Place{-1, 0};  // padding
-  const int64_t page = kv_page(p.a.table, p.a.table_rows, p.a.table_cols, p.a.table_stride, p.c.pages, p.c.page_size, s, idx);
-  if (page < 0 && threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
-  return Place{page, uint64_t(idx) % p.c.page_size};
+// A token's place in the cache (below 2^31: 32-bit division); page -1:
+// nothing of it is stored.
+__device__ __forceinline__ KvPlace token_place(const AppendArgs& p, int64_t seq, int32_t idx) {
+  if (seq < 0 || idx < 0) return KvPlace{-1, 0};  // padding
+  const KvPlace at = kv_place(p.a.table, p.a.table_rows, p.a.table_cols, p.a.table_stride, p.c.pages, uint32_t(p.c.page_size), seq, idx);
+  if (at.page < 0 && threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
+  return at;
 }
 
+// Eight elements as 32-bit words (E4M3: two, 16-bit types: four, FP32: eight).
 template <class T>
-struct alignas(sizeof(T) * 8 >= 16 ? 16 : 8) Eight {
-  T x[8];
+struct alignas(sizeof(T) == 1 ? 8 : 16) Eight {
+  uint32_t w[sizeof(T) * 2];
 };
+__device__ __forceinline__ void spread(const Eight<__nv_bfloat16>& a, float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(a.w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(a.w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void spread(const Eight<__half>& a, float* x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a.w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void spread(const Eight<float>& a, float* x) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(a.w[i]);
+}
+__device__ __forceinline__ void gather(const float* x, Eight<__nv_bfloat16>& a) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    a.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+__device__ __forceinline__ void gather(const float* x, Eight<__half>& a) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    a.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+__device__ __forceinline__ void gather(const float* x, Eight<float>& a) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a.w[i] = __float_as_uint(x[i]);
+}
+__device__ __forceinline__ void gather(const float* x, Eight<E4m3>& a) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
+    a.w[i] = lo | hi << 16;
+  }
+}
 
-// Rows of 16-byte pieces (alignment, and rotated pairs that fill them).  An
-// item is 8 elements of a row, in a row rotated by halves with their partners
-// half a rotation further on.
+// Rows of 16-byte pieces (alignment, and rotated pairs that fill them) whose
+// heads lie less than 2^31 elements apart.
 template <class TI, class TC>
-__global__ void __launch_bounds__(AT) kv_append_kernel(const AppendArgs p) {
-  __shared__ __align__(16) float cs[kMaxPairs], sn[kMaxPairs];
+__global__ void __launch_bounds__(AT, kPerSm) kv_append_kernel(const AppendArgs p) {
+  __shared__ __align__(16) float cs[2][kMaxPairs], sn[2][kMaxPairs];
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const uint64_t t = blockIdx.x;
+  using In = Eight<TI>;
+  using Out = Eight<TC>;
   const uint32_t D = p.c.head_dim, rot = p.a.rot_dim, H = p.c.kv_heads, nq = p.a.q ? p.a.q_heads : 0;
   const bool inter = p.a.flags & XKSV_KV_INTERLEAVED;
-  const uint32_t pairs = inter ? 0 : rot / 16;  // items that hold two pieces
+  const uint32_t pairs = inter ? 0 : rot / 16;  // threads of a row that hold two pieces
   const uint32_t per = D / 8 - pairs, vper = D / 8;
-  const uint32_t turned = (nq + H) * per, items = turned + H * vper;
-  // item w: its row in the inputs, first piece, and the partner's distance (0: none)
-  struct Item {
-    const TI* src;
-    uint32_t head, d, partner;
-    int kind;  // 0 query, 1 key, 2 value
+  const uint32_t rows = nq + H, step = AT / per, vstep = AT / vper;
+  // this thread's piece of a query or key row, and the first of its rows; the
+  // same for values (a row beyond the last: nothing to do)
+  const uint32_t c = threadIdx.x % per, d = c < pairs ? 8 * c : 8 * (c + pairs), half = c < pairs ? rot / 2 : 0;
+  const uint32_t row0 = threadIdx.x / per < step ? threadIdx.x / per : rows;
+  const uint32_t vd = 8 * (threadIdx.x % vper), vrow0 = threadIdx.x / vper < vstep ? threadIdx.x / vper : H;
+  const bool turn = half || (inter && d < rot);
+  struct Token {
+    int32_t idx, pos;
+    int64_t seq;
   };
-  auto item = [&](uint32_t w) {
-    Item it;
-    if (w < turned) {
-      const uint32_t row = w / per, c = w - row * per;
-      it.kind = row < nq ? 0 : 1;
-      it.head = row < nq ? row : row - nq;
-      it.d = c < pairs ? 8 * c : 8 * (c + pairs);
-      it.partner = c < pairs ? rot / 2 : 0;
-      it.src = it.kind == 0 ? static_cast<const TI*>(p.a.q) + t * p.a.q_stride[0] + it.head * p.a.q_stride[1]
-                            : static_cast<const TI*>(p.a.k) + t * p.a.k_stride[0] + it.head * p.a.k_stride[1];
-    } else {
-      it.kind = 2;
-      it.head = (w - turned) / vper;
-      it.d = 8 * (w - turned - it.head * vper);
-      it.partner = 0;
-      it.src = static_cast<const TI*>(p.a.v) + t * p.a.v_stride[0] + it.head * p.a.v_stride[1];
+  auto token = [&](uint64_t t) {
+    Token k;
+    k.idx = p.a.index[t];
+    k.seq = p.a.seq ? int64_t(p.a.seq[t]) : int64_t(t);
+    k.pos = p.a.positions ? p.a.positions[t] : int32_t(k.idx);
+    return k;
+  };
+  // head strides fit 32 bits here, and so does a row's offset from its token's
+  const uint32_t qs = uint32_t(p.a.q_stride[1]), ks = uint32_t(p.a.k_stride[1]), vs = uint32_t(p.a.v_stride[1]);
+  auto source = [&](uint64_t t, uint32_t r) {
+    return r < nq ? static_cast<const TI*>(p.a.q) + t * p.a.q_stride[0] + (r * qs + d)
+                  : static_cast<const TI*>(p.a.k) + t * p.a.k_stride[0] + ((r - nq) * ks + d);
+  };
+  auto store = [&](TC* dst, float* x, const float* scale, uint32_t h) {
+    if (scale) {
+      const float f = scale[h];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] /= f;
     }
-    return it;
+    Out y;
+    gather(x, y);
+    *reinterpret_cast<Out*>(dst) = y;
   };
-  using In = Eight<TI>;
-  auto fetch = [&](const Item& it, In& a, In& b) {
-    a = *reinterpret_cast<const In*>(it.src + it.d);
-    if (it.partner) b = *reinterpret_cast<const In*>(it.src + it.d + it.partner);
-  };
-  // the first items are on their way while the page and the angles are found
-  // (a padding token's rows are not read)
-  const int64_t idx = p.a.index[t];
-  const int32_t pos = p.a.positions ? p.a.positions[t] : int32_t(idx);
-  if (idx < 0 || (p.a.seq && p.a.seq[t] < 0)) return;
-  constexpr int kAhead = 2;
-  Item it[kAhead];
-  In a[kAhead], b[kAhead];
+  // pieces read before the angles are there: two rows' pairs, or four rows
+  constexpr int kAhead = 4;
+  uint32_t buf = 0;
+  Token k = token(blockIdx.x);
+  for (uint64_t t = blockIdx.x; t < p.a.tokens; t += gridDim.x, buf ^= 1) {
+    const bool live = k.idx >= 0 && k.seq >= 0;  // padding's rows are not read
+    In a[kAhead], v;
 #pragma unroll
-  for (int x = 0; x < kAhead; ++x)
-    if (threadIdx.x + x * AT < items) {
-      it[x] = item(threadIdx.x + x * AT);
-      fetch(it[x], a[x], b[x]);
+    for (int y = 0; y < kAhead; ++y) {
+      const uint32_t r = row0 + (half ? y / 2 : y) * step;
+      if (live && r < rows) a[y] = *reinterpret_cast<const In*>(source(t, r) + (half && y % 2 ? half : 0));
     }
-  const Place at = token_place(p, t, idx);
-  angles(p.a, pos, cs, sn);
-  if (at.page < 0) return;  // the whole CTA
-  __syncthreads();
-  TC* ck = static_cast<TC*>(p.c.k) + uint64_t(at.page) * p.c.k_stride[0] + at.place * p.c.k_stride[1];
-  TC* cv = static_cast<TC*>(p.c.v) + uint64_t(at.page) * p.c.v_stride[0] + at.place * p.c.v_stride[1];
-  TI* qo = static_cast<TI*>(p.a.q_out) + t * p.a.q_out_stride[0];
-  auto put = [&](const Item& i, uint32_t d, const float* x) {
-    if (i.kind == 0) {
-      In y;
+    const TI* vsrc = static_cast<const TI*>(p.a.v) + t * p.a.v_stride[0] + vd;
+    if (live && vrow0 < H) v = *reinterpret_cast<const In*>(vsrc + vrow0 * vs);
+    const KvPlace at = token_place(p, k.seq, k.idx);
+    if (live) angles(p.a, k.pos, cs[buf], sn[buf]);
+    if (t + gridDim.x < p.a.tokens) k = token(t + gridDim.x);
+    __syncthreads();
+    if (at.page < 0) continue;
+    // halves: eight angles; pairs: four, each for two elements
+    const float4* c4 = reinterpret_cast<const float4*>(&cs[buf][half ? d : d / 2]);
+    const float4* s4 = reinterpret_cast<const float4*>(&sn[buf][half ? d : d / 2]);
+    TC* ck = static_cast<TC*>(p.c.k) + uint64_t(at.page) * p.c.k_stride[0] + at.place * p.c.k_stride[1] + d;
+    TC* cv = static_cast<TC*>(p.c.v) + uint64_t(at.page) * p.c.v_stride[0] + at.place * p.c.v_stride[1] + vd;
+    TI* qo = static_cast<TI*>(p.a.q_out) + t * p.a.q_out_stride[0] + d;
+    auto work = [&](uint32_t r, const In& a, const In& b) {
+      float x[8], y[8];
+      spread(a, x);
+      if (half) {
+        spread(b, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y.x[e] = from_float<TI>(x[e]);
-      *reinterpret_cast<In*>(qo + i.head * p.a.q_out_stride[1] + d) = y;
-    } else {
-      const float* sc = i.kind == 1 ? p.c.k_scale : p.c.v_scale;
-      const float f = sc ? sc[i.head] : 1.f;
-      Eight<TC> y;
+        for (int g = 0; g < 2; ++g) {
+          const float4 cv4 = c4[g], sv4 = s4[g];
+          const float co[4] = {cv4.x, cv4.y, cv4.z, cv4.w}, si[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y.x[e] = from_float<TC>(sc ? x[e] / f : x[e]);
-      TC* dst = i.kind == 1 ? ck + i.head * p.c.k_stride[2] : cv + i.head * p.c.v_stride[2];
-      *reinterpret_cast<Eight<TC>*>(dst + d) = y;
-    }
-  };
-  auto work = [&](const Item& i, const In& a, const In& b) {
-    float x[8], y[8];
-    if (i.partner) {
+          for (int e = 0; e < 4; ++e) {
+            const float u = x[4 * g + e], w = y[4 * g + e];
+            x[4 * g + e] = u * co[e] - w * si[e];
+            y[4 * g + e] = w * co[e] + u * si[e];
+          }
+        }
+      } else if (turn) {
+        const float4 cv4 = c4[0], sv4 = s4[0];
+        const float co[4] = {cv4.x, cv4.y, cv4.z, cv4.w}, si[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float u = to_float(a.x[e]), v = to_float(b.x[e]), c = cs[i.d + e], s = sn[i.d + e];
-        x[e] = u * c - v * s;
-        y[e] = v * c + u * s;
+        for (int e = 0; e < 4; ++e) {
+          const float u = x[2 * e], w = x[2 * e + 1];
+          x[2 * e] = u * co[e] - w * si[e];
+          x[2 * e + 1] = w * co[e] + u * si[e];
+        }
       }
-      put(i, i.d + i.partner, y);
-    } else if (inter && i.kind != 2 && i.d < rot) {
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float u = to_float(a.x[e]), v = to_float(a.x[e + 1]), c = cs[(i.d + e) / 2], s = sn[(i.d + e) / 2];
-        x[e] = u * c - v * s;
-        x[e + 1] = v * c + u * s;
+      if (r < nq) {
+        TI* dst = qo + r * uint32_t(p.a.q_out_stride[1]);
+        In o;
+        gather(x, o);
+        *reinterpret_cast<In*>(dst) = o;
+        if (half) {
+          gather(y, o);
+          *reinterpret_cast<In*>(dst + half) = o;
+        }
+      } else {
+        TC* dst = ck + (r - nq) * uint32_t(p.c.k_stride[2]);
+        store(dst, x, p.c.k_scale, r - nq);
+        if (half) store(dst + half, y, p.c.k_scale, r - nq);
       }
+    };
+    uint32_t r = row0;
+    if (half) {
+#pragma unroll
+      for (int y = 0; y < kAhead / 2; ++y, r += step)
+        if (r < rows) work(r, a[2 * y], a[2 * y + 1]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = to_float(a.x[e]);
+      for (int y = 0; y < kAhead; ++y, r += step)
+        if (r < rows) work(r, a[y], a[y]);
     }
-    put(i, i.d, x);
-  };
-#pragma unroll
-  for (int x = 0; x < kAhead; ++x)
-    if (threadIdx.x + x * AT < items) work(it[x], a[x], b[x]);
-  for (uint32_t w = threadIdx.x + kAhead * AT; w < items; w += AT) {
-    it[0] = item(w);
-    fetch(it[0], a[0], b[0]);
-    work(it[0], a[0], b[0]);
+    for (; r < rows; r += step) {
+      const TI* src = source(t, r);
+      a[0] = *reinterpret_cast<const In*>(src);
+      if (half) a[1] = *reinterpret_cast<const In*>(src + half);
+      work(r, a[0], a[1]);
+    }
+    for (uint32_t r = vrow0; r < H; r += vstep) {
+      if (r != vrow0) v = *reinterpret_cast<const In*>(vsrc + r * vs);
+      float x[8];
+      spread(v, x);
+      store(cv + r * uint32_t(p.c.v_stride[2]), x, p.c.v_scale, r);
+    }
   }
 }
 
@@ -227,11 +297,11 @@ __global__ void __launch_bounds__(AT) kv_append_any_kernel(const AppendArgs p) {
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const uint64_t t = blockIdx.x;
-  const int64_t idx = p.a.index[t];
-  const Place at = token_place(p, t, idx);
+  const int32_t idx = p.a.index[t];
+  const KvPlace at = token_place(p, p.a.seq ? int64_t(p.a.seq[t]) : int64_t(t), idx);
   if (at.page < 0) return;
   const uint32_t D = p.c.head_dim, half = p.a.rot_dim / 2;
-  angles(p.a, p.a.positions ? p.a.positions[t] : int32_t(idx), cs, sn);
+  angles(p.a, p.a.positions ? p.a.positions[t] : idx, cs, sn);
   __syncthreads();
   const bool inter = p.a.flags & XKSV_KV_INTERLEAVED;
   const uint32_t items = D - half;  // pairs, then single elements
@@ -272,15 +342,20 @@ __global__ void __launch_bounds__(AT) kv_append_any_kernel(const AppendArgs p) {
 }
 
 template <class TI, class TC>
-cudaError_t append_launch(const AppendArgs& p, cudaStream_t st) {
+cudaError_t append_launch(const AppendArgs& p, int sms, cudaStream_t st) {
   auto whole = [](const void* ptr, const uint64_t* stride) {  // rows of 16-byte pieces
     return (reinterpret_cast<uintptr_t>(ptr) | stride[0] * sizeof(TI) | stride[1] * sizeof(TI)) % 16 == 0;
   };
-  const bool pieces = p.a.rot_dim % (p.a.flags & XKSV_KV_INTERLEAVED ? 8 : 16) == 0 && whole(p.a.k, p.a.k_stride) &&
+  auto near = [](uint64_t heads, uint64_t stride) { return stride < (1ull << 31) / heads; };
+  const bool close = near(p.c.kv_heads, p.a.k_stride[1]) && near(p.c.kv_heads, p.a.v_stride[1]) &&
+                     near(p.c.kv_heads, p.c.k_stride[2]) && near(p.c.kv_heads, p.c.v_stride[2]) &&
+                     (!p.a.q || (near(p.a.q_heads, p.a.q_stride[1]) && near(p.a.q_heads, p.a.q_out_stride[1])));
+  const bool pieces = close && p.a.rot_dim % (p.a.flags & XKSV_KV_INTERLEAVED ? 8 : 16) == 0 && whole(p.a.k, p.a.k_stride) &&
                       whole(p.a.v, p.a.v_stride) &&
                       (!p.a.q || (whole(p.a.q, p.a.q_stride) && whole(p.a.q_out, p.a.q_out_stride)));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(uint32_t(p.a.tokens));
+  // the piecewise kernel's CTAs loop over the tokens, as many as the GPU holds
+  cfg.gridDim = dim3(uint32_t(pieces ? std::min<uint64_t>(p.a.tokens, kPerSm * sms) : p.a.tokens));
   cfg.blockDim = dim3(AT);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -292,11 +367,11 @@ cudaError_t append_launch(const AppendArgs& p, cudaStream_t st) {
 }
 
 template <class TI>
-cudaError_t append_cache(const AppendArgs& p, cudaStream_t st) {
+cudaError_t append_cache(const AppendArgs& p, int sms, cudaStream_t st) {
   switch (p.c.type) {
-    case XKSV_BF16: return append_launch<TI, __nv_bfloat16>(p, st);
-    case XKSV_FP16: return append_launch<TI, __half>(p, st);
-    default: return append_launch<TI, E4m3>(p, st);
+    case XKSV_BF16: return append_launch<TI, __nv_bfloat16>(p, sms, st);
+    case XKSV_FP16: return append_launch<TI, __half>(p, sms, st);
+    default: return append_launch<TI, E4m3>(p, sms, st);
   }
 }
 
@@ -340,11 +415,11 @@ bool strides_small(const uint64_t* stride) { return stride[0] < (1ull << 40) && 
 
 }  // namespace
 
-cudaError_t launch_kv_append(const AppendArgs& p, cudaStream_t st) {
+cudaError_t launch_kv_append(const AppendArgs& p, int sms, cudaStream_t st) {
   switch (p.a.type) {
-    case XKSV_BF16: return append_cache<__nv_bfloat16>(p, st);
-    case XKSV_FP16: return append_cache<__half>(p, st);
-    default: return append_cache<float>(p, st);
+    case XKSV_BF16: return append_cache<__nv_bfloat16>(p, sms, st);
+    case XKSV_FP16: return append_cache<__half>(p, sms, st);
+    default: return append_cache<float>(p, sms, st);
   }
 }
 
@@ -424,7 +499,7 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* a, void* stream
   if (!guard.ok) return 1;
   const AppendArgs p{*a, kv->d, kv->d_status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return launch_kv_append(p, st) == cudaSuccess ? 0 : 1;
+  return launch_kv_append(p, kv->sms, st) == cudaSuccess ? 0 : 1;
 }
 
 size_t xksv_kv_attend_workspace(const xksv_kv* kv, size_t seqs, size_t q_heads, size_t table_cols) {

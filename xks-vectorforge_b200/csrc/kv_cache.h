@@ -11,7 +11,7 @@ struct AppendArgs {
   xksv_kv_desc c;
   int* status;
 };
-cudaError_t launch_kv_append(const AppendArgs& p, cudaStream_t st);
+cudaError_t launch_kv_append(const AppendArgs& p, int sms, cudaStream_t st);
 
 struct AttendArgs {
   xksv_kv_attend_args a;

@@ -11,17 +11,21 @@
 
 namespace xksv {
 
-// Page that holds token `index` of sequence `seq`, read from a page table of
-// `rows` sequences by `cols` pages whose rows are `stride` entries apart; -1
+// Where token `index` of sequence `seq` lives, from a page table of `rows`
+// sequences by `cols` pages whose rows are `stride` entries apart; page -1
 // when the token lies outside the table or its page outside the cache.  The
-// table is read only inside its bounds.
-XKSV_HD int64_t kv_page(const int32_t* table, uint64_t rows, uint64_t cols, uint64_t stride, uint64_t pages,
-                        uint64_t page_size, int64_t seq, int64_t index) {
-  if (seq < 0 || uint64_t(seq) >= rows || index < 0) return -1;
-  const uint64_t col = uint64_t(index) / page_size;
-  if (col >= cols) return -1;
-  const int64_t page = table[uint64_t(seq) * stride + col];
-  return page < 0 || uint64_t(page) >= pages ? -1 : page;
+// table is read only inside its bounds.  Indexes are below 2^31: 32-bit division.
+struct KvPlace {
+  int32_t page;
+  uint32_t place;
+};
+XKSV_HD KvPlace kv_place(const int32_t* table, uint64_t rows, uint64_t cols, uint64_t stride, uint64_t pages,
+                         uint32_t page_size, int64_t seq, int32_t index) {
+  if (seq < 0 || uint64_t(seq) >= rows || index < 0) return KvPlace{-1, 0};
+  const uint32_t col = uint32_t(index) / page_size;
+  if (col >= cols) return KvPlace{-1, 0};
+  const int32_t page = table[uint64_t(seq) * stride + col];
+  return page < 0 || uint64_t(page) >= pages ? KvPlace{-1, 0} : KvPlace{page, uint32_t(index) - col * page_size};
 }
 
 // Cached tokens that a new token attends to: [first, length).  A length
