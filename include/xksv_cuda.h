@@ -358,6 +358,8 @@ typedef struct xksv_linear_args {
  * xksv_plan_gemm, batches that share a row between several CTAs add in an
  * order that may differ between runs (the last bits of the FP32 sums). */
 size_t xksv_plan_linear_workspace(const xksv_plan* plan, size_t batch);
+/* The device the plan was created on (-1 for NULL). */
+int xksv_plan_device(const xksv_plan* plan);
 int xksv_plan_linear(const xksv_plan* plan, const void* d_payload, size_t payload_size,
                      const xksv_linear_args* args, void* d_workspace, size_t workspace_bytes, void* stream);
 

@@ -227,6 +227,8 @@ struct xksv_plan {
   uint32_t n_runs = 0;
   uint64_t max_run = 0;
   xksv::RowRun* d_runs = nullptr;
+  std::vector<xksv::LinearSeg> segs;  // decoded weights of the tensor-core route
+  int sms = 148;
   // xksv_plan_decode_host: copy stream and per-chunk events (created on first use)
   cudaStream_t copy_st = nullptr;
   cudaEvent_t chunk_ev[9] = {};
@@ -596,6 +598,13 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
     std::vector<Slab> tc_slabs;
     if (ok && raw_gemm_ok && build_tc_groups(all, groups, tc_slabs, p->scratch_bytes, p->x_cols, p->x_base)) {
       p->ngroups = uint32_t(groups.size());
+      for (const TcGroup& g : groups) {  // in scratch order: X columns, then Y rows
+        LinearSeg* b = p->segs.empty() ? nullptr : &p->segs.back();
+        if (b && b->xoff == g.xoff && b->cols == g.cols && b->row0 + b->rows == g.y_row0 && b->rows < (1u << 30))
+          b->rows += g.rows;
+        else
+          p->segs.push_back(LinearSeg{g.a_off, g.y_row0, g.xoff, g.rows, g.cols});
+      }
       uint32_t minch = ~0u;
       for (const TcGroup& g : groups) minch = std::min<uint32_t>(minch, (g.cols + 63) / 64);
       const uint32_t want = (2 * uint32_t(sms) + p->ngroups - 1) / p->ngroups;
@@ -608,6 +617,7 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
                      cudaSuccess;
     }
   }
+  p->sms = sms;
   // runs of covered Y rows (linear layer)
   if (ok && raw_gemm_ok) {
     std::vector<RowRun> runs;
@@ -799,6 +809,33 @@ bool gemm_fused(const xksv_plan* p, const void* d_payload, size_t batch) {
          p->gemm_route != XKSV_GEMM_SCRATCH;
 }
 
+// Enqueues the decode of every slab into its BF16 row group of the scratch.
+cudaError_t decode_scratch(xksv_plan* p, const uint8_t* pay, uint8_t* scratch, cudaStream_t st) {
+  const bool indexed = p->d_tidx && pay == p->indexed_payload;
+  cudaError_t e = cudaSuccess;
+  const uint32_t tser0 = indexed && p->n_items ? p->n_ser_idx : 0;
+  if (tser0) {
+    e = tile_decode(p, p->d_tc_slabs, pay, scratch, st);
+    ++p->launches;
+  }
+  if (e == cudaSuccess && p->n_ser > tser0) {
+    e = launch_serial_decode(p->d_tc_slabs + tser0, p->n_ser - tser0, pay, scratch, p->d_status,
+                             p->grid_ser, st);
+    ++p->launches;
+  }
+  if (e == cudaSuccess && p->n_par) {
+    e = launch_parallel_decode(p->d_tc_slabs + p->n_ser, p->n_par, pay, scratch, p->d_status,
+                               p->grid_par, st);
+    ++p->launches;
+  }
+  if (e == cudaSuccess && p->n_raw) {
+    e = launch_raw_decode(p->d_tc_slabs + p->n_ser + p->n_par, p->n_raw, pay, scratch,
+                          p->grid_raw, st);
+    ++p->launches;
+  }
+  return e;
+}
+
 // Enqueues Y = W X (xksv_plan_gemm after its checks) with the given buffers
 // for X^T in BF16 [256][x_cols] and the decoded weights, which only the
 // tensor-core routes touch.
@@ -842,26 +879,7 @@ int gemm_run(xksv_plan* p, const uint8_t* pay, const float* d_x, float* d_y, siz
   if (p->tc_ok && batch >= 4) {
     // decode every slab into its BF16 row group, then the tensor-core GEMM,
     // up to 256 batch columns per pass over the same decoded scratch
-    const uint32_t tser0 = indexed && p->n_items ? p->n_ser_idx : 0;
-    if (tser0) {
-      e = tile_decode(p, p->d_tc_slabs, pay, scratch, st);
-      ++p->launches;
-    }
-    if (e == cudaSuccess && p->n_ser > tser0) {
-      e = launch_serial_decode(p->d_tc_slabs + tser0, p->n_ser - tser0, pay, scratch, p->d_status,
-                               p->grid_ser, st);
-      ++p->launches;
-    }
-    if (e == cudaSuccess && p->n_par) {
-      e = launch_parallel_decode(p->d_tc_slabs + p->n_ser, p->n_par, pay, scratch, p->d_status,
-                                 p->grid_par, st);
-      ++p->launches;
-    }
-    if (e == cudaSuccess && p->n_raw) {
-      e = launch_raw_decode(p->d_tc_slabs + p->n_ser + p->n_par, p->n_raw, pay, scratch,
-                            p->grid_raw, st);
-      ++p->launches;
-    }
+    e = decode_scratch(p, pay, scratch, st);
     for (size_t b0 = 0; b0 < batch && e == cudaSuccess; b0 += 256) {
       TcGemmArgs g{};
       g.groups = p->d_groups;
@@ -958,17 +976,26 @@ struct Carve {
   }
 };
 struct LinearSpace {
+  bool gemm;  // decoded weights, x in place (or its rows copied to xt), no x / z
   uint64_t x, z, xt, scratch, total;
 };
-LinearSpace linear_space(const xksv_plan* p, uint64_t batch) {
+constexpr uint64_t pitch_of(uint64_t cols) { return (cols + 7) / 8 * 8; }
+// What a call needs of each part; the payload decides whether the tile index
+// (and so the fused kernel) is there: null counts for any.
+LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload) {
   Carve c;
   LinearSpace s{};
+  const bool fused = payload && gemm_fused(p, payload, batch);
+  if (p->tc_ok && batch >= 4 && !fused) {
+    s.gemm = true;
+    s.xt = c.take(batch * pitch_of(p->need_x_rows) * 2);
+    s.scratch = c.take(p->scratch_bytes);
+    s.total = c.pos;
+    return s;
+  }
   s.x = c.take(p->need_x_rows * batch * sizeof(float));
   s.z = c.take(p->need_y_rows * batch * sizeof(float));
-  if (p->tc_ok && batch >= 4) {
-    s.xt = c.take(256 * p->x_cols * 2);
-    s.scratch = c.take(p->scratch_bytes);
-  }
+  if (fused) s.xt = c.take(256 * p->x_cols * 2);
   s.total = c.pos;
   return s;
 }
@@ -991,9 +1018,12 @@ struct OnDevice {
 };
 }  // namespace
 
+int xksv_plan_device(const xksv_plan* p) { return p ? p->device : -1; }
+
 size_t xksv_plan_linear_workspace(const xksv_plan* p, size_t batch) {
   if (!p || !p->linear_ok || !batch || batch >= kMaxBatch) return 0;
-  return size_t(linear_space(p, batch).total);
+  // a later index may switch the route: room for either
+  return size_t(std::max(linear_space(p, batch, nullptr).total, linear_space(p, batch, p->indexed_payload).total));
 }
 
 int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_size, const xksv_linear_args* a,
@@ -1012,7 +1042,7 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
   p->launches = 0;
   if (!a->batch || !p->n_runs) return 0;
   if (!d_payload || !a->x || !a->y) return 1;
-  const LinearSpace sp = linear_space(p, a->batch);
+  const LinearSpace sp = linear_space(p, a->batch, d_payload);
   if (!d_workspace || workspace_bytes < sp.total || misaligned(d_workspace, 256)) return 1;
   OnDevice dev(p->device);
   if (!dev.ok) return 1;
@@ -1033,8 +1063,40 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
   ep.bias_f32 = a->bias_type == XKSV_FP32;
   ep.mul_f32 = a->mul_type == XKSV_FP32;
   ep.residual_f32 = a->residual_type == XKSV_FP32;
+  // eight columns of an operand from a multiple of 8: whole 16-byte words
+  auto whole = [](const void* ptr, uint64_t stride, bool f32) {
+    const uint64_t size = f32 ? 4 : 2;
+    return !ptr || (reinterpret_cast<uintptr_t>(ptr) | stride * size) % 16 == 0;
+  };
+  ep.vec = whole(ep.y, ep.y_stride, ep.y_f32) && whole(ep.bias, 0, ep.bias_f32) &&
+           whole(ep.mul, ep.mul_stride, ep.mul_f32) && whole(ep.residual, ep.residual_stride, ep.residual_f32);
+  for (const LinearSeg& g : p->segs) ep.vec = ep.vec && g.row0 % 8 == 0;
+  const auto* pay = static_cast<const uint8_t*>(d_payload);
+  if (sp.gemm) {
+    // decode, then one tensor-core product with its epilogue per weight
+    const uint64_t xs = a->batch > 1 ? a->x_stride : pitch_of(a->x_cols);
+    const void* xp = a->x;
+    uint64_t pitch = xs;
+    bool direct = true;
+    for (const LinearSeg& g : p->segs) direct = direct && linear_rows_direct(a->x, xs, p->x_base + g.xoff);
+    if (!direct) {  // (X offsets of a tensor-core plan are multiples of 8)
+      xp = ws + sp.xt;
+      pitch = pitch_of(p->need_x_rows);
+      if (launch_linear_rows(a->x, a->x_stride, a->batch, p->need_x_rows, pitch, ws + sp.xt, st) != cudaSuccess) return 1;
+      ++p->launches;
+    }
+    if (decode_scratch(p, pay, ws + sp.scratch, st) != cudaSuccess) return 1;
+    for (const LinearSeg& g : p->segs) {
+      if (launch_linear_gemm(ws + sp.scratch + g.a_off, g.rows, g.cols,
+                             static_cast<const uint16_t*>(xp) + p->x_base + g.xoff, pitch, uint32_t(a->batch), g.row0,
+                             ep, p->d_status, p->sms, st) != cudaSuccess)
+        return 1;
+      ++p->launches;
+    }
+    return 0;
+  }
   if (launch_linear_x(a->x, a->x_stride, a->batch, p->need_x_rows, x, st) != cudaSuccess) return 1;
-  if (gemm_run(p, static_cast<const uint8_t*>(d_payload), x, z, a->batch, ws + sp.xt, ws + sp.scratch, st)) return 1;
+  if (gemm_run(p, pay, x, z, a->batch, ws + sp.xt, ws + sp.scratch, st)) return 1;
   if (launch_linear_y(z, a->batch, p->d_runs, p->n_runs, p->max_run, ep, st) != cudaSuccess) return 1;
   p->launches += 2;
   return 0;

@@ -184,6 +184,7 @@ struct Epilogue {
   uint64_t y_stride, mul_stride, residual_stride;
   uint32_t act;
   bool y_f32, bias_f32, mul_f32, residual_f32;
+  bool vec;  // eight columns from a multiple of 8 are 16-byte aligned in every operand
 };
 // x BF16 [batch, cols] (rows `stride` elements apart) to FP32 [cols, batch].
 cudaError_t launch_linear_x(const void* x, uint64_t stride, uint64_t batch, uint64_t cols, float* xt, cudaStream_t st);
@@ -191,6 +192,23 @@ cudaError_t launch_linear_x(const void* x, uint64_t stride, uint64_t batch, uint
 // (nruns of them, `rows` the longest).
 cudaError_t launch_linear_y(const float* z, uint64_t batch, const RowRun* runs, uint32_t nruns, uint64_t rows,
                             const Epilogue& e, cudaStream_t st);
+
+// A decoded weight for the linear layer's tensor-core product: `rows` rows of
+// `cols` BF16 from byte a_off of the scratch, giving rows row0 .. of Y from X's
+// columns xoff ..
+struct LinearSeg {
+  uint64_t a_off, row0, xoff;
+  uint32_t rows, cols;
+};
+// The product and epilogue for one such weight: w BF16 [rows, cols]; x at its
+// first column, rows x_pitch elements apart (both 16-byte aligned, pitches too).
+cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, const void* x, uint64_t x_pitch, uint32_t batch,
+                               uint64_t row0, const Epilogue& e, int* status, int sms, cudaStream_t st);
+// x can be read by TMA from column xoff on; else launch_linear_rows copies
+// its first `cols` columns to rows of `pitch` elements.
+bool linear_rows_direct(const void* x, uint64_t stride, uint64_t xoff);
+cudaError_t launch_linear_rows(const void* x, uint64_t stride, uint64_t batch, uint64_t cols, uint64_t pitch, void* out,
+                               cudaStream_t st);
 
 // SHA-256 (FIPS 180-4) of n ranges {offset, length} (device array of 2n u64)
 // of d_base; 32-byte big-endian digests to d_digests.

@@ -32,4 +32,68 @@ __device__ __forceinline__ void epilogue_store(const Epilogue& e, uint64_t b, ui
     static_cast<__nv_bfloat16*>(e.y)[b * e.y_stride + row] = __float2bfloat16_rn(z);
 }
 
+// Eight elements at index i of a BF16 or FP32 array, 16-byte aligned there.
+__device__ __forceinline__ void load8(const void* p, uint64_t i, bool f32, float* v) {
+  if (f32) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + i);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[2 * k] = __uint_as_float(w[k] << 16);
+      v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+  }
+}
+
+// z[0 .. 7] of token b into y's columns row .. row + 7 (n of them exist):
+// 16-byte accesses where every operand allows them (Epilogue::vec, row a
+// multiple of 8 past a multiple-of-8 start), else one by one.
+__device__ __forceinline__ void epilogue_store8(const Epilogue& e, uint64_t b, uint64_t row, float* z, int n) {
+  if (!e.vec || n < 8) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) epilogue_store(e, b, row + k, z[k]);
+    return;
+  }
+  float t[8];
+  if (e.bias) {
+    load8(e.bias, row, e.bias_f32, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] += t[k];
+  }
+  if (e.act) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] = act_apply(e.act, z[k]);
+  }
+  if (e.mul) {
+    load8(e.mul, b * e.mul_stride + row, e.mul_f32, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] *= t[k];
+  }
+  if (e.residual) {
+    load8(e.residual, b * e.residual_stride + row, e.residual_f32, t);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z[k] += t[k];
+  }
+  const uint64_t at = b * e.y_stride + row;
+  if (e.y_f32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(e.y) + at);
+    q[0] = make_float4(z[0], z[1], z[2], z[3]);
+    q[1] = make_float4(z[4], z[5], z[6], z[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(z[2 * k], z[2 * k + 1]);
+      w[k] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(e.y) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
 }  // namespace xksv

@@ -1,0 +1,308 @@
+// Linear layer of a prompt: y[tokens, rows] = epilogue(x W^T) on the 5th-
+// generation tensor cores, W decoded into a BF16 scratch before.
+//
+// Bound: the tensor cores (2 tokens rows cols operations; both operands come
+// from L2).  A persistent CTA per SM takes tiles of 128 tokens by `tn` weight
+// rows; within it
+//   * one thread loads 64-column slices of x and W by TMA (128-byte swizzled
+//     rows, zero past the edges) into a ring of stages,
+//   * one thread issues tcgen05.mma kind::f16, M = 128 tokens, N = tn, K = 16,
+//     into one of two TMEM accumulators,
+//   * four warps read the other accumulator (a lane is a token, its registers
+//     consecutive rows of y), apply bias, activation, factor and residual in
+//     FP32 and write y: the epilogue of a tile runs behind the products of the next.
+// tn is the multiple of 16 whose waves of tiles cost least on this GPU's SMs
+// (gemm_tile).  Tokens as the MMA's rows rather than weight rows: y is
+// token-major, so a lane's results are contiguous.
+// Every wait is bounded: on a timeout the CTA sets an error bit, lets its
+// copies and MMAs drain, frees its TMEM and returns.
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "kernels.h"
+#include "linear_epilogue.cuh"
+#include "tcgen05.cuh"
+
+namespace xksv {
+namespace {
+
+constexpr int GM = 128;          // tokens of a tile
+constexpr int GK = 64;           // columns of a stage: 128-byte rows
+constexpr int GTHREADS = 192;    // producer, MMA and four epilogue warps
+constexpr uint32_t kMaxStages = 8;
+constexpr uint32_t kABytes = GM * GK * 2;
+constexpr size_t kRing = 220 * 1024;  // stages' shared memory
+
+struct GemmShared {
+  uint64_t full[kMaxStages], empty[kMaxStages], tfull[2], tempty[2];
+  uint32_t tmem;
+  int abort_flag;
+};
+
+struct GemmArgs {
+  Epilogue e;
+  uint64_t row0;  // row of Y that the segment's first weight row gives
+  uint32_t batch, rows, cols, tn, stages, tmem_cols;
+  int* status;
+};
+
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
+  for (uint32_t i = 0; i < kSpin; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255) == 255 && *abort_flag) return false;
+    if (i > 64) __nanosleep(32);
+  }
+  return false;
+}
+
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(bytes) : "memory");
+}
+// Box of `map` at (x, y) into dst; bytes counted on bar.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+// Shared-memory descriptor of a K-major operand of 128-byte swizzled rows:
+// eight rows are 1024 bytes (SBO), layout type 2 in bits 61-63.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+  return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(64) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
+}
+
+__global__ void __launch_bounds__(GTHREADS, 1)
+    linear_gemm_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const GemmArgs a) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ GemmShared S;
+  uint8_t* ring = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t stage_bytes = kABytes + a.tn * GK * 2;
+  const uint32_t mt = (a.batch + GM - 1) / GM, nt = (a.rows + a.tn - 1) / a.tn, tiles = mt * nt;
+  const uint32_t ksteps = (a.cols + GK - 1) / GK;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&S.tmem)), "r"(a.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < a.stages; ++s) {
+      mbar_init(smem_addr(&S.full[s]), 1);
+      mbar_init(smem_addr(&S.empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_addr(&S.tfull[b]), 1);
+      mbar_init(smem_addr(&S.tempty[b]), 128);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    S.abort_flag = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = S.tmem;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t n = 0;  // slices loaded
+      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        const uint32_t m0 = t % mt * GM, n0 = t / mt * a.tn;
+        for (uint32_t k = 0; k < ksteps; ++k, ++n) {
+          const uint32_t s = n % a.stages, bar = smem_addr(&S.full[s]);
+          ok = wait_or_abort(smem_addr(&S.empty[s]), ((n / a.stages) & 1) ^ 1, &S.abort_flag);
+          if (!ok) break;
+          const uint32_t dst = smem_addr(ring) + s * stage_bytes;
+          expect_bytes(bar, stage_bytes);
+          tma_load(dst, &mx, k * GK, m0, bar);
+          tma_load(dst + kABytes, &mw, k * GK, n0, bar);
+        }
+      }
+      if (!ok) S.abort_flag = 1;
+      // every copy has landed before the CTA ends
+      for (uint32_t i = n > a.stages ? n - a.stages : 0; i < n; ++i)
+        if (!mbar_wait(smem_addr(&S.full[i % a.stages]), (i / a.stages) & 1)) ok = false;
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_bf16(GM, a.tn);
+      uint32_t n = 0, ti = 0;  // slices multiplied, tiles begun
+      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
+        const uint32_t buf = ti & 1, d = tmem + buf * (a.tmem_cols / 2);
+        ok = wait_or_abort(smem_addr(&S.tempty[buf]), ((ti >> 1) & 1) ^ 1, &S.abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        for (uint32_t k = 0; k < ksteps; ++k, ++n) {
+          const uint32_t s = n % a.stages;
+          ok = wait_or_abort(smem_addr(&S.full[s]), (n / a.stages) & 1, &S.abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t src = smem_addr(ring) + s * stage_bytes;
+          const uint64_t da = desc_sw128(src), db = desc_sw128(src + kABytes);
+#pragma unroll
+          for (uint32_t j = 0; j < GK / 16; ++j)  // 32 bytes further along the rows
+            umma_bf16(d, da + 2 * j, db + 2 * j, idesc, (k | j) != 0);
+          umma_commit(smem_addr(&S.empty[s]));
+        }
+        if (ok) umma_commit(smem_addr(&S.tfull[buf]));
+      }
+      if (!ok) S.abort_flag = 1;
+      // the MMAs issued are done before TMEM is freed: they complete in
+      // order, and the last slice's commit follows them all
+      if (n && !mbar_wait(smem_addr(&S.empty[(n - 1) % a.stages]), ((n - 1) / a.stages) & 1)) ok = false;
+    }
+  } else {
+    const uint32_t quarter = warp & 3, ti0 = quarter * 32;  // this warp's TMEM lanes
+    uint32_t ti = 0;
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, ++ti) {
+      const uint32_t m0 = t % mt * GM, n0 = t / mt * a.tn, buf = ti & 1;
+      ok = wait_or_abort(smem_addr(&S.tfull[buf]), (ti >> 1) & 1, &S.abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t b = m0 + ti0 + lane;
+      const uint32_t top = min(a.tn, a.rows - n0);
+      for (uint32_t c = 0; c < top; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(tmem + (ti0 << 16) + buf * (a.tmem_cols / 2) + c, r);
+        if (b < a.batch) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float v[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(r[8 * g + x]);
+            epilogue_store8(a.e, b, a.row0 + n0 + c + 8 * g, v, int(top) - int(c + 8 * g));
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(smem_addr(&S.tempty[buf]));
+    }
+    if (!ok) S.abort_flag = 1;
+  }
+  if (!ok && lane == 0) atomicOr(a.status, kStatusInternal);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+  }
+}
+
+// x's columns [0, cols) as BF16 rows of `pitch` elements (zeros behind), for
+// rows that TMA cannot address.
+__global__ void linear_rows_kernel(const uint16_t* __restrict__ x, uint64_t stride, uint64_t batch, uint64_t cols,
+                                   uint64_t pitch, uint16_t* __restrict__ out) {
+  for (uint64_t i = blockIdx.x * uint64_t(blockDim.x) + threadIdx.x; i < batch * pitch; i += uint64_t(gridDim.x) * blockDim.x) {
+    const uint64_t b = i / pitch, c = i - b * pitch;
+    out[i] = c < cols ? x[b * stride + c] : uint16_t(0);
+  }
+}
+
+// Weight rows of a tile: the multiple of 16 whose waves of tiles cost least,
+// a tile costing its products (tn) and a fixed part of about 32 rows' worth
+// (its slices of x, its start and epilogue).
+uint32_t gemm_tile(uint32_t batch, uint32_t rows, int sms) {
+  const uint64_t mt = (batch + GM - 1) / GM;
+  uint64_t best = ~uint64_t(0);
+  uint32_t tn = 256;
+  for (uint32_t n = 256; n >= 32; n -= 16) {
+    const uint64_t waves = (mt * ((rows + n - 1) / n) + sms - 1) / sms, cost = waves * (n + 32);
+    if (cost < best) {
+      best = cost;
+      tn = n;
+    }
+  }
+  return tn;
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static std::once_flag once;
+  static EncodeTiled fn = nullptr;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(p);
+  });
+  return fn;
+}
+
+// BF16 [rows, cols], rows `pitch` elements apart, read in boxes of 64 columns by `box` rows.
+bool tensor_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box) {
+  const EncodeTiled fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch * 2};
+  const cuuint32_t boxes[2] = {GK, box}, steps[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, steps,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+bool linear_rows_direct(const void* x, uint64_t stride, uint64_t xoff) {
+  return ((reinterpret_cast<uintptr_t>(x) + xoff * 2) | stride * 2) % 16 == 0;
+}
+
+cudaError_t launch_linear_rows(const void* x, uint64_t stride, uint64_t batch, uint64_t cols, uint64_t pitch, void* out,
+                               cudaStream_t st) {
+  const uint64_t n = batch * pitch;
+  linear_rows_kernel<<<uint32_t(std::min<uint64_t>((n + 255) / 256, 8192)), 256, 0, st>>>(
+      static_cast<const uint16_t*>(x), stride, batch, cols, pitch, static_cast<uint16_t*>(out));
+  return cudaGetLastError();
+}
+
+cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, const void* x, uint64_t x_pitch, uint32_t batch,
+                               uint64_t row0, const Epilogue& e, int* status, int sms, cudaStream_t st) {
+  GemmArgs a{};
+  a.e = e;
+  a.row0 = row0;
+  a.batch = batch;
+  a.rows = rows;
+  a.cols = cols;
+  a.status = status;
+  a.tn = gemm_tile(batch, rows, sms);
+  const uint32_t stage = kABytes + a.tn * GK * 2;
+  a.stages = std::min<uint32_t>(kMaxStages, uint32_t(kRing / stage));
+  a.tmem_cols = 32;
+  while (a.tmem_cols < 2 * ((a.tn + 31) / 32 * 32)) a.tmem_cols *= 2;
+  CUtensorMap mx, mw;
+  if (!tensor_map(&mx, x, batch, cols, x_pitch, GM) || !tensor_map(&mw, w, rows, cols, cols, a.tn)) return cudaErrorInvalidValue;
+  const size_t smem = size_t(a.stages) * stage + 1024;
+  // one CTA an SM, whatever the tile: its TMEM columns are its own
+  const size_t ask = std::max<size_t>(smem, 120 * 1024);
+  const cudaError_t err = cudaFuncSetAttribute(linear_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRing + 1024));
+  if (err != cudaSuccess) return err;
+  const uint64_t tiles = uint64_t((batch + GM - 1) / GM) * ((rows + a.tn - 1) / a.tn);
+  linear_gemm_kernel<<<uint32_t(std::min<uint64_t>(tiles, uint64_t(sms))), GTHREADS, ask, st>>>(mx, mw, a);
+  return cudaGetLastError();
+}
+
+}  // namespace xksv

@@ -48,9 +48,9 @@ class KvDesc(ctypes.Structure):
 class KvAppendArgs(ctypes.Structure):
     """xksv_kv_append_args."""
     _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
-                ("q_stride", ctypes.c_uint64 * 2), ("k_stride", ctypes.c_uint64 * 2),
-                ("v_stride", ctypes.c_uint64 * 2), ("q_out_stride", ctypes.c_uint64 * 2),
-                ("tokens", ctypes.c_uint64), ("table", ctypes.c_void_p), ("table_rows", ctypes.c_uint64),
+                ("q_token", ctypes.c_uint64), ("q_head", ctypes.c_uint64), ("k_token", ctypes.c_uint64),
+                ("k_head", ctypes.c_uint64), ("v_token", ctypes.c_uint64), ("v_head", ctypes.c_uint64),
+                ("q_out_token", ctypes.c_uint64), ("q_out_head", ctypes.c_uint64), ("tokens", ctypes.c_uint64), ("table", ctypes.c_void_p), ("table_rows", ctypes.c_uint64),
                 ("table_cols", ctypes.c_uint64), ("table_stride", ctypes.c_uint64), ("seq", ctypes.c_void_p),
                 ("index", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
                 ("rot_scale", ctypes.c_float), ("rot_dim", ctypes.c_uint32), ("q_heads", ctypes.c_uint32),
@@ -60,7 +60,8 @@ class KvAppendArgs(ctypes.Structure):
 class KvAttendArgs(ctypes.Structure):
     """xksv_kv_attend_args."""
     _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
-                ("q_stride", ctypes.c_uint64 * 2), ("out_stride", ctypes.c_uint64 * 2), ("seqs", ctypes.c_uint64),
+                ("q_seq", ctypes.c_uint64), ("q_head", ctypes.c_uint64), ("out_seq", ctypes.c_uint64),
+                ("out_head", ctypes.c_uint64), ("seqs", ctypes.c_uint64),
                 ("table", ctypes.c_void_p), ("table_cols", ctypes.c_uint64), ("table_stride", ctypes.c_uint64),
                 ("lens", ctypes.c_void_p), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
                 ("window", ctypes.c_uint64), ("q_heads", ctypes.c_uint32), ("type", ctypes.c_uint32)]
@@ -129,6 +130,7 @@ _SIGS = {
     "xksv_cuda_decode_noalloc": ([ctypes.POINTER(Slab), ctypes.c_size_t, ctypes.c_void_p,
                                   ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t,
                                   ctypes.c_void_p], ctypes.c_int),
+    "xksv_plan_device": ([ctypes.c_void_p], ctypes.c_int),
     "xksv_plan_linear_workspace": ([ctypes.c_void_p, ctypes.c_size_t], ctypes.c_size_t),
     "xksv_plan_linear": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.POINTER(LinearArgs),
                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
@@ -144,7 +146,6 @@ _SIGS = {
 
 # element types and activations of the linear layer and the key/value cache
 BF16, FP16, FP32, E4M3 = 1, 2, 3, 4
-TYPE_BY_NAME = {"torch.bfloat16": BF16, "torch.float16": FP16, "torch.float32": FP32, "torch.float8_e4m3fn": E4M3}
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 KV_INTERLEAVED = 1
 
@@ -294,54 +295,73 @@ def _rows(buf, nrows, batch, what):
     return int(buf), int(nrows)
 
 
+_types = {}
+
+
 def _type(t, allowed, what):
     """The element type code of tensor t, one of `allowed`."""
-    code = TYPE_BY_NAME.get(str(t.dtype))
+    if not _types:
+        import torch
+        _types.update({torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32, torch.float8_e4m3fn: E4M3})
+    code = _types.get(t.dtype)
     if code not in allowed:
         raise ValueError(f"{what}: dtype {t.dtype} is not supported")
     return code
 
 
-def _matrix(t, rows, cols, what, device, least=False):
-    """(address, row stride) of a [rows, cols] tensor whose rows are contiguous
-    (with `least`, cols or more columns)."""
-    if t.dim() != 2 or t.shape[0] != rows or (t.shape[1] < cols if least else t.shape[1] != cols):
+def _matrix(t, rows, cols, what, device):
+    """(address, row stride) of a [rows, cols] tensor whose rows are contiguous."""
+    if t.shape != (rows, cols):
         raise ValueError(f"{what}: shape {tuple(t.shape)} is not [{rows}, {cols}]")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    row, one = t.stride()
+    if one != 1 and cols > 1:
         raise ValueError(f"{what}: rows must be contiguous")
-    if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, expected {device}")
-    return t.data_ptr(), max(t.stride(0), 0)
+    if t.get_device() != device:
+        raise ValueError(f"{what}: on {t.device}, expected CUDA device {device}")
+    return t.data_ptr(), row
 
 
 def _heads(t, rows, heads, dim, what, device):
-    """(address, (row, head) strides) of a [rows, heads, dim] tensor whose
+    """(address, row stride, head stride) of a [rows, heads, dim] tensor whose
     last dimension is contiguous."""
-    if tuple(t.shape) != (rows, heads, dim):
+    if t.shape != (rows, heads, dim):
         raise ValueError(f"{what}: shape {tuple(t.shape)} is not [{rows}, {heads}, {dim}]")
-    if t.stride(2) != 1 and dim > 1:
+    row, head, one = t.stride()
+    if one != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous")
-    if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, expected {device}")
-    return t.data_ptr(), (t.stride(0), t.stride(1))
+    if t.get_device() != device:
+        raise ValueError(f"{what}: on {t.device}, expected CUDA device {device}")
+    return t.data_ptr(), row, head
 
 
 def _ints(t, n, what, device):
     """Address of a contiguous int32 [n] tensor."""
-    if str(t.dtype) != "torch.int32" or tuple(t.shape) != (n,) or (n > 1 and t.stride(0) != 1):
+    if t.dtype != _int32() or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 [{n}] tensor is needed")
-    if t.device != device:
-        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    if t.get_device() != device:
+        raise ValueError(f"{what}: on {t.device}, expected CUDA device {device}")
     return t.data_ptr()
+
+
+def _int32():
+    global _i32
+    if _i32 is None:
+        import torch
+        _i32 = torch.int32
+    return _i32
+
+
+_i32 = None
 
 
 def _table(t, device):
     """(address, rows, columns, row stride) of an int32 page table."""
-    if str(t.dtype) != "torch.int32" or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dtype != _int32() or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError("table: an int32 [sequences, pages] tensor with contiguous rows is needed")
-    if t.device != device:
-        raise ValueError(f"table: on {t.device}, expected {device}")
-    return t.data_ptr(), t.shape[0], t.shape[1], t.stride(0)
+    if t.get_device() != device:
+        raise ValueError(f"table: on {t.device}, expected CUDA device {device}")
+    rows, cols = t.shape
+    return t.data_ptr(), rows, cols, t.stride(0)
 
 
 def _workspace(given, nbytes, device, stream):
@@ -376,6 +396,7 @@ class Plan:
             raise ValueError("xksv_plan_create rejected the slab table")
         self.handle = h
         self.n = n
+        self.device = self.lib.xksv_plan_device(h)  # its calls' tensors live there
 
     def decode(self, d_payload, d_out, stream=0, payload_bytes=None, out_bytes=None):
         pay, npay = dev_buffer(d_payload, payload_bytes, "payload")
@@ -409,7 +430,7 @@ class Plan:
         linear_workspace(batch) bytes) defaults to a new buffer per call."""
         if act not in ACTS:
             raise ValueError(f"unknown activation {act}")
-        device = x.device
+        device = self.device
         pay, npay = dev_buffer(d_payload, payload_bytes, "payload")
         if x.dim() != 2 or y.dim() != 2:
             raise ValueError("x and y are [batch, columns]")
@@ -421,8 +442,8 @@ class Plan:
         a.y_type = _type(y, (BF16, FP32), "y")
         if bias is not None:
             a.bias_type = _type(bias, (BF16, FP32), "bias")
-            if tuple(bias.shape) != (rows,) or (rows > 1 and bias.stride(0) != 1) or bias.device != device:
-                raise ValueError(f"bias: a contiguous [{rows}] tensor on {device} is needed")
+            if tuple(bias.shape) != (rows,) or (rows > 1 and bias.stride(0) != 1) or bias.get_device() != device:
+                raise ValueError(f"bias: a contiguous [{rows}] tensor on CUDA device {device} is needed")
             a.bias = bias.data_ptr()
         if mul is not None:
             a.mul_type = _type(mul, (BF16, FP32), "mul")
@@ -431,7 +452,7 @@ class Plan:
             a.residual_type = _type(residual, (BF16, FP32), "residual")
             a.residual, a.residual_stride = _matrix(residual, batch, rows, "residual", device)
         a.act = ACTS[act]
-        ws, wp, wn = _workspace(workspace, self.linear_workspace(batch), device, stream)
+        ws, wp, wn = _workspace(workspace, self.linear_workspace(batch), x.device, stream)
         if self.lib.xksv_plan_linear(self.handle, pay, npay, ctypes.byref(a), wp, wn, stream):
             raise RuntimeError("xksv_plan_linear refused the call or failed to launch")
 
@@ -508,7 +529,7 @@ class KVCache:
         self.lib = lib or load()
         self.handle = None
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device, self.type = k.device, _type(k, (BF16, FP16, E4M3), "k")
+        self.device, self.index, self.type = k.device, k.get_device(), _type(k, (BF16, FP16, E4M3), "k")
         order = (0, 1, 2) if layout == "nhd" else (0, 2, 1)  # page, token, head
         self.pages, self.page_size, self.kv_heads = (k.shape[i] for i in order)
         self.head_dim = k.shape[3]
@@ -537,36 +558,34 @@ class KVCache:
         seq[t] (default t; negative: padding, skipped), rotated by positions[t]
         (default index[t]) and inv_freq FP32 [rotated dims / 2] (None: no
         rotation).  q_out defaults to q, in place."""
-        n, dev = k.shape[0], self.device
-        a = KvAppendArgs()
-        a.type = _type(k, (BF16, FP16, FP32), "k")
-        a.k, a.k_stride[:] = _heads(k, n, self.kv_heads, self.head_dim, "k", dev)
-        a.v, a.v_stride[:] = _heads(v, n, self.kv_heads, self.head_dim, "v", dev)
+        n, dev, dim = k.shape[0], self.index, self.head_dim
+        code = _type(k, (BF16, FP16, FP32), "k")
+        kp, k0, k1 = _heads(k, n, self.kv_heads, dim, "k", dev)
+        vp, v0, v1 = _heads(v, n, self.kv_heads, dim, "v", dev)
         if v.dtype != k.dtype:
             raise ValueError("k and v are of one dtype")
+        qp = q0 = q1 = op = o0 = o1 = heads = 0
         if q is not None:
             q_out = q if q_out is None else q_out
             if q.dtype != k.dtype or q_out.dtype != k.dtype or q.dim() != 3:
                 raise ValueError("q and q_out are [tokens, heads, dim] of k's dtype")
-            a.q_heads = q.shape[1]
-            a.q, a.q_stride[:] = _heads(q, n, q.shape[1], self.head_dim, "q", dev)
-            a.q_out, a.q_out_stride[:] = _heads(q_out, n, q.shape[1], self.head_dim, "q_out", dev)
+            heads = q.shape[1]
+            qp, q0, q1 = _heads(q, n, heads, dim, "q", dev)
+            op, o0, o1 = _heads(q_out, n, heads, dim, "q_out", dev)
         elif q_out is not None:
             raise ValueError("q_out without q")
-        a.tokens = n
-        a.table, a.table_rows, a.table_cols, a.table_stride = _table(table, dev)
-        a.index = _ints(index, n, "index", dev)
-        if seq is not None:
-            a.seq = _ints(seq, n, "seq", dev)
-        if positions is not None:
-            a.positions = _ints(positions, n, "positions", dev)
+        tp, rows, cols, stride = _table(table, dev)
+        ip = _ints(index, n, "index", dev)
+        sp = None if seq is None else _ints(seq, n, "seq", dev)
+        pp = None if positions is None else _ints(positions, n, "positions", dev)
+        fp, rot = None, 0
         if inv_freq is not None:
-            if str(inv_freq.dtype) != "torch.float32" or inv_freq.dim() != 1 or inv_freq.device != dev \
-                    or (inv_freq.numel() > 1 and inv_freq.stride(0) != 1):
-                raise ValueError(f"inv_freq: a contiguous FP32 vector on {dev} is needed")
-            a.inv_freq, a.rot_dim = inv_freq.data_ptr(), 2 * inv_freq.numel()
-        a.rot_scale = rot_scale
-        a.flags = KV_INTERLEAVED if interleaved else 0
+            _type(inv_freq, (FP32,), "inv_freq")
+            if inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
+                raise ValueError(f"inv_freq: a contiguous FP32 vector on CUDA device {dev} is needed")
+            fp, rot = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
+        a = KvAppendArgs(qp, kp, vp, op, q0, q1, k0, k1, v0, v1, o0, o1, n, tp, rows, cols, stride, sp, ip, pp, fp,
+                         rot_scale, rot, heads, code, KV_INTERLEAVED if interleaved else 0)
         if self.lib.xksv_kv_append(self.handle, ctypes.byref(a), stream):
             raise RuntimeError("xksv_kv_append refused the call or failed to launch")
 
@@ -577,30 +596,30 @@ class KVCache:
         heads] or None; scale defaults to dim ** -0.5; window 0 sees the whole
         sequence; softcap 0 is off.  `workspace` (uint8, at least
         attend_workspace(...) bytes) defaults to a new buffer per call."""
-        dev, n = self.device, lens.shape[0]
+        dev, n, dim = self.index, lens.shape[0], self.head_dim
         if q.dim() != 3 or out.dtype != q.dtype:
             raise ValueError("q and out are [sequences, heads, dim] of one dtype")
         heads = q.shape[1]
-        a = KvAttendArgs()
-        a.type = _type(q, (BF16, FP16), "q")
-        a.q, a.q_stride[:] = _heads(q, n, heads, self.head_dim, "q", dev)
-        a.out, a.out_stride[:] = _heads(out, n, heads, self.head_dim, "out", dev)
+        code = _type(q, (BF16, FP16), "q")
+        qp, q0, q1 = _heads(q, n, heads, dim, "q", dev)
+        op, o0, o1 = _heads(out, n, heads, dim, "out", dev)
+        lp = None
         if lse is not None:
-            if str(lse.dtype) != "torch.float32" or tuple(lse.shape) != (n, heads) or not lse.is_contiguous() \
-                    or lse.device != dev:
-                raise ValueError(f"lse: a contiguous FP32 [{n}, {heads}] tensor on {dev} is needed")
-            a.lse = lse.data_ptr()
-        a.table, rows, a.table_cols, a.table_stride = _table(table, dev)
+            _type(lse, (FP32,), "lse")
+            if lse.shape != (n, heads) or not lse.is_contiguous() or lse.get_device() != dev:
+                raise ValueError(f"lse: a contiguous FP32 [{n}, {heads}] tensor on CUDA device {dev} is needed")
+            lp = lse.data_ptr()
+        tp, rows, cols, stride = _table(table, dev)
         if rows < n:
             raise ValueError(f"table: {rows} rows for {n} sequences")
-        a.seqs, a.q_heads = n, heads
-        a.lens = _ints(lens, n, "lens", dev)
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
         if window < 0:
             raise ValueError("window is not negative")
-        a.window, a.softcap = window, softcap
-        need = self.lib.xksv_kv_attend_workspace(self.handle, n, heads, a.table_cols)
-        ws, wp, wn = _workspace(workspace, need, dev, stream)
+        a = KvAttendArgs(qp, op, lp, q0, q1, o0, o1, n, tp, cols, stride, _ints(lens, n, "lens", dev),
+                         dim ** -0.5 if scale is None else scale, softcap, window, heads, code)
+        ws, wp, wn = workspace, None, 0
+        if n:
+            need = self.lib.xksv_kv_attend_workspace(self.handle, n, heads, cols)
+            ws, wp, wn = _workspace(workspace, need, self.device, stream)
         if self.lib.xksv_kv_attend(self.handle, ctypes.byref(a), wp, wn, stream):
             raise RuntimeError("xksv_kv_attend refused the call or failed to launch")
 
