@@ -220,6 +220,8 @@ struct xksv_plan {
   xksv::FusedGroup* d_fgroups = nullptr;
   uint32_t* d_fmembers = nullptr;
   void* d_ftabs = nullptr;  // per group: its lane tables, built with the index
+  uint32_t n_fgroups = 0;
+  uint32_t* d_fparts = nullptr;  // per group: the segments its rows are summed from
   uint64_t* d_hash_ranges = nullptr;  // per slab in creation order: {dst, decoded bytes}
   // linear layer (xksv_plan_linear): the runs of Y rows the slabs cover; off
   // when two slabs cover one row or a slab has no rows and columns
@@ -248,6 +250,8 @@ void free_index(xksv_plan* p) {
   if (p->d_fgroups) cudaFree(p->d_fgroups);
   if (p->d_fmembers) cudaFree(p->d_fmembers);
   if (p->d_ftabs) cudaFree(p->d_ftabs);
+  if (p->d_fparts) cudaFree(p->d_fparts);
+  p->d_fparts = nullptr;
   p->d_ftabs = nullptr;
   p->d_fseg0 = nullptr;
   p->d_ftasks = nullptr;
@@ -836,6 +840,40 @@ cudaError_t decode_scratch(xksv_plan* p, const uint8_t* pay, uint8_t* scratch, c
   return e;
 }
 
+// The indexed kernels' arguments that only depend on the plan.
+GemvArgs gemv_args(const xksv_plan* p, const uint8_t* pay) {
+  GemvArgs g{};
+  g.items = p->d_items;
+  g.nitems = p->n_items;
+  g.slabs = p->d_slabs;
+  g.tbase = p->d_tbase;
+  g.tidx = p->d_tidx;
+  g.gtabs = p->d_gtabs;
+  g.tmid = p->d_tmid;
+  g.payload = pay;
+  g.partials = p->d_partials;
+  g.counters = p->d_counters;
+  g.status = p->d_status;
+  return g;
+}
+FusedArgs fused_args(const xksv_plan* p, const uint8_t* pay, size_t batch) {
+  FusedArgs f{};
+  f.seg0 = p->d_fseg0;
+  f.tasks = p->d_ftasks;
+  f.groups = p->d_fgroups;
+  f.members = p->d_fmembers;
+  f.slabs = p->d_slabs;
+  f.tbase = p->d_tbase;
+  f.tidx = p->d_tidx;
+  f.tmid = p->d_tmid;
+  f.tabs = p->d_ftabs;
+  f.payload = pay;
+  f.nb = uint32_t(batch);
+  f.npad = (f.nb + 15) / 16 * 16;
+  f.status = p->d_status;
+  return f;
+}
+
 // Enqueues Y = W X (xksv_plan_gemm after its checks) with the given buffers
 // for X^T in BF16 [256][x_cols] and the decoded weights, which only the
 // tensor-core routes touch.
@@ -854,24 +892,11 @@ int gemm_run(xksv_plan* p, const uint8_t* pay, const float* d_x, float* d_y, siz
   if (fused) {
     // one kernel decodes every tile row into tensor-core operand stages,
     // after a prep kernel (X^T in BF16, zeroed Y rows) that it overlaps
-    FusedArgs f{};
-    f.seg0 = p->d_fseg0;
-    f.tasks = p->d_ftasks;
-    f.groups = p->d_fgroups;
-    f.members = p->d_fmembers;
-    f.slabs = p->d_slabs;
-    f.tbase = p->d_tbase;
-    f.tidx = p->d_tidx;
-    f.tmid = p->d_tmid;
-    f.tabs = p->d_ftabs;
-    f.payload = pay;
+    FusedArgs f = fused_args(p, pay, batch);
     f.xt = xt;
     f.xt_ld = p->x_cols;
     f.y = d_y;
     f.ld = ld;
-    f.nb = uint32_t(batch);
-    f.npad = (f.nb + 15) / 16 * 16;
-    f.status = p->d_status;
     e = launch_fused_gemm(f, p->n_fctas, d_x + p->x_base * ld, p->x_cols, p->d_groups, p->ngroups, st);
     p->launches = 2;
     return e == cudaSuccess ? 0 : 1;
@@ -903,22 +928,11 @@ int gemm_run(xksv_plan* p, const uint8_t* pay, const float* d_x, float* d_y, siz
   const uint32_t ser0 = indexed ? p->n_ser_idx : 0;
   if (indexed && p->n_items) {
     for (size_t b0 = 0; b0 < batch && e == cudaSuccess; b0 += 4) {
-      GemvArgs g{};
-      g.items = p->d_items;
-      g.nitems = p->n_items;
-      g.slabs = p->d_slabs;
-      g.tbase = p->d_tbase;
-      g.tidx = p->d_tidx;
-      g.gtabs = p->d_gtabs;
-      g.tmid = p->d_tmid;
-      g.payload = pay;
+      GemvArgs g = gemv_args(p, pay);
       g.x = d_x + b0;
       g.y = d_y + b0;
       g.ld = ld;
       g.nb = uint32_t(std::min<size_t>(4, batch - b0));
-      g.partials = p->d_partials;
-      g.counters = p->d_counters;
-      g.status = p->d_status;
       e = launch_serial_tile_gemm(g, st);
       ++p->launches;
     }
@@ -975,28 +989,38 @@ struct Carve {
     return at;
   }
 };
-struct LinearSpace {
-  bool gemm;  // decoded weights, x in place (or its rows copied to xt), no x / z
-  uint64_t x, z, xt, scratch, total;
-};
 constexpr uint64_t pitch_of(uint64_t cols) { return (cols + 7) / 8 * 8; }
-// What a call needs of each part; the payload decides whether the tile index
-// (and so the fused kernel) is there: null counts for any.
+// How a call runs: every slab indexed and up to three tokens (the tile kernel
+// with its epilogue), up to 128 (the fused kernel with its epilogue), decoded
+// weights and the tensor-core product (from four tokens), or any plan's
+// product between two layout changes.
+enum class Route { Tile, Fused, Gemm, Any };
+struct LinearSpace {
+  Route route;
+  uint64_t x, z, rows, scratch, total;  // workspace offsets; rows: x's rows, aligned
+};
+// The payload decides whether the tile index is there: null counts for none.
 LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload) {
   Carve c;
   LinearSpace s{};
-  const bool fused = payload && gemm_fused(p, payload, batch);
-  if (p->tc_ok && batch >= 4 && !fused) {
-    s.gemm = true;
-    s.xt = c.take(batch * pitch_of(p->need_x_rows) * 2);
+  const bool indexed = payload && p->d_tidx && payload == p->indexed_payload && p->n_items;
+  const bool all = indexed && p->n_ser_idx == p->n_ser + p->n_par + p->n_raw;
+  if (all && batch <= 3) {
+    s.route = Route::Tile;
+  } else if (payload && gemm_fused(p, payload, batch)) {
+    s.route = Route::Fused;
+    s.z = c.take(uint64_t(p->n_fgroups) * (16 * ((batch + 15) / 16 * 16) * 32 + 1) * 4 + 16);
+    s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
+  } else if (p->tc_ok && batch >= 4) {
+    s.route = Route::Gemm;
+    s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
     s.scratch = c.take(p->scratch_bytes);
-    s.total = c.pos;
-    return s;
+  } else {
+    s.route = Route::Any;
+    s.x = c.take(p->need_x_rows * batch * sizeof(float));
+    s.z = c.take(p->need_y_rows * batch * sizeof(float));
   }
-  s.x = c.take(p->need_x_rows * batch * sizeof(float));
-  s.z = c.take(p->need_y_rows * batch * sizeof(float));
-  if (fused) s.xt = c.take(256 * p->x_cols * 2);
-  s.total = c.pos;
+  s.total = std::max<uint64_t>(c.pos, 256);
   return s;
 }
 constexpr uint64_t kMaxBatch = 1ull << 20;
@@ -1048,8 +1072,6 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
   if (!dev.ok) return 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto* ws = static_cast<uint8_t*>(d_workspace);
-  auto* x = reinterpret_cast<float*>(ws + sp.x);
-  auto* z = reinterpret_cast<float*>(ws + sp.z);
   Epilogue ep{};
   ep.y = a->y;
   ep.bias = a->bias;
@@ -1072,33 +1094,57 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
            whole(ep.mul, ep.mul_stride, ep.mul_f32) && whole(ep.residual, ep.residual_stride, ep.residual_f32);
   for (const LinearSeg& g : p->segs) ep.vec = ep.vec && g.row0 % 8 == 0;
   const auto* pay = static_cast<const uint8_t*>(d_payload);
-  if (sp.gemm) {
-    // decode, then one tensor-core product with its epilogue per weight
-    const uint64_t xs = a->batch > 1 ? a->x_stride : pitch_of(a->x_cols);
-    const void* xp = a->x;
-    uint64_t pitch = xs;
-    bool direct = true;
-    for (const LinearSeg& g : p->segs) direct = direct && linear_rows_direct(a->x, xs, p->x_base + g.xoff);
-    if (!direct) {  // (X offsets of a tensor-core plan are multiples of 8)
-      xp = ws + sp.xt;
-      pitch = pitch_of(p->need_x_rows);
-      if (launch_linear_rows(a->x, a->x_stride, a->batch, p->need_x_rows, pitch, ws + sp.xt, st) != cudaSuccess) return 1;
-      ++p->launches;
-    }
-    if (decode_scratch(p, pay, ws + sp.scratch, st) != cudaSuccess) return 1;
-    for (const LinearSeg& g : p->segs) {
-      if (launch_linear_gemm(ws + sp.scratch + g.a_off, g.rows, g.cols,
-                             static_cast<const uint16_t*>(xp) + p->x_base + g.xoff, pitch, uint32_t(a->batch), g.row0,
-                             ep, p->d_status, p->sms, st) != cudaSuccess)
-        return 1;
-      ++p->launches;
-    }
+  const uint64_t xs = a->batch > 1 ? a->x_stride : pitch_of(a->x_cols);
+  if (sp.route == Route::Tile) {
+    GemvArgs g = gemv_args(p, pay);
+    g.xb = a->x;
+    g.xb_stride = xs;
+    g.nb = uint32_t(a->batch);
+    g.e = ep;
+    p->launches = 1;
+    return launch_serial_tile_linear(g, st) == cudaSuccess ? 0 : 1;
+  }
+  if (sp.route == Route::Any) {
+    auto* x = reinterpret_cast<float*>(ws + sp.x);
+    auto* z = reinterpret_cast<float*>(ws + sp.z);
+    if (launch_linear_x(a->x, xs, a->batch, p->need_x_rows, x, st) != cudaSuccess) return 1;
+    if (gemm_run(p, pay, x, z, a->batch, nullptr, nullptr, st)) return 1;
+    if (launch_linear_y(z, a->batch, p->d_runs, p->n_runs, p->max_run, ep, st) != cudaSuccess) return 1;
+    p->launches += 2;
     return 0;
   }
-  if (launch_linear_x(a->x, a->x_stride, a->batch, p->need_x_rows, x, st) != cudaSuccess) return 1;
-  if (gemm_run(p, pay, x, z, a->batch, ws + sp.xt, ws + sp.scratch, st)) return 1;
-  if (launch_linear_y(z, a->batch, p->d_runs, p->n_runs, p->max_run, ep, st) != cudaSuccess) return 1;
-  p->launches += 2;
+  // the tensor cores read x's rows as 16-byte words: in place when they are,
+  // else copied (X offsets of a tensor-core plan are multiples of 8)
+  const void* xp = a->x;
+  uint64_t pitch = xs;
+  bool direct = true;
+  for (const LinearSeg& g : p->segs) direct = direct && linear_rows_direct(a->x, xs, p->x_base + g.xoff);
+  if (!direct) {
+    xp = ws + sp.rows;
+    pitch = pitch_of(p->need_x_rows);
+    if (launch_linear_rows(a->x, xs, a->batch, p->need_x_rows, pitch, ws + sp.rows, st) != cudaSuccess) return 1;
+    ++p->launches;
+  }
+  const uint16_t* x0 = static_cast<const uint16_t*>(xp) + p->x_base;
+  if (sp.route == Route::Fused) {
+    FusedArgs f = fused_args(p, pay, a->batch);
+    f.xt = x0;
+    f.xt_ld = pitch;
+    f.y = reinterpret_cast<float*>(ws + sp.z);
+    f.arrived = reinterpret_cast<uint32_t*>(f.y + uint64_t(p->n_fgroups) * 16 * f.npad * 32);
+    f.parts = p->d_fparts;
+    f.e = ep;
+    p->launches += 2;
+    return launch_fused_linear(f, p->n_fctas, p->n_fgroups, st) == cudaSuccess ? 0 : 1;
+  }
+  // decode, then one tensor-core product with its epilogue per weight
+  if (decode_scratch(p, pay, ws + sp.scratch, st) != cudaSuccess) return 1;
+  for (const LinearSeg& g : p->segs) {
+    if (launch_linear_gemm(ws + sp.scratch + g.a_off, g.rows, g.cols, x0 + g.xoff, pitch, uint32_t(a->batch), g.row0, ep,
+                           p->d_status, p->sms, st) != cudaSuccess)
+      return 1;
+    ++p->launches;
+  }
   return 0;
 }
 
@@ -1188,6 +1234,8 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   std::vector<uint32_t> members, seg0;
   std::vector<FusedTask> tasks;
   build_fused(p->h_slabs, p->x_base, sms, fused_producers(16, nullptr), groups, members, tasks, seg0);
+  std::vector<uint32_t> parts(groups.size(), 0);
+  for (const FusedTask& t : tasks) ++parts[t.group];
   good = !tasks.empty() && seg0.size() >= 2 &&
          cudaMalloc(&p->d_fseg0, seg0.size() * sizeof(uint32_t)) == cudaSuccess &&
          cudaMemcpyAsync(p->d_fseg0, seg0.data(), seg0.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) ==
@@ -1201,6 +1249,9 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
                          st) == cudaSuccess &&
          cudaMemcpyAsync(p->d_fmembers, members.data(), members.size() * sizeof(uint32_t), cudaMemcpyHostToDevice,
                          st) == cudaSuccess &&
+         cudaMalloc(&p->d_fparts, groups.size() * sizeof(uint32_t)) == cudaSuccess &&
+         cudaMemcpyAsync(p->d_fparts, parts.data(), parts.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) ==
+             cudaSuccess &&
          cudaMalloc(&p->d_ftabs, groups.size() * fused_tables_bytes()) == cudaSuccess &&
          cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
          launch_fused_tables(p->d_fgroups, uint32_t(groups.size()), p->d_fmembers, p->d_slabs, d_payload, p->d_ftabs,
@@ -1216,6 +1267,8 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
     if (p->d_fgroups) cudaFree(p->d_fgroups);
     if (p->d_fmembers) cudaFree(p->d_fmembers);
     if (p->d_ftabs) cudaFree(p->d_ftabs);
+    if (p->d_fparts) cudaFree(p->d_fparts);
+    p->d_fparts = nullptr;
     p->d_ftabs = nullptr;
     p->d_ftasks = nullptr;
     p->d_fgroups = nullptr;
@@ -1223,6 +1276,7 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
     return;
   }
   p->n_fctas = uint32_t(seg0.size() - 1);
+  p->n_fgroups = uint32_t(groups.size());
   p->fused_ok = true;
 }
 

@@ -40,6 +40,7 @@
 
 #include "kernels.h"
 #include "lane_decode.cuh"
+#include "linear_epilogue.cuh"
 #include "tcgen05.cuh"
 #include "xksv_device.cuh"
 
@@ -78,6 +79,7 @@ struct FusedShared {
   uint32_t tmem_base;
   uint32_t qmask;  // accumulators D_q written by some MMA (a one-half-tile task writes two)
   int abort_flag;
+  bool last;  // linear layer: this segment completes its group
 };
 constexpr size_t kHdrBytes = (sizeof(FusedShared) + 127) & ~size_t(127);
 
@@ -126,6 +128,8 @@ __device__ __forceinline__ uint32_t kmajor_off(uint32_t r, uint32_t h) {
   return (r >> 3) * 256 + h * 128 + (r & 7) * 16;
 }
 
+// LIN: a linear layer's call (the tokens' rows as X^T, epilogue out).
+template <bool LIN>
 __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, uint32_t nprod) {
   extern __shared__ __align__(128) uint8_t smem[];
   FusedShared& S = *reinterpret_cast<FusedShared*>(smem);
@@ -186,7 +190,11 @@ __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, ui
       const __nv_bfloat16* xt = static_cast<const __nv_bfloat16*>(a.xt) + grp.xoff + 16 * uint64_t(k);
       for (uint32_t i = lane; i < 2 * npad; i += 32) {
         const uint32_t n = i >> 1, h = i & 1;
-        cp_async16(bring + slot * npad * 32 + kmajor_off(n, h), xt + uint64_t(n) * a.xt_ld + 8 * h);
+        if (LIN)  // tokens past the batch are zeros
+          cp_async16_zfill(smem_addr(bring + slot * npad * 32 + kmajor_off(n, h)),
+                           n < a.nb ? xt + uint64_t(n) * a.xt_ld + 8 * h : xt, n < a.nb ? 16u : 0u);
+        else
+          cp_async16(bring + slot * npad * 32 + kmajor_off(n, h), xt + uint64_t(n) * a.xt_ld + 8 * h);
       }
     };
     if (active && ha < hb) {
@@ -342,7 +350,13 @@ __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, ui
         for (uint32_t n0 = 0; n0 < npad; n0 += 16) {
           float v[16];
           tmem_ld16(tmem + ((warp * 32) << 16) + q * npad + n0, v);
-          if (mine) {
+          if (LIN) {
+            // [row 4q + r][token][slab]: a warp's adds are consecutive
+            float* z = a.y + ((uint64_t(task.group) * 16 + 4 * q + warp) * npad + n0) * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (mine && n0 + uint32_t(i) < a.nb) atomicAdd(z + 32 * i, v[i]);
+          } else if (mine) {
             float* yr = a.y + (row0 + 4 * q + warp) * uint64_t(a.ld);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -352,10 +366,25 @@ __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, ui
       }
     }
     // the accumulators, stage areas and tables are free for the next segment
+    if (LIN) __threadfence();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (S.abort_flag) break;
+    if (LIN) {
+      // the segment that completes its group takes the group's rows through
+      // the epilogue, consecutive threads consecutive rows of Y
+      if (threadIdx.x == 0) S.last = atomicAdd(a.arrived + task.group, 1u) + 1 == a.parts[task.group];
+      __syncthreads();
+      if (S.last) {
+        __threadfence();
+        for (uint32_t i = threadIdx.x; i < grp.nslabs * 16 * a.nb; i += blockDim.x) {
+          const uint32_t row = i % (grp.nslabs * 16), n = i / (grp.nslabs * 16), j = row >> 4, r = row & 15;
+          const float z = __ldcg(a.y + ((uint64_t(task.group) * 16 + r) * npad + n) * 32 + j);
+          epilogue_store(a.e, n, a.slabs[a.members[grp.m0 + j]].dst + r, z);
+        }
+      }
+    }
   }
   if (warp == P) {
     tc_fence_after();
@@ -384,6 +413,14 @@ __global__ void fused_prep_kernel(const float* __restrict__ x, uint32_t ld, uint
       y[(g.y_row0 + m) * uint64_t(ld) + n] = 0.f;
     }
   }
+}
+
+// Zeroes the linear layer's sums and counts ahead of the fused kernel, which
+// may start meanwhile.
+__global__ void fused_zero_kernel(uint4* p, uint64_t n) {
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  for (uint64_t i = blockIdx.x * uint64_t(blockDim.x) + threadIdx.x; i < n; i += uint64_t(gridDim.x) * blockDim.x)
+    p[i] = make_uint4(0, 0, 0, 0);
 }
 
 // One warp per group: lane j builds slab j's tables (the codes of its 256
@@ -462,9 +499,11 @@ cudaError_t launch_fused_check(const Slab* slabs, uint32_t n, const uint8_t* pay
   return cudaGetLastError();
 }
 
-cudaError_t launch_fused_gemm(const FusedArgs& args, uint32_t nctas, const float* x, uint64_t x_cols,
-                              const TcGroup* groups, uint32_t ngroups, cudaStream_t st) {
-  if (!nctas) return cudaSuccess;
+namespace {
+// The fused CTAs, launched to overlap the kernel before them (which they wait
+// for ahead of their first load of X).
+template <bool LIN>
+cudaError_t launch_fused_ctas(const FusedArgs& args, uint32_t nctas, cudaStream_t st) {
   size_t smem = 0;
   const uint32_t p = fused_producers(args.npad, &smem);
   if (!p) return cudaErrorInvalidValue;
@@ -475,17 +514,10 @@ cudaError_t launch_fused_gemm(const FusedArgs& args, uint32_t nctas, const float
   const uint64_t bit = dev < 64 ? (1ull << dev) : 0ull;
   if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
     const cudaError_t e =
-        cudaFuncSetAttribute(fused_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemLimit));
+        cudaFuncSetAttribute(fused_gemm_kernel<LIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemLimit));
     if (e != cudaSuccess) return e;
     if (bit) done.fetch_or(bit, std::memory_order_release);
   }
-  const uint64_t work = std::max<uint64_t>(x_cols * args.npad, uint64_t(ngroups) * 256);
-  const int pb = int(std::min<uint64_t>((work + 255) / 256, 1024));
-  fused_prep_kernel<<<pb, 256, 0, st>>>(x, args.ld, args.nb, x_cols, args.npad,
-                                        static_cast<__nv_bfloat16*>(const_cast<void*>(args.xt)), args.xt_ld, groups,
-                                        ngroups, args.y);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(nctas);
   cfg.blockDim = dim3((p + 1) * 32);
@@ -496,7 +528,30 @@ cudaError_t launch_fused_gemm(const FusedArgs& args, uint32_t nctas, const float
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fused_gemm_kernel, args, p);
+  return cudaLaunchKernelEx(&cfg, fused_gemm_kernel<LIN>, args, p);
+}
+}  // namespace
+
+cudaError_t launch_fused_gemm(const FusedArgs& args, uint32_t nctas, const float* x, uint64_t x_cols,
+                              const TcGroup* groups, uint32_t ngroups, cudaStream_t st) {
+  if (!nctas) return cudaSuccess;
+  if (!fused_producers(args.npad, nullptr)) return cudaErrorInvalidValue;
+  const uint64_t work = std::max<uint64_t>(x_cols * args.npad, uint64_t(ngroups) * 256);
+  const int pb = int(std::min<uint64_t>((work + 255) / 256, 1024));
+  fused_prep_kernel<<<pb, 256, 0, st>>>(x, args.ld, args.nb, x_cols, args.npad,
+                                        static_cast<__nv_bfloat16*>(const_cast<void*>(args.xt)), args.xt_ld, groups,
+                                        ngroups, args.y);
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_fused_ctas<false>(args, nctas, st);
+}
+
+cudaError_t launch_fused_linear(const FusedArgs& args, uint32_t nctas, uint32_t ngroups, cudaStream_t st) {
+  if (!nctas) return cudaSuccess;
+  if (!fused_producers(args.npad, nullptr)) return cudaErrorInvalidValue;
+  const uint64_t n = (uint64_t(ngroups) * (16 * args.npad * 32 + 1) * 4 + 15) / 16;
+  fused_zero_kernel<<<uint32_t(std::min<uint64_t>((n + 255) / 256, 2048)), 256, 0, st>>>(reinterpret_cast<uint4*>(args.y), n);
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_fused_ctas<true>(args, nctas, st);
 }
 
 }  // namespace xksv

@@ -57,6 +57,23 @@ struct alignas(16) GemvTabs {
 };
 static_assert(sizeof(GemvTabs) == 5920, "per-slab table bytes, as documented and counted by bench.py");
 
+// A run of consecutive rows of Y that a plan's slabs cover.
+struct RowRun {
+  uint64_t row0, rows;
+};
+// What a linear layer does with z[b, row] on its way into y (mirrors
+// xksv_linear_args; null pointers are absent).
+struct Epilogue {
+  void* y;
+  const void* bias;
+  const void* mul;
+  const void* residual;
+  uint64_t y_stride, mul_stride, residual_stride;
+  uint32_t act;
+  bool y_f32, bias_f32, mul_f32, residual_f32;
+  bool vec;  // eight columns from a multiple of 8 are 16-byte aligned in every operand
+};
+
 struct GemvArgs {
   const GemvItem* items;
   uint32_t nitems;
@@ -83,9 +100,16 @@ struct GemvArgs {
   uint64_t peer_row0, peer_rows;  // this rank's block of the gathered Y
   uint32_t* done;          // grid completion counter (zero between launches)
   uint32_t* epoch;         // this rank's completed fused calls
+  // linear layer: X in BF16 [nb, xb_stride] in place of x, rows through the
+  // epilogue in place of y
+  const void* xb;
+  uint64_t xb_stride;
+  Epilogue e;
 };
 // Indexed fused GEMV/GEMM (nb <= 4) over 16-row serial-codec slabs.
 cudaError_t launch_serial_tile_gemm(const GemvArgs& args, cudaStream_t st);
+// The same for a linear layer of nb <= 4 tokens (xb, e).
+cudaError_t launch_serial_tile_linear(const GemvArgs& args, cudaStream_t st);
 // Fused TP: waits (bounded) until every rank's flag reaches this rank's epoch.
 cudaError_t launch_tp_wait(const uint32_t* flags, uint32_t world, const uint32_t* epoch, int* status,
                            cudaStream_t st);
@@ -151,6 +175,13 @@ struct FusedArgs {
   float* y;              // Y at batch column b0 (row stride ld), rows zeroed
   uint32_t ld, nb, npad;
   int* status;
+  // linear layer: X^T is the tokens' rows themselves (nb of them), y the
+  // groups' sums [group][16][npad][32] and `arrived` their counts of finished
+  // segments, both zeroed; the segment that completes a group (parts[group])
+  // takes its rows through the epilogue
+  uint32_t* arrived;
+  const uint32_t* parts;
+  Epilogue e;
 };
 // Producer warps and dynamic shared memory for a batch pass of npad columns
 // (16 <= npad <= 128, a multiple of 16); 0 producers when it does not fit.
@@ -170,22 +201,6 @@ cudaError_t launch_fused_check(const Slab* slabs, uint32_t n, const uint8_t* pay
 cudaError_t launch_fused_gemm(const FusedArgs& args, uint32_t nctas, const float* x, uint64_t x_cols,
                               const TcGroup* groups, uint32_t ngroups, cudaStream_t st);
 
-// A run of consecutive rows of Y that a plan's slabs cover.
-struct RowRun {
-  uint64_t row0, rows;
-};
-// What a linear layer does with z[b, row] on its way into y (mirrors
-// xksv_linear_args; null pointers are absent).
-struct Epilogue {
-  void* y;
-  const void* bias;
-  const void* mul;
-  const void* residual;
-  uint64_t y_stride, mul_stride, residual_stride;
-  uint32_t act;
-  bool y_f32, bias_f32, mul_f32, residual_f32;
-  bool vec;  // eight columns from a multiple of 8 are 16-byte aligned in every operand
-};
 // x BF16 [batch, cols] (rows `stride` elements apart) to FP32 [cols, batch].
 cudaError_t launch_linear_x(const void* x, uint64_t stride, uint64_t batch, uint64_t cols, float* xt, cudaStream_t st);
 // z FP32 [Y rows, batch] through the epilogue into y, for the rows of `runs`
@@ -209,6 +224,10 @@ cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, cons
 bool linear_rows_direct(const void* x, uint64_t stride, uint64_t xoff);
 cudaError_t launch_linear_rows(const void* x, uint64_t stride, uint64_t batch, uint64_t cols, uint64_t pitch, void* out,
                                cudaStream_t st);
+
+// The same for a linear layer: zeroes args.y and args.arrived (`ngroups` groups
+// of the fused schedule, adjacent: sums first), then the fused CTAs.
+cudaError_t launch_fused_linear(const FusedArgs& args, uint32_t nctas, uint32_t ngroups, cudaStream_t st);
 
 // SHA-256 (FIPS 180-4) of n ranges {offset, length} (device array of 2n u64)
 // of d_base; 32-byte big-endian digests to d_digests.

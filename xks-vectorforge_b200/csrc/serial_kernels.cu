@@ -31,6 +31,7 @@
 #include <atomic>
 
 #include "kernels.h"
+#include "linear_epilogue.cuh"
 #include "tcgen05.cuh"
 #include "xksv_device.cuh"
 
@@ -757,6 +758,14 @@ __device__ __forceinline__ void store_y(const GemvArgs& a, uint64_t row, uint32_
   y[row * a.ld + b] = v;
 }
 
+template <bool LIN>
+__device__ __forceinline__ void store_row(const GemvArgs& a, uint64_t row, uint32_t b, float v) {
+  if (LIN)
+    epilogue_store(a.e, b, row, v);
+  else
+    store_y(a, row, b, v);
+}
+
 // acc[b] += w(e_k, byte k of sw) * x[4q + k][b] for the block's four codes;
 // xr4 holds the block's x values, column-major in k then b (NB per column).
 template <int NB>
@@ -774,7 +783,8 @@ __device__ __forceinline__ void fma4(float* acc, uint32_t e0, uint32_t e1, uint3
 }
 
 // NB == 0: decode mode (BF16 tile rows to a.out + slab dst); NB >= 1: GEMV/GEMM.
-template <int NB, int SPLIT>
+// LIN: a linear layer's call (BF16 tokens in, epilogue out).
+template <int NB, int SPLIT, bool LIN = false>
 __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) serial_tile_gemv_kernel(GemvArgs a) {
   static_assert(SPLIT == 1 || (SPLIT == 2 && NB <= 1), "two threads per tile at batch <= 1");
   constexpr int NT = GT * SPLIT;   // threads
@@ -878,6 +888,28 @@ __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) seri
     float xr[NB > 0 ? 16 * NB : 1];
     if (NB == 0) {
       // decode mode: no x
+    } else if (LIN) {
+      const uint16_t* xb = static_cast<const uint16_t*>(a.xb) + sd.xoff + uint64_t(tile) * 16;
+      const bool words = ((reinterpret_cast<uintptr_t>(xb) | a.xb_stride * 2) & 15) == 0;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        if (uint32_t(b) >= a.nb) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) xr[c * NB + b] = 0.f;
+        } else if (words) {
+          const uint4* q = reinterpret_cast<const uint4*>(xb + b * a.xb_stride);
+          const uint4 u = __ldg(q), v = __ldg(q + 1);
+          const uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            xr[2 * c * NB + b] = __uint_as_float(w[c] << 16);
+            xr[(2 * c + 1) * NB + b] = __uint_as_float(w[c] & 0xffff0000u);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 16; ++c) xr[c * NB + b] = __uint_as_float(uint32_t(__ldg(xb + b * a.xb_stride + c)) << 16);
+        }
+      }
     } else if (NB == 1 && a.ld == 1 && (reinterpret_cast<uintptr_t>(xs) & 15) == 0) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -1004,7 +1036,7 @@ __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) seri
     if (comb)
       for (int w = 0; w < NT / 32; ++w) v += S.red[rr][w][bb];
     if (it.nitems == 1) {
-      if (comb) store_y(a, sd.dst + rr, bb, v);
+      if (comb) store_row<LIN>(a, sd.dst + rr, bb, v);
     } else {
       if (comb) a.partials[uint64_t(ii) * 16 * GNB + rr * GNB + bb] = v;
       __threadfence();
@@ -1017,14 +1049,14 @@ __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) seri
           float sum = 0.f;
           for (uint32_t j = 0; j < it.nitems; ++j)
             sum += __ldcg(&a.partials[uint64_t(it.first + j) * 16 * GNB + rr * GNB + bb]);
-          store_y(a, sd.dst + rr, bb, sum);
+          store_row<LIN>(a, sd.dst + rr, bb, sum);
         }
         if (t == 0) a.counters[it.slab] = 0;
       }
     }
     __syncthreads();
   }
-  if (NB > 0 && a.npeers) {
+  if (NB > 0 && !LIN && a.npeers) {
     // fused all-gather: the last CTA to finish copies this rank's block of Y
     // into every other rank's gathered buffer (peer stores over NVLink), makes
     // them visible system-wide, and publishes the new epoch to every rank
@@ -1092,6 +1124,10 @@ void serial_set_attr() {
   cudaFuncSetAttribute(serial_tile_gemv_kernel<1, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
   cudaFuncSetAttribute(serial_tile_gemv_kernel<2, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
   cudaFuncSetAttribute(serial_tile_gemv_kernel<4, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
+  cudaFuncSetAttribute(serial_tile_gemv_kernel<1, 1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
+  cudaFuncSetAttribute(serial_tile_gemv_kernel<1, 2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
+  cudaFuncSetAttribute(serial_tile_gemv_kernel<2, 1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
+  cudaFuncSetAttribute(serial_tile_gemv_kernel<4, 1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
   if (bit) done.fetch_or(bit, std::memory_order_release);
 }
 
@@ -1133,7 +1169,7 @@ cudaError_t launch_serial_index(const Slab* slabs, uint32_t n, const uint8_t* pa
 // The indexed kernel is launched with programmatic stream serialisation: its
 // CTAs may start (table build, bit staging) while the stream's previous
 // kernel finishes, and wait for it before touching shared data.
-template <int NB, int SPLIT>
+template <int NB, int SPLIT, bool LIN = false>
 cudaError_t launch_tile_kernel(const GemvArgs& args, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(args.nitems);
@@ -1145,7 +1181,7 @@ cudaError_t launch_tile_kernel(const GemvArgs& args, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, serial_tile_gemv_kernel<NB, SPLIT>, args);
+  return cudaLaunchKernelEx(&cfg, serial_tile_gemv_kernel<NB, SPLIT, LIN>, args);
 }
 
 // Two threads per tile when the items fill under one wave of 256-thread CTAs
@@ -1171,6 +1207,16 @@ cudaError_t launch_serial_tile_gemm(const GemvArgs& args, cudaStream_t st) {
     return tile_split(args.nitems) ? launch_tile_kernel<1, 2>(args, st) : launch_tile_kernel<1, 1>(args, st);
   if (args.nb == 2) return launch_tile_kernel<2, 1>(args, st);
   return launch_tile_kernel<4, 1>(args, st);
+}
+
+cudaError_t launch_serial_tile_linear(const GemvArgs& args, cudaStream_t st) {
+  if (!args.nitems) return cudaSuccess;
+  if (args.nb < 1 || args.nb > uint32_t(GNB) || !args.gtabs || !args.tmid) return cudaErrorInvalidValue;
+  serial_set_attr();
+  if (args.nb == 1)
+    return tile_split(args.nitems) ? launch_tile_kernel<1, 2, true>(args, st) : launch_tile_kernel<1, 1, true>(args, st);
+  if (args.nb == 2) return launch_tile_kernel<2, 1, true>(args, st);
+  return launch_tile_kernel<4, 1, true>(args, st);
 }
 
 cudaError_t launch_serial_tile_decode(const GemvArgs& args, cudaStream_t st) {
