@@ -220,8 +220,8 @@ struct xksv_plan {
   xksv::FusedGroup* d_fgroups = nullptr;
   uint32_t* d_fmembers = nullptr;
   void* d_ftabs = nullptr;  // per group: its lane tables, built with the index
-  uint32_t n_fgroups = 0;
-  uint32_t* d_fparts = nullptr;  // per group: the segments its rows are summed from
+  uint32_t n_fgroups = 0, n_fsegs = 0;
+  uint32_t* d_fgsegs = nullptr;  // group g's segments: entries [e[g], e[g + 1]) behind the n_fgroups + 1 first
   uint64_t* d_hash_ranges = nullptr;  // per slab in creation order: {dst, decoded bytes}
   // linear layer (xksv_plan_linear): the runs of Y rows the slabs cover; off
   // when two slabs cover one row or a slab has no rows and columns
@@ -250,8 +250,8 @@ void free_index(xksv_plan* p) {
   if (p->d_fgroups) cudaFree(p->d_fgroups);
   if (p->d_fmembers) cudaFree(p->d_fmembers);
   if (p->d_ftabs) cudaFree(p->d_ftabs);
-  if (p->d_fparts) cudaFree(p->d_fparts);
-  p->d_fparts = nullptr;
+  if (p->d_fgsegs) cudaFree(p->d_fgsegs);
+  p->d_fgsegs = nullptr;
   p->d_ftabs = nullptr;
   p->d_fseg0 = nullptr;
   p->d_ftasks = nullptr;
@@ -1009,7 +1009,7 @@ LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload
     s.route = Route::Tile;
   } else if (payload && gemm_fused(p, payload, batch)) {
     s.route = Route::Fused;
-    s.z = c.take(uint64_t(p->n_fgroups) * (16 * ((batch + 15) / 16 * 16) * 32 + 1) * 4 + 16);
+    s.z = c.take(uint64_t(p->n_fsegs) * 16 * ((batch + 15) / 16 * 16) * 32 * sizeof(float));
     s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
   } else if (p->tc_ok && batch >= 4) {
     s.route = Route::Gemm;
@@ -1131,11 +1131,10 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
     f.xt = x0;
     f.xt_ld = pitch;
     f.y = reinterpret_cast<float*>(ws + sp.z);
-    f.arrived = reinterpret_cast<uint32_t*>(f.y + uint64_t(p->n_fgroups) * 16 * f.npad * 32);
-    f.parts = p->d_fparts;
-    f.e = ep;
     p->launches += 2;
-    return launch_fused_linear(f, p->n_fctas, p->n_fgroups, st) == cudaSuccess ? 0 : 1;
+    return launch_fused_linear(f, p->n_fctas, p->n_fgroups, p->d_fgsegs, p->d_fgsegs + p->n_fgroups + 1, ep, st) == cudaSuccess
+               ? 0
+               : 1;
   }
   // decode, then one tensor-core product with its epilogue per weight
   if (decode_scratch(p, pay, ws + sp.scratch, st) != cudaSuccess) return 1;
@@ -1234,8 +1233,14 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   std::vector<uint32_t> members, seg0;
   std::vector<FusedTask> tasks;
   build_fused(p->h_slabs, p->x_base, sms, fused_producers(16, nullptr), groups, members, tasks, seg0);
-  std::vector<uint32_t> parts(groups.size(), 0);
-  for (const FusedTask& t : tasks) ++parts[t.group];
+  std::vector<uint32_t> gsegs(groups.size() + 1, 0);
+  for (const FusedTask& t : tasks) ++gsegs[t.group + 1];
+  for (size_t g = 0; g < groups.size(); ++g) gsegs[g + 1] += gsegs[g];
+  gsegs.resize(groups.size() + 1 + tasks.size());
+  {
+    std::vector<uint32_t> at(gsegs.begin(), gsegs.begin() + groups.size());
+    for (size_t i = 0; i < tasks.size(); ++i) gsegs[groups.size() + 1 + at[tasks[i].group]++] = uint32_t(i);
+  }
   good = !tasks.empty() && seg0.size() >= 2 &&
          cudaMalloc(&p->d_fseg0, seg0.size() * sizeof(uint32_t)) == cudaSuccess &&
          cudaMemcpyAsync(p->d_fseg0, seg0.data(), seg0.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) ==
@@ -1249,8 +1254,8 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
                          st) == cudaSuccess &&
          cudaMemcpyAsync(p->d_fmembers, members.data(), members.size() * sizeof(uint32_t), cudaMemcpyHostToDevice,
                          st) == cudaSuccess &&
-         cudaMalloc(&p->d_fparts, groups.size() * sizeof(uint32_t)) == cudaSuccess &&
-         cudaMemcpyAsync(p->d_fparts, parts.data(), parts.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) ==
+         cudaMalloc(&p->d_fgsegs, gsegs.size() * sizeof(uint32_t)) == cudaSuccess &&
+         cudaMemcpyAsync(p->d_fgsegs, gsegs.data(), gsegs.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) ==
              cudaSuccess &&
          cudaMalloc(&p->d_ftabs, groups.size() * fused_tables_bytes()) == cudaSuccess &&
          cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
@@ -1267,8 +1272,8 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
     if (p->d_fgroups) cudaFree(p->d_fgroups);
     if (p->d_fmembers) cudaFree(p->d_fmembers);
     if (p->d_ftabs) cudaFree(p->d_ftabs);
-    if (p->d_fparts) cudaFree(p->d_fparts);
-    p->d_fparts = nullptr;
+    if (p->d_fgsegs) cudaFree(p->d_fgsegs);
+    p->d_fgsegs = nullptr;
     p->d_ftabs = nullptr;
     p->d_ftasks = nullptr;
     p->d_fgroups = nullptr;
@@ -1277,6 +1282,7 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   }
   p->n_fctas = uint32_t(seg0.size() - 1);
   p->n_fgroups = uint32_t(groups.size());
+  p->n_fsegs = uint32_t(tasks.size());
   p->fused_ok = true;
 }
 

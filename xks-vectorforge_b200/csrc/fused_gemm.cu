@@ -79,7 +79,6 @@ struct FusedShared {
   uint32_t tmem_base;
   uint32_t qmask;  // accumulators D_q written by some MMA (a one-half-tile task writes two)
   int abort_flag;
-  bool last;  // linear layer: this segment completes its group
 };
 constexpr size_t kHdrBytes = (sizeof(FusedShared) + 127) & ~size_t(127);
 
@@ -128,7 +127,8 @@ __device__ __forceinline__ uint32_t kmajor_off(uint32_t r, uint32_t h) {
   return (r >> 3) * 256 + h * 128 + (r & 7) * 16;
 }
 
-// LIN: a linear layer's call (the tokens' rows as X^T, epilogue out).
+// LIN: a linear layer's call (the tokens' rows as X^T; every segment's sums
+// kept apart for fused_out_kernel).
 template <bool LIN>
 __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, uint32_t nprod) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -190,11 +190,9 @@ __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, ui
       const __nv_bfloat16* xt = static_cast<const __nv_bfloat16*>(a.xt) + grp.xoff + 16 * uint64_t(k);
       for (uint32_t i = lane; i < 2 * npad; i += 32) {
         const uint32_t n = i >> 1, h = i & 1;
-        if (LIN)  // tokens past the batch are zeros
-          cp_async16_zfill(smem_addr(bring + slot * npad * 32 + kmajor_off(n, h)),
-                           n < a.nb ? xt + uint64_t(n) * a.xt_ld + 8 * h : xt, n < a.nb ? 16u : 0u);
-        else
-          cp_async16(bring + slot * npad * 32 + kmajor_off(n, h), xt + uint64_t(n) * a.xt_ld + 8 * h);
+        // (a linear layer's columns past its tokens repeat the last one: nothing reads their sums)
+        const uint32_t src = LIN ? min(n, a.nb - 1) : n;
+        cp_async16(bring + slot * npad * 32 + kmajor_off(n, h), xt + uint64_t(src) * a.xt_ld + 8 * h);
       }
     };
     if (active && ha < hb) {
@@ -346,16 +344,21 @@ __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, ui
       const bool mine = lane < grp.nslabs;
       const uint64_t row0 = mine ? a.slabs[a.members[grp.m0 + lane]].dst : 0;
       for (uint32_t q = 0; q < 4; ++q) {
-        if (!((S.qmask >> q) & 1)) continue;  // no MMA wrote D_q: nothing to add
+        const bool written = (S.qmask >> q) & 1;
+        if (!LIN && !written) continue;  // no MMA wrote D_q: nothing to add
         for (uint32_t n0 = 0; n0 < npad; n0 += 16) {
           float v[16];
-          tmem_ld16(tmem + ((warp * 32) << 16) + q * npad + n0, v);
+          if (written)
+            tmem_ld16(tmem + ((warp * 32) << 16) + q * npad + n0, v);
+          else
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = 0.f;
           if (LIN) {
-            // [row 4q + r][token][slab]: a warp's adds are consecutive
-            float* z = a.y + ((uint64_t(task.group) * 16 + 4 * q + warp) * npad + n0) * 32 + lane;
+            // the segment's own sums [row 4q + r][token][slab]: a warp's are consecutive
+            float* z = a.y + ((uint64_t(sg) * 16 + 4 * q + warp) * npad + n0) * 32 + lane;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (mine && n0 + uint32_t(i) < a.nb) atomicAdd(z + 32 * i, v[i]);
+              if (mine && n0 + uint32_t(i) < a.nb) z[32 * i] = v[i];
           } else if (mine) {
             float* yr = a.y + (row0 + 4 * q + warp) * uint64_t(a.ld);
 #pragma unroll
@@ -366,25 +369,10 @@ __global__ void __launch_bounds__(FTHREADS, 1) fused_gemm_kernel(FusedArgs a, ui
       }
     }
     // the accumulators, stage areas and tables are free for the next segment
-    if (LIN) __threadfence();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (S.abort_flag) break;
-    if (LIN) {
-      // the segment that completes its group takes the group's rows through
-      // the epilogue, consecutive threads consecutive rows of Y
-      if (threadIdx.x == 0) S.last = atomicAdd(a.arrived + task.group, 1u) + 1 == a.parts[task.group];
-      __syncthreads();
-      if (S.last) {
-        __threadfence();
-        for (uint32_t i = threadIdx.x; i < grp.nslabs * 16 * a.nb; i += blockDim.x) {
-          const uint32_t row = i % (grp.nslabs * 16), n = i / (grp.nslabs * 16), j = row >> 4, r = row & 15;
-          const float z = __ldcg(a.y + ((uint64_t(task.group) * 16 + r) * npad + n) * 32 + j);
-          epilogue_store(a.e, n, a.slabs[a.members[grp.m0 + j]].dst + r, z);
-        }
-      }
-    }
   }
   if (warp == P) {
     tc_fence_after();
@@ -415,12 +403,43 @@ __global__ void fused_prep_kernel(const float* __restrict__ x, uint32_t ld, uint
   }
 }
 
-// Zeroes the linear layer's sums and counts ahead of the fused kernel, which
-// may start meanwhile.
-__global__ void fused_zero_kernel(uint4* p, uint64_t n) {
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
-  for (uint64_t i = blockIdx.x * uint64_t(blockDim.x) + threadIdx.x; i < n; i += uint64_t(gridDim.x) * blockDim.x)
-    p[i] = make_uint4(0, 0, 0, 0);
+// The linear layer's rows: CTA (g, s, n) takes eight slabs of group g and
+// sixteen tokens, adds the sums that the group's segments left (in their
+// order) and writes y through the epilogue.  The sums are read along the
+// slabs and written along the rows, by way of shared memory.
+constexpr int OT = 256, OJ = 8;
+__global__ void __launch_bounds__(OT) fused_out_kernel(FusedArgs a, const uint32_t* __restrict__ gseg0,
+                                                       const uint32_t* __restrict__ gsegs, Epilogue e) {
+  __shared__ float T[16][OJ * 17];
+  const FusedGroup g = a.groups[blockIdx.x];
+  const uint32_t j0 = blockIdx.y * OJ, n0 = blockIdx.z * 16, t = threadIdx.x;
+  if (j0 >= g.nslabs) return;
+  // reads: slab j0 + t % 8, its row t / 8 % 16, tokens t / 128 + 2 k
+  // writes: the row of slab j0 + t / 16 % 8, tokens t / 128 + 2 k
+  const uint32_t rj = t & 7, rr = (t >> 3) & 15, wj = (t >> 4) & 7, wr = t & 15, nt = t >> 7;
+  const bool write = j0 + wj < g.nslabs;
+  const uint64_t row = write ? a.slabs[a.members[g.m0 + j0 + wj]].dst + wr : 0;
+  const uint32_t s0 = gseg0[blockIdx.x], s1 = gseg0[blockIdx.x + 1];
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  EpilogueOps ops[8];
+  float z[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    z[k] = 0.f;
+    if (write && n0 + nt + 2 * k < a.nb) ops[k] = epilogue_read(e, n0 + nt + 2 * k, row);
+  }
+  for (uint32_t s = s0; s < s1; ++s) {
+    const float* src = a.y + ((uint64_t(gsegs[s]) * 16 + rr) * a.npad + n0 + nt) * 32 + j0 + rj;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (j0 + rj < g.nslabs && n0 + nt + 2 * k < a.nb) z[k] += __ldcg(src + 64 * k);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) T[nt + 2 * k][rj * 17 + rr] = z[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (write && n0 + nt + 2 * k < a.nb) epilogue_write(e, n0 + nt + 2 * k, row, T[nt + 2 * k][wj * 17 + wr], ops[k]);
 }
 
 // One warp per group: lane j builds slab j's tables (the codes of its 256
@@ -545,13 +564,21 @@ cudaError_t launch_fused_gemm(const FusedArgs& args, uint32_t nctas, const float
   return e != cudaSuccess ? e : launch_fused_ctas<false>(args, nctas, st);
 }
 
-cudaError_t launch_fused_linear(const FusedArgs& args, uint32_t nctas, uint32_t ngroups, cudaStream_t st) {
+cudaError_t launch_fused_linear(const FusedArgs& args, uint32_t nctas, uint32_t ngroups, const uint32_t* gseg0,
+                                const uint32_t* gsegs, const Epilogue& e, cudaStream_t st) {
   if (!nctas) return cudaSuccess;
-  if (!fused_producers(args.npad, nullptr)) return cudaErrorInvalidValue;
-  const uint64_t n = (uint64_t(ngroups) * (16 * args.npad * 32 + 1) * 4 + 15) / 16;
-  fused_zero_kernel<<<uint32_t(std::min<uint64_t>((n + 255) / 256, 2048)), 256, 0, st>>>(reinterpret_cast<uint4*>(args.y), n);
-  const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_fused_ctas<true>(args, nctas, st);
+  const cudaError_t err = launch_fused_ctas<true>(args, nctas, st);
+  if (err != cudaSuccess) return err;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ngroups, 32 / OJ, args.npad / 16);
+  cfg.blockDim = dim3(OT);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fused_out_kernel, args, gseg0, gsegs, e);
 }
 
 }  // namespace xksv

@@ -176,12 +176,7 @@ struct FusedArgs {
   uint32_t ld, nb, npad;
   int* status;
   // linear layer: X^T is the tokens' rows themselves (nb of them), y the
-  // groups' sums [group][16][npad][32] and `arrived` their counts of finished
-  // segments, both zeroed; the segment that completes a group (parts[group])
-  // takes its rows through the epilogue
-  uint32_t* arrived;
-  const uint32_t* parts;
-  Epilogue e;
+  // segments' sums [segment][16][npad][32]
 };
 // Producer warps and dynamic shared memory for a batch pass of npad columns
 // (16 <= npad <= 128, a multiple of 16); 0 producers when it does not fit.
@@ -225,9 +220,10 @@ bool linear_rows_direct(const void* x, uint64_t stride, uint64_t xoff);
 cudaError_t launch_linear_rows(const void* x, uint64_t stride, uint64_t batch, uint64_t cols, uint64_t pitch, void* out,
                                cudaStream_t st);
 
-// The same for a linear layer: zeroes args.y and args.arrived (`ngroups` groups
-// of the fused schedule, adjacent: sums first), then the fused CTAs.
-cudaError_t launch_fused_linear(const FusedArgs& args, uint32_t nctas, uint32_t ngroups, cudaStream_t st);
+// The same for a linear layer: the fused CTAs, then the rows of each group
+// (segments gsegs[gseg0[g]] .. gsegs[gseg0[g + 1])) through the epilogue.
+cudaError_t launch_fused_linear(const FusedArgs& args, uint32_t nctas, uint32_t ngroups, const uint32_t* gseg0,
+                                const uint32_t* gsegs, const Epilogue& e, cudaStream_t st);
 
 // SHA-256 (FIPS 180-4) of n ranges {offset, length} (device array of 2n u64)
 // of d_base; 32-byte big-endian digests to d_digests.

@@ -21,15 +21,29 @@ __device__ __forceinline__ float load_elem(const void* p, uint64_t i, bool f32) 
   return f32 ? static_cast<const float*>(p)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-__device__ __forceinline__ void epilogue_store(const Epilogue& e, uint64_t b, uint64_t row, float z) {
-  if (e.bias) z += load_elem(e.bias, row, e.bias_f32);
+// The epilogue's operands at token b and a row, apart from its arithmetic: a
+// caller with several elements reads all of them first (y may be mul or
+// residual, so that no read moves past a write by itself).
+struct EpilogueOps {
+  float bias, mul, residual;
+};
+__device__ __forceinline__ EpilogueOps epilogue_read(const Epilogue& e, uint64_t b, uint64_t row) {
+  return EpilogueOps{e.bias ? load_elem(e.bias, row, e.bias_f32) : 0.f,
+                     e.mul ? load_elem(e.mul, b * e.mul_stride + row, e.mul_f32) : 1.f,
+                     e.residual ? load_elem(e.residual, b * e.residual_stride + row, e.residual_f32) : 0.f};
+}
+__device__ __forceinline__ void epilogue_write(const Epilogue& e, uint64_t b, uint64_t row, float z, const EpilogueOps& o) {
+  if (e.bias) z += o.bias;
   z = act_apply(e.act, z);
-  if (e.mul) z *= load_elem(e.mul, b * e.mul_stride + row, e.mul_f32);
-  if (e.residual) z += load_elem(e.residual, b * e.residual_stride + row, e.residual_f32);
+  if (e.mul) z *= o.mul;
+  if (e.residual) z += o.residual;
   if (e.y_f32)
     static_cast<float*>(e.y)[b * e.y_stride + row] = z;
   else
     static_cast<__nv_bfloat16*>(e.y)[b * e.y_stride + row] = __float2bfloat16_rn(z);
+}
+__device__ __forceinline__ void epilogue_store(const Epilogue& e, uint64_t b, uint64_t row, float z) {
+  epilogue_write(e, b, row, z, epilogue_read(e, b, row));
 }
 
 // Eight elements at index i of a BF16 or FP32 array, 16-byte aligned there.
