@@ -153,7 +153,8 @@ int run_single(Kind kind, const void* input, size_t size, uint64_t rows, uint64_
   if (!gemm) {
     e = kind == Kind::Serial
             ? launch_serial_decode(c->d_slab, 1, payload, static_cast<uint8_t*>(output), c->d_status, 1, st)
-            : launch_parallel_decode(c->d_slab, 1, payload, static_cast<uint8_t*>(output), c->d_status, 1, st);
+            : launch_parallel_decode(c->d_slab, 1, payload, static_cast<uint8_t*>(output), c->d_status, 1, st,
+                                     parallel_whole(rows, cols));
   } else {
     float* y = static_cast<float*>(output);
     for (size_t b0 = 0; b0 < batch && e == cudaSuccess; b0 += 8) {
@@ -177,6 +178,7 @@ struct xksv_plan {
   xksv::Slab* d_slabs = nullptr;  // [serial | parallel | raw]
   uint32_t n_ser = 0, n_par = 0, n_raw = 0;
   bool raw_gemm_ok = true;
+  bool par_whole = true;  // every parallel slab lies in whole rows (parallel_whole)
   bool odd_dst = false;  // a coded slab with an odd byte offset: decode refused
   // buffer extents the slab table needs, checked against the sizes every call
   // is given before anything is launched: payload bytes (max src end),
@@ -568,6 +570,7 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
   p->n_par = uint32_t(par.size());
   p->n_raw = uint32_t(raw.size());
   p->raw_gemm_ok = raw_gemm_ok;
+  for (const Slab& s : par) p->par_whole = p->par_whole && parallel_whole(s.rows, s.cols);
   p->odd_dst = odd_dst;
   p->need_payload = need_payload;
   p->need_out = need_out;
@@ -708,7 +711,7 @@ int xksv_plan_decode(const xksv_plan* pc, const void* d_payload, size_t payload_
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_par) {
-    e = launch_parallel_decode(p->d_slabs + p->n_ser, p->n_par, pay, out, p->d_status, p->grid_par, st);
+    e = launch_parallel_decode(p->d_slabs + p->n_ser, p->n_par, pay, out, p->d_status, p->grid_par, st, p->par_whole);
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_raw) {
@@ -793,7 +796,8 @@ int xksv_plan_decode_host(const xksv_plan* pc, const void* h_payload, size_t pay
         ++p->launches;
       }
     if (e == cudaSuccess && upto[2] > done[2]) {
-      e = launch_parallel_decode(p->d_slabs + done[2], upto[2] - done[2], pay, out, p->d_status, p->grid_par, st);
+      e = launch_parallel_decode(p->d_slabs + done[2], upto[2] - done[2], pay, out, p->d_status, p->grid_par, st,
+                                 p->par_whole);
       ++p->launches;
     }
     if (e == cudaSuccess && upto[3] > done[3]) {
@@ -829,7 +833,7 @@ cudaError_t decode_scratch(xksv_plan* p, const uint8_t* pay, uint8_t* scratch, c
   }
   if (e == cudaSuccess && p->n_par) {
     e = launch_parallel_decode(p->d_tc_slabs + p->n_ser, p->n_par, pay, scratch, p->d_status,
-                               p->grid_par, st);
+                               p->grid_par, st, p->par_whole);
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_raw) {

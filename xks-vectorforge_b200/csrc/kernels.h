@@ -14,8 +14,11 @@ size_t serial_smem_bytes();
 // Decode slabs[0..n) from payload into out (+ slab.dst bytes each).
 struct GemvTabs;
 
+// whole: every slab has 16 rows and a multiple of 32 columns (parallel_whole).
 cudaError_t launch_parallel_decode(const Slab* slabs, uint32_t n, const uint8_t* payload,
-                                   uint8_t* out, int* status, int grid, cudaStream_t st);
+                                   uint8_t* out, int* status, int grid, cudaStream_t st, bool whole);
+// The slab's 32 substreams start at whole 16-word rows of its tiles.
+inline bool parallel_whole(uint64_t rows, uint64_t cols) { return rows == 16 && cols % 32 == 0; }
 cudaError_t launch_serial_decode(const Slab* slabs, uint32_t n, const uint8_t* payload,
                                  uint8_t* out, int* status, int grid, cudaStream_t st);
 cudaError_t launch_raw_decode(const Slab* slabs, uint32_t n, const uint8_t* payload, uint8_t* out,

@@ -115,14 +115,108 @@ __device__ __forceinline__ void emit_one(const Out& o, uint32_t p, uint32_t word
   }
 }
 
+// A slab's elements in packed order: 16-column tiles (the last one w wide) of
+// the slab's rows (at most 16), row-major inside.
+struct Walk {
+  uint32_t rows, cols, t0, w, r, c;
+  __device__ __forceinline__ Walk(uint32_t p, uint32_t rows_, uint32_t cols_) : rows(rows_), cols(cols_) {
+    const uint32_t t = p / (16 * rows), local = p - t * 16 * rows;
+    t0 = 16 * t;
+    w = cols - t0 < 16 ? cols - t0 : 16;
+    r = local / w;
+    c = local - r * w;
+  }
+  __device__ __forceinline__ uint32_t col() const { return t0 + c; }
+  __device__ __forceinline__ void next() {
+    if (++c < w) return;
+    c = 0;
+    if (++r < rows) return;
+    r = 0;
+    t0 += 16;
+    w = cols - t0 < 16 ? cols - t0 : 16;
+  }
+};
+
+// A substream whose elements do not lie in whole 16-word rows (slabs of
+// other shapes, or a start inside a row): sixteen codes at a time like the
+// whole rows, their places stepped along instead of divided out (16 x 1848
+// slabs, 128 of them: 614 us one code at a time, 130 us so).  Out of line, so that the
+// whole-row loop keeps its registers.
+template <int MODE>
+__device__ __noinline__ bool decode_ragged(const Seg s, WarpTabs& W, int lane, const ldec::Code lc, ldec::Stream b, const Out o) {
+  bool bad = false;
+  Walk at(s.start, o.rows, o.cols);
+  auto emit = [&](uint32_t e, uint32_t sm) {
+    const uint32_t word = merge1(e, sm);
+    if (MODE == 0) {
+      o.out[size_t(at.r) * o.cols + at.col()] = uint16_t(word);
+    } else {
+      const float w = __uint_as_float(word << 16);
+      for (uint32_t k = 0; k < o.nb; ++k)
+        atomicAdd(&o.ysm[at.r * PMAXB + k], w * __ldg(&o.x[uint64_t(at.col()) * o.ld + k]));
+    }
+    at.next();
+  };
+  uint32_t i = 0;
+  // sign/mantissa bytes as aligned words (five hold any sixteen bytes; the
+  // exponent bits behind them belong to the substream too)
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(s.sm) & ~uintptr_t(3));
+  const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(s.sm) & 3) * 8;
+  for (; i + 16 <= s.count && i + 20 <= s.count + s.ebytes; i += 16) {
+    uint32_t w[5], e[16];
+#pragma unroll
+    for (int k = 0; k < 5; ++k) w[k] = __ldg(words + i / 4 + k);
+    b.maintain(W.ring, lane);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      ldec::dec4<PCfg>(b, W.ring, W.t, lane, lc, bad, e[4 * k], e[4 * k + 1], e[4 * k + 2], e[4 * k + 3]);
+    uint4 s16;
+    s16.x = __funnelshift_r(w[0], w[1], shift);
+    s16.y = __funnelshift_r(w[1], w[2], shift);
+    s16.z = __funnelshift_r(w[2], w[3], shift);
+    s16.w = __funnelshift_r(w[3], w[4], shift);
+    if (MODE == 0 && at.w == 16 && (at.c == 0 || at.r + 1 < at.rows || at.t0 + 32 <= at.cols)) {
+      // the rest of this tile row and the beginning of the next one
+      uint4 v0, v1;
+      ldec::merge16(e, s16, v0, v1);
+      const uint32_t v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+      const bool same = at.r + 1 < at.rows;
+      const int left = 16 - int(at.c);
+      uint16_t* p0 = o.out + size_t(at.r) * o.cols + at.col();
+      uint16_t* p1 = (same ? o.out + size_t(at.r + 1) * o.cols + at.t0 : o.out + at.t0 + 16) - left;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) (k < left ? p0 : p1)[k] = uint16_t(k & 1 ? v[k / 2] >> 16 : v[k / 2]);
+      if (same) {
+        ++at.r;
+      } else {
+        at.r = 0;
+        at.t0 += 16;
+        at.w = at.cols - at.t0 < 16 ? at.cols - at.t0 : 16;
+      }
+    } else {
+      const uint32_t sw[4] = {s16.x, s16.y, s16.z, s16.w};
+#pragma unroll
+      for (int k = 0; k < 16; ++k) emit(e[k], (sw[k >> 2] >> (8 * (k & 3))) & 255u);
+    }
+  }
+  for (; i < s.count; ++i) emit(ldec::dec_one<PCfg>(b, W.ring, W.t, lane, lc, bad), __ldg(s.sm + i));
+  return bad || uint64_t(b.pos - b.pos0) != s.nbits;
+}
+
 // Decodes one substream.  `rows16`: 16-row slab, cols % 16 == 0, the
 // substream starts on a tile row and (decode) the output is 16-byte aligned;
 // whole tile rows then leave as 32-byte stores.  The caller has started `b`
 // and `smr` (sign/mantissa bytes, 16 per group) and put the first words into
 // the ring.
-template <int MODE>
+// `WHOLE`: the caller's slabs all lie in whole rows, so that other substreams
+// (there are none) may go code by code; else decode_ragged takes them.
+template <int MODE, bool WHOLE>
 __device__ void decode_segment(const Seg& s, WarpTabs& W, int lane, const ldec::Code& lc, bool rows16,
                                ldec::Stream& b, ldec::SmStream& smr, const Out& o, bool& bad) {
+  if (!WHOLE && !rows16) {
+    if (decode_ragged<MODE>(s, W, lane, lc, b, o)) bad = true;
+    return;
+  }
   uint32_t i = 0;
   if (rows16) {
     const uint32_t ng = s.count >> 4;
@@ -239,7 +333,7 @@ __device__ __forceinline__ uint64_t warp_incl_scan(uint64_t v, int lane) {
   return v;
 }
 
-template <int MODE>
+template <int MODE, bool WHOLE>
 __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
     parallel_slab_kernel(const Slab* __restrict__ slabs, uint32_t nslabs,
                          const uint8_t* __restrict__ payload, uint8_t* __restrict__ out,
@@ -401,7 +495,7 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
     if (active && tb == 0) {
       b.init_ring(W.ring, lane);
       cp_async_wait_all();
-      decode_segment<MODE>(s, W, lane, lc, rows16, b, smr, o, bad);
+      decode_segment<MODE, WHOLE>(s, W, lane, lc, rows16, b, smr, o, bad);
     }
     cp_async_wait_all();
     // ---- substreams that need the generic decoder ----
@@ -445,8 +539,9 @@ void set_attr_once() {
   cudaGetDevice(&dev);
   const uint64_t bit = dev < 64 ? (1ull << dev) : 0ull;
   if (bit && (done.load(std::memory_order_acquire) & bit)) return;
-  cudaFuncSetAttribute(parallel_slab_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
-  cudaFuncSetAttribute(parallel_slab_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[1]));
+  cudaFuncSetAttribute(parallel_slab_kernel<0, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
+  cudaFuncSetAttribute(parallel_slab_kernel<0, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
+  cudaFuncSetAttribute(parallel_slab_kernel<1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[1]));
   if (bit) done.fetch_or(bit, std::memory_order_release);
 }
 
@@ -455,12 +550,16 @@ void set_attr_once() {
 size_t parallel_smem_bytes() { return kSmemBytes[0]; }
 
 cudaError_t launch_parallel_decode(const Slab* slabs, uint32_t n, const uint8_t* payload,
-                                   uint8_t* out, int* status, int grid, cudaStream_t st) {
+                                   uint8_t* out, int* status, int grid, cudaStream_t st, bool whole) {
   if (!n) return cudaSuccess;
   set_attr_once();
-  const int need = int((n + PWARPS - 1) / PWARPS);
-  parallel_slab_kernel<0><<<grid < need ? grid : need, PWARPS * 32, kSmemBytes[0], st>>>(
-      slabs, n, payload, out, nullptr, nullptr, 1, 1, status);
+  const int need = int((n + PWARPS - 1) / PWARPS), g = grid < need ? grid : need;
+  // the ragged path costs the whole rows 1.7 % (its call's registers: 8192
+  // slabs of 16 x 2048 456 us against 448), hence two kernels
+  if (whole)
+    parallel_slab_kernel<0, true><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status);
+  else
+    parallel_slab_kernel<0, false><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status);
   return cudaGetLastError();
 }
 
@@ -470,7 +569,7 @@ cudaError_t launch_parallel_gemm(const Slab* slabs, uint32_t n, const uint8_t* p
   if (!n) return cudaSuccess;
   set_attr_once();
   const int need = int((n + PWARPS - 1) / PWARPS);
-  parallel_slab_kernel<1><<<grid < need ? grid : need, PWARPS * 32, kSmemBytes[1], st>>>(
+  parallel_slab_kernel<1, false><<<grid < need ? grid : need, PWARPS * 32, kSmemBytes[1], st>>>(
       slabs, n, payload, nullptr, x + b0, y + b0, ld, nb, status);
   return cudaGetLastError();
 }
