@@ -1,0 +1,160 @@
+"""GPU: serving on compressed weights -- archives compiled here, loaded with
+fused layers, prompts and steps through the paged cache -- against the model's
+own Transformers forward on decoded weights; fused layers with bias and the
+fused feed-forward layer against torch in 64 bits.
+
+A session's logits differ from the Transformers forward's by BF16 roundings at
+other places (the fused epilogues round once where Transformers rounds after
+every operation): two roundings of 2^-8 per layer operation, about eight such operations a
+layer, in relative L2 at most (they add in quadrature): 2^-8 * sqrt(2 * 8 * layers + 8) < 3e-2
+for the two layers here."""
+import json
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytest.importorskip("transformers")
+pytestmark = pytest.mark.gpu
+
+import xksv_compile as xc  # noqa: E402
+import xksv_gpu as xg  # noqa: E402
+import xksv_runtime as rt  # noqa: E402
+import xksv_serve as serve  # noqa: E402
+from golden.make_archives import write_safetensors  # noqa: E402
+
+DEV = "cuda:0"
+BASE = {"hidden_size": 128, "intermediate_size": 352, "num_hidden_layers": 2, "num_attention_heads": 8,
+        "num_key_value_heads": 2, "vocab_size": 256, "max_position_embeddings": 512, "rms_norm_eps": 1e-5,
+        "tie_word_embeddings": False, "torch_dtype": "bfloat16"}
+CONFIGS = {
+    "llama": dict(BASE, architectures=["LlamaForCausalLM"], model_type="llama", hidden_act="silu", rope_theta=10000.0),
+    "llama-gelu": dict(BASE, architectures=["LlamaForCausalLM"], model_type="llama", hidden_act="gelu_pytorch_tanh",
+                       mlp_bias=True, attention_bias=True, rope_theta=500000.0),
+    "qwen2": dict(BASE, architectures=["Qwen2ForCausalLM"], model_type="qwen2", hidden_act="silu", rope_theta=10000.0),
+    "mistral": dict(BASE, architectures=["MistralForCausalLM"], model_type="mistral", hidden_act="silu",
+                    rope_theta=10000.0, sliding_window=24, head_dim=32),
+}
+
+
+def archive(tmp_path, name, codec="dfloat11"):
+    """An archive of a seeded model of CONFIGS[name]."""
+    from transformers import AutoConfig, AutoModelForCausalLM
+    src = tmp_path / name
+    src.mkdir()
+    (src / "config.json").write_text(json.dumps(CONFIGS[name]))
+    model = AutoModelForCausalLM.from_config(AutoConfig.from_pretrained(src))
+    g = torch.Generator().manual_seed(1)
+    tensors = []
+    for n, t in model.state_dict().items():
+        v = torch.randn(t.shape, generator=g) * (0.3 if n.endswith("bias") else 0.08)
+        v = torch.ones(t.shape) if n.endswith("norm.weight") else v
+        v = v.to(torch.bfloat16)
+        tensors.append((n, "BF16", list(t.shape), v.view(torch.uint8).numpy().tobytes()))
+    write_safetensors(src / "model.safetensors", tensors)
+    return xc.compile_checkpoint(src, tmp_path / f"{name}.xksv", codec)
+
+
+def close(a, b, tol=3e-2):
+    return float((a.float() - b.float()).norm() / b.float().norm()) < tol
+
+
+@pytest.mark.parametrize("name", list(CONFIGS))
+@pytest.mark.parametrize("kv", ["bf16", "e4m3"])
+def test_session_matches_transformers(tmp_path, name, kv):
+    path = archive(tmp_path, name)
+    ref, _, _ = rt.load_archive(path, DEV)
+    s = serve.load_session(path, DEV, pages=64, page_size=8, max_seqs=4, kv_dtype=kv)
+    assert all(hasattr(l.self_attn.q_proj, "xksv_fused") and hasattr(l.mlp, "xksv_fused_mlp") for l in s.layers)
+    # an 8-bit cache rounds keys and values by 2^-4 more
+    tol = 3e-2 if kv == "bf16" else 1e-1
+    g = torch.Generator().manual_seed(2)
+    prompts = [torch.randint(0, 256, (n,), generator=g) for n in (1, 40, 17)]
+    ids = [p.to(DEV) for p in prompts]
+    with torch.no_grad():
+        seqs, logits = s.prefill(prompts)
+        for step in range(12):
+            want = torch.stack([ref(x[None]).logits[0, -1] for x in ids])
+            assert close(logits, want, tol), step
+            # a step of all, then of some, in another order
+            order = [0, 1, 2] if step % 3 else [2, 0]
+            token = want.argmax(-1)
+            if len(order) < 3:
+                part = s.step([seqs[i] for i in order], token[torch.tensor(order, device=DEV)])
+                rest = s.step([seqs[1]], token[1:2])
+                logits = torch.stack([part[1], rest[0], part[0]])
+            else:
+                logits = s.step(seqs, token)
+            ids = [torch.cat((x, t[None])) for x, t in zip(ids, token)]
+    s._check()
+    s.release(seqs)
+    assert len(s.free_pages) == 64 and not s.length
+    s.close()
+
+
+def test_generate_is_the_greedy_continuation(tmp_path):
+    """Every generated token is among the best of the Transformers logits at its
+    place (within the logits' own tolerance)."""
+    path = archive(tmp_path, "llama")
+    ref, _, _ = rt.load_archive(path, DEV)
+    s = serve.load_session(path, DEV, pages=40, page_size=16, max_seqs=3)
+    prompts = [[5, 9, 200], [77] * 20]
+    out = s.generate(prompts, 10)
+    assert [len(o) for o in out] == [10, 10] and len(s.free_pages) == 40
+    for p, o in zip(prompts, out):
+        with torch.no_grad():
+            logits = ref(torch.tensor([p + o], device=DEV)).logits[0].float()
+        for k, t in enumerate(o):
+            row = logits[len(p) + k - 1]
+            assert row.max() - row[t] <= 3e-2 * 2 * row.norm()
+    assert s.generate([[5, 9, 200]], 10, eos=out[0][3])[0] == out[0][:out[0].index(out[0][3]) + 1]
+    s.close()
+
+
+def test_session_refusals(tmp_path):
+    path = archive(tmp_path, "llama")
+    s = serve.load_session(path, DEV, pages=4, page_size=16, max_seqs=2, max_tokens=48)
+    for bad, match in (([torch.zeros(0, dtype=torch.long)], "empty"), ([[1]] * 3, "too many"), ([[1] * 49], "exceeds"),
+                       ([[1] * 33, [1] * 33], "full")):
+        with pytest.raises(rt.ArchiveError, match=match):
+            s.prefill(bad)
+        assert len(s.free_pages) == 4 and len(s.free_seqs) == 2
+    seqs, _ = s.prefill([[1] * 48, [2] * 15])
+    s.step(seqs[1:], [3])
+    for bad, match in ((seqs[:1], "exceeds"), (seqs[1:], "full"), ([seqs[1], seqs[1]], "repeated"), ([], "no sequence"),
+                       ([9], "unknown")):
+        with pytest.raises(rt.ArchiveError, match=match):
+            s.step(bad, [1] * len(bad))
+    s.release(seqs[:1])
+    assert s.step(seqs[1:], [4]).shape == (1, 256)
+    with pytest.raises(rt.ArchiveError, match="dtype"):
+        serve.PagedSession(s.model, 4, kv_dtype="int8")
+    s.close()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch", [1, 2, 9, 150])
+def test_fused_weight_epilogue(tmp_path, dtype, batch):
+    """FusedWeight's epilogue for BF16 activations (one linear call) and others."""
+    path = archive(tmp_path, "llama-gelu")
+    a = rt.ResidentArchive(path, DEV)
+    a.verify()
+    name = "model.layers.0.mlp.up_proj"
+    fw, W, bias = a.fused(name + ".weight"), a.tensor(name + ".weight").double(), a.tensor(name + ".bias")
+    g = torch.Generator(device=DEV).manual_seed(batch)
+    x, mul, res = (torch.randn(batch, n, generator=g, device=DEV).to(dtype) for n in (128, 352, 352))
+    y = fw(x, bias=bias, act="gelu", mul=mul, residual=res)
+    z = x.to(torch.bfloat16).double() @ W.t() if batch >= 4 else x.double() @ W.t()
+    want = torch.nn.functional.gelu(z + bias.double()) * mul.double() + res.double()
+    assert y.dtype == dtype and y.shape == (batch, 352)
+    # half a step of the type, and FP32 sums of 128 products
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -16 * (1 + mul.double().abs()) * (1 + z.abs())
+    assert ((y.double() - want).abs() <= tol).all()
+    # operands of any strides and shape: transposed, expanded, FP16 factors
+    xt = x.t().contiguous().t()
+    again = fw(xt, bias=bias.half(), act="gelu", mul=mul.t().contiguous().t(), residual=res)
+    assert ((again.double() - want).abs() <= tol + 2.0 ** -10).all()
+    same = fw(x[:1].expand(batch, -1))
+    assert ((same - fw(x[:1])).abs() <= 2.0 ** -7 * (1 + same.abs())).all()
+    cube = fw(x[:, None, None], residual=res[:, None, None])
+    assert cube.shape == (batch, 1, 1, 352)
+    fw.close()

@@ -187,14 +187,15 @@ def fusable(t):
                    or (b["codec"] != "raw" and b["cols"] != cols) for b in t["blocks"])
 
 
-def fused_candidates(model, tensors):
+def fused_candidates(model, tensors, biased=False):
     """Names of the linear layers install_fused_gemv replaces: bias-free
     nn.Linear modules other than lm_head whose weight is fusable
-    (python/runtime.py:256-263)."""
+    (python/runtime.py:256-263); with `biased`, layers that have a bias too
+    (the reference leaves those decoded)."""
     import torch
     names = []
     for name, module in model.named_modules():
-        if not isinstance(module, torch.nn.Linear) or module.bias is not None or name == "lm_head":
+        if not isinstance(module, torch.nn.Linear) or name == "lm_head" or (module.bias is not None and not biased):
             continue
         if fusable(tensors.get(name + ".weight")):
             names.append(name)
@@ -494,6 +495,33 @@ class ResidentArchive:
         self.payload = None
 
 
+def _torch_acts():
+    import torch.nn.functional as F
+    return {"none": lambda z: z, "relu": F.relu, "silu": F.silu, "gelu": F.gelu,
+            "gelu_tanh": lambda z: F.gelu(z, approximate="tanh")}
+
+
+class _Acts(dict):
+    """xksv_gpu.ACTS as torch functions, looked up on first use."""
+
+    def __missing__(self, name):
+        self.update(_torch_acts())
+        return self[name] if name in _torch_acts() else fail(f"unknown activation {name}")
+
+
+TORCH_ACTS = _Acts()
+
+
+def _dense(t, rows, cols):
+    """t as [rows, cols] with contiguous rows that do not overlap (a copy where
+    it is transposed or expanded), BF16 or FP32."""
+    import torch
+    t = t.reshape(rows, cols)
+    if t.dtype not in (torch.bfloat16, torch.float32):
+        t = t.float()
+    return t if (cols == 1 or t.stride(1) == 1) and (rows == 1 or t.stride(0) >= cols) else t.contiguous()
+
+
 class FusedWeight:
     """y = x W^T for a weight that stays compressed in HBM: one plan over the
     weight's blocks (tile index built once for its 16-row serial blocks).
@@ -518,7 +546,12 @@ class FusedWeight:
         archive._tc_need = max(archive._tc_need, self._scratch_need)
         self._lent = None
 
-    def __call__(self, x):
+    def __call__(self, x, bias=None, act="none", mul=None, residual=None):
+        """act(x W^T + bias) * mul + residual, of x's dtype: mul and residual are
+        [..., rows] like the result, act a key of xksv_gpu.ACTS.  BF16 activations
+        run as one linear call with its epilogue; others as the FP32 product
+        (tensor cores from TC_MIN_BATCH on, with x rounded to BF16) and torch
+        operations."""
         import torch
         if x.shape[-1] != self.cols:
             raise ValueError(f"{self.name}: input width {x.shape[-1]} != {self.cols}")
@@ -528,6 +561,15 @@ class FusedWeight:
         if batch == 0:
             return x.new_empty(*lead, self.rows)
         stream = torch.cuda.current_stream(x.device).cuda_stream
+        if x.dtype == torch.bfloat16:
+            y = torch.empty(batch, self.rows, device=x.device, dtype=x.dtype)
+            if bias is not None and bias.dtype not in (torch.bfloat16, torch.float32):
+                bias = bias.float()
+            self.plan.linear(self.archive.payload, _dense(x, batch, self.cols), y, bias=bias, act=act,
+                             mul=None if mul is None else _dense(mul, batch, self.rows),
+                             residual=None if residual is None else _dense(residual, batch, self.rows), stream=stream)
+            self._check(stream)
+            return y.reshape(*lead, self.rows)
         if batch >= xksv_gpu.TC_MIN_BATCH and self._scratch_need:
             buf = self.archive.shared_scratch()
             if self._lent is not buf:  # keeps the lent buffer alive while the plan points at it
@@ -540,25 +582,82 @@ class FusedWeight:
             xt = xb.t().float().contiguous()
             y = torch.empty(self.rows, batch, device=x.device, dtype=torch.float32)
         self.plan.gemm(self.archive.payload, xt, y, batch, stream)
+        self._check(stream)
+        out = y if batch == 1 else y.t()
+        if bias is not None or act != "none" or mul is not None or residual is not None:
+            out = out.reshape(batch, self.rows)
+            if bias is not None:
+                out = out + bias.float()
+            out = TORCH_ACTS[act](out)
+            if mul is not None:
+                out = out * mul.reshape(batch, self.rows).float()
+            if residual is not None:
+                out = out + residual.reshape(batch, self.rows).float()
+        return out.to(x.dtype).reshape(*lead, self.rows)
+
+    def _check(self, stream):
         if not self.archive.verified and self.plan.status(stream):
             fail(f"fused GEMV failed: {self.name}")
-        out = y if batch == 1 else y.t()
-        return out.to(x.dtype).reshape(*lead, self.rows)
 
     def close(self):
         self.plan.close()
 
 
-def install_fused_gemv(model, archive):
+class FusedLinear:
+    """A linear layer's forward on its FusedWeight, the layer's bias added in the
+    epilogue; further epilogue operands as FusedWeight takes them."""
+
+    def __init__(self, weight, module):
+        self.weight, self.module = weight, module
+
+    def __call__(self, x, **epilogue):
+        return self.weight(x, bias=self.module.bias, **epilogue)
+
+
+def install_fused_gemv(model, archive, biased=False):
     """Replaces the forward of every eligible linear layer with its resident
-    FusedWeight (python/runtime.py:248-287); returns how many."""
+    FusedWeight (python/runtime.py:248-287); returns how many.  With `biased`,
+    layers with a bias too, added in the product's epilogue."""
     installed = 0
     modules = dict(model.named_modules())
-    for name in fused_candidates(model, archive.tensors):
+    for name in fused_candidates(model, archive.tensors, biased):
         fw = archive.fused(name + ".weight")
-        modules[name].forward = fw
-        modules[name].xksv_fused = fw
+        module = modules[name]
+        module.forward = fw if module.bias is None else FusedLinear(fw, module)
+        module.xksv_fused = fw
         installed += 1
+    return installed
+
+
+# config.hidden_act names whose activation the product's epilogue computes
+EPILOGUE_ACTS = {"silu": "silu", "swish": "silu", "gelu": "gelu", "gelu_new": "gelu_tanh",
+                 "gelu_pytorch_tanh": "gelu_tanh", "relu": "relu"}
+
+
+class FusedMLP:
+    """A gated feed-forward layer on fused weights: down(act(gate(x)) * up(x)) in
+    three products, the activation, the gating product and (given a residual)
+    the addition in their epilogues."""
+
+    def __init__(self, module, act):
+        self.gate, self.up, self.down, self.act = module.gate_proj, module.up_proj, module.down_proj, act
+
+    def __call__(self, x, residual=None):
+        return self.down.forward(self.up.forward(x, mul=self.gate.forward(x, act=self.act)), residual=residual)
+
+
+def install_fused_mlp(model):
+    """Replaces the forward of every gated feed-forward module (gate_proj,
+    up_proj, down_proj) whose three layers are fused and whose activation
+    (config.hidden_act) the epilogue has, by a FusedMLP; returns how many."""
+    act = EPILOGUE_ACTS.get(getattr(getattr(model, "config", None), "hidden_act", None))
+    installed = 0
+    for module in model.modules():
+        parts = [getattr(module, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
+        if act and all(hasattr(p, "xksv_fused") for p in parts):
+            module.forward = FusedMLP(module, act)
+            module.xksv_fused_mlp = True
+            installed += 1
     return installed
 
 
@@ -606,12 +705,14 @@ def backend_class(config):
     return AutoModelForCausalLM
 
 
-def load_archive(path, device, model=None, verify=True, fused_gemv=False):
+def load_archive(path, device, model=None, verify=True, fused_gemv=False, fused_mlp=False):
     """The ``load_archive(..., gpu_decode=True)`` flow (python/runtime.py:31-117)
     on a resident archive: upload, device verification, one-launch decode into
     the model, optional fused linear layers.  Without `model`, the model is
     built from the archive's config.json asset with Transformers, as the
     reference does, and a tokenizer is loaded when the assets hold one.
+    `fused_mlp` (with fused_gemv) fuses layers with a bias too and the gated
+    feed-forward layers' activation and product (install_fused_mlp).
     Returns (model, tokenizer or None, archive)."""
     import torch
     archive = ResidentArchive(path, device)
@@ -634,7 +735,7 @@ def load_archive(path, device, model=None, verify=True, fused_gemv=False):
     # not decoded, and the parameter becomes a zero-element placeholder (the
     # fused forward never reads it), so the model holds the compressed bytes
     # once instead of compressed + decoded
-    fused = [n + ".weight" for n in fused_candidates(model, archive.tensors)] if fused_gemv else []
+    fused = [n + ".weight" for n in fused_candidates(model, archive.tensors, fused_mlp)] if fused_gemv else []
     if fused_gemv and not fused:
         fail("no compatible linear layers for fused GEMV")
     keep = [n for n in archive.tensors if n not in set(fused)]
@@ -644,6 +745,8 @@ def load_archive(path, device, model=None, verify=True, fused_gemv=False):
     assign_tensors(model, tensors)
     model.to(archive.device)
     if fused_gemv:
-        install_fused_gemv(model, archive)
+        install_fused_gemv(model, archive, biased=fused_mlp)
+        if fused_mlp:
+            install_fused_mlp(model)
     torch.cuda.synchronize(archive.device)
     return model, tokenizer, archive
