@@ -117,6 +117,7 @@ def test_binding_refuses_before_the_library():
         xg.KVCache(k, k.clone())
     with pytest.raises(ValueError, match="layout"):
         xg.KVCache(k, k.clone(), layout="dhn")
+    xg._torch_types()
     dev = -1  # get_device() of a CPU tensor
     x = torch.zeros(4, 8)
     assert xg._matrix(x, 4, 8, "x", dev) == (x.data_ptr(), 8)
@@ -136,6 +137,39 @@ def test_binding_refuses_before_the_library():
         xg._ints(torch.zeros(8, dtype=torch.int32)[::2], 4, "index", dev)
     with pytest.raises(ValueError):
         xg._table(torch.zeros(4, 4, dtype=torch.int32).t(), dev)
+
+
+def test_argument_blocks_match_the_header(tmp_path):
+    """The packed argument blocks have the C structs' sizes and field offsets."""
+    import xksv_gpu as xg
+    fields = {
+        "xksv_linear_args": (xg.LINEAR_ARGS, "x x_cols x_stride y y_cols y_stride batch bias mul mul_stride residual "
+                             "residual_stride y_type bias_type mul_type residual_type act flags"),
+        "xksv_kv_append_args": (xg.KV_APPEND_ARGS, "q k v q_out q_stride[0] q_stride[1] k_stride[0] k_stride[1] v_stride[0] "
+                                "v_stride[1] q_out_stride[0] q_out_stride[1] tokens table table_rows table_cols table_stride "
+                                "seq index positions inv_freq rot_scale rot_dim q_heads type flags"),
+        "xksv_kv_attend_args": (xg.KV_ATTEND_ARGS, "q out lse q_stride[0] q_stride[1] out_stride[0] out_stride[1] seqs table "
+                                "table_cols table_stride lens scale softcap window q_heads type"),
+    }
+    src = tmp_path / "f.cpp"
+    lines = ['#include "xksv_cuda.h"', "#include <cstddef>", "#include <cstdio>", "int main() {"]
+    for name, (_, names) in fields.items():
+        lines += [f'std::printf("%zu\\n", offsetof({name}, {n}));' for n in names.split()]
+        lines.append(f'std::printf("%zu\\n", sizeof({name}));')
+    src.write_text("\n".join(lines) + "\n}\n")
+    exe = tmp_path / "f"
+    subprocess.run(["g++", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
+    got = iter(int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split())
+    for name, (packed, names) in fields.items():
+        n = len(names.split())
+        # a block whose k-th field alone is 1 (or 1.0) differs from zeros at that field's offset
+        zero = packed.pack(*[0] * n)
+        for k in range(n):
+            one = packed.pack(*[int(k == i) for i in range(n)])
+            at = next(i for i in range(len(zero)) if one[i] != zero[i])
+            want = next(got)
+            assert want <= at < want + 4, (name, names.split()[k])
+        assert packed.size == next(got), name
 
 
 def test_null_arguments_are_refused():

@@ -8,6 +8,7 @@ callers.  There is no fallback: a missing library raises.
 """
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -25,17 +26,6 @@ class Slab(ctypes.Structure):
                 ("codec", ctypes.c_uint32), ("flags", ctypes.c_uint32)]
 
 
-class LinearArgs(ctypes.Structure):
-    """xksv_linear_args."""
-    _fields_ = [("x", ctypes.c_void_p), ("x_cols", ctypes.c_uint64), ("x_stride", ctypes.c_uint64),
-                ("y", ctypes.c_void_p), ("y_cols", ctypes.c_uint64), ("y_stride", ctypes.c_uint64),
-                ("batch", ctypes.c_uint64), ("bias", ctypes.c_void_p), ("mul", ctypes.c_void_p),
-                ("mul_stride", ctypes.c_uint64), ("residual", ctypes.c_void_p),
-                ("residual_stride", ctypes.c_uint64), ("y_type", ctypes.c_uint32), ("bias_type", ctypes.c_uint32),
-                ("mul_type", ctypes.c_uint32), ("residual_type", ctypes.c_uint32), ("act", ctypes.c_uint32),
-                ("flags", ctypes.c_uint32)]
-
-
 class KvDesc(ctypes.Structure):
     """xksv_kv_desc."""
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_bytes", ctypes.c_uint64),
@@ -45,26 +35,11 @@ class KvDesc(ctypes.Structure):
                 ("type", ctypes.c_uint32), ("flags", ctypes.c_uint32)]
 
 
-class KvAppendArgs(ctypes.Structure):
-    """xksv_kv_append_args."""
-    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
-                ("q_token", ctypes.c_uint64), ("q_head", ctypes.c_uint64), ("k_token", ctypes.c_uint64),
-                ("k_head", ctypes.c_uint64), ("v_token", ctypes.c_uint64), ("v_head", ctypes.c_uint64),
-                ("q_out_token", ctypes.c_uint64), ("q_out_head", ctypes.c_uint64), ("tokens", ctypes.c_uint64), ("table", ctypes.c_void_p), ("table_rows", ctypes.c_uint64),
-                ("table_cols", ctypes.c_uint64), ("table_stride", ctypes.c_uint64), ("seq", ctypes.c_void_p),
-                ("index", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
-                ("rot_scale", ctypes.c_float), ("rot_dim", ctypes.c_uint32), ("q_heads", ctypes.c_uint32),
-                ("type", ctypes.c_uint32), ("flags", ctypes.c_uint32)]
-
-
-class KvAttendArgs(ctypes.Structure):
-    """xksv_kv_attend_args."""
-    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p), ("lse", ctypes.c_void_p),
-                ("q_seq", ctypes.c_uint64), ("q_head", ctypes.c_uint64), ("out_seq", ctypes.c_uint64),
-                ("out_head", ctypes.c_uint64), ("seqs", ctypes.c_uint64),
-                ("table", ctypes.c_void_p), ("table_cols", ctypes.c_uint64), ("table_stride", ctypes.c_uint64),
-                ("lens", ctypes.c_void_p), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
-                ("window", ctypes.c_uint64), ("q_heads", ctypes.c_uint32), ("type", ctypes.c_uint32)]
+# Argument blocks of the calls made once a token, packed as the C structs of
+# the same name lie in memory (a ctypes.Structure takes 3 us to fill).
+LINEAR_ARGS = struct.Struct("@3Q3QQQ2Q2Q6I")     # xksv_linear_args
+KV_APPEND_ARGS = struct.Struct("@4Q8QQ4Q4Qf4I4x")  # xksv_kv_append_args
+KV_ATTEND_ARGS = struct.Struct("@3Q4QQ3QQ2fQ2I")  # xksv_kv_attend_args
 
 
 _SIGS = {
@@ -132,15 +107,15 @@ _SIGS = {
                                   ctypes.c_void_p], ctypes.c_int),
     "xksv_plan_device": ([ctypes.c_void_p], ctypes.c_int),
     "xksv_plan_linear_workspace": ([ctypes.c_void_p, ctypes.c_size_t], ctypes.c_size_t),
-    "xksv_plan_linear": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.POINTER(LinearArgs),
+    "xksv_plan_linear": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
     "xksv_kv_create": ([ctypes.POINTER(KvDesc), ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
     "xksv_kv_destroy": ([ctypes.c_void_p], None),
     "xksv_kv_status": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
-    "xksv_kv_append": ([ctypes.c_void_p, ctypes.POINTER(KvAppendArgs), ctypes.c_void_p], ctypes.c_int),
+    "xksv_kv_append": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
     "xksv_kv_attend_workspace": ([ctypes.c_void_p, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t],
                                  ctypes.c_size_t),
-    "xksv_kv_attend": ([ctypes.c_void_p, ctypes.POINTER(KvAttendArgs), ctypes.c_void_p, ctypes.c_size_t,
+    "xksv_kv_attend": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                         ctypes.c_void_p], ctypes.c_int),
 }
 
@@ -296,17 +271,24 @@ def _rows(buf, nrows, batch, what):
 
 
 _types = {}
+_i32 = None
 
 
 def _type(t, allowed, what):
     """The element type code of tensor t, one of `allowed`."""
     if not _types:
-        import torch
-        _types.update({torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32, torch.float8_e4m3fn: E4M3})
+        _torch_types()
     code = _types.get(t.dtype)
     if code not in allowed:
         raise ValueError(f"{what}: dtype {t.dtype} is not supported")
     return code
+
+
+def _torch_types():
+    global _i32
+    import torch
+    _i32 = torch.int32
+    _types.update({torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32, torch.float8_e4m3fn: E4M3})
 
 
 def _matrix(t, rows, cols, what, device):
@@ -336,27 +318,16 @@ def _heads(t, rows, heads, dim, what, device):
 
 def _ints(t, n, what, device):
     """Address of a contiguous int32 [n] tensor."""
-    if t.dtype != _int32() or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype != _i32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous int32 [{n}] tensor is needed")
     if t.get_device() != device:
         raise ValueError(f"{what}: on {t.device}, expected CUDA device {device}")
     return t.data_ptr()
 
 
-def _int32():
-    global _i32
-    if _i32 is None:
-        import torch
-        _i32 = torch.int32
-    return _i32
-
-
-_i32 = None
-
-
 def _table(t, device):
     """(address, rows, columns, row stride) of an int32 page table."""
-    if t.dtype != _int32() or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dtype != _i32 or t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError("table: an int32 [sequences, pages] tensor with contiguous rows is needed")
     if t.get_device() != device:
         raise ValueError(f"table: on {t.device}, expected CUDA device {device}")
@@ -434,26 +405,27 @@ class Plan:
         pay, npay = dev_buffer(d_payload, payload_bytes, "payload")
         if x.dim() != 2 or y.dim() != 2:
             raise ValueError("x and y are [batch, columns]")
-        batch, rows = x.shape[0], y.shape[1]
+        (batch, cols), rows = x.shape, y.shape[1]
         _type(x, (BF16,), "x")
-        xp, xs = _matrix(x, batch, x.shape[1], "x", device)
+        xp, xs = _matrix(x, batch, cols, "x", device)
         yp, ys = _matrix(y, batch, rows, "y", device)
-        a = LinearArgs(xp, x.shape[1], xs, yp, rows, ys, batch)
-        a.y_type = _type(y, (BF16, FP32), "y")
+        y_type = _type(y, (BF16, FP32), "y")
+        bp = mp = ms = rp = rs = b_type = m_type = r_type = 0
         if bias is not None:
-            a.bias_type = _type(bias, (BF16, FP32), "bias")
-            if tuple(bias.shape) != (rows,) or (rows > 1 and bias.stride(0) != 1) or bias.get_device() != device:
+            b_type = _type(bias, (BF16, FP32), "bias")
+            if bias.shape != (rows,) or not bias.is_contiguous() or bias.get_device() != device:
                 raise ValueError(f"bias: a contiguous [{rows}] tensor on CUDA device {device} is needed")
-            a.bias = bias.data_ptr()
+            bp = bias.data_ptr()
         if mul is not None:
-            a.mul_type = _type(mul, (BF16, FP32), "mul")
-            a.mul, a.mul_stride = _matrix(mul, batch, rows, "mul", device)
+            m_type = _type(mul, (BF16, FP32), "mul")
+            mp, ms = _matrix(mul, batch, rows, "mul", device)
         if residual is not None:
-            a.residual_type = _type(residual, (BF16, FP32), "residual")
-            a.residual, a.residual_stride = _matrix(residual, batch, rows, "residual", device)
-        a.act = ACTS[act]
-        ws, wp, wn = _workspace(workspace, self.linear_workspace(batch), x.device, stream)
-        if self.lib.xksv_plan_linear(self.handle, pay, npay, ctypes.byref(a), wp, wn, stream):
+            r_type = _type(residual, (BF16, FP32), "residual")
+            rp, rs = _matrix(residual, batch, rows, "residual", device)
+        a = LINEAR_ARGS.pack(xp, cols, xs, yp, rows, ys, batch, bp, mp, ms, rp, rs, y_type, b_type, m_type, r_type,
+                             ACTS[act], 0)
+        ws, wp, wn = _workspace(workspace, self.lib.xksv_plan_linear_workspace(self.handle, batch), x.device, stream)
+        if self.lib.xksv_plan_linear(self.handle, pay, npay, a, wp, wn, stream):
             raise RuntimeError("xksv_plan_linear refused the call or failed to launch")
 
     def linear_workspace(self, batch):
@@ -576,17 +548,17 @@ class KVCache:
             raise ValueError("q_out without q")
         tp, rows, cols, stride = _table(table, dev)
         ip = _ints(index, n, "index", dev)
-        sp = None if seq is None else _ints(seq, n, "seq", dev)
-        pp = None if positions is None else _ints(positions, n, "positions", dev)
-        fp, rot = None, 0
+        sp = 0 if seq is None else _ints(seq, n, "seq", dev)
+        pp = 0 if positions is None else _ints(positions, n, "positions", dev)
+        fp = rot = 0
         if inv_freq is not None:
             _type(inv_freq, (FP32,), "inv_freq")
             if inv_freq.dim() != 1 or not inv_freq.is_contiguous() or inv_freq.get_device() != dev:
                 raise ValueError(f"inv_freq: a contiguous FP32 vector on CUDA device {dev} is needed")
             fp, rot = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
-        a = KvAppendArgs(qp, kp, vp, op, q0, q1, k0, k1, v0, v1, o0, o1, n, tp, rows, cols, stride, sp, ip, pp, fp,
-                         rot_scale, rot, heads, code, KV_INTERLEAVED if interleaved else 0)
-        if self.lib.xksv_kv_append(self.handle, ctypes.byref(a), stream):
+        a = KV_APPEND_ARGS.pack(qp, kp, vp, op, q0, q1, k0, k1, v0, v1, o0, o1, n, tp, rows, cols, stride, sp, ip, pp, fp,
+                                rot_scale, rot, heads, code, KV_INTERLEAVED if interleaved else 0)
+        if self.lib.xksv_kv_append(self.handle, a, stream):
             raise RuntimeError("xksv_kv_append refused the call or failed to launch")
 
     def attend(self, q, table, lens, out, lse=None, scale=None, window=0, softcap=0.0, stream=0, workspace=None):
@@ -603,7 +575,7 @@ class KVCache:
         code = _type(q, (BF16, FP16), "q")
         qp, q0, q1 = _heads(q, n, heads, dim, "q", dev)
         op, o0, o1 = _heads(out, n, heads, dim, "out", dev)
-        lp = None
+        lp = 0
         if lse is not None:
             _type(lse, (FP32,), "lse")
             if lse.shape != (n, heads) or not lse.is_contiguous() or lse.get_device() != dev:
@@ -614,13 +586,13 @@ class KVCache:
             raise ValueError(f"table: {rows} rows for {n} sequences")
         if window < 0:
             raise ValueError("window is not negative")
-        a = KvAttendArgs(qp, op, lp, q0, q1, o0, o1, n, tp, cols, stride, _ints(lens, n, "lens", dev),
-                         dim ** -0.5 if scale is None else scale, softcap, window, heads, code)
+        a = KV_ATTEND_ARGS.pack(qp, op, lp, q0, q1, o0, o1, n, tp, cols, stride, _ints(lens, n, "lens", dev),
+                                dim ** -0.5 if scale is None else scale, softcap, window, heads, code)
         ws, wp, wn = workspace, None, 0
         if n:
             need = self.lib.xksv_kv_attend_workspace(self.handle, n, heads, cols)
             ws, wp, wn = _workspace(workspace, need, self.device, stream)
-        if self.lib.xksv_kv_attend(self.handle, ctypes.byref(a), wp, wn, stream):
+        if self.lib.xksv_kv_attend(self.handle, a, wp, wn, stream):
             raise RuntimeError("xksv_kv_attend refused the call or failed to launch")
 
     def attend_workspace(self, seqs, q_heads, table_cols):
