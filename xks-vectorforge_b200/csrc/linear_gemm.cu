@@ -1,19 +1,22 @@
 // Linear layer of a prompt: y[tokens, rows] = epilogue(x W^T) on the 5th-
 // generation tensor cores, W decoded into a BF16 scratch before.
 //
-// Bound: the tensor cores (2 tokens rows cols operations; both operands come
-// from L2).  A persistent CTA per SM takes tiles of 128 tokens by `tn` weight
-// rows; within it
+// Bound: the tensor cores (2 tokens rows cols operations) or the operands' way
+// from L2, about 64 bytes a clock and SM: a 128 x 256 tile multiplies a
+// 64-column slice in 512 clocks and reads 48 KB for it.  Two CTAs of a pair
+// (PAIR) share a 256 x tn tile: each brings 128 tokens and half of the weight
+// rows, 32 KB a slice, and tcgen05.mma cta_group::2 reads both.  A persistent
+// CTA (or pair) per SM takes tiles; within it
 //   * one thread loads 64-column slices of x and W by TMA (128-byte swizzled
 //     rows, zero past the edges) into a ring of stages,
-//   * one thread issues tcgen05.mma kind::f16, M = 128 tokens, N = tn, K = 16,
-//     into one of two TMEM accumulators,
+//   * one thread (of the pair's first CTA) issues tcgen05.mma kind::f16,
+//     M = 128 (256) tokens, N = tn, K = 16, into one of two TMEM accumulators,
 //   * four warps read the other accumulator (a lane is a token, its registers
 //     consecutive rows of y), apply bias, activation, factor and residual in
 //     FP32 and write y: the epilogue of a tile runs behind the products of the next.
-// tn is the multiple of 16 whose waves of tiles cost least on this GPU's SMs
-// (gemm_tile).  Tokens as the MMA's rows rather than weight rows: y is
-// token-major, so a lane's results are contiguous.
+// gemm_plan chooses tn and the pair by a model of both costs.  Tokens as the
+// MMA's rows rather than weight rows: y is token-major, so a lane's results
+// are contiguous.
 // Every wait is bounded: on a timeout the CTA sets an error bit, lets its
 // copies and MMAs drain, frees its TMEM and returns.
 #include <cuda.h>
@@ -49,11 +52,12 @@ struct GemmArgs {
   int* status;
 };
 
+// (Cluster scope: the pair's CTAs arrive on each other's barriers.)
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
   for (uint32_t i = 0; i < kSpin; ++i) {
     uint32_t done;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
         " selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(done)
         : "r"(bar), "r"(parity)
@@ -75,6 +79,49 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, u
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// The same, its bytes counted on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t x, uint32_t y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+// A shared-memory address of this CTA in CTA `rank` of its cluster.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;\n" ::: "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if (!PAIR) {
+    umma_bf16(d, a, b, idesc, accumulate);
+    return;
+  }
+  const uint32_t z = 0;
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(z)
+      : "memory");
+}
+// Arrives on a barrier (of both CTAs) when the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (PAIR)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+                 "h"(uint16_t(3))
+                 : "memory");
+  else
+    umma_commit(bar);
+}
+
 // Shared-memory descriptor of a K-major operand of 128-byte swizzled rows:
 // eight rows are 1024 bytes (SBO), layout type 2 in bits 61-63.
 __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
@@ -93,19 +140,31 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
 
+template <bool PAIR>
 __global__ void __launch_bounds__(GTHREADS, 1)
     linear_gemm_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const GemmArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ GemmShared S;
+  constexpr uint32_t CTAS = PAIR ? 2 : 1, TM = GM * CTAS;  // tokens of a tile
   uint8_t* ring = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t stage_bytes = kABytes + a.tn * GK * 2;
-  const uint32_t mt = (a.batch + GM - 1) / GM, nt = (a.rows + a.tn - 1) / a.tn, tiles = mt * nt;
+  uint32_t rank = 0;
+  if (PAIR) asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
+  const uint32_t bn = a.tn / CTAS;  // weight rows that this CTA brings
+  const uint32_t stage_bytes = kABytes + bn * GK * 2;
+  const uint32_t mt = (a.batch + TM - 1) / TM, nt = (a.rows + a.tn - 1) / a.tn, tiles = mt * nt;
   const uint32_t ksteps = (a.cols + GK - 1) / GK;
+  const uint32_t first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;  // this CTA's (pair's) tiles
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&S.tmem)), "r"(a.tmem_cols)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&S.tmem)), "r"(a.tmem_cols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_addr(&S.tmem)), "r"(a.tmem_cols)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
   }
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < a.stages; ++s) {
@@ -114,59 +173,80 @@ __global__ void __launch_bounds__(GTHREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_addr(&S.tfull[b]), 1);
-      mbar_init(smem_addr(&S.tempty[b]), 128);
+      mbar_init(smem_addr(&S.tempty[b]), 128 * CTAS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     S.abort_flag = 0;
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // the other CTA's barriers are there
   tc_fence_after();
   const uint32_t tmem = S.tmem;
   bool ok = true;
 
   if (warp == 0) {
     if (lane == 0) {
-      uint32_t n = 0;  // slices loaded
-      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const uint32_t m0 = t % mt * GM, n0 = t / mt * a.tn;
+      // stage and round of the next slice, stepped along: a division a slice
+      // would take this thread longer than the MMAs
+      uint32_t n = 0, s = 0, round = 0;
+      for (uint32_t t = first; t < tiles && ok; t += stride) {
+        const uint32_t m0 = t % mt * TM + rank * GM, n0 = t / mt * a.tn + rank * bn;
         for (uint32_t k = 0; k < ksteps; ++k, ++n) {
-          const uint32_t s = n % a.stages, bar = smem_addr(&S.full[s]);
-          ok = wait_or_abort(smem_addr(&S.empty[s]), ((n / a.stages) & 1) ^ 1, &S.abort_flag);
-          if (!ok) break;
           const uint32_t dst = smem_addr(ring) + s * stage_bytes;
-          expect_bytes(bar, stage_bytes);
-          tma_load(dst, &mx, k * GK, m0, bar);
-          tma_load(dst + kABytes, &mw, k * GK, n0, bar);
+          ok = wait_or_abort(smem_addr(&S.empty[s]), (round & 1) ^ 1, &S.abort_flag);
+          if (!ok) break;
+          // the first CTA's barrier counts both CTAs' bytes (the second's may
+          // come before it is armed: its phase waits for the arming)
+          if (rank == 0) expect_bytes(smem_addr(&S.full[s]), CTAS * stage_bytes);
+          if (PAIR) {
+            const uint32_t bar = in_cta(smem_addr(&S.full[s]), 0);
+            tma_load_pair(dst, &mx, k * GK, m0, bar);
+            tma_load_pair(dst + kABytes, &mw, k * GK, n0, bar);
+          } else {
+            const uint32_t bar = smem_addr(&S.full[s]);
+            tma_load(dst, &mx, k * GK, m0, bar);
+            tma_load(dst + kABytes, &mw, k * GK, n0, bar);
+          }
+          if (++s == a.stages) {
+            s = 0;
+            ++round;
+          }
         }
       }
       if (!ok) S.abort_flag = 1;
-      // every copy has landed before the CTA ends
-      for (uint32_t i = n > a.stages ? n - a.stages : 0; i < n; ++i)
-        if (!mbar_wait(smem_addr(&S.full[i % a.stages]), (i / a.stages) & 1)) ok = false;
+      // every copy has landed before the CTA (the pair) ends
+      if (rank == 0)
+        for (uint32_t i = n > a.stages ? n - a.stages : 0; i < n; ++i)
+          if (!mbar_wait(smem_addr(&S.full[i % a.stages]), (i / a.stages) & 1)) ok = false;
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_bf16(GM, a.tn);
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = umma_idesc_bf16(TM, a.tn);
       uint32_t n = 0, ti = 0;  // slices multiplied, tiles begun
-      for (uint32_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++ti) {
+      uint32_t s = 0, round = 0;
+      const uint64_t desc0 = desc_sw128(smem_addr(ring));
+      for (uint32_t t = first; t < tiles && ok; t += stride, ++ti) {
         const uint32_t buf = ti & 1, d = tmem + buf * (a.tmem_cols / 2);
         ok = wait_or_abort(smem_addr(&S.tempty[buf]), ((ti >> 1) & 1) ^ 1, &S.abort_flag);
         if (!ok) break;
         tc_fence_after();
         for (uint32_t k = 0; k < ksteps; ++k, ++n) {
-          const uint32_t s = n % a.stages;
-          ok = wait_or_abort(smem_addr(&S.full[s]), (n / a.stages) & 1, &S.abort_flag);
+          ok = wait_or_abort(smem_addr(&S.full[s]), round & 1, &S.abort_flag);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t src = smem_addr(ring) + s * stage_bytes;
-          const uint64_t da = desc_sw128(src), db = desc_sw128(src + kABytes);
+          // (addresses below 256 KB: a descriptor's address field does not overflow)
+          const uint64_t da = desc0 + ((s * stage_bytes) >> 4), db = da + (kABytes >> 4);
 #pragma unroll
           for (uint32_t j = 0; j < GK / 16; ++j)  // 32 bytes further along the rows
-            umma_bf16(d, da + 2 * j, db + 2 * j, idesc, (k | j) != 0);
-          umma_commit(smem_addr(&S.empty[s]));
+            mma_f16<PAIR>(d, da + 2 * j, db + 2 * j, idesc, (k | j) != 0);
+          commit<PAIR>(smem_addr(&S.empty[s]));
+          if (++s == a.stages) {
+            s = 0;
+            ++round;
+          }
         }
-        if (ok) umma_commit(smem_addr(&S.tfull[buf]));
+        if (ok) commit<PAIR>(smem_addr(&S.tfull[buf]));
       }
       if (!ok) S.abort_flag = 1;
       // the MMAs issued are done before TMEM is freed: they complete in
@@ -174,10 +254,10 @@ __global__ void __launch_bounds__(GTHREADS, 1)
       if (n && !mbar_wait(smem_addr(&S.empty[(n - 1) % a.stages]), ((n - 1) / a.stages) & 1)) ok = false;
     }
   } else {
-    const uint32_t quarter = warp & 3, ti0 = quarter * 32;  // this warp's TMEM lanes
+    const uint32_t ti0 = (warp & 3) * 32;  // this warp's TMEM lanes
     uint32_t ti = 0;
-    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x, ++ti) {
-      const uint32_t m0 = t % mt * GM, n0 = t / mt * a.tn, buf = ti & 1;
+    for (uint32_t t = first; t < tiles; t += stride, ++ti) {
+      const uint32_t m0 = t % mt * TM + rank * GM, n0 = t / mt * a.tn, buf = ti & 1;
       ok = wait_or_abort(smem_addr(&S.tfull[buf]), (ti >> 1) & 1, &S.abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -198,16 +278,23 @@ __global__ void __launch_bounds__(GTHREADS, 1)
         }
       }
       tc_fence_before();
-      mbar_arrive(smem_addr(&S.tempty[buf]));
+      if (PAIR)
+        arrive_cluster(in_cta(smem_addr(&S.tempty[buf]), 0));
+      else
+        mbar_arrive(smem_addr(&S.tempty[buf]));
     }
     if (!ok) S.abort_flag = 1;
   }
   if (!ok && lane == 0) atomicOr(a.status, kStatusInternal);
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // neither CTA ends (or frees TMEM) while the other's work needs it
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+    if (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(a.tmem_cols) : "memory");
   }
 }
 
@@ -221,21 +308,31 @@ __global__ void linear_rows_kernel(const uint16_t* __restrict__ x, uint64_t stri
   }
 }
 
-// Weight rows of a tile: the multiple of 16 whose waves of tiles cost least,
-// a tile costing its products (tn) and a fixed part of about 32 rows' worth
-// (its slices of x, its start and epilogue).
-uint32_t gemm_tile(uint32_t batch, uint32_t rows, int sms) {
-  const uint64_t mt = (batch + GM - 1) / GM;
-  uint64_t best = ~uint64_t(0);
-  uint32_t tn = 256;
-  for (uint32_t n = 256; n >= 32; n -= 16) {
-    const uint64_t waves = (mt * ((rows + n - 1) / n) + sms - 1) / sms, cost = waves * (n + 32);
-    if (cost < best) {
-      best = cost;
-      tn = n;
+// Tile and pairing: the waves of tiles, each slice of a tile costing the
+// slower of its products (2 tn clocks) and its copies (64 bytes a clock), a
+// tile 2000 clocks besides (start and epilogue).
+struct GemmPlan {
+  bool pair;
+  uint32_t tn;
+};
+GemmPlan gemm_plan(uint32_t batch, uint32_t rows, uint32_t cols, int sms) {
+  GemmPlan best{false, 256};
+  uint64_t least = ~uint64_t(0);
+  for (const bool pair : {false, true}) {
+    const uint32_t ctas = pair ? 2 : 1;
+    const uint64_t mt = (batch + GM * ctas - 1) / (GM * ctas);
+    // the MMA's N: steps of 16, of 32 for a pair
+    for (uint32_t n = 256; n >= 32; n -= 16 * ctas) {
+      const uint64_t tiles = mt * ((rows + n - 1) / n), waves = (tiles * ctas + sms - 1) / sms;
+      const uint64_t slice = std::max<uint64_t>(2 * n, (kABytes + n / ctas * GK * 2) / 64);
+      const uint64_t cost = waves * (slice * ((cols + GK - 1) / GK) + 2000);
+      if (cost < least) {
+        least = cost;
+        best = GemmPlan{pair, n};
+      }
     }
   }
-  return tn;
+  return best;
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -288,21 +385,34 @@ cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, cons
   a.rows = rows;
   a.cols = cols;
   a.status = status;
-  a.tn = gemm_tile(batch, rows, sms);
-  const uint32_t stage = kABytes + a.tn * GK * 2;
+  const GemmPlan plan = gemm_plan(batch, rows, cols, sms);
+  const uint32_t ctas = plan.pair ? 2 : 1;
+  a.tn = plan.tn;
+  const uint32_t stage = kABytes + a.tn / ctas * GK * 2;
   a.stages = std::min<uint32_t>(kMaxStages, uint32_t(kRing / stage));
   a.tmem_cols = 32;
   while (a.tmem_cols < 2 * ((a.tn + 31) / 32 * 32)) a.tmem_cols *= 2;
   CUtensorMap mx, mw;
-  if (!tensor_map(&mx, x, batch, cols, x_pitch, GM) || !tensor_map(&mw, w, rows, cols, cols, a.tn)) return cudaErrorInvalidValue;
+  if (!tensor_map(&mx, x, batch, cols, x_pitch, GM) || !tensor_map(&mw, w, rows, cols, cols, a.tn / ctas)) return cudaErrorInvalidValue;
   const size_t smem = size_t(a.stages) * stage + 1024;
   // one CTA an SM, whatever the tile: its TMEM columns are its own
   const size_t ask = std::max<size_t>(smem, 120 * 1024);
-  const cudaError_t err = cudaFuncSetAttribute(linear_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRing + 1024));
+  auto kernel = plan.pair ? linear_gemm_kernel<true> : linear_gemm_kernel<false>;
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRing + 1024));
   if (err != cudaSuccess) return err;
-  const uint64_t tiles = uint64_t((batch + GM - 1) / GM) * ((rows + a.tn - 1) / a.tn);
-  linear_gemm_kernel<<<uint32_t(std::min<uint64_t>(tiles, uint64_t(sms))), GTHREADS, ask, st>>>(mx, mw, a);
-  return cudaGetLastError();
+  const uint64_t tiles = uint64_t((batch + GM * ctas - 1) / (GM * ctas)) * ((rows + a.tn - 1) / a.tn);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(uint32_t(std::min<uint64_t>(tiles, uint64_t(sms) / ctas)) * ctas);
+  cfg.blockDim = dim3(GTHREADS);
+  cfg.dynamicSmemBytes = ask;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, mx, mw, a);
 }
 
 }  // namespace xksv
