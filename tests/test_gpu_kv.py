@@ -257,7 +257,7 @@ def test_attend_lengths_and_types(lens, kind, cache):
 
 
 @pytest.mark.parametrize("Q,H,D", [(1, 1, 64), (7, 7, 80), (12, 2, 96), (32, 8, 128), (24, 1, 64), (40, 2, 256),
-                                   (6, 3, 192), (9, 3, 16), (130, 2, 32), (3, 1, 144)])
+                                   (6, 3, 192), (9, 3, 16), (130, 2, 32), (3, 1, 144), (17, 1, 48)])
 @pytest.mark.parametrize("page,layout,cache", [(16, "nhd", "bf16"), (1, "hnd", "e4m3"), (48, "hnd", "bf16"), (7, "nhd", "e4m3"),
                                                (256, "nhd", "bf16")])
 def test_attend_heads_and_pages(Q, H, D, page, layout, cache):
@@ -373,6 +373,65 @@ def test_append_then_attend_in_a_graph():
         assert ((q.double() - turned).abs() <= half_step("bf16", turned) + 2.0 ** -20 * mag).all()
         want, _, tol, _ = attend64(q, k.double(), v.double(), [s + i + 1 for s in start], table, page, D ** -0.5)
         assert ((out.double() - want).abs() <= half_step("bf16", want) + tol).all()
+    assert c.status() == 0
+    c.close()
+
+
+def test_offsets_past_32_bits():
+    """Pages whose offsets pass 2^32 bytes and 2^31 elements: append and attend
+    at the far end of a 5.6 GB buffer."""
+    g = gen(14)
+    page, D, step, pages = 16, 64, 1 << 20, 2700  # a page every 2 MB
+    k, v = (torch.empty(pages * step, dtype=torch.bfloat16, device=DEV).as_strided((pages, page, 1, D), (step, D, D, 1))
+            for _ in range(2))
+    c = xg.KVCache(k, v)
+    table = torch.tensor([[2699, 5, 2600]], dtype=torch.int32, device=DEV)
+    n = 40
+    kn, vn = (torch.randn(n, 1, D, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    index = torch.arange(n, dtype=torch.int32, device=DEV)
+    c.append(kn, vn, table, index, seq=torch.zeros_like(index))
+    rows = table[0, index.long() // page].long()
+    assert torch.equal(k[rows, index.long() % page], kn) and torch.equal(v[rows, index.long() % page], vn)
+    q = torch.randn(1, 3, D, generator=g, device=DEV).to(torch.bfloat16)
+    out = torch.empty_like(q)
+    c.attend(q, table, torch.tensor([n], dtype=torch.int32, device=DEV), out)
+    want, _, tol, _ = attend64(q, kn.double()[:, None], vn.double()[:, None], [n], torch.arange(n, device=DEV)[None], 1, 0.125)
+    assert ((out.double() - want).abs() <= half_step("bf16", want) + tol).all() and c.status() == 0
+    c.close()
+
+
+def test_calls_on_several_streams():
+    """Two sequences' attention at once on two streams, a call for the default
+    stream made inside a side stream, and a caller's own workspace."""
+    g = gen(15)
+    table, pages = table_of(g, [5000, 3000], 16)
+    k, v, _, _, c = make_cache(g, "bf16", pages, 16, 2, 64, "nhd")
+    q = torch.randn(2, 8, 64, generator=g, device=DEV).to(torch.bfloat16)
+    lens = torch.tensor([5000, 3000], dtype=torch.int32, device=DEV)
+    want, _, tol, _ = attend64(q, k.double(), v.double(), [5000, 3000], table, 16, 0.125)
+    torch.cuda.synchronize()
+    outs = [torch.zeros(1, 8, 64, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                c.attend(q[i:i + 1], table[i:i + 1], lens[i:i + 1], outs[i], stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert ((outs[i].double() - want[i:i + 1]).abs() <= (half_step("bf16", want) + tol)[i:i + 1]).all()
+    out = torch.zeros_like(q)
+    ws = torch.empty(c.attend_workspace(2, 8, table.shape[1]), dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(sides[0]):
+        c.attend(q, table, lens, out)  # the legacy default stream
+        torch.cuda.default_stream().synchronize()
+        first = out.clone()
+        c.attend(q, table, lens, out, workspace=ws, stream=sides[0].cuda_stream)
+    torch.cuda.synchronize()
+    assert ((out.double() - want).abs() <= half_step("bf16", want) + tol).all() and torch.equal(out, first)
+    with pytest.raises(RuntimeError):
+        c.attend(q, table, lens, out, workspace=ws[:256])
     assert c.status() == 0
     c.close()
 

@@ -114,7 +114,7 @@ def test_session_refusals(tmp_path):
     path = archive(tmp_path, "llama")
     s = serve.load_session(path, DEV, pages=4, page_size=16, max_seqs=2, max_tokens=48)
     for bad, match in (([torch.zeros(0, dtype=torch.long)], "empty"), ([[1]] * 3, "too many"), ([[1] * 49], "exceeds"),
-                       ([[1] * 33, [1] * 33], "full")):
+                       ([[1] * 33, [1] * 33], "full"), ([], "empty"), ([[1, 256]], "vocabulary"), ([[-1]], "vocabulary")):
         with pytest.raises(rt.ArchiveError, match=match):
             s.prefill(bad)
         assert len(s.free_pages) == 4 and len(s.free_seqs) == 2
@@ -124,6 +124,10 @@ def test_session_refusals(tmp_path):
                        ([9], "unknown")):
         with pytest.raises(rt.ArchiveError, match=match):
             s.step(bad, [1] * len(bad))
+    for bad, match in (([1, 2], "one token"), ([256], "vocabulary")):
+        with pytest.raises(rt.ArchiveError, match=match):
+            s.step(seqs[1:], bad)
+    assert s.length[seqs[1]] == 16  # refused steps add nothing
     s.release(seqs[:1])
     assert s.step(seqs[1:], [4]).shape == (1, 256)
     with pytest.raises(rt.ArchiveError, match="dtype"):

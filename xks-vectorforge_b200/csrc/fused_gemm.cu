@@ -526,17 +526,9 @@ cudaError_t launch_fused_ctas(const FusedArgs& args, uint32_t nctas, cudaStream_
   size_t smem = 0;
   const uint32_t p = fused_producers(args.npad, &smem);
   if (!p) return cudaErrorInvalidValue;
-  // dynamic shared memory opt-in, once per device (concurrent first calls set the same value)
   static std::atomic<uint64_t> done{0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const uint64_t bit = dev < 64 ? (1ull << dev) : 0ull;
-  if (!bit || !(done.load(std::memory_order_acquire) & bit)) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(fused_gemm_kernel<LIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemLimit));
-    if (e != cudaSuccess) return e;
-    if (bit) done.fetch_or(bit, std::memory_order_release);
-  }
+  const cudaError_t e = opt_in_smem(fused_gemm_kernel<LIN>, kSmemLimit, done);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(nctas);
   cfg.blockDim = dim3((p + 1) * 32);

@@ -1,5 +1,6 @@
 // Launchers for the slab kernels (host side, one per codec and mode).
 #pragma once
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -7,6 +8,19 @@
 #include "xksv_types.h"
 
 namespace xksv {
+
+// Dynamic shared memory opt-in of `kernel`, once per device and call site's
+// `done` (concurrent first calls set the same value).
+template <class K>
+inline cudaError_t opt_in_smem(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess && bit) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 size_t parallel_smem_bytes();
 size_t serial_smem_bytes();

@@ -34,6 +34,7 @@
 
 #include <algorithm>
 
+#include "kernels.h"
 #include "kv_cache.h"
 #include "kv_index.h"
 #include "tcgen05.cuh"
@@ -806,7 +807,8 @@ template <bool MB, bool E8, int DP, int NG, bool FULL>
 cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
   using Sh = Shape<E8, DP, NG>;
   auto kernel = kv_attend_kernel<MB, E8, DP, NG, FULL>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::CTA);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = opt_in_smem(kernel, Sh::CTA, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((pl.warps + kWarps - 1) / kWarps);

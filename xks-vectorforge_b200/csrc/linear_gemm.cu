@@ -398,7 +398,8 @@ cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, cons
   // one CTA an SM, whatever the tile: its TMEM columns are its own
   const size_t ask = std::max<size_t>(smem, 120 * 1024);
   auto kernel = plan.pair ? linear_gemm_kernel<true> : linear_gemm_kernel<false>;
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRing + 1024));
+  static std::atomic<uint64_t> done[2] = {};
+  const cudaError_t err = opt_in_smem(kernel, kRing + 1024, done[plan.pair]);
   if (err != cudaSuccess) return err;
   const uint64_t tiles = uint64_t((batch + GM * ctas - 1) / (GM * ctas)) * ((rows + a.tn - 1) / a.tn);
   cudaLaunchConfig_t cfg = {};

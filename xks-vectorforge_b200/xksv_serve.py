@@ -140,9 +140,14 @@ class PagedSession:
         """Begins a sequence per prompt (1-D token ids of any length above 0);
         returns (sequences, the logits [n, vocabulary] after each prompt)."""
         import torch
-        prompts = [torch.as_tensor(p, device=self.device).reshape(-1) for p in prompts]
-        if any(p.numel() == 0 for p in prompts):
+        prompts = [torch.as_tensor(p).reshape(-1) for p in prompts]
+        if not prompts or any(p.numel() == 0 for p in prompts):
             fail("empty prompt")
+        for p in prompts:  # (an id outside the vocabulary would fault the embedding)
+            low, high = p.aminmax()
+            if low < 0 or high >= self.config.vocab_size:
+                fail("token id outside the vocabulary")
+        prompts = [p.to(self.device) for p in prompts]
         if len(prompts) > len(self.free_seqs):
             fail("too many sequences")
         seqs = [self.free_seqs.pop() for _ in prompts]
@@ -150,9 +155,13 @@ class PagedSession:
             self.owned[s], self.length[s] = [], 0
         try:
             self._grow({s: p.numel() for s, p in zip(seqs, prompts)})
-        except ValueError:
+            return seqs, self._prefill(seqs, prompts)
+        except Exception:
             self.release(seqs)
             raise
+
+    def _prefill(self, seqs, prompts):
+        import torch
         counts = [p.numel() for p in prompts]
         place = torch.cat([torch.arange(n, device=self.device) for n in counts])
         owner = torch.repeat_interleave(torch.tensor(seqs, device=self.device), torch.tensor(counts, device=self.device))
@@ -175,7 +184,7 @@ class PagedSession:
             last = torch.tensor(counts, device=self.device).cumsum(0) - 1
             logits = self.model.lm_head(self.core.norm(h[last]))
         self._check()
-        return seqs, logits
+        return logits
 
     def _cached(self, c, page, slot, dtype):
         import torch
@@ -197,21 +206,24 @@ class PagedSession:
         return out[0].transpose(0, 1)
 
     def step(self, seqs, tokens):
-        """One more token of each sequence (`tokens` [n]); returns the logits
-        [n, vocabulary] after it."""
+        """One more token of each sequence (`tokens` [n]; ids on the device are
+        taken as they are); returns the logits [n, vocabulary] after it."""
         import torch
         if len(set(seqs)) != len(seqs) or any(s not in self.length for s in seqs):
             fail("step: unknown or repeated sequence")
         if not len(seqs):
             fail("step: no sequence")
+        tokens = torch.as_tensor(tokens).reshape(-1)
+        if tokens.numel() != len(seqs):
+            fail("step: one token per sequence")
+        if not tokens.is_cuda and (tokens.min() < 0 or tokens.max() >= self.config.vocab_size):
+            fail("token id outside the vocabulary")
         self._grow({s: self.length[s] + 1 for s in seqs})
         with torch.no_grad(), torch.cuda.device(self.device):
             rows = torch.tensor(seqs, device=self.device)
             lens = torch.tensor([self.length[s] for s in seqs], dtype=torch.int32, device=self.device)
             table, index = self.table[rows], lens - 1
-            h = self.core.embed_tokens(torch.as_tensor(tokens, device=self.device).reshape(-1))
-            if h.shape[0] != len(seqs):
-                fail("step: one token per sequence")
+            h = self.core.embed_tokens(tokens.to(self.device))
             stream = self._stream()
             for layer, cache, window in zip(self.layers, self.caches, self.windows):
                 q, k, v = self._project(layer, h)
