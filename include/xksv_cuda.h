@@ -165,6 +165,10 @@ int xksv_plan_launches(const xksv_plan* plan);
  * the same d_payload pointer decode those slabs tile-parallel (one or two
  * threads per tile) instead of re-synchronising each slab's single bit
  * stream on every call.
+ * Of the plan's parallel-codec slabs, when they are too few to fill the GPU
+ * with one warp each, it records where parts of their substreams begin (4
+ * bytes per 128 or more codes), so that a decode shares each slab among
+ * several warps.
  * The index describes the payload's contents at this call: rebuild it if they
  * change.  No reference counterpart (the reference decodes every slab from
  * its first bit, cuda/decode.cu:12-45); it is an acceleration structure on

@@ -1,0 +1,97 @@
+"""GPU: the part index of parallel-codec slabs (xksv_plan_index on plans of few
+slabs) and the ragged serial decode: decoded bytes against the source words,
+bit for bit, over shapes whose substreams begin and end anywhere, codebooks of
+every kind, odd payload offsets, and streams changed after the index."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import xksv_gpu as xg  # noqa: E402
+from helpers import words_for  # noqa: E402
+
+DEV = "cuda:0"
+
+
+def slabs(shapes, codec, kind, seed, lead=5):
+    rng = np.random.default_rng(seed)
+    payload, entries, words, dst = bytearray(b"\0" * lead), [], [], 0
+    for rows, cols in shapes:
+        w = words_for(kind, rows * cols, rng).astype("<u2")
+        blob = xg.host_pack(w.tobytes(), rows, cols, codec)
+        entries.append(dict(src_offset=len(payload), src_size=len(blob), rows=rows, cols=cols, dst_offset=dst, codec=codec))
+        payload += blob + b"\x5a"
+        words.append(w)
+        dst += rows * cols * 2
+    return torch.frombuffer(payload, dtype=torch.uint8).to(DEV), entries, np.concatenate(words)
+
+
+# whole rows, odd numbers of tiles, ragged last tiles, few rows, and substreams too short for a second part
+SHAPES = [[(16, 8192)], [(16, 4112), (16, 2064)], [(16, 1848)] * 5, [(7, 3000), (16, 13000), (1, 9000)],
+          [(16, 40), (3, 5), (16, 9000)], [(16, 28672)] * 3]
+
+
+@pytest.mark.parametrize("shapes", SHAPES)
+@pytest.mark.parametrize("kind", ["normal002", "student3", "uniform", "three_exp", "single"])
+def test_parallel_parts_decode_the_same_bytes(shapes, kind):
+    payload, entries, want = slabs(shapes, xg.CODEC_PARALLEL32, kind, len(shapes))
+    plan = xg.Plan(entries)
+    for shift in (0, 2):  # 32-byte aligned output, and not
+        for indexed in (False, True):
+            if indexed:
+                assert plan.index(payload) == 0
+            out = torch.full((want.size * 2 + 8,), 0xEE, dtype=torch.uint8, device=DEV)
+            plan.decode(payload, out[shift:])
+            assert plan.status() == 0
+            got = out.cpu().numpy()
+            assert (got[shift:shift + want.size * 2].view("<u2") == want).all()
+            assert (got[shift + want.size * 2:] == 0xEE).all() and (got[:shift] == 0xEE).all()
+    plan.close()
+
+
+def test_parallel_parts_report_a_changed_stream():
+    payload, entries, want = slabs([(16, 8192)], xg.CODEC_PARALLEL32, "normal002", 3)
+    plan = xg.Plan(entries)
+    assert plan.index(payload) == 0
+    out = torch.empty(want.size * 2, dtype=torch.uint8, device=DEV)
+    good = payload.clone()
+    # bits of the last substream's end, its bit count, a code length, the container's magic
+    e = entries[0]
+    seg = e["src_offset"] + 32 + 8 * 32
+    for at in (e["src_offset"] + e["src_size"] - 40, seg + 8, seg + 16 + 120, e["src_offset"]):
+        payload.copy_(good)
+        payload[at:at + 4] ^= 0x55
+        plan.decode(payload, out)
+        bad = plan.status()
+        same = bool((out.cpu().numpy().view("<u2") == want).all())
+        assert bad == 1 or same, at
+    payload.copy_(good)
+    plan.decode(payload, out)
+    assert plan.status() == 0 and (out.cpu().numpy().view("<u2") == want).all()
+    plan.close()
+
+
+def test_index_of_a_bad_parallel_slab_leaves_the_decode_to_report_it():
+    payload, entries, want = slabs([(16, 8192)], xg.CODEC_PARALLEL32, "normal002", 4)
+    payload[entries[0]["src_offset"] + 32 + 8 * 32 + 8] ^= 1
+    plan = xg.Plan(entries)
+    assert plan.index(payload) == 0 and plan.status() == 0
+    plan.decode(payload, torch.empty(want.size * 2, dtype=torch.uint8, device=DEV))
+    assert plan.status() == 1
+    plan.close()
+
+
+@pytest.mark.parametrize("shapes", [[(14, 11104)], [(16, 1848)] * 3, [(5, 17), (16, 33), (1, 1), (9, 4096)], [(40, 200)]])
+@pytest.mark.parametrize("kind", ["normal002", "uniform", "single"])
+def test_ragged_serial_slabs_decode(shapes, kind):
+    payload, entries, want = slabs(shapes, xg.CODEC_TILE16, kind, len(shapes))
+    plan = xg.Plan(entries)
+    for indexed in (False, True):
+        if indexed:
+            assert plan.index(payload) == 0
+        out = torch.zeros(want.size * 2, dtype=torch.uint8, device=DEV)
+        plan.decode(payload, out)
+        assert plan.status() == 0
+        assert (out.cpu().numpy().view("<u2") == want).all()
+    plan.close()

@@ -152,7 +152,7 @@ int run_single(Kind kind, const void* input, size_t size, uint64_t rows, uint64_
   cudaError_t e = cudaSuccess;
   if (!gemm) {
     e = kind == Kind::Serial
-            ? launch_serial_decode(c->d_slab, 1, payload, static_cast<uint8_t*>(output), c->d_status, 1, st)
+            ? launch_serial_decode(c->d_slab, 1, payload, static_cast<uint8_t*>(output), c->d_status, 1, st, serial_whole(rows, cols))
             : launch_parallel_decode(c->d_slab, 1, payload, static_cast<uint8_t*>(output), c->d_status, 1, st,
                                      parallel_whole(rows, cols));
   } else {
@@ -222,6 +222,9 @@ struct xksv_plan {
   xksv::FusedGroup* d_fgroups = nullptr;
   uint32_t* d_fmembers = nullptr;
   void* d_ftabs = nullptr;  // per group: its lane tables, built with the index
+  // part index of the parallel slabs (xksv_plan_index of few slabs)
+  uint32_t par_parts = 1;
+  uint32_t* d_ppos = nullptr;
   uint32_t n_fgroups = 0, n_fsegs = 0;
   uint32_t* d_fgsegs = nullptr;  // group g's segments: entries [e[g], e[g + 1]) behind the n_fgroups + 1 first
   uint64_t* d_hash_ranges = nullptr;  // per slab in creation order: {dst, decoded bytes}
@@ -253,6 +256,9 @@ void free_index(xksv_plan* p) {
   if (p->d_fmembers) cudaFree(p->d_fmembers);
   if (p->d_ftabs) cudaFree(p->d_ftabs);
   if (p->d_fgsegs) cudaFree(p->d_fgsegs);
+  if (p->d_ppos) cudaFree(p->d_ppos);
+  p->d_ppos = nullptr;
+  p->par_parts = 1;
   p->d_fgsegs = nullptr;
   p->d_ftabs = nullptr;
   p->d_fseg0 = nullptr;
@@ -668,6 +674,14 @@ void xksv_plan_destroy(xksv_plan* p) {
 }
 
 namespace {
+// Decode of the plan's parallel slabs to out + slab dst, by parts where the
+// payload's index has them.
+cudaError_t parallel_decode(xksv_plan* p, const xksv::Slab* slabs, const uint8_t* pay, uint8_t* out, cudaStream_t st) {
+  if (p->d_ppos && pay == p->indexed_payload)
+    return xksv::launch_parallel_parts(slabs, p->n_par, pay, out, p->d_ppos, p->par_parts, p->d_status, p->par_whole, st);
+  return xksv::launch_parallel_decode(slabs, p->n_par, pay, out, p->d_status, p->grid_par, st, p->par_whole);
+}
+
 // Indexed decode of the plan's 16-row serial slabs (slabs[0, n_ser_idx)) to
 // out + slab dst; the caller decodes the remaining serial slabs.
 cudaError_t tile_decode(xksv_plan* p, const xksv::Slab* slabs, const uint8_t* pay, uint8_t* out,
@@ -707,11 +721,12 @@ int xksv_plan_decode(const xksv_plan* pc, const void* d_payload, size_t payload_
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_ser > ser0) {
-    e = launch_serial_decode(p->d_slabs + ser0, p->n_ser - ser0, pay, out, p->d_status, p->grid_ser, st);
+    e = launch_serial_decode(p->d_slabs + ser0, p->n_ser - ser0, pay, out, p->d_status, p->grid_ser, st,
+                             p->n_ser == p->n_ser_idx);
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_par) {
-    e = launch_parallel_decode(p->d_slabs + p->n_ser, p->n_par, pay, out, p->d_status, p->grid_par, st, p->par_whole);
+    e = parallel_decode(p, p->d_slabs + p->n_ser, pay, out, st);
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_raw) {
@@ -792,7 +807,7 @@ int xksv_plan_decode_host(const xksv_plan* pc, const void* h_payload, size_t pay
     e = cudaStreamWaitEvent(st, p->chunk_ev[c], 0);
     for (int g = 0; g < 2 && e == cudaSuccess; ++g)
       if (upto[g] > done[g]) {
-        e = launch_serial_decode(p->d_slabs + done[g], upto[g] - done[g], pay, out, p->d_status, p->grid_ser, st);
+        e = launch_serial_decode(p->d_slabs + done[g], upto[g] - done[g], pay, out, p->d_status, p->grid_ser, st, g == 0);
         ++p->launches;
       }
     if (e == cudaSuccess && upto[2] > done[2]) {
@@ -828,12 +843,11 @@ cudaError_t decode_scratch(xksv_plan* p, const uint8_t* pay, uint8_t* scratch, c
   }
   if (e == cudaSuccess && p->n_ser > tser0) {
     e = launch_serial_decode(p->d_tc_slabs + tser0, p->n_ser - tser0, pay, scratch, p->d_status,
-                             p->grid_ser, st);
+                             p->grid_ser, st, p->n_ser == p->n_ser_idx);
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_par) {
-    e = launch_parallel_decode(p->d_tc_slabs + p->n_ser, p->n_par, pay, scratch, p->d_status,
-                               p->grid_par, st, p->par_whole);
+    e = parallel_decode(p, p->d_tc_slabs + p->n_ser, pay, scratch, st);
     ++p->launches;
   }
   if (e == cudaSuccess && p->n_raw) {
@@ -996,8 +1010,8 @@ struct Carve {
 constexpr uint64_t pitch_of(uint64_t cols) { return (cols + 7) / 8 * 8; }
 // How a call runs: every slab indexed and up to three tokens (the tile kernel
 // with its epilogue), up to 128 (the fused kernel with its epilogue), decoded
-// weights and the tensor-core product (from four tokens), or any plan's
-// product between two layout changes.
+// weights and the tensor-core product, or, where columns or X offsets are no
+// multiples of 8, any plan's product between two layout changes.
 enum class Route { Tile, Fused, Gemm, Any };
 struct LinearSpace {
   Route route;
@@ -1015,7 +1029,7 @@ LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload
     s.route = Route::Fused;
     s.z = c.take(uint64_t(p->n_fsegs) * 16 * ((batch + 15) / 16 * 16) * 32 * sizeof(float));
     s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
-  } else if (p->tc_ok && batch >= 4) {
+  } else if (p->tc_ok) {
     s.route = Route::Gemm;
     s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
     s.scratch = c.take(p->scratch_bytes);
@@ -1290,6 +1304,31 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   p->fused_ok = true;
 }
 
+// After an index: the part index of the parallel slabs, for plans of too few
+// to fill the GPU with one warp each.  Any failure here (a bad slab too: a
+// decode reports it) only leaves the parts off.
+static void setup_parts(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st) {
+  uint64_t most = 0;
+  for (uint32_t i = p->n_ser; i < p->n_ser + p->n_par; ++i) most = std::max(most, p->h_slabs[i].rows * p->h_slabs[i].cols);
+  const uint32_t parts = parallel_parts(most, p->n_par, p->sms);
+  if (parts < 2) return;
+  const size_t bytes = size_t(p->n_par) * parts * 32 * sizeof(uint32_t);
+  const bool ok = cudaMalloc(&p->d_ppos, bytes) == cudaSuccess && cudaMemsetAsync(p->d_ppos, 0, bytes, st) == cudaSuccess &&
+                  cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
+                  launch_parallel_index(p->d_slabs + p->n_ser, p->n_par, d_payload, p->d_ppos, parts, p->d_status, st) ==
+                      cudaSuccess &&
+                  cudaMemcpyAsync(p->h_status, p->d_status, sizeof(int), cudaMemcpyDeviceToHost, st) == cudaSuccess &&
+                  cudaStreamSynchronize(st) == cudaSuccess && *p->h_status == 0;
+  cudaMemsetAsync(p->d_status, 0, sizeof(int), st);
+  cudaStreamSynchronize(st);
+  if (ok) {
+    p->par_parts = parts;
+    return;
+  }
+  if (p->d_ppos) cudaFree(p->d_ppos);
+  p->d_ppos = nullptr;
+}
+
 int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, void* stream) {
   if (!p || !d_payload || p->need_payload > payload_size) return 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -1298,6 +1337,7 @@ int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, vo
   const uint32_t n = p->n_ser_idx;
   if (!n) {
     p->indexed_payload = d_payload;
+    setup_parts(p, static_cast<const uint8_t*>(d_payload), st);
     return 0;
   }
   const std::vector<Slab>& sl = p->h_slabs;
@@ -1350,6 +1390,7 @@ int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, vo
   p->n_items = uint32_t(items.size());
   p->indexed_payload = d_payload;
   setup_fused(p, static_cast<const uint8_t*>(d_payload), st);
+  setup_parts(p, static_cast<const uint8_t*>(d_payload), st);
   return 0;
 }
 

@@ -60,7 +60,7 @@ extern "C" int xksv_cuda_decode_noalloc(const xksv_slab* slabs, size_t n, const 
   Slab* d_tab = reinterpret_cast<Slab*>(base + kNoallocStatusBytes);
   // group by codec into the host buffer: serial | parallel | raw
   uint32_t counts[3] = {0, 0, 0};
-  bool whole = true;
+  bool whole = true, ser_whole = true;
   for (size_t i = 0; i < n; ++i) {
     const xksv_slab& s = slabs[i];
     if (s.flags || s.codec > XKSV_CODEC_PARALLEL32) return 1;
@@ -73,6 +73,7 @@ extern "C" int xksv_cuda_decode_noalloc(const xksv_slab* slabs, size_t n, const 
     if (s.codec != XKSV_CODEC_RAW && s.cols > kMax / 2 / s.rows) return 1;
     const uint64_t dec = s.codec == XKSV_CODEC_RAW ? s.src_size : s.rows * s.cols * 2;
     if (s.dst_offset > kMax - dec || s.dst_offset + dec > out_size) return 1;
+    if (s.codec == XKSV_CODEC_TILE16) ser_whole = ser_whole && serial_whole(s.rows, s.cols);
     if (s.codec == XKSV_CODEC_PARALLEL32) whole = whole && parallel_whole(s.rows, s.cols);
     ++counts[s.codec == XKSV_CODEC_TILE16 ? 0 : s.codec == XKSV_CODEC_PARALLEL32 ? 1 : 2];
   }
@@ -89,7 +90,7 @@ extern "C" int xksv_cuda_decode_noalloc(const xksv_slab* slabs, size_t n, const 
   const uint8_t* pay = static_cast<const uint8_t*>(d_payload);
   uint8_t* out = static_cast<uint8_t*>(d_out);
   const int grid = 1 << 30;
-  cudaError_t e = launch_serial_decode(d_tab, counts[0], pay, out, d_status, grid, st);
+  cudaError_t e = launch_serial_decode(d_tab, counts[0], pay, out, d_status, grid, st, ser_whole);
   if (e == cudaSuccess) e = launch_parallel_decode(d_tab + counts[0], counts[1], pay, out, d_status, grid, st, whole);
   if (e == cudaSuccess) e = launch_raw_decode(d_tab + counts[0] + counts[1], counts[2], pay, out, grid, st);
   if (e != cudaSuccess) return 1;

@@ -41,6 +41,7 @@
 // table memory, idle until the tables are filled) and its first sign/mantissa
 // chunks.  A warp that goes on to another slab (grids smaller than the slab
 // count) prefetches that slab's headers and length tables into L2 meanwhile.
+#include <algorithm>
 #include <atomic>
 
 #include "kernels.h"
@@ -91,7 +92,19 @@ struct Seg {
   uint32_t start;  // packed index of the substream's first element
   uint64_t nbits;
   uint64_t ebytes;
+  uint64_t room;   // bytes of the substream from sm on
 };
+
+// A part of every substream of a slab: sixteen-code groups [part * per,
+// (part + 1) * per) of each, the last part with what follows.
+struct PartIndex {
+  uint32_t* pos;   // [slab][part][lane]: bit offset of the part's first code (part 0: not stored)
+  uint32_t parts;  // of every slab
+};
+__device__ __forceinline__ uint32_t groups_per_part(uint32_t total, uint32_t chunks, uint32_t parts) {
+  const uint32_t most = (total + chunks - 1) / chunks / 16;
+  return max(1u, (most + parts - 1) / parts);
+}
 
 struct Out {
   uint16_t* out;   // decode: slab output
@@ -115,35 +128,12 @@ __device__ __forceinline__ void emit_one(const Out& o, uint32_t p, uint32_t word
   }
 }
 
-// A slab's elements in packed order: 16-column tiles (the last one w wide) of
-// the slab's rows (at most 16), row-major inside.
-struct Walk {
-  uint32_t rows, cols, t0, w, r, c;
-  __device__ __forceinline__ Walk(uint32_t p, uint32_t rows_, uint32_t cols_) : rows(rows_), cols(cols_) {
-    const uint32_t t = p / (16 * rows), local = p - t * 16 * rows;
-    t0 = 16 * t;
-    w = cols - t0 < 16 ? cols - t0 : 16;
-    r = local / w;
-    c = local - r * w;
-  }
-  __device__ __forceinline__ uint32_t col() const { return t0 + c; }
-  __device__ __forceinline__ void next() {
-    if (++c < w) return;
-    c = 0;
-    if (++r < rows) return;
-    r = 0;
-    t0 += 16;
-    w = cols - t0 < 16 ? cols - t0 : 16;
-  }
-};
-
 // A substream whose elements do not lie in whole 16-word rows (slabs of
 // other shapes, or a start inside a row): sixteen codes at a time like the
 // whole rows, their places stepped along instead of divided out (16 x 1848
-// slabs, 128 of them: 614 us one code at a time, 130 us so).  Out of line, so that the
-// whole-row loop keeps its registers.
+// slabs, 128 of them: 614 us one code at a time, 130 us so).
 template <int MODE>
-__device__ __noinline__ bool decode_ragged(const Seg s, WarpTabs& W, int lane, const ldec::Code lc, ldec::Stream b, const Out o) {
+__device__ __forceinline__ bool ragged_codes(const Seg s, WarpTabs& W, int lane, const ldec::Code lc, ldec::Stream b, const Out o) {
   bool bad = false;
   Walk at(s.start, o.rows, o.cols);
   auto emit = [&](uint32_t e, uint32_t sm) {
@@ -162,7 +152,7 @@ __device__ __noinline__ bool decode_ragged(const Seg s, WarpTabs& W, int lane, c
   // exponent bits behind them belong to the substream too)
   const uint32_t* words = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(s.sm) & ~uintptr_t(3));
   const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(s.sm) & 3) * 8;
-  for (; i + 16 <= s.count && i + 20 <= s.count + s.ebytes; i += 16) {
+  for (; i + 16 <= s.count && i + 20 <= s.room; i += 16) {
     uint32_t w[5], e[16];
 #pragma unroll
     for (int k = 0; k < 5; ++k) w[k] = __ldg(words + i / 4 + k);
@@ -203,6 +193,32 @@ __device__ __noinline__ bool decode_ragged(const Seg s, WarpTabs& W, int lane, c
   return bad || uint64_t(b.pos - b.pos0) != s.nbits;
 }
 
+// The same out of line, so that the whole-row loop keeps its registers.
+template <int MODE>
+__device__ __noinline__ bool decode_ragged(const Seg s, WarpTabs& W, int lane, const ldec::Code lc, ldec::Stream b, const Out o) {
+  return ragged_codes<MODE>(s, W, lane, lc, b, o);
+}
+
+// Walks one substream's codes and notes where its parts begin (a part behind
+// the last code begins at the end); true when the stream is not what it says.
+__device__ __noinline__ bool index_segment(const Seg s, WarpTabs& W, int lane, const ldec::Code lc, ldec::Stream b,
+                                           uint32_t* pos, uint32_t parts, uint32_t per) {
+  bool bad = false;
+  uint32_t part = 1, i = 0;
+  for (; i + 16 <= s.count; i += 16) {
+    if (part < parts && i == 16 * part * per) pos[32 * part++ + lane] = b.pos - b.pos0;
+    b.maintain(W.ring, lane);
+    uint32_t e[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      ldec::dec4<PCfg>(b, W.ring, W.t, lane, lc, bad, e[4 * k], e[4 * k + 1], e[4 * k + 2], e[4 * k + 3]);
+  }
+  if (part < parts && i < s.count && i == 16 * part * per) pos[32 * part++ + lane] = b.pos - b.pos0;
+  for (; i < s.count; ++i) ldec::dec_one<PCfg>(b, W.ring, W.t, lane, lc, bad);
+  for (; part < parts; ++part) pos[32 * part + lane] = uint32_t(s.nbits);
+  return bad || uint64_t(b.pos - b.pos0) != s.nbits;
+}
+
 // Decodes one substream.  `rows16`: 16-row slab, cols % 16 == 0, the
 // substream starts on a tile row and (decode) the output is 16-byte aligned;
 // whole tile rows then leave as 32-byte stores.  The caller has started `b`
@@ -210,11 +226,11 @@ __device__ __noinline__ bool decode_ragged(const Seg s, WarpTabs& W, int lane, c
 // the ring.
 // `WHOLE`: the caller's slabs all lie in whole rows, so that other substreams
 // (there are none) may go code by code; else decode_ragged takes them.
-template <int MODE, bool WHOLE>
+template <int MODE, bool WHOLE, bool PART>
 __device__ void decode_segment(const Seg& s, WarpTabs& W, int lane, const ldec::Code& lc, bool rows16,
                                ldec::Stream& b, ldec::SmStream& smr, const Out& o, bool& bad) {
   if (!WHOLE && !rows16) {
-    if (decode_ragged<MODE>(s, W, lane, lc, b, o)) bad = true;
+    if (PART ? ragged_codes<MODE>(s, W, lane, lc, b, o) : decode_ragged<MODE>(s, W, lane, lc, b, o)) bad = true;
     return;
   }
   uint32_t i = 0;
@@ -333,18 +349,24 @@ __device__ __forceinline__ uint64_t warp_incl_scan(uint64_t v, int lane) {
   return v;
 }
 
-template <int MODE, bool WHOLE>
+// MODE 0 decodes, 1 multiplies, 2 writes the part index.  PART (MODE 0): the
+// warps share every slab's substreams by parts, for plans of too few slabs to
+// fill the GPU.
+template <int MODE, bool WHOLE, bool PART>
 __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
     parallel_slab_kernel(const Slab* __restrict__ slabs, uint32_t nslabs,
                          const uint8_t* __restrict__ payload, uint8_t* __restrict__ out,
                          const float* __restrict__ x, float* __restrict__ y, uint32_t ld,
-                         uint32_t nb, int* __restrict__ status) {
+                         uint32_t nb, int* __restrict__ status, PartIndex pi) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   WarpTabs& W = reinterpret_cast<WarpTabs*>(smem)[warp];
   float* ysm = MODE == 1 ? reinterpret_cast<float*>(smem + kSmemTabs) + warp * 16 * PMAXB : nullptr;
 
-  for (uint32_t si = blockIdx.x * PWARPS + warp; si < nslabs; si += gridDim.x * PWARPS) {
+  const uint32_t items = PART ? nslabs * pi.parts : nslabs;
+  for (uint32_t wi = blockIdx.x * PWARPS + warp; wi < items; wi += gridDim.x * PWARPS) {
+    const uint32_t si = PART ? wi / pi.parts : wi, part = PART ? wi - si * pi.parts : 0;
+    const bool last_part = !PART || part + 1 == pi.parts;
     const Slab sd = slabs[si];
     const uint8_t* p = payload + sd.src;
     const uint64_t n = sd.size;
@@ -355,7 +377,7 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
     const uint32_t sn = si + gridDim.x * PWARPS;
     const uint8_t* np = nullptr;
     uint64_t nsize = 0, nlen = 0, ntotal = 0;
-    if (sn < nslabs) {
+    if (!PART && sn < nslabs) {
       const Slab nd = slabs[sn];
       np = payload + nd.src;
       nsize = nd.size;
@@ -416,6 +438,18 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
     const bool rows16 = nice && (s.start & 15) == 0;
     ldec::Stream b;
     ldec::SmStream smr;
+    // this part's codes [c0, c1) of the lane's substream and its first bit
+    uint32_t c0 = 0, c1 = uint32_t(expect), bit0 = 0;
+    if (PART) {
+      const uint32_t per = groups_per_part(total, uint32_t(chunks), pi.parts);
+      const uint32_t* pos = pi.pos + uint64_t(si) * pi.parts * 32 + lane;
+      c0 = min(16 * part * per, c1);
+      if (!last_part) c1 = min(16 * (part + 1) * per, c1);
+      if (active && part) bit0 = pos[32 * part];
+      if (active && !last_part) s.nbits = pos[32 * (part + 1)];  // where it ends, until below
+      if (active && lok && c0 > len - kHdr) c0 = c1 = 0;         // (a header the checks below refuse)
+    }
+    const uint32_t part_end = PART && !last_part ? uint32_t(s.nbits) : 0;
     if (active && lok) {
       lok = base + len <= n;
       if (lok) {
@@ -426,8 +460,8 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
         // the slab is well formed; the copies stay inside the slab anyway)
         ldec::stage_lengths<PCfg>(W.t, q + 16, lane);
         if (rows16) {
-          const uint8_t* sm = q + kHdr;
-          const uint8_t* sme = sm + expect <= p + n ? sm + expect : p + n;
+          const uint8_t* sm = q + kHdr + c0;
+          const uint8_t* sme = sm + (expect - c0) <= p + n ? sm + (expect - c0) : p + n;
           smr.init(W.smring, lane, sm, sme > sm ? sme : sm + 1);
         }
         const uint64_t count = ld8_any(q, p + n);
@@ -438,6 +472,7 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
         s.lens = q + 16;
         s.sm = q + kHdr;
         s.bits = q + kHdr + count;
+        s.room = count + s.ebytes;
       }
     }
     cp_async_commit();
@@ -456,8 +491,22 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
       if (lane == 0) atomicOr(status, kStatusInternal);
       continue;
     }
+    const Seg all = s;  // the whole substream
+    bool bad_part = false;
+    if (PART && active) {
+      const uint64_t end = last_part ? s.nbits : part_end;
+      bad_part = bit0 > end || end > s.nbits;  // an index that does not describe this payload
+      if (bad_part) bit0 = 0, c1 = c0;
+      s.start += c0;
+      s.sm += c0;
+      s.room -= c0;
+      s.count = c1 - c0;
+      s.nbits = bad_part ? 0 : end - bit0;
+      s.bits += bit0 >> 3;
+      s.ebytes -= bit0 >> 3;
+    }
     // ---- first bit loads, overlapping the table build ----
-    if (active) b.start(s.bits, s.ebytes);
+    if (active) b.start(s.bits, s.ebytes, PART ? bit0 & 7 : 0);
     // ---- per-lane tables, from the staged lengths ----
     cp_async_wait_all();
     ldec::Code lc{0, 0, 0};
@@ -491,28 +540,34 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
       for (int k = lane; k < 16 * PMAXB; k += 32) ysm[k] = 0.f;
       __syncwarp();
     }
-    bool bad = false;
+    bool bad = bad_part;
     if (active && tb == 0) {
       b.init_ring(W.ring, lane);
       cp_async_wait_all();
-      decode_segment<MODE, WHOLE>(s, W, lane, lc, rows16, b, smr, o, bad);
+      if constexpr (MODE == 2)
+        bad = index_segment(s, W, lane, lc, b, pi.pos + uint64_t(si) * pi.parts * 32, pi.parts,
+                            groups_per_part(total, uint32_t(chunks), pi.parts));
+      else
+        decode_segment<MODE, WHOLE, PART>(s, W, lane, lc, rows16, b, smr, o, bad);
     }
     cp_async_wait_all();
     // ---- substreams that need the generic decoder ----
+    // (whole, by the first part's warp)
     uint32_t gmask = __ballot_sync(0xffffffffu, active && tb == 1);
+    if (MODE == 2 || (PART && part)) gmask = 0;
     __syncwarp();
     while (gmask) {
       const int g = __ffs(gmask) - 1;
       gmask &= gmask - 1;
       Seg sg;
-      sg.lens = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(s.lens), g));
-      sg.sm = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(s.sm), g));
-      sg.bits = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(s.bits), g));
-      sg.count = __shfl_sync(0xffffffffu, s.count, g);
-      sg.start = __shfl_sync(0xffffffffu, s.start, g);
-      sg.nbits = __shfl_sync(0xffffffffu, s.nbits, g);
-      sg.ebytes = __shfl_sync(0xffffffffu, s.ebytes, g);
-      if (lane == 0 && !decode_segment_generic<MODE>(sg, *reinterpret_cast<GenericTab*>(&W.t.lut[0][0]), o))
+      sg.lens = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(all.lens), g));
+      sg.sm = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(all.sm), g));
+      sg.bits = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(all.bits), g));
+      sg.count = __shfl_sync(0xffffffffu, all.count, g);
+      sg.start = __shfl_sync(0xffffffffu, all.start, g);
+      sg.nbits = __shfl_sync(0xffffffffu, all.nbits, g);
+      sg.ebytes = __shfl_sync(0xffffffffu, all.ebytes, g);
+      if (lane == 0 && !decode_segment_generic<MODE == 1 ? 1 : 0>(sg, *reinterpret_cast<GenericTab*>(&W.t.lut[0][0]), o))
         bad = true;
       __syncwarp();
     }
@@ -539,9 +594,12 @@ void set_attr_once() {
   cudaGetDevice(&dev);
   const uint64_t bit = dev < 64 ? (1ull << dev) : 0ull;
   if (bit && (done.load(std::memory_order_acquire) & bit)) return;
-  cudaFuncSetAttribute(parallel_slab_kernel<0, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
-  cudaFuncSetAttribute(parallel_slab_kernel<0, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
-  cudaFuncSetAttribute(parallel_slab_kernel<1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[1]));
+  cudaFuncSetAttribute(parallel_slab_kernel<0, true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
+  cudaFuncSetAttribute(parallel_slab_kernel<0, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
+  cudaFuncSetAttribute(parallel_slab_kernel<0, true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
+  cudaFuncSetAttribute(parallel_slab_kernel<0, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
+  cudaFuncSetAttribute(parallel_slab_kernel<1, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[1]));
+  cudaFuncSetAttribute(parallel_slab_kernel<2, false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmemBytes[0]));
   if (bit) done.fetch_or(bit, std::memory_order_release);
 }
 
@@ -556,11 +614,41 @@ cudaError_t launch_parallel_decode(const Slab* slabs, uint32_t n, const uint8_t*
   const int need = int((n + PWARPS - 1) / PWARPS), g = grid < need ? grid : need;
   // the ragged path costs the whole rows 1.7 % (its call's registers: 8192
   // slabs of 16 x 2048 456 us against 448), hence two kernels
+  const PartIndex none{};
   if (whole)
-    parallel_slab_kernel<0, true><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status);
+    parallel_slab_kernel<0, true, false><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status, none);
   else
-    parallel_slab_kernel<0, false><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status);
+    parallel_slab_kernel<0, false, false><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status, none);
   return cudaGetLastError();
+}
+
+cudaError_t launch_parallel_index(const Slab* slabs, uint32_t n, const uint8_t* payload, uint32_t* pos, uint32_t parts,
+                                  int* status, cudaStream_t st) {
+  if (!n) return cudaSuccess;
+  set_attr_once();
+  parallel_slab_kernel<2, false, false><<<(n + PWARPS - 1) / PWARPS, PWARPS * 32, kSmemBytes[0], st>>>(
+      slabs, n, payload, nullptr, nullptr, nullptr, 1, 1, status, PartIndex{pos, parts});
+  return cudaGetLastError();
+}
+
+cudaError_t launch_parallel_parts(const Slab* slabs, uint32_t n, const uint8_t* payload, uint8_t* out, uint32_t* pos,
+                                  uint32_t parts, int* status, bool whole, cudaStream_t st) {
+  if (!n) return cudaSuccess;
+  set_attr_once();
+  const uint32_t g = (n * parts + PWARPS - 1) / PWARPS;
+  const PartIndex pi{pos, parts};
+  if (whole)
+    parallel_slab_kernel<0, true, true><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status, pi);
+  else
+    parallel_slab_kernel<0, false, true><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status, pi);
+  return cudaGetLastError();
+}
+
+uint32_t parallel_parts(uint64_t max_elements, uint32_t n, int sms) {
+  // a part of 128 codes or more a lane (its warp builds the slab's tables
+  // again, about 300 codes' time), and no more warps than the GPU holds
+  const uint64_t codes = max_elements / 32, fill = n ? uint64_t(sms) * 16 / n : 0;
+  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({fill, codes / 128, 64})));
 }
 
 cudaError_t launch_parallel_gemm(const Slab* slabs, uint32_t n, const uint8_t* payload,
@@ -569,8 +657,8 @@ cudaError_t launch_parallel_gemm(const Slab* slabs, uint32_t n, const uint8_t* p
   if (!n) return cudaSuccess;
   set_attr_once();
   const int need = int((n + PWARPS - 1) / PWARPS);
-  parallel_slab_kernel<1, false><<<grid < need ? grid : need, PWARPS * 32, kSmemBytes[1], st>>>(
-      slabs, n, payload, nullptr, x + b0, y + b0, ld, nb, status);
+  parallel_slab_kernel<1, false, false><<<grid < need ? grid : need, PWARPS * 32, kSmemBytes[1], st>>>(
+      slabs, n, payload, nullptr, x + b0, y + b0, ld, nb, status, PartIndex{});
   return cudaGetLastError();
 }
 

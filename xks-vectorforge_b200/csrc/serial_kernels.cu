@@ -322,7 +322,9 @@ __device__ __forceinline__ void semit_one(const SOut& o, uint32_t p, uint32_t wo
   }
 }
 
-template <int MODE>
+// RAGGED (decode): slabs of other shapes than whole 16 x 16 tiles among them
+// step their elements' places along instead of dividing them out.
+template <int MODE, bool RAGGED = false>
 __global__ void __launch_bounds__(ST, 3) serial_slab_kernel(const Slab* __restrict__ slabs,
                                                          uint32_t nslabs, SerialArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -586,7 +588,32 @@ __global__ void __launch_bounds__(ST, 3) serial_slab_kernel(const Slab* __restri
         bool dead = false;
         uint32_t g = base + my_off;
         const uint32_t gend = g + myN;
-        if (MODE == 0 && o.nice) {
+        if (RAGGED && !o.nice && rows <= 16) {
+          Walk at(g, uint32_t(rows), uint32_t(cols));
+          auto put = [&](uint32_t word) {
+            o.out[size_t(at.r) * cols + at.col()] = uint16_t(word);
+            at.next();
+          };
+          if (g + 8 <= gend) {
+            ByteReader8 smr;
+            smr.init(sm + g, sm + cnt32);
+            for (; g + 8 <= gend; g += 8) {
+              const uint64_t s8 = smr.take();
+              uint32_t e[8];
+              r.refill_to<4 * SK>();
+              code4<7>(S, r, dead, e[0], e[1], e[2], e[3]);
+              r.refill_to<4 * SK>();
+              code4<7>(S, r, dead, e[4], e[5], e[6], e[7]);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) put(merge1(e[q], uint32_t(s8 >> (8 * q)) & 255u));
+            }
+          }
+          for (; g < gend; ++g) {
+            r.refill();
+            const uint32_t e = code1<7>(S, r, dead);
+            put(merge1(e, __ldg(sm + g)));
+          }
+        } else if (MODE == 0 && o.nice) {
           // whole tile rows: 16 codes -> one 32-byte store (two 16-byte
           // stores when the output is only 16-byte aligned)
           for (; g < gend && (g & 15); ++g) {
@@ -1116,6 +1143,7 @@ void serial_set_attr() {
   const uint64_t bit = dev < 64 ? (1ull << dev) : 0ull;
   if (bit && (done.load(std::memory_order_acquire) & bit)) return;
   cudaFuncSetAttribute(serial_slab_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SerialShared)));
+  cudaFuncSetAttribute(serial_slab_kernel<0, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SerialShared)));
   cudaFuncSetAttribute(serial_slab_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SerialShared)));
   cudaFuncSetAttribute(serial_slab_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SerialShared)));
   cudaFuncSetAttribute(serial_tile_gemv_kernel<0, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
@@ -1136,12 +1164,15 @@ void serial_set_attr() {
 size_t serial_smem_bytes() { return sizeof(SerialShared); }
 
 cudaError_t launch_serial_decode(const Slab* slabs, uint32_t n, const uint8_t* payload,
-                                 uint8_t* out, int* status, int grid, cudaStream_t st) {
+                                 uint8_t* out, int* status, int grid, cudaStream_t st, bool whole) {
   if (!n) return cudaSuccess;
   serial_set_attr();
   SerialArgs a{payload, out, nullptr, nullptr, 1, 1, status, nullptr, nullptr};
   const int g = grid < int(n) ? grid : int(n);
-  serial_slab_kernel<0><<<g, ST, sizeof(SerialShared), st>>>(slabs, n, a);
+  if (whole)
+    serial_slab_kernel<0><<<g, ST, sizeof(SerialShared), st>>>(slabs, n, a);
+  else
+    serial_slab_kernel<0, true><<<g, ST, sizeof(SerialShared), st>>>(slabs, n, a);
   return cudaGetLastError();
 }
 

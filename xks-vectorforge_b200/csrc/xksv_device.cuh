@@ -388,6 +388,28 @@ __device__ __forceinline__ uint64_t untile_index(uint64_t p, uint64_t rows, uint
   return (blk * 16 + i) * cols + t * 16 + j;
 }
 
+// A slab's elements in packed order: 16-column tiles (the last one w wide) of
+// the slab's rows (at most 16), row-major inside.
+struct Walk {
+  uint32_t rows, cols, t0, w, r, c;
+  __device__ __forceinline__ Walk(uint32_t p, uint32_t rows_, uint32_t cols_) : rows(rows_), cols(cols_) {
+    const uint32_t t = p / (16 * rows), local = p - t * 16 * rows;
+    t0 = 16 * t;
+    w = cols - t0 < 16 ? cols - t0 : 16;
+    r = local / w;
+    c = local - r * w;
+  }
+  __device__ __forceinline__ uint32_t col() const { return t0 + c; }
+  __device__ __forceinline__ void next() {
+    if (++c < w) return;
+    c = 0;
+    if (++r < rows) return;
+    r = 0;
+    t0 += 16;
+    w = cols - t0 < 16 ? cols - t0 : 16;
+  }
+};
+
 // -------------------------------------------------- generic decoder -------
 // Bit-serial canonical decoding valid for every code length the format
 // allows (1..255).  cnt[l] = number of codes of length l, sorted[] = symbols
