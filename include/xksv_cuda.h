@@ -165,7 +165,8 @@ int xksv_plan_launches(const xksv_plan* plan);
  * the same d_payload pointer decode those slabs tile-parallel (one or two
  * threads per tile) instead of re-synchronising each slab's single bit
  * stream on every call.
- * Of the plan's parallel-codec slabs, when they are too few to fill the GPU
+ * Serial-codec slabs of other shapes up to 16 rows get an index for decoding
+ * (xksv_plan_decode, and layers that decode first).  Of the plan's parallel-codec slabs, when they are too few to fill the GPU
  * with one warp each, it records where parts of their substreams begin (4
  * bytes per 128 or more codes), so that a decode shares each slab among
  * several warps.

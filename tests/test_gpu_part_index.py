@@ -82,7 +82,25 @@ def test_index_of_a_bad_parallel_slab_leaves_the_decode_to_report_it():
     plan.close()
 
 
-@pytest.mark.parametrize("shapes", [[(14, 11104)], [(16, 1848)] * 3, [(5, 17), (16, 33), (1, 1), (9, 4096)], [(40, 200)]])
+def test_ragged_tiles_report_a_changed_stream():
+    payload, entries, want = slabs([(14, 9000), (16, 520)], xg.CODEC_TILE16, "normal002", 6)
+    plan = xg.Plan(entries)
+    assert plan.index(payload) == 0
+    out = torch.empty(want.size * 2, dtype=torch.uint8, device=DEV)
+    bits = entries[0]["src_offset"] + 272 + 14 * 9000
+    good = payload.clone()
+    for at in (bits + 100, entries[0]["src_offset"] + entries[0]["src_size"] - 8):
+        payload.copy_(good)
+        payload[at:at + 6] ^= 0x3C
+        plan.decode(payload, out)
+        assert plan.status() in (0, 1)  # tiles before the change may still read as codes of the right length
+        plan.decode(good, out)          # another payload pointer: without the index
+        assert plan.status() == 0 and (out.cpu().numpy().view("<u2") == want).all()
+    plan.close()
+
+
+@pytest.mark.parametrize("shapes", [[(14, 11104)], [(16, 1848)] * 3, [(5, 17), (16, 33), (1, 1), (9, 4096)], [(40, 200)],
+                                    [(16, 512), (3, 512), (16, 500), (20, 64)], [(1, 30000), (13, 7)]])
 @pytest.mark.parametrize("kind", ["normal002", "uniform", "single"])
 def test_ragged_serial_slabs_decode(shapes, kind):
     payload, entries, want = slabs(shapes, xg.CODEC_TILE16, kind, len(shapes))

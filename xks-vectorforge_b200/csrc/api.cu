@@ -222,6 +222,13 @@ struct xksv_plan {
   xksv::FusedGroup* d_fgroups = nullptr;
   uint32_t* d_fmembers = nullptr;
   void* d_ftabs = nullptr;  // per group: its lane tables, built with the index
+  // tile index of the ragged serial slabs, [n_ser_idx, n_ser_idx + n_ser_rag):
+  // up to 16 rows, not of whole 16 x 16 tiles; decode only (r_items 0: none)
+  uint32_t n_ser_rag = 0, r_items = 0;
+  uint32_t* d_r_tidx = nullptr;
+  uint64_t* d_r_tbase = nullptr;
+  xksv::GemvTabs* d_r_gtabs = nullptr;
+  xksv::GemvItem* d_r_items = nullptr;
   // part index of the parallel slabs (xksv_plan_index of few slabs)
   uint32_t par_parts = 1;
   uint32_t* d_ppos = nullptr;
@@ -242,6 +249,18 @@ struct xksv_plan {
 };
 
 namespace {
+void free_ragged(xksv_plan* p) {
+  if (p->d_r_tidx) cudaFree(p->d_r_tidx);
+  if (p->d_r_tbase) cudaFree(p->d_r_tbase);
+  if (p->d_r_gtabs) cudaFree(p->d_r_gtabs);
+  if (p->d_r_items) cudaFree(p->d_r_items);
+  p->d_r_tidx = nullptr;
+  p->d_r_tbase = nullptr;
+  p->d_r_gtabs = nullptr;
+  p->d_r_items = nullptr;
+  p->r_items = 0;
+}
+
 void free_index(xksv_plan* p) {
   if (p->d_tidx) cudaFree(p->d_tidx);
   if (p->d_tmid) cudaFree(p->d_tmid);
@@ -257,6 +276,7 @@ void free_index(xksv_plan* p) {
   if (p->d_ftabs) cudaFree(p->d_ftabs);
   if (p->d_fgsegs) cudaFree(p->d_fgsegs);
   if (p->d_ppos) cudaFree(p->d_ppos);
+  free_ragged(p);
   p->d_ppos = nullptr;
   p->par_parts = 1;
   p->d_fgsegs = nullptr;
@@ -561,10 +581,13 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
   }
   // indexable serial slabs first (the order of slabs within a codec is free:
   // every slab carries its own output offset)
-  std::stable_partition(ser.begin(), ser.end(), tile_indexable);
+  auto ragged = std::stable_partition(ser.begin(), ser.end(), tile_indexable);
+  auto tall = std::stable_partition(ragged, ser.end(), [](const Slab& s) { return s.rows <= 16 && s.cols < (1ull << 27); });
+  const uint32_t n_rag = uint32_t(tall - ragged);
   auto* p = new xksv_plan();
   cudaGetDevice(&p->device);
-  p->n_ser_idx = uint32_t(std::count_if(ser.begin(), ser.end(), tile_indexable));
+  p->n_ser_idx = uint32_t(ragged - ser.begin());
+  p->n_ser_rag = n_rag;
   int sms = 148;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, p->device);
   // one CTA per slab (per PWARPS slabs for the parallel codec): the block
@@ -682,6 +705,42 @@ cudaError_t parallel_decode(xksv_plan* p, const xksv::Slab* slabs, const uint8_t
   return xksv::launch_parallel_decode(slabs, p->n_par, pay, out, p->d_status, p->grid_par, st, p->par_whole);
 }
 
+// Decode of the plan's serial slabs: those of whole tiles and the ragged ones
+// by their tile indexes where the payload's index has them, the others
+// resynchronising their streams.
+cudaError_t tile_decode(xksv_plan* p, const xksv::Slab* slabs, const uint8_t* pay, uint8_t* out, cudaStream_t st);
+cudaError_t serial_decode(xksv_plan* p, const xksv::Slab* slabs, const uint8_t* pay, uint8_t* out, cudaStream_t st) {
+  const bool indexed = pay == p->indexed_payload;
+  uint32_t s0 = 0;
+  cudaError_t e = cudaSuccess;
+  if (indexed && p->d_tidx && p->n_items) {
+    e = tile_decode(p, slabs, pay, out, st);
+    ++p->launches;
+    s0 = p->n_ser_idx;
+  }
+  if (e == cudaSuccess && s0 == p->n_ser_idx && indexed && p->r_items) {
+    xksv::GemvArgs g{};
+    g.items = p->d_r_items;
+    g.nitems = p->r_items;
+    g.slabs = slabs + s0;
+    g.tbase = p->d_r_tbase;
+    g.tidx = p->d_r_tidx;
+    g.gtabs = p->d_r_gtabs;
+    g.payload = pay;
+    g.status = p->d_status;
+    g.out = out;
+    g.nb = 1;
+    e = xksv::launch_serial_tile_decode(g, st);
+    ++p->launches;
+    s0 += p->n_ser_rag;
+  }
+  if (e == cudaSuccess && p->n_ser > s0) {
+    e = xksv::launch_serial_decode(slabs + s0, p->n_ser - s0, pay, out, p->d_status, p->grid_ser, st, p->n_ser == p->n_ser_idx);
+    ++p->launches;
+  }
+  return e;
+}
+
 // Indexed decode of the plan's 16-row serial slabs (slabs[0, n_ser_idx)) to
 // out + slab dst; the caller decodes the remaining serial slabs.
 cudaError_t tile_decode(xksv_plan* p, const xksv::Slab* slabs, const uint8_t* pay, uint8_t* out,
@@ -712,19 +771,9 @@ int xksv_plan_decode(const xksv_plan* pc, const void* d_payload, size_t payload_
   uint8_t* out = static_cast<uint8_t*>(d_out);
   p->launches = 0;
   cudaError_t e = cudaSuccess;
-  // with a tile index of this payload, the 16-row serial slabs decode one
-  // thread per tile; the other serial slabs resynchronise their streams
-  const bool indexed = p->d_tidx && d_payload == p->indexed_payload && p->n_items;
-  const uint32_t ser0 = indexed ? p->n_ser_idx : 0;
-  if (indexed) {
-    e = tile_decode(p, p->d_slabs, pay, out, st);
-    ++p->launches;
-  }
-  if (e == cudaSuccess && p->n_ser > ser0) {
-    e = launch_serial_decode(p->d_slabs + ser0, p->n_ser - ser0, pay, out, p->d_status, p->grid_ser, st,
-                             p->n_ser == p->n_ser_idx);
-    ++p->launches;
-  }
+  // with a tile index of this payload, the serial slabs decode one thread per
+  // tile; the others resynchronise their streams
+  e = serial_decode(p, p->d_slabs, pay, out, st);
   if (e == cudaSuccess && p->n_par) {
     e = parallel_decode(p, p->d_slabs + p->n_ser, pay, out, st);
     ++p->launches;
@@ -762,11 +811,12 @@ int xksv_plan_decode_host(const xksv_plan* pc, const void* h_payload, size_t pay
   uint64_t end = 0;
   for (const Slab& s : hs) end = std::max(end, s.src + s.size);
   if (end > payload_size) return 1;  // a slab outside the host payload
-  // groups: tile-indexable serial slabs, the other serial slabs (plan
+  // groups: serial slabs of whole tiles, ragged ones and the rest (plan
   // creation keeps each part in table order), parallel, raw
-  constexpr int NG = 4;
-  const uint32_t lo[NG] = {0, p->n_ser_idx, p->n_ser, p->n_ser + p->n_par};
-  const uint32_t hi[NG] = {p->n_ser_idx, p->n_ser, p->n_ser + p->n_par, p->n_ser + p->n_par + p->n_raw};
+  constexpr int NG = 5;
+  const uint32_t rag = p->n_ser_idx + p->n_ser_rag;
+  const uint32_t lo[NG] = {0, p->n_ser_idx, rag, p->n_ser, p->n_ser + p->n_par};
+  const uint32_t hi[NG] = {p->n_ser_idx, rag, p->n_ser, p->n_ser + p->n_par, p->n_ser + p->n_par + p->n_raw};
   const bool indexed = p->d_tidx && d_payload == p->indexed_payload && p->n_items;
   bool ordered = !indexed && end > 0;
   for (int g = 0; g < NG && ordered; ++g)
@@ -793,7 +843,7 @@ int xksv_plan_decode_host(const xksv_plan* pc, const void* h_payload, size_t pay
     a = b;
   }
   p->launches = 0;
-  uint32_t done[NG] = {lo[0], lo[1], lo[2], lo[3]};
+  uint32_t done[NG] = {lo[0], lo[1], lo[2], lo[3], lo[4]};
   for (int c = 0; c < kHostChunks && e == cudaSuccess; ++c) {
     const uint64_t b = chunk_end(end, c);
     uint32_t upto[NG];
@@ -805,18 +855,18 @@ int xksv_plan_decode_host(const xksv_plan* pc, const void* h_payload, size_t pay
     }
     if (!any) continue;
     e = cudaStreamWaitEvent(st, p->chunk_ev[c], 0);
-    for (int g = 0; g < 2 && e == cudaSuccess; ++g)
+    for (int g = 0; g < 3 && e == cudaSuccess; ++g)
       if (upto[g] > done[g]) {
         e = launch_serial_decode(p->d_slabs + done[g], upto[g] - done[g], pay, out, p->d_status, p->grid_ser, st, g == 0);
         ++p->launches;
       }
-    if (e == cudaSuccess && upto[2] > done[2]) {
-      e = launch_parallel_decode(p->d_slabs + done[2], upto[2] - done[2], pay, out, p->d_status, p->grid_par, st,
+    if (e == cudaSuccess && upto[3] > done[3]) {
+      e = launch_parallel_decode(p->d_slabs + done[3], upto[3] - done[3], pay, out, p->d_status, p->grid_par, st,
                                  p->par_whole);
       ++p->launches;
     }
-    if (e == cudaSuccess && upto[3] > done[3]) {
-      e = launch_raw_decode(p->d_slabs + done[3], upto[3] - done[3], pay, out, p->grid_raw, st);
+    if (e == cudaSuccess && upto[4] > done[4]) {
+      e = launch_raw_decode(p->d_slabs + done[4], upto[4] - done[4], pay, out, p->grid_raw, st);
       ++p->launches;
     }
     for (int g = 0; g < NG; ++g) done[g] = upto[g];
@@ -834,18 +884,7 @@ bool gemm_fused(const xksv_plan* p, const void* d_payload, size_t batch) {
 
 // Enqueues the decode of every slab into its BF16 row group of the scratch.
 cudaError_t decode_scratch(xksv_plan* p, const uint8_t* pay, uint8_t* scratch, cudaStream_t st) {
-  const bool indexed = p->d_tidx && pay == p->indexed_payload;
-  cudaError_t e = cudaSuccess;
-  const uint32_t tser0 = indexed && p->n_items ? p->n_ser_idx : 0;
-  if (tser0) {
-    e = tile_decode(p, p->d_tc_slabs, pay, scratch, st);
-    ++p->launches;
-  }
-  if (e == cudaSuccess && p->n_ser > tser0) {
-    e = launch_serial_decode(p->d_tc_slabs + tser0, p->n_ser - tser0, pay, scratch, p->d_status,
-                             p->grid_ser, st, p->n_ser == p->n_ser_idx);
-    ++p->launches;
-  }
+  cudaError_t e = serial_decode(p, p->d_tc_slabs, pay, scratch, st);
   if (e == cudaSuccess && p->n_par) {
     e = parallel_decode(p, p->d_tc_slabs + p->n_ser, pay, scratch, st);
     ++p->launches;
@@ -1304,6 +1343,42 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   p->fused_ok = true;
 }
 
+// After an index: the tile index of the ragged serial slabs.  Any failure here
+// (a bad slab too: a decode reports it) only leaves it off.
+static void setup_ragged(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st) {
+  const uint32_t n = p->n_ser_rag, s0 = p->n_ser_idx;
+  if (!n) return;
+  std::vector<uint64_t> tbase(n);
+  std::vector<GemvItem> items;
+  uint64_t total = 0;
+  for (uint32_t i = 0; i < n; ++i) {
+    const uint32_t tiles = uint32_t((p->h_slabs[s0 + i].cols + 15) / 16), ni = (tiles + 255) / 256, per = (tiles + ni - 1) / ni;
+    tbase[i] = total;
+    total += uint64_t(tiles) + 1;
+    for (uint32_t t0 = 0; t0 < tiles; t0 += per) items.push_back(GemvItem{i, t0, std::min(per, tiles - t0), 0, ni, 0, 0, 0});
+  }
+  if (total > std::numeric_limits<uint32_t>::max() || items.size() > (1u << 31)) return;
+  const bool ok = cudaMalloc(&p->d_r_tidx, total * sizeof(uint32_t)) == cudaSuccess &&
+                  cudaMalloc(&p->d_r_tbase, n * sizeof(uint64_t)) == cudaSuccess &&
+                  cudaMalloc(&p->d_r_gtabs, n * sizeof(GemvTabs)) == cudaSuccess &&
+                  cudaMalloc(&p->d_r_items, items.size() * sizeof(GemvItem)) == cudaSuccess &&
+                  cudaMemcpyAsync(p->d_r_tbase, tbase.data(), n * sizeof(uint64_t), cudaMemcpyHostToDevice, st) == cudaSuccess &&
+                  cudaMemcpyAsync(p->d_r_items, items.data(), items.size() * sizeof(GemvItem), cudaMemcpyHostToDevice, st) ==
+                      cudaSuccess &&
+                  cudaMemsetAsync(p->d_r_tidx, 0, total * sizeof(uint32_t), st) == cudaSuccess &&
+                  cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
+                  launch_serial_index(p->d_slabs + s0, n, d_payload, p->d_r_tidx, nullptr, p->d_r_tbase, p->d_r_gtabs,
+                                      p->d_status, st) == cudaSuccess &&
+                  cudaMemcpyAsync(p->h_status, p->d_status, sizeof(int), cudaMemcpyDeviceToHost, st) == cudaSuccess &&
+                  cudaStreamSynchronize(st) == cudaSuccess && *p->h_status == 0;
+  cudaMemsetAsync(p->d_status, 0, sizeof(int), st);
+  cudaStreamSynchronize(st);
+  if (ok)
+    p->r_items = uint32_t(items.size());
+  else
+    free_ragged(p);
+}
+
 // After an index: the part index of the parallel slabs, for plans of too few
 // to fill the GPU with one warp each.  Any failure here (a bad slab too: a
 // decode reports it) only leaves the parts off.
@@ -1337,6 +1412,7 @@ int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, vo
   const uint32_t n = p->n_ser_idx;
   if (!n) {
     p->indexed_payload = d_payload;
+    setup_ragged(p, static_cast<const uint8_t*>(d_payload), st);
     setup_parts(p, static_cast<const uint8_t*>(d_payload), st);
     return 0;
   }
@@ -1390,6 +1466,7 @@ int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, vo
   p->n_items = uint32_t(items.size());
   p->indexed_payload = d_payload;
   setup_fused(p, static_cast<const uint8_t*>(d_payload), st);
+  setup_ragged(p, static_cast<const uint8_t*>(d_payload), st);
   setup_parts(p, static_cast<const uint8_t*>(d_payload), st);
   return 0;
 }

@@ -63,7 +63,8 @@ cudaError_t launch_raw_gemm(const Slab* slabs, uint32_t n, const uint8_t* payloa
 
 // Tile index of 16-row serial-codec slabs: tidx[tbase[i] + k] = bit offset of
 // tile k's first code in slab i's stream, tidx[tbase[i] + tiles] = bit count;
-// tmid[tbase[i] + k] = bit offset of tile k's row 8 (its 129th code).
+// tmid[tbase[i] + k] = bit offset of tile k's row 8 (its 129th code).  tmid
+// null: ragged slabs (up to 16 rows, any columns), tiles of the slab's rows.
 cudaError_t launch_serial_index(const Slab* slabs, uint32_t n, const uint8_t* payload,
                                 uint32_t* tidx, uint32_t* tmid, const uint64_t* tbase, GemvTabs* gtabs,
                                 int* status, cudaStream_t st);
@@ -142,7 +143,7 @@ cudaError_t launch_serial_tile_linear(const GemvArgs& args, cudaStream_t st);
 cudaError_t launch_tp_wait(const uint32_t* flags, uint32_t world, const uint32_t* epoch, int* status,
                            cudaStream_t st);
 // Indexed decode of the same slabs to BF16 at args.out + slab dst (x, y,
-// partials and counters unused).
+// partials and counters unused); tmid null: of ragged slabs.
 cudaError_t launch_serial_tile_decode(const GemvArgs& args, cudaStream_t st);
 
 // Tensor-core GEMM over decoded row groups (batch >= 16 path).

@@ -570,17 +570,29 @@ __global__ void __launch_bounds__(ST, 3) serial_slab_kernel(const Slab* __restri
       // ---- 5. exact decode straight to the output ----
       if (MODE == 2 && myN) {
         // tile index: the stream offset of every 256th code (a 16x16 tile
-        // start) and of every tile's 129th code (its row 8)
+        // start) and of every tile's 129th code (its row 8); RAGGED: of every
+        // tile of the slab's rows, 16 columns each
         SmemWin96 r;
         r.init(S.win, t == 0 ? p0rel : S.endpos[t - 1]);
         bool dead = false;
         uint32_t* ti = a.tidx + a.tbase[si];
-        uint32_t* tm = a.tmid + a.tbase[si];
-        const uint32_t gend = base + my_off + myN;
-        for (uint32_t g = base + my_off; g < gend; ++g) {
-          if ((g & 127u) == 0) ((g & 128u) ? tm : ti)[g >> 8] = R0 + r.pos();
-          r.refill();
-          code1<7>(S, r, dead);
+        uint32_t g = base + my_off;
+        const uint32_t gend = g + myN;
+        if (RAGGED) {
+          const uint32_t tile = 16 * uint32_t(rows);
+          uint32_t k = (g + tile - 1) / tile;
+          for (; g < gend; ++g) {
+            if (g == k * tile) ti[k++] = R0 + r.pos();
+            r.refill();
+            code1<7>(S, r, dead);
+          }
+        } else {
+          uint32_t* tm = a.tmid + a.tbase[si];
+          for (; g < gend; ++g) {
+            if ((g & 127u) == 0) ((g & 128u) ? tm : ti)[g >> 8] = R0 + r.pos();
+            r.refill();
+            code1<7>(S, r, dead);
+          }
         }
       } else if (myN) {
         SmemWin96 r;
@@ -588,7 +600,7 @@ __global__ void __launch_bounds__(ST, 3) serial_slab_kernel(const Slab* __restri
         bool dead = false;
         uint32_t g = base + my_off;
         const uint32_t gend = g + myN;
-        if (RAGGED && !o.nice && rows <= 16) {
+        if (MODE == 0 && RAGGED && !o.nice && rows <= 16) {
           Walk at(g, uint32_t(rows), uint32_t(cols));
           auto put = [&](uint32_t word) {
             o.out[size_t(at.r) * cols + at.col()] = uint16_t(word);
@@ -721,7 +733,7 @@ __global__ void __launch_bounds__(ST, 3) serial_slab_kernel(const Slab* __restri
     if (err) {
       if (t == 0) atomicOr(a.status, err);
     } else if (MODE == 2) {
-      if (t == 0) a.tidx[a.tbase[si] + (cnt32 >> 8)] = nb32;  // end sentinel
+      if (t == 0) a.tidx[a.tbase[si] + (RAGGED ? uint32_t((cols + 15) / 16) : cnt32 >> 8)] = nb32;  // end sentinel
     } else if (MODE == 1 && o.nice) {
       for (uint32_t k = t; k < 16 * a.nb; k += ST) {
         const uint32_t r = k / a.nb, b = k - r * a.nb;
@@ -810,10 +822,12 @@ __device__ __forceinline__ void fma4(float* acc, uint32_t e0, uint32_t e1, uint3
 }
 
 // NB == 0: decode mode (BF16 tile rows to a.out + slab dst); NB >= 1: GEMV/GEMM.
-// LIN: a linear layer's call (BF16 tokens in, epilogue out).
-template <int NB, int SPLIT, bool LIN = false>
+// LIN: a linear layer's call (BF16 tokens in, epilogue out).  RAGGED (decode):
+// slabs of up to 16 rows whose last tile may be narrower.
+template <int NB, int SPLIT, bool LIN = false, bool RAGGED = false>
 __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) serial_tile_gemv_kernel(GemvArgs a) {
   static_assert(SPLIT == 1 || (SPLIT == 2 && NB <= 1), "two threads per tile at batch <= 1");
+  static_assert(!RAGGED || (NB == 0 && SPLIT == 1), "ragged slabs are decoded, one thread per tile");
   constexpr int NT = GT * SPLIT;   // threads
   constexpr int RPT = 16 / SPLIT;  // tile rows per thread
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -956,7 +970,9 @@ __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) seri
     // the tile's 256 sign/mantissa bytes, one 16-byte row per step from
     // aligned 16-byte loads (the misalignment is the same for the whole slab;
     // the chunk past the tile is the slab's next bytes, so loads stay inside)
-    const uintptr_t sma = reinterpret_cast<uintptr_t>(sm + uint64_t(tile) * 256);
+    const uint32_t nrows = RAGGED ? uint32_t(sd.rows) : 16;
+    const uint32_t width = RAGGED ? min(16u, uint32_t(sd.cols) - 16 * tile) : 16;
+    const uintptr_t sma = reinterpret_cast<uintptr_t>(sm + uint64_t(tile) * 16 * nrows);
     const int soff = int(sma & 15);
     const uint4* sq = reinterpret_cast<const uint4*>(sma & ~uintptr_t(15));
     const bool ostore16 = NB == 0 && ((reinterpret_cast<uintptr_t>(a.out + sd.dst) | (sd.cols * 2)) & 15) == 0;
@@ -978,12 +994,20 @@ __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) seri
       bool dead = false;
       // sign/mantissa rows loaded one row ahead of use
       const int row0 = part * RPT;
-      uint4 nlo = ldg16(sq + row0), nhi = soff ? ldg16(sq + row0 + 1) : make_uint4(0, 0, 0, 0);
-      for (int row = row0; row < row0 + RPT; ++row) {
+      // (a narrower tile's rows are not 16 bytes: read byte by byte below)
+      const bool full = !RAGGED || width == 16;
+      uint4 nlo = make_uint4(0, 0, 0, 0), nhi = nlo;
+      if (full) {
+        nlo = ldg16(sq + row0);
+        if (soff) nhi = ldg16(sq + row0 + 1);
+      }
+      for (int row = row0; row < (RAGGED ? int(nrows) : row0 + RPT); ++row) {
         const uint4 lo = nlo, hi = nhi;
-        const int nr = row < 15 ? row + 1 : 15;
-        nlo = ldg16(sq + nr);
-        if (soff) nhi = ldg16(sq + nr + 1);
+        const int nr = row < int(nrows) - 1 ? row + 1 : int(nrows) - 1;
+        if (full) {
+          nlo = ldg16(sq + nr);
+          if (soff) nhi = ldg16(sq + nr + 1);
+        }
         float acc[NB > 0 ? NB : 1];
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = 0.f;
@@ -992,7 +1016,14 @@ __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) seri
           atomicOr(a.status, kStatusStream);
           act = false;
         }
-        if (act && NB == 0) {
+        if (RAGGED && act && !full) {
+          const uint8_t* srow = sm + uint64_t(tile) * 16 * nrows + row * width;
+          uint16_t* orow = reinterpret_cast<uint16_t*>(a.out + sd.dst) + uint64_t(row) * sd.cols + uint64_t(tile) * 16;
+          for (uint32_t c = 0; c < width; ++c) {
+            r.refill();
+            orow[c] = uint16_t(merge1(code1<7>(S, r, dead), __ldg(srow + c)));
+          }
+        } else if (act && NB == 0) {
           // decode: tile row `row` = 16 BF16 words, two 16-byte halves
           const uint4 s16 = realign16(lo, hi, soff);
           const uint32_t sw[4] = {s16.x, s16.y, s16.z, s16.w};
@@ -1147,6 +1178,8 @@ void serial_set_attr() {
   cudaFuncSetAttribute(serial_slab_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SerialShared)));
   cudaFuncSetAttribute(serial_slab_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SerialShared)));
   cudaFuncSetAttribute(serial_tile_gemv_kernel<0, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
+  cudaFuncSetAttribute(serial_tile_gemv_kernel<0, 1, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
+  cudaFuncSetAttribute(serial_slab_kernel<2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(SerialShared)));
   cudaFuncSetAttribute(serial_tile_gemv_kernel<0, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
   cudaFuncSetAttribute(serial_tile_gemv_kernel<1, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
   cudaFuncSetAttribute(serial_tile_gemv_kernel<1, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(GemvShared)));
@@ -1193,14 +1226,17 @@ cudaError_t launch_serial_index(const Slab* slabs, uint32_t n, const uint8_t* pa
   if (!n) return cudaSuccess;
   serial_set_attr();
   SerialArgs a{payload, nullptr, nullptr, nullptr, 1, 1, status, tidx, tbase, tmid, gtabs};
-  serial_slab_kernel<2><<<n, ST, sizeof(SerialShared), st>>>(slabs, n, a);
+  if (tmid)
+    serial_slab_kernel<2><<<n, ST, sizeof(SerialShared), st>>>(slabs, n, a);
+  else
+    serial_slab_kernel<2, true><<<n, ST, sizeof(SerialShared), st>>>(slabs, n, a);
   return cudaGetLastError();
 }
 
 // The indexed kernel is launched with programmatic stream serialisation: its
 // CTAs may start (table build, bit staging) while the stream's previous
 // kernel finishes, and wait for it before touching shared data.
-template <int NB, int SPLIT, bool LIN = false>
+template <int NB, int SPLIT, bool LIN = false, bool RAGGED = false>
 cudaError_t launch_tile_kernel(const GemvArgs& args, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(args.nitems);
@@ -1212,7 +1248,7 @@ cudaError_t launch_tile_kernel(const GemvArgs& args, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, serial_tile_gemv_kernel<NB, SPLIT, LIN>, args);
+  return cudaLaunchKernelEx(&cfg, serial_tile_gemv_kernel<NB, SPLIT, LIN, RAGGED>, args);
 }
 
 // Two threads per tile when the items fill under one wave of 256-thread CTAs
@@ -1252,8 +1288,9 @@ cudaError_t launch_serial_tile_linear(const GemvArgs& args, cudaStream_t st) {
 
 cudaError_t launch_serial_tile_decode(const GemvArgs& args, cudaStream_t st) {
   if (!args.nitems) return cudaSuccess;
-  if (!args.gtabs || !args.tmid) return cudaErrorInvalidValue;
+  if (!args.gtabs) return cudaErrorInvalidValue;
   serial_set_attr();
+  if (!args.tmid) return launch_tile_kernel<0, 1, false, true>(args, st);
   return tile_split(args.nitems) ? launch_tile_kernel<0, 2>(args, st) : launch_tile_kernel<0, 1>(args, st);
 }
 
