@@ -220,8 +220,8 @@ __device__ __noinline__ bool index_segment(const Seg s, WarpTabs& W, int lane, c
 }
 
 // Decodes one substream.  `rows16`: 16-row slab, cols % 16 == 0, the
-// substream starts on a tile row and (decode) the output is 16-byte aligned;
-// whole tile rows then leave as 32-byte stores.  The caller has started `b`
+// substream starts on a tile row (decode: or half of one) and (decode) the
+// output is 16-byte aligned; whole tile rows then leave as 32-byte stores.  The caller has started `b`
 // and `smr` (sign/mantissa bytes, 16 per group) and put the first words into
 // the ring.
 // `WHOLE`: the caller's slabs all lie in whole rows, so that other substreams
@@ -252,7 +252,12 @@ __device__ void decode_segment(const Seg& s, WarpTabs& W, int lane, const ldec::
         uint4 v0, v1;
         ldec::merge16(e, s16, v0, v1);
         uint4* dst = reinterpret_cast<uint4*>(o.out + size_t(r) * o.cols + c);
-        if (o.out32) {
+        if (!WHOLE && (p & 15)) {
+          // from the middle of a row: its second half, the next row's first
+          const uint32_t p1 = p + 8, r1 = (p1 >> 4) & 15, c1 = (p1 >> 8) * 16;
+          dst[1] = v0;
+          *reinterpret_cast<uint4*>(o.out + size_t(r1) * o.cols + c1) = v1;
+        } else if (o.out32) {
           st_global_32B(dst, v0, v1);
         } else {
           dst[0] = v0;
@@ -435,7 +440,8 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
     Seg s{};
     s.start = uint32_t(uint64_t(total) * uint64_t(lane) / chunks);
     const uint64_t expect = uint64_t(total) * uint64_t(lane + 1) / chunks - s.start;
-    const bool rows16 = nice && (s.start & 15) == 0;
+    // (a decode also takes starts in the middle of a row: slabs of an odd number of tiles)
+    const bool rows16 = nice && (s.start & (MODE == 0 && !WHOLE ? 7 : 15)) == 0;
     ldec::Stream b;
     ldec::SmStream smr;
     // this part's codes [c0, c1) of the lane's substream and its first bit
