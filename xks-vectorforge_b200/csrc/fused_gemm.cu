@@ -404,42 +404,63 @@ __global__ void fused_prep_kernel(const float* __restrict__ x, uint32_t ld, uint
 }
 
 // The linear layer's rows: CTA (g, s, n) takes eight slabs of group g and
-// sixteen tokens, adds the sums that the group's segments left (in their
-// order) and writes y through the epilogue.  The sums are read along the
-// slabs and written along the rows, by way of shared memory.
-constexpr int OT = 256, OJ = 8;
-__global__ void __launch_bounds__(OT) fused_out_kernel(FusedArgs a, const uint32_t* __restrict__ gseg0,
-                                                       const uint32_t* __restrict__ gsegs, Epilogue e) {
-  __shared__ float T[16][OJ * 17];
+// sixteen tokens, adds the sums that the group's segments left (in a fixed
+// order) and writes y through the epilogue.  A plan of few groups has many
+// segments a group (74 for a 1024 x 1024 weight), so four quarters of the
+// threads add a quarter of them each, four segments' loads in flight (one
+// thread per sum and one load after another: 1024 x 1024 at 16 tokens 79 us,
+// 272 x 7056 132 us, 14336 x 4096 119 us; so 37, 47 and 115 us).  The sums are read along the slabs and written along the rows, by way of shared memory.
+constexpr int OT = 256, OQ = 4, OJ = 8;
+__global__ void __launch_bounds__(OT * OQ) fused_out_kernel(FusedArgs a, const uint32_t* __restrict__ gseg0,
+                                                            const uint32_t* __restrict__ gsegs, Epilogue e) {
+  __shared__ float T[OQ][16][OJ * 17];
   const FusedGroup g = a.groups[blockIdx.x];
-  const uint32_t j0 = blockIdx.y * OJ, n0 = blockIdx.z * 16, t = threadIdx.x;
+  const uint32_t j0 = blockIdx.y * OJ, n0 = blockIdx.z * 16, quarter = threadIdx.x / OT, t = threadIdx.x % OT;
   if (j0 >= g.nslabs) return;
   // reads: slab j0 + t % 8, its row t / 8 % 16, tokens t / 128 + 2 k
-  // writes: the row of slab j0 + t / 16 % 8, tokens t / 128 + 2 k
+  // writes: the row of slab j0 + t / 16 % 8, tokens t / 128 + 2 k, k of this quarter
   const uint32_t rj = t & 7, rr = (t >> 3) & 15, wj = (t >> 4) & 7, wr = t & 15, nt = t >> 7;
+  constexpr int KW = 8 / OQ;
   const bool write = j0 + wj < g.nslabs;
   const uint64_t row = write ? a.slabs[a.members[g.m0 + j0 + wj]].dst + wr : 0;
-  const uint32_t s0 = gseg0[blockIdx.x], s1 = gseg0[blockIdx.x + 1];
+  const uint32_t g0 = gseg0[blockIdx.x], gn = gseg0[blockIdx.x + 1] - g0;
+  const uint32_t s0 = g0 + gn * quarter / OQ, s1 = g0 + gn * (quarter + 1) / OQ;
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  EpilogueOps ops[8];
-  float z[8];
+  EpilogueOps ops[KW];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    z[k] = 0.f;
-    if (write && n0 + nt + 2 * k < a.nb) ops[k] = epilogue_read(e, n0 + nt + 2 * k, row);
+  for (int k = 0; k < KW; ++k) {
+    const uint32_t n = n0 + nt + 2 * (KW * quarter + k);
+    if (write && n < a.nb) ops[k] = epilogue_read(e, n, row);
   }
-  for (uint32_t s = s0; s < s1; ++s) {
-    const float* src = a.y + ((uint64_t(gsegs[s]) * 16 + rr) * a.npad + n0 + nt) * 32 + j0 + rj;
+  float z[8] = {};
+  const bool read = j0 + rj < g.nslabs;
+  for (uint32_t s = s0; s < s1; s += 4) {
+    float v[4][8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (j0 + rj < g.nslabs && n0 + nt + 2 * k < a.nb) z[k] += __ldcg(src + 64 * k);
+    for (int q = 0; q < 4; ++q) {
+      const bool here = read && s + q < s1;
+      const float* src = here ? a.y + ((uint64_t(gsegs[s + q]) * 16 + rr) * a.npad + n0 + nt) * 32 + j0 + rj : a.y;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[q][k] = here && n0 + nt + 2 * k < a.nb ? __ldcg(src + 64 * k) : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) z[k] += v[q][k];
   }
 #pragma unroll
-  for (int k = 0; k < 8; ++k) T[nt + 2 * k][rj * 17 + rr] = z[k];
+  for (int k = 0; k < 8; ++k) T[quarter][nt + 2 * k][rj * 17 + rr] = z[k];
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (write && n0 + nt + 2 * k < a.nb) epilogue_write(e, n0 + nt + 2 * k, row, T[nt + 2 * k][wj * 17 + wr], ops[k]);
+  for (int k = 0; k < KW; ++k) {
+    const uint32_t n = nt + 2 * (KW * quarter + k);
+    if (write && n0 + n < a.nb) {
+      float sum = T[0][n][wj * 17 + wr];
+#pragma unroll
+      for (int q = 1; q < OQ; ++q) sum += T[q][n][wj * 17 + wr];
+      epilogue_write(e, n0 + n, row, sum, ops[k]);
+    }
+  }
 }
 
 // One warp per group: lane j builds slab j's tables (the codes of its 256
@@ -563,7 +584,7 @@ cudaError_t launch_fused_linear(const FusedArgs& args, uint32_t nctas, uint32_t 
   if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ngroups, 32 / OJ, args.npad / 16);
-  cfg.blockDim = dim3(OT);
+  cfg.blockDim = dim3(OT * OQ);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
