@@ -161,6 +161,26 @@ def test_linear_larger_weight(batch):
     plan.close()
 
 
+@pytest.mark.parametrize("batch", [1, 16, 70, 300])
+@pytest.mark.parametrize("cols", [520, 8200])
+def test_linear_fp32_sums_stay_fp32(batch, cols):
+    """An FP32 result's relative error does not grow with the columns.  The
+    tensor cores cut each addition towards zero by at most the last place of
+    the running sum, 2^-23 (2^-24 on average), 32 additions of 16 columns to an
+    accumulator: 32 * 2^-24 of the result's norm, with what is added in FP32
+    behind it far below."""
+    payload, entries, ws = pack([(64, cols, 0, 0, xg.CODEC_PARALLEL32), (64, cols, 64, 0, xg.CODEC_TILE16)], 5)
+    plan = xg.Plan(entries)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(batch, cols, generator=g, device=DEV).bfloat16()
+    y = torch.empty(batch, 128, device=DEV)
+    plan.linear(payload, x, y)
+    torch.cuda.synchronize()
+    assert plan.status() == 0
+    want = x.double() @ torch.cat([w for w, _, _ in ws]).double().t()
+    assert float((y - want).norm() / want.norm()) <= 32 * 2.0 ** -24
+
+
 @pytest.mark.parametrize("batch", [1, 3, 16, 200])
 def test_linear_in_place_and_special_values(batch):
     """The residual and the factor may be y itself; infinities and NaN in one

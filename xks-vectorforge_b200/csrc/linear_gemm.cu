@@ -11,9 +11,16 @@
 //     rows, zero past the edges) into a ring of stages,
 //   * one thread (of the pair's first CTA) issues tcgen05.mma kind::f16,
 //     M = 128 (256) tokens, N = tn, K = 16, into one of two TMEM accumulators,
-//   * four warps read the other accumulator (a lane is a token, its registers
+//   * eight warps read the other accumulator (a lane is a token, its registers
 //     consecutive rows of y), apply bias, activation, factor and residual in
 //     FP32 and write y: the epilogue of a tile runs behind the products of the next.
+// The tensor cores add in FP32 but cut what falls below the sum's last place,
+// always towards zero: 1.1e-9 of the result a column, 1.6e-5 at 14336.  A BF16
+// result is rounded a hundred times coarser.  For FP32 results (EXACT) an
+// accumulator holds 512 columns only, and the epilogue's warps add its sums to
+// theirs, in registers, rounded to nearest: relative error 4.8e-7 at every
+// length (1024 columns: 1.0e-6), with the decode 166 us against 160 at 77
+// tokens, 288 against 256 at 2048 (4096 x 14336).
 // gemm_plan chooses tn and the pair by a model of both costs.  Tokens as the
 // MMA's rows rather than weight rows: y is token-major, so a lane's results
 // are contiguous.
@@ -34,7 +41,9 @@ namespace {
 
 constexpr int GM = 128;          // tokens of a tile
 constexpr int GK = 64;           // columns of a stage: 128-byte rows
-constexpr int GTHREADS = 192;    // producer, MMA and four epilogue warps
+constexpr int EPI = 256;         // epilogue threads: two warps for each 32 tokens
+constexpr int GTHREADS = 64 + EPI;  // producer and MMA warps besides
+constexpr uint32_t kExactSlices = 8;  // slices (512 columns) of an accumulator, EXACT
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kABytes = GM * GK * 2;
 constexpr size_t kRing = 220 * 1024;  // stages' shared memory
@@ -140,7 +149,7 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
   asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
 
-template <bool PAIR>
+template <bool PAIR, bool EXACT>
 __global__ void __launch_bounds__(GTHREADS, 1)
     linear_gemm_kernel(const __grid_constant__ CUtensorMap mx, const __grid_constant__ CUtensorMap mw, const GemmArgs a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -154,6 +163,7 @@ __global__ void __launch_bounds__(GTHREADS, 1)
   const uint32_t stage_bytes = kABytes + bn * GK * 2;
   const uint32_t mt = (a.batch + TM - 1) / TM, nt = (a.rows + a.tn - 1) / a.tn, tiles = mt * nt;
   const uint32_t ksteps = (a.cols + GK - 1) / GK;
+  const uint32_t kpart = EXACT ? kExactSlices : ksteps;  // slices of an accumulator
   const uint32_t first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;  // this CTA's (pair's) tiles
   if (warp == 1) {
     if (PAIR) {
@@ -173,7 +183,7 @@ __global__ void __launch_bounds__(GTHREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_addr(&S.tfull[b]), 1);
-      mbar_init(smem_addr(&S.tempty[b]), 128 * CTAS);
+      mbar_init(smem_addr(&S.tempty[b]), EPI * CTAS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     S.abort_flag = 0;
@@ -223,30 +233,33 @@ __global__ void __launch_bounds__(GTHREADS, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = umma_idesc_bf16(TM, a.tn);
-      uint32_t n = 0, ti = 0;  // slices multiplied, tiles begun
+      uint32_t n = 0, ai = 0;  // slices multiplied, accumulators begun
       uint32_t s = 0, round = 0;
       const uint64_t desc0 = desc_sw128(smem_addr(ring));
-      for (uint32_t t = first; t < tiles && ok; t += stride, ++ti) {
-        const uint32_t buf = ti & 1, d = tmem + buf * (a.tmem_cols / 2);
-        ok = wait_or_abort(smem_addr(&S.tempty[buf]), ((ti >> 1) & 1) ^ 1, &S.abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        for (uint32_t k = 0; k < ksteps; ++k, ++n) {
-          ok = wait_or_abort(smem_addr(&S.full[s]), round & 1, &S.abort_flag);
+      for (uint32_t t = first; t < tiles && ok; t += stride) {
+        for (uint32_t k0 = 0; k0 < ksteps && ok; k0 += kpart, ++ai) {
+          const uint32_t buf = ai & 1, d = tmem + buf * (a.tmem_cols / 2);
+          const uint32_t slices = min(kpart, ksteps - k0);
+          ok = wait_or_abort(smem_addr(&S.tempty[buf]), ((ai >> 1) & 1) ^ 1, &S.abort_flag);
           if (!ok) break;
           tc_fence_after();
-          // (addresses below 256 KB: a descriptor's address field does not overflow)
-          const uint64_t da = desc0 + ((s * stage_bytes) >> 4), db = da + (kABytes >> 4);
+          for (uint32_t k = 0; k < slices; ++k, ++n) {
+            ok = wait_or_abort(smem_addr(&S.full[s]), round & 1, &S.abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            // (addresses below 256 KB: a descriptor's address field does not overflow)
+            const uint64_t da = desc0 + ((s * stage_bytes) >> 4), db = da + (kABytes >> 4);
 #pragma unroll
-          for (uint32_t j = 0; j < GK / 16; ++j)  // 32 bytes further along the rows
-            mma_f16<PAIR>(d, da + 2 * j, db + 2 * j, idesc, (k | j) != 0);
-          commit<PAIR>(smem_addr(&S.empty[s]));
-          if (++s == a.stages) {
-            s = 0;
-            ++round;
+            for (uint32_t j = 0; j < GK / 16; ++j)  // 32 bytes further along the rows
+              mma_f16<PAIR>(d, da + 2 * j, db + 2 * j, idesc, (k | j) != 0);
+            commit<PAIR>(smem_addr(&S.empty[s]));
+            if (++s == a.stages) {
+              s = 0;
+              ++round;
+            }
           }
+          if (ok) commit<PAIR>(smem_addr(&S.tfull[buf]));
         }
-        if (ok) commit<PAIR>(smem_addr(&S.tfull[buf]));
       }
       if (!ok) S.abort_flag = 1;
       // the MMAs issued are done before TMEM is freed: they complete in
@@ -254,34 +267,58 @@ __global__ void __launch_bounds__(GTHREADS, 1)
       if (n && !mbar_wait(smem_addr(&S.empty[(n - 1) % a.stages]), ((n - 1) / a.stages) & 1)) ok = false;
     }
   } else {
-    const uint32_t ti0 = (warp & 3) * 32;  // this warp's TMEM lanes
-    uint32_t ti = 0;
-    for (uint32_t t = first; t < tiles; t += stride, ++ti) {
-      const uint32_t m0 = t % mt * TM + rank * GM, n0 = t / mt * a.tn, buf = ti & 1;
-      ok = wait_or_abort(smem_addr(&S.tfull[buf]), (ti >> 1) & 1, &S.abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
+    const uint32_t ti0 = (warp & 3) * 32;            // this warp's TMEM lanes
+    const uint32_t half = uint32_t(warp - 2) >> 2;   // 32-row groups half, half + 2, ... of a tile
+    uint32_t ai = 0;
+    for (uint32_t t = first; t < tiles && ok; t += stride) {
+      const uint32_t m0 = t % mt * TM + rank * GM, n0 = t / mt * a.tn;
       const uint64_t b = m0 + ti0 + lane;
       const uint32_t top = min(a.tn, a.rows - n0);
-      for (uint32_t c = 0; c < top; c += 32) {
-        uint32_t r[32];
-        tmem_ld32(tmem + (ti0 << 16) + buf * (a.tmem_cols / 2) + c, r);
-        if (b < a.batch) {
+      const auto store = [&](uint32_t c, float* v) {
+        if (b >= a.batch) return;
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float v[8];
+        for (int g = 0; g < 4; ++g) epilogue_store8(a.e, b, a.row0 + n0 + c + 8 * g, v + 8 * g, int(top) - int(c + 8 * g));
+      };
+      float sum[EXACT ? 4 : 1][32];  // EXACT: of the tile's accumulators so far
+      for (uint32_t k0 = 0; k0 < ksteps; k0 += kpart, ++ai) {
+        const uint32_t buf = ai & 1, acc = tmem + (ti0 << 16) + buf * (a.tmem_cols / 2);
+        ok = wait_or_abort(smem_addr(&S.tfull[buf]), (ai >> 1) & 1, &S.abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (EXACT) {
 #pragma unroll
-            for (int x = 0; x < 8; ++x) v[x] = __uint_as_float(r[8 * g + x]);
-            epilogue_store8(a.e, b, a.row0 + n0 + c + 8 * g, v, int(top) - int(c + 8 * g));
+          for (uint32_t g = 0; g < 8; ++g) {
+            const uint32_t c = 32 * (g & ~1u) + 32 * half + 16 * (g & 1);
+            if (c < top) {
+              float r[16];
+              tmem_ld16(acc + c, r);
+              float* z = sum[EXACT ? g / 2 : 0] + 16 * (g & 1);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) z[x] = r[x] + (k0 ? z[x] : 0.f);
+            }
+          }
+        } else {
+          for (uint32_t c = 32 * half; c < top; c += 64) {
+            uint32_t r[32];
+            tmem_ld32(acc + c, r);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) sum[0][x] = __uint_as_float(r[x]);
+            store(c, sum[0]);
           }
         }
+        tc_fence_before();
+        if (PAIR)
+          arrive_cluster(in_cta(smem_addr(&S.tempty[buf]), 0));
+        else
+          mbar_arrive(smem_addr(&S.tempty[buf]));
       }
-      tc_fence_before();
-      if (PAIR)
-        arrive_cluster(in_cta(smem_addr(&S.tempty[buf]), 0));
-      else
-        mbar_arrive(smem_addr(&S.tempty[buf]));
+      if (EXACT && ok)
+#pragma unroll
+        for (uint32_t g = 0; g < 4; ++g) {
+          const uint32_t c = 32 * (2 * g + half);
+          if (c < top) store(c, sum[EXACT ? g : 0]);
+        }
     }
     if (!ok) S.abort_flag = 1;
   }
@@ -397,9 +434,10 @@ cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, cons
   const size_t smem = size_t(a.stages) * stage + 1024;
   // one CTA an SM, whatever the tile: its TMEM columns are its own
   const size_t ask = std::max<size_t>(smem, 120 * 1024);
-  auto kernel = plan.pair ? linear_gemm_kernel<true> : linear_gemm_kernel<false>;
-  static std::atomic<uint64_t> done[2] = {};
-  const cudaError_t err = opt_in_smem(kernel, kRing + 1024, done[plan.pair]);
+  auto kernel = e.y_f32 ? plan.pair ? linear_gemm_kernel<true, true> : linear_gemm_kernel<false, true>
+                        : plan.pair ? linear_gemm_kernel<true, false> : linear_gemm_kernel<false, false>;
+  static std::atomic<uint64_t> done[2][2] = {};
+  const cudaError_t err = opt_in_smem(kernel, kRing + 1024, done[e.y_f32][plan.pair]);
   if (err != cudaSuccess) return err;
   const uint64_t tiles = uint64_t((batch + GM * ctas - 1) / (GM * ctas)) * ((rows + a.tn - 1) / a.tn);
   cudaLaunchConfig_t cfg = {};
