@@ -346,7 +346,8 @@ def _workspace(given, nbytes, device, stream):
         return given, given.data_ptr(), given.numel() * given.element_size()
     if not nbytes:
         return None, None, 0
-    if stream == torch.cuda.current_stream(device).cuda_stream:
+    # (the raw handle: building a torch Stream object takes 3.5 us of a 20 us call)
+    if stream == torch._C._cuda_getCurrentRawStream(device.index):
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
     else:
         with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
