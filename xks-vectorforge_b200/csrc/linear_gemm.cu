@@ -194,6 +194,8 @@ __global__ void __launch_bounds__(GTHREADS, 1)
   tc_fence_after();
   const uint32_t tmem = S.tmem;
   bool ok = true;
+  // the start above runs behind the decode's end; its weight is complete here
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
   if (warp == 0) {
     if (lane == 0) {
@@ -445,12 +447,14 @@ cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, cons
   cfg.blockDim = dim3(GTHREADS);
   cfg.dynamicSmemBytes = ask;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ctas;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kernel, mx, mw, a);
 }
 

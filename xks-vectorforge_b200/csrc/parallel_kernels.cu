@@ -136,6 +136,8 @@ template <int MODE>
 __device__ __forceinline__ bool ragged_codes(const Seg s, WarpTabs& W, int lane, const ldec::Code lc, ldec::Stream b, const Out o) {
   bool bad = false;
   Walk at(s.start, o.rows, o.cols);
+  // four codes at a time lie in one row, 8-byte aligned
+  const bool quads = ((s.start | o.cols) & 3) == 0 && (reinterpret_cast<uintptr_t>(o.out) & 7) == 0;
   auto emit = [&](uint32_t e, uint32_t sm) {
     const uint32_t word = merge1(e, sm);
     if (MODE == 0) {
@@ -165,7 +167,16 @@ __device__ __forceinline__ bool ragged_codes(const Seg s, WarpTabs& W, int lane,
     s16.y = __funnelshift_r(w[1], w[2], shift);
     s16.z = __funnelshift_r(w[2], w[3], shift);
     s16.w = __funnelshift_r(w[3], w[4], shift);
-    if (MODE == 0 && at.w == 16 && (at.c == 0 || at.r + 1 < at.rows || at.t0 + 32 <= at.cols)) {
+    if (MODE == 0 && quads) {
+      uint4 v0, v1;
+      ldec::merge16(e, s16, v0, v1);
+      const uint2 v[4] = {{v0.x, v0.y}, {v0.z, v0.w}, {v1.x, v1.y}, {v1.z, v1.w}};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        *reinterpret_cast<uint2*>(o.out + size_t(at.r) * o.cols + at.col()) = v[k];
+        at.next4();
+      }
+    } else if (MODE == 0 && at.w == 16 && (at.c == 0 || at.r + 1 < at.rows || at.t0 + 32 <= at.cols)) {
       // the rest of this tile row and the beginning of the next one
       uint4 v0, v1;
       ldec::merge16(e, s16, v0, v1);

@@ -401,7 +401,13 @@ struct Walk {
   }
   __device__ __forceinline__ uint32_t col() const { return t0 + c; }
   __device__ __forceinline__ void next() {
-    if (++c < w) return;
+    if (++c >= w) next_row();
+  }
+  // Four elements along, c and cols multiples of 4.
+  __device__ __forceinline__ void next4() {
+    if ((c += 4) >= w) next_row();
+  }
+  __device__ __forceinline__ void next_row() {
     c = 0;
     if (++r < rows) return;
     r = 0;
