@@ -409,7 +409,8 @@ __global__ void fused_prep_kernel(const float* __restrict__ x, uint32_t ld, uint
 // segments a group (74 for a 1024 x 1024 weight), so four quarters of the
 // threads add a quarter of them each, four segments' loads in flight (one
 // thread per sum and one load after another: 1024 x 1024 at 16 tokens 79 us,
-// 272 x 7056 132 us, 14336 x 4096 119 us; so 37, 47 and 115 us).  The sums are read along the slabs and written along the rows, by way of shared memory.
+// 272 x 7056 132 us, 14336 x 4096 119 us; so 37, 47 and 115 us).  The sums are
+// read along the slabs and written along the rows, by way of shared memory.
 constexpr int OT = 256, OQ = 4, OJ = 8;
 __global__ void __launch_bounds__(OT * OQ) fused_out_kernel(FusedArgs a, const uint32_t* __restrict__ gseg0,
                                                             const uint32_t* __restrict__ gsegs, Epilogue e) {

@@ -8,7 +8,7 @@
 // rows, 32 KB a slice, and tcgen05.mma cta_group::2 reads both.  A persistent
 // CTA (or pair) per SM takes tiles; within it
 //   * one thread loads 64-column slices of x and W by TMA (128-byte swizzled
-//     rows, zero past the edges) into a ring of stages,
+//     rows, zero past the edges), two to a stage, into a ring of stages,
 //   * one thread (of the pair's first CTA) issues tcgen05.mma kind::f16,
 //     M = 128 (256) tokens, N = tn, K = 16, into one of two TMEM accumulators,
 //   * eight warps read the other accumulator (a lane is a token, its registers
@@ -19,8 +19,8 @@
 // result is rounded a hundred times coarser.  For FP32 results (EXACT) an
 // accumulator holds 512 columns only, and the epilogue's warps add its sums to
 // theirs, in registers, rounded to nearest: relative error 4.8e-7 at every
-// length (1024 columns: 1.0e-6), with the decode 166 us against 160 at 77
-// tokens, 288 against 256 at 2048 (4096 x 14336).
+// length (1024 columns: 1.0e-6), with the decode 150 us against 141 at 77
+// tokens, 272 against 244 at 2048 (4096 x 14336).
 // gemm_plan chooses tn and the pair by a model of both costs.  Tokens as the
 // MMA's rows rather than weight rows: y is token-major, so a lane's results
 // are contiguous.
@@ -40,10 +40,14 @@ namespace xksv {
 namespace {
 
 constexpr int GM = 128;          // tokens of a tile
-constexpr int GK = 64;           // columns of a stage: 128-byte rows
+constexpr int GK = 64;           // columns of a slice: 128-byte rows
 constexpr int EPI = 256;         // epilogue threads: two warps for each 32 tokens
 constexpr int GTHREADS = 64 + EPI;  // producer and MMA warps besides
-constexpr uint32_t kExactSlices = 8;  // slices (512 columns) of an accumulator, EXACT
+// Slices of a stage.  The threads that copy and multiply wait once a stage, and
+// those waits limited tiles of few rows: 4096 x 14336 with 77 tokens 75 us a
+// slice at a time, 55 us two; with 2048 tokens and FP32 results 193, 182 us.
+constexpr uint32_t SL = 2;
+constexpr uint32_t kExact = 4;  // stages (512 columns) of an accumulator, EXACT
 constexpr uint32_t kMaxStages = 8;
 constexpr uint32_t kABytes = GM * GK * 2;
 constexpr size_t kRing = 220 * 1024;  // stages' shared memory
@@ -160,10 +164,10 @@ __global__ void __launch_bounds__(GTHREADS, 1)
   uint32_t rank = 0;
   if (PAIR) asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(rank));
   const uint32_t bn = a.tn / CTAS;  // weight rows that this CTA brings
-  const uint32_t stage_bytes = kABytes + bn * GK * 2;
+  const uint32_t w_bytes = bn * GK * 2, stage_bytes = SL * (kABytes + w_bytes);
   const uint32_t mt = (a.batch + TM - 1) / TM, nt = (a.rows + a.tn - 1) / a.tn, tiles = mt * nt;
-  const uint32_t ksteps = (a.cols + GK - 1) / GK;
-  const uint32_t kpart = EXACT ? kExactSlices : ksteps;  // slices of an accumulator
+  const uint32_t ksteps = (a.cols + SL * GK - 1) / (SL * GK);
+  const uint32_t kpart = EXACT ? kExact : ksteps;  // stages of an accumulator
   const uint32_t first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;  // this CTA's (pair's) tiles
   if (warp == 1) {
     if (PAIR) {
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(GTHREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      // stage and round of the next slice, stepped along: a division a slice
+      // stage and round of the next copy, stepped along: a division for each
       // would take this thread longer than the MMAs
       uint32_t n = 0, s = 0, round = 0;
       for (uint32_t t = first; t < tiles && ok; t += stride) {
@@ -213,12 +217,18 @@ __global__ void __launch_bounds__(GTHREADS, 1)
           if (rank == 0) expect_bytes(smem_addr(&S.full[s]), CTAS * stage_bytes);
           if (PAIR) {
             const uint32_t bar = in_cta(smem_addr(&S.full[s]), 0);
-            tma_load_pair(dst, &mx, k * GK, m0, bar);
-            tma_load_pair(dst + kABytes, &mw, k * GK, n0, bar);
+#pragma unroll
+            for (uint32_t q = 0; q < SL; ++q) {
+              tma_load_pair(dst + q * kABytes, &mx, (SL * k + q) * GK, m0, bar);
+              tma_load_pair(dst + SL * kABytes + q * w_bytes, &mw, (SL * k + q) * GK, n0, bar);
+            }
           } else {
             const uint32_t bar = smem_addr(&S.full[s]);
-            tma_load(dst, &mx, k * GK, m0, bar);
-            tma_load(dst + kABytes, &mw, k * GK, n0, bar);
+#pragma unroll
+            for (uint32_t q = 0; q < SL; ++q) {
+              tma_load(dst + q * kABytes, &mx, (SL * k + q) * GK, m0, bar);
+              tma_load(dst + SL * kABytes + q * w_bytes, &mw, (SL * k + q) * GK, n0, bar);
+            }
           }
           if (++s == a.stages) {
             s = 0;
@@ -235,25 +245,27 @@ __global__ void __launch_bounds__(GTHREADS, 1)
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t idesc = umma_idesc_bf16(TM, a.tn);
-      uint32_t n = 0, ai = 0;  // slices multiplied, accumulators begun
+      uint32_t n = 0, ai = 0;  // stages multiplied, accumulators begun
       uint32_t s = 0, round = 0;
       const uint64_t desc0 = desc_sw128(smem_addr(ring));
       for (uint32_t t = first; t < tiles && ok; t += stride) {
         for (uint32_t k0 = 0; k0 < ksteps && ok; k0 += kpart, ++ai) {
           const uint32_t buf = ai & 1, d = tmem + buf * (a.tmem_cols / 2);
-          const uint32_t slices = min(kpart, ksteps - k0);
+          const uint32_t parts = min(kpart, ksteps - k0);
           ok = wait_or_abort(smem_addr(&S.tempty[buf]), ((ai >> 1) & 1) ^ 1, &S.abort_flag);
           if (!ok) break;
           tc_fence_after();
-          for (uint32_t k = 0; k < slices; ++k, ++n) {
+          for (uint32_t k = 0; k < parts; ++k, ++n) {
             ok = wait_or_abort(smem_addr(&S.full[s]), round & 1, &S.abort_flag);
             if (!ok) break;
             tc_fence_after();
             // (addresses below 256 KB: a descriptor's address field does not overflow)
-            const uint64_t da = desc0 + ((s * stage_bytes) >> 4), db = da + (kABytes >> 4);
+            const uint64_t da = desc0 + ((s * stage_bytes) >> 4), db = da + ((SL * kABytes) >> 4);
 #pragma unroll
-            for (uint32_t j = 0; j < GK / 16; ++j)  // 32 bytes further along the rows
-              mma_f16<PAIR>(d, da + 2 * j, db + 2 * j, idesc, (k | j) != 0);
+            for (uint32_t q = 0; q < SL; ++q)
+#pragma unroll
+              for (uint32_t j = 0; j < GK / 16; ++j)  // 32 bytes further along the rows
+                mma_f16<PAIR>(d, da + q * (kABytes >> 4) + 2 * j, db + q * (w_bytes >> 4) + 2 * j, idesc, (k | q | j) != 0);
             commit<PAIR>(smem_addr(&S.empty[s]));
             if (++s == a.stages) {
               s = 0;
@@ -427,7 +439,7 @@ cudaError_t launch_linear_gemm(const void* w, uint32_t rows, uint32_t cols, cons
   const GemmPlan plan = gemm_plan(batch, rows, cols, sms);
   const uint32_t ctas = plan.pair ? 2 : 1;
   a.tn = plan.tn;
-  const uint32_t stage = kABytes + a.tn / ctas * GK * 2;
+  const uint32_t stage = SL * (kABytes + a.tn / ctas * GK * 2);
   a.stages = std::min<uint32_t>(kMaxStages, uint32_t(kRing / stage));
   a.tmem_cols = 32;
   while (a.tmem_cols < 2 * ((a.tn + 31) / 32 * 32)) a.tmem_cols *= 2;
