@@ -356,7 +356,10 @@ typedef struct xksv_linear_args {
  * contents free before and after; calls that may overlap need their own (and
  * their own plan: one call in flight per plan).  Allocates nothing, so it can
  * be captured into a graph.  A tile index (xksv_plan_index) speeds it up as
- * it does xksv_plan_gemm.  Returns 1 without launching for a slab outside the
+ * it does xksv_plan_gemm, and xksv_plan_set_gemm_route selects the route of 4
+ * to 128 tokens here too (XKSV_GEMM_AUTO: fused up to 64 tokens; past them,
+ * and for other plans of columns in multiples of 8, the weight is decoded into
+ * the workspace, 2 bytes an element).  Returns 1 without launching for a slab outside the
  * payload, x or y, two slabs covering the same row of Y, a raw slab that is
  * not rows x cols, unknown types or activations, or a workspace too small;
  * batch 0 does nothing.  Slab errors are read with xksv_plan_status.  As in

@@ -129,6 +129,21 @@ def test_linear_matches_64_bits(name, batch):
     plan.close()
 
 
+@pytest.mark.parametrize("name", ["serial", "serial-many"])
+@pytest.mark.parametrize("route", [xg.GEMM_FUSED, xg.GEMM_SCRATCH])
+@pytest.mark.parametrize("batch", [4, 64, 65, 100, 128])
+def test_linear_routes_that_a_caller_picks(name, route, batch):
+    payload, entries, ws, xn, yn = build(name)
+    plan = xg.Plan(entries)
+    assert plan.index(payload) == 0
+    auto = plan.linear_workspace(batch)
+    plan.set_gemm_route(route)
+    check(plan, payload, ws, xn, yn, batch, bias="fp32", act="gelu", residual="bf16", seed=batch)
+    # the default decodes on its own past 64 tokens
+    assert (plan.linear_workspace(batch) == auto) or (route == xg.GEMM_FUSED) == (batch > 64)
+    plan.close()
+
+
 @pytest.mark.parametrize("act", list(xg.ACTS))
 @pytest.mark.parametrize("batch", [1, 3, 20, 200])
 def test_linear_epilogues(act, batch):

@@ -1064,7 +1064,12 @@ LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload
   const bool all = indexed && p->n_ser_idx == p->n_ser + p->n_par + p->n_raw;
   if (all && batch <= 3) {
     s.route = Route::Tile;
-  } else if (payload && gemm_fused(p, payload, batch)) {
+  } else if (payload && gemm_fused(p, payload, batch) &&
+             (batch <= 64 || !p->tc_ok || p->gemm_route == XKSV_GEMM_FUSED)) {
+    // the decode's work grows with the tokens here: past 64 a decode of its own
+    // and the GEMM are faster (4096 x 4096: 64 tokens 55 us both ways, 128
+    // tokens 71 against 54; 14336 x 4096: 133 against 141, 163 against 141;
+    // 4096 x 14336: 123 against 151, 146 against 151)
     s.route = Route::Fused;
     s.z = c.take(uint64_t(p->n_fsegs) * 16 * ((batch + 15) / 16 * 16) * 32 * sizeof(float));
     s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
