@@ -166,10 +166,12 @@ int xksv_plan_launches(const xksv_plan* plan);
  * threads per tile) instead of re-synchronising each slab's single bit
  * stream on every call.
  * Serial-codec slabs of other shapes up to 16 rows get an index for decoding
- * (xksv_plan_decode, and layers that decode first).  Of the plan's parallel-codec slabs, when they are too few to fill the GPU
- * with one warp each, it records where parts of their substreams begin (4
- * bytes per 128 or more codes), so that a decode shares each slab among
- * several warps.
+ * (xksv_plan_decode, and layers that decode first).  Of the plan's
+ * parallel-codec slabs, when they are too few to fill the GPU with one warp
+ * each and the largest has 16384 elements or more, it records where parts of
+ * their substreams begin (4 bytes per 32 or more codes) and their decode
+ * tables (10 KB a slab), so that a decode shares each slab among several
+ * warps.
  * The index describes the payload's contents at this call: rebuild it if they
  * change.  No reference counterpart (the reference decodes every slab from
  * its first bit, cuda/decode.cu:12-45); it is an acceleration structure on

@@ -50,6 +50,23 @@ def test_parallel_parts_decode_the_same_bytes(shapes, kind):
     plan.close()
 
 
+@pytest.mark.parametrize("shapes", [[(16, 1024)] * 2, [(16, 1008)], [(16, 1032), (1, 64), (2, 33)], [(13, 1300)] * 40])
+@pytest.mark.parametrize("kind", ["normal002", "uniform", "three_exp"])
+def test_parallel_parts_of_few_codes(shapes, kind):
+    """Around the smallest slabs that are shared, and parts of two groups."""
+    payload, entries, want = slabs(shapes, xg.CODEC_PARALLEL32, kind, 9)
+    plan = xg.Plan(entries)
+    assert plan.index(payload) == 0
+    out = torch.full((want.size * 2 + 8,), 0xEE, dtype=torch.uint8, device=DEV)
+    for _ in range(2):
+        plan.decode(payload, out)
+        assert plan.status() == 0
+        got = out.cpu().numpy()
+        assert (got[:want.size * 2].view("<u2") == want).all() and (got[want.size * 2:] == 0xEE).all()
+        assert plan.index(payload) == 0  # built again
+    plan.close()
+
+
 def test_parallel_parts_report_a_changed_stream():
     payload, entries, want = slabs([(16, 8192)], xg.CODEC_PARALLEL32, "normal002", 3)
     plan = xg.Plan(entries)

@@ -232,6 +232,7 @@ struct xksv_plan {
   // part index of the parallel slabs (xksv_plan_index of few slabs)
   uint32_t par_parts = 1;
   uint32_t* d_ppos = nullptr;
+  void* d_ptabs = nullptr;  // kPartTabBytes a slab
   uint32_t n_fgroups = 0, n_fsegs = 0;
   uint32_t* d_fgsegs = nullptr;  // group g's segments: entries [e[g], e[g + 1]) behind the n_fgroups + 1 first
   uint64_t* d_hash_ranges = nullptr;  // per slab in creation order: {dst, decoded bytes}
@@ -276,8 +277,10 @@ void free_index(xksv_plan* p) {
   if (p->d_ftabs) cudaFree(p->d_ftabs);
   if (p->d_fgsegs) cudaFree(p->d_fgsegs);
   if (p->d_ppos) cudaFree(p->d_ppos);
+  if (p->d_ptabs) cudaFree(p->d_ptabs);
   free_ragged(p);
   p->d_ppos = nullptr;
+  p->d_ptabs = nullptr;
   p->par_parts = 1;
   p->d_fgsegs = nullptr;
   p->d_ftabs = nullptr;
@@ -701,7 +704,8 @@ namespace {
 // payload's index has them.
 cudaError_t parallel_decode(xksv_plan* p, const xksv::Slab* slabs, const uint8_t* pay, uint8_t* out, cudaStream_t st) {
   if (p->d_ppos && pay == p->indexed_payload)
-    return xksv::launch_parallel_parts(slabs, p->n_par, pay, out, p->d_ppos, p->par_parts, p->d_status, p->par_whole, st);
+    return xksv::launch_parallel_parts(slabs, p->n_par, pay, out, p->d_ppos, p->par_parts, p->d_ptabs, p->d_status, p->par_whole,
+                                       st);
   return xksv::launch_parallel_decode(slabs, p->n_par, pay, out, p->d_status, p->grid_par, st, p->par_whole);
 }
 
@@ -1393,9 +1397,10 @@ static void setup_parts(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   const uint32_t parts = parallel_parts(most, p->n_par, p->sms);
   if (parts < 2) return;
   const size_t bytes = size_t(p->n_par) * parts * 32 * sizeof(uint32_t);
-  const bool ok = cudaMalloc(&p->d_ppos, bytes) == cudaSuccess && cudaMemsetAsync(p->d_ppos, 0, bytes, st) == cudaSuccess &&
+  const bool ok = cudaMalloc(&p->d_ppos, bytes) == cudaSuccess &&
+                  cudaMalloc(&p->d_ptabs, p->n_par * kPartTabBytes) == cudaSuccess && cudaMemsetAsync(p->d_ppos, 0, bytes, st) == cudaSuccess &&
                   cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
-                  launch_parallel_index(p->d_slabs + p->n_ser, p->n_par, d_payload, p->d_ppos, parts, p->d_status, st) ==
+                  launch_parallel_index(p->d_slabs + p->n_ser, p->n_par, d_payload, p->d_ppos, parts, p->d_ptabs, p->d_status, st) ==
                       cudaSuccess &&
                   cudaMemcpyAsync(p->h_status, p->d_status, sizeof(int), cudaMemcpyDeviceToHost, st) == cudaSuccess &&
                   cudaStreamSynchronize(st) == cudaSuccess && *p->h_status == 0;
@@ -1406,7 +1411,9 @@ static void setup_parts(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
     return;
   }
   if (p->d_ppos) cudaFree(p->d_ppos);
+  if (p->d_ptabs) cudaFree(p->d_ptabs);
   p->d_ppos = nullptr;
+  p->d_ptabs = nullptr;
 }
 
 int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, void* stream) {

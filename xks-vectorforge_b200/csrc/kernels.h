@@ -32,13 +32,15 @@ struct GemvTabs;
 cudaError_t launch_parallel_decode(const Slab* slabs, uint32_t n, const uint8_t* payload,
                                    uint8_t* out, int* status, int grid, cudaStream_t st, bool whole);
 // Part index of parallel slabs (pos[slab][part][lane]: where each of `parts`
-// parts of every substream begins) and the decode that uses it: n * parts
-// warps instead of n.  parallel_parts: parts worth having for n slabs of at
-// most max_elements elements (1: none).
+// parts of every substream begins; tabs: every slab's decode tables,
+// kPartTabBytes each) and the decode that uses it: n * parts warps instead of
+// n.  parallel_parts: parts worth having for n slabs of at most max_elements
+// elements (1: none).
 cudaError_t launch_parallel_index(const Slab* slabs, uint32_t n, const uint8_t* payload, uint32_t* pos, uint32_t parts,
-                                  int* status, cudaStream_t st);
+                                  void* tabs, int* status, cudaStream_t st);
 cudaError_t launch_parallel_parts(const Slab* slabs, uint32_t n, const uint8_t* payload, uint8_t* out, uint32_t* pos,
-                                  uint32_t parts, int* status, bool whole, cudaStream_t st);
+                                  uint32_t parts, void* tabs, int* status, bool whole, cudaStream_t st);
+constexpr size_t kPartTabBytes = 10240;
 uint32_t parallel_parts(uint64_t max_elements, uint32_t n, int sms);
 // The slab's 32 substreams start at whole 16-word rows of its tiles.
 inline bool parallel_whole(uint64_t rows, uint64_t cols) { return rows == 16 && cols % 32 == 0; }

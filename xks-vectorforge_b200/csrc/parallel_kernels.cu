@@ -95,11 +95,21 @@ struct Seg {
   uint64_t room;   // bytes of the substream from sm on
 };
 
+// A slab's tables as its index pass built them.
+struct PartTabs {
+  ldec::Tables<PCfg> t;
+  uint32_t F[32], L2[32];
+  int32_t maxlen[32], kind[32];  // kind: build_tables' answer (1: the generic decoder's)
+};
+static_assert(sizeof(ldec::Tables<PCfg>) % 16 == 0 && sizeof(PartTabs) % 16 == 0, "copied in 16-byte pieces");
+static_assert(sizeof(PartTabs) <= kPartTabBytes, "the caller's allocation");
+
 // A part of every substream of a slab: sixteen-code groups [part * per,
 // (part + 1) * per) of each, the last part with what follows.
 struct PartIndex {
   uint32_t* pos;   // [slab][part][lane]: bit offset of the part's first code (part 0: not stored)
   uint32_t parts;  // of every slab
+  PartTabs* tabs;  // per slab: its substreams' tables, which every part would build again
 };
 __device__ __forceinline__ uint32_t groups_per_part(uint32_t total, uint32_t chunks, uint32_t parts) {
   const uint32_t most = (total + chunks - 1) / chunks / 16;
@@ -133,7 +143,7 @@ __device__ __forceinline__ void emit_one(const Out& o, uint32_t p, uint32_t word
 // whole rows, their places stepped along instead of divided out, and stored
 // in fours where start and columns are multiples of four (128 slabs of
 // 16 x 1848: 614 us one code at a time, 130 us in twos, 78 us so; in seven
-// parts 65 and 33 us).
+// parts that build their tables 65 and 33 us).
 template <int MODE>
 __device__ __forceinline__ bool ragged_codes(const Seg s, WarpTabs& W, int lane, const ldec::Code lc, ldec::Stream b, const Out o) {
   bool bad = false;
@@ -469,6 +479,10 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
       if (active && lok && c0 > len - kHdr) c0 = c1 = 0;         // (a header the checks below refuse)
     }
     const uint32_t part_end = PART && !last_part ? uint32_t(s.nbits) : 0;
+    const PartTabs* saved = PART ? pi.tabs + si : nullptr;
+    if (PART)
+      for (uint32_t k = lane; k < sizeof(ldec::Tables<PCfg>) / 16; k += 32)
+        cp_async16(reinterpret_cast<uint4*>(&W.t) + k, reinterpret_cast<const uint4*>(&saved->t) + k);
     if (active && lok) {
       lok = base + len <= n;
       if (lok) {
@@ -477,7 +491,7 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
         // the warp's table memory, idle until the fill pass) and its first
         // sign/mantissa chunks (the substream holds `expect` of them when
         // the slab is well formed; the copies stay inside the slab anyway)
-        ldec::stage_lengths<PCfg>(W.t, q + 16, lane);
+        if (!PART) ldec::stage_lengths<PCfg>(W.t, q + 16, lane);
         if (rows16) {
           const uint8_t* sm = q + kHdr + c0;
           const uint8_t* sme = sm + (expect - c0) <= p + n ? sm + (expect - c0) : p + n;
@@ -531,12 +545,25 @@ __global__ void __launch_bounds__(PWARPS * 32, MODE == 0 ? 8 : 1)
     ldec::Code lc{0, 0, 0};
     uint32_t L = 0;
     int tb = 0;
-    if (active) {
+    if (PART) {
+      if (active) tb = saved->kind[lane];
+      lc.F = saved->F[lane];
+      lc.maxlen = saved->maxlen[lane];
+    } else if (active) {
       ldec::TabLens<PCfg> lens(W.t, s.lens, &W.ring[kSaveChunk], lane);
       tb = ldec::build_tables<PCfg>(lens, W.t, W.lpos, lane, lc.F, lc.maxlen, L);
     }
-    lc.L2 = L << PCfg::K2;
+    lc.L2 = PART ? saved->L2[lane] : L << PCfg::K2;
     __syncwarp();
+    if (MODE == 2) {  // for the decodes by parts
+      PartTabs& to = pi.tabs[si];
+      for (uint32_t k = lane; k < sizeof(ldec::Tables<PCfg>) / 16; k += 32)
+        reinterpret_cast<uint4*>(&to.t)[k] = reinterpret_cast<const uint4*>(&W.t)[k];
+      to.F[lane] = lc.F;
+      to.L2[lane] = lc.L2;
+      to.maxlen[lane] = lc.maxlen;
+      to.kind[lane] = tb;
+    }
     if (np) {  // next slab's substream headers and length tables to L2
       const uint64_t nch = ntotal < 32 ? ntotal : 32;
       const bool na = uint64_t(lane) < nch;
@@ -642,20 +669,20 @@ cudaError_t launch_parallel_decode(const Slab* slabs, uint32_t n, const uint8_t*
 }
 
 cudaError_t launch_parallel_index(const Slab* slabs, uint32_t n, const uint8_t* payload, uint32_t* pos, uint32_t parts,
-                                  int* status, cudaStream_t st) {
+                                  void* tabs, int* status, cudaStream_t st) {
   if (!n) return cudaSuccess;
   set_attr_once();
   parallel_slab_kernel<2, false, false><<<(n + PWARPS - 1) / PWARPS, PWARPS * 32, kSmemBytes[0], st>>>(
-      slabs, n, payload, nullptr, nullptr, nullptr, 1, 1, status, PartIndex{pos, parts});
+      slabs, n, payload, nullptr, nullptr, nullptr, 1, 1, status, PartIndex{pos, parts, static_cast<PartTabs*>(tabs)});
   return cudaGetLastError();
 }
 
 cudaError_t launch_parallel_parts(const Slab* slabs, uint32_t n, const uint8_t* payload, uint8_t* out, uint32_t* pos,
-                                  uint32_t parts, int* status, bool whole, cudaStream_t st) {
+                                  uint32_t parts, void* tabs, int* status, bool whole, cudaStream_t st) {
   if (!n) return cudaSuccess;
   set_attr_once();
   const uint32_t g = (n * parts + PWARPS - 1) / PWARPS;
-  const PartIndex pi{pos, parts};
+  const PartIndex pi{pos, parts, static_cast<PartTabs*>(tabs)};
   if (whole)
     parallel_slab_kernel<0, true, true><<<g, PWARPS * 32, kSmemBytes[0], st>>>(slabs, n, payload, out, nullptr, nullptr, 1, 1, status, pi);
   else
@@ -664,10 +691,15 @@ cudaError_t launch_parallel_parts(const Slab* slabs, uint32_t n, const uint8_t* 
 }
 
 uint32_t parallel_parts(uint64_t max_elements, uint32_t n, int sms) {
-  // a part of 128 codes or more a lane (its warp builds the slab's tables
-  // again, about 300 codes' time), and no more warps than the GPU holds
+  // Parts of 32 codes or more a lane, and no more warps than the GPU holds.
+  // The saved tables (10 KB a slab) take the place of each part's own build:
+  // 4096 x 4096 decoded and multiplied by 16 tokens 64 us in parts that build,
+  // 49 us so; 2040 x 1848 44 us, 34 us in parts of 128 codes, 31 us so.
+  // Slabs below 512 codes a lane (25 KB) have none: the tables would weigh
+  // half of them.
   const uint64_t codes = max_elements / 32, fill = n ? uint64_t(sms) * 16 / n : 0;
-  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({fill, codes / 128, 64})));
+  if (codes < 512) return 1;
+  return uint32_t(std::max<uint64_t>(1, std::min<uint64_t>({fill, codes / 32, 64})));
 }
 
 cudaError_t launch_parallel_gemm(const Slab* slabs, uint32_t n, const uint8_t* payload,
