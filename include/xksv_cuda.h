@@ -458,8 +458,8 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* str
  * FP32.  A length that is negative or above table_cols * page_size gives
  * zeros and -infinity, a page outside the cache counts as masked; both are
  * reported by xksv_kv_status.  d_workspace: as for xksv_plan_linear, of at
- * least xksv_kv_attend_workspace(kv, seqs, q_heads, table_cols) bytes.  The
- * work is split over the tokens and joined in a fixed order: the same call
+ * least xksv_kv_attend_workspace(kv, seqs, q_heads, table_cols) bytes (0 for
+ * few sequences of short tables: NULL will do).  The work is split over the tokens and joined in a fixed order: the same call
  * gives the same bits. */
 typedef struct xksv_kv_attend_args {
   const void* q;

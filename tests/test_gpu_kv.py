@@ -221,9 +221,12 @@ def attend64(q, k, v, lens, table, page, scale, window=0, softcap=0.0):
     return out, lse, tol, tol_lse
 
 
-def check_attend(kind, cache, lens, page, Q, H, D, layout, window=0, softcap=0.0, scale=None, seed=0, q_mag=1.0):
+def check_attend(kind, cache, lens, page, Q, H, D, layout, window=0, softcap=0.0, scale=None, seed=0, q_mag=1.0,
+                 wide=0):
     g = gen(seed)
     table, pages = table_of(g, lens, page)
+    if wide:  # a table of `wide` more columns, unused
+        table = torch.cat([table, torch.full((len(lens), wide), -1, dtype=torch.int32, device=DEV)], 1)
     k, v, ks, vs, c = make_cache(g, cache, pages, page, H, D, layout)
     # whatever lies behind a sequence's last token must not matter
     for i, n in enumerate(lens):
@@ -262,6 +265,26 @@ def test_attend_lengths_and_types(lens, kind, cache):
                                                (256, "nhd", "bf16")])
 def test_attend_heads_and_pages(Q, H, D, page, layout, cache):
     check_attend("bf16", cache, [301, 1, 64], page, Q, H, D, layout, seed=Q + D)
+
+
+# The same with tables of room for many more tokens: these calls split the
+# work over all warps and join in a second kernel.
+@pytest.mark.parametrize("lens", LENS)
+@pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "e4m3"), ("fp16", "e4m3")])
+def test_attend_in_a_long_table(lens, kind, cache):
+    check_attend(kind, cache, lens, 16, 8, 2, 128, "nhd", seed=len(lens), wide=5000)
+
+
+@pytest.mark.parametrize("Q,H,D", [(1, 1, 64), (7, 7, 80), (12, 2, 96), (32, 8, 128), (24, 1, 64), (40, 2, 256),
+                                   (6, 3, 192), (9, 3, 16), (130, 2, 32), (3, 1, 144), (17, 1, 48)])
+@pytest.mark.parametrize("page,layout,cache", [(16, "nhd", "bf16"), (1, "hnd", "e4m3"), (48, "hnd", "bf16"), (7, "nhd", "e4m3")])
+def test_attend_heads_and_pages_in_a_long_table(Q, H, D, page, layout, cache):
+    check_attend("bf16", cache, [301, 1, 64], page, Q, H, D, layout, seed=Q + D, wide=5000)
+
+
+@pytest.mark.parametrize("window,softcap", [(1, 0.0), (15, 20.0), (64, 0.0), (5000, 20.0)])
+def test_attend_window_and_softcap_in_a_long_table(window, softcap):
+    check_attend("bf16", "bf16", [333, 16, 1, 100], 16, 8, 2, 128, "nhd", window=window, softcap=softcap, seed=3, wide=500)
 
 
 @pytest.mark.parametrize("window", [1, 15, 16, 64, 100, 5000])

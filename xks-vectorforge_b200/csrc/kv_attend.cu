@@ -28,9 +28,11 @@
 //   * A unit that one warp holds alone is written at once; the others leave
 //     their pieces (sums, maximum, weight) in slots, which the second kernel
 //     joins in a fixed order: results do not depend on timing.
+//   * Calls of few units over short tables give each unit a cluster of CTAs
+//     instead, which joins its pieces through shared memory (CL, kShort).
 // Measured on one B200 (32 query and 8 KV heads of 128, BF16): 131071 tokens
 // of one sequence 100 us, 5370 GB/s with the join (a copy: 6554); 64 uneven
-// sequences to 16384 tokens 395 us, 5440 GB/s; one of 777 tokens 10 us.  E4M3,
+// sequences to 16384 tokens 395 us, 5440 GB/s; one of 777 tokens 7.5 us.  E4M3,
 // 28 and 4 heads, 130 uneven sequences to 6000: 86 us, 4360 GB/s, the
 // conversion's instructions besides the reads.
 #include <cuda_bf16.h>
@@ -49,6 +51,8 @@ namespace xksv {
 namespace {
 
 constexpr int kWarps = 4;   // per CTA
+constexpr int kCluster = 8;  // CTAs of a unit whose pieces meet in shared memory (CL)
+static_assert(kCluster * kWarps == 32, "the join reads a piece's statistics per lane");
 constexpr int kStages = 2;  // blocks in a warp's ring: one landing while one is worked on
 
 // Shape of a kernel: the cache's elements (E8: E4M3), rows padded to DP dims,
@@ -152,8 +156,24 @@ struct Ranges {
   uint64_t before[kWarps];  // blocks ahead of that sequence
 };
 
+// A float of this shared-memory address in CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;\n" ::: "memory");
+}
+
 // MB: BF16 products (else FP16); FULL: head_dim is DP.
-template <bool MB, bool E8, int DP, int NG, bool FULL>
+// CL (calls of few units and short tables): a unit's blocks are shared by the
+// 32 warps of a cluster of CTAs, which then join their pieces from one
+// another's shared memory: no second kernel and no workspace.
+template <bool MB, bool E8, int DP, int NG, bool FULL, bool CL>
 __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_attend_kernel(const AttendArgs p, const AttendPlan pl) {
   using Sh = Shape<E8, DP, NG>;
   constexpr int CH = Sh::CH, BT = Sh::BT, RB = Sh::RB;
@@ -172,52 +192,77 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
 
   // ---- the blocks of all sequences, and where this CTA's warps start ----
   const uint64_t S = p.a.seqs;
-  const uint64_t per = (S + kWarps * 32 - 1) / (kWarps * 32), s0 = min(S, per * threadIdx.x), s1 = min(S, s0 + per);
+  KvShare share{};
+  uint32_t me = 0;
+  uint64_t a = 0, b = 0;
+  const uint32_t cl_seq = CL ? blockIdx.x / kCluster / U : 0, cl_unit = CL ? blockIdx.x / kCluster % U : 0;
+  const uint32_t cl_group = p.a.q_heads / p.c.kv_heads, cl_chunk = cl_unit % pl.chunks;
+  const uint32_t cl_head0 = cl_unit / pl.chunks * cl_group + cl_chunk * pl.heads;
+  const uint32_t cl_heads = CL ? min(pl.heads, cl_group - cl_chunk * pl.heads) : 0;
   auto span_of = [&](uint64_t s) { return kv_span(p.a.lens[s], p.a.table_cols, p.c.page_size, p.a.window); };
   auto blocks_of = [&](uint64_t s) { return kv_blocks(span_of(s), BT) * U; };
-  uint64_t mine = 0;
-  for (uint64_t s = s0; s < s1; ++s) {
-    mine += blocks_of(s);
-    if (blockIdx.x == 0 && !span_of(s).ok) atomicOr(p.status, kStatusHeader);
-  }
-  uint64_t incl = mine;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint64_t x = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += x;
-  }
-  if (lane == 31) wsum[warp] = incl;
-  __syncthreads();
-  uint64_t total = 0, ahead = incl - mine;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) ahead += wsum[w];
-    total += wsum[w];
-  }
-  // sequences without a token to attend to: zeros, by the CTAs in turn
-  for (uint64_t s = blockIdx.x; s < S; s += gridDim.x) {
-    if (blocks_of(s)) continue;
-    uint16_t* out = static_cast<uint16_t*>(p.a.out) + s * p.a.out_stride[0];
-    for (uint32_t x = threadIdx.x; x < p.a.q_heads * D; x += kWarps * 32) out[x / D * p.a.out_stride[1] + x % D] = 0;
-    for (uint32_t h = threadIdx.x; p.a.lse && h < p.a.q_heads; h += kWarps * 32) p.a.lse[s * p.a.q_heads + h] = -INFINITY;
-  }
-  const KvShare share = kv_share(total, pl.warps);
-  for (int w = 0; w < kWarps; ++w) {
-    const uint32_t i = blockIdx.x * kWarps + w;
-    if (i >= share.workers) break;
-    const uint64_t a = kv_start(share, i);
-    if (a >= ahead && a < ahead + mine) {
-      uint64_t at = ahead, s = s0;
-      for (uint64_t n; at + (n = blocks_of(s)) <= a; ++s) at += n;
-      R.seq[w] = uint32_t(s);
-      R.before[w] = at;
+  if constexpr (CL) {
+    const KvSpan sp = span_of(cl_seq);
+    const uint32_t rank = blockIdx.x % kCluster;
+    if (!sp.ok && cl_unit == 0 && rank == 0 && threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
+    share = kv_share(kv_blocks(sp, BT), kCluster * kWarps);
+    if (!share.total) {  // the whole cluster: nothing to attend to
+      if (rank) return;
+      for (uint32_t h = warp; h < cl_heads; h += kWarps) {
+        uint16_t* out = static_cast<uint16_t*>(p.a.out) + cl_seq * p.a.out_stride[0] + (cl_head0 + h) * p.a.out_stride[1];
+        for (uint32_t d = lane; d < D; d += 32) out[d] = 0;
+        if (lane == 0 && p.a.lse) p.a.lse[uint64_t(cl_seq) * p.a.q_heads + cl_head0 + h] = -INFINITY;
+      }
+      return;
     }
+    me = rank * kWarps + warp;
+    if (me < share.workers) a = kv_start(share, me), b = kv_start(share, me + 1);
+  } else {
+    const uint64_t per = (S + kWarps * 32 - 1) / (kWarps * 32), s0 = min(S, per * threadIdx.x), s1 = min(S, s0 + per);
+    uint64_t mine = 0;
+    for (uint64_t s = s0; s < s1; ++s) {
+      mine += blocks_of(s);
+      if (blockIdx.x == 0 && !span_of(s).ok) atomicOr(p.status, kStatusHeader);
+    }
+    uint64_t incl = mine;
+  #pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint64_t x = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += x;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    uint64_t total = 0, ahead = incl - mine;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) ahead += wsum[w];
+      total += wsum[w];
+    }
+    // sequences without a token to attend to: zeros, by the CTAs in turn
+    for (uint64_t s = blockIdx.x; s < S; s += gridDim.x) {
+      if (blocks_of(s)) continue;
+      uint16_t* out = static_cast<uint16_t*>(p.a.out) + s * p.a.out_stride[0];
+      for (uint32_t x = threadIdx.x; x < p.a.q_heads * D; x += kWarps * 32) out[x / D * p.a.out_stride[1] + x % D] = 0;
+      for (uint32_t h = threadIdx.x; p.a.lse && h < p.a.q_heads; h += kWarps * 32) p.a.lse[s * p.a.q_heads + h] = -INFINITY;
+    }
+    share = kv_share(total, pl.warps);
+    for (int w = 0; w < kWarps; ++w) {
+      const uint32_t i = blockIdx.x * kWarps + w;
+      if (i >= share.workers) break;
+      const uint64_t a = kv_start(share, i);
+      if (a >= ahead && a < ahead + mine) {
+        uint64_t at = ahead, s = s0;
+        for (uint64_t n; at + (n = blocks_of(s)) <= a; ++s) at += n;
+        R.seq[w] = uint32_t(s);
+        R.before[w] = at;
+      }
+    }
+    __syncthreads();
+    me = blockIdx.x * kWarps + warp;
+    if (me >= pl.warps) return;
+    if (lane == 0) p.joins[me] = make_int4(0, 0, 0, 0);
+    if (me >= share.workers) return;  // all of them when there is no block
+    a = kv_start(share, me), b = kv_start(share, me + 1);
   }
-  __syncthreads();
-  const uint32_t me = blockIdx.x * kWarps + warp;
-  if (me >= pl.warps) return;
-  if (lane == 0) p.joins[me] = make_int4(0, 0, 0, 0);
-  if (me >= share.workers) return;  // all of them when there is no block
-  const uint64_t a = kv_start(share, me), b = kv_start(share, me + 1);
 
   uint8_t* ws = smem + warp * Sh::WARP;
   const uint32_t ring = smem_addr(ws), qsm = ring + kStages * 2 * Sh::KV;
@@ -256,9 +301,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
   const uint32_t row_ch = D * Sh::ES / 16;  // 16-byte pieces that a row really has
   const bool run = p.c.page_size % 16 == 0;  // a block's sixteen tokens lie in one page
   Cursor ld;  // of the next block to copy
-  ld.seq = R.seq[warp];
+  ld.seq = CL ? cl_seq : R.seq[warp];
   enter(ld);
-  {
+  if (CL) {
+    ld.unit = cl_unit;
+    ld.block = uint32_t(a);
+  } else {
     const uint64_t in = a - R.before[warp];
     ld.unit = uint32_t(in / ld.blocks);
     ld.block = uint32_t(in - uint64_t(ld.unit) * ld.blocks);
@@ -411,7 +459,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], d);
     const uint64_t u0 = t - cu.block, u1 = u0 + cu.blocks;
-    const KvPiece piece = kv_piece(share, me, a, b, u0, u1);
+    const KvPiece piece = CL ? KvPiece{0, 0} : kv_piece(share, me, a, b, u0, u1);
     if (piece.slot < 0) {
       const float vs = E8 && p.c.v_scale ? p.c.v_scale[cu.unit / pl.chunks] : 1.f;
 #pragma unroll
@@ -433,7 +481,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
                 some ? (m[n][h] == -INFINITY ? 0.f : m[n][h] + log2f(l[n][h]) - kUp) * kLn2 : -INFINITY;
         }
     } else {
-      float* slot = p.slots + uint64_t(piece.slot) * pl.slot_floats;
+      // (CL: over the ring, whose last block every lane has read by now)
+      if (CL) __syncwarp();
+      float* slot = CL ? reinterpret_cast<float*>(ws) : p.slots + uint64_t(piece.slot) * pl.slot_floats;
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -450,11 +500,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
             slot[pl.heads * DP + 2 * head + 1] = l[n][h];
           }
         }
-      if (piece.parts && lane == 0) p.joins[me] = make_int4(int(cu.seq), int(cu.unit), int(piece.parts), 0);
+      if (!CL && piece.parts && lane == 0) p.joins[me] = make_int4(int(cu.seq), int(cu.unit), int(piece.parts), 0);
     }
   };
 
-  look_up();
+  if (a < b) look_up();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
     if (a + i < b) {
@@ -466,7 +516,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   }
-  begin();
+  if (a < b) begin();
   uint32_t stage = 0, put = kStages - 1;  // stages to read and to fill next
   for (uint64_t t = a; t < b; ++t) {
     asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 2) : "memory");
@@ -648,6 +698,47 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
     }
   }
   asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+  if constexpr (CL) {
+    cluster_barrier();
+    // warp `me`: a head, and every other run of 32 dims (or further apart)
+    const uint32_t runs = 32 / cl_heads, head = me % cl_heads, run0 = me / cl_heads;
+    if (run0 < runs) {
+      auto piece = [&](uint32_t k) { return smem_addr(smem) + (k % kWarps) * Sh::WARP; };
+      float m1 = -INFINITY, l1 = 0.f;
+      if (uint32_t(lane) < share.workers) {
+        m1 = ld_cluster(piece(lane) + (pl.heads * DP + 2 * head) * 4, lane / kWarps);
+        l1 = ld_cluster(piece(lane) + (pl.heads * DP + 2 * head + 1) * 4, lane / kWarps);
+      }
+      float base = m1;
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) base = fmaxf(base, __shfl_xor_sync(0xffffffffu, base, d));
+      base = base == -INFINITY ? 0.f : base;
+      const float w = uint32_t(lane) < share.workers ? exp2f(m1 - base) : 0.f;
+      float lt = l1 * w;
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, d);
+      const bool some = lt > 0.f || lt != lt;
+      const float f = some ? (E8 && p.c.v_scale ? p.c.v_scale[cl_unit / pl.chunks] : 1.f) / lt : 0.f;
+      uint16_t* out = static_cast<uint16_t*>(p.a.out) + cl_seq * p.a.out_stride[0] + (cl_head0 + head) * p.a.out_stride[1];
+      for (uint32_t d0 = run0 * 32; d0 < D; d0 += runs * 32) {
+        const uint32_t d = d0 + lane;
+        float v[32];
+#pragma unroll
+        for (uint32_t k = 0; k < 32; ++k)
+          v[k] = k < share.workers && d < D ? ld_cluster(piece(k) + (head * DP + d) * 4, k / kWarps) : 0.f;
+        float acc = 0.f;
+#pragma unroll
+        for (uint32_t k = 0; k < 32; ++k) {
+          const float wk = __shfl_sync(0xffffffffu, w, k);
+          acc += k < share.workers ? v[k] * wk : 0.f;
+        }
+        if (d < D) store16(bf, out + d, some ? acc * f : 0.f);
+      }
+      if (run0 == 0 && lane == 0 && p.a.lse)
+        p.a.lse[uint64_t(cl_seq) * p.a.q_heads + cl_head0 + head] = some ? (base + log2f(lt) - kUp) * kLn2 : -INFINITY;
+    }
+    cluster_barrier();  // no CTA ends while another reads its shared memory
+  }
 }
 
 constexpr int JT = 256;                // threads of a join
@@ -808,25 +899,29 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
 
 int pad_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-template <bool MB, bool E8, int DP, int NG, bool FULL>
+template <bool MB, bool E8, int DP, int NG, bool FULL, bool CL>
 cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
   using Sh = Shape<E8, DP, NG>;
-  auto kernel = kv_attend_kernel<MB, E8, DP, NG, FULL>;
+  static_assert(8 * NG * (DP + 2) * 4 <= Sh::WARP, "a piece fits the warp's shared memory");
+  auto kernel = kv_attend_kernel<MB, E8, DP, NG, FULL, CL>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = opt_in_smem(kernel, Sh::CTA, done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((pl.warps + kWarps - 1) / kWarps);
+  cfg.gridDim = dim3(CL ? pl.clusters * kCluster : (pl.warps + kWarps - 1) / kWarps);
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = Sh::CTA;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = kCluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = CL ? 2 : 1;
   const cudaError_t f = cudaLaunchKernelEx(&cfg, kernel, p, pl);
-  if (f != cudaSuccess) return f;
+  if (f != cudaSuccess || CL) return f;
   cfg.gridDim = dim3((pl.warps + kJoin - 1) / kJoin, pl.heads);
   cfg.blockDim = dim3(JT);
   cfg.dynamicSmemBytes = pl.warps * sizeof(float);
@@ -835,8 +930,11 @@ cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_
 
 template <bool MB, bool E8, int DP, int NG>
 cudaError_t launch_full(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
-  return p.c.head_dim == DP ? launch_attend<MB, E8, DP, NG, true>(p, pl, st)
-                            : launch_attend<MB, E8, DP, NG, false>(p, pl, st);
+  if (pl.clusters)
+    return p.c.head_dim == DP ? launch_attend<MB, E8, DP, NG, true, true>(p, pl, st)
+                              : launch_attend<MB, E8, DP, NG, false, true>(p, pl, st);
+  return p.c.head_dim == DP ? launch_attend<MB, E8, DP, NG, true, false>(p, pl, st)
+                            : launch_attend<MB, E8, DP, NG, false, false>(p, pl, st);
 }
 template <bool MB, bool E8, int DP>
 cudaError_t launch_heads(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
@@ -862,6 +960,14 @@ void shape_of(uint32_t dp, uint32_t* block, uint32_t* per_sm) {
 
 }  // namespace
 
+// Where the units' clusters fit the GPU at once and the table's room is at most
+// kShort tokens, a cluster takes a unit, else all warps share all blocks and a
+// second kernel joins.  8 KV heads of 128 in BF16, clusters against that: one
+// sequence of 777 tokens 7.8 and 10.0 us, of 4000 14.1 and 14.7; two of 4000
+// 16.2 and 15.8; six of 777 10.4 and 14.3.  Past one wave the clusters lose:
+// eight uneven sequences to 777 15.0 and 12.1, 64 of them 81 and 28.
+constexpr uint64_t kShort = 4096;
+
 AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads, uint64_t table_cols, int sms) {
   AttendPlan pl{};
   const uint32_t group = q_heads / c.kv_heads;
@@ -885,6 +991,10 @@ AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads
   pl.slot_floats = (uint64_t(pl.heads) * (pl.pad_dim + 2) + 31) / 32 * 32;
   pl.joins_off = 2 * pl.warps * pl.slot_floats * sizeof(float);
   pl.bytes = pl.joins_off + pl.warps * sizeof(int4);
+  if (blocks * kCluster <= uint64_t(sms) * per_sm && table_cols * c.page_size <= kShort) {
+    pl.clusters = uint32_t(blocks);
+    pl.bytes = 0;
+  }
   return pl;
 }
 

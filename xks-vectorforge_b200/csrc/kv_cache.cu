@@ -525,7 +525,7 @@ int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* a, void* d_work
       !rows_distinct(a->seqs, a->q_heads, kv->d.head_dim, a->out_stride))
     return 1;
   const AttendPlan pl = kv_attend_plan(kv->d, a->seqs, a->q_heads, a->table_cols, kv->sms);
-  if (!d_workspace || workspace_bytes < pl.bytes || off_align(d_workspace, 256)) return 1;
+  if (pl.bytes && (!d_workspace || workspace_bytes < pl.bytes || off_align(d_workspace, 256))) return 1;
   DeviceGuard guard(kv->device);
   if (!guard.ok) return 1;
   auto* ws = static_cast<uint8_t*>(d_workspace);

@@ -27,6 +27,7 @@ struct AttendArgs {
 struct AttendPlan {
   uint32_t warps, chunks, heads, pad_dim;  // query-head chunks per KV head, heads per chunk, padded head_dim
   int page_shift;  // log2 page_size, -1 when that is no power of two
+  uint32_t clusters;  // clusters of CTAs, one a unit, that join by themselves (0: the split over all warps)
   uint64_t slot_floats, joins_off, bytes;
 };
 AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads, uint64_t table_cols, int sms);
