@@ -177,7 +177,8 @@ int xksv_plan_launches(const xksv_plan* plan);
  * its first bit, cuda/decode.cu:12-45); it is an acceleration structure on
  * the side, the slab format is unchanged.  Synchronises `stream`; 0 on
  * success, 1 on a bad slab or CUDA error (no index is kept then).  Calls on
- * one plan must not overlap. */
+ * one plan must not overlap, and a former index is freed: graphs captured
+ * with it are not replayed after this call. */
 int xksv_plan_index(xksv_plan* plan, const void* d_payload, size_t payload_size, void* stream);
 
 
