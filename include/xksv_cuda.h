@@ -451,17 +451,18 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* str
  * (0: all of them),
  *   t_j = scale * q[s, h] . K[j, g]   (softcap c > 0: c * tanh(t_j / c))
  *   out[s, h] = sum_j softmax(t)_j V[j, g],   lse[s, h] = log sum_j exp(t_j).
- * No score above -infinity (L = 0 among them): zeros and -infinity.  Tokens
- * behind L, and the rest of their pages, are not read.  q and out are [seqs, q_heads, head_dim] of `type`, strides
- * in elements ([0] sequence, [1] head), the last dimension contiguous; type
- * is the cache's, or BF16 or FP16 over an E4M3 cache.  lse is FP32 [seqs,
- * q_heads] contiguous, or NULL.  Scores, softmax statistics and sums are
- * FP32.  A length that is negative or above table_cols * page_size gives
- * zeros and -infinity, a page outside the cache counts as masked; both are
- * reported by xksv_kv_status.  d_workspace: as for xksv_plan_linear, of at
+ * No score above -infinity (L = 0 among them): zeros and -infinity; a score
+ * that is NaN or +infinity: NaN in both. Tokens behind L, and the rest of
+ * their pages, are not read. q and out are [seqs, q_heads, head_dim] of
+ * `type`, strides in elements ([0] sequence, [1] head), the last dimension
+ * contiguous; type is the cache's, or BF16 or FP16 over an E4M3 cache. lse is
+ * FP32 [seqs, q_heads] contiguous, or NULL. Scores, softmax statistics and
+ * sums are FP32. A length that is negative or above table_cols * page_size
+ * gives zeros and -infinity, a page outside the cache counts as masked; both
+ * are reported by xksv_kv_status. d_workspace: as for xksv_plan_linear, of at
  * least xksv_kv_attend_workspace(kv, seqs, q_heads, table_cols) bytes (0 for
- * few sequences of short tables: NULL will do).  The work is split over the tokens and joined in a fixed order: the same call
- * gives the same bits. */
+ * few sequences of short tables: NULL will do). The work is split over the
+ * tokens and joined in a fixed order: the same call gives the same bits. */
 typedef struct xksv_kv_attend_args {
   const void* q;
   void* out;

@@ -510,3 +510,47 @@ def test_refusals():
     c.attend(q[:0], table, idx[:0], torch.empty_like(q[:0]))  # no sequences: nothing happens
     assert c.status() == 0
     c.close()
+
+
+# ------------------------------------------------- special scores, precision
+# how a unit's blocks are worked off: by a cluster of CTAs, split over all
+# warps and joined, or (many short sequences) by one warp alone
+WAYS = {"cluster": (3, 60, 0), "split": (3, 60, 5000), "alone": (900, 40, 5000)}
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("fp16", "fp16"), ("bf16", "e4m3")])
+def test_attend_nan_and_infinite_scores(way, kind, cache):
+    """A score that is NaN or +infinity makes its head's row and lse NaN; scores of -infinity only
+    are an empty row; neither touches another row."""
+    S, n, wide = WAYS[way]
+    g = gen(16)
+    Q, H, D, page = 4, 2, 64, 16
+    lens = [n] * S
+    table, pages = table_of(g, lens, page, slack=wide)
+    k, v, ks, vs, c = make_cache(g, cache, pages, page, H, D, "nhd")
+    q = torch.randn(S, Q, D, generator=g, device=DEV).to(DT[kind])
+    q[0, 1, 3] = float("nan")           # every score of one head
+    k[int(table[1, 0]), 2, 1, 5] = float("nan")  # one score of the heads of KV head 1
+    if cache != "e4m3":
+        q[2] = q[2].abs() + 0.5
+        for p in table[2, :-(-n // page)].tolist():
+            k[p, :, 0] = -float("inf")  # every score of KV head 0
+        q[1, :2, 7] = 0.5
+        k[int(table[1, 0]), 3, 0, 7] = float("inf")  # one score of its heads
+    out, lse = torch.full_like(q, 9.0), torch.full((S, Q), 9.0, device=DEV)
+    c.attend(q, table, torch.tensor(lens, dtype=torch.int32, device=DEV), out, lse=lse)
+    assert c.status() == 0
+    nan = torch.zeros(S, Q, dtype=torch.bool, device=DEV)
+    nan[0, 1] = nan[1, 2:] = True
+    empty = torch.zeros_like(nan)
+    if cache != "e4m3":
+        empty[2, :2] = nan[1, :2] = True
+    assert torch.isnan(out[nan]).all() and torch.isnan(lse[nan]).all()
+    assert (out[empty] == 0).all() and (lse[empty] == -math.inf).all()
+    k64, v64 = (torch.nan_to_num(rows64(t, s, "nhd"), posinf=0.0, neginf=0.0) for t, s in ((k, ks), (v, vs)))
+    want, wlse, tol, tlse = attend64(torch.nan_to_num(q), k64, v64, lens, table, page, D ** -0.5)
+    rest = ~(nan | empty)
+    assert ((out.double() - want).abs() <= half_step(kind, want) + tol)[rest].all()
+    assert ((lse.double() - wlse).abs() <= tlse)[rest].all()
+    c.close()

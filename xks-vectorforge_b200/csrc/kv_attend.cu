@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
               if (FULL || dim_of(i, y) < D) store16(bf, out + dim_of(i, y), some ? o[n][i][2 * y + h] * f : 0.f);
           if (hr == 0 && p.a.lse)
             p.a.lse[uint64_t(cu.seq) * p.a.q_heads + head0 + head] =
-                some ? (m[n][h] == -INFINITY ? 0.f : m[n][h] + log2f(l[n][h]) - kUp) * kLn2 : -INFINITY;
+                some ? ((m[n][h] == -INFINITY ? 0.f : m[n][h]) + log2f(l[n][h]) - kUp) * kLn2 : -INFINITY;
         }
     } else {
       // (CL: over the ring, whose last block every lane has read by now)
