@@ -457,7 +457,7 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* str
  * `type`, strides in elements ([0] sequence, [1] head), the last dimension
  * contiguous; type is the cache's, or BF16 or FP16 over an E4M3 cache. lse is
  * FP32 [seqs, q_heads] contiguous, or NULL. Scores, softmax statistics and
- * sums are FP32. A length that is negative or above table_cols * page_size
+ * sums are FP32, a weight enters its product within 2^-17. A length that is negative or above table_cols * page_size
  * gives zeros and -infinity, a page outside the cache counts as masked; both
  * are reported by xksv_kv_status. d_workspace: as for xksv_plan_linear, of at
  * least xksv_kv_attend_workspace(kv, seqs, q_heads, table_cols) bytes (0 for

@@ -18,10 +18,12 @@
 //     such product, and their softmax no padded rows; the weights pass from
 //     the first product's layout to the second's by movmatrix.  Softmax
 //     statistics and sums are FP32 registers.
-//   * Weights reach the second product as 16-bit numbers.  BF16: as a pair
-//     hi + lo of two products (2^-17 relative; one BF16 rounding, 2^-9, would
-//     be as coarse as the output's own).  FP16 and E4M3: as FP16 scaled by 2^15,
-//     so that weights down to 2^-29 of the largest keep 11 bits.
+//   * Weights reach the second product as 16-bit numbers, a pair hi + lo of two
+//     products (BF16: 2^-17 relative, FP16 and E4M3: FP16, 2^-23): one rounding
+//     would be as coarse as a result of the same type.  FP16 weights are scaled
+//     by 2^15: what the pair drops is below 2^-40 of the largest.  (One FP16
+//     rounding: 64 uneven FP16 sequences 375 us against 377, E4M3 105 against
+//     107, and an FP16 result 1.35 times as far from the exact one.)
 //   * E4M3 keys and values become FP16 exactly; the query is brought to FP16
 //     after a power of two per row that puts its largest element in [2^14,
 //     2^15), so that what FP16 drops is below 2^-39 of it.
@@ -659,7 +661,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
           const float s0 = sc[tb][n][2 * y], s1 = sc[tb][n][2 * y + 1];
           const uint32_t w = MB ? pack_bf16(s0, s1) : pack_f16(s0, s1);
           hi[n][y] = transpose8(w);
-          if (MB) lo[n][y] = transpose8(pack_bf16(s0 - __uint_as_float(w << 16), s1 - __uint_as_float(w & 0xffff0000u)));
+          if (MB) {
+            lo[n][y] = transpose8(pack_bf16(s0 - __uint_as_float(w << 16), s1 - __uint_as_float(w & 0xffff0000u)));
+          } else {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w));
+            lo[n][y] = transpose8(pack_f16(s0 - h.x, s1 - h.y));
+          }
         }
 #pragma unroll
       for (int i = 0; i < KS; i += E8 ? 2 : 1) {  // 16 dims a product
@@ -676,7 +683,10 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
             e4m3x4(__byte_perm(r[2 * y], 0, 0x3120), va[0], va[1]);
             e4m3x4(__byte_perm(r[2 * y + 1], 0, 0x3120), va[2], va[3]);
 #pragma unroll
-            for (int n = 0; n < NG; ++n) mma<false>(o[n][i + y], va, hi[n][0], hi[n][1]);
+            for (int n = 0; n < NG; ++n) {
+              mma<false>(o[n][i + y], va, hi[n][0], hi[n][1]);
+              mma<false>(o[n][i + y], va, lo[n][0], lo[n][1]);
+            }
           }
         } else {
           // dims 0 .. 7 and 8 .. 15 of tokens 0 .. 7, then of tokens 8 .. 15
@@ -685,7 +695,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
 #pragma unroll
           for (int n = 0; n < NG; ++n) {
             mma<MB>(o[n][i], r, hi[n][0], hi[n][1]);
-            if (MB) mma<MB>(o[n][i], r, lo[n][0], lo[n][1]);
+            mma<MB>(o[n][i], r, lo[n][0], lo[n][1]);
           }
         }
       }
