@@ -304,3 +304,36 @@ def test_linear_refusals():
     with pytest.raises(RuntimeError):
         two.linear(payload, x, y)
     two.close()
+
+
+@pytest.mark.parametrize("batch", [4, 16, 64])
+def test_linear_fp32_sums_stay_fp32_where_a_cta_holds_all_columns(batch):
+    """The fused route: more groups of slabs than SMs (each reads other columns
+    of x), so that a CTA adds all 8192 columns of its groups.  Weights and x are
+    above zero, so what is cut off adds up: each addition cuts less than the
+    running sum's last place, 2^-23 of it, 32 additions of 16 columns to an
+    accumulator; the 16 accumulators of 512 columns are added in FP32, half a
+    last place each, 16 * 2^-24 (one accumulator for all columns: 512 * 2^-24
+    on average)."""
+    cols, n = 8192, 160
+    rng = np.random.default_rng(23)
+    payload, entries, ws = bytearray(), [], []
+    for i in range(n):
+        w = (words_for("normal002", 16 * cols, rng) & 0x7FFF).astype("<u2")
+        blob = xg.host_pack(w.tobytes(), 16, cols, SERIAL)
+        entries.append(dict(src_offset=len(payload), src_size=len(blob), rows=16, cols=cols, dst_offset=16 * i,
+                            x_offset=16 * i, codec=SERIAL))
+        payload += blob
+        ws.append(bf16_to_f32(w).reshape(16, cols))
+    payload = torch.frombuffer(payload, dtype=torch.uint8).to(DEV)
+    plan = xg.Plan(entries)
+    assert plan.index(payload) == 0 and plan.fused_ready(payload)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.rand(batch, cols + 16 * n, generator=g, device=DEV).bfloat16()
+    want = torch.cat([x[:, 16 * i:16 * i + cols].double() @ torch.from_numpy(w).to(DEV).double().t()
+                      for i, w in enumerate(ws)], 1)
+    y = torch.empty(batch, 16 * n, device=DEV)
+    plan.linear(payload, x, y)
+    assert plan.status() == 0
+    assert float((y - want).norm() / want.norm()) <= 32 * 2.0 ** -23 + 16 * 2.0 ** -24
+    plan.close()

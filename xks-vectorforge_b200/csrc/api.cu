@@ -173,6 +173,14 @@ int run_single(Kind kind, const void* input, size_t size, uint64_t rows, uint64_
 }  // namespace
 }  // namespace xksv
 
+// The segments of the fused CTAs' work (build_fused), on the device.
+struct FusedSegs {
+  uint32_t n = 0;
+  uint32_t* seg0 = nullptr;  // CTA c's segments: tasks[seg0[c] .. seg0[c + 1])
+  xksv::FusedTask* tasks = nullptr;
+  uint32_t* gsegs = nullptr;  // group g's segments: entries [e[g], e[g + 1]) behind the groups + 1 first
+};
+
 struct xksv_plan {
   int device = 0;
   xksv::Slab* d_slabs = nullptr;  // [serial | parallel | raw]
@@ -217,8 +225,8 @@ struct xksv_plan {
   bool fused_ok = false;
   int gemm_route = 0;  // XKSV_GEMM_*
   uint32_t n_fctas = 0;
-  uint32_t* d_fseg0 = nullptr;  // CTA c's segments: d_ftasks[d_fseg0[c] .. d_fseg0[c + 1])
-  xksv::FusedTask* d_ftasks = nullptr;
+  FusedSegs fsegs;   // the fused CTAs' segments
+  FusedSegs fexact;  // the same in pieces of up to kExactUnits half tiles, for FP32 results (n 0: no segment is longer)
   xksv::FusedGroup* d_fgroups = nullptr;
   uint32_t* d_fmembers = nullptr;
   void* d_ftabs = nullptr;  // per group: its lane tables, built with the index
@@ -233,8 +241,7 @@ struct xksv_plan {
   uint32_t par_parts = 1;
   uint32_t* d_ppos = nullptr;
   void* d_ptabs = nullptr;  // kPartTabBytes a slab
-  uint32_t n_fgroups = 0, n_fsegs = 0;
-  uint32_t* d_fgsegs = nullptr;  // group g's segments: entries [e[g], e[g + 1]) behind the n_fgroups + 1 first
+  uint32_t n_fgroups = 0;
   uint64_t* d_hash_ranges = nullptr;  // per slab in creation order: {dst, decoded bytes}
   // linear layer (xksv_plan_linear): the runs of Y rows the slabs cover; off
   // when two slabs cover one row or a slab has no rows and columns
@@ -262,6 +269,13 @@ void free_ragged(xksv_plan* p) {
   p->r_items = 0;
 }
 
+void free_segs(FusedSegs& f) {
+  if (f.seg0) cudaFree(f.seg0);
+  if (f.tasks) cudaFree(f.tasks);
+  if (f.gsegs) cudaFree(f.gsegs);
+  f = FusedSegs{};
+}
+
 void free_index(xksv_plan* p) {
   if (p->d_tidx) cudaFree(p->d_tidx);
   if (p->d_tmid) cudaFree(p->d_tmid);
@@ -270,22 +284,18 @@ void free_index(xksv_plan* p) {
   if (p->d_items) cudaFree(p->d_items);
   if (p->d_partials) cudaFree(p->d_partials);
   if (p->d_counters) cudaFree(p->d_counters);
-  if (p->d_fseg0) cudaFree(p->d_fseg0);
-  if (p->d_ftasks) cudaFree(p->d_ftasks);
+  free_segs(p->fsegs);
+  free_segs(p->fexact);
   if (p->d_fgroups) cudaFree(p->d_fgroups);
   if (p->d_fmembers) cudaFree(p->d_fmembers);
   if (p->d_ftabs) cudaFree(p->d_ftabs);
-  if (p->d_fgsegs) cudaFree(p->d_fgsegs);
   if (p->d_ppos) cudaFree(p->d_ppos);
   if (p->d_ptabs) cudaFree(p->d_ptabs);
   free_ragged(p);
   p->d_ppos = nullptr;
   p->d_ptabs = nullptr;
   p->par_parts = 1;
-  p->d_fgsegs = nullptr;
   p->d_ftabs = nullptr;
-  p->d_fseg0 = nullptr;
-  p->d_ftasks = nullptr;
   p->d_fgroups = nullptr;
   p->d_fmembers = nullptr;
   p->n_fctas = 0;
@@ -473,6 +483,28 @@ void build_fused(const std::vector<xksv::Slab>& all, uint64_t x_base, int sms, u
   const Sched& best = cost(shares) < cost(by_group) ? shares : by_group;
   segs = best.first;
   seg0 = best.second;
+}
+
+// The tensor cores cut a running sum at its last place, always towards zero:
+// over 8192 columns 3e-5 of the result.  For FP32 results a segment ends after
+// 512 columns at the latest (32 tiles, in either half of a slab's rows) and
+// the segments' sums are added in FP32, rounded to nearest.  14336 x 4096, 16
+// tokens: segments of 775 columns, relative error 7.4e-7 in 130 us; in two
+// pieces 3.6e-7 in 141 us.
+constexpr uint32_t kExactUnits = 64;
+// Cuts every CTA's segments into even pieces of up to kExactUnits half tiles.
+void cut_segments(const std::vector<xksv::FusedTask>& segs, const std::vector<uint32_t>& seg0,
+                  std::vector<xksv::FusedTask>& out, std::vector<uint32_t>& out0) {
+  for (size_t c = 0; c + 1 < seg0.size(); ++c) {
+    out0.push_back(uint32_t(out.size()));
+    for (uint32_t i = seg0[c]; i < seg0[c + 1]; ++i) {
+      const xksv::FusedTask& t = segs[i];
+      const uint64_t span = t.h1 - t.h0, n = (span + kExactUnits - 1) / kExactUnits;
+      for (uint64_t k = 0; k < n; ++k)
+        out.push_back(xksv::FusedTask{t.group, t.h0 + uint32_t(span * k / n), t.h0 + uint32_t(span * (k + 1) / n), 0});
+    }
+  }
+  out0.push_back(uint32_t(out.size()));
 }
 }  // namespace
 
@@ -919,8 +951,8 @@ GemvArgs gemv_args(const xksv_plan* p, const uint8_t* pay) {
 }
 FusedArgs fused_args(const xksv_plan* p, const uint8_t* pay, size_t batch) {
   FusedArgs f{};
-  f.seg0 = p->d_fseg0;
-  f.tasks = p->d_ftasks;
+  f.seg0 = p->fsegs.seg0;
+  f.tasks = p->fsegs.tasks;
   f.groups = p->d_fgroups;
   f.members = p->d_fmembers;
   f.slabs = p->d_slabs;
@@ -1060,8 +1092,10 @@ struct LinearSpace {
   Route route;
   uint64_t x, z, rows, scratch, total;  // workspace offsets; rows: x's rows, aligned
 };
+// FP32 results add the tensor cores' sums of short segments (kExactUnits).
+const FusedSegs& linear_segs(const xksv_plan* p, bool f32) { return f32 && p->fexact.n ? p->fexact : p->fsegs; }
 // The payload decides whether the tile index is there: null counts for none.
-LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload) {
+LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload, bool f32) {
   Carve c;
   LinearSpace s{};
   const bool indexed = payload && p->d_tidx && payload == p->indexed_payload && p->n_items;
@@ -1075,7 +1109,7 @@ LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload
     // tokens 71 against 54; 14336 x 4096: 133 against 141, 163 against 141;
     // 4096 x 14336: 123 against 151, 146 against 151)
     s.route = Route::Fused;
-    s.z = c.take(uint64_t(p->n_fsegs) * 16 * ((batch + 15) / 16 * 16) * 32 * sizeof(float));
+    s.z = c.take(uint64_t(linear_segs(p, f32).n) * 16 * ((batch + 15) / 16 * 16) * 32 * sizeof(float));
     s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
   } else if (p->tc_ok) {
     s.route = Route::Gemm;
@@ -1113,7 +1147,8 @@ int xksv_plan_device(const xksv_plan* p) { return p ? p->device : -1; }
 size_t xksv_plan_linear_workspace(const xksv_plan* p, size_t batch) {
   if (!p || !p->linear_ok || !batch || batch >= kMaxBatch) return 0;
   // a later index may switch the route: room for either
-  return size_t(std::max(linear_space(p, batch, nullptr).total, linear_space(p, batch, p->indexed_payload).total));
+  return size_t(std::max({linear_space(p, batch, nullptr, false).total, linear_space(p, batch, p->indexed_payload, false).total,
+                          linear_space(p, batch, p->indexed_payload, true).total}));
 }
 
 int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_size, const xksv_linear_args* a,
@@ -1132,7 +1167,7 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
   p->launches = 0;
   if (!a->batch || !p->n_runs) return 0;
   if (!d_payload || !a->x || !a->y) return 1;
-  const LinearSpace sp = linear_space(p, a->batch, d_payload);
+  const LinearSpace sp = linear_space(p, a->batch, d_payload, a->y_type == XKSV_FP32);
   if (!d_workspace || workspace_bytes < sp.total || misaligned(d_workspace, 256)) return 1;
   OnDevice dev(p->device);
   if (!dev.ok) return 1;
@@ -1193,14 +1228,16 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
   }
   const uint16_t* x0 = static_cast<const uint16_t*>(xp) + p->x_base;
   if (sp.route == Route::Fused) {
+    const FusedSegs& segs = linear_segs(p, ep.y_f32);
     FusedArgs f = fused_args(p, pay, a->batch);
+    f.seg0 = segs.seg0;
+    f.tasks = segs.tasks;
     f.xt = x0;
     f.xt_ld = pitch;
     f.y = reinterpret_cast<float*>(ws + sp.z);
     p->launches += 2;
-    return launch_fused_linear(f, p->n_fctas, p->n_fgroups, p->d_fgsegs, p->d_fgsegs + p->n_fgroups + 1, ep, st) == cudaSuccess
-               ? 0
-               : 1;
+    return launch_fused_linear(f, p->n_fctas, p->n_fgroups, segs.gsegs, segs.gsegs + p->n_fgroups + 1, ep, st) == cudaSuccess ? 0
+                                                                                                                             : 1;
   }
   // decode, then one tensor-core product with its epilogue per weight
   if (decode_scratch(p, pay, ws + sp.scratch, st) != cudaSuccess) return 1;
@@ -1282,6 +1319,24 @@ int xksv_plan_sha256(const xksv_plan* p, const void* d_out, size_t out_size, voi
 // tensor-core path and every codebook fits the fused decoder's tables; each
 // group's lane tables are built here, once.  Any failure here only leaves
 // the fused route off.
+static bool put_segs(FusedSegs& f, const std::vector<FusedTask>& tasks, const std::vector<uint32_t>& seg0, size_t groups,
+                     cudaStream_t st) {
+  std::vector<uint32_t> gsegs(groups + 1, 0);
+  for (const FusedTask& t : tasks) ++gsegs[t.group + 1];
+  for (size_t g = 0; g < groups; ++g) gsegs[g + 1] += gsegs[g];
+  std::vector<uint32_t> at(gsegs.begin(), gsegs.begin() + groups);
+  gsegs.resize(groups + 1 + tasks.size());
+  for (size_t i = 0; i < tasks.size(); ++i) gsegs[groups + 1 + at[tasks[i].group]++] = uint32_t(i);
+  f.n = uint32_t(tasks.size());
+  return cudaMalloc(&f.seg0, seg0.size() * sizeof(uint32_t)) == cudaSuccess &&
+         cudaMalloc(&f.tasks, tasks.size() * sizeof(FusedTask)) == cudaSuccess &&
+         cudaMalloc(&f.gsegs, gsegs.size() * sizeof(uint32_t)) == cudaSuccess &&
+         cudaMemcpyAsync(f.seg0, seg0.data(), seg0.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) == cudaSuccess &&
+         cudaMemcpyAsync(f.tasks, tasks.data(), tasks.size() * sizeof(FusedTask), cudaMemcpyHostToDevice, st) == cudaSuccess &&
+         cudaMemcpyAsync(f.gsegs, gsegs.data(), gsegs.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) == cudaSuccess &&
+         cudaStreamSynchronize(st) == cudaSuccess;  // the vectors end here
+}
+
 static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st) {
   const uint32_t n = p->n_ser + p->n_par + p->n_raw;
   if (!p->tc_ok || !n || p->n_ser_idx != n) return;
@@ -1299,30 +1354,17 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   std::vector<uint32_t> members, seg0;
   std::vector<FusedTask> tasks;
   build_fused(p->h_slabs, p->x_base, sms, fused_producers(16, nullptr), groups, members, tasks, seg0);
-  std::vector<uint32_t> gsegs(groups.size() + 1, 0);
-  for (const FusedTask& t : tasks) ++gsegs[t.group + 1];
-  for (size_t g = 0; g < groups.size(); ++g) gsegs[g + 1] += gsegs[g];
-  gsegs.resize(groups.size() + 1 + tasks.size());
-  {
-    std::vector<uint32_t> at(gsegs.begin(), gsegs.begin() + groups.size());
-    for (size_t i = 0; i < tasks.size(); ++i) gsegs[groups.size() + 1 + at[tasks[i].group]++] = uint32_t(i);
-  }
-  good = !tasks.empty() && seg0.size() >= 2 &&
-         cudaMalloc(&p->d_fseg0, seg0.size() * sizeof(uint32_t)) == cudaSuccess &&
-         cudaMemcpyAsync(p->d_fseg0, seg0.data(), seg0.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) ==
-             cudaSuccess &&
-         cudaMalloc(&p->d_ftasks, tasks.size() * sizeof(FusedTask)) == cudaSuccess &&
+  std::vector<FusedTask> pieces;
+  std::vector<uint32_t> piece0;
+  cut_segments(tasks, seg0, pieces, piece0);
+  good = !tasks.empty() && seg0.size() >= 2 && put_segs(p->fsegs, tasks, seg0, groups.size(), st) &&
+         (pieces.size() == tasks.size() || put_segs(p->fexact, pieces, piece0, groups.size(), st)) &&
          cudaMalloc(&p->d_fgroups, groups.size() * sizeof(FusedGroup)) == cudaSuccess &&
          cudaMalloc(&p->d_fmembers, members.size() * sizeof(uint32_t)) == cudaSuccess &&
-         cudaMemcpyAsync(p->d_ftasks, tasks.data(), tasks.size() * sizeof(FusedTask), cudaMemcpyHostToDevice, st) ==
-             cudaSuccess &&
          cudaMemcpyAsync(p->d_fgroups, groups.data(), groups.size() * sizeof(FusedGroup), cudaMemcpyHostToDevice,
                          st) == cudaSuccess &&
          cudaMemcpyAsync(p->d_fmembers, members.data(), members.size() * sizeof(uint32_t), cudaMemcpyHostToDevice,
                          st) == cudaSuccess &&
-         cudaMalloc(&p->d_fgsegs, gsegs.size() * sizeof(uint32_t)) == cudaSuccess &&
-         cudaMemcpyAsync(p->d_fgsegs, gsegs.data(), gsegs.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) ==
-             cudaSuccess &&
          cudaMalloc(&p->d_ftabs, groups.size() * fused_tables_bytes()) == cudaSuccess &&
          cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
          launch_fused_tables(p->d_fgroups, uint32_t(groups.size()), p->d_fmembers, p->d_slabs, d_payload, p->d_ftabs,
@@ -1332,23 +1374,18 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   cudaMemsetAsync(p->d_status, 0, sizeof(int), st);
   cudaStreamSynchronize(st);
   if (!good) {
-    if (p->d_fseg0) cudaFree(p->d_fseg0);
-    p->d_fseg0 = nullptr;
-    if (p->d_ftasks) cudaFree(p->d_ftasks);
+    free_segs(p->fsegs);
+    free_segs(p->fexact);
     if (p->d_fgroups) cudaFree(p->d_fgroups);
     if (p->d_fmembers) cudaFree(p->d_fmembers);
     if (p->d_ftabs) cudaFree(p->d_ftabs);
-    if (p->d_fgsegs) cudaFree(p->d_fgsegs);
-    p->d_fgsegs = nullptr;
     p->d_ftabs = nullptr;
-    p->d_ftasks = nullptr;
     p->d_fgroups = nullptr;
     p->d_fmembers = nullptr;
     return;
   }
   p->n_fctas = uint32_t(seg0.size() - 1);
   p->n_fgroups = uint32_t(groups.size());
-  p->n_fsegs = uint32_t(tasks.size());
   p->fused_ok = true;
 }
 

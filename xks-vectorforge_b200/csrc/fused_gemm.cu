@@ -27,7 +27,9 @@
 //     while the producer decodes its next row);
 //   * the epilogue reads D_q with tcgen05.ld (warp r of the first four holds
 //     TMEM lanes 32 r .., i.e. row 4q + r of every slab) and adds into Y
-//     (several CTAs share a group's rows when its tiles are split).
+//     (several CTAs share a group's rows when its tiles are split).  A linear
+//     layer's call leaves each segment's sums apart instead, of up to 512
+//     columns when its result is FP32.
 // Shared memory holds the tables once and, per producer warp, one stage, two
 // B slices and the lane rings; no decoded tile is buffered whole, so 19
 // producer warps fit one SM beside the stages.  Every wait is bounded: on a
