@@ -130,3 +130,39 @@ def test_ragged_serial_slabs_decode(shapes, kind):
         assert plan.status() == 0
         assert (out.cpu().numpy().view("<u2") == want).all()
     plan.close()
+
+
+def test_ragged_tiles_of_a_changed_stream_are_reported_or_read_alike():
+    """Bits changed after the index: every element is the source's, or the call
+    reports the slab; tiles whose bits are as they were read the same, and
+    nothing is written outside the output."""
+    rows, cols = 14, 9000
+    payload, entries, want = slabs([(rows, cols), (16, 520)], xg.CODEC_TILE16, "normal002", 6)
+    plan = xg.Plan(entries)
+    assert plan.index(payload) == 0
+    first, e = 64, entries[0]
+    bits = e["src_offset"] + 272 + rows * cols
+    good, last = payload.clone(), e["src_offset"] + e["src_size"]
+    words = want[:rows * cols].reshape(rows, cols)
+    reported = 0
+    # inside the stream, in its first and its last bytes
+    for at in (bits, bits + 100, (bits + last) // 2, last - 8):
+        for mask in (0x01, 0x3C, 0xFF):
+            payload.copy_(good)
+            payload[at:at + 2] ^= mask
+            out = torch.full((first + want.size * 2 + first,), 0xEE, dtype=torch.uint8, device=DEV)
+            plan.decode(payload, out[first:])
+            bad = plan.status()
+            got = out.cpu().numpy()
+            assert (got[:first] == 0xEE).all() and (got[-first:] == 0xEE).all()
+            elems = got[first:-first].view("<u2")
+            assert (elems[rows * cols:] == want[rows * cols:]).all()  # the other slab
+            wrong = (elems[:rows * cols].reshape(rows, cols) != words).any(0).nonzero()[0] // 16
+            assert len(set(wrong.tolist())) <= 2, (at, mask)  # two bytes lie in at most two tiles' bits
+            reported += bad
+    assert reported  # a tile whose codes no longer end where the next one begins
+    payload.copy_(good)
+    out = torch.empty(want.size * 2, dtype=torch.uint8, device=DEV)
+    plan.decode(payload, out)
+    assert plan.status() == 0 and (out.cpu().numpy().view("<u2") == want).all()
+    plan.close()

@@ -1080,6 +1080,9 @@ __global__ void __launch_bounds__(GT * SPLIT, SPLIT == 2 || NB > 1 ? 2 : 4) seri
           if (lane == 0) S.red[row][warp][b] += v;
         }
       }
+      // the tile's codes end where the next tile's begin (the index describes
+      // another payload otherwise)
+      if (RAGGED && act && (dead || r.pos() != b1 - base_bit + slack)) atomicOr(a.status, kStatusStream);
       __syncthreads();
       ta = tb;
     }
