@@ -166,3 +166,16 @@ def test_ragged_tiles_of_a_changed_stream_are_reported_or_read_alike():
     plan.decode(payload, out)
     assert plan.status() == 0 and (out.cpu().numpy().view("<u2") == want).all()
     plan.close()
+
+
+def test_index_keeps_an_unread_error():
+    """An error that no status call has read yet is still there after an index."""
+    for codec, shape in ((xg.CODEC_PARALLEL32, (16, 8192)), (xg.CODEC_TILE16, (16, 1000)), (xg.CODEC_TILE16, (16, 1024))):
+        payload, entries, want = slabs([shape], codec, "normal002", 5)
+        good = payload.clone()
+        plan = xg.Plan(entries)
+        payload[entries[0]["src_offset"] + 8:entries[0]["src_offset"] + 10] ^= 1  # a size in the header
+        plan.decode(payload, torch.empty(want.size * 2, dtype=torch.uint8, device=DEV))
+        assert plan.index(good) == 0
+        assert plan.status() == 1 and plan.status() == 0, (codec, shape)
+        plan.close()

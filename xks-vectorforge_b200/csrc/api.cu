@@ -1453,10 +1453,33 @@ static void setup_parts(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   p->d_ptabs = nullptr;
 }
 
+namespace {
+// The index passes use the plan's status word: what earlier calls left there
+// is put back behind them.
+struct KeepStatus {
+  xksv_plan* p;
+  cudaStream_t st;
+  int kept = 0;
+  bool ok;
+  KeepStatus(xksv_plan* plan, cudaStream_t stream) : p(plan), st(stream) {
+    ok = cudaMemcpyAsync(p->h_status, p->d_status, sizeof(int), cudaMemcpyDeviceToHost, st) == cudaSuccess &&
+         cudaStreamSynchronize(st) == cudaSuccess;
+    if (ok) kept = *p->h_status;
+  }
+  ~KeepStatus() {
+    if (!kept) return;
+    *p->h_status = kept;
+    cudaMemcpyAsync(p->d_status, p->h_status, sizeof(int), cudaMemcpyHostToDevice, st);
+    cudaStreamSynchronize(st);
+  }
+};
+}  // namespace
+
 int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, void* stream) {
   if (!p || !d_payload || p->need_payload > payload_size) return 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cudaStreamSynchronize(st) != cudaSuccess) return 1;
+  const KeepStatus keep(p, st);
+  if (!keep.ok) return 1;
   free_index(p);
   const uint32_t n = p->n_ser_idx;
   if (!n) {
