@@ -179,3 +179,24 @@ def test_index_keeps_an_unread_error():
         assert plan.index(good) == 0
         assert plan.status() == 1 and plan.status() == 0, (codec, shape)
         plan.close()
+
+
+def test_calls_after_an_index_without_room_for_the_parts():
+    """Too little memory for the part index leaves it off, and no more."""
+    payload, entries, want = slabs([(16, 1024)] * 1000, xg.CODEC_PARALLEL32, "normal002", 8)
+    plan = xg.Plan(entries)
+    out = torch.empty(want.size * 2, dtype=torch.uint8, device=DEV)
+    plan.decode(payload, out)
+    assert plan.status() == 0
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    full = torch.empty(free - (6 << 20), dtype=torch.uint8, device=DEV)  # the parts' tables take 10 MB
+    try:
+        assert plan.index(payload) == 0
+        plan.decode(payload, out)
+        assert plan.status() == 0
+    finally:
+        del full
+        torch.cuda.empty_cache()
+    assert (out.cpu().numpy().view("<u2") == want).all()
+    plan.close()

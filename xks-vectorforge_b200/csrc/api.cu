@@ -84,6 +84,16 @@ bool parallel_header_ok(const uint8_t* p, size_t n, uint64_t* rows_out, uint64_t
   return true;
 }
 
+// Device memory; a refusal is the caller's to handle and leaves no error
+// behind that the next launch's check would take for its own.
+template <class T>
+bool dev_alloc(T** p, size_t bytes) {
+  if (cudaMalloc(reinterpret_cast<void**>(p), bytes) == cudaSuccess) return true;
+  *p = nullptr;
+  cudaGetLastError();
+  return false;
+}
+
 struct DevCtx {
   std::mutex mu;
   bool init = false;
@@ -101,8 +111,8 @@ DevCtx* ctx_current() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || size_t(dev) >= kMaxDevices) return nullptr;
   DevCtx& c = g_ctx[dev];
   if (!c.init) {
-    if (cudaMalloc(&c.d_slab, sizeof(Slab)) != cudaSuccess) return nullptr;
-    if (cudaMalloc(&c.d_status, sizeof(int)) != cudaSuccess) return nullptr;
+    if (!dev_alloc(&c.d_slab, sizeof(Slab))) return nullptr;
+    if (!dev_alloc(&c.d_status, sizeof(int))) return nullptr;
     if (cudaMallocHost(&c.h_status, sizeof(int)) != cudaSuccess) return nullptr;
     cudaDeviceGetAttribute(&c.sms, cudaDevAttrMultiProcessorCount, dev);
     c.init = true;
@@ -136,7 +146,7 @@ int run_single(Kind kind, const void* input, size_t size, uint64_t rows, uint64_
     if (size > c->cap) {
       if (c->stage) cudaFree(c->stage);
       size_t cap = std::max<size_t>(size + 64, c->cap * 2);
-      if (cudaMalloc(&c->stage, cap) != cudaSuccess) {
+      if (!dev_alloc(&c->stage, cap)) {
         c->stage = nullptr;
         c->cap = 0;
         return 1;
@@ -645,11 +655,11 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
   all.insert(all.end(), ser.begin(), ser.end());
   all.insert(all.end(), par.begin(), par.end());
   all.insert(all.end(), raw.begin(), raw.end());
-  bool ok = cudaMalloc(&p->d_status, sizeof(int)) == cudaSuccess &&
+  bool ok = dev_alloc(&p->d_status, sizeof(int)) &&
             cudaMallocHost(&p->h_status, sizeof(int)) == cudaSuccess &&
             cudaMemset(p->d_status, 0, sizeof(int)) == cudaSuccess;
   if (ok && n) {
-    ok = cudaMalloc(&p->d_slabs, n * sizeof(Slab)) == cudaSuccess &&
+    ok = dev_alloc(&p->d_slabs, n * sizeof(Slab)) &&
          cudaMemcpy(p->d_slabs, all.data(), n * sizeof(Slab), cudaMemcpyHostToDevice) == cudaSuccess;
   }
   // decoded byte ranges in the caller's slab order (xksv_plan_sha256)
@@ -659,7 +669,7 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
       hr[2 * i] = slabs[i].dst_offset;
       hr[2 * i + 1] = slabs[i].codec == XKSV_CODEC_RAW ? slabs[i].src_size : slabs[i].rows * slabs[i].cols * 2;
     }
-    ok = cudaMalloc(&p->d_hash_ranges, hr.size() * sizeof(uint64_t)) == cudaSuccess &&
+    ok = dev_alloc(&p->d_hash_ranges, hr.size() * sizeof(uint64_t)) &&
          cudaMemcpy(p->d_hash_ranges, hr.data(), hr.size() * sizeof(uint64_t), cudaMemcpyHostToDevice) ==
              cudaSuccess;
   }
@@ -680,8 +690,8 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
       for (const TcGroup& g : groups) minch = std::min<uint32_t>(minch, (g.cols + 63) / 64);
       const uint32_t want = (2 * uint32_t(sms) + p->ngroups - 1) / p->ngroups;
       p->tc_ksplit = std::max<uint32_t>(1, std::min<uint32_t>(want, minch));
-      p->tc_ok = cudaMalloc(&p->d_groups, groups.size() * sizeof(TcGroup)) == cudaSuccess &&
-                 cudaMalloc(&p->d_tc_slabs, n * sizeof(Slab)) == cudaSuccess &&
+      p->tc_ok = dev_alloc(&p->d_groups, groups.size() * sizeof(TcGroup)) &&
+                 dev_alloc(&p->d_tc_slabs, n * sizeof(Slab)) &&
                  cudaMemcpy(p->d_groups, groups.data(), groups.size() * sizeof(TcGroup),
                             cudaMemcpyHostToDevice) == cudaSuccess &&
                  cudaMemcpy(p->d_tc_slabs, tc_slabs.data(), n * sizeof(Slab), cudaMemcpyHostToDevice) ==
@@ -697,7 +707,7 @@ int xksv_plan_create(const xksv_slab* slabs, size_t n, xksv_plan** out) {
     if (p->linear_ok && !runs.empty()) {
       p->n_runs = uint32_t(runs.size());
       for (const RowRun& r : runs) p->max_run = std::max(p->max_run, r.rows);
-      ok = cudaMalloc(&p->d_runs, runs.size() * sizeof(RowRun)) == cudaSuccess &&
+      ok = dev_alloc(&p->d_runs, runs.size() * sizeof(RowRun)) &&
            cudaMemcpy(p->d_runs, runs.data(), runs.size() * sizeof(RowRun), cudaMemcpyHostToDevice) == cudaSuccess;
     }
   }
@@ -1063,9 +1073,9 @@ int xksv_plan_gemm(const xksv_plan* pc, const void* d_payload, size_t payload_si
   // the plan's own tensor-core buffers, allocated on first use and kept
   if (p->tc_ok && batch >= 4) {
     if (!gemm_fused(p, d_payload, batch) && !p->d_scratch &&
-        cudaMalloc(&p->d_scratch, std::max<uint64_t>(16, p->scratch_bytes)) != cudaSuccess)
+        !dev_alloc(&p->d_scratch, std::max<uint64_t>(16, p->scratch_bytes)))
       return 1;
-    if (!p->d_xt && cudaMalloc(&p->d_xt, 256 * p->x_cols * 2) != cudaSuccess) return 1;
+    if (!p->d_xt && !dev_alloc(&p->d_xt, 256 * p->x_cols * 2)) return 1;
   }
   return gemm_run(p, static_cast<const uint8_t*>(d_payload), d_x, d_y, batch, p->d_xt, p->d_scratch,
                   static_cast<cudaStream_t>(stream));
@@ -1328,9 +1338,9 @@ static bool put_segs(FusedSegs& f, const std::vector<FusedTask>& tasks, const st
   gsegs.resize(groups + 1 + tasks.size());
   for (size_t i = 0; i < tasks.size(); ++i) gsegs[groups + 1 + at[tasks[i].group]++] = uint32_t(i);
   f.n = uint32_t(tasks.size());
-  return cudaMalloc(&f.seg0, seg0.size() * sizeof(uint32_t)) == cudaSuccess &&
-         cudaMalloc(&f.tasks, tasks.size() * sizeof(FusedTask)) == cudaSuccess &&
-         cudaMalloc(&f.gsegs, gsegs.size() * sizeof(uint32_t)) == cudaSuccess &&
+  return dev_alloc(&f.seg0, seg0.size() * sizeof(uint32_t)) &&
+         dev_alloc(&f.tasks, tasks.size() * sizeof(FusedTask)) &&
+         dev_alloc(&f.gsegs, gsegs.size() * sizeof(uint32_t)) &&
          cudaMemcpyAsync(f.seg0, seg0.data(), seg0.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) == cudaSuccess &&
          cudaMemcpyAsync(f.tasks, tasks.data(), tasks.size() * sizeof(FusedTask), cudaMemcpyHostToDevice, st) == cudaSuccess &&
          cudaMemcpyAsync(f.gsegs, gsegs.data(), gsegs.size() * sizeof(uint32_t), cudaMemcpyHostToDevice, st) == cudaSuccess &&
@@ -1342,7 +1352,7 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   if (!p->tc_ok || !n || p->n_ser_idx != n) return;
   uint8_t* d_ok = nullptr;
   std::vector<uint8_t> ok(n, 0);
-  bool good = cudaMalloc(&d_ok, n) == cudaSuccess && launch_fused_check(p->d_slabs, n, d_payload, d_ok, st) == cudaSuccess &&
+  bool good = dev_alloc(&d_ok, n) && launch_fused_check(p->d_slabs, n, d_payload, d_ok, st) == cudaSuccess &&
               cudaMemcpyAsync(ok.data(), d_ok, n, cudaMemcpyDeviceToHost, st) == cudaSuccess &&
               cudaStreamSynchronize(st) == cudaSuccess;
   if (d_ok) cudaFree(d_ok);
@@ -1359,13 +1369,13 @@ static void setup_fused(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   cut_segments(tasks, seg0, pieces, piece0);
   good = !tasks.empty() && seg0.size() >= 2 && put_segs(p->fsegs, tasks, seg0, groups.size(), st) &&
          (pieces.size() == tasks.size() || put_segs(p->fexact, pieces, piece0, groups.size(), st)) &&
-         cudaMalloc(&p->d_fgroups, groups.size() * sizeof(FusedGroup)) == cudaSuccess &&
-         cudaMalloc(&p->d_fmembers, members.size() * sizeof(uint32_t)) == cudaSuccess &&
+         dev_alloc(&p->d_fgroups, groups.size() * sizeof(FusedGroup)) &&
+         dev_alloc(&p->d_fmembers, members.size() * sizeof(uint32_t)) &&
          cudaMemcpyAsync(p->d_fgroups, groups.data(), groups.size() * sizeof(FusedGroup), cudaMemcpyHostToDevice,
                          st) == cudaSuccess &&
          cudaMemcpyAsync(p->d_fmembers, members.data(), members.size() * sizeof(uint32_t), cudaMemcpyHostToDevice,
                          st) == cudaSuccess &&
-         cudaMalloc(&p->d_ftabs, groups.size() * fused_tables_bytes()) == cudaSuccess &&
+         dev_alloc(&p->d_ftabs, groups.size() * fused_tables_bytes()) &&
          cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
          launch_fused_tables(p->d_fgroups, uint32_t(groups.size()), p->d_fmembers, p->d_slabs, d_payload, p->d_ftabs,
                              p->d_status, st) == cudaSuccess &&
@@ -1404,10 +1414,10 @@ static void setup_ragged(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st
     for (uint32_t t0 = 0; t0 < tiles; t0 += per) items.push_back(GemvItem{i, t0, std::min(per, tiles - t0), 0, ni, 0, 0, 0});
   }
   if (total > std::numeric_limits<uint32_t>::max() || items.size() > (1u << 31)) return;
-  const bool ok = cudaMalloc(&p->d_r_tidx, total * sizeof(uint32_t)) == cudaSuccess &&
-                  cudaMalloc(&p->d_r_tbase, n * sizeof(uint64_t)) == cudaSuccess &&
-                  cudaMalloc(&p->d_r_gtabs, n * sizeof(GemvTabs)) == cudaSuccess &&
-                  cudaMalloc(&p->d_r_items, items.size() * sizeof(GemvItem)) == cudaSuccess &&
+  const bool ok = dev_alloc(&p->d_r_tidx, total * sizeof(uint32_t)) &&
+                  dev_alloc(&p->d_r_tbase, n * sizeof(uint64_t)) &&
+                  dev_alloc(&p->d_r_gtabs, n * sizeof(GemvTabs)) &&
+                  dev_alloc(&p->d_r_items, items.size() * sizeof(GemvItem)) &&
                   cudaMemcpyAsync(p->d_r_tbase, tbase.data(), n * sizeof(uint64_t), cudaMemcpyHostToDevice, st) == cudaSuccess &&
                   cudaMemcpyAsync(p->d_r_items, items.data(), items.size() * sizeof(GemvItem), cudaMemcpyHostToDevice, st) ==
                       cudaSuccess &&
@@ -1434,8 +1444,8 @@ static void setup_parts(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st)
   const uint32_t parts = parallel_parts(most, p->n_par, p->sms);
   if (parts < 2) return;
   const size_t bytes = size_t(p->n_par) * parts * 32 * sizeof(uint32_t);
-  const bool ok = cudaMalloc(&p->d_ppos, bytes) == cudaSuccess &&
-                  cudaMalloc(&p->d_ptabs, p->n_par * kPartTabBytes) == cudaSuccess && cudaMemsetAsync(p->d_ppos, 0, bytes, st) == cudaSuccess &&
+  const bool ok = dev_alloc(&p->d_ppos, bytes) &&
+                  dev_alloc(&p->d_ptabs, p->n_par * kPartTabBytes) && cudaMemsetAsync(p->d_ppos, 0, bytes, st) == cudaSuccess &&
                   cudaMemsetAsync(p->d_status, 0, sizeof(int), st) == cudaSuccess &&
                   launch_parallel_index(p->d_slabs + p->n_ser, p->n_par, d_payload, p->d_ppos, parts, p->d_ptabs, p->d_status, st) ==
                       cudaSuccess &&
@@ -1509,13 +1519,13 @@ int xksv_plan_index(xksv_plan* p, const void* d_payload, size_t payload_size, vo
   if (total > std::numeric_limits<uint32_t>::max() || items.size() > (1u << 31)) return 1;
   // every copy and fill on the caller's stream, ahead of the index kernel
   // (a non-blocking stream does not wait for the legacy default stream)
-  bool ok = cudaMalloc(&p->d_tidx, total * sizeof(uint32_t)) == cudaSuccess &&
-            cudaMalloc(&p->d_tmid, total * sizeof(uint32_t)) == cudaSuccess &&
-            cudaMalloc(&p->d_tbase, n * sizeof(uint64_t)) == cudaSuccess &&
-            cudaMalloc(&p->d_gtabs, n * sizeof(GemvTabs)) == cudaSuccess &&
-            cudaMalloc(&p->d_items, items.size() * sizeof(GemvItem)) == cudaSuccess &&
-            cudaMalloc(&p->d_partials, items.size() * 16 * 4 * sizeof(float)) == cudaSuccess &&
-            cudaMalloc(&p->d_counters, n * sizeof(uint32_t)) == cudaSuccess &&
+  bool ok = dev_alloc(&p->d_tidx, total * sizeof(uint32_t)) &&
+            dev_alloc(&p->d_tmid, total * sizeof(uint32_t)) &&
+            dev_alloc(&p->d_tbase, n * sizeof(uint64_t)) &&
+            dev_alloc(&p->d_gtabs, n * sizeof(GemvTabs)) &&
+            dev_alloc(&p->d_items, items.size() * sizeof(GemvItem)) &&
+            dev_alloc(&p->d_partials, items.size() * 16 * 4 * sizeof(float)) &&
+            dev_alloc(&p->d_counters, n * sizeof(uint32_t)) &&
             cudaMemcpyAsync(p->d_tbase, tbase.data(), n * sizeof(uint64_t), cudaMemcpyHostToDevice, st) == cudaSuccess &&
             cudaMemcpyAsync(p->d_items, items.data(), items.size() * sizeof(GemvItem), cudaMemcpyHostToDevice, st) == cudaSuccess &&
             cudaMemsetAsync(p->d_counters, 0, n * sizeof(uint32_t), st) == cudaSuccess &&
@@ -1578,7 +1588,7 @@ int xksv_tp_fused_create(int world, int rank, size_t max_rows_shard, size_t max_
   c->done_off = c->epoch_off + 256;
   const size_t total = c->done_off + 256;
   cudaIpcMemHandle_t h;
-  const bool ok = cudaMalloc(&c->base, total) == cudaSuccess && cudaMemset(c->base, 0, total) == cudaSuccess &&
+  const bool ok = dev_alloc(&c->base, total) && cudaMemset(c->base, 0, total) == cudaSuccess &&
                   cudaIpcGetMemHandle(&h, c->base) == cudaSuccess && cudaDeviceSynchronize() == cudaSuccess;
   if (!ok) {
     xksv_tp_fused_destroy(c);
@@ -1609,8 +1619,8 @@ int xksv_tp_fused_open(xksv_tp_fused* c, const void* handles) {
     fl[g] = reinterpret_cast<uint32_t*>(b + c->flags_off);
   }
   const size_t pb = c->world * sizeof(void*);
-  const bool ok = cudaMalloc(&c->d_peer_y[0], pb) == cudaSuccess && cudaMalloc(&c->d_peer_y[1], pb) == cudaSuccess &&
-                  cudaMalloc(&c->d_peer_flags, pb) == cudaSuccess &&
+  const bool ok = dev_alloc(&c->d_peer_y[0], pb) && dev_alloc(&c->d_peer_y[1], pb) &&
+                  dev_alloc(&c->d_peer_flags, pb) &&
                   cudaMemcpy(c->d_peer_y[0], y0.data(), pb, cudaMemcpyHostToDevice) == cudaSuccess &&
                   cudaMemcpy(c->d_peer_y[1], y1.data(), pb, cudaMemcpyHostToDevice) == cudaSuccess &&
                   cudaMemcpy(c->d_peer_flags, fl.data(), pb, cudaMemcpyHostToDevice) == cudaSuccess &&

@@ -454,6 +454,7 @@ int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** out) {
                   cudaMallocHost(&kv->h_status, sizeof(int)) == cudaSuccess &&
                   cudaMemset(kv->d_status, 0, sizeof(int)) == cudaSuccess && cudaStreamSynchronize(nullptr) == cudaSuccess;
   if (!ok) {
+    cudaGetLastError();  // not the next launch's
     xksv_kv_destroy(kv);
     return 1;
   }
