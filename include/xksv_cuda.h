@@ -354,21 +354,26 @@ typedef struct xksv_linear_args {
 } xksv_linear_args;
 
 /* Enqueues the layer on `stream`, on the device the plan was created on.
- * d_workspace is caller-owned device memory of at least
- * xksv_plan_linear_workspace(plan, batch) bytes, 256-byte aligned, its
- * contents free before and after; calls that may overlap need their own (and
- * their own plan: one call in flight per plan).  Allocates nothing, so it can
- * be captured into a graph.  A tile index (xksv_plan_index) speeds it up as
- * it does xksv_plan_gemm, and xksv_plan_set_gemm_route selects the route of 4
- * to 128 tokens here too (XKSV_GEMM_AUTO: fused up to 64 tokens; past them,
- * and for other plans of columns in multiples of 8, the weight is decoded into
- * the workspace, 2 bytes an element).  Returns 1 without launching for a slab outside the
- * payload, x or y, two slabs covering the same row of Y, a raw slab that is
- * not rows x cols, unknown types or activations, or a workspace too small;
- * batch 0 does nothing.  Slab errors are read with xksv_plan_status.  As in
+ * d_workspace is caller-owned device memory, 256-byte aligned, its contents
+ * free before and after; calls that may overlap need their own (and their own
+ * plan: one call in flight per plan).  xksv_plan_linear_workspace(plan, batch)
+ * bytes serve every call of that batch, whatever the payload and the result's
+ * type, before and after xksv_plan_index and xksv_plan_set_gemm_route (some
+ * route decodes the weight there); xksv_plan_linear_workspace_for gives what a
+ * call on d_payload takes as the plan stands, often far less: ask again after
+ * either of the two.  Allocates nothing, so it can be captured into a graph.  A
+ * tile index (xksv_plan_index) speeds it up as it does xksv_plan_gemm, and
+ * xksv_plan_set_gemm_route selects the route of 4 to 128 tokens here too
+ * (XKSV_GEMM_AUTO: fused up to 64 tokens; past them, and for other plans of
+ * columns in multiples of 8, the weight is decoded into the workspace, 2 bytes
+ * an element).  Returns 1 without launching for a slab outside the payload, x
+ * or y, two slabs covering the same row of Y, a raw slab that is not rows x
+ * cols, unknown types or activations, or a workspace too small; batch 0 does
+ * nothing.  Slab errors are read with xksv_plan_status.  As in
  * xksv_plan_gemm, batches that share a row between several CTAs add in an
  * order that may differ between runs (the last bits of the FP32 sums). */
 size_t xksv_plan_linear_workspace(const xksv_plan* plan, size_t batch);
+size_t xksv_plan_linear_workspace_for(const xksv_plan* plan, const void* d_payload, size_t batch, uint32_t y_type);
 /* The device the plan was created on (-1 for NULL). */
 int xksv_plan_device(const xksv_plan* plan);
 int xksv_plan_linear(const xksv_plan* plan, const void* d_payload, size_t payload_size,

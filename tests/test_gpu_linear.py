@@ -337,3 +337,58 @@ def test_linear_fp32_sums_stay_fp32_where_a_cta_holds_all_columns(batch):
     assert plan.status() == 0
     assert float((y - want).norm() / want.norm()) <= 32 * 2.0 ** -23 + 16 * 2.0 ** -24
     plan.close()
+
+
+def plan_of(R, C, seed, kind="normal002"):
+    """An indexed plan of one serial weight: (payload, plan, FP32 weight)."""
+    w = words_for(kind, R * C, np.random.default_rng(seed)).reshape(R, C)
+    words = np.ascontiguousarray(w.astype("<u2"))
+    pay, slabs = xg.host_pack_tensor(words.ctypes.data, R * C * 2, R, C, SERIAL)
+    for s in slabs:
+        s["dst_offset"] //= 2 * C
+        s["rows"], s["cols"] = s["rows"] or s["src_size"] // (2 * C), C
+    return torch.from_numpy(pay).to(DEV), xg.Plan(slabs), torch.from_numpy(bf16_to_f32(w)).to(DEV)
+
+
+@pytest.mark.parametrize("batch", [1, 4, 16, 64, 65])
+def test_workspace_asked_for_before_an_index_serves_after_it(batch):
+    payload, plan, w = plan_of(1024, 4096, 21)
+    ws = torch.empty(plan.linear_workspace(batch), dtype=torch.uint8, device=DEV)
+    x = torch.randn(batch, 4096, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3)).bfloat16()
+    for step in range(3):
+        if step == 1:
+            assert plan.index(payload) == 0
+        elif step == 2:
+            plan.set_gemm_route(xg.GEMM_FUSED)
+        for out in (torch.bfloat16, torch.float32):
+            y = torch.empty(batch, 1024, device=DEV, dtype=out)
+            plan.linear(payload, x, y, workspace=ws)
+            want, tol, _ = expected([(w, 0, 0)], x, 1024, None, "none", None, None)
+            assert ((y.double() - want).abs() <= torch.finfo(out).eps / 2 * want.abs() + tol).all()
+    assert plan.status() == 0
+    plan.close()
+
+
+def test_calls_reserve_what_their_route_uses():
+    """One token through an indexed weight reserves no decoded copy of it."""
+    payload, plan, w = plan_of(1024, 4096, 22)
+    assert plan.index(payload) == 0
+    x = torch.ones(64, 4096, dtype=torch.bfloat16, device=DEV)
+    y = torch.empty(64, 1024, dtype=torch.bfloat16, device=DEV)
+
+    def taken(batch):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        plan.linear(payload, x[:batch], y[:batch])
+        return torch.cuda.max_memory_allocated() - before
+
+    assert taken(1) <= 4096 and taken(3) <= 4096
+    assert taken(4) < 8 << 20  # the segments' sums of 16 tokens; the decoded weight is 8 MB
+    other = payload.clone()  # another payload than the indexed one is decoded first
+    want = y[:1].clone()
+    plan.linear(payload, x[:1], want)
+    plan.linear(other, x[:1], y[:1])
+    assert ((y[0].double() - want[0].double()).abs() <= 2.0 ** -8 * want[0].double().abs() + 2.0 ** -12).all()
+    assert plan.status() == 0
+    plan.close()

@@ -11,6 +11,7 @@
 #include <limits>
 #include <map>
 #include <mutex>
+#include <new>
 #include <queue>
 #include <vector>
 
@@ -252,6 +253,7 @@ struct xksv_plan {
   uint32_t* d_ppos = nullptr;
   void* d_ptabs = nullptr;  // kPartTabBytes a slab
   uint32_t n_fgroups = 0;
+  uint32_t most_segs = 0;  // pieces the fused segments would be cut into (0: not counted yet)
   uint64_t* d_hash_ranges = nullptr;  // per slab in creation order: {dst, decoded bytes}
   // linear layer (xksv_plan_linear): the runs of Y rows the slabs cover; off
   // when two slabs cover one row or a slab has no rows and columns
@@ -1102,6 +1104,9 @@ struct LinearSpace {
   Route route;
   uint64_t x, z, rows, scratch, total;  // workspace offsets; rows: x's rows, aligned
 };
+// The fused route's sums of n segments, and x's rows where they are copied.
+uint64_t segs_bytes(uint64_t n, uint64_t batch) { return n * 16 * ((batch + 15) / 16 * 16) * 32 * sizeof(float); }
+uint64_t rows_bytes(const xksv_plan* p, uint64_t batch) { return batch * pitch_of(p->need_x_rows) * 2; }
 // FP32 results add the tensor cores' sums of short segments (kExactUnits).
 const FusedSegs& linear_segs(const xksv_plan* p, bool f32) { return f32 && p->fexact.n ? p->fexact : p->fsegs; }
 // The payload decides whether the tile index is there: null counts for none.
@@ -1119,11 +1124,11 @@ LinearSpace linear_space(const xksv_plan* p, uint64_t batch, const void* payload
     // tokens 71 against 54; 14336 x 4096: 133 against 141, 163 against 141;
     // 4096 x 14336: 123 against 151, 146 against 151)
     s.route = Route::Fused;
-    s.z = c.take(uint64_t(linear_segs(p, f32).n) * 16 * ((batch + 15) / 16 * 16) * 32 * sizeof(float));
-    s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
+    s.z = c.take(segs_bytes(linear_segs(p, f32).n, batch));
+    s.rows = c.take(rows_bytes(p, batch));
   } else if (p->tc_ok) {
     s.route = Route::Gemm;
-    s.rows = c.take(batch * pitch_of(p->need_x_rows) * 2);
+    s.rows = c.take(rows_bytes(p, batch));
     s.scratch = c.take(p->scratch_bytes);
   } else {
     s.route = Route::Any;
@@ -1154,11 +1159,33 @@ struct OnDevice {
 
 int xksv_plan_device(const xksv_plan* p) { return p ? p->device : -1; }
 
-size_t xksv_plan_linear_workspace(const xksv_plan* p, size_t batch) {
+size_t xksv_plan_linear_workspace(const xksv_plan* pc, size_t batch) {
+  auto* p = const_cast<xksv_plan*>(pc);
   if (!p || !p->linear_ok || !batch || batch >= kMaxBatch) return 0;
-  // a later index may switch the route: room for either
-  return size_t(std::max({linear_space(p, batch, nullptr, false).total, linear_space(p, batch, p->indexed_payload, false).total,
-                          linear_space(p, batch, p->indexed_payload, true).total}));
+  uint64_t most = linear_space(p, batch, nullptr, false).total;  // without an index
+  if (p->tc_ok && p->n_ser_idx == p->n_ser + p->n_par + p->n_raw && batch >= 4 && batch <= 128) {
+    // the fused route, whether its index is there by now or not
+    if (!p->most_segs) try {
+        std::vector<FusedGroup> groups;
+        std::vector<uint32_t> members, seg0, piece0;
+        std::vector<FusedTask> tasks, pieces;
+        build_fused(p->h_slabs, p->x_base, p->sms, fused_producers(16, nullptr), groups, members, tasks, seg0);
+        cut_segments(tasks, seg0, pieces, piece0);
+        p->most_segs = uint32_t(pieces.size());
+      } catch (const std::bad_alloc&) {
+        return 0;
+      }
+    Carve c;
+    c.take(segs_bytes(p->most_segs, batch));
+    c.take(rows_bytes(p, batch));
+    most = std::max(most, c.pos);
+  }
+  return size_t(most);
+}
+
+size_t xksv_plan_linear_workspace_for(const xksv_plan* p, const void* d_payload, size_t batch, uint32_t y_type) {
+  if (!p || !p->linear_ok || !batch || batch >= kMaxBatch || (y_type != XKSV_BF16 && y_type != XKSV_FP32)) return 0;
+  return size_t(linear_space(p, batch, d_payload, y_type == XKSV_FP32).total);
 }
 
 int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_size, const xksv_linear_args* a,

@@ -107,6 +107,8 @@ _SIGS = {
                                   ctypes.c_void_p], ctypes.c_int),
     "xksv_plan_device": ([ctypes.c_void_p], ctypes.c_int),
     "xksv_plan_linear_workspace": ([ctypes.c_void_p, ctypes.c_size_t], ctypes.c_size_t),
+    "xksv_plan_linear_workspace_for": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32],
+                                       ctypes.c_size_t),
     "xksv_plan_linear": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
     "xksv_kv_create": ([ctypes.POINTER(KvDesc), ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
@@ -399,7 +401,8 @@ class Plan:
         [batch, x columns], y BF16 or FP32 [batch, Y rows]; bias [Y rows], mul and
         residual [batch, Y rows] are BF16 or FP32; act is a key of ACTS.  Rows may
         be strided; residual or mul may be y.  `workspace` (uint8, at least
-        linear_workspace(batch) bytes) defaults to a new buffer per call."""
+        linear_workspace(batch) bytes) defaults to a new buffer per call, of
+        the bytes this call takes."""
         if act not in ACTS:
             raise ValueError(f"unknown activation {act}")
         device = self.device
@@ -425,12 +428,14 @@ class Plan:
             rp, rs = _matrix(residual, batch, rows, "residual", device)
         a = LINEAR_ARGS.pack(xp, cols, xs, yp, rows, ys, batch, bp, mp, ms, rp, rs, y_type, b_type, m_type, r_type,
                              ACTS[act], 0)
-        ws, wp, wn = _workspace(workspace, self.lib.xksv_plan_linear_workspace(self.handle, batch), x.device, stream)
+        need = self.lib.xksv_plan_linear_workspace_for(self.handle, pay, batch, y_type)
+        ws, wp, wn = _workspace(workspace, need, x.device, stream)
         if self.lib.xksv_plan_linear(self.handle, pay, npay, a, wp, wn, stream):
             raise RuntimeError("xksv_plan_linear refused the call or failed to launch")
 
     def linear_workspace(self, batch):
-        """Bytes of workspace a linear call of `batch` tokens needs."""
+        """Bytes of workspace that serve any linear call of `batch` tokens, before
+        and after an index or another route."""
         return self.lib.xksv_plan_linear_workspace(self.handle, batch)
 
     def index(self, d_payload, stream=0, payload_bytes=None):
