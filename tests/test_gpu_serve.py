@@ -162,3 +162,39 @@ def test_fused_weight_epilogue(tmp_path, dtype, batch):
     cube = fw(x[:, None, None], residual=res[:, None, None])
     assert cube.shape == (batch, 1, 1, 352)
     fw.close()
+
+
+@pytest.mark.parametrize("at", ["layer", "head"])
+def test_a_step_that_raises_leaves_the_sequences_as_they_were(tmp_path, at):
+    """A step that fails in its second layer, or behind the last one, and is made
+    again gives the logits of a session that never failed; pages taken for it are
+    free again.  (The cache holds large values at first, so that a place left
+    unwritten would show.)"""
+    path = archive(tmp_path, "llama")
+    a = serve.load_session(path, DEV, pages=24, page_size=8, max_seqs=2)
+    b = serve.PagedSession(a.model, 24, page_size=8, max_seqs=2)
+    for s in (a, b):
+        s.kv.fill_(8.0)
+    prompts, tokens = [list(range(16)), [7, 9, 11]], [3, 4]  # the first one's next token needs a new page
+    seqs, _ = a.prefill(prompts)
+    other, _ = b.prefill(prompts)
+    module = a.layers[1].mlp if at == "layer" else a.model.lm_head
+    whole, (lengths, pages) = module.forward, (dict(a.length), list(a.free_pages))
+    owned = {s: list(p) for s, p in a.owned.items()}
+
+    def fails(*args, **kwargs):
+        raise MemoryError("no room")
+
+    module.forward = fails
+    for _ in range(2):
+        with pytest.raises(MemoryError):
+            a.step(seqs, tokens)
+        assert a.length == lengths and a.owned == owned and a.free_pages == pages
+    module.forward = whole
+    want = b.step(other, tokens)
+    assert close(a.step(seqs, tokens), want, 1e-2)
+    assert a.length == {s: n + 1 for s, n in lengths.items()} and len(a.free_pages) == len(pages) - 1
+    assert close(a.step(seqs, tokens), b.step(other, tokens), 1e-2)
+    a._check()
+    a.close()
+    b.close()

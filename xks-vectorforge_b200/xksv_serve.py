@@ -104,6 +104,16 @@ class PagedSession:
             self.table[at[0], at[1]] = torch.tensor(pages, dtype=torch.int32, device=self.device)
         self.length.update(needs)
 
+    def _held(self, seqs):
+        """What _shrink takes the sequences back to."""
+        return {s: (self.length[s], len(self.owned[s])) for s in seqs}
+
+    def _shrink(self, held):
+        for s, (length, pages) in held.items():
+            self.free_pages.extend(reversed(self.owned[s][pages:]))
+            del self.owned[s][pages:]
+            self.length[s] = length
+
     def release(self, seqs):
         """Ends sequences; their pages become free."""
         for s in seqs:
@@ -156,7 +166,7 @@ class PagedSession:
         try:
             self._grow({s: p.numel() for s, p in zip(seqs, prompts)})
             return seqs, self._prefill(seqs, prompts)
-        except Exception:
+        except BaseException:
             self.release(seqs)
             raise
 
@@ -207,7 +217,8 @@ class PagedSession:
 
     def step(self, seqs, tokens):
         """One more token of each sequence (`tokens` [n]; ids on the device are
-        taken as they are); returns the logits [n, vocabulary] after it."""
+        taken as they are); returns the logits [n, vocabulary] after it.  A step
+        that raises leaves the sequences as they were."""
         import torch
         if len(set(seqs)) != len(seqs) or any(s not in self.length for s in seqs):
             fail("step: unknown or repeated sequence")
@@ -218,7 +229,16 @@ class PagedSession:
             fail("step: one token per sequence")
         if not tokens.is_cuda and (tokens.min() < 0 or tokens.max() >= self.config.vocab_size):
             fail("token id outside the vocabulary")
-        self._grow({s: self.length[s] + 1 for s in seqs})
+        held = self._held(seqs)
+        try:
+            self._grow({s: self.length[s] + 1 for s in seqs})
+            return self._step(seqs, tokens)
+        except BaseException:  # some layers hold the token's keys, others do not
+            self._shrink(held)
+            raise
+
+    def _step(self, seqs, tokens):
+        import torch
         with torch.no_grad(), torch.cuda.device(self.device):
             rows = torch.tensor(seqs, device=self.device)
             lens = torch.tensor([self.length[s] for s in seqs], dtype=torch.int32, device=self.device)
