@@ -366,10 +366,10 @@ typedef struct xksv_linear_args {
  * xksv_plan_set_gemm_route selects the route of 4 to 128 tokens here too
  * (XKSV_GEMM_AUTO: fused up to 64 tokens; past them, and for other plans of
  * columns in multiples of 8, the weight is decoded into the workspace, 2 bytes
- * an element).  Returns 1 without launching for a slab outside the payload, x
- * or y, two slabs covering the same row of Y, a raw slab that is not rows x
- * cols, unknown types or activations, or a workspace too small; batch 0 does
- * nothing.  Slab errors are read with xksv_plan_status.  As in
+ * an element).  Returns 1 without launching for 2^20 tokens or more, a slab
+ * outside the payload, x or y, two slabs covering the same row of Y, a raw slab
+ * that is not rows x cols, unknown types or activations, or a workspace too
+ * small; batch 0 does nothing.  Slab errors are read with xksv_plan_status.  As in
  * xksv_plan_gemm, batches that share a row between several CTAs add in an
  * order that may differ between runs (the last bits of the FP32 sums). */
 size_t xksv_plan_linear_workspace(const xksv_plan* plan, size_t batch);

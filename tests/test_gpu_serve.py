@@ -198,3 +198,23 @@ def test_a_step_that_raises_leaves_the_sequences_as_they_were(tmp_path, at):
     a._check()
     a.close()
     b.close()
+
+
+def test_fused_weight_takes_more_tokens_than_one_call(tmp_path):
+    """2^20 tokens and more, which one linear call refuses, on a weight of 256 x
+    128: the first, the last and the tokens around the parts' borders."""
+    path = archive(tmp_path, "llama")
+    a = rt.ResidentArchive(path, DEV)
+    a.verify()
+    name = "lm_head.weight"
+    fw, W = a.fused(name), a.tensor(name).double()
+    n = (1 << 20) + 3
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x, res = (torch.randn(n, c, generator=g, device=DEV, dtype=torch.bfloat16) for c in (128, 256))
+    y = fw(x, act="relu", residual=res)
+    at = torch.tensor([0, (1 << 19) - 1, 1 << 19, (1 << 20) - 1, 1 << 20, n - 1], device=DEV)
+    want = torch.relu(x[at].double() @ W.t()) + res[at].double()
+    # half a step of BF16, and a FP32 sum of 128 products and the residual
+    tol = 129 * 2.0 ** -24 * (x[at].double().abs() @ W.abs().t()) + 2.0 ** -23 * (want.abs() + res[at].double().abs())
+    assert ((y[at].double() - want).abs() <= 2.0 ** -8 * want.abs() + tol).all()
+    fw.close()

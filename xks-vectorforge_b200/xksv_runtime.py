@@ -512,6 +512,9 @@ class _Acts(dict):
 TORCH_ACTS = _Acts()
 
 
+LINEAR_TOKENS = 1 << 19  # of one linear call (xksv_plan_linear takes fewer than 2^20)
+
+
 def _dense(t, rows, cols):
     """t as [rows, cols] with contiguous rows that do not overlap (a copy where
     it is transposed or expanded), BF16 or FP32."""
@@ -565,9 +568,13 @@ class FusedWeight:
             y = torch.empty(batch, self.rows, device=x.device, dtype=x.dtype)
             if bias is not None and bias.dtype not in (torch.bfloat16, torch.float32):
                 bias = bias.float()
-            self.plan.linear(self.archive.payload, _dense(x, batch, self.cols), y, bias=bias, act=act,
-                             mul=None if mul is None else _dense(mul, batch, self.rows),
-                             residual=None if residual is None else _dense(residual, batch, self.rows), stream=stream)
+            xb = _dense(x, batch, self.cols)
+            mul = None if mul is None else _dense(mul, batch, self.rows)
+            residual = None if residual is None else _dense(residual, batch, self.rows)
+            for a in range(0, batch, LINEAR_TOKENS):
+                cut = (lambda t: None if t is None else t[a:a + LINEAR_TOKENS]) if batch > LINEAR_TOKENS else lambda t: t
+                self.plan.linear(self.archive.payload, cut(xb), cut(y), bias=bias, act=act, mul=cut(mul),
+                                 residual=cut(residual), stream=stream)
             self._check(stream)
             return y.reshape(*lead, self.rows)
         if batch >= xksv_gpu.TC_MIN_BATCH and self._scratch_need:
