@@ -218,3 +218,28 @@ def test_fused_weight_takes_more_tokens_than_one_call(tmp_path):
     tol = 129 * 2.0 ** -24 * (x[at].double().abs() @ W.abs().t()) + 2.0 ** -23 * (want.abs() + res[at].double().abs())
     assert ((y[at].double() - want).abs() <= 2.0 ** -8 * want.abs() + tol).all()
     fw.close()
+
+
+def test_hooks_of_fused_modules_run(tmp_path):
+    """Forward hooks of every layer that a session calls run, once a step, and
+    what a hook returns is used."""
+    path = archive(tmp_path, "llama-gelu")
+    s = serve.load_session(path, DEV, pages=8, page_size=8, max_seqs=1)
+    seen = []
+    for layer in s.layers:
+        for name, m in layer.named_modules():
+            if name.rsplit(".", 1)[-1] in ("q_proj", "k_proj", "v_proj", "o_proj", "mlp", "gate_proj", "up_proj", "down_proj"):
+                m.register_forward_hook(lambda m, args, out, name=name: seen.append(name))
+    seqs, want = s.prefill([[1, 2, 3]])
+    assert len(seen) == 8 * len(s.layers) and len(set(seen)) == 8
+    seen.clear()
+    s.step(seqs, [4])
+    assert len(seen) == 8 * len(s.layers) and len(set(seen)) == 8
+    s.release(seqs)
+    handle = s.layers[1].mlp.gate_proj.register_forward_hook(lambda m, args, out: torch.zeros_like(out))
+    seqs, other = s.prefill([[1, 2, 3]])
+    assert not close(other, want)
+    s.release(seqs)
+    handle.remove()
+    assert close(s.prefill([[1, 2, 3]])[1], want)
+    s.close()

@@ -650,7 +650,8 @@ class FusedMLP:
         self.gate, self.up, self.down, self.act = module.gate_proj, module.up_proj, module.down_proj, act
 
     def __call__(self, x, residual=None):
-        return self.down.forward(self.up.forward(x, mul=self.gate.forward(x, act=self.act)), residual=residual)
+        # (the modules themselves, so that their hooks run)
+        return self.down(self.up(x, mul=self.gate(x, act=self.act)), residual=residual)
 
 
 def install_fused_mlp(model):

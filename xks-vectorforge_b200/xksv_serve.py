@@ -133,9 +133,9 @@ class PagedSession:
         """The output product, the feed-forward layer and their residuals."""
         o = layer.self_attn.o_proj
         x = attended.flatten(-2)
-        h = o.forward(x, residual=h) if hasattr(o, "xksv_fused") else h + o(x)
+        h = o(x, residual=h) if hasattr(o, "xksv_fused") else h + o(x)
         x = layer.post_attention_layernorm(h)
-        return layer.mlp.forward(x, residual=h) if hasattr(layer.mlp, "xksv_fused_mlp") else h + layer.mlp(x)
+        return layer.mlp(x, residual=h) if hasattr(layer.mlp, "xksv_fused_mlp") else h + layer.mlp(x)
 
     def _check(self):
         stream = self._stream()
