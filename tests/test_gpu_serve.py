@@ -243,3 +243,37 @@ def test_hooks_of_fused_modules_run(tmp_path):
     handle.remove()
     assert close(s.prefill([[1, 2, 3]])[1], want)
     s.close()
+
+
+def test_scales_of_layers_and_heads(tmp_path):
+    """Keys of large biases (qwen2) in an 8-bit cache: with a scale per layer,
+    kind and head each stored element is its value rounded once (2^-4 relative,
+    and the BF16 key's own 2^-8), where the default saturates at 28."""
+    path = archive(tmp_path, "qwen2")
+    s = serve.load_session(path, DEV, pages=4, page_size=8, max_seqs=1)
+    with torch.no_grad():
+        for layer in s.layers:
+            layer.self_attn.k_proj.bias.mul_(200)
+    prompt = [list(range(20))]
+    s.prefill(prompt)
+    exact = s.kv.double()  # BF16 [layers, 2, pages, page_size, heads, dim]
+    top = exact.abs().amax((2, 3, 5))
+    assert float(top[0, 0].min()) > 28 and (top[0, :, 0] != top[0, :, 1]).all()  # each head a scale of its own
+
+    def stored(scale):
+        e = serve.PagedSession(s.model, 4, page_size=8, max_seqs=1, kv_dtype="e4m3", **scale)
+        e.prefill(prompt)
+        rows = torch.stack([torch.stack([c.view(torch.uint8).view(torch.float8_e4m3fn).double() * f.double()[:, None]
+                                         for c, f in ((x.k, x.k_scale), (x.v, x.v_scale))]) for x in e.caches])
+        e._check()
+        e.close()
+        return rows
+
+    # (the second layer's input already holds the first one's roundings)
+    got, want, step = stored(dict(kv_scale=top.float() / 400))[0], exact[0], top[0] / 400
+    assert ((got - want).abs() <= (2.0 ** -4 + 2.0 ** -7) * want.abs() + 2.0 ** -10 * step[:, None, None, :, None]).all()
+    assert float(stored({})[0, 0].abs().max()) == 28.0
+    for bad, match in ((torch.ones(3, device=DEV), "shape"), (0.0, "above zero"), (float("nan"), "above zero")):
+        with pytest.raises(rt.ArchiveError, match=match):
+            serve.PagedSession(s.model, 4, kv_dtype="e4m3", kv_scale=bad)
+    s.close()

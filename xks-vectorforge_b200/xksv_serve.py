@@ -41,7 +41,10 @@ class PagedSession:
     feed-forward layer, two norms a layer) over a paged cache of `pages` pages
     of `page_size` tokens.  `max_tokens` bounds one sequence (default: the
     model's positions).  kv_dtype "bf16" keeps the model's BF16; "e4m3" halves
-    the cache, its elements times `kv_scale`."""
+    the cache: an element stands for its value times `kv_scale`, a number or a
+    tensor that broadcasts to [layers, 2 (keys, values), KV heads].  Keys and
+    values beyond 448 kv_scale (28 by default) saturate there, unreported:
+    models with large key or value biases need scales of their own."""
 
     def __init__(self, model, pages, page_size=16, max_tokens=None, max_seqs=256, kv_dtype="bf16", kv_scale=1.0 / 16,
                  device=None):
@@ -66,8 +69,17 @@ class PagedSession:
         store = torch.bfloat16 if kv_dtype == "bf16" else torch.float8_e4m3fn
         shape = (len(self.layers), 2, pages, page_size, self.kv_heads, self.dim)
         self.kv = torch.zeros(shape, dtype=torch.uint8 if kv_dtype == "e4m3" else store, device=self.device).view(store)
-        self.scale = torch.full((self.kv_heads,), kv_scale, device=self.device) if kv_dtype == "e4m3" else None
-        self.caches = [xksv_gpu.KVCache(l[0], l[1], k_scale=self.scale, v_scale=self.scale) for l in self.kv]
+        scales = [(None, None)] * len(self.layers)
+        if kv_dtype == "e4m3":
+            scale = torch.as_tensor(kv_scale, dtype=torch.float32, device=self.device)
+            shape = (len(self.layers), 2, self.kv_heads)
+            try:
+                scales = scale.expand(shape).contiguous()
+            except RuntimeError:
+                fail(f"kv_scale of shape {list(scale.shape)} for {list(shape)} [layers, 2, heads]")
+            if not bool(((scales > 0) & torch.isfinite(scales)).all()):
+                fail("kv_scale is above zero and finite")
+        self.caches = [xksv_gpu.KVCache(l[0], l[1], k_scale=s[0], v_scale=s[1]) for l, s in zip(self.kv, scales)]
         self.table = torch.full((max_seqs, -(-self.max_tokens // page_size)), -1, dtype=torch.int32, device=self.device)
         self.free_pages = list(range(pages))[::-1]
         self.free_seqs = list(range(max_seqs))[::-1]
@@ -184,7 +196,7 @@ class PagedSession:
                 cache.append(k, v, self.table, index, seq=seq, inv_freq=self.inv_freq, rot_scale=self.rot_scale, q=q,
                              stream=self._stream())
                 # the keys and values as later steps will read them
-                k, v = (self._cached(c, page, slot, q.dtype) for c in (cache.k, cache.v))
+                k, v = (self._cached(c, s, page, slot, q.dtype) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
                 out = torch.empty_like(q)
                 at = 0
                 for n in counts:
@@ -196,12 +208,12 @@ class PagedSession:
         self._check()
         return logits
 
-    def _cached(self, c, page, slot, dtype):
+    def _cached(self, c, scale, page, slot, dtype):
         import torch
         if c.dtype == dtype:
             return c[page, slot]
         rows = c.view(torch.uint8)[page, slot].view(c.dtype).float()
-        return (rows * self.scale[:, None]).to(dtype)
+        return (rows * scale[:, None]).to(dtype)
 
     def _causal(self, q, k, v, window):
         import torch
