@@ -200,3 +200,20 @@ def test_calls_after_an_index_without_room_for_the_parts():
         torch.cuda.empty_cache()
     assert (out.cpu().numpy().view("<u2") == want).all()
     plan.close()
+
+
+def test_index_without_parts():
+    """The part index can be left off: its memory is not taken, and decodes are the same."""
+    payload, entries, want = slabs([(16, 1024)] * 1000, xg.CODEC_PARALLEL32, "normal002", 9)
+    torch.cuda.synchronize()
+    taken = []
+    for parts in (True, False, True):
+        plan = xg.Plan(entries)
+        before = torch.cuda.mem_get_info()[0]
+        assert plan.index(payload, parts=parts) == 0
+        taken.append(before - torch.cuda.mem_get_info()[0])
+        out = torch.empty(want.size * 2, dtype=torch.uint8, device=DEV)
+        plan.decode(payload, out)
+        assert plan.status() == 0 and (out.cpu().numpy().view("<u2") == want).all()
+        plan.close()
+    assert taken[0] >= 8 << 20 and taken[1] <= 2 << 20 and taken[2] >= 8 << 20  # 10 KB a slab

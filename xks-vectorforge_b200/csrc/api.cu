@@ -249,6 +249,7 @@ struct xksv_plan {
   xksv::GemvTabs* d_r_gtabs = nullptr;
   xksv::GemvItem* d_r_items = nullptr;
   // part index of the parallel slabs (xksv_plan_index of few slabs)
+  bool parts_on = true;  // xksv_plan_set_parts
   uint32_t par_parts = 1;
   uint32_t* d_ppos = nullptr;
   void* d_ptabs = nullptr;  // kPartTabBytes a slab
@@ -1287,6 +1288,12 @@ int xksv_plan_linear(const xksv_plan* pc, const void* d_payload, size_t payload_
   return 0;
 }
 
+int xksv_plan_set_parts(xksv_plan* p, int on) {
+  if (!p) return 1;
+  p->parts_on = on != 0;
+  return 0;
+}
+
 int xksv_plan_set_gemm_route(xksv_plan* p, int route) {
   if (!p || route < XKSV_GEMM_AUTO || route > XKSV_GEMM_FUSED) return 1;
   p->gemm_route = route;
@@ -1468,7 +1475,7 @@ static void setup_ragged(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st
 static void setup_parts(xksv_plan* p, const uint8_t* d_payload, cudaStream_t st) {
   uint64_t most = 0;
   for (uint32_t i = p->n_ser; i < p->n_ser + p->n_par; ++i) most = std::max(most, p->h_slabs[i].rows * p->h_slabs[i].cols);
-  const uint32_t parts = parallel_parts(most, p->n_par, p->sms);
+  const uint32_t parts = p->parts_on ? parallel_parts(most, p->n_par, p->sms) : 1;
   if (parts < 2) return;
   const size_t bytes = size_t(p->n_par) * parts * 32 * sizeof(uint32_t);
   const bool ok = dev_alloc(&p->d_ppos, bytes) &&

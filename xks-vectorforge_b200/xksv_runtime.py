@@ -216,6 +216,7 @@ class ResidentArchive:
         import numpy as np
         import torch
         self.path = str(path)
+        self.part_index = True  # False: fused weights keep no parts of parallel-codec slabs (Plan.index)
         self.device = torch.device(device)
         if self.device.type != "cuda":
             fail("GPU decode requires a CUDA device")
@@ -540,7 +541,7 @@ class FusedWeight:
         self.rows, self.cols = t["shape"]
         self.plan = xksv_gpu.Plan(gemm_entries(t), lib=archive.lib)
         with torch.cuda.device(archive.device):
-            if self.plan.index(archive.payload, archive._stream()):
+            if self.plan.index(archive.payload, archive._stream(), parts=archive.part_index):
                 fail(f"fused GEMV failed: {self.name}")
         # batch >= TC_MIN_BATCH decodes the weight into a BF16 scratch for the tensor
         # cores: borrow the archive's shared one instead of keeping a
@@ -713,17 +714,19 @@ def backend_class(config):
     return AutoModelForCausalLM
 
 
-def load_archive(path, device, model=None, verify=True, fused_gemv=False, fused_mlp=False):
+def load_archive(path, device, model=None, verify=True, fused_gemv=False, fused_mlp=False, part_index=True):
     """The ``load_archive(..., gpu_decode=True)`` flow (python/runtime.py:31-117)
     on a resident archive: upload, device verification, one-launch decode into
     the model, optional fused linear layers.  Without `model`, the model is
     built from the archive's config.json asset with Transformers, as the
     reference does, and a tokenizer is loaded when the assets hold one.
     `fused_mlp` (with fused_gemv) fuses layers with a bias too and the gated
-    feed-forward layers' activation and product (install_fused_mlp).
+    feed-forward layers' activation and product (install_fused_mlp);
+    `part_index` False saves the memory of parallel-codec weights' part index.
     Returns (model, tokenizer or None, archive)."""
     import torch
     archive = ResidentArchive(path, device)
+    archive.part_index = part_index
     if verify:
         archive.verify()
     tokenizer = None

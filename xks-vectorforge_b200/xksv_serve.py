@@ -27,10 +27,11 @@ from xksv_runtime import fail, load_archive
 MODEL_TYPES = ("llama", "mistral", "qwen2")
 
 
-def load_session(path, device, verify=True, **session):
+def load_session(path, device, verify=True, part_index=True, **session):
     """load_archive(fused_gemv=True, fused_mlp=True) and a PagedSession on it;
-    the keyword arguments are PagedSession's."""
-    model, tokenizer, archive = load_archive(path, device, verify=verify, fused_gemv=True, fused_mlp=True)
+    the further keyword arguments are PagedSession's."""
+    model, tokenizer, archive = load_archive(path, device, verify=verify, fused_gemv=True, fused_mlp=True,
+                                             part_index=part_index)
     s = PagedSession(model, device=archive.device, **session)
     s.tokenizer, s.archive = tokenizer, archive
     return s
