@@ -187,3 +187,49 @@ def test_truncated_file(tmp_path):
     p.write_bytes(b"XKSV\x00")
     with pytest.raises(rt.ArchiveError):
         read(p)
+
+
+def test_fused_mlp_follows_the_modules_own_formula():
+    """A gated feed-forward module is replaced where its own forward is
+    down(act(gate(x)) * up(x)) of an activation that the epilogue has -- whatever
+    the model's config says -- and keeps its forward otherwise."""
+    import types
+
+    import torch
+    import torch.nn.functional as F
+
+    class Gated(torch.nn.Module):
+        def __init__(self, f):
+            super().__init__()
+            self.f = f
+            for n in ("gate_proj", "up_proj", "down_proj"):
+                layer = torch.nn.Linear(4, 4)
+                layer.xksv_fused = layer.forward = object()
+                self.add_module(n, layer)
+
+        def forward(self, x):
+            return self.f(self, x)
+
+    def gated(act, factor=1.0, out=1.0, residual=0.0):
+        return lambda m, x: m.down_proj(m.up_proj(x) * act(m.gate_proj(x) * factor)) * out + residual * x
+
+    cases = [
+        (gated(F.silu), "silu"), (gated(F.gelu), "gelu"), (gated(F.relu), "relu"),
+        (gated(lambda z: F.gelu(z, approximate="tanh")), "gelu_tanh"),
+        (gated(F.silu, factor=0.9), None), (gated(F.silu, out=2.0), None), (gated(F.silu, residual=1.0), None),
+        (gated(torch.tanh), None), (gated(lambda z: F.silu(z.clamp(max=5))), None),
+        (lambda m, x: m.down_proj((m.up_proj(x) + 1) * F.silu(m.gate_proj(x))), None),
+        (lambda m, x: m.down_proj(m.up_proj(m.gate_proj(x))), None),
+        (lambda m, x: F.linear(x, m.gate_proj.weight[:, :0]), None),
+    ]
+    model = torch.nn.ModuleList([Gated(f) for f, _ in cases])
+    model.config = types.SimpleNamespace(hidden_act="silu")
+    forwards = [[p.forward for p in (m.gate_proj, m.up_proj, m.down_proj)] for m in model]
+    assert rt.install_fused_mlp(model) == 4
+    for m, (_, act), own in zip(model, cases, forwards):
+        assert hasattr(m, "xksv_fused_mlp") == (act is not None)
+        assert act is None or m.forward.act == act
+        assert [p.forward for p in (m.gate_proj, m.up_proj, m.down_proj)] == own
+    plain = torch.nn.ModuleList([Gated(gated(F.silu))])
+    del plain[0].up_proj.xksv_fused  # one layer is not fused
+    assert rt.install_fused_mlp(plain) == 0

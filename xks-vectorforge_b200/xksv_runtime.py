@@ -637,9 +637,34 @@ def install_fused_gemv(model, archive, biased=False):
     return installed
 
 
-# config.hidden_act names whose activation the product's epilogue computes
-EPILOGUE_ACTS = {"silu": "silu", "swish": "silu", "gelu": "gelu", "gelu_new": "gelu_tanh",
-                 "gelu_pytorch_tanh": "gelu_tanh", "relu": "relu"}
+def gated_act(module):
+    """The activation (a key of xksv_gpu.ACTS) with which a module's own forward
+    computes down_proj(act(gate_proj(x)) * up_proj(x)), found by running it
+    with stand-ins for the three layers; None for any other formula (factors,
+    clamps and sparse gates among them)."""
+    import torch
+    parts = [module.gate_proj, module.up_proj, module.down_proj]
+    own = [p.__dict__.get("forward") for p in parts]
+    g, u = torch.linspace(-6, 6, 97), torch.linspace(1, -2, 97)
+    x = torch.tensor([1.0, 0.5])[None, :, None].expand(1, 2, 97)
+    try:
+        for p, stand_in in zip(parts, (lambda t: t * g, lambda t: t * u, lambda t: t)):
+            p.forward = stand_in
+        with torch.no_grad():
+            got = type(module).forward(module, x)
+            for act, f in _torch_acts().items():
+                # (FP32 roundings of values up to 12; the two GELUs differ by 5e-4)
+                if torch.allclose(got, f(x * g) * (x * u), rtol=0, atol=2e-5):
+                    return act
+    except Exception:
+        pass
+    finally:
+        for p, f in zip(parts, own):
+            if f is None:
+                p.__dict__.pop("forward", None)
+            else:
+                p.forward = f
+    return None
 
 
 class FusedMLP:
@@ -657,13 +682,13 @@ class FusedMLP:
 
 def install_fused_mlp(model):
     """Replaces the forward of every gated feed-forward module (gate_proj,
-    up_proj, down_proj) whose three layers are fused and whose activation
-    (config.hidden_act) the epilogue has, by a FusedMLP; returns how many."""
-    act = EPILOGUE_ACTS.get(getattr(getattr(model, "config", None), "hidden_act", None))
+    up_proj, down_proj) whose three layers are fused and whose formula and
+    activation the epilogue has (gated_act), by a FusedMLP; returns how many."""
     installed = 0
     for module in model.modules():
         parts = [getattr(module, n, None) for n in ("gate_proj", "up_proj", "down_proj")]
-        if act and all(hasattr(p, "xksv_fused") for p in parts):
+        act = gated_act(module) if all(hasattr(p, "xksv_fused") for p in parts) else None
+        if act:
             module.forward = FusedMLP(module, act)
             module.xksv_fused_mlp = True
             installed += 1
@@ -721,7 +746,8 @@ def load_archive(path, device, model=None, verify=True, fused_gemv=False, fused_
     built from the archive's config.json asset with Transformers, as the
     reference does, and a tokenizer is loaded when the assets hold one.
     `fused_mlp` (with fused_gemv) fuses layers with a bias too and the gated
-    feed-forward layers' activation and product (install_fused_mlp);
+    feed-forward layers' activation and product (install_fused_mlp: layers of
+    another formula keep their own forward);
     `part_index` False saves the memory of parallel-codec weights' part index.
     Returns (model, tokenizer or None, archive)."""
     import torch
