@@ -34,8 +34,8 @@
 //     instead, which joins its pieces through shared memory (CL, kShort).
 // Measured on one B200 (32 query and 8 KV heads of 128, BF16): 131071 tokens
 // of one sequence 100 us, 5370 GB/s with the join (a copy: 6554); 64 uneven
-// sequences to 16384 tokens 395 us, 5440 GB/s; one of 777 tokens 7.5 us.  E4M3,
-// 28 and 4 heads, 130 uneven sequences to 6000: 86 us, 4360 GB/s, the
+// sequences to 16384 tokens 395 us, 5440 GB/s; one of 777 tokens 7.6 us.  E4M3,
+// 28 and 4 heads, 130 uneven sequences to 6000: 88 us, 4250 GB/s, the
 // conversion's instructions besides the reads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -973,8 +973,8 @@ void shape_of(uint32_t dp, uint32_t* block, uint32_t* per_sm) {
 // Where the units' clusters fit the GPU at once and the table's room is at most
 // kShort tokens, a cluster takes a unit, else all warps share all blocks and a
 // second kernel joins.  8 KV heads of 128 in BF16, clusters against that: one
-// sequence of 777 tokens 7.8 and 10.0 us, of 4000 14.1 and 14.7; two of 4000
-// 16.2 and 15.8; six of 777 10.4 and 14.3.  Past one wave the clusters lose:
+// sequence of 777 tokens 7.6 and 10.2 us, of 4000 14.6 and 15.9; two of 4000
+// 16.7 and 17.2; six of 777 11.0 and 15.8.  Past one wave the clusters lose:
 // eight uneven sequences to 777 15.0 and 12.1, 64 of them 81 and 28.
 constexpr uint64_t kShort = 4096;
 
