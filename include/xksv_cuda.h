@@ -463,7 +463,8 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* str
  *   t_j = scale * q[s, h] . K[j, g]   (softcap c > 0: c * tanh(t_j / c))
  *   out[s, h] = sum_j softmax(t)_j V[j, g],   lse[s, h] = log sum_j exp(t_j).
  * No score above -infinity (L = 0 among them): zeros and -infinity; a score
- * that is NaN or +infinity: NaN in both. Tokens behind L, and the rest of
+ * that is NaN or +infinity: NaN in both; an infinite element of an attended
+ * value: infinity or NaN there. Tokens behind L, and the rest of
  * their pages, are not read. q and out are [seqs, q_heads, head_dim] of
  * `type`, strides in elements ([0] sequence, [1] head), the last dimension
  * contiguous; type is the cache's, or BF16 or FP16 over an E4M3 cache. lse is

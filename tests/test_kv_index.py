@@ -185,3 +185,13 @@ def test_null_arguments_are_refused():
     assert lib.xksv_plan_linear(None, None, 0, None, None, 0, None) == 1
     assert lib.xksv_plan_linear_workspace(None, 4) == 0
     lib.xksv_kv_destroy(None)
+
+
+def test_plan_calls_without_a_plan():
+    import build as b
+    b.build()
+    import xksv_gpu as xg
+    lib = xg.load()
+    assert lib.xksv_plan_linear_workspace_for(None, None, 4, xg.BF16) == 0
+    assert lib.xksv_plan_set_parts(None, 0) == 1
+    assert lib.xksv_plan_device(None) == -1
