@@ -190,7 +190,15 @@ def test_calls_after_an_index_without_room_for_the_parts():
     assert plan.status() == 0
     torch.cuda.empty_cache()
     free, _ = torch.cuda.mem_get_info()
-    full = torch.empty(free - (6 << 20), dtype=torch.uint8, device=DEV)  # the parts' tables take 10 MB
+    full = None
+    for spare in (6, 7, 8, 9):  # the parts' tables take 10 MB
+        try:
+            full = torch.empty(free - (spare << 20), dtype=torch.uint8, device=DEV)
+            break
+        except torch.OutOfMemoryError:
+            continue
+    if full is None:
+        pytest.skip("the memory is not there to be taken")
     try:
         assert plan.index(payload) == 0
         plan.decode(payload, out)

@@ -21,7 +21,7 @@
 //   * Weights reach the second product as 16-bit numbers, a pair hi + lo of two
 //     products (BF16: 2^-17 relative, FP16 and E4M3: FP16, 2^-23): one rounding
 //     would be as coarse as a result of the same type.  FP16 weights are scaled
-//     by 2^15: what the pair drops is below 2^-40 of the largest.  (One FP16
+//     by 2^15, so that less than 2^-40 of the largest falls out of FP16's range.  (One FP16
 //     rounding: 64 uneven FP16 sequences 375 us against 377, E4M3 105 against
 //     107, and an FP16 result 1.35 times as far from the exact one.)
 //   * E4M3 keys and values become FP16 exactly; the query is brought to FP16
