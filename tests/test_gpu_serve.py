@@ -277,3 +277,20 @@ def test_scales_of_layers_and_heads(tmp_path):
         with pytest.raises(rt.ArchiveError, match=match):
             serve.PagedSession(s.model, 4, kv_dtype="e4m3", kv_scale=bad)
     s.close()
+
+
+def test_ids_on_the_device_outside_the_vocabulary(tmp_path):
+    """They give rows of NaN and change no other sequence."""
+    path = archive(tmp_path, "llama")
+    a = serve.load_session(path, DEV, pages=8, page_size=8, max_seqs=3)
+    b = serve.PagedSession(a.model, 8, page_size=8, max_seqs=3)
+    prompts = [[1, 2], [3, 4, 5], [6]]
+    seqs, _ = a.prefill(prompts)
+    other, _ = b.prefill(prompts)
+    got = a.step(seqs, torch.tensor([256, 7, -1], device=DEV))
+    want = b.step(other, torch.tensor([255, 7, 0], device=DEV))
+    assert torch.isnan(got[0]).all() and torch.isnan(got[2]).all() and torch.isfinite(want).all()
+    assert close(got[1:2], want[1:2], 1e-2)
+    a._check()
+    a.close()
+    b.close()

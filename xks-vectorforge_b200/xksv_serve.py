@@ -229,9 +229,10 @@ class PagedSession:
         return out[0].transpose(0, 1)
 
     def step(self, seqs, tokens):
-        """One more token of each sequence (`tokens` [n]; ids on the device are
-        taken as they are); returns the logits [n, vocabulary] after it.  A step
-        that raises leaves the sequences as they were."""
+        """One more token of each sequence (`tokens` [n]); returns the logits [n,
+        vocabulary] after it.  Ids outside the vocabulary are refused; ids on
+        the device are not waited for: there such a row's logits are NaN.  A
+        step that raises leaves the sequences as they were."""
         import torch
         if len(set(seqs)) != len(seqs) or any(s not in self.length for s in seqs):
             fail("step: unknown or repeated sequence")
@@ -256,7 +257,9 @@ class PagedSession:
             rows = torch.tensor(seqs, device=self.device)
             lens = torch.tensor([self.length[s] for s in seqs], dtype=torch.int32, device=self.device)
             table, index = self.table[rows], lens - 1
-            h = self.core.embed_tokens(tokens.to(self.device))
+            ids = tokens.to(self.device)
+            inside = ids.clamp(0, self.config.vocab_size - 1)  # (another id would fault the embedding)
+            h = self.core.embed_tokens(inside)
             stream = self._stream()
             for layer, cache, window in zip(self.layers, self.caches, self.windows):
                 q, k, v = self._project(layer, h)
@@ -264,7 +267,8 @@ class PagedSession:
                 out = torch.empty_like(q)
                 cache.attend(q, table, lens, out, window=window, stream=stream)
                 h = self._finish(layer, h, out)
-            return self.model.lm_head(self.core.norm(h))
+            logits = self.model.lm_head(self.core.norm(h))
+            return logits.masked_fill_((ids != inside)[:, None], float("nan")) if tokens.is_cuda else logits
 
     def generate(self, prompts, max_new_tokens, eos=None):
         """Greedy continuations of the prompts: a list of token lists, each ended
