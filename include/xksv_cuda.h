@@ -492,6 +492,52 @@ size_t xksv_kv_attend_workspace(const xksv_kv* kv, size_t seqs, size_t q_heads, 
 int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* args, void* d_workspace, size_t workspace_bytes,
                    void* stream);
 
+/* ---------------- Part 9: sampling -------------------------------------- */
+/* No reference counterpart.  Draws one token for each row of logits [rows,
+ * vocab] (contiguous rows, `stride` elements apart, 0 for one and the same; any
+ * alignment of the type).
+ * With the row's tokens ordered by logit z, equal ones by index, and w =
+ * exp((z - largest z) / temperature), a token is kept when
+ *   - fewer than top_k tokens are before it (top_k <= 0: all),
+ *   - the weights before it sum to less than top_p times the sum of those that
+ *     top_k keeps (top_p >= 1: all; the first is always kept), and
+ *   - w >= min_p (min_p <= 0: all; above 1 as 1) and w >= exp(-700).
+ * The token is the first, by index, whose kept weights up to and including its
+ * own sum to more than u[row] times all kept ones (u below 0 as 0; u >= 1: the
+ * last kept).
+ * Temperature 0 takes the first token of the order, else it lies in
+ * [1e-6, 1e6].  Weights and sums are FP64 in a fixed order.  Tokens at -infinity
+ * are never kept.  A row with a NaN, without a logit above -infinity or with
+ * one at infinity, or with a temperature outside these or a NaN among its
+ * settings gives token -1, kept 0 and logprob NaN.
+ * tokens is int64 [rows]; kept (int32 [rows], NULL or the number of kept
+ * tokens) and logprob (FP32 [rows], NULL or the log of the token's share of
+ * the kept weights).  temperature, top_k, top_p and min_p are [rows] on the
+ * device, or NULL for the `_all` number.  Runs on CUDA device `device`,
+ * whichever is current; no workspace.  Returns 1 without launching for bad
+ * arguments: more than XKSV_SAMPLE_MAX_VOCAB tokens or 2^24 rows, misaligned
+ * pointers, a temperature_all outside its range, a NaN. */
+#define XKSV_SAMPLE_MAX_VOCAB (1u << 22)
+typedef struct xksv_sample_args {
+  const void* logits;
+  uint64_t rows, vocab, stride;
+  const float* u;
+  int64_t* tokens;
+  int32_t* kept;
+  float* logprob;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+  uint32_t type;   /* XKSV_BF16, XKSV_FP16 or XKSV_FP32 */
+  int32_t device;
+  uint32_t flags;  /* must be 0 */
+} xksv_sample_args;
+int xksv_sample(const xksv_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

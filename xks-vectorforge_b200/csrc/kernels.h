@@ -9,6 +9,20 @@
 
 namespace xksv {
 
+// Runs a call on device `dev`, whichever is current.
+struct DeviceGuard {
+  int before = -1;
+  bool ok = false;
+  explicit DeviceGuard(int dev) {
+    if (cudaGetDevice(&before) != cudaSuccess) return;
+    ok = before == dev || cudaSetDevice(dev) == cudaSuccess;
+    if (before == dev) before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
 // Dynamic shared memory opt-in of `kernel`, once per device and call site's
 // `done` (concurrent first calls set the same value).
 template <class K>

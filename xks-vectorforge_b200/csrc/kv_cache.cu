@@ -12,6 +12,7 @@
 #include <new>
 #include <utility>
 
+#include "kernels.h"
 #include "kv_cache.h"
 #include "kv_index.h"
 #include "xksv_types.h"
@@ -25,20 +26,6 @@ struct xksv_kv {
 
 namespace xksv {
 namespace {
-
-// Runs a call on the handle's device, whichever is current.
-struct DeviceGuard {
-  int before = -1;
-  bool ok = false;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&before) != cudaSuccess) return;
-    ok = before == dev || cudaSetDevice(dev) == cudaSuccess;
-    if (before == dev) before = -1;
-  }
-  ~DeviceGuard() {
-    if (before >= 0) cudaSetDevice(before);
-  }
-};
 
 // ------------------------------------------------------------- elements ---
 struct E4m3 {

@@ -40,6 +40,7 @@ class KvDesc(ctypes.Structure):
 LINEAR_ARGS = struct.Struct("@3Q3QQQ2Q2Q6I")     # xksv_linear_args
 KV_APPEND_ARGS = struct.Struct("@4Q8QQ4Q4Qf4I4x")  # xksv_kv_append_args
 KV_ATTEND_ARGS = struct.Struct("@3Q4QQ3QQ2fQ2I")  # xksv_kv_attend_args
+SAMPLE_ARGS = struct.Struct("@12Qfi2fIiI4x")  # xksv_sample_args
 
 
 _SIGS = {
@@ -120,6 +121,7 @@ _SIGS = {
                                  ctypes.c_size_t),
     "xksv_kv_attend": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                         ctypes.c_void_p], ctypes.c_int),
+    "xksv_sample": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
 }
 
 # element types and activations of the linear layer and the key/value cache
@@ -625,6 +627,54 @@ class KVCache:
             self.close()
         except Exception:
             pass
+
+
+# ----------------------------------------------------------------- sampling
+def _setting(v, rows, types, what, device):
+    """(address, number) of one of a call's settings: a number for all rows, or a
+    contiguous [rows] tensor."""
+    if not hasattr(v, "data_ptr"):
+        return 0, v
+    if v.dtype not in types or v.shape != (rows,) or not v.is_contiguous() or v.get_device() != device:
+        raise ValueError(f"{what}: a number or a contiguous {types[0]} [{rows}] tensor on CUDA device {device} is needed")
+    return v.data_ptr(), 0
+
+
+def sample(logits, u, tokens=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, kept=None, logprob=None, stream=0, lib=None):
+    """One token for each row of logits (xksv_sample): logits [rows, vocabulary] of
+    BF16, FP16 or FP32, rows strided or not; u FP32 [rows] of numbers in [0, 1)
+    that decide the draw.  temperature (0: the largest logit), top_k (0: off),
+    top_p (1: off) and min_p (0: off) are numbers or tensors [rows] (FP32, top_k
+    int32).  Writes tokens (int64 [rows], a new tensor by default), kept (int32
+    [rows] or None: how many tokens the draw was among) and logprob (FP32 [rows]
+    or None: the log of the token's share among them), and returns tokens.  A row
+    with NaN, without a finite logit or with settings outside their range gives
+    token -1."""
+    import torch
+    code = _type(logits, (BF16, FP16, FP32), "logits")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or not logits.is_cuda:
+        raise ValueError("logits: a CUDA tensor [rows, vocabulary] with contiguous rows is needed")
+    rows, vocab = logits.shape
+    dev = logits.get_device()
+    if tokens is None:
+        tokens = _workspace(None, 8 * rows, logits.device, stream)[0].view(torch.int64) if rows else u.new_empty(0, dtype=torch.int64)
+    f32, addr = (torch.float32,), []
+    for t, types, what in ((u, f32, "u"), (tokens, (torch.int64,), "tokens"), (kept, (_i32,), "kept"), (logprob, f32, "logprob")):
+        if t is None and what not in ("u", "tokens"):
+            addr.append(0)
+        elif t.dtype not in types or t.shape != (rows,) or not t.is_contiguous() or t.get_device() != dev:
+            raise ValueError(f"{what}: a contiguous {types[0]} [{rows}] tensor on CUDA device {dev} is needed")
+        else:
+            addr.append(t.data_ptr())
+    hp, heat = _setting(temperature, rows, f32, "temperature", dev)
+    kp, k = _setting(top_k, rows, (_i32,), "top_k", dev)
+    pp, p = _setting(top_p, rows, f32, "top_p", dev)
+    mp, m = _setting(min_p, rows, f32, "min_p", dev)
+    a = SAMPLE_ARGS.pack(logits.data_ptr(), rows, vocab, logits.stride(0), *addr, hp, kp, pp, mp, heat, max(0, min(k, 2 ** 31 - 1)), p, m,
+                         code, dev, 0)
+    if (lib or load()).xksv_sample(a, stream):
+        raise RuntimeError("xksv_sample refused the call or failed to launch")
+    return tokens
 
 
 # ---------------------------------------------------------- tensor parallel
