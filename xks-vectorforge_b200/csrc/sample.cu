@@ -28,30 +28,37 @@
 namespace xksv {
 namespace {
 
-constexpr int NT = 512;         // threads of a CTA
+constexpr int NT = 512;  // threads of a CTA
 constexpr int NW = NT / 32;
-constexpr int NB = 2048;        // bins of a histogram
-constexpr int kBinsPerUnit = 64;  // of the first one: bins per unit of distance (top-k) or exponent (top-p)
-constexpr int CAP = 1024;       // candidates that are sorted
 constexpr int kMaxCluster = 8;
-constexpr double kTiny = -700.0;  // weights below exp(kTiny) count as zero
-
-// What the first CTA tells the others: the border lies among the keys [klo,
-// khi], `inside` tokens with `ahead` above them; or it is key klo, index khi.
-struct Ctl {
-  uint32_t klo, khi, inside, ahead;
-};
+constexpr int kParts = kMaxCluster * NW;  // warps of a row
+constexpr int kGroups = 1024;             // groups of lanes whose largest logits guess the border
+constexpr int NB = 2048;                  // bins of the histogram of logits
+constexpr float kPerUnit = 128.f;         // of them, a unit of distance from the largest
+constexpr uint32_t kEvery = 8;            // a vector in so many is sampled
+constexpr int kGuessBins = 256;           // bins of the groups' largest logits
+constexpr float kGuessPerUnit = 8.f;
+constexpr int CAP = 2048;                 // candidates that are sorted
+constexpr double kTiny = -700.0;          // weights below exp(kTiny) count as zero
 
 struct Shared {
   uint32_t hist[NB];
-  uint64_t list[CAP], all[CAP], sorted[CAP];
-  double sum[NW + 1];      // the warps' weights, and the CTA's
-  uint64_t best[NW + 1];   // their largest logits
-  double part_w[4][NW + 1], scan_l[NW], scan_u[NW];
-  uint32_t part_c[4][NW + 1], scan_c[NW];
-  uint32_t count[NW + 1];  // their tokens
-  uint32_t listed, low, high, ahead, inside, found;
-  Ctl ctl;
+  float group[kGroups];
+  uint32_t guess[kGuessBins];
+  uint64_t list[CAP];  // this CTA's candidates: ~key, index
+  uint64_t all[CAP];   // of the first CTA: all of them
+  double part_w[2][2][kParts];  // of the row's warps, in turn
+  uint32_t part_c[2][2][kParts];
+  double quarter_w[2][4][kParts];
+  uint32_t quarter_c[2][4][kParts];
+  uint32_t part_lo[2][kParts], part_hi[2][kParts];  // their candidates' least and largest keys
+  double scan_w[NW];
+  uint32_t scan_c[NW];
+  float best[kParts];
+  double pow[16];  // 2^(i / 16)
+  double guessed;
+  uint32_t listed, low, first, found;
+  uint32_t ctl[2];
 };
 
 // Order-preserving integer of a float (no NaN; -0 is +0 by then).
@@ -63,6 +70,13 @@ __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
+// The larger; NaN when one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <class T>
 struct Elems;  // of a 16-byte vector
 template <>
@@ -70,6 +84,9 @@ struct Elems<float> {
   static constexpr int N = 4;
   static __device__ __forceinline__ void get(const uint4& v, float* z) {
     z[0] = __uint_as_float(v.x), z[1] = __uint_as_float(v.y), z[2] = __uint_as_float(v.z), z[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ float most(const uint4& v) {
+    return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
 };
 template <>
@@ -79,6 +96,11 @@ struct Elems<__nv_bfloat16> {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) z[2 * i] = __uint_as_float(w[i] << 16), z[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+  static __device__ __forceinline__ float most(const uint4& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __bfloat162float(__hmax_nan(m.x, m.y));
   }
 };
 template <>
@@ -92,6 +114,11 @@ struct Elems<__half> {
       z[2 * i] = f.x, z[2 * i + 1] = f.y;
     }
   }
+  static __device__ __forceinline__ float most(const uint4& v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+    const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    return __half2float(__hmax_nan(m.x, m.y));
+  }
 };
 template <class T>
 __device__ __forceinline__ T lowest();  // -infinity: no weight
@@ -102,29 +129,42 @@ __device__ __forceinline__ __nv_bfloat16 lowest<__nv_bfloat16>() { return __usho
 template <>
 __device__ __forceinline__ __half lowest<__half>() { return __ushort_as_half(0xfc00); }
 
-// Reads of another CTA's shared memory at this address.
+// Another CTA's shared memory at this address.
 __device__ __forceinline__ uint32_t at_rank(const void* p, uint32_t rank) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t remote(const uint32_t* p, uint32_t rank) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(at_rank(p, rank)) : "memory");
+__device__ __forceinline__ void push(double* p, uint32_t rank, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;\n" ::"r"(at_rank(p, rank)), "d"(v) : "memory");
+}
+__device__ __forceinline__ void push(uint32_t* p, uint32_t rank, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(at_rank(p, rank)), "r"(v) : "memory");
+}
+__device__ __forceinline__ void push(float* p, uint32_t rank, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;\n" ::"r"(at_rank(p, rank)), "f"(v) : "memory");
+}
+__device__ __forceinline__ uint4 pull4(const uint32_t* p, uint32_t rank) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at_rank(p, rank))
+               : "memory");
   return v;
 }
-__device__ __forceinline__ uint64_t remote(const uint64_t* p, uint32_t rank) {
+__device__ __forceinline__ uint64_t pull(const uint64_t* p, uint32_t rank) {
   uint64_t v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];\n" : "=l"(v) : "r"(at_rank(p, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ double remote(const double* p, uint32_t rank) {
-  double v;
-  asm volatile("ld.shared::cluster.f64 %0, [%1];\n" : "=d"(v) : "r"(at_rank(p, rank)) : "memory");
-  return v;
+__device__ __forceinline__ void min_at(uint32_t* p, uint32_t rank, uint32_t n) {
+  asm volatile("red.shared::cluster.min.u32 [%0], %1;\n" ::"r"(at_rank(p, rank)), "r"(n) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 
 __device__ __forceinline__ double warp_sum(double x) {
@@ -132,7 +172,16 @@ __device__ __forceinline__ double warp_sum(double x) {
   for (int d = 16; d >= 1; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
   return x;
 }
-
+// Inclusive scan over the warp's lanes.
+template <class X>
+__device__ __forceinline__ X warp_scan(X x, uint32_t lane) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const X o = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += o;
+  }
+  return x;
+}
 template <class T>
 __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   using E = Elems<T>;
@@ -142,16 +191,21 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   uint4* const held = reinterpret_cast<uint4*>(dyn + p.held_off);
   const uint32_t C = p.cluster, rank = blockIdx.x % C;
   const uint64_t row = blockIdx.x / C;
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t V = uint32_t(p.a.vocab);
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = rank * NW + warp;
+  const uint32_t V = uint32_t(p.a.vocab), parts = C * NW;
+  cluster_arrive();  // (no CTA writes to another before it has begun)
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
 
   // this row's settings
-  float heat = p.a.temperature ? p.a.temperature[row] : p.a.temperature_all;
+  const float heat = p.a.temperature ? p.a.temperature[row] : p.a.temperature_all;
   const int32_t top_k = p.a.top_k ? p.a.top_k[row] : p.a.top_k_all;
   const float top_p = p.a.top_p ? p.a.top_p[row] : p.a.top_p_all;
   const float min_p = p.a.min_p ? p.a.min_p[row] : p.a.min_p_all;
   const float u = p.a.u[row];
   const bool sane = (heat == 0.f || (heat >= kSampleColdest && heat <= kSampleHottest)) && top_p == top_p && min_p == min_p && u == u;
+  if (tid < 16) s.pow[tid] = exp2(tid / 16.0);
+  if (tid == 0) s.listed = 0, s.first = ~0u;
 
   // ---- the row's 16-byte vectors; its first element is element `skew` of
   // the first vector; this warp's vectors [wv0, wv1)
@@ -179,446 +233,784 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     for (int i = 0; i < EPV; ++i) z[i] += 0.f;  // -0 becomes +0
   };
 
-  // ---- the largest logit and its first index; NaN among them ----
-  uint64_t best = 0;
-  bool nan = false;
+  // ---- the largest logit, of the row and of the groups of lanes ----
+  float mine = -INFINITY;
+#pragma unroll 4
   for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
     const uint4 w = read(v);
     if (resident) held[v - v0] = w;
-    float z[EPV];
-    E::get(w, z);
-#pragma unroll
-    for (int i = 0; i < EPV; ++i) {
-      z[i] += 0.f;
-      nan |= z[i] != z[i];
-      const uint64_t me = uint64_t(key_of(z[i])) << 32 | ~(v * EPV + i - skew);
-      best = me > best ? me : best;
-    }
+    mine = max_nan(mine, E::most(w));
   }
-  if (nan) best = ~0ull;
+  // groups: a lane, or two or four; every CTA gets all of them
+  const uint32_t groups = min(uint32_t(kGroups), C * NT), wide = C * NT / groups;
+  cluster_wait();
+  {
+    float g = mine;
+    if (wide > 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, 1));
+    if (wide > 2) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, 2));
+    for (uint32_t r = lane % wide; r < C; r += wide) push(&s.group[(rank * NT + tid) / wide], r, g);
 #pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) {
-    const uint64_t o = __shfl_xor_sync(0xffffffffu, best, d);
-    best = o > best ? o : best;
-  }
-  if (lane == 0) s.best[warp] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < NW; ++w) best = s.best[w] > best ? s.best[w] : best;
-    s.best[NW] = best;
+    for (int d = 16; d >= 1; d >>= 1) mine = max_nan(mine, __shfl_xor_sync(0xffffffffu, mine, d));
+    if (lane < C) push(&s.best[me], lane, mine);
   }
   cluster_sync();
-  best = 0;
-  for (uint32_t r = 0; r < C; ++r) {
-    const uint64_t o = remote(&s.best[NW], r);
-    best = o > best ? o : best;
-  }
-  const float zmax = value_of(uint32_t(best >> 32));
-  const uint32_t first = ~uint32_t(best);
+  float zmax = -INFINITY;
+  for (uint32_t i = lane; i < parts; i += 32) zmax = max_nan(zmax, s.best[i]);
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) zmax = max_nan(zmax, __shfl_xor_sync(0xffffffffu, zmax, d));
+  zmax += 0.f;
 
   auto answer = [&](int64_t token, int32_t kept, float logprob) {
     p.a.tokens[row] = token;
     if (p.a.kept) p.a.kept[row] = kept;
     if (p.a.logprob) p.a.logprob[row] = logprob;
   };
-  // NaN's key is above infinity's; a largest of +-infinity has no distribution
-  const bool bad = !sane || !(fabsf(zmax) < INFINITY);
-  if (bad || heat == 0.f || top_k == 1 || top_p <= 0.f) {
-    if (rank == 0 && tid == 0) answer(bad ? -1 : int64_t(first), bad ? 0 : 1, bad ? NAN : 0.f);
-    cluster_sync();  // nobody's shared memory ends while it is read
+  // a largest of NaN or +-infinity has no distribution
+  if (!sane || !(fabsf(zmax) < INFINITY)) {
+    if (rank == 0 && tid == 0) answer(-1, 0, NAN);
     return;
   }
+  if (heat == 0.f || top_k == 1 || top_p <= 0.f) {  // the first of the largest
+    uint32_t first = ~0u;
+    for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+      float z[EPV];
+      fetch(v, z);
+#pragma unroll
+      for (int i = 0; i < EPV; ++i)
+        if (z[i] == zmax) first = min(first, v * EPV + i - skew);
+    }
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0 && first != ~0u) min_at(&s.first, 0, first);
+    cluster_sync();
+    if (rank == 0 && tid == 0) answer(s.first, 1, 0.f);
+    return;
+  }
+  // exp((z - zmax) / heat) = 2^(n / 16) exp(r), with n whole, |r| <= log(2) / 32
+  // and the series of exp(r) to the 6th power (the 7th: 5e-16)
   const double zm = zmax, cool = 1.0 / double(heat);
-  auto weight = [&](float z) { return exp((double(z) - zm) * cool); };
+  auto weight = [&](float z) {
+    constexpr double kLn2By16 = 0.69314718055994530942 / 16, kBig = 6755399441055744.0;  // 1.5 * 2^52
+    const double x = (double(z) - zm) * cool;
+    const double big = fma(x, 1.0 / kLn2By16, kBig);
+    const int n = __double2loint(big);
+    const double r = fma(big - kBig, -kLn2By16, x);
+    double e = fma(r, 1.0 / 720, 1.0 / 120);
+    e = fma(e, r, 1.0 / 24);
+    e = fma(e, r, 1.0 / 6);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    e *= s.pow[n & 15];
+    e = __hiloint2double(__double2hiint(e) + (n >> 4 << 20), __double2loint(e));
+    return x < kTiny ? 0.0 : e;
+  };
   // the least logit that min-p and the smallest weight leave
   const double lowest_x = min_p > 0.f ? fmax(kTiny, log(fmin(1.0, double(min_p)))) : kTiny;
   const float floor_z = __double2float_ru(zm + lowest_x * double(heat));
 
-  // the tokens that are still in: key above bkey, or bkey with an index up to
-  // bidx (at first all above -infinity)
-  uint32_t bkey = key_of(-INFINITY);
-  int32_t bidx = -1;
-  auto in = [&](uint32_t k, uint32_t i) { return k > bkey || (k == bkey && int32_t(i) <= bidx); };
+  const bool by_k = top_k > 0 && uint32_t(top_k) < V, by_p = top_p < 1.f;
 
-  // The lanes' weights and counts summed into s.sum[NW] and s.count[NW].
-  auto cta_sums = [&](double w, uint32_t c) {
+  // Every warp's numbers to every CTA; after the barrier that follows all warps
+  // hold the same sums, added in the same order.  Two sets in turn: one may
+  // still be read while the next is written.
+  uint32_t turn = 0;
+  auto share_w = [&](int i, double w) {
     w = warp_sum(w);
+    if (lane < C) push(&s.part_w[turn][i][me], lane, w);
+  };
+  auto share_c = [&](int i, uint32_t c) {
     c = __reduce_add_sync(0xffffffffu, c);
-    if (lane == 0) s.sum[warp] = w, s.count[warp] = c;
+    if (lane < C) push(&s.part_c[turn][i][me], lane, c);
+  };
+  auto sum_of = [&](const double* part) {
+    double t = 0.0;
+    for (uint32_t i = lane; i < parts; i += 32) t += part[i];
+    return warp_sum(t);
+  };
+  auto count_of = [&](const uint32_t* part) {
+    uint32_t t = 0;
+    for (uint32_t i = lane; i < parts; i += 32) t += part[i];
+    return __reduce_add_sync(0xffffffffu, t);
+  };
+  // A token to this CTA's list.
+  auto list_it = [&](float z, uint32_t at) {
+    const uint32_t n = atomicAdd(&s.listed, 1);
+    if (n < CAP) s.list[n] = uint64_t(~key_of(z)) << 32 | at;
+  };
+  // The first CTA: s.all[0, n) in rising order (bitonic, `full` a power of two).
+  auto sort_all = [&](uint32_t n) {
+    uint32_t full = 32;
+    while (full < n) full *= 2;
+    if (full <= NT) {  // an entry a thread; the nearer exchanges within a warp
+      uint64_t x = tid < n ? s.all[tid] : ~0ull;
+      uint64_t* box = s.list;  // (the gathered list has been read)
+      __syncthreads();
+      for (uint32_t size = 2; size <= full; size *= 2)
+        for (uint32_t far = size / 2; far; far /= 2) {
+          uint64_t y;
+          if (far >= 32) {
+            box[tid] = x;
+            __syncthreads();
+            y = box[tid ^ far];
+            box = box == s.list ? s.list + NT : s.list;
+          } else {
+            y = __shfl_xor_sync(0xffffffffu, x, far);
+          }
+          if ((x > y) == (!(tid & far) == !(tid & size))) x = y;
+        }
+      s.all[tid] = x;
+      __syncthreads();
+      return;
+    }
+    for (uint32_t i = n + tid; i < full; i += NT) s.all[i] = ~0ull;
+    __syncthreads();
+    for (uint32_t size = 2; size <= full; size *= 2)
+      for (uint32_t far = size / 2; far; far /= 2) {
+        for (uint32_t i = tid; i < full / 2; i += NT) {
+          const uint32_t a = 2 * i - (i & (far - 1)), b = a + far;
+          const uint64_t x = s.all[a], y = s.all[b];
+          if ((x > y) == !(a & size)) s.all[a] = y, s.all[b] = x;
+        }
+        __syncthreads();
+      }
+  };
+  // The first CTA gathers the candidates of all (their numbers are the
+  // parts' counts `c`) and sorts them.
+  auto gather = [&](const uint32_t* c) {
+    static_assert(NW == 16 && kParts == 128, "four lanes hold a CTA's parts");
+    uint32_t mine = 0, n = 0, begin[kMaxCluster];
+    for (int i = 0; i < 4; ++i) mine += 4 * lane + i < parts ? c[4 * lane + i] : 0;
+    mine += __shfl_xor_sync(0xffffffffu, mine, 1);
+    mine += __shfl_xor_sync(0xffffffffu, mine, 2);
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      begin[r] = n;
+      n += __shfl_sync(0xffffffffu, mine, 4 * r);
+    }
+    for (uint32_t i = tid; i < n; i += NT) {
+      uint32_t from = 0, at = i;
+#pragma unroll
+      for (int r = 1; r < kMaxCluster; ++r)
+        if (r < C && i >= begin[r]) from = r, at = i - begin[r];
+      s.all[i] = pull(&s.list[at], from);
+    }
+    if (tid == 0) s.low = 0;
+    cluster_sync();  // (the other CTAs wait here before they touch their lists)
+    sort_all(n);
+    return n;
+  };
+  auto weight_at = [&](uint32_t i) { return weight(value_of(~uint32_t(s.all[i] >> 32))); };
+  constexpr int EACH = CAP / NT;  // entries of a thread
+  // How many of the n sorted tokens are kept, each while the weight before it
+  // is short of the target.
+  auto kept_of = [&](uint32_t n, double above, double target) {
+    double x[EACH], t = 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) t += x[i] = tid * EACH + i < n ? weight_at(tid * EACH + i) : 0.0;
+    const double inc = warp_scan(t, lane);
+    if (lane == 31) s.scan_w[warp] = inc;
+    __syncthreads();
+    double before = above;
+    for (uint32_t y = 0; y < warp; ++y) before += s.scan_w[y];
+    before += inc - t;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (tid * EACH + i < n && before < target) atomicMax(&s.low, tid * EACH + i + 1);
+      before += x[i];
+    }
+    __syncthreads();
+    return s.low;
+  };
+  // The draw, where all kept tokens are the first CTA's first n sorted ones or
+  // fewer: the ones that top-p and min-p leave, ordered by index.
+  auto draw_sorted = [&](uint32_t n, double whole) {
+    if (by_p) {
+      if (by_k) {
+        double x = 0.0;
+        for (uint32_t i = tid; i < n; i += NT) x += weight_at(i);
+        x = warp_sum(x);
+        if (lane == 0) s.scan_w[warp] = x;
+        __syncthreads();
+        whole = 0.0;
+        for (int y = 0; y < NW; ++y) whole += s.scan_w[y];
+        __syncthreads();
+      }
+      n = kept_of(n, 0.0, double(top_p) * whole);
+    }
+    // min-p leaves a prefix too
+    uint32_t keep = 0;
+    for (uint32_t i = tid; i < (n + NT - 1) / NT * NT; i += NT)
+      keep += __syncthreads_count(i < n && value_of(~uint32_t(s.all[i < n ? i : 0] >> 32)) >= floor_z);
+    n = keep;
+    for (uint32_t i = tid; i < n; i += NT) s.all[i] = s.all[i] << 32 | s.all[i] >> 32;
+    if (tid == 0) s.low = ~0u;
+    sort_all(n);
+    // (sort_all's padding is no token)
+    double x[EACH], t = 0.0;
+    auto z_of = [&](uint32_t i) { return value_of(~uint32_t(s.all[i])); };
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) t += x[i] = tid * EACH + i < n ? weight(z_of(tid * EACH + i)) : 0.0;
+    const double inc = warp_scan(t, lane);
+    if (lane == 31) s.scan_w[warp] = inc;
+    __syncthreads();
+    double before = inc - t, all = 0.0;
+    for (uint32_t y = 0; y < NW; ++y) {
+      before += y < warp ? s.scan_w[y] : 0.0;
+      all += s.scan_w[y];
+    }
+    const double target = fmax(double(u), 0.0) * all;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      before += x[i];
+      if (tid * EACH + i < n && before > target) atomicMin(&s.low, tid * EACH + i);
+    }
     __syncthreads();
     if (tid == 0) {
-      double t = 0.0;
-      uint32_t n = 0;
-      for (int i = 0; i < NW; ++i) t += s.sum[i], n += s.count[i];
-      s.sum[NW] = t, s.count[NW] = n;
+      const uint32_t i = min(s.low, n - 1);
+      answer(int64_t(s.all[i] >> 32), int32_t(n), float((double(z_of(i)) - zm) * cool - log(all)));
     }
   };
-  auto cluster_weight = [&]() {
-    double t = 0.0;
-    for (uint32_t r = 0; r < C; ++r) t += remote(&s.sum[NW], r);
-    return t;
+
+  // the tokens that are still in: key above bkey, or bkey with an index up to
+  // bidx (at first all above -infinity)
+  float nearest = -1.f;  // the distance that few candidates were looked for within,
+  double weight_near = 0.0;  // and their weight
+  uint32_t bkey = key_of(-INFINITY);
+  int32_t bidx = -1;
+  bool cut = false;
+  auto in = [&](uint32_t k, uint32_t i) { return k > bkey || (k == bkey && int32_t(i) <= bidx); };
+  double whole = -1.0;  // all tokens' weight, when known
+
+  // Every warp finds the first of the 256 or 2048 bins up to which `want` lie;
+  // with none, their number.
+  auto bin_with = [&](const uint32_t* bins, uint32_t want) {
+    uint32_t t = 0, bin = kGuessBins;
+    constexpr int PER = kGuessBins / 32;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) t += bins[lane * PER + i];
+    uint32_t run = warp_scan(t, lane) - t;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      run += bins[lane * PER + i];
+      if (run >= want && bin == kGuessBins) bin = lane * PER + i;
+    }
+    return __reduce_min_sync(0xffffffffu, bin);
+  };
+  // The first CTA: the bins of all CTAs' histograms, four a thread.
+  auto all_bins = [&](uint32_t* h) {
+    h[0] = h[1] = h[2] = h[3] = 0;
+    static_assert(NB / NT == 4, "a vector of bins a thread");
+#pragma unroll
+    for (uint32_t r = 0; r < kMaxCluster; ++r) {
+      if (r >= C) break;
+      const uint4 x = pull4(&s.hist[tid * 4], r);
+      h[0] += x.x, h[1] += x.y, h[2] += x.z, h[3] += x.w;
+    }
+  };
+  // Inclusive scan over the CTA's threads.
+  auto cta_scan = [&](auto x, auto* parts_of) {
+    x = warp_scan(x, lane);
+    if (lane == 31) parts_of[warp] = x;
+    __syncthreads();
+    for (uint32_t y = 0; y < warp; ++y) x += parts_of[y];
+    return x;
+  };
+  // Counts a logit by its distance from the largest, less `start`, rounded to
+  // bins: those farther than `beyond`, and none behind the last bin.
+  float start = 0.f, beyond = -1.f, per_unit = kPerUnit;
+  auto count_it = [&](float z) {
+    const float d = zmax - z, x = (d - start) * per_unit;
+    if (d > beyond && x < float(NB) - 1.5f) atomicAdd(&s.hist[__float2uint_rn(x)], 1);
   };
 
-  // The border of a prefix: by_weight, the shortest whose weight reaches share
-  // of the whole; else the first `k` tokens.
-  auto select = [&](bool by_weight, uint32_t k, double share) {
-    const float bins = by_weight ? float(kBinsPerUnit * cool) : float(kBinsPerUnit);
-    // rounded distance in bins; the last bin is for all beyond and not counted
-    auto bin_of = [&](float z) {
-      const float x = (zmax - z) * bins;
-      return x < float(NB - 1) ? __float2uint_rn(x) : uint32_t(NB - 1);
-    };
+  // ---- few candidates: all tokens within `reach` of the largest logit, guessed so
+  // that they are as many as are kept or a few more.  Up to three quarters of
+  // the groups: `want` groups have a token as near as the farthest of
+  // their largest ones.  Above that, from a sample.
+  if (by_k ? uint32_t(top_k) <= CAP * 3 / 4 : by_p) {
+    float reach = -1.f;
+    const uint32_t want = by_k ? uint32_t(top_k) : groups / 4;
+    if (want <= 3 * groups / 4) {
+      if (tid < kGuessBins) s.guess[tid] = 0;
+      __syncthreads();
+      for (uint32_t i = tid; i < groups; i += NT) {
+        const float x = (zmax - s.group[i]) * kGuessPerUnit;
+        if (x < float(kGuessBins) - 1.5f) atomicAdd(&s.guess[__float2uint_rn(x)], 1);
+      }
+      __syncthreads();
+      const uint32_t bin = bin_with(s.guess, want);
+      if (bin < kGuessBins) reach = (bin + 0.5f) / kGuessPerUnit;  // (a distance of at most that has no later bin)
+    } else {
+      for (uint32_t i = tid; i < NB; i += NT) s.hist[i] = 0;
+      __syncthreads();
+      for (uint32_t v = wv0 + lane, it = lane; v < wv1; v += 32, ++it) {
+        if (it % kEvery) continue;
+        float z[EPV];
+        fetch(v, z);
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) count_it(z[i]);
+      }
+      cluster_sync();
+      if (rank == 0) {
+        uint32_t h[4];
+        all_bins(h);
+        // four standard deviations more than wanted
+        const uint32_t some = uint32_t(ceilf(want / float(kEvery) + 4.f * sqrtf(want / float(kEvery))));
+        if (tid == 0) s.low = NB;
+        const uint32_t c = h[0] + h[1] + h[2] + h[3];
+        uint32_t run = cta_scan(c, s.scan_c) - c;
+        for (int i = 0; i < 4; ++i) {
+          run += h[i];
+          if (run >= some) atomicMin(&s.low, tid * 4 + i);
+        }
+        __syncthreads();
+        if (tid < C) push(&s.ctl[0], tid, s.low);
+      }
+      cluster_sync();
+      if (s.ctl[0] < NB) reach = (s.ctl[0] + 0.5f) / kPerUnit;
+    }
+    if (reach >= 0.f) {
+      double w = 0.0, wl = 0.0;
+      uint32_t n = 0;
+      for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+        const uint4 raw = resident ? held[v - v0] : read(v);
+        const bool any = zmax - E::most(raw) <= reach;
+        if (by_k && !any) continue;
+        float z[EPV];
+        E::get(raw, z);
+        if (!by_k) {
+          double e[EPV];
+#pragma unroll
+          for (int i = 0; i < EPV; ++i) e[i] = weight(z[i]);
+#pragma unroll
+          for (int i = 0; i < EPV; ++i) {
+            w += e[i];
+            if (zmax - z[i] <= reach) wl += e[i];
+          }
+        }
+        if (!any) continue;
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) {
+          z[i] += 0.f;
+          if (zmax - z[i] <= reach) {
+            ++n;
+            list_it(z[i], v * EPV + i - skew);
+          }
+        }
+      }
+      share_c(0, n);
+      if (!by_k) share_w(0, w), share_w(1, wl);
+      cluster_sync();
+      n = count_of(s.part_c[turn][0]);
+      bool enough = n <= CAP && (!by_k || n >= want);
+      if (!by_k) {
+        whole = sum_of(s.part_w[turn][0]);
+        nearest = reach, weight_near = sum_of(s.part_w[turn][1]);
+        enough = enough && weight_near >= double(top_p) * whole * (1.0 + 1e-12);
+      }
+      if (enough) {  // all that is kept is among them
+        if (rank == 0) {
+          gather(s.part_c[turn][0]);
+          draw_sorted(by_k ? want : n, whole);
+        } else {
+          cluster_sync();
+        }
+        return;
+      }
+      turn ^= 1;
+      if (tid == 0) s.listed = 0;
+    }
+  }
+
+  // The border of a prefix: by weight, the shortest whose weight reaches top_p
+  // of the whole; else the first top_k tokens.  A histogram says where it lies,
+  // exactly for counts and nearly for weights; the tokens there are the
+  // candidates, and the weight above them is summed.  `passed`: this lane's weights above
+  // the candidates' keys [klo, khi].
+  double passed = 0.0;
+  uint32_t klo = 0, khi = 0, passed_n = 0;
+  auto select = [&](bool by_weight) {
+    const uint32_t k = uint32_t(top_k);
+    // The weight of the tokens nearer than `start` is known to fall short where
+    // the guess above was tried; behind `end` all V tokens weigh less
+    // than the whole leaves.
+    const bool tried = by_weight && !cut && whole >= 0.0 && nearest >= 0.f;
+    start = 0.f, beyond = -1.f, per_unit = kPerUnit;
+    if (tried) {
+      const float end = float(log(V / ((1.0 - double(top_p)) * whole)) * double(heat));
+      start = beyond = nearest;
+      per_unit = fminf(fmaxf((NB - 2) / fmaxf(end - start, 1e-3f), kPerUnit), 4096.f);
+    }
+    const double known = tried ? weight_near : 0.0;
     for (uint32_t i = tid; i < NB; i += NT) s.hist[i] = 0;
-    if (tid == 0) s.listed = 0;
     __syncthreads();
+    const bool weigh = by_weight && (cut || whole < 0.0);
     double w = 0.0;
     for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
       float z[EPV];
       fetch(v, z);
 #pragma unroll
-      for (int i = 0; i < EPV; ++i) {
-        if (!in(key_of(z[i]), v * EPV + i - skew)) continue;
-        const uint32_t b = bin_of(z[i]);
-        if (b < NB - 1) atomicAdd(&s.hist[b], 1);
-        if (by_weight) w += weight(z[i]);
+      for (int i = 0; i < EPV; ++i)
+        if (cut && !in(key_of(z[i]), v * EPV + i - skew)) z[i] = -INFINITY;
+      if (weigh) {
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) w += weight(z[i]);
       }
+#pragma unroll
+      for (int i = 0; i < EPV; ++i) count_it(z[i]);
     }
-    cta_sums(w, 0);
+    if (weigh) share_w(0, w);
     cluster_sync();
-    const double whole = by_weight ? cluster_weight() : 0.0, target = share * whole;
-    if (rank == 0) {
-      // The bins of all CTAs, four a thread.  The border's bin: counts are
-      // exact; a bin's weights lie between those of its edges (and the FP32
-      // distance's slack), so that the border lies between the first bin up to
-      // whose end they may reach the target and the first where they must.
-      constexpr int PER = NB / NT;
-      uint32_t h[PER], c = 0;
-      double wl[PER], wu[PER], tl = 0.0, tu = 0.0;
+    if (weigh) whole = sum_of(s.part_w[turn][0]);
+    turn ^= 1;
+    const double target = double(top_p) * whole;
+    uint32_t inside = 0, ahead = 0, listed = 0;  // candidates, tokens above them, the set of their counts
+    double above = 0.0, astray = 0.0;            // weight of all keys above khi
+    bool hit = false;
+    for (int tries = 0; tries < 3; ++tries) {
+      if (rank == 0) {
+        // bins before which the border cannot lie (counts) or should not (weights:
+        // a bin's are taken as those of its middle), and the last it may
+        uint32_t h[4];
+        all_bins(h);
+        if (tid == 0) s.low = NB, s.found = NB;
+        if (by_weight) {
+          double x[4], t = 0.0;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const uint32_t b = tid * PER + i;
-        h[i] = 0;
-        for (uint32_t r = 0; r < C; ++r) h[i] += remote(&s.hist[b], r);
-        wl[i] = by_weight && h[i] ? h[i] * exp(-(b + 0.5) / kBinsPerUnit) * (1.0 - 1e-4) : 0.0;
-        wu[i] = by_weight && h[i] ? h[i] * exp(-(b - 0.5) / kBinsPerUnit) * (1.0 + 1e-4) : 0.0;
-        c += h[i], tl += wl[i], tu += wu[i];
-      }
-      uint32_t ic = c;
-      double il = tl, iu = tu;
+          for (int i = 0; i < 4; ++i) t += x[i] = h[i] ? h[i] * weight(zmax - start - (tid * 4 + i) / per_unit) : 0.0;
+          double run = known + (cta_scan(t, s.scan_w) - t);
+          // (a value may lie half a bin off its middle, and they mostly even out)
+          const double slack = (2e-5 + 0.2 * cool / per_unit) * target, goal = target + astray;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t oc = __shfl_up_sync(0xffffffffu, ic, d);
-        const double ol = __shfl_up_sync(0xffffffffu, il, d), ou = __shfl_up_sync(0xffffffffu, iu, d);
-        if (lane >= d) ic += oc, il += ol, iu += ou;
-      }
-      if (tid == 0) s.low = s.high = NB - 1, s.ahead = s.inside = 0;
-      if (lane == 31) s.scan_c[warp] = ic, s.scan_l[warp] = il, s.scan_u[warp] = iu;
-      __syncthreads();
-      ic -= c, il -= tl, iu -= tu;
-      for (uint32_t x = 0; x < warp; ++x) ic += s.scan_c[x], il += s.scan_l[x], iu += s.scan_u[x];
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const uint32_t b = tid * PER + i;
-        ic += h[i], il += wl[i], iu += wu[i];
-        if (b < NB - 1 && (by_weight ? iu >= target : ic >= k)) atomicMin(&s.low, b);
-        if (b < NB - 1 && (by_weight ? il >= target : ic >= k)) atomicMin(&s.high, b);
-      }
-      __syncthreads();
-      const uint32_t lo = s.low, hi = s.high;
-      uint32_t before = 0, within = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const uint32_t b = tid * PER + i;
-        before += b < lo ? h[i] : 0;
-        within += b >= lo && b <= hi ? h[i] : 0;
-      }
-      before = __reduce_add_sync(0xffffffffu, before);
-      within = __reduce_add_sync(0xffffffffu, within);
-      if (lane == 0) atomicAdd(&s.ahead, before), atomicAdd(&s.inside, within);
-      __syncthreads();
-      if (warp == 0) {
-        // the bins' keys.  Bins fall as keys rise: the largest key whose bin is
-        // at least b, five bits of it a step
-        auto last_of = [&](uint32_t b) {
-          uint32_t at = 0;
-          for (int sh = 27; sh >= -3; sh -= 5) {
-            const uint32_t c = at + (sh >= 0 ? lane << sh : lane >> -sh);
-            const bool ok = c <= key_of(-INFINITY) || (c <= key_of(zmax) && bin_of(value_of(c)) >= b);
-            at = __shfl_sync(0xffffffffu, c, 31 - __clz(__ballot_sync(0xffffffffu, ok)));
+          for (int i = 0; i < 4; ++i) {
+            run += x[i];
+            if (run >= goal - slack) atomicMin(&s.low, tid * 4 + i);
+            if (run >= goal + slack) atomicMin(&s.found, tid * 4 + i);
           }
-          return at;
-        };
-        const uint32_t top = lo == 0 ? key_of(zmax) : last_of(lo);
-        const uint32_t end = hi >= NB - 1 ? key_of(-INFINITY) : last_of(hi + 1);
-        if (lane == 0) {
-          // (the last bin's tokens have not been counted)
-          s.ctl = Ctl{end + 1, top, hi >= NB - 1 ? ~0u : s.inside, s.ahead};
-        }
-      }
-    }
-    cluster_sync();
-    uint32_t klo = remote(&s.ctl.klo, 0), khi = remote(&s.ctl.khi, 0);
-    uint32_t inside = remote(&s.ctl.inside, 0), ahead = remote(&s.ctl.ahead, 0);
-    uint32_t prev = ~0u;  // keys above it are in `above`
-    double above = 0.0;
-    // The candidates, keys [klo, khi]: few enough are sorted; else a quarter of
-    // the keys' range is kept a round (at most 16), down to a single key, of
-    // which the first by index are counted off.
-    for (;;) {
-      const bool listing = inside <= CAP, single = !listing && klo == khi;
-      const int shift = max(0, 32 - __clz(khi - klo) - 2);
-      if (tid == 0) s.listed = 0;
-      __syncthreads();
-      double w = 0.0, wq[4] = {};
-      uint32_t cq[4] = {};
-      for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
-        float z[EPV];
-        fetch(v, z);
+          __syncthreads();
+          run -= x[0] + x[1] + x[2] + x[3];
 #pragma unroll
-        for (int i = 0; i < EPV; ++i) {
-          const uint32_t kz = key_of(z[i]), at = v * EPV + i - skew;
-          if (kz < klo || !in(kz, at)) continue;
-          if (kz > khi) {
-            if (by_weight && kz <= prev) w += weight(z[i]);
-          } else if (listing) {
-            const uint32_t n = atomicAdd(&s.listed, 1);
-            if (n < CAP) s.list[n] = uint64_t(~kz) << 32 | at;
-          } else {
-            const uint32_t q = (khi - kz) >> shift;
-            const double x = by_weight && !single ? weight(z[i]) : 0.0;
+          for (int i = 0; i < 4; ++i) {
+            if (s.low == tid * 4 + i) s.guessed = run;
+            run += x[i];
+          }
+        } else {
+          const uint32_t c = h[0] + h[1] + h[2] + h[3];
+          uint32_t run = cta_scan(c, s.scan_c) - c;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
-              if (q == j) ++cq[j], wq[j] += x;
+          for (int i = 0; i < 4; ++i) {
+            run += h[i];
+            if (run >= k) atomicMin(&s.low, tid * 4 + i);
+            if (run >= k) atomicMin(&s.found, tid * 4 + i);
           }
         }
-      }
-      if (!listing && !single) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          wq[j] = warp_sum(wq[j]);
-          cq[j] = __reduce_add_sync(0xffffffffu, cq[j]);
-          if (lane == 0) s.part_w[j][warp] = wq[j], s.part_c[j][warp] = cq[j];
-        }
-      }
-      cta_sums(w, cq[0]);
-      if (!listing && !single && tid < 4) {
-        double t = 0.0;
-        uint32_t n = 0;
-        for (int i = 0; i < NW; ++i) t += s.part_w[tid][i], n += s.part_c[tid][i];
-        s.part_w[tid][NW] = t, s.part_c[tid][NW] = n;
+        __syncthreads();
+        if (tid < C) push(&s.ctl[0], tid, s.low), push(&s.ctl[1], tid, s.found);
       }
       cluster_sync();
-      if (by_weight) above += cluster_weight();
-      prev = khi;
+      // The candidates' distances; with no border among the bins, all there are
+      const bool some = s.ctl[0] < NB;
+      const float near = some ? start + (s.ctl[0] - 0.5f) / per_unit : -1.f;
+      const float far = s.ctl[1] < NB ? start + (s.ctl[1] + 0.5f) / per_unit : INFINITY;
+      uint32_t n = 0, lo = ~0u, hi = 0, over = 0;
+      double wl = 0.0;
+      w = 0.0;
+      if (some)
+        for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+          const uint4 raw = resident ? held[v - v0] : read(v);
+          if (zmax - E::most(raw) > far) continue;
+          float z[EPV];
+          E::get(raw, z);
+          bool any = false;
+          double e[EPV];
+#pragma unroll
+          for (int i = 0; i < EPV; ++i) {
+            z[i] += 0.f;
+            if (cut && !in(key_of(z[i]), v * EPV + i - skew)) z[i] = -INFINITY;
+            const float d = zmax - z[i];
+            any |= d >= near && d <= far;
+            over += d < near;
+            if (by_weight) e[i] = d < near ? weight(z[i]) : 0.0;
+          }
+          if (by_weight) {
+#pragma unroll
+            for (int i = 0; i < EPV; ++i) w += e[i];
+          }
+          if (!any) continue;
+#pragma unroll
+          for (int i = 0; i < EPV; ++i)
+            if (zmax - z[i] >= near && zmax - z[i] <= far && z[i] > -INFINITY) {
+              const uint32_t kz = key_of(z[i]);
+              ++n, lo = min(lo, kz), hi = max(hi, kz);
+              if (by_weight) wl += weight(z[i]);
+              list_it(z[i], v * EPV + i - skew);
+            }
+        }
+      share_c(0, n);
+      share_c(1, over);
+      lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+      if (lane < C) push(&s.part_lo[turn][me], lane, lo), push(&s.part_hi[turn][me], lane, hi);
+      if (by_weight) share_w(0, w), share_w(1, wl);
+      cluster_sync();
+      inside = count_of(s.part_c[turn][0]), ahead = count_of(s.part_c[turn][1]);
+      klo = ~0u, khi = 0;
+      for (uint32_t i = lane; i < parts; i += 32) klo = min(klo, s.part_lo[turn][i]), khi = max(khi, s.part_hi[turn][i]);
+      klo = __reduce_min_sync(0xffffffffu, klo), khi = __reduce_max_sync(0xffffffffu, khi);
+      above = by_weight ? sum_of(s.part_w[turn][0]) : 0.0;  // weight of all keys above khi
+      hit = inside && (by_weight ? above < target && above + sum_of(s.part_w[turn][1]) >= target : ahead < k && ahead + inside >= k);
+      listed = turn;
+      turn ^= 1;
+      if (hit) {
+        passed += w, passed_n += over;
+        break;
+      }
+      // the weight above the candidates is known now, and so how far the bins'
+      // sums are out there
+      if (!some || !by_weight) break;
+      astray = s.guessed - above;  // (of the first CTA)
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+    }
+    bool listing = hit && inside <= CAP;
+    if (!hit) {  // the border lies elsewhere: in the whole range
+      klo = key_of(-INFINITY) + 1, khi = key_of(zmax), inside = ~0u, ahead = 0, above = 0.0;
+      passed = 0.0, passed_n = 0;
+    }
+    // Few enough candidates are sorted; else a quarter of the keys' range is
+    // kept a round (at most 16), down to a single key, of which the first by
+    // index are counted off.
+    for (;;) {
       uint32_t key = klo;
       int32_t index = INT32_MAX;
       bool found = true;
       if (listing) {
         if (rank == 0) {
-          // the candidates of all CTAs, in order
-          uint32_t n = 0;
-          for (uint32_t r = 0; r < C; ++r) {
-            const uint32_t m = min(remote(&s.listed, r), CAP - n);
-            for (uint32_t i = tid; i < m; i += NT) s.all[n + i] = remote(&s.list[i], r);
-            n += m;
-          }
-          __syncthreads();
-          for (uint32_t i = tid; i < n; i += NT) {
-            const uint64_t me = s.all[i];
-            uint32_t below = 0;
-            for (uint32_t j = 0; j < n; ++j) below += s.all[j] < me;
-            s.sorted[below] = me;
-          }
-          if (tid == 0) s.low = by_weight ? 0 : k - ahead;
-          __syncthreads();
-          if (by_weight) {  // kept while the weight before is short of the target
-            constexpr int PER = CAP / NT;
-            double x[PER], t = 0.0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              const uint32_t j = tid * PER + i;
-              x[i] = j < n ? weight(value_of(~uint32_t(s.sorted[j] >> 32))) : 0.0;
-              t += x[i];
-            }
-            double inc = t;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-              const double o = __shfl_up_sync(0xffffffffu, inc, d);
-              if (lane >= d) inc += o;
-            }
-            if (lane == 31) s.scan_l[warp] = inc;
-            __syncthreads();
-            double before = above + (inc - t);
-            for (uint32_t y = 0; y < warp; ++y) before += s.scan_l[y];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              if (tid * PER + i < n && before < target) atomicMax(&s.low, tid * PER + i + 1);
-              before += x[i];
-            }
-            __syncthreads();
-          }
-          if (tid == 0) {
+          gather(s.part_c[listed][0]);
+          const uint32_t keep = by_weight ? kept_of(inside, above, target) : min(k - ahead, inside);
+          if (tid < C) {
             // (no candidate, by rounding: all that lies above)
-            const uint32_t keep = min(s.low, n);
-            const uint64_t end = keep ? s.sorted[keep - 1] : 0;
-            s.ctl = Ctl{keep ? ~uint32_t(end >> 32) : khi, keep ? uint32_t(end) : ~0u, 0, 0};
+            const uint64_t end = keep ? s.all[keep - 1] : 0;
+            push(&s.ctl[0], tid, keep ? ~uint32_t(end >> 32) : khi);
+            push(&s.ctl[1], tid, keep ? uint32_t(end) : ~0u);
           }
+        } else {
+          cluster_sync();
         }
         cluster_sync();
-        key = remote(&s.ctl.klo, 0);
-        index = int32_t(remote(&s.ctl.khi, 0));
-      } else if (single) {
-        // the first `m` by index of the tokens of one key
-        uint32_t m = k - ahead, before = 0, owner = 0, n;
-        if (by_weight) {
-          const double need = ceil((target - above) / weight(value_of(khi)));
-          m = need < 1.0 ? 1u : need > 4e9 ? ~0u : uint32_t(need);
-        }
-        while (owner < C && m > before + (n = remote(&s.count[NW], owner))) before += n, ++owner;
-        if (rank == owner) {
-          uint32_t left = m - before, x = 0;
-          while (left > s.count[x]) left -= s.count[x++];
-          if (warp == x) {
-            for (uint32_t v = wv0 + lane; v - lane < wv1; v += 32) {
-              float z[EPV];
-              uint32_t mine = 0;
-              if (v < wv1) {
-                fetch(v, z);
+        key = s.ctl[0];
+        index = int32_t(s.ctl[1]);
+      } else {
+        const bool single = klo == khi;
+        const int shift = max(0, 32 - __clz(khi - klo) - 2);
+        double wq[4] = {};
+        uint32_t cq[4] = {};
+        listing = inside <= CAP;
+        if (tid == 0) s.listed = 0;
+        __syncthreads();
+        for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+          float z[EPV];
+          fetch(v, z);
 #pragma unroll
-                for (int i = 0; i < EPV; ++i)
-                  mine |= uint32_t(key_of(z[i]) == khi && in(khi, v * EPV + i - skew)) << i;
-              }
-              uint32_t inc = __popc(mine);
+          for (int i = 0; i < EPV; ++i) {
+            const uint32_t kz = key_of(z[i]), at = v * EPV + i - skew;
+            if (kz < klo || kz > khi || (cut && !in(kz, at))) continue;
+            if (listing) {
+              list_it(z[i], at), ++cq[0];
+            } else {
+              const uint32_t q = (khi - kz) >> shift;
+              const double x = by_weight && !single ? weight(z[i]) : 0.0;
 #pragma unroll
-              for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t o = __shfl_up_sync(0xffffffffu, inc, d);
-                if (lane >= d) inc += o;
-              }
-              const uint32_t ex = inc - __popc(mine);
-              if (left > ex && left <= inc) s.found = v * EPV + __fns(mine, 0, int(left - ex)) - skew;
-              const uint32_t got = __shfl_sync(0xffffffffu, inc, 31);
-              if (left <= got) break;
-              left -= got;
+              for (uint32_t j = 0; j < 4; ++j)
+                if (q == j) ++cq[j], wq[j] += x;
             }
           }
         }
-        cluster_sync();
-        if (owner < C) index = int32_t(remote(&s.found, owner));
-      } else {
-        double run = above;
-        uint32_t count = ahead;
-        found = true;  // the quarters together fall short: all of them
-        for (uint32_t j = 0; j < 4; ++j) {
-          uint32_t n = 0;
-          double t = 0.0;
-          for (uint32_t r = 0; r < C; ++r) n += remote(&s.part_c[j][NW], r), t += remote(&s.part_w[j][NW], r);
-          if (n && (by_weight ? run + t >= target : count + n >= k)) {
-            const uint32_t top = khi - (j << shift), step = 1u << shift;
-            klo = top - klo >= step ? top - step + 1 : klo;
-            khi = prev = top;
-            inside = n, ahead = count, above = run;
-            found = false;
-            break;
+        if (listing || single) {
+          share_c(0, cq[0]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const double x = warp_sum(wq[j]);
+            const uint32_t c = __reduce_add_sync(0xffffffffu, cq[j]);
+            if (lane < C) push(&s.quarter_w[turn][j][me], lane, x), push(&s.quarter_c[turn][j][me], lane, c);
           }
-          run += t, count += n;
+        }
+        cluster_sync();
+        const uint32_t now = turn;
+        turn ^= 1;
+        if (listing) {
+          listed = now;
+          continue;
+        }
+        if (single) {
+          // the first `m` by index of the tokens of one key
+          uint32_t m = k - ahead;
+          if (by_weight) {
+            const double need = ceil((target - above) / weight(value_of(khi)));
+            m = need < 1.0 ? 1u : need > 4e9 ? ~0u : uint32_t(need);
+          }
+          // every warp finds the row's warp that holds the m-th
+          constexpr int PER = kParts / 32;
+          uint32_t c[PER], t = 0, owner = ~0u, before = 0;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) t += c[i] = lane * PER + i < parts ? s.part_c[now][0][lane * PER + i] : 0;
+          uint32_t run = warp_scan(t, lane) - t;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            if (m > run && m - run <= c[i]) owner = lane * PER + i, before = run;
+            run += c[i];
+          }
+          const uint32_t who = __ballot_sync(0xffffffffu, owner != ~0u);
+          if (who) {
+            owner = __shfl_sync(0xffffffffu, owner, __ffs(who) - 1);
+            before = __shfl_sync(0xffffffffu, before, __ffs(who) - 1);
+            if (me == owner) {
+              uint32_t left = m - before;
+              for (uint32_t v = wv0 + lane; v - lane < wv1; v += 32) {
+                float z[EPV];
+                uint32_t mask = 0;
+                if (v < wv1) {
+                  fetch(v, z);
+#pragma unroll
+                  for (int i = 0; i < EPV; ++i)
+                    mask |= uint32_t(key_of(z[i]) == khi && in(khi, v * EPV + i - skew)) << i;
+                }
+                const uint32_t inc = warp_scan(uint32_t(__popc(mask)), lane), ex = inc - __popc(mask);
+                if (left > ex && left <= inc) {
+                  const uint32_t at = v * EPV + __fns(mask, 0, int(left - ex)) - skew;
+                  for (uint32_t r = 0; r < C; ++r) push(&s.found, r, at);
+                }
+                const uint32_t got = __shfl_sync(0xffffffffu, inc, 31);
+                if (left <= got) break;
+                left -= got;
+              }
+            }
+          }
+          cluster_sync();
+          if (who) index = int32_t(s.found);
+        } else {
+          double run = above;
+          uint32_t count = ahead;
+          // (should the quarters together fall short: all of them)
+          for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t c = count_of(s.quarter_c[now][j]);
+            const double t = sum_of(s.quarter_w[now][j]);
+            if (c && (by_weight ? run + t >= target : count + c >= k)) {
+              const uint32_t top = khi - (j << shift), step = 1u << shift;
+              klo = top - klo >= step ? top - step + 1 : klo;
+              khi = top;
+              inside = c, ahead = count, above = run;
+              found = false;
+              break;
+            }
+            run += t, count += c;
+            passed += j == 0 ? wq[0] : j == 1 ? wq[1] : j == 2 ? wq[2] : wq[3];
+            passed_n += j == 0 ? cq[0] : j == 1 ? cq[1] : j == 2 ? cq[2] : cq[3];
+          }
         }
       }
-      // the next round's writes wait for these reads
-      cluster_sync();
       if (found) {
         // (a border that keeps all of a key leaves an earlier one as it is)
         if (key > bkey || (key == bkey && index < bidx)) bkey = key, bidx = index;
+        cut = true;
+        if (tid == 0) s.listed = 0;
         return;
       }
     }
   };
-  if (top_k > 0 && uint32_t(top_k) < V) select(false, uint32_t(top_k), 0.0);
-  if (top_p < 1.f) select(true, 0, double(top_p));
+  if (by_k) select(false);
+  if (by_p) {
+    passed = 0.0, passed_n = 0;
+    select(true);
+  }
 
-  // ---- the kept tokens' weights, and the draw by index ----
+  // ---- the kept tokens' weights, and the draw by index.  Where top-p was the
+  // last cut and min-p leaves all of them, the weights above its candidates
+  // have been summed already.
   const float border = value_of(bkey);
   auto kept = [&](float z, uint32_t i) { return z >= floor_z && (z > border || (z == border && int32_t(i) <= bidx)); };
-  double w = 0.0;
-  uint32_t n = 0;
+  const bool summed = by_p && floor_z <= value_of(klo);
+  const float upto = summed ? value_of(khi) : INFINITY, from = fmaxf(floor_z, border);
+  double w = summed ? passed : 0.0;
+  uint32_t n = summed ? passed_n : 0;
   for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+    const uint4 raw = resident ? held[v - v0] : read(v);
+    if (E::most(raw) < from) continue;
     float z[EPV];
-    fetch(v, z);
+    E::get(raw, z);
 #pragma unroll
-    for (int i = 0; i < EPV; ++i)
-      if (kept(z[i], v * EPV + i - skew)) w += weight(z[i]), ++n;
-  }
-  cta_sums(w, n);
-  cluster_sync();
-  double total = 0.0, before = 0.0;
-  uint32_t many = 0, last = 0;
-  for (uint32_t r = 0; r < C; ++r) {
-    const uint32_t c = remote(&s.count[NW], r);
-    many += c;
-    if (c) last = r;
-    total += remote(&s.sum[NW], r);
-  }
-  const double target = fmax(double(u), 0.0) * total;
-  // the CTA whose weights pass the target; else the last one that keeps any
-  uint32_t owner = last;
-  double run = 0.0;
-  for (uint32_t r = 0; r < C; ++r) {
-    const double next = run + remote(&s.sum[NW], r);
-    if (next > target) {
-      owner = r;
-      break;
+    for (int i = 0; i < EPV; ++i) {
+      z[i] += 0.f;
+      if (z[i] <= upto && kept(z[i], v * EPV + i - skew)) w += weight(z[i]), ++n;
     }
-    if (r < last) run = next;
   }
-  before = run;
-  if (rank == owner) {
-    uint32_t x = 0, last_warp = 0;
-    for (int i = 0; i < NW; ++i)
-      if (s.count[i]) last_warp = i;
-    while (x < last_warp && !(before + s.sum[x] > target)) before += s.sum[x++];
-    if (warp == x) {
-      int32_t token = -1;
-      float z_token = 0.f;
-      for (uint32_t v = wv0 + lane; v - lane < wv1 ; v += 32) {
-        float z[EPV];
-        double e[EPV], t = 0.0;
-        if (v < wv1) fetch(v, z);
+  share_w(0, w);
+  share_c(0, n);
+  cluster_sync();
+  const uint32_t many = count_of(s.part_c[turn][0]);
+  // every warp finds the row's warp whose weights pass the target; else the
+  // last one that keeps any
+  constexpr int PER = kParts / 32;
+  double x[PER], t = 0.0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) t += x[i] = lane * PER + i < parts ? s.part_w[turn][0][lane * PER + i] : 0.0;
+  const double inc = warp_scan(t, lane), total = __shfl_sync(0xffffffffu, inc, 31);
+  const double target = fmax(double(u), 0.0) * total;
+  uint32_t owner = ~0u, last = 0;
+  double run = inc - t, before = 0.0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (x[i] > 0.0) {
+      last = lane * PER + i + 1;
+      if (owner == ~0u && run + x[i] > target) owner = last - 1, before = run;
+    }
+    run += x[i];
+  }
+  const uint32_t who = __ballot_sync(0xffffffffu, owner != ~0u);
+  last = __reduce_max_sync(0xffffffffu, last) - 1;
+  if (who) {
+    owner = __shfl_sync(0xffffffffu, owner, __ffs(who) - 1);
+    before = __shfl_sync(0xffffffffu, before, __ffs(who) - 1);
+  } else {
+    owner = last;
+    before = -INFINITY;  // (no token of it passes: its last one)
+  }
+  if (me != owner) return;
+  int32_t token = -1;
+  float z_token = 0.f;
+  for (uint32_t v = wv0 + lane; v - lane < wv1; v += 32) {
+    float z[EPV];
+    double e[EPV], t = 0.0;
+    if (v < wv1) fetch(v, z);
+#pragma unroll
+    for (int i = 0; i < EPV; ++i) {
+      e[i] = v < wv1 && kept(z[i], v * EPV + i - skew) ? weight(z[i]) : 0.0;
+      t += e[i];
+    }
+    const double inc = warp_scan(t, lane);
+    // the first lane that passes the target, else the last that keeps any
+    const uint32_t some = __ballot_sync(0xffffffffu, t > 0.0);
+    const uint32_t past = __ballot_sync(0xffffffffu, t > 0.0 && before + inc > target);
+    if (some) {
+      const int who = past ? __ffs(past) - 1 : 31 - __clz(some);
+      int32_t got = -1;
+      float zg = 0.f;
+      if (lane == who) {
+        double c = before + (inc - t);
+        bool done = false;
 #pragma unroll
         for (int i = 0; i < EPV; ++i) {
-          e[i] = v < wv1 && kept(z[i], v * EPV + i - skew) ? weight(z[i]) : 0.0;
-          t += e[i];
+          c += e[i];
+          if (e[i] > 0.0 && !done) got = int32_t(v * EPV + i - skew), zg = z[i], done = c > target;
         }
-        double inc = t;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const double o = __shfl_up_sync(0xffffffffu, inc, d);
-          if (lane >= d) inc += o;
-        }
-        // the first lane that passes the target, else the last that keeps any
-        const uint32_t some = __ballot_sync(0xffffffffu, t > 0.0);
-        const uint32_t past = __ballot_sync(0xffffffffu, t > 0.0 && before + inc > target);
-        if (some) {
-          const int who = past ? __ffs(past) - 1 : 31 - __clz(some);
-          int32_t got = -1;
-          float zg = 0.f;
-          if (lane == who) {
-            double c = before + (inc - t);
-            bool done = false;
-#pragma unroll
-            for (int i = 0; i < EPV; ++i) {
-              c += e[i];
-              if (e[i] > 0.0 && !done) got = int32_t(v * EPV + i - skew), zg = z[i], done = c > target;
-            }
-          }
-          token = __shfl_sync(0xffffffffu, got, who);
-          z_token = __shfl_sync(0xffffffffu, zg, who);
-        }
-        if (past) break;
-        before += __shfl_sync(0xffffffffu, inc, 31);
       }
-      if (lane == 0) answer(token, int32_t(many), float((double(z_token) - zm) * cool - log(total)));
+      token = __shfl_sync(0xffffffffu, got, who);
+      z_token = __shfl_sync(0xffffffffu, zg, who);
     }
+    if (past) break;
+    before += __shfl_sync(0xffffffffu, inc, 31);
   }
-  cluster_sync();
+  if (lane == 0) answer(token, int32_t(many), float((double(z_token) - zm) * cool - log(total)));
 }
 
 template <class T>
@@ -643,12 +1035,14 @@ cudaError_t launch(const SampleArgs& given, int sms, cudaStream_t st) {
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = c;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
 }
 
