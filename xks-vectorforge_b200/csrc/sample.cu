@@ -20,6 +20,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 #include "sample.h"
@@ -42,7 +43,7 @@ constexpr int CAP = 2048;                 // candidates that are sorted
 constexpr double kTiny = -700.0;          // weights below exp(kTiny) count as zero
 
 struct Shared {
-  uint32_t hist[NB];
+  alignas(16) uint32_t hist[NB];
   float group[kGroups];
   uint32_t guess[kGuessBins];
   uint64_t list[CAP];  // this CTA's candidates: ~key, index
@@ -57,6 +58,7 @@ struct Shared {
   float best[kParts];
   double pow[16];  // 2^(i / 16)
   double guessed;
+  float spread;
   uint32_t listed, low, first, found;
   uint32_t ctl[2];
 };
@@ -76,6 +78,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+
+// A float as a double, put together from its bits: the converter's rate (a
+// quarter of FP64's) would bound every pass of weights.  Zero and subnormal numbers become
+// numbers of 2^-127, infinity 2^128.
+__device__ __forceinline__ double widened(float z) {
+  const uint32_t b = __float_as_uint(z);
+  return __hiloint2double(int((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), int(b << 29));
+}
+// A float of [0, 2^22) rounded to an integer, by the adder for the same reason.
+__device__ __forceinline__ uint32_t rounded(float x) { return __float_as_uint(x + 12582912.f) - 0x4b400000u; }
 
 template <class T>
 struct Elems;  // of a 16-byte vector
@@ -182,7 +194,8 @@ __device__ __forceinline__ X warp_scan(X x, uint32_t lane) {
   }
   return x;
 }
-template <class T>
+// HELD: the row lies in the cluster's shared memory (else every pass reads HBM or L2).
+template <class T, bool HELD>
 __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   using E = Elems<T>;
   constexpr int EPV = E::N;
@@ -226,9 +239,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     }
     return w;
   };
-  const bool resident = p.resident;
   auto fetch = [&](uint32_t v, float* z) {
-    E::get(resident ? held[v - v0] : read(v), z);
+    E::get(HELD ? held[v - v0] : read(v), z);
 #pragma unroll
     for (int i = 0; i < EPV; ++i) z[i] += 0.f;  // -0 becomes +0
   };
@@ -238,7 +250,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
 #pragma unroll 4
   for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
     const uint4 w = read(v);
-    if (resident) held[v - v0] = w;
+    if (HELD) held[v - v0] = w;
     mine = max_nan(mine, E::most(w));
   }
   // groups: a lane, or two or four; every CTA gets all of them
@@ -285,28 +297,25 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     if (rank == 0 && tid == 0) answer(s.first, 1, 0.f);
     return;
   }
-  // exp((z - zmax) / heat) = 2^(n / 16) exp(r), with n whole, |r| <= log(2) / 32
-  // and the series of exp(r) to the 6th power (the 7th: 5e-16)
-  const double zm = zmax, cool = 1.0 / double(heat);
+  // exp((z - zmax) / heat) = 2^((n + f) / 16) with n whole and |f| <= 1/2; the
+  // series of exp(r), r = f log(2) / 16, to the 6th power (the 7th: 5e-16), in
+  // short chains: a pass of weights is bound by their latency.  No branch: a
+  // token that does not count enters with -infinity.
+  const double zm = widened(zmax), cool = 1.0 / double(heat);
+  constexpr double kLn2 = 0.69314718055994530942, kBig = 6755399441055744.0;  // 1.5 * 2^52
+  const double cool16 = 16.0 / kLn2 * cool;
   auto weight = [&](float z) {
-    constexpr double kLn2By16 = 0.69314718055994530942 / 16, kBig = 6755399441055744.0;  // 1.5 * 2^52
-    const double x = (double(z) - zm) * cool;
-    const double big = fma(x, 1.0 / kLn2By16, kBig);
+    const double y = (widened(z) - zm) * cool16;
+    const double big = y + kBig;
     const int n = __double2loint(big);
-    const double r = fma(big - kBig, -kLn2By16, x);
-    double e = fma(r, 1.0 / 720, 1.0 / 120);
-    e = fma(e, r, 1.0 / 24);
-    e = fma(e, r, 1.0 / 6);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    e *= s.pow[n & 15];
-    e = __hiloint2double(__double2hiint(e) + (n >> 4 << 20), __double2loint(e));
-    return x < kTiny ? 0.0 : e;
+    const double r = (y - (big - kBig)) * (kLn2 / 16), r2 = r * r;
+    const double a = fma(r, 1.0 / 6, 0.5), b = fma(r, 1.0 / 120, 1.0 / 24);
+    const double e = s.pow[n & 15] * fma(r2, fma(r2, fma(r2, 1.0 / 720, b), a), 1.0 + r);
+    return y < kTiny * 16.0 / kLn2 ? 0.0 : __hiloint2double(__double2hiint(e) + (n >> 4 << 20), __double2loint(e));
   };
   // the least logit that min-p and the smallest weight leave
   const double lowest_x = min_p > 0.f ? fmax(kTiny, log(fmin(1.0, double(min_p)))) : kTiny;
-  const float floor_z = __double2float_ru(zm + lowest_x * double(heat));
+  const float floor_z = __double2float_ru(double(zmax) + lowest_x * double(heat));
 
   const bool by_k = top_k > 0 && uint32_t(top_k) < V, by_p = top_p < 1.f;
 
@@ -337,42 +346,73 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     const uint32_t n = atomicAdd(&s.listed, 1);
     if (n < CAP) s.list[n] = uint64_t(~key_of(z)) << 32 | at;
   };
-  // The first CTA: s.all[0, n) in rising order (bitonic, `full` a power of two).
-  auto sort_all = [&](uint32_t n) {
-    uint32_t full = 32;
+  // The first CTA: s.all[0, n) in rising order (bitonic), E entries a thread in
+  // registers: exchanges within a thread, then a warp, the farthest through
+  // shared memory, two boxes in turn (the histogram's halves; of four entries
+  // s.list too, which has been read by then).
+  auto sort_by = [&](uint32_t n, auto entries) {
+    constexpr uint32_t E = decltype(entries)::value;
+    uint32_t full = 32 * E;
     while (full < n) full *= 2;
-    if (full <= NT) {  // an entry a thread; the nearer exchanges within a warp
-      uint64_t x = tid < n ? s.all[tid] : ~0ull;
-      uint64_t* box = s.list;  // (the gathered list has been read)
-      __syncthreads();
-      for (uint32_t size = 2; size <= full; size *= 2)
-        for (uint32_t far = size / 2; far; far /= 2) {
-          uint64_t y;
-          if (far >= 32) {
-            box[tid] = x;
-            __syncthreads();
-            y = box[tid ^ far];
-            box = box == s.list ? s.list + NT : s.list;
-          } else {
-            y = __shfl_xor_sync(0xffffffffu, x, far);
-          }
-          if ((x > y) == (!(tid & far) == !(tid & size))) x = y;
-        }
-      s.all[tid] = x;
-      __syncthreads();
-      return;
-    }
-    for (uint32_t i = n + tid; i < full; i += NT) s.all[i] = ~0ull;
+    uint64_t x[E];
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) x[e] = tid * E + e < n ? s.all[tid * E + e] : ~0ull;
     __syncthreads();
+    bool flip = false;
     for (uint32_t size = 2; size <= full; size *= 2)
       for (uint32_t far = size / 2; far; far /= 2) {
-        for (uint32_t i = tid; i < full / 2; i += NT) {
-          const uint32_t a = 2 * i - (i & (far - 1)), b = a + far;
-          const uint64_t x = s.all[a], y = s.all[b];
-          if ((x > y) == !(a & size)) s.all[a] = y, s.all[b] = x;
+        const bool up = !(tid * E & size);  // (of sizes up to E: by the entry)
+        if (far < E) {
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e) {
+            const uint32_t o = e ^ far;
+            if (o > e && o < E) {
+              const bool rise = size < E ? !(e & size) : up;
+              uint64_t hi = 0;
+#pragma unroll
+              for (uint32_t j = 0; j < E; ++j)
+                if (j == o) hi = x[j];
+              if ((x[e] > hi) == rise) {
+#pragma unroll
+                for (uint32_t j = 0; j < E; ++j)
+                  if (j == o) x[j] = x[e];
+                x[e] = hi;
+              }
+            }
+          }
+        } else if (far < 32 * E) {
+          const bool least = !(tid * E & far) == up;
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e) {
+            const uint64_t y = __shfl_xor_sync(0xffffffffu, x[e], far / E);
+            if ((x[e] > y) == least) x[e] = y;
+          }
+        } else {
+          uint64_t* const halves = reinterpret_cast<uint64_t*>(s.hist);
+          uint64_t* box = E == 1 ? halves + flip * NT : flip ? s.all : s.list;
+          flip = !flip;
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e) box[e * NT + tid] = x[e];
+          __syncthreads();
+          const bool least = !(tid * E & far) == up;
+#pragma unroll
+          for (uint32_t e = 0; e < E; ++e) {
+            const uint64_t y = box[e * NT + (tid ^ far / E)];
+            if ((x[e] > y) == least) x[e] = y;
+          }
         }
-        __syncthreads();
       }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t e = 0; e < E; ++e) s.all[tid * E + e] = x[e];
+    __syncthreads();
+  };
+  auto sort_all = [&](uint32_t n) {
+    static_assert(CAP == 4 * NT, "up to four entries a thread");
+    if (n <= NT)
+      sort_by(n, std::integral_constant<uint32_t, 1>());
+    else
+      sort_by(n, std::integral_constant<uint32_t, 4>());
   };
   // The first CTA gathers the candidates of all (their numbers are the
   // parts' counts `c`) and sorts them.
@@ -467,7 +507,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     __syncthreads();
     if (tid == 0) {
       const uint32_t i = min(s.low, n - 1);
-      answer(int64_t(s.all[i] >> 32), int32_t(n), float((double(z_of(i)) - zm) * cool - log(all)));
+      answer(int64_t(s.all[i] >> 32), int32_t(n), float((widened(z_of(i)) - zm) * cool - log(all)));
     }
   };
 
@@ -520,7 +560,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   float start = 0.f, beyond = -1.f, per_unit = kPerUnit;
   auto count_it = [&](float z) {
     const float d = zmax - z, x = (d - start) * per_unit;
-    if (d > beyond && x < float(NB) - 1.5f) atomicAdd(&s.hist[__float2uint_rn(x)], 1);
+    if (d > beyond && x < float(NB) - 1.5f) atomicAdd(&s.hist[rounded(x)], 1);
   };
 
   // ---- few candidates: all tokens within `reach` of the largest logit, guessed so
@@ -535,7 +575,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       __syncthreads();
       for (uint32_t i = tid; i < groups; i += NT) {
         const float x = (zmax - s.group[i]) * kGuessPerUnit;
-        if (x < float(kGuessBins) - 1.5f) atomicAdd(&s.guess[__float2uint_rn(x)], 1);
+        if (x < float(kGuessBins) - 1.5f) atomicAdd(&s.guess[rounded(x)], 1);
       }
       __syncthreads();
       const uint32_t bin = bin_with(s.guess, want);
@@ -573,7 +613,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       double w = 0.0, wl = 0.0;
       uint32_t n = 0;
       for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
-        const uint4 raw = resident ? held[v - v0] : read(v);
+        const uint4 raw = HELD ? held[v - v0] : read(v);
         const bool any = zmax - E::most(raw) <= reach;
         if (by_k && !any) continue;
         float z[EPV];
@@ -629,6 +669,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   // the candidates' keys [klo, khi].
   double passed = 0.0;
   uint32_t klo = 0, khi = 0, passed_n = 0;
+  bool whole_list = false;  // this CTA's list still holds its candidates
   auto select = [&](bool by_weight) {
     const uint32_t k = uint32_t(top_k);
     // The weight of the tokens nearer than `start` is known to fall short where
@@ -643,6 +684,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     }
     const double known = tried ? weight_near : 0.0;
     for (uint32_t i = tid; i < NB; i += NT) s.hist[i] = 0;
+    if (tid == 0) s.listed = 0;
     __syncthreads();
     const bool weigh = by_weight && (cut || whole < 0.0);
     double w = 0.0;
@@ -664,6 +706,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     if (weigh) whole = sum_of(s.part_w[turn][0]);
     turn ^= 1;
     const double target = double(top_p) * whole;
+    bool have_list = false;  // the list holds the keys [klo, khi]
     uint32_t inside = 0, ahead = 0, listed = 0;  // candidates, tokens above them, the set of their counts
     double above = 0.0, astray = 0.0;            // weight of all keys above khi
     bool hit = false;
@@ -676,11 +719,16 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         if (tid == 0) s.low = NB, s.found = NB;
         if (by_weight) {
           double x[4], t = 0.0;
+          if (tid == 0) s.spread = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) t += x[i] = h[i] ? h[i] * weight(zmax - start - (tid * 4 + i) / per_unit) : 0.0;
           double run = known + (cta_scan(t, s.scan_w) - t);
-          // (a value may lie half a bin off its middle, and they mostly even out)
-          const double slack = (2e-5 + 0.2 * cool / per_unit) * target, goal = target + astray;
+          // four standard deviations, were the bins' weights off by even chances
+          // of up to half a bin
+          const float squares = warp_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
+          if (lane == 0) atomicAdd(&s.spread, squares);
+          __syncthreads();
+          const double slack = 4 * 0.2887 * cool / per_unit * sqrtf(s.spread) + 1e-7 * target, goal = target + astray;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             run += x[i];
@@ -717,7 +765,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       w = 0.0;
       if (some)
         for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
-          const uint4 raw = resident ? held[v - v0] : read(v);
+          const uint4 raw = HELD ? held[v - v0] : read(v);
           if (zmax - E::most(raw) > far) continue;
           float z[EPV];
           E::get(raw, z);
@@ -730,7 +778,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
             const float d = zmax - z[i];
             any |= d >= near && d <= far;
             over += d < near;
-            if (by_weight) e[i] = d < near ? weight(z[i]) : 0.0;
+            if (by_weight) e[i] = weight(d < near ? z[i] : -INFINITY);
           }
           if (by_weight) {
 #pragma unroll
@@ -771,7 +819,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       if (tid == 0) s.listed = 0;
       __syncthreads();
     }
-    bool listing = hit && inside <= CAP;
+    bool listing = hit && inside <= CAP && klo != khi, counted = hit && klo == khi;
     if (!hit) {  // the border lies elsewhere: in the whole range
       klo = key_of(-INFINITY) + 1, khi = key_of(zmax), inside = ~0u, ahead = 0, above = 0.0;
       passed = 0.0, passed_n = 0;
@@ -800,14 +848,16 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         key = s.ctl[0];
         index = int32_t(s.ctl[1]);
       } else {
-        const bool single = klo == khi;
+        const bool single = klo == khi, have = counted;
+        have_list = counted;
+        counted = false;
         const int shift = max(0, 32 - __clz(khi - klo) - 2);
         double wq[4] = {};
         uint32_t cq[4] = {};
-        listing = inside <= CAP;
-        if (tid == 0) s.listed = 0;
+        listing = inside <= CAP && !single;
+        if (!have && tid == 0) s.listed = 0;
         __syncthreads();
-        for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+        for (uint32_t v = have ? wv1 : wv0 + lane; v < wv1; v += 32) {
           float z[EPV];
           fetch(v, z);
 #pragma unroll
@@ -825,7 +875,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
             }
           }
         }
-        if (listing || single) {
+        if (have) {
+        } else if (listing || single) {
           share_c(0, cq[0]);
         } else {
 #pragma unroll
@@ -835,9 +886,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
             if (lane < C) push(&s.quarter_w[turn][j][me], lane, x), push(&s.quarter_c[turn][j][me], lane, c);
           }
         }
-        cluster_sync();
-        const uint32_t now = turn;
-        turn ^= 1;
+        if (!have) cluster_sync();
+        const uint32_t now = have ? listed : turn;
+        if (!have) turn ^= 1;
         if (listing) {
           listed = now;
           continue;
@@ -913,7 +964,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         // (a border that keeps all of a key leaves an earlier one as it is)
         if (key > bkey || (key == bkey && index < bidx)) bkey = key, bidx = index;
         cut = true;
-        if (tid == 0) s.listed = 0;
+        whole_list = hit && (listing ? inside <= NT : have_list && inside <= CAP);
         return;
       }
     }
@@ -933,16 +984,39 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   const float upto = summed ? value_of(khi) : INFINITY, from = fmaxf(floor_z, border);
   double w = summed ? passed : 0.0;
   uint32_t n = summed ? passed_n : 0;
-  for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
-    const uint4 raw = resident ? held[v - v0] : read(v);
+  if (summed && whole_list) {
+    // each warp takes its own of them; their order is not fixed, so they are
+    // added as integers
+    uint64_t fixed = 0;
+    const uint32_t many = s.listed;
+    for (uint32_t i = lane; i < many; i += 32) {
+      const uint32_t at = uint32_t(s.list[i]), v = (at + skew) / EPV;
+      const float z = value_of(~uint32_t(s.list[i] >> 32));
+      if (v >= wv0 && v < wv1 && kept(z, at)) fixed += uint64_t(weight(z) * 0x1p52 + 0.5), ++n;
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) fixed += __shfl_xor_sync(0xffffffffu, fixed, d);
+    if (lane == 0) w += double(fixed) * 0x1p-52;
+  } else for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+    const uint4 raw = HELD ? held[v - v0] : read(v);
     if (E::most(raw) < from) continue;
     float z[EPV];
     E::get(raw, z);
+    bool any = false;
 #pragma unroll
     for (int i = 0; i < EPV; ++i) {
       z[i] += 0.f;
-      if (z[i] <= upto && kept(z[i], v * EPV + i - skew)) w += weight(z[i]), ++n;
+      const bool now = z[i] <= upto && kept(z[i], v * EPV + i - skew);
+      z[i] = now ? z[i] : -INFINITY;
+      n += now;
+      any |= now;
     }
+    if (!any) continue;
+    double e[EPV];
+#pragma unroll
+    for (int i = 0; i < EPV; ++i) e[i] = weight(z[i]);
+#pragma unroll
+    for (int i = 0; i < EPV; ++i) w += e[i];
   }
   share_w(0, w);
   share_c(0, n);
@@ -984,7 +1058,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     if (v < wv1) fetch(v, z);
 #pragma unroll
     for (int i = 0; i < EPV; ++i) {
-      e[i] = v < wv1 && kept(z[i], v * EPV + i - skew) ? weight(z[i]) : 0.0;
+      e[i] = weight(v < wv1 && kept(z[i], v * EPV + i - skew) ? z[i] : -INFINITY);
       t += e[i];
     }
     const double inc = warp_scan(t, lane);
@@ -1010,7 +1084,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     if (past) break;
     before += __shfl_sync(0xffffffffu, inc, 31);
   }
-  if (lane == 0) answer(token, int32_t(many), float((double(z_token) - zm) * cool - log(total)));
+  if (lane == 0) answer(token, int32_t(many), float((widened(z_token) - zm) * cool - log(total)));
 }
 
 template <class T>
@@ -1024,11 +1098,12 @@ cudaError_t launch(const SampleArgs& given, int sms, cudaStream_t st) {
   uint32_t c = 1;
   while (c < kMaxCluster && (p.a.rows * c * 2 <= uint64_t(sms) || bytes(c) > kMost / 2)) c *= 2;
   p.cluster = c;
-  p.resident = bytes(c) <= kMost;
+  const bool holds = bytes(c) <= kMost;
   p.held_off = uint32_t(kOver);
-  const uint64_t smem = p.resident ? bytes(c) : kOver;
-  static std::atomic<uint64_t> done{0};
-  const cudaError_t e = opt_in_smem(sample_kernel<T>, kMost, done);
+  const uint64_t smem = holds ? bytes(c) : kOver;
+  auto kernel = holds ? sample_kernel<T, true> : sample_kernel<T, false>;
+  static std::atomic<uint64_t> done[2] = {};
+  const cudaError_t e = opt_in_smem(kernel, kMost, done[holds]);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(uint32_t(p.a.rows * c));
@@ -1043,7 +1118,7 @@ cudaError_t launch(const SampleArgs& given, int sms, cudaStream_t st) {
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, p);
+  return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 }  // namespace
@@ -1081,7 +1156,7 @@ int xksv_sample(const xksv_sample_args* a, void* stream) {
     cudaGetLastError();  // not the next launch's
     return 1;
   }
-  return launch_sample(SampleArgs{*a, 0, 0, 0}, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0 : 1;
+  return launch_sample(SampleArgs{*a, 0, 0}, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0 : 1;
 }
 
 }  // extern "C"

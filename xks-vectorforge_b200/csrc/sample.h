@@ -12,8 +12,7 @@ constexpr float kSampleColdest = 1e-6f, kSampleHottest = 1e6f;
 struct SampleArgs {
   xksv_sample_args a;
   uint32_t cluster;   // CTAs that share a row
-  uint32_t resident;  // the row fits their shared memory
-  uint32_t held_off;  // where in it
+  uint32_t held_off;  // where the row lies in their shared memory
 };
 cudaError_t launch_sample(const SampleArgs& p, int sms, cudaStream_t st);
 
