@@ -328,7 +328,7 @@ int xksv_tp_gemm(const xksv_plan* plan, const void* d_payload, size_t payload_si
 /* No reference counterpart (the reference's GEMV takes one FP32 column and
  * leaves bias, activation and residual to the caller, python/runtime.py:
  * 264-284).  Element types of activations and caches: */
-enum { XKSV_BF16 = 1, XKSV_FP16 = 2, XKSV_FP32 = 3, XKSV_E4M3 = 4 };
+enum { XKSV_BF16 = 1, XKSV_FP16 = 2, XKSV_FP32 = 3, XKSV_E4M3 = 4, XKSV_INT8 = 5 };
 enum { XKSV_ACT_NONE = 0, XKSV_ACT_RELU = 1, XKSV_ACT_SILU = 2, XKSV_ACT_GELU = 3, XKSV_ACT_GELU_TANH = 4 };
 
 /* For every token b and every row r of Y that a slab covers:
@@ -413,6 +413,35 @@ typedef struct xksv_kv xksv_kv;
  * whose row is no multiple of 16 bytes, and scales with a 16-bit type.
  * Every call below runs on this device, whichever is current. */
 int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** kv);
+
+/* A cache of 8-bit elements with a scale for each block of tokens and head:
+ * type is XKSV_E4M3 or XKSV_INT8 (two's complement, -127 .. 127), k_scale and v_scale of the
+ * desc are NULL, and an element of place t and head h of a page stands for its
+ * value times the FP32 number scale[page * stride[0] + t / block * stride[1] +
+ * h * stride[2]] (strides in elements; `block` divides page_size).  No scale
+ * needs to be known beforehand: xksv_kv_append sets them.  The tokens of one
+ * call that go to one block make each head's scale the least power of two 2^e, e >= -60,
+ * that holds their largest finite element (448 or 127 times the scale), or
+ * leave the block's scale as it is where that is larger and the block's first
+ * new token is not its first place; where the scale rises, the
+ * elements of the block's places before are rounded to it again.  A call that writes a block's
+ * first place begins the block anew; its places behind the new tokens hold
+ * nothing.  In such a call the tokens of one sequence stand next to each
+ * other, their index rising by one (padding may stand between sequences): a call that breaks
+ * this, or two sequences that write to one block, leave the
+ * elements of the blocks concerned undefined; the former is reported by
+ * xksv_kv_status.  NaN becomes E4M3's NaN, or an integer zero, reported by
+ * xksv_kv_status.  Infinite elements saturate.  xksv_kv_attend takes any
+ * positive finite scales.  Returns 1 as xksv_kv_create does, and for scales that
+ * leave their buffers or overlap. */
+typedef struct xksv_kv_blocks {
+  float* k_scale;
+  float* v_scale;
+  uint64_t k_bytes, v_bytes; /* buffer sizes */
+  uint64_t block;
+  uint64_t k_stride[3], v_stride[3]; /* page, block, head */
+} xksv_kv_blocks;
+int xksv_kv_create_blocks(const xksv_kv_desc* desc, const xksv_kv_blocks* blocks, xksv_kv** kv);
 void xksv_kv_destroy(xksv_kv* kv);
 /* Synchronises `stream`; 0 when no call reported an error since the last one
  * (then clears the word), else 1: a page outside the cache, a sequence or a
@@ -467,7 +496,7 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* str
  * value: infinity or NaN there. Tokens behind L, and the rest of
  * their pages, are not read. q and out are [seqs, q_heads, head_dim] of
  * `type`, strides in elements ([0] sequence, [1] head), the last dimension
- * contiguous; type is the cache's, or BF16 or FP16 over an E4M3 cache. lse is
+ * contiguous; type is the cache's, or BF16 or FP16 over an 8-bit cache. lse is
  * FP32 [seqs, q_heads] contiguous, or NULL. Scores, softmax statistics and
  * sums are FP32, a weight enters its product within 2^-17. A length that is negative or above table_cols * page_size
  * gives zeros and -infinity, a page outside the cache counts as masked; both

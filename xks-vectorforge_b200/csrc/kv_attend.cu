@@ -57,10 +57,15 @@ constexpr int kCluster = 8;  // CTAs of a unit whose pieces meet in shared memor
 static_assert(kCluster * kWarps == 32, "the join reads a piece's statistics per lane");
 constexpr int kStages = 2;  // blocks in a warp's ring: one landing while one is worked on
 
-// Shape of a kernel: the cache's elements (E8: E4M3), rows padded to DP dims,
-// NG groups of eight query heads.
-template <bool E8, int DP, int NG>
+// The cache's elements: 16 bits; E4M3 with a scale per head; E4M3 or integers
+// with one for each block of tokens.
+enum : int { EL16 = 0, ELE4M3 = 1, ELE4M3Blocks = 2, ELInt8Blocks = 3 };
+
+// Shape of a kernel: the cache's elements, rows padded to DP dims, NG groups of
+// eight query heads.
+template <int EL, int DP, int NG>
 struct Shape {
+  static constexpr bool E8 = EL != EL16, BS = EL >= ELE4M3Blocks;
   static constexpr int ES = E8 ? 1 : 2;
   static constexpr int RB = DP * ES;              // bytes of a staged row
   static constexpr int CH = RB / 16;              // 16-byte pieces of a row (4 .. 32)
@@ -68,7 +73,8 @@ struct Shape {
   static constexpr int KV = BT * RB;              // bytes of a block's keys (or values)
   static constexpr bool QS = DP * NG > 256;       // query fragments in shared memory, not registers
   static constexpr int QB = QS ? DP / 16 * 32 * 8 * NG : 0;
-  static constexpr int WARP = kStages * 2 * KV + QB + 16;  // + the stages' token masks
+  static constexpr int SB = BS ? kStages * 2 * BT * 4 : 0;      // the stages' scales
+  static constexpr int WARP = kStages * 2 * KV + QB + SB + 16;  // + the stages' token masks
   static constexpr int CTA = kWarps * WARP;
   // CTAs an SM holds.  Three of two stages against two of three stages: 64
   // uneven sequences 399 us against 409, E4M3 85 against 92
@@ -83,6 +89,10 @@ __device__ __forceinline__ uint32_t swz(uint32_t r, uint32_t c) {
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+}
+// Four bytes, or zeros for n = 0.
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, uint32_t n) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
@@ -114,6 +124,25 @@ __device__ __forceinline__ void e4m3x4(uint32_t x, uint32_t& lo, uint32_t& hi) {
   asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
       : "=r"(lo), "=r"(hi)
       : "r"(x));
+}
+// Four integers as two pairs of FP16: v + 128 as the low bits of 1024 + (v + 128).
+// In order, or the first and third, then the second and fourth.
+template <bool ACROSS>
+__device__ __forceinline__ void int8x4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  constexpr uint32_t kBase = 0x64806480u;  // 1152
+  x ^= 0x80808080u;
+  lo = __byte_perm(x, 0x64646464u, ACROSS ? 0x4240 : 0x4140);
+  hi = __byte_perm(x, 0x64646464u, ACROSS ? 0x4341 : 0x4342);
+  asm("sub.rn.f16x2 %0, %0, %1;\n" : "+r"(lo) : "r"(kBase));
+  asm("sub.rn.f16x2 %0, %0, %1;\n" : "+r"(hi) : "r"(kBase));
+}
+// Four bytes of the cache, in order or across, as FP16.
+template <int EL, bool ACROSS>
+__device__ __forceinline__ void widen4(uint32_t x, uint32_t& lo, uint32_t& hi) {
+  if (EL == ELInt8Blocks)
+    int8x4<ACROSS>(x, lo, hi);
+  else
+    e4m3x4(ACROSS ? __byte_perm(x, 0, 0x3120) : x, lo, hi);
 }
 // The 8 x 8 matrix of 16-bit elements that the warp holds, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -175,9 +204,10 @@ __device__ __forceinline__ void cluster_barrier() {
 // CL (calls of few units and short tables): a unit's blocks are shared by the
 // 32 warps of a cluster of CTAs, which then join their pieces from one
 // another's shared memory: no second kernel and no workspace.
-template <bool MB, bool E8, int DP, int NG, bool FULL, bool CL>
-__global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_attend_kernel(const AttendArgs p, const AttendPlan pl) {
-  using Sh = Shape<E8, DP, NG>;
+template <bool MB, int EL, int DP, int NG, bool FULL, bool CL>
+__global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_attend_kernel(const AttendArgs p, const AttendPlan pl) {
+  using Sh = Shape<EL, DP, NG>;
+  constexpr bool E8 = Sh::E8, BS = Sh::BS;
   constexpr int CH = Sh::CH, BT = Sh::BT, RB = Sh::RB;
   constexpr int KS = DP / 16;  // 16-dim steps
   constexpr int TB = BT / 16;  // 16-token steps
@@ -268,7 +298,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
 
   uint8_t* ws = smem + warp * Sh::WARP;
   const uint32_t ring = smem_addr(ws), qsm = ring + kStages * 2 * Sh::KV;
-  volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(ws + kStages * 2 * Sh::KV + Sh::QB);
+  volatile uint32_t* masks = reinterpret_cast<volatile uint32_t*>(ws + kStages * 2 * Sh::KV + Sh::QB + Sh::SB);
+  // a stage's scales: BT keys', BT values'; masked tokens' are zero
+  const volatile float* scales = reinterpret_cast<const volatile float*>(ws + kStages * 2 * Sh::KV + Sh::QB);
   // dims past head_dim stay zero: no copy writes there
   if (D < DP) {
     for (uint32_t i = lane; i < kStages * 2 * Sh::KV / 16; i += 32)
@@ -317,6 +349,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
   // this lane's token of the next block to copy: its rows' offsets in bytes
   bool ld_ok = false;
   uint64_t ld_k = 0, ld_v = 0;
+  const float *ld_ks = p.b.k_scale, *ld_vs = p.b.v_scale;
   const uint32_t psize = uint32_t(p.c.page_size);
   auto look_up = [&]() {
     const uint32_t j = (uint32_t(ld.first) / BT + ld.block) * BT + lane;
@@ -330,6 +363,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
         ld_ok = true;
         ld_k = (uint32_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2]) * Sh::ES;
         ld_v = (uint32_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2]) * Sh::ES;
+        if (BS) {
+          const uint32_t block = pl.block_shift >= 0 ? place >> pl.block_shift : place / uint32_t(p.b.block);
+          ld_ks = p.b.k_scale + uint32_t(page) * p.b.k_stride[0] + block * p.b.k_stride[1] + g * p.b.k_stride[2];
+          ld_vs = p.b.v_scale + uint32_t(page) * p.b.v_stride[0] + block * p.b.v_stride[1] + g * p.b.v_stride[2];
+        }
       } else {
         atomicOr(p.status, kStatusHeader);  // a page outside the cache
       }
@@ -344,6 +382,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
     const uint32_t mask = __ballot_sync(0xffffffffu, ld_ok);
     if (lane == 0) masks[stage] = mask;
     const uint32_t kd = ring + stage * 2 * Sh::KV, vd = kd + Sh::KV;
+    if (BS && lane < BT) {
+      const uint32_t sd = qsm + Sh::QB + (stage * 2 * BT + lane) * 4;
+      copy4(sd, ld_ks, ld_ok ? 4 : 0);
+      copy4(sd + BT * 4, ld_vs, ld_ok ? 4 : 0);
+    }
     if (FULL && run && mask == (BT == 32 ? 0xffffffffu : 0xffffu)) {
       // sixteen tokens of a page lie one token's stride apart
 #pragma unroll
@@ -525,6 +568,16 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
     __syncwarp();
     const uint32_t kd = ring + stage * 2 * Sh::KV, vd = kd + Sh::KV;
     const uint32_t mask = masks[stage];
+    float ks[TB][2], vs[TB][2];  // of this lane's tokens
+    if (BS) {
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          ks[tb][y] = scales[stage * 2 * BT + tb * 16 + hr + 8 * y];
+          vs[tb][y] = scales[stage * 2 * BT + BT + tb * 16 + hr + 8 * y];
+        }
+    }
     // the stage before this one is free: every lane has passed the barrier
     if (t + kStages - 1 < b) {
       issue(put);
@@ -574,8 +627,8 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
 #pragma unroll
           for (int y = 0; y < Y; ++y) {
             uint32_t ka[4];
-            e4m3x4(r[2 * y], ka[0], ka[2]);
-            e4m3x4(r[2 * y + 1], ka[1], ka[3]);
+            widen4<EL, false>(r[2 * y], ka[0], ka[2]);
+            widen4<EL, false>(r[2 * y + 1], ka[1], ka[3]);
 #pragma unroll
             for (int n = 0; n < NG; ++n) mma<false>(sc[tb][n], ka, qb[y][n][0], qb[y][n][1]);
           }
@@ -584,6 +637,14 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
           for (int n = 0; n < NG; ++n) mma<MB>(sc[tb][n], r, qb[0][n][0], qb[0][n][1]);
         }
       }
+    }
+    if (BS) {
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sc[tb][n][x] *= ks[tb][x >> 1];
     }
     // ---- softmax step, in powers of two ----
     if (p.a.softcap > 0.f) {
@@ -653,6 +714,25 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
     // ---- O^T += V^T P^T ----
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb) {
+      // Block scales: a weight enters with its token's scale as a part of the
+      // sixteen tokens' largest, which the FP32 sums take in.  Where they share
+      // one there is nothing to do for it.
+      float high = 1.f;
+      if (BS) {
+        high = vs[tb][0];
+        if (!pl.even || ((mask >> (16 * tb)) & 0xffffu) != 0xffffu) {
+          high = fmaxf(high, vs[tb][1]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            // (NaN scales stay NaN)
+            const float part = vs[tb][y] == high ? 1.f : vs[tb][y] / high;
+#pragma unroll
+            for (int n = 0; n < NG; ++n) sc[tb][n][2 * y] *= part, sc[tb][n][2 * y + 1] *= part;
+          }
+        }
+      }
       uint32_t hi[NG][2], lo[NG][2];
 #pragma unroll
       for (int n = 0; n < NG; ++n)
@@ -680,12 +760,20 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<E8, DP, NG>::PER_SM) kv_att
           for (int y = 0; y < 2; ++y) {
             // bytes (dim 2n, 2n + 1) of two tokens -> dim 2n of both, dim 2n + 1 of both
             uint32_t va[4];
-            e4m3x4(__byte_perm(r[2 * y], 0, 0x3120), va[0], va[1]);
-            e4m3x4(__byte_perm(r[2 * y + 1], 0, 0x3120), va[2], va[3]);
+            widen4<EL, true>(r[2 * y], va[0], va[1]);
+            widen4<EL, true>(r[2 * y + 1], va[2], va[3]);
 #pragma unroll
             for (int n = 0; n < NG; ++n) {
-              mma<false>(o[n][i + y], va, hi[n][0], hi[n][1]);
-              mma<false>(o[n][i + y], va, lo[n][0], lo[n][1]);
+              if (BS) {
+                float some[4] = {};
+                mma<false>(some, va, hi[n][0], hi[n][1]);
+                mma<false>(some, va, lo[n][0], lo[n][1]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[n][i + y][x] += some[x] * high;
+              } else {
+                mma<false>(o[n][i + y], va, hi[n][0], hi[n][1]);
+                mma<false>(o[n][i + y], va, lo[n][0], lo[n][1]);
+              }
             }
           }
         } else {
@@ -909,11 +997,11 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
 
 int pad_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-template <bool MB, bool E8, int DP, int NG, bool FULL, bool CL>
+template <bool MB, int EL, int DP, int NG, bool FULL, bool CL>
 cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
-  using Sh = Shape<E8, DP, NG>;
+  using Sh = Shape<EL, DP, NG>;
   static_assert(8 * NG * (DP + 2) * 4 <= Sh::WARP, "a piece fits the warp's shared memory");
-  auto kernel = kv_attend_kernel<MB, E8, DP, NG, FULL, CL>;
+  auto kernel = kv_attend_kernel<MB, EL, DP, NG, FULL, CL>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = opt_in_smem(kernel, Sh::CTA, done);
   if (e != cudaSuccess) return e;
@@ -938,32 +1026,32 @@ cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_
   return cudaLaunchKernelEx(&cfg, kv_join_kernel, p, pl, MB ? 0.f : 15.f);
 }
 
-template <bool MB, bool E8, int DP, int NG>
+template <bool MB, int EL, int DP, int NG>
 cudaError_t launch_full(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
   if (pl.clusters)
-    return p.c.head_dim == DP ? launch_attend<MB, E8, DP, NG, true, true>(p, pl, st)
-                              : launch_attend<MB, E8, DP, NG, false, true>(p, pl, st);
-  return p.c.head_dim == DP ? launch_attend<MB, E8, DP, NG, true, false>(p, pl, st)
-                            : launch_attend<MB, E8, DP, NG, false, false>(p, pl, st);
+    return p.c.head_dim == DP ? launch_attend<MB, EL, DP, NG, true, true>(p, pl, st)
+                              : launch_attend<MB, EL, DP, NG, false, true>(p, pl, st);
+  return p.c.head_dim == DP ? launch_attend<MB, EL, DP, NG, true, false>(p, pl, st)
+                            : launch_attend<MB, EL, DP, NG, false, false>(p, pl, st);
 }
-template <bool MB, bool E8, int DP>
+template <bool MB, int EL, int DP>
 cudaError_t launch_heads(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
-  return pl.heads <= 8 ? launch_full<MB, E8, DP, 1>(p, pl, st) : launch_full<MB, E8, DP, 2>(p, pl, st);
+  return pl.heads <= 8 ? launch_full<MB, EL, DP, 1>(p, pl, st) : launch_full<MB, EL, DP, 2>(p, pl, st);
 }
-template <bool MB, bool E8>
+template <bool MB, int EL>
 cudaError_t launch_dim(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
   switch (pl.pad_dim) {
-    case 64: return launch_heads<MB, E8, 64>(p, pl, st);
-    case 128: return launch_heads<MB, E8, 128>(p, pl, st);
-    default: return launch_heads<MB, E8, 256>(p, pl, st);
+    case 64: return launch_heads<MB, EL, 64>(p, pl, st);
+    case 128: return launch_heads<MB, EL, 128>(p, pl, st);
+    default: return launch_heads<MB, EL, 256>(p, pl, st);
   }
 }
 
-template <bool E8, int NG>
+template <int EL, int NG>
 void shape_of(uint32_t dp, uint32_t* block, uint32_t* per_sm) {
-  using A = Shape<E8, 64, NG>;
-  using B = Shape<E8, 128, NG>;
-  using C = Shape<E8, 256, NG>;
+  using A = Shape<EL, 64, NG>;
+  using B = Shape<EL, 128, NG>;
+  using C = Shape<EL, 256, NG>;
   *block = dp == 64 ? A::BT : dp == 128 ? B::BT : C::BT;
   *per_sm = dp == 64 ? A::PER_SM : dp == 128 ? B::PER_SM : C::PER_SM;
 }
@@ -978,21 +1066,26 @@ void shape_of(uint32_t dp, uint32_t* block, uint32_t* per_sm) {
 // eight uneven sequences to 777 15.0 and 12.1, 64 of them 81 and 28.
 constexpr uint64_t kShort = 4096;
 
-AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads, uint64_t table_cols, int sms) {
+AttendPlan kv_attend_plan(const xksv_kv_desc& c, const xksv_kv_blocks& b, uint64_t seqs, uint32_t q_heads, uint64_t table_cols, int sms) {
   AttendPlan pl{};
   const uint32_t group = q_heads / c.kv_heads;
   pl.chunks = (group + 15) / 16;
   pl.heads = (group + pl.chunks - 1) / pl.chunks;
   pl.pad_dim = uint32_t(pad_dim(c.head_dim));
-  pl.page_shift = -1;
+  pl.page_shift = pl.block_shift = -1;
   for (int k = 0; k < 31; ++k)
     if (c.page_size == 1ull << k) pl.page_shift = k;
   uint32_t block = 16, per_sm = 1;
-  const bool e8 = c.type == XKSV_E4M3;
-  if (pl.heads <= 8)
-    e8 ? shape_of<true, 1>(pl.pad_dim, &block, &per_sm) : shape_of<false, 1>(pl.pad_dim, &block, &per_sm);
-  else
-    e8 ? shape_of<true, 2>(pl.pad_dim, &block, &per_sm) : shape_of<false, 2>(pl.pad_dim, &block, &per_sm);
+  if (b.block) {
+    for (int k = 0; k < 31; ++k)
+      if (b.block == 1ull << k) pl.block_shift = k;
+    pl.even = b.block % 16 == 0;
+    pl.heads <= 8 ? shape_of<ELE4M3Blocks, 1>(pl.pad_dim, &block, &per_sm) : shape_of<ELE4M3Blocks, 2>(pl.pad_dim, &block, &per_sm);
+  } else if (c.type == XKSV_E4M3) {
+    pl.heads <= 8 ? shape_of<ELE4M3, 1>(pl.pad_dim, &block, &per_sm) : shape_of<ELE4M3, 2>(pl.pad_dim, &block, &per_sm);
+  } else {
+    pl.heads <= 8 ? shape_of<EL16, 1>(pl.pad_dim, &block, &per_sm) : shape_of<EL16, 2>(pl.pad_dim, &block, &per_sm);
+  }
   // no more workers than blocks of the longest sequences the table can hold
   const uint64_t longest = table_cols * c.page_size / block + 1;
   const uint64_t blocks = seqs * c.kv_heads * pl.chunks;
@@ -1009,8 +1102,9 @@ AttendPlan kv_attend_plan(const xksv_kv_desc& c, uint64_t seqs, uint32_t q_heads
 }
 
 cudaError_t launch_kv_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
-  if (p.c.type == XKSV_E4M3) return launch_dim<false, true>(p, pl, st);
-  return p.c.type == XKSV_BF16 ? launch_dim<true, false>(p, pl, st) : launch_dim<false, false>(p, pl, st);
+  if (p.c.type == XKSV_INT8) return launch_dim<false, ELInt8Blocks>(p, pl, st);
+  if (p.c.type == XKSV_E4M3) return p.b.block ? launch_dim<false, ELE4M3Blocks>(p, pl, st) : launch_dim<false, ELE4M3>(p, pl, st);
+  return p.c.type == XKSV_BF16 ? launch_dim<true, EL16>(p, pl, st) : launch_dim<false, EL16>(p, pl, st);
 }
 
 }  // namespace xksv

@@ -4,54 +4,26 @@
 //
 // This file holds the kernels and their C entries; the cache itself is the
 // caller's memory, the handle its geometry and a device status word.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
 #include <algorithm>
 #include <new>
 #include <utility>
 
 #include "kernels.h"
 #include "kv_cache.h"
+#include "kv_elements.cuh"
 #include "kv_index.h"
 #include "xksv_types.h"
 
 struct xksv_kv {
   int device = 0, sms = 148;
   xksv_kv_desc d{};
+  xksv_kv_blocks b{};  // block 0: no block scales
   int* d_status = nullptr;
   int* h_status = nullptr;
 };
 
 namespace xksv {
 namespace {
-
-// ------------------------------------------------------------- elements ---
-struct E4m3 {
-  __nv_fp8_storage_t b;
-};
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_float(float x) { return x; }
-template <class T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
-  return __float2bfloat16_rn(x);
-}
-template <>
-__device__ __forceinline__ __half from_float<__half>(float x) {
-  return __float2half_rn(x);
-}
-template <>
-__device__ __forceinline__ float from_float<float>(float x) {
-  return x;
-}
-template <>
-__device__ __forceinline__ E4m3 from_float<E4m3>(float x) {
-  return E4m3{__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3)};
-}
 
 // --------------------------------------------------------------- append ---
 // Bound: memory (every element is read once and written once) for prompts,
@@ -65,18 +37,9 @@ constexpr int AT = 128;         // threads per token
 constexpr int kMaxPairs = 128;  // head_dim <= 256
 constexpr int kPerSm = 6;       // CTAs an SM holds (16384 tokens: 71 us; three of 256 threads 83 us)
 
-// cos and sin of a token's angles into shared memory.  The angle is formed in
-// 64 bits, less its whole turns: an FP32 product would be wrong by radians at
-// far positions.
+// cos and sin of a token's angles into shared memory.
 __device__ __forceinline__ void angles(const xksv_kv_append_args& a, int32_t pos, float* cs, float* sn) {
-  constexpr double kTurn = 6.283185307179586476925286766559, kTurns = 1.0 / kTurn, kHalfTurns = 2.0 / kTurn;
-  for (uint32_t i = threadIdx.x; i < a.rot_dim / 2; i += AT) {
-    const double angle = double(pos) * double(a.inv_freq[i]);
-    float sv, cv;
-    sincospif(float(fma(-rint(angle * kTurns), kTurn, angle) * kHalfTurns), &sv, &cv);
-    cs[i] = cv * a.rot_scale;
-    sn[i] = sv * a.rot_scale;
-  }
+  for (uint32_t i = threadIdx.x; i < a.rot_dim / 2; i += AT) angle_of(pos, a.inv_freq[i], a.rot_scale, &cs[i], &sn[i]);
 }
 
 // A token's place in the cache (below 2^31: 32-bit division); page -1:
@@ -86,57 +49,6 @@ __device__ __forceinline__ KvPlace token_place(const AppendArgs& p, int64_t seq,
   const KvPlace at = kv_place(p.a.table, p.a.table_rows, p.a.table_cols, p.a.table_stride, p.c.pages, uint32_t(p.c.page_size), seq, idx);
   if (at.page < 0 && threadIdx.x == 0) atomicOr(p.status, kStatusHeader);
   return at;
-}
-
-// Eight elements as 32-bit words (E4M3: two, 16-bit types: four, FP32: eight).
-template <class T>
-struct alignas(sizeof(T) == 1 ? 8 : 16) Eight {
-  uint32_t w[sizeof(T) * 2];
-};
-__device__ __forceinline__ void spread(const Eight<__nv_bfloat16>& a, float* x) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(a.w[i] << 16);
-    x[2 * i + 1] = __uint_as_float(a.w[i] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ void spread(const Eight<__half>& a, float* x) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a.w[i]));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-  }
-}
-__device__ __forceinline__ void spread(const Eight<float>& a, float* x) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(a.w[i]);
-}
-__device__ __forceinline__ void gather(const float* x, Eight<__nv_bfloat16>& a) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    a.w[i] = *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-__device__ __forceinline__ void gather(const float* x, Eight<__half>& a) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 v = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-    a.w[i] = *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-__device__ __forceinline__ void gather(const float* x, Eight<float>& a) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a.w[i] = __float_as_uint(x[i]);
-}
-__device__ __forceinline__ void gather(const float* x, Eight<E4m3>& a) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]), __NV_SATFINITE, __NV_E4M3);
-    a.w[i] = lo | hi << 16;
-  }
 }
 
 // Rows of 16-byte pieces (alignment, and rotated pairs that fill them) whose
@@ -365,30 +277,39 @@ cudaError_t append_cache(const AppendArgs& p, int sms, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------- C entry checks
-uint64_t elem_bytes(uint32_t type) { return type == XKSV_E4M3 ? 1 : type == XKSV_FP32 ? 4 : 2; }
+uint64_t elem_bytes(uint32_t type) { return type == XKSV_E4M3 || type == XKSV_INT8 ? 1 : type == XKSV_FP32 ? 4 : 2; }
 bool off_align(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0; }
 
-// The elements of a cache buffer lie inside it, on 16-byte rows, and no two
-// (page, token, head) rows overlap: ordered by stride, each dimension steps
-// past the whole extent of the smaller ones.
-bool strides_ok(const xksv_kv_desc& d, const void* base, uint64_t bytes, const uint64_t* stride) {
-  const uint64_t e = elem_bytes(d.type), total = bytes / e;
-  if (!base || off_align(base, 16)) return false;
+// Rows of `row` elements of e bytes at [page, token, head] lie inside the
+// buffer, strides are multiples of `align` bytes, and no two rows overlap: ordered by
+// stride, each dimension steps past the whole extent of the smaller ones.
+bool strides_fit(const uint64_t* n, const uint64_t* stride, uint64_t row, uint64_t e, uint64_t align, uint64_t bytes) {
+  const uint64_t total = bytes / e;
   struct Dim {
     uint64_t n, stride;
-  } dim[3] = {{d.pages, stride[0]}, {d.page_size, stride[1]}, {d.kv_heads, stride[2]}};
+  } dim[3] = {{n[0], stride[0]}, {n[1], stride[1]}, {n[2], stride[2]}};
   for (int i = 0; i < 3; ++i)
     for (int j = i + 1; j < 3; ++j)
       if (dim[j].stride < dim[i].stride) std::swap(dim[i], dim[j]);
-  uint64_t extent = d.head_dim;
+  uint64_t extent = row;
   if (extent > total) return false;
   for (const Dim& x : dim) {
     if (x.n == 1) continue;
-    if (x.stride * e % 16 || x.stride < extent) return false;
+    if (x.stride * e % align || x.stride < extent) return false;
     if (x.stride > (total - extent) / (x.n - 1)) return false;
     extent += x.stride * (x.n - 1);
   }
   return true;
+}
+bool strides_ok(const xksv_kv_desc& d, const void* base, uint64_t bytes, const uint64_t* stride) {
+  const uint64_t n[3] = {d.pages, d.page_size, d.kv_heads};
+  return base && !off_align(base, 16) && strides_fit(n, stride, d.head_dim, elem_bytes(d.type), 16, bytes);
+}
+bool scales_ok(const xksv_kv_desc& d, const xksv_kv_blocks& b, const void* base, uint64_t bytes, const uint64_t* stride) {
+  const uint64_t n[3] = {d.pages, d.page_size / b.block, d.kv_heads};
+  for (int i = 0; i < 3; ++i)
+    if (stride[i] >= (1ull << 48)) return false;
+  return base && !off_align(base, 4) && strides_fit(n, stride, 1, 4, 4, bytes);
 }
 
 // No two rows of an output [n, heads, dim] overlap.
@@ -418,23 +339,30 @@ using namespace xksv;
 
 extern "C" {
 
-int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** out) {
+static int create(const xksv_kv_desc* desc, const xksv_kv_blocks* blocks, xksv_kv** out) {
   if (!out) return 1;
   *out = nullptr;
-  if (!desc || desc->flags || (desc->type != XKSV_BF16 && desc->type != XKSV_FP16 && desc->type != XKSV_E4M3)) return 1;
+  if (!desc || desc->flags) return 1;
   const xksv_kv_desc& d = *desc;
+  const bool e8 = d.type == XKSV_E4M3 || (blocks && d.type == XKSV_INT8);
+  if (!e8 && (blocks || (d.type != XKSV_BF16 && d.type != XKSV_FP16))) return 1;
   constexpr uint64_t kDim = 1ull << 31;
   if (!d.pages || !d.page_size || !d.kv_heads || !d.head_dim || d.head_dim > 256 || d.pages >= kDim ||
       d.page_size >= kDim || d.kv_heads > 65535 || d.head_dim * elem_bytes(d.type) % 16)
     return 1;
-  if (d.type != XKSV_E4M3 && (d.k_scale || d.v_scale)) return 1;
+  if ((!e8 || blocks) && (d.k_scale || d.v_scale)) return 1;
   if (off_align(d.k_scale, 4) || off_align(d.v_scale, 4)) return 1;
   for (int i = 0; i < 3; ++i)
     if (d.k_stride[i] >= (1ull << 48) || d.v_stride[i] >= (1ull << 48)) return 1;
   if (!strides_ok(d, d.k, d.k_bytes, d.k_stride) || !strides_ok(d, d.v, d.v_bytes, d.v_stride)) return 1;
+  if (blocks && (!blocks->block || d.page_size % blocks->block ||
+                 !scales_ok(d, *blocks, blocks->k_scale, blocks->k_bytes, blocks->k_stride) ||
+                 !scales_ok(d, *blocks, blocks->v_scale, blocks->v_bytes, blocks->v_stride)))
+    return 1;
   auto* kv = new (std::nothrow) xksv_kv();
   if (!kv) return 1;
   kv->d = d;
+  if (blocks) kv->b = *blocks;
   const bool ok = cudaGetDevice(&kv->device) == cudaSuccess &&
                   cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, kv->device) == cudaSuccess &&
                   cudaMalloc(&kv->d_status, sizeof(int)) == cudaSuccess &&
@@ -447,6 +375,13 @@ int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** out) {
   }
   *out = kv;
   return 0;
+}
+
+int xksv_kv_create(const xksv_kv_desc* desc, xksv_kv** out) { return create(desc, nullptr, out); }
+
+int xksv_kv_create_blocks(const xksv_kv_desc* desc, const xksv_kv_blocks* blocks, xksv_kv** out) {
+  if (out) *out = nullptr;
+  return blocks ? create(desc, blocks, out) : 1;
 }
 
 void xksv_kv_destroy(xksv_kv* kv) {
@@ -487,22 +422,24 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* a, void* stream
     return 1;
   DeviceGuard guard(kv->device);
   if (!guard.ok) return 1;
-  const AppendArgs p{*a, kv->d, kv->d_status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (kv->b.block)
+    return launch_kv_append_blocks(AppendBlocksArgs{*a, kv->d, kv->d_status, kv->b, 0}, kv->sms, st) == cudaSuccess ? 0 : 1;
+  const AppendArgs p{*a, kv->d, kv->d_status};
   return launch_kv_append(p, kv->sms, st) == cudaSuccess ? 0 : 1;
 }
 
 size_t xksv_kv_attend_workspace(const xksv_kv* kv, size_t seqs, size_t q_heads, size_t table_cols) {
   if (!kv || !seqs || !q_heads || q_heads % kv->d.kv_heads || q_heads > 65535 || !table_cols || table_cols >= (1ull << 31))
     return 0;
-  return size_t(kv_attend_plan(kv->d, seqs, uint32_t(q_heads), table_cols, kv->sms).bytes);
+  return size_t(kv_attend_plan(kv->d, kv->b, seqs, uint32_t(q_heads), table_cols, kv->sms).bytes);
 }
 
 int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* a, void* d_workspace, size_t workspace_bytes,
                    void* stream) {
   if (!kv || !a || !a->q_heads || a->q_heads % kv->d.kv_heads || a->q_heads > 65535) return 1;
   if (a->type != XKSV_BF16 && a->type != XKSV_FP16) return 1;
-  if (kv->d.type != XKSV_E4M3 && kv->d.type != a->type) return 1;
+  if (elem_bytes(kv->d.type) > 1 && kv->d.type != a->type) return 1;
   if (!(a->softcap >= 0.f) || a->seqs >= (1ull << 31)) return 1;
   if (!a->seqs) return 0;
   if (!a->q || !a->out || !a->table || !a->lens || !a->table_cols || a->table_cols >= (1ull << 31) ||
@@ -512,12 +449,12 @@ int xksv_kv_attend(const xksv_kv* kv, const xksv_kv_attend_args* a, void* d_work
   if (!strides_small(a->q_stride) || !strides_small(a->out_stride) ||
       !rows_distinct(a->seqs, a->q_heads, kv->d.head_dim, a->out_stride))
     return 1;
-  const AttendPlan pl = kv_attend_plan(kv->d, a->seqs, a->q_heads, a->table_cols, kv->sms);
+  const AttendPlan pl = kv_attend_plan(kv->d, kv->b, a->seqs, a->q_heads, a->table_cols, kv->sms);
   if (pl.bytes && (!d_workspace || workspace_bytes < pl.bytes || off_align(d_workspace, 256))) return 1;
   DeviceGuard guard(kv->device);
   if (!guard.ok) return 1;
   auto* ws = static_cast<uint8_t*>(d_workspace);
-  const AttendArgs p{*a, kv->d, kv->d_status, reinterpret_cast<float*>(ws), reinterpret_cast<int4*>(ws + pl.joins_off)};
+  const AttendArgs p{*a, kv->d, kv->d_status, reinterpret_cast<float*>(ws), reinterpret_cast<int4*>(ws + pl.joins_off), kv->b};
   return launch_kv_attend(p, pl, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0 : 1;
 }
 

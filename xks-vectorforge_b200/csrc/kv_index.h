@@ -28,6 +28,22 @@ XKSV_HD KvPlace kv_place(const int32_t* table, uint64_t rows, uint64_t cols, uin
   return page < 0 || uint64_t(page) >= pages ? KvPlace{-1, 0} : KvPlace{page, uint32_t(index) - col * page_size};
 }
 
+// Whether token t (above 0) goes on with the one before it in the same block of
+// `block` tokens: of the same sequence, its place one higher.  Without `seq`
+// every token is a sequence of its own.
+XKSV_HD bool kv_follows(const int32_t* seq, const int32_t* index, uint64_t t, uint32_t block) {
+  return seq && t > 0 && seq[t] >= 0 && seq[t] == seq[t - 1] && index[t - 1] >= 0 && index[t - 1] < index[t] &&
+         index[t] - index[t - 1] == 1 && uint32_t(index[t]) % block != 0;
+}
+
+// The exponent of the least power of two 2^e, e >= -60, with high <= 448 * 2^e
+// (E4M3) or high <= 127 * 2^e; from the bits of a finite FP32 number >= 0.
+XKSV_HD int kv_scale_exponent(uint32_t high, bool integer) {
+  // 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6
+  const int e = int(high >> 23) - 127 - (integer ? 6 : 8) + ((high & 0x7fffffu) > (integer ? 0x7e0000u : 0x600000u) ? 1 : 0);
+  return e < -60 ? -60 : e;
+}
+
 // Cached tokens that a new token attends to: [first, length).  A length
 // outside [0, cols * page_size] is an error and attends to nothing.
 struct KvSpan {

@@ -35,6 +35,13 @@ class KvDesc(ctypes.Structure):
                 ("type", ctypes.c_uint32), ("flags", ctypes.c_uint32)]
 
 
+class KvBlocks(ctypes.Structure):
+    """xksv_kv_blocks."""
+    _fields_ = [("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("k_bytes", ctypes.c_uint64),
+                ("v_bytes", ctypes.c_uint64), ("block", ctypes.c_uint64), ("k_stride", ctypes.c_uint64 * 3),
+                ("v_stride", ctypes.c_uint64 * 3)]
+
+
 # Argument blocks of the calls made once a token, packed as the C structs of
 # the same name lie in memory (a ctypes.Structure takes 3 us to fill).
 LINEAR_ARGS = struct.Struct("@3Q3QQQ2Q2Q6I")     # xksv_linear_args
@@ -114,6 +121,8 @@ _SIGS = {
     "xksv_plan_linear": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p,
                           ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p], ctypes.c_int),
     "xksv_kv_create": ([ctypes.POINTER(KvDesc), ctypes.POINTER(ctypes.c_void_p)], ctypes.c_int),
+    "xksv_kv_create_blocks": ([ctypes.POINTER(KvDesc), ctypes.POINTER(KvBlocks), ctypes.POINTER(ctypes.c_void_p)],
+                              ctypes.c_int),
     "xksv_kv_destroy": ([ctypes.c_void_p], None),
     "xksv_kv_status": ([ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
     "xksv_kv_append": ([ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
@@ -125,7 +134,7 @@ _SIGS = {
 }
 
 # element types and activations of the linear layer and the key/value cache
-BF16, FP16, FP32, E4M3 = 1, 2, 3, 4
+BF16, FP16, FP32, E4M3, INT8 = 1, 2, 3, 4, 5
 ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 KV_INTERLEAVED = 1
 
@@ -293,7 +302,8 @@ def _torch_types():
     global _i32
     import torch
     _i32 = torch.int32
-    _types.update({torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32, torch.float8_e4m3fn: E4M3})
+    _types.update({torch.bfloat16: BF16, torch.float16: FP16, torch.float32: FP32, torch.float8_e4m3fn: E4M3,
+                   torch.int8: INT8})
 
 
 def _matrix(t, rows, cols, what, device):
@@ -500,7 +510,10 @@ class KVCache:
     """A paged key/value cache over two torch tensors (xksv_kv_*): k and v are
     [pages, page_size, heads, dim] (layout "nhd") or [pages, heads, page_size,
     dim] ("hnd") of BF16, FP16 or float8_e4m3fn, any strides that are
-    multiples of 16 bytes; k_scale and v_scale are FP32 [heads] for float8.
+    multiples of 16 bytes.  For float8, k_scale and v_scale are FP32 [heads], set by the
+    caller and only read; or, for float8 or int8, FP32 [pages, blocks, heads] of
+    any strides, one for each page_size / blocks tokens and head: append sets those
+    (xksv_kv_create_blocks), and attend reads them.
     A page table is an int32 [sequences, pages] tensor of page numbers."""
 
     def __init__(self, k, v, k_scale=None, v_scale=None, layout="nhd", lib=None):
@@ -514,25 +527,41 @@ class KVCache:
         self.lib = lib or load()
         self.handle = None
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device, self.index, self.type = k.device, k.get_device(), _type(k, (BF16, FP16, E4M3), "k")
+        blocked = k_scale is not None and k_scale.dim() == 3
+        self.device, self.index = k.device, k.get_device()
+        self.type = _type(k, (E4M3, INT8) if blocked else (BF16, FP16, E4M3), "k")
         order = (0, 1, 2) if layout == "nhd" else (0, 2, 1)  # page, token, head
         self.pages, self.page_size, self.kv_heads = (k.shape[i] for i in order)
         self.head_dim = k.shape[3]
+        if blocked:
+            blocks = k_scale.shape[1]
+            for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+                if (s is None or s.dtype != torch.float32 or tuple(s.shape) != (self.pages, blocks, self.kv_heads)
+                        or s.device != self.device or not blocks or self.page_size % blocks):
+                    raise ValueError(f"{name}: an FP32 [{self.pages}, blocks, {self.kv_heads}] tensor on {self.device} "
+                                     f"whose blocks divide {self.page_size} is needed")
         for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-            if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (self.kv_heads,)
-                                  or not s.is_contiguous() or s.device != self.device):
+            if not blocked and s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (self.kv_heads,)
+                                                  or not s.is_contiguous() or s.device != self.device):
                 raise ValueError(f"{name}: a contiguous FP32 [{self.kv_heads}] tensor on {self.device} is needed")
-        nbytes = [(t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()) for t in (k, v)]
-        d = KvDesc(k.data_ptr(), v.data_ptr(), nbytes[0], nbytes[1], self.pages, self.page_size)
+        behind = lambda t: t.untyped_storage().nbytes() - t.storage_offset() * t.element_size()
+        d = KvDesc(k.data_ptr(), v.data_ptr(), behind(k), behind(v), self.pages, self.page_size)
         d.k_stride[:] = [k.stride(i) for i in order]
         d.v_stride[:] = [v.stride(i) for i in order]
-        d.k_scale = k_scale.data_ptr() if k_scale is not None else None
-        d.v_scale = v_scale.data_ptr() if v_scale is not None else None
+        if not blocked:
+            d.k_scale = k_scale.data_ptr() if k_scale is not None else None
+            d.v_scale = v_scale.data_ptr() if v_scale is not None else None
         d.kv_heads, d.head_dim, d.type = self.kv_heads, self.head_dim, self.type
         h = ctypes.c_void_p()
         with torch.cuda.device(self.device):
-            if self.lib.xksv_kv_create(ctypes.byref(d), ctypes.byref(h)):
-                raise ValueError("xksv_kv_create rejected the cache")
+            if blocked:
+                b = KvBlocks(k_scale.data_ptr(), v_scale.data_ptr(), behind(k_scale), behind(v_scale), self.page_size // blocks)
+                b.k_stride[:], b.v_stride[:] = k_scale.stride(), v_scale.stride()
+                refused = self.lib.xksv_kv_create_blocks(ctypes.byref(d), ctypes.byref(b), ctypes.byref(h))
+            else:
+                refused = self.lib.xksv_kv_create(ctypes.byref(d), ctypes.byref(h))
+            if refused:
+                raise ValueError(f"xksv_kv_create{'_blocks' if blocked else ''} rejected the cache")
         self.handle = h
 
     def append(self, k, v, table, index, seq=None, positions=None, inv_freq=None, rot_scale=1.0, interleaved=False,
@@ -542,7 +571,9 @@ class KVCache:
         query heads, dim] of one dtype; token t is token index[t] of sequence
         seq[t] (default t; negative: padding, skipped), rotated by positions[t]
         (default index[t]) and inv_freq FP32 [rotated dims / 2] (None: no
-        rotation).  q_out defaults to q, in place."""
+        rotation).  q_out defaults to q, in place.  With block scales the tokens
+        of one sequence stand next to each other, their index rising by one; each block's
+        scale rises to what its new elements need, or begins anew with its first place."""
         n, dev, dim = k.shape[0], self.index, self.head_dim
         code = _type(k, (BF16, FP16, FP32), "k")
         kp, k0, k1 = _heads(k, n, self.kv_heads, dim, "k", dev)
@@ -577,7 +608,7 @@ class KVCache:
     def attend(self, q, table, lens, out, lse=None, scale=None, window=0, softcap=0.0, stream=0, workspace=None):
         """Attention of one new token per sequence over its lens[s] cached
         tokens (xksv_kv_attend): q and out [sequences, query heads, dim] of the
-        cache's dtype (BF16 or FP16 over float8), lse FP32 [sequences, query
+        cache's dtype (BF16 or FP16 over float8 and int8), lse FP32 [sequences, query
         heads] or None; scale defaults to dim ** -0.5; window 0 sees the whole
         sequence; softcap 0 is off.  `workspace` (uint8, at least
         attend_workspace(...) bytes) defaults to a new buffer per call."""
