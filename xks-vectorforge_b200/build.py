@@ -16,7 +16,7 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libxksv_cuda.so"
 SOURCES = ["api.cu", "parallel_kernels.cu", "serial_kernels.cu", "raw_kernels.cu", "pack_host.cpp", "noalloc.cu",
            "tp.cpp", "tc_gemm.cu", "fused_gemm.cu", "sha256.cu", "pack_gpu.cu",
-           "linear.cu", "linear_gemm.cu", "kv_cache.cu", "kv_attend.cu", "kv_blocks.cu", "sample.cu"]
+           "linear.cu", "linear_gemm.cu", "kv_cache.cu", "kv_attend.cu", "kv_attend_blocks.cu", "kv_blocks.cu", "sample.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -44,5 +44,6 @@ struct AttendPlan {
 };
 AttendPlan kv_attend_plan(const xksv_kv_desc& c, const xksv_kv_blocks& b, uint64_t seqs, uint32_t q_heads, uint64_t table_cols, int sms);
 cudaError_t launch_kv_attend(const AttendArgs& p, const AttendPlan& plan, cudaStream_t st);
+cudaError_t launch_kv_attend_blocks(const AttendArgs& p, const AttendPlan& plan, cudaStream_t st);
 
 }  // namespace xksv
