@@ -22,6 +22,7 @@ namespace {
 constexpr int BTH = 128;        // threads of a CTA
 constexpr uint32_t kTile = 16;  // tokens whose angles lie in shared memory at a time
 constexpr uint32_t kHeads = 64; // KV heads of a CTA at most
+constexpr uint64_t kFew = 512;  // tokens, up to which one kernel does all
 
 struct I8 {
   int8_t b;
@@ -54,15 +55,35 @@ __device__ __forceinline__ void spread(const Eight<E4m3>& a, float* x) {
   }
 }
 template <class TC>
-struct Top;
+constexpr bool kInteger = false;
 template <>
-struct Top<E4m3> {
-  static constexpr bool kInt = false;
-};
-template <>
-struct Top<I8> {
-  static constexpr bool kInt = true;
-};
+constexpr bool kInteger<I8> = true;
+
+// Whether token o, a run's first, breaks the order that a call's tokens have to
+// keep, next to the one before: a sequence's tokens stand together and rise by
+// one.  `begins`: it is its sequence's first, which must not have come before.
+__device__ __forceinline__ bool out_of_order(const xksv_kv_append_args& a, uint64_t o, bool& begins) {
+  begins = false;
+  if (!a.seq || !o) return false;
+  begins = a.seq[o - 1] != a.seq[o];
+  return !begins && int64_t(a.index[o - 1]) + 1 != a.index[o];
+}
+// Whether token o's sequence has come before: this thread's share of all tokens before
+// (many loads at a time: a loop of single ones took longer than all the rest of a
+// prompt's append).
+__device__ __forceinline__ bool came_before(const xksv_kv_append_args& a, uint64_t o) {
+  const int32_t seq = a.seq[o];
+  bool wrong = false;
+  constexpr int kAtOnce = 16;
+  for (uint64_t e = threadIdx.x; e + 1 < o; e += kAtOnce * blockDim.x) {
+    int32_t other[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) other[i] = e + i * blockDim.x + 1 < o ? a.seq[e + i * blockDim.x] : ~seq;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) wrong |= other[i] == seq;
+  }
+  return wrong;
+}
 
 // PIECES: rows of 16-byte pieces, rotated pairs that fill them; else any strides,
 // alignment and rotation, element by element.
@@ -106,15 +127,9 @@ __global__ void __launch_bounds__(BTH, 8) kv_append_blocks_kernel(const AppendBl
     }
     const KvPlace at = kv_place(a.table, a.table_rows, a.table_cols, a.table_stride, p.c.pages, P, seq, index);
     if (y == 0) {
-      bool wrong = at.page < 0 && tid == 0;
-      if (a.seq && t > 0) {
-        // a sequence's tokens stand together and rise by one
-        if (int64_t(a.seq[t - 1]) == seq) {
-          wrong |= int64_t(a.index[t - 1]) + 1 != index;
-        } else {
-          for (uint64_t o = tid; o + 1 < t; o += BTH) wrong |= int64_t(a.seq[o]) == seq;
-        }
-      }
+      bool first;
+      bool wrong = out_of_order(a, t, first) || at.page < 0;
+      if (first && came_before(a, t)) wrong = true;
       if (wrong) atomicOr(p.status, kStatusHeader);
     }
     if (at.page < 0) continue;
@@ -201,7 +216,7 @@ __global__ void __launch_bounds__(BTH, 8) kv_append_blocks_kernel(const AppendBl
           }
         }
         atomicMax(&need[!key][h], __float_as_uint(high));
-        if (Top<TC>::kInt && nan) atomicOr(p.status, kStatusHeader);  // (an integer holds none)
+        if (kInteger<TC> && nan) atomicOr(p.status, kStatusHeader);  // (an integer holds none)
       }
     }
     __syncthreads();
@@ -212,7 +227,7 @@ __global__ void __launch_bounds__(BTH, 8) kv_append_blocks_kernel(const AppendBl
       const uint32_t h = key ? i : i - hn;
       const uint64_t* st = key ? p.b.k_stride : p.b.v_stride;
       float* where = (key ? p.b.k_scale : p.b.v_scale) + uint64_t(at.page) * st[0] + block * st[1] + (h0 + h) * st[2];
-      float now = __int_as_float((kv_scale_exponent(need[!key][h], Top<TC>::kInt) + 127) << 23), less = 1.f;
+      float now = __int_as_float((kv_scale_exponent(need[!key][h], kInteger<TC>) + 127) << 23), less = 1.f;
       if (in) {
         const float had = *where;
         if (had < now)
@@ -332,6 +347,359 @@ __global__ void __launch_bounds__(BTH, 8) kv_append_blocks_kernel(const AppendBl
   }
 }
 
+// ---- many tokens: keys and values by runs, a warp a head (the queries go
+// through the 16-bit caches' kernel) ----
+constexpr int RT = 256;          // threads of a CTA
+constexpr uint32_t kWarps = RT / 32;
+constexpr uint32_t kChunk = 16;  // tokens whose runs a CTA takes
+constexpr uint32_t kSpan = 32;   // tokens of a tile at most
+
+// The magnitudes' largest, as the bits of FP32 numbers (infinity and NaN above all others).
+__device__ __forceinline__ uint32_t largest(const float* x, uint32_t high) {
+#pragma unroll
+  for (int e = 0; e < 8; e += 2)
+    high = __vimax3_u32(high, __float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(x[e + 1]) & 0x7fffffffu);
+  return high;
+}
+// The same with what is no number left out, and whether there was NaN.
+__device__ __forceinline__ uint32_t largest_finite(const float* x, uint32_t high, bool& nan) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t m = __float_as_uint(x[e]) & 0x7fffffffu;
+    nan |= m > 0x7f800000u;
+    high = m < 0x7f800000u ? max(high, m) : high;
+  }
+  return high;
+}
+
+// The largest magnitude of eight stored elements, as such bits: 16-bit ones two
+// at a time, since their bits are ordered as they are.
+__device__ __forceinline__ uint32_t largest(const Eight<__nv_bfloat16>& a) {
+  // (no sign bits: as signed numbers, whose maximum of three is one instruction)
+  const uint32_t m = __vimax3_s16x2(__vimax3_s16x2(a.w[0] & 0x7fff7fffu, a.w[1] & 0x7fff7fffu, a.w[2] & 0x7fff7fffu), a.w[3] & 0x7fff7fffu, 0);
+  return max(m << 16, m & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t largest(const Eight<__half>& a) {
+  // (no sign bits: as signed numbers, whose maximum of three is one instruction)
+  const uint32_t m = __vimax3_s16x2(__vimax3_s16x2(a.w[0] & 0x7fff7fffu, a.w[1] & 0x7fff7fffu, a.w[2] & 0x7fff7fffu), a.w[3] & 0x7fff7fffu, 0);
+  return __float_as_uint(__half2float(__ushort_as_half(uint16_t(max(m & 0xffffu, m >> 16)))));
+}
+__device__ __forceinline__ uint32_t largest(const Eight<float>& a) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, a.w[i] & 0x7fffffffu);
+  return m;
+}
+
+// What the first warp finds for the CTA: the next runs, and their tokens' places.
+struct Tile {
+  uint64_t t;        // first token
+  uint32_t len;      // tokens of the runs (0: no more)
+  uint32_t firsts;   // the runs' first tokens, from t
+  uint32_t good;     // tokens whose page is in the cache
+  uint32_t begin;    // the firsts that begin a sequence
+  uint32_t next;     // where this CTA goes on
+  int32_t page[kSpan];
+  uint32_t place[kSpan];
+};
+
+// A CTA takes the runs that begin among its 16 tokens, of four heads: as many as
+// lie in a tile of 32, or a longer one tile by tile.  Each warp has a head's keys
+// or values: it reads them into registers, all at once and while the CTA computes
+// the tile's angles; then, without a barrier, finds what they need, sets the scales and
+// stores them.
+template <class TI, class TC>
+__global__ void __launch_bounds__(RT, 3) kv_append_runs_kernel(const AppendBlocksArgs p) {
+  extern __shared__ __align__(16) float trig[];  // cosines [kSpan][pairs], then sines
+  __shared__ Tile tile;
+  __shared__ uint32_t need[kWarps][kSpan];                        // a warp's runs: what they need,
+  __shared__ float inverse[kWarps][kSpan], ratio[kWarps][kSpan];  // their scales' inverses and rise
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const xksv_kv_append_args& a = p.a;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t D = p.c.head_dim, rot = a.rot_dim, pairs = rot / 2, B = uint32_t(p.b.block), P = uint32_t(p.c.page_size);
+  const bool inter = a.flags & XKSV_KV_INTERLEAVED;
+  // this CTA's heads
+  const uint32_t y = blockIdx.y, ys = gridDim.y;
+  const uint32_t h0 = uint32_t(uint64_t(p.c.kv_heads) * y / ys), hn = uint32_t(uint64_t(p.c.kv_heads) * (y + 1) / ys) - h0;
+  float *const cs = trig, *const sn = trig + kSpan * pairs;
+  // Lanes of a row: of values one a piece; a key's lane takes both elements of
+  // its pairs, of rotated halves a piece and its partner (`both` such lanes)
+  const uint32_t vper = D / 8, both = inter ? 0 : rot / 16, per = vper - both;
+
+  auto seq_of = [&](uint64_t t) { return a.seq ? int64_t(a.seq[t]) : int64_t(t); };
+  const uint64_t t0 = uint64_t(blockIdx.x) * p.chunk;
+  // the first warp: of the 32 tokens from t0, which begin a run and which go on
+  uint32_t follow = 0, begins = 0;
+  if (warp == 0) {
+    bool live = false, goes = false;
+    if (t0 + lane < a.tokens) {
+      live = seq_of(t0 + lane) >= 0 && a.index[t0 + lane] >= 0;
+      goes = live && kv_follows(a.seq, a.index, t0 + lane, B);
+    }
+    follow = __ballot_sync(0xffffffffu, goes);
+    begins = __ballot_sync(0xffffffffu, live) & ~follow;
+  }
+  auto find_places = [&](uint64_t t, uint32_t n) {  // of the tile's tokens, by the first warp
+    KvPlace w{-1, 0};
+    if (lane < n) {
+      w = kv_place(a.table, a.table_rows, a.table_cols, a.table_stride, p.c.pages, P, seq_of(t + lane), a.index[t + lane]);
+      tile.page[lane] = w.page;
+      tile.place[lane] = w.place;
+    }
+    const uint32_t good = __ballot_sync(0xffffffffu, w.page >= 0);
+    if (lane == 0) tile.good = good;
+    if (lane < n && w.page < 0 && y == 0) atomicOr(p.status, kStatusHeader);
+  };
+  auto find_tile = [&](uint32_t at) {  // the first warp: the runs from token `at` on
+    auto end_of = [&](uint32_t from) {  // of the run that begins at `from` (32: there or later)
+      const uint32_t rest = from < 31 ? ~follow & ~((2u << from) - 1) : 0;
+      return rest ? uint32_t(__ffs(rest)) - 1 : 32u;
+    };
+    const uint32_t starts = at < 32 ? begins & ~((1u << at) - 1) : 0;
+    at = starts ? __ffs(starts) - 1 : 32;
+    if (at >= p.chunk) {
+      if (lane == 0) tile.len = 0;
+      return;
+    }
+    const uint64_t t = t0 + at;
+    uint32_t end = end_of(at), len = end - at, firsts = 1;
+    if (end < 32 && len <= kSpan) {
+      for (uint32_t next; end < p.chunk && (begins >> end & 1) && (next = end_of(end)) < 32 && next - at <= kSpan; end = next)
+        firsts |= 1u << (end - at);
+      len = end - at;
+    } else if (end == 32) {
+      for (uint32_t more = ~0u; more == ~0u; len += more == ~0u ? 32 : __ffs(~more) - 1) {
+        const uint64_t o = t + len + lane;
+        more = __ballot_sync(0xffffffffu, o < a.tokens && kv_follows(a.seq, a.index, o, B));
+      }
+    }
+    find_places(t, min(len, kSpan));
+    bool begin = false;
+    if (y == 0 && lane < kSpan && (firsts >> lane & 1) && out_of_order(a, t + lane, begin)) atomicOr(p.status, kStatusHeader);
+    const uint32_t begin_set = __ballot_sync(0xffffffffu, begin);
+    if (lane == 0) tile.t = t, tile.len = len, tile.firsts = firsts, tile.next = end, tile.begin = begin_set;
+  };
+  auto tile_angles = [&](uint64_t t, uint32_t n) {  // of n tokens from t
+    if (!pairs) return;
+    for (uint32_t k = tid / pairs, f = tid % pairs, at_k = RT / pairs, at_f = RT % pairs; k < n;) {
+      // of rotated halves the pairs 8 j .. 8 j + 3 first, then 8 j + 4 .. 8 j + 7:
+      // a row's lanes read next to each other
+      const uint32_t where = k * pairs + (inter ? f : (f >> 2 & 1) * (pairs / 2) + (f >> 3) * 4 + (f & 3));
+      angle_of(a.positions ? a.positions[t + k] : a.index[t + k], a.inv_freq[f], a.rot_scale, &cs[where], &sn[where]);
+      k += at_k, f += at_f;
+      if (f >= pairs) f -= pairs, ++k;
+    }
+  };
+  auto run_of = [&](uint32_t i) { return tile.len <= kSpan ? 31 - __clz(tile.firsts & ((2u << i) - 1)) : 0; };
+
+  // ---- a head's keys or values, by this warp: lanes that take row `sub` of
+  // `once` at a time, from dim d on ----
+  const uint32_t r = warp, h = h0 + (r < hn ? r : r - hn);
+  const bool key = r < hn, mine = r < 2 * hn;
+  const uint32_t lanes = key ? per : vper, once = 32 / lanes, sub = lane / lanes, c = lane - sub * lanes;
+  const uint32_t d = key && c >= both ? 8 * (c + both) : 8 * c;
+  const bool pair = key && c < both, idle = !mine || sub >= once;
+  const uint64_t from_step = key ? a.k_stride[0] : a.v_stride[0];
+  const TI* const from = static_cast<const TI*>(key ? a.k : a.v) + h * (key ? a.k_stride[1] : a.v_stride[1]) + d;
+  const uint64_t to_page = key ? p.c.k_stride[0] : p.c.v_stride[0], to_place = key ? p.c.k_stride[1] : p.c.v_stride[1];
+  TC* const to = static_cast<TC*>(key ? p.c.k : p.c.v) + h * (key ? p.c.k_stride[2] : p.c.v_stride[2]) + d;
+  constexpr uint32_t kRaw = sizeof(TI) == 4 ? 4 : 8;  // pieces a lane holds: a key's with their partners
+  const uint32_t batch = (key ? kRaw / 2 : kRaw) * once;
+  Eight<TI> raw[kRaw];
+  // the batch's rows of the tile's n tokens from t
+  auto fetch = [&](uint64_t t, uint32_t n, uint32_t b0) {
+    if (idle) return;
+    const TI* row = from + (t + b0 + sub) * from_step;
+    if (key) {
+#pragma unroll
+      for (uint32_t z = 0; z < kRaw / 2; ++z, row += once * from_step)
+        if (b0 + sub + z * once < n) {
+          raw[2 * z] = *reinterpret_cast<const Eight<TI>*>(row);
+          if (pair) raw[2 * z + 1] = *reinterpret_cast<const Eight<TI>*>(row + pairs);
+        }
+    } else {
+#pragma unroll
+      for (uint32_t z = 0; z < kRaw; ++z, row += once * from_step)
+        if (b0 + sub + z * once < n) raw[z] = *reinterpret_cast<const Eight<TI>*>(row);
+    }
+  };
+  uint32_t high = 0;  // what a single run needs so far
+  auto note = [&](uint32_t i, uint32_t m, auto again) {
+    if (m >= 0x7f800000u) {  // an infinite element saturates, and an integer holds no NaN
+      bool nan = false;
+      m = again(nan);
+      if (kInteger<TC> && nan && tile.good >> i & 1) atomicOr(p.status, kStatusHeader);
+    }
+    if (tile.firsts == 1)
+      high = max(high, m);
+    else
+      atomicMax(&need[warp][run_of(i)], m);
+  };
+  auto held = [&](TC* at, float f, float* x) {
+    if (f > 0.f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] *= f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __fdiv_rn(x[e], -f);
+    }
+    Eight<TC> e;
+    gather(x, e);
+    *reinterpret_cast<Eight<TC>*>(at) = e;
+  };
+  // the batch: what it needs, or, `put`, into its places
+  auto work = [&](uint32_t n, uint32_t b0, bool put) {
+    if (idle) return;
+    if (key) {
+#pragma unroll
+      for (uint32_t z = 0; z < kRaw / 2; ++z) {
+        const uint32_t i = b0 + sub + z * once;
+        if (i >= n) break;
+        float x[8], o[8];
+        spread(raw[2 * z], x);
+        const float *co = cs + i * pairs, *si = sn + i * pairs;
+        if (pair) {
+          spread(raw[2 * z + 1], o);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const uint32_t at = g * (pairs / 2) + 4 * c;
+            const float4 c4 = *reinterpret_cast<const float4*>(co + at), s4 = *reinterpret_cast<const float4*>(si + at);
+            const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float l = x[4 * g + j], w = o[4 * g + j];
+              x[4 * g + j] = l * cc[j] - w * ss[j];
+              o[4 * g + j] = w * cc[j] + l * ss[j];
+            }
+          }
+        } else if (inter && d < rot) {
+          const float4 c4 = *reinterpret_cast<const float4*>(co + 4 * c), s4 = *reinterpret_cast<const float4*>(si + 4 * c);
+          const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float l = x[2 * j], w = x[2 * j + 1];
+            x[2 * j] = l * cc[j] - w * ss[j];
+            x[2 * j + 1] = w * cc[j] + l * ss[j];
+          }
+        }
+        if (!put) {
+          note(i, pair ? largest(o, largest(x, 0)) : largest(x, 0), [&](bool& nan) {
+            const uint32_t m = largest_finite(x, 0, nan);
+            return pair ? largest_finite(o, m, nan) : m;
+          });
+        } else if (tile.good >> i & 1) {
+          const float f = inverse[warp][run_of(i)];
+          TC* at = to + uint64_t(tile.page[i]) * to_page + tile.place[i] * to_place;
+          held(at, f, x);
+          if (pair) held(at + pairs, f, o);
+        }
+      }
+    } else {
+#pragma unroll
+      for (uint32_t z = 0; z < kRaw; ++z) {
+        const uint32_t i = b0 + sub + z * once;
+        if (i >= n) break;
+        if (!put) {
+          note(i, largest(raw[z]), [&](bool& nan) {
+            float x[8];
+            spread(raw[z], x);
+            return largest_finite(x, 0, nan);
+          });
+        } else if (tile.good >> i & 1) {
+          float x[8];
+          spread(raw[z], x);
+          held(to + uint64_t(tile.page[i]) * to_page + tile.place[i] * to_place, inverse[warp][run_of(i)], x);
+        }
+      }
+    }
+  };
+  // the runs' scales (lane: the run's first token), and where they rise the
+  // blocks' earlier elements
+  auto set_scales = [&] {
+    if (tile.firsts == 1) {
+      high = __reduce_max_sync(0xffffffffu, high);
+      if (lane == 0) need[warp][0] = high;
+    }
+    __syncwarp();
+    const uint64_t* st = key ? p.b.k_stride : p.b.v_stride;
+    bool risen = false;
+    if (lane < kSpan && (tile.firsts >> lane & 1) && tile.page[lane] >= 0) {
+      float* where = (key ? p.b.k_scale : p.b.v_scale) + uint64_t(tile.page[lane]) * st[0] + tile.place[lane] / B * st[1] + h * st[2];
+      float now = __int_as_float((kv_scale_exponent(need[warp][lane], kInteger<TC>) + 127) << 23), less = 1.f;
+      if (tile.place[lane] % B) {
+        const float had = *where;
+        if (had < now)
+          less = had / now;
+        else if (had >= now)  // (not NaN)
+          now = had;
+      }
+      *where = now;
+      // a power of two's inverse is exact; another scale divides
+      inverse[warp][lane] = (__float_as_uint(now) & 0x7fffffu) == 0 ? 1.f / now : -now;
+      ratio[warp][lane] = less;
+      risen = less != 1.f;
+    }
+    uint32_t some = __ballot_sync(0xffffffffu, risen);
+    __syncwarp();
+    const uint32_t v_once = 32 / vper, v_sub = lane / vper;
+    for (; some; some &= some - 1) {
+      const uint32_t i = __ffs(some) - 1, in = tile.place[i] % B;
+      const float less = ratio[warp][i];
+      for (uint32_t j = v_sub < v_once ? v_sub : ~0u; j < in; j += v_once) {
+        TC* at = to - d + 8 * (lane - v_sub * vper) + uint64_t(tile.page[i]) * to_page + (tile.place[i] - in + j) * to_place;
+        Eight<TC> e = *reinterpret_cast<const Eight<TC>*>(at);
+        float x[8];
+        spread(e, x);
+#pragma unroll
+        for (int z = 0; z < 8; ++z) x[z] *= less;
+        gather(x, e);
+        *reinterpret_cast<Eight<TC>*>(at) = e;
+      }
+    }
+  };
+  for (uint32_t at = 0;; at = tile.next) {
+    __syncthreads();
+    if (warp == 0) find_tile(at);
+    __syncthreads();
+    const uint32_t len = tile.len;
+    if (!len) return;
+    const uint64_t t = tile.t;
+    high = 0;
+    if (lane < kSpan) need[warp][lane] = 0;
+    const bool small = len <= kSpan;
+    for (int put = 0; put < 2; ++put) {
+      for (uint32_t i0 = 0; i0 < len; i0 += kSpan) {
+        const uint32_t n = min(kSpan, len - i0);
+        const bool again = put && small;  // (the tile is as it was)
+        if (!again || n > batch) fetch(t + i0, n, 0);
+        if (!again) {
+          if (!small) {
+            __syncthreads();
+            if (warp == 0) find_places(t + i0, n);
+          }
+          tile_angles(t + i0, n);
+          __syncthreads();
+        }
+        for (uint32_t b0 = 0; b0 < n; b0 += batch) {
+          if (b0) fetch(t + i0, n, b0);
+          work(n, b0, put);
+        }
+      }
+      if (put) break;
+      for (uint32_t f = tile.begin; f; f &= f - 1)
+        if (came_before(a, t + __ffs(f) - 1)) atomicOr(p.status, kStatusHeader);
+      if (!small) {
+        __syncthreads();
+        if (warp == 0) find_places(t, kSpan);
+        __syncthreads();
+      }
+      if (mine) set_scales();
+    }
+  }
+}
+
 template <class TI, class TC>
 cudaError_t append_launch(const AppendBlocksArgs& given, int sms, cudaStream_t st) {
   AppendBlocksArgs p = given;
@@ -341,11 +709,33 @@ cudaError_t append_launch(const AppendBlocksArgs& given, int sms, cudaStream_t s
   const bool pieces = p.a.rot_dim % (p.a.flags & XKSV_KV_INTERLEAVED ? 8 : 16) == 0 && whole(p.a.k, p.a.k_stride) &&
                       whole(p.a.v, p.a.v_stride) &&
                       (!p.a.q || (whole(p.a.q, p.a.q_stride) && whole(p.a.q_out, p.a.q_out_stride)));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  const uint64_t room = 6 * uint64_t(sms);
+  if (pieces && p.a.tokens > kFew) {
+    if (p.a.q) {
+      AppendArgs q{p.a, p.c, p.status};
+      q.c.kv_heads = 0;
+      const cudaError_t e = launch_kv_append(q, sms, st);
+      if (e != cudaSuccess) return e;
+    }
+    p.chunk = kChunk;
+    const uint64_t tiles = (p.a.tokens + kChunk - 1) / kChunk, splits = (p.c.kv_heads + kWarps / 2 - 1) / (kWarps / 2);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(uint32_t(tiles), uint32_t(splits));
+    cfg.blockDim = dim3(RT);
+    cfg.dynamicSmemBytes = kSpan * p.a.rot_dim * sizeof(float);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv_append_runs_kernel<TI, TC>, p);
+  }
   // few tokens: each its own CTA (a run's first one works); else as many as a
   // block has, up to a tile.  The heads are split where there are fewer runs
   // than the GPU holds CTAs.
-  p.chunk = p.a.tokens <= 512 ? 1 : uint32_t(std::min<uint64_t>(kTile, p.b.block));
-  const uint64_t runs = (p.a.tokens + p.b.block - 1) / p.b.block, room = 6 * uint64_t(sms);
+  p.chunk = p.a.tokens <= kFew ? 1 : uint32_t(std::min<uint64_t>(kTile, p.b.block));
+  const uint64_t runs = (p.a.tokens + p.b.block - 1) / p.b.block;
   uint64_t splits = std::max<uint64_t>((p.c.kv_heads + kHeads - 1) / kHeads, std::min<uint64_t>(p.c.kv_heads, room / runs));
   splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, 65535));
   cudaLaunchConfig_t cfg = {};
@@ -353,9 +743,6 @@ cudaError_t append_launch(const AppendBlocksArgs& given, int sms, cudaStream_t s
   cfg.blockDim = dim3(BTH);
   cfg.dynamicSmemBytes = kTile * p.a.rot_dim * sizeof(float);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, pieces ? kv_append_blocks_kernel<TI, TC, true> : kv_append_blocks_kernel<TI, TC, false>, p);

@@ -247,7 +247,7 @@ cudaError_t append_launch(const AppendArgs& p, int sms, cudaStream_t st) {
   auto whole = [](const void* ptr, const uint64_t* stride) {  // rows of 16-byte pieces
     return (reinterpret_cast<uintptr_t>(ptr) | stride[0] * sizeof(TI) | stride[1] * sizeof(TI)) % 16 == 0;
   };
-  auto near = [](uint64_t heads, uint64_t stride) { return stride < (1ull << 31) / heads; };
+  auto near = [](uint64_t heads, uint64_t stride) { return stride < (1ull << 31) / std::max<uint64_t>(1, heads); };
   const bool close = near(p.c.kv_heads, p.a.k_stride[1]) && near(p.c.kv_heads, p.a.v_stride[1]) &&
                      near(p.c.kv_heads, p.c.k_stride[2]) && near(p.c.kv_heads, p.c.v_stride[2]) &&
                      (!p.a.q || (near(p.a.q_heads, p.a.q_stride[1]) && near(p.a.q_heads, p.a.q_out_stride[1])));
@@ -325,6 +325,7 @@ bool strides_small(const uint64_t* stride) { return stride[0] < (1ull << 40) && 
 
 }  // namespace
 
+// (kv_heads 0: the queries alone)
 cudaError_t launch_kv_append(const AppendArgs& p, int sms, cudaStream_t st) {
   switch (p.a.type) {
     case XKSV_BF16: return append_cache<__nv_bfloat16>(p, sms, st);
