@@ -3,13 +3,14 @@ key/value cache in pages, one call per token step.
 
 ``load_session(path, device, ...)`` loads an archive with fused layers
 (xksv_runtime.load_archive) and opens a ``PagedSession`` on the model.  The
-session keeps every layer's keys and values in one paged buffer (BF16, or
-float8 with a scale per head), gives sequences pages from a free list, and
-runs the model's modules itself:
+session keeps every layer's keys and values in one paged buffer (BF16, or 8
+bits with a scale per head or per block of tokens and head), gives sequences
+pages from a free list, and runs the model's modules itself:
 
     session = xksv_serve.load_session("model.xksv", "cuda:0", pages=4096)
     seqs, logits = session.prefill([ids_a, ids_b])      # prompts of any lengths
     logits = session.step(seqs, logits.argmax(-1))      # one token each
+    logits = session.step(seqs, session.sample(logits, temperature=0.8, top_p=0.95))
     session.release(seqs)
 
 A step's layer is: the input norm, the q / k / v products (with their biases),
@@ -25,6 +26,7 @@ import xksv_gpu
 from xksv_runtime import fail, load_archive
 
 MODEL_TYPES = ("llama", "mistral", "qwen2")
+KV_DTYPES = ("bf16", "e4m3", "e4m3-blocks", "int8-blocks")
 
 
 def load_session(path, device, verify=True, part_index=True, **session):
@@ -45,16 +47,22 @@ class PagedSession:
     the cache: an element stands for its value times `kv_scale`, a number or a
     tensor that broadcasts to [layers, 2 (keys, values), KV heads].  Keys and
     values beyond 448 kv_scale (28 by default) saturate there, unreported:
-    models with large key or value biases need scales of their own."""
+    models with large key or value biases need scales of their own.
+    "e4m3-blocks" and "int8-blocks" need none: each `kv_block` tokens of a page
+    (default: all of it) and head have a scale that their own elements set
+    (KVCache.append); 4 bytes a block more."""
 
     def __init__(self, model, pages, page_size=16, max_tokens=None, max_seqs=256, kv_dtype="bf16", kv_scale=1.0 / 16,
-                 device=None):
+                 kv_block=None, device=None):
         import torch
         config = model.config
         if config.model_type not in MODEL_TYPES:
             fail(f"paged sessions serve {', '.join(MODEL_TYPES)} models, not {config.model_type}")
-        if kv_dtype not in ("bf16", "e4m3"):
+        if kv_dtype not in KV_DTYPES:
             fail(f"unknown cache dtype {kv_dtype}")
+        blocked = kv_dtype.endswith("-blocks")
+        if kv_block is not None and (not blocked or kv_block < 1 or page_size % kv_block):
+            fail(f"kv_block {kv_block} for pages of {page_size} tokens of {kv_dtype}")
         self.model, self.core, self.config = model, model.model, config
         self.layers = list(self.core.layers)
         self.device = torch.device(device or next(model.parameters()).device)
@@ -67,10 +75,13 @@ class PagedSession:
         self.dim = getattr(config, "head_dim", None) or config.hidden_size // self.heads
         self.windows = [self._window(i) for i in range(len(self.layers))]
         self.page_size, self.max_tokens = page_size, max_tokens or config.max_position_embeddings
-        store = torch.bfloat16 if kv_dtype == "bf16" else torch.float8_e4m3fn
+        store = {"bf16": torch.bfloat16, "int8-blocks": torch.int8}.get(kv_dtype, torch.float8_e4m3fn)
         shape = (len(self.layers), 2, pages, page_size, self.kv_heads, self.dim)
-        self.kv = torch.zeros(shape, dtype=torch.uint8 if kv_dtype == "e4m3" else store, device=self.device).view(store)
+        self.kv = torch.zeros(shape, dtype=torch.bfloat16 if kv_dtype == "bf16" else torch.uint8, device=self.device).view(store)
         scales = [(None, None)] * len(self.layers)
+        self.kv_block = (kv_block or page_size) if blocked else 0
+        if blocked:
+            scales = torch.zeros((len(self.layers), 2, pages, page_size // self.kv_block, self.kv_heads), device=self.device)
         if kv_dtype == "e4m3":
             scale = torch.as_tensor(kv_scale, dtype=torch.float32, device=self.device)
             shape = (len(self.layers), 2, self.kv_heads)
@@ -214,7 +225,7 @@ class PagedSession:
         if c.dtype == dtype:
             return c[page, slot]
         rows = c.view(torch.uint8)[page, slot].view(c.dtype).float()
-        return (rows * scale[:, None]).to(dtype)
+        return (rows * (scale[page, slot // self.kv_block] if self.kv_block else scale)[..., None]).to(dtype)
 
     def _causal(self, q, k, v, window):
         import torch
@@ -232,7 +243,8 @@ class PagedSession:
         """One more token of each sequence (`tokens` [n]); returns the logits [n,
         vocabulary] after it.  Ids outside the vocabulary are refused; ids on
         the device are not waited for: there such a row's logits are NaN.  A
-        step that raises leaves the sequences as they were."""
+        step that raises leaves the sequences as they were (with block scales, to
+        a rounding: the block's scale may have risen)."""
         import torch
         if len(set(seqs)) != len(seqs) or any(s not in self.length for s in seqs):
             fail("step: unknown or repeated sequence")
@@ -270,24 +282,45 @@ class PagedSession:
             logits = self.model.lm_head(self.core.norm(h))
             return logits.masked_fill_((ids != inside)[:, None], float("nan")) if tokens.is_cuda else logits
 
-    def generate(self, prompts, max_new_tokens, eos=None):
-        """Greedy continuations of the prompts: a list of token lists, each ended
-        by `eos` or max_new_tokens."""
+    def sample(self, logits, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, generator=None):
+        """A token for each row of logits (xksv_gpu.sample; the settings are
+        numbers or tensors [rows]), drawn with `generator`'s numbers; token -1
+        for a row without a distribution (NaN)."""
         import torch
+        u = torch.rand(logits.shape[0], generator=generator, device=logits.device)
+        return xksv_gpu.sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, stream=self._stream())
+
+    def generate(self, prompts, max_new_tokens, eos=None, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None):
+        """Continuations of the prompts: a list of token lists, each ended by `eos`
+        or max_new_tokens.  Greedy, or sampled (xksv_gpu.sample) with a
+        temperature above 0; each setting is a number or one for each prompt, and
+        `generator` a torch generator on the session's device."""
+        import torch
+        how = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        for name, v in how.items():
+            if hasattr(v, "__len__"):
+                if len(v) != len(prompts):
+                    fail(f"generate: {len(v)} values of {name} for {len(prompts)} prompts")
+                how[name] = torch.as_tensor(v, dtype=torch.int32 if name == "top_k" else torch.float32).to(self.device)
+        greedy = not torch.is_tensor(how["temperature"]) and how["temperature"] == 0
         seqs, logits = self.prefill(prompts)
         out = [[] for _ in seqs]
         live = list(range(len(seqs)))
         try:
             for k in range(max_new_tokens):
-                token = logits.argmax(-1)
+                token = logits.argmax(-1) if greedy else self.sample(logits, generator=generator, **how)
                 ids = token.tolist()
+                if min(ids) < 0:
+                    fail("generate: a row of logits without a distribution, or a setting outside its range")
                 for i, t in zip(live, ids):
                     out[i].append(t)
                 keep = [j for j, t in enumerate(ids) if t != eos]
                 live = [live[j] for j in keep]
                 if not live or k + 1 == max_new_tokens:
                     break
-                logits = self.step([seqs[i] for i in live], token[torch.tensor(keep, device=self.device)])
+                rows = torch.tensor(keep, device=self.device)
+                how = {n: v[rows] if torch.is_tensor(v) else v for n, v in how.items()}
+                logits = self.step([seqs[i] for i in live], token[rows])
             self._check()
         finally:
             self.release(seqs)
