@@ -559,8 +559,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   // bins: those farther than `beyond`, and none behind the last bin.
   float start = 0.f, beyond = -1.f, per_unit = kPerUnit;
   auto count_it = [&](float z) {
-    const float d = zmax - z, x = (d - start) * per_unit;
-    if (d > beyond && x < float(NB) - 1.5f) atomicAdd(&s.hist[rounded(x)], 1);
+    const float d = zmax - z, x = fminf((d - start) * per_unit, NB - 1.f);
+    atomicAdd(&s.hist[rounded(d > beyond ? x : NB - 1.f)], 1);  // (without a branch: the last bin takes what does not count)
   };
 
   // ---- few candidates: all tokens within `reach` of the largest logit, guessed so
@@ -670,6 +670,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   double passed = 0.0;
   uint32_t klo = 0, khi = 0, passed_n = 0;
   bool whole_list = false;  // this CTA's list still holds its candidates
+  bool ties_in = false;     // `passed` has what is kept of a border of one logit already
   auto select = [&](bool by_weight) {
     const uint32_t k = uint32_t(top_k);
     // The weight of the tokens nearer than `start` is known to fall short where
@@ -905,12 +906,15 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
           uint32_t c[PER], t = 0, owner = ~0u, before = 0;
 #pragma unroll
           for (int i = 0; i < PER; ++i) t += c[i] = lane * PER + i < parts ? s.part_c[now][0][lane * PER + i] : 0;
-          uint32_t run = warp_scan(t, lane) - t;
+          uint32_t run = warp_scan(t, lane) - t, mine = 0;
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
             if (m > run && m - run <= c[i]) owner = lane * PER + i, before = run;
+            if (lane * PER + i == me) mine = m > run ? min(c[i], m - run) : 0;  // of this warp's, that are kept
             run += c[i];
           }
+          if (by_weight && mine) passed += mine * weight(value_of(khi)), passed_n += mine;
+          ties_in = by_weight;
           const uint32_t who = __ballot_sync(0xffffffffu, owner != ~0u);
           if (who) {
             owner = __shfl_sync(0xffffffffu, owner, __ffs(who) - 1);
@@ -984,7 +988,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   const float upto = summed ? value_of(khi) : INFINITY, from = fmaxf(floor_z, border);
   double w = summed ? passed : 0.0;
   uint32_t n = summed ? passed_n : 0;
-  if (summed && whole_list) {
+  if (summed && ties_in) {
+  } else if (summed && whole_list) {
     // each warp takes its own of them; their order is not fixed, so they are
     // added as integers
     uint64_t fixed = 0;
