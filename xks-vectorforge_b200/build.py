@@ -8,6 +8,8 @@ object (include/xksv_cuda.h) that ctypes, cgo or C++ callers load directly.
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -30,16 +32,23 @@ def build(verbose=False, force=False):
     deps = srcs + list(CSRC.glob("*.h")) + list(CSRC.glob("*.cuh")) + [ROOT / "include" / "xksv_cuda.h"]
     if LIB.exists() and not force and all(LIB.stat().st_mtime >= d.stat().st_mtime for d in deps):
         return LIB
-    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-shared", "--threads", "0", "-Xcompiler", "-fPIC,-pthread",
-           "-I", str(ROOT / "include"), "-o", str(LIB) + ".tmp", *map(str, srcs), "-ldl"]
-    if verbose:
-        cmd[1:1] = ["-Xptxas", "-v"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
-        raise RuntimeError("nvcc failed building libxksv_cuda.so")
-    if verbose:
-        sys.stderr.write(r.stderr)
+    # every source by itself, several at a time: the largest take minutes
+    def run(cmd):
+        if verbose:
+            cmd[1:1] = ["-Xptxas", "-v"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            raise RuntimeError("nvcc failed building libxksv_cuda.so")
+        if verbose:
+            sys.stderr.write(r.stderr)
+
+    flags = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-pthread", "-I", str(ROOT / "include")]
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(os.cpu_count()) as pool:
+        objects = [str(Path(tmp) / (s.name + ".o")) for s in srcs]
+        first = sorted(zip(srcs, objects), key=lambda x: "attend" not in x[0].name)  # the longest
+        list(pool.map(lambda x: run([*flags, "-c", "-o", x[1], str(x[0])]), first))
+        run([*flags, "-shared", "-o", str(LIB) + ".tmp", *objects, "-ldl"])
     os.replace(str(LIB) + ".tmp", LIB)
     return LIB
 
