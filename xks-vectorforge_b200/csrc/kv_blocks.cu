@@ -403,11 +403,11 @@ struct Tile {
   uint32_t place[kSpan];
 };
 
-// A CTA takes the runs that begin among its 16 tokens, of four heads: as many as
-// lie in a tile of 32, or a longer one tile by tile.  Each warp has a head's keys
-// or values: it reads them into registers, all at once and while the CTA computes
-// the tile's angles; then, without a barrier, finds what they need, sets the scales and
-// stores them.
+// A CTA takes the runs that begin among its 16 tokens, eight heads' keys or eight
+// heads' values: as many as lie in a tile of 32, or a longer one tile by tile.
+// Each warp has a head: it reads its rows into registers, all at once and, of
+// keys, while the CTA computes the tile's angles; then, without a barrier, finds
+// what they need, sets the scales and stores them.
 template <class TI, class TC>
 __global__ void __launch_bounds__(RT, 3) kv_append_runs_kernel(const AppendBlocksArgs p) {
   extern __shared__ __align__(16) float trig[];  // cosines [kSpan][pairs], then sines
@@ -422,7 +422,9 @@ __global__ void __launch_bounds__(RT, 3) kv_append_runs_kernel(const AppendBlock
   const bool inter = a.flags & XKSV_KV_INTERLEAVED;
   // this CTA's heads
   const uint32_t y = blockIdx.y, ys = gridDim.y;
-  const uint32_t h0 = uint32_t(uint64_t(p.c.kv_heads) * y / ys), hn = uint32_t(uint64_t(p.c.kv_heads) * (y + 1) / ys) - h0;
+  const bool key = y < ys / 2;  // (the others: values)
+  const uint32_t group = key ? y : y - ys / 2, h0 = uint32_t(uint64_t(p.c.kv_heads) * group / (ys / 2));
+  const uint32_t hn = uint32_t(uint64_t(p.c.kv_heads) * (group + 1) / (ys / 2)) - h0;
   float *const cs = trig, *const sn = trig + kSpan * pairs;
   // Lanes of a row: of values one a piece; a key's lane takes both elements of
   // its pairs, of rotated halves a piece and its partner (`both` such lanes)
@@ -482,7 +484,7 @@ __global__ void __launch_bounds__(RT, 3) kv_append_runs_kernel(const AppendBlock
     if (lane == 0) tile.t = t, tile.len = len, tile.firsts = firsts, tile.next = end, tile.begin = begin_set;
   };
   auto tile_angles = [&](uint64_t t, uint32_t n) {  // of n tokens from t
-    if (!pairs) return;
+    if (!key || !pairs) return;
     for (uint32_t k = tid / pairs, f = tid % pairs, at_k = RT / pairs, at_f = RT % pairs; k < n;) {
       // of rotated halves the pairs 8 j .. 8 j + 3 first, then 8 j + 4 .. 8 j + 7:
       // a row's lanes read next to each other
@@ -496,8 +498,8 @@ __global__ void __launch_bounds__(RT, 3) kv_append_runs_kernel(const AppendBlock
 
   // ---- a head's keys or values, by this warp: lanes that take row `sub` of
   // `once` at a time, from dim d on ----
-  const uint32_t r = warp, h = h0 + (r < hn ? r : r - hn);
-  const bool key = r < hn, mine = r < 2 * hn;
+  const uint32_t h = h0 + warp;
+  const bool mine = warp < hn;
   const uint32_t lanes = key ? per : vper, once = 32 / lanes, sub = lane / lanes, c = lane - sub * lanes;
   const uint32_t d = key && c >= both ? 8 * (c + both) : 8 * c;
   const bool pair = key && c < both, idle = !mine || sub >= once;
@@ -721,7 +723,7 @@ cudaError_t append_launch(const AppendBlocksArgs& given, int sms, cudaStream_t s
       if (e != cudaSuccess) return e;
     }
     p.chunk = kChunk;
-    const uint64_t tiles = (p.a.tokens + kChunk - 1) / kChunk, splits = (p.c.kv_heads + kWarps / 2 - 1) / (kWarps / 2);
+    const uint64_t tiles = (p.a.tokens + kChunk - 1) / kChunk, splits = 2 * ((p.c.kv_heads + kWarps - 1) / kWarps);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(uint32_t(tiles), uint32_t(splits));
     cfg.blockDim = dim3(RT);
