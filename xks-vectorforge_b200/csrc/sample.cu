@@ -414,11 +414,11 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     else
       sort_by(n, std::integral_constant<uint32_t, 4>());
   };
-  // The first CTA gathers the candidates of all (their numbers are the
-  // parts' counts `c`) and sorts them.
-  auto gather = [&](const uint32_t* c) {
+  // Where each CTA's candidates begin among all (their numbers are the parts'
+  // counts `c`), and how many there are.
+  auto begins_of = [&](const uint32_t* c, uint32_t* begin) {
     static_assert(NW == 16 && kParts == 128, "four lanes hold a CTA's parts");
-    uint32_t mine = 0, n = 0, begin[kMaxCluster];
+    uint32_t mine = 0, n = 0;
     for (int i = 0; i < 4; ++i) mine += 4 * lane + i < parts ? c[4 * lane + i] : 0;
     mine += __shfl_xor_sync(0xffffffffu, mine, 1);
     mine += __shfl_xor_sync(0xffffffffu, mine, 2);
@@ -427,13 +427,20 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
       begin[r] = n;
       n += __shfl_sync(0xffffffffu, mine, 4 * r);
     }
-    for (uint32_t i = tid; i < n; i += NT) {
-      uint32_t from = 0, at = i;
+    return n;
+  };
+  auto candidate = [&](const uint32_t* begin, uint32_t i) {  // from the list of the CTA that holds it
+    uint32_t from = 0, at = i;
 #pragma unroll
-      for (int r = 1; r < kMaxCluster; ++r)
-        if (r < C && i >= begin[r]) from = r, at = i - begin[r];
-      s.all[i] = pull(&s.list[at], from);
-    }
+    for (int r = 1; r < kMaxCluster; ++r)
+      if (r < C && i >= begin[r]) from = r, at = i - begin[r];
+    return pull(&s.list[at], from);
+  };
+  // The first CTA gathers the candidates of all and sorts them.
+  auto gather = [&](const uint32_t* c) {
+    uint32_t begin[kMaxCluster];
+    const uint32_t n = begins_of(c, begin);
+    for (uint32_t i = tid; i < n; i += NT) s.all[i] = candidate(begin, i);
     if (tid == 0) s.low = 0;
     cluster_sync();  // (the other CTAs wait here before they touch their lists)
     sort_all(n);
@@ -460,6 +467,73 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     }
     __syncthreads();
     return s.low;
+  };
+  // The draw by one warp, where all kept tokens are among up to 64 candidates:
+  // two a lane, sorted in registers, without a barrier (k: top-k's, or n).
+  auto draw_few = [&](const uint32_t* c, uint32_t k, double whole) {
+    uint32_t begin[kMaxCluster];
+    const uint32_t n = begins_of(c, begin);
+    uint64_t x[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) x[e] = 2 * lane + e < n ? candidate(begin, 2 * lane + e) : ~0ull;
+    cluster_arrive();  // (the lists may go)
+#pragma unroll
+    for (uint32_t size = 2; size <= 64; size *= 2) {
+      const bool up = !(2 * lane & size);
+#pragma unroll
+      for (uint32_t far = size / 2; far >= 2; far /= 2) {
+        const bool least = !(2 * lane & far) == up;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint64_t y = __shfl_xor_sync(0xffffffffu, x[e], far / 2);
+          if ((x[e] > y) == least) x[e] = y;
+        }
+      }
+      if ((x[0] > x[1]) == up) {
+        const uint64_t y = x[0];
+        x[0] = x[1], x[1] = y;
+      }
+    }
+    // kept: the first k, while the weight before is short of top-p's share, above min-p's border
+    float z[2];
+    double w[2];
+    uint32_t at[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      at[e] = uint32_t(x[e]);
+      z[e] = value_of(~uint32_t(x[e] >> 32));
+      const bool in = 2 * lane + e < min(n, k);
+      z[e] = in ? z[e] : -INFINITY;
+      w[e] = weight(z[e]);
+    }
+    const double inc = warp_scan(w[0] + w[1], lane);
+    if (by_k) whole = __shfl_sync(0xffffffffu, inc, 31);
+    const double target = by_p ? double(top_p) * whole : INFINITY, before = inc - (w[0] + w[1]);
+    const bool keep0 = z[0] >= floor_z && z[0] > -INFINITY && before < target;
+    const bool keep1 = z[1] >= floor_z && z[1] > -INFINITY && before + w[0] < target;
+    const uint32_t set0 = __ballot_sync(0xffffffffu, keep0), set1 = __ballot_sync(0xffffffffu, keep1);
+    const uint32_t kept = __popc(set0) + __popc(set1);
+    // each kept token's weights up to its own, by index
+    double all = 0.0, sum[2] = {};
+    for (uint32_t j = 0; j < kept; ++j) {
+      const uint32_t other = __shfl_sync(0xffffffffu, j & 1 ? at[1] : at[0], j / 2);
+      const double v = __shfl_sync(0xffffffffu, j & 1 ? w[1] : w[0], j / 2);
+      all += v;
+      if (other <= at[0]) sum[0] += v;
+      if (other <= at[1]) sum[1] += v;
+    }
+    const double goal = fmax(double(u), 0.0) * all;
+    uint32_t first = ~0u, last = 0;
+    if (keep0) first = sum[0] > goal ? at[0] : ~0u, last = at[0];
+    if (keep1) first = sum[1] > goal ? min(first, at[1]) : first, last = max(last, at[1]);
+    first = __reduce_min_sync(0xffffffffu, first);
+    last = __reduce_max_sync(0xffffffffu, last);
+    const uint32_t token = first != ~0u ? first : last;
+    if ((keep0 && at[0] == token) || (keep1 && at[1] == token)) {
+      const float mine = keep0 && at[0] == token ? z[0] : z[1];
+      answer(int64_t(token), int32_t(kept), float((widened(mine) - zm) * cool - log(all)));
+    }
+    cluster_wait();
   };
   // The draw, where all kept tokens are the first CTA's first n sorted ones or
   // fewer: the ones that top-p and min-p leave, ordered by index.
@@ -649,7 +723,12 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         enough = enough && weight_near >= double(top_p) * whole * (1.0 + 1e-12);
       }
       if (enough) {  // all that is kept is among them
-        if (rank == 0) {
+        if (rank == 0 && n <= 64) {
+          if (warp == 0)
+            draw_few(s.part_c[turn][0], by_k ? want : n, whole);
+          else
+            cluster_sync();
+        } else if (rank == 0) {
           gather(s.part_c[turn][0]);
           draw_sorted(by_k ? want : n, whole);
         } else {
