@@ -319,9 +319,13 @@ def test_bad_pages_and_disorder_are_reported():
     for index, seq in (([1, 0, 2, 3, 4], [0, 0, 0, 0, 0]), ([0, 2, 3, 4, 5], [0] * 5), ([0, 1, 0, 2, 3], [0, 0, 1, 0, 0])):
         c.c.append(new, new, table, ints(index), seq=ints(seq), q=q.clone())
         assert c.c.status() == 1
-    # padding between sequences is fine
-    c.c.append(new, new, table, ints([0, 1, 0, 0, 1]), seq=ints([0, 0, -1, 1, 1]))
-    assert c.c.status() == 0
+    # padding between sequences is fine, marked by either, before or behind the tokens
+    for index, seq in (([0, 1, 0, 0, 1], [0, 0, -1, 1, 1]), ([-1, 5, 6, -7, 3], [0, 0, 0, 1, 1]), ([5, 6, -1, 3, -1], [0, 0, 0, 1, 1])):
+        c.c.append(new, new, table, ints(index), seq=ints(seq))
+        assert c.c.status() == 0
+    # but not between a sequence's tokens
+    c.c.append(new, new, table, ints([5, -1, 6, 0, 1]), seq=ints([0, 0, 0, 1, 1]))
+    assert c.c.status() == 1
     c.c.append(new[:0], new[:0], table, ints([]))
     assert c.c.status() == 0
     c.c.close()
@@ -432,6 +436,24 @@ def test_attend_scales_far_apart(block, cache):
     """Scales over a range of 2^20: each token's keys and values by its own."""
     check_attend("bf16", cache, [500, 77], 16, block, 8, 2, 64, "nhd", seed=block, spread=10, odd=True)
     check_attend("bf16", cache, [500, 77], 16, block, 8, 2, 64, "nhd", seed=block, spread=10, wide=700, scale=2.0 ** -14)
+
+
+def test_attend_scales_at_the_ends_of_fp32():
+    """Keys of 2^100 with queries of 2^-100, and values whose scales are near the
+    smallest and the largest numbers."""
+    g = gen(21)
+    table, pages = table_of(g, [40], 16)
+    c = Cache(g, "int8", pages, 16, 16, 1, 64)
+    q = torch.randn(1, 4, 64, generator=g, device=DEV).to(torch.bfloat16) * 2.0 ** -100
+    for k_unit, v_unit in ((2.0 ** 97, 2.0 ** 100), (2.0 ** 97, 2.0 ** -110), (2.0 ** 97, 2.0 ** -140)):
+        c.ks.fill_(k_unit)
+        c.vs.fill_(v_unit)
+        out = torch.empty_like(q)
+        c.c.attend(q, table, ints([40]), out)
+        want, _, tol, _ = attend64(q, c.stands_for("k"), c.stands_for("v"), [40], table, 16, 0.125)
+        # (2^-133: the smallest step of a BF16 result)
+        assert ((out.double() - want).abs() <= half_step("bf16", want) + tol + 2.0 ** -134 + 40 * 2.0 ** -149).all()
+    c.c.close()
 
 
 @pytest.mark.parametrize("lens", [[20000], [3000, 0, 9000, 70, 1]])

@@ -2,12 +2,23 @@
 // tokens and head (include/xksv_cuda.h, part 8).
 //
 // A run is what one call adds to one block: tokens of a sequence that stand
-// next to each other.  A CTA takes whole runs (and a share of the heads, where
-// there are few): it needs a head's largest element of the run before it can
-// store the first, so it goes over the run's keys and values twice, the second time
-// from L1.  Scales are powers of two: a raised scale costs an earlier
-// element at most the bits that fall below its new least one, and an E4M3
-// element none but near zero.
+// next to each other.  A head's elements of a run can only be stored once the
+// largest of them is known.  Scales are powers of two: a raised scale costs an
+// earlier element at most the bits that fall below its new least one, and an
+// E4M3 element none but near zero.
+//   * Up to 512 tokens, and any strides and alignment: a CTA takes runs, whole
+//     (and a share of the heads, where there are few runs), and goes over their
+//     keys and values twice, the second time from L1.  Bound by the chain of
+//     loads: place, page, rows, scale.
+//   * More: the queries go through the 16-bit caches' append kernel, keys and
+//     values by runs, a warp a head, which holds its rows in registers between
+//     the two passes.  Bound by instructions (1.8 a cycle, 24 warps an SM), about twice those
+//     of the 16-bit append's keys and values.
+// Measured on one B200 (a graph of calls): one token of 32 + 8 heads of 128 6.0 us, 200
+// tokens of 28 + 4 heads 8.1, 3001 of 20 + 20 heads of 80 41, 16384 of 32 + 8
+// heads 112 (3290 GB/s; the 16-bit append 71).  All by the first kernel: 16384
+// tokens 159 us; the second with four heads' keys and values a CTA 126, which computes the
+// angles twice; queries in it too 146 (registers spill).
 #include <algorithm>
 
 #include "kernels.h"
@@ -61,11 +72,12 @@ constexpr bool kInteger<I8> = true;
 
 // Whether token o, a run's first, breaks the order that a call's tokens have to
 // keep, next to the one before: a sequence's tokens stand together and rise by
-// one.  `begins`: it is its sequence's first, which must not have come before.
+// one.  `begins`: it is its sequence's first (behind another's or padding), which
+// must not have come before.
 __device__ __forceinline__ bool out_of_order(const xksv_kv_append_args& a, uint64_t o, bool& begins) {
   begins = false;
   if (!a.seq || !o) return false;
-  begins = a.seq[o - 1] != a.seq[o];
+  begins = a.seq[o - 1] != a.seq[o] || a.index[o - 1] < 0;
   return !begins && int64_t(a.index[o - 1]) + 1 != a.index[o];
 }
 // Whether token o's sequence has come before: this thread's share of all tokens before
@@ -80,7 +92,7 @@ __device__ __forceinline__ bool came_before(const xksv_kv_append_args& a, uint64
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) other[i] = e + i * blockDim.x + 1 < o ? a.seq[e + i * blockDim.x] : ~seq;
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) wrong |= other[i] == seq;
+    for (int i = 0; i < kAtOnce; ++i) wrong |= other[i] == seq && a.index[e + i * blockDim.x] >= 0;
   }
   return wrong;
 }

@@ -7,15 +7,31 @@
 // through the kept tokens by index, so nothing is sorted but the few
 // candidates next to the border:
 //   * a cluster of CTAs takes a row and holds it in shared memory: the logits
-//     are read from HBM once;
-//   * a histogram of the distances from the largest logit bounds the border
-//     (counts are exact; a bin's weights are known within its width), further
-//     histograms over the bits of the border's bins narrow it until the
-//     candidates fit a list, which one CTA sorts;
+//     are read from HBM once (a row larger than eight CTAs hold is read again by
+//     every pass);
+//   * few kept tokens: the largest logits of groups of lanes guess a distance
+//     from the largest logit that as many tokens lie within as are wanted, or a few
+//     more; those are gathered, sorted and drawn from by the first CTA, up to 64
+//     of them by one warp without a barrier;
+//   * many: a histogram of the distances says where the border lies, a pass sums
+//     the weights above it, and the tokens next to it are sorted; too many of
+//     them are narrowed by quarters of their bits, and of equal logits the first by
+//     index are counted off;
 //   * weights exp((z - largest) / temperature) and their sums are FP64: FP32
 //     sums of 10^5 weights are off by more than the smaller ones, so that the
 //     border and the drawn token would depend on the order of the additions.
 //     All sums have a fixed order: the same call gives the same tokens.
+//   * the CTAs of a row tell each other their numbers by stores into all the
+//     others' shared memory ahead of a cluster barrier, so that each has all of them after it.
+// Bound: for one row the chain of passes and cluster barriers (1 us each); for
+// many the instructions of the passes, 45 of them an FP64 weight.  Measured on one
+// B200: one row of 32000 BF16 logits, top-k 40 and top-p, 6.4 us; one of
+// 128256 FP32 logits with 98000 tokens in the nucleus 40 us; 77 rows of 32003,
+// each with its own settings, 47 us; 256 rows of 128256 so 167 us (a read of the
+// logits: 10 us).
+// Clusters of 1, 2, 4 and 8 CTAs: 9.2, 8.6, 7.5 and 6.9 us for the first, 177, 90, 51
+// and 39 for the second, 55, 47, 40 and 46 for the third, 593, 160, 172 and 171
+// for the last.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
