@@ -27,11 +27,8 @@
 // many the instructions of the passes, 45 of them an FP64 weight.  Measured on one
 // B200: one row of 32000 BF16 logits, top-k 40 and top-p, 6.4 us; one of
 // 128256 FP32 logits with 98000 tokens in the nucleus 40 us; 77 rows of 32003,
-// each with its own settings, 47 us; 256 rows of 128256 so 167 us (a read of the
+// each with its own settings, 42 us; 256 rows of 128256 so 167 us (a read of the
 // logits: 10 us).
-// Clusters of 1, 2, 4 and 8 CTAs: 9.2, 8.6, 7.5 and 6.9 us for the first, 177, 90, 51
-// and 39 for the second, 55, 47, 40 and 46 for the third, 593, 160, 172 and 171
-// for the last.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -1193,10 +1190,17 @@ cudaError_t launch(const SampleArgs& given, int sms, cudaStream_t st) {
   constexpr uint64_t kOver = (sizeof(Shared) + 15) / 16 * 16, kMost = 227 * 1024;
   const uint64_t row = (p.a.vocab + 16 / sizeof(T)) * sizeof(T);  // and its skew
   auto bytes = [&](uint32_t c) { return kOver + (row / 16 / c + 2) * 16; };
-  // few rows: as many CTAs a row as the GPU has; many rows: as many as let two
-  // CTAs share an SM
+  // Where a row, in eight pieces or fewer, leaves an SM room for two CTAs, no
+  // fewer pieces than that and up to four CTAs an SM; else up to eight.  Clusters of
+  // 1, 2, 4 and 8 CTAs, rows with settings of their own, us: of 32003 BF16 40 rows 60,
+  // 42, 37 and 37; 77 59, 42, 42 and 52; 150 70, 58, 63 and 79; 500 99, 92, 118 and
+  // 185; of 128256 BF16 77 rows 269, 126, 80 and 72; 300 718, 404, 316 and 259; of
+  // 128256 FP32, which do not fit twice, 77 rows 325, 192, 83 and 79; 150 216, 129, 117
+  // and 147; 500 311, 220, 303 and 438.
+  const bool twice = bytes(kMaxCluster) <= kMost / 2;
+  const uint64_t most = uint64_t(sms) * (twice ? 4 : 8);
   uint32_t c = 1;
-  while (c < kMaxCluster && (p.a.rows * c * 2 <= uint64_t(sms) || bytes(c) > kMost / 2)) c *= 2;
+  while (c < kMaxCluster && (p.a.rows * c * 2 <= most || (twice && bytes(c) > kMost / 2))) c *= 2;
   p.cluster = c;
   const bool holds = bytes(c) <= kMost;
   p.held_off = uint32_t(kOver);
