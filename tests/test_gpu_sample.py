@@ -257,3 +257,32 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             xg.sample(**{**dict(logits=z, u=u), **bad})
     assert xg.sample(z[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.parametrize("vocab,rows", [(40009, 3), (40009, 170), (901, 20)])
+@pytest.mark.parametrize("centre,scale,heat", [(0.0, 3.0, 1.0), (0.0, 3e-4, 1e-3), (0.0, 1e-3, 1.0), (0.0, 0.02, 0.01), (-80.0, 20.0, 30.0),
+                                               (300.0, 100.0, 50.0), (-1000.0, 3.0, 1.0), (0.0, 1e30, 1.0), (0.0, 2e5, 1e5), (5.0, 1e-30, 1.0)])
+def test_nucleus_of_bf16_logits_of_any_magnitude(centre, scale, heat, vocab, rows):
+    # logits near zero, far from it and on both sides; zeros and masked tokens among them
+    z = torch.randn((rows, vocab), generator=gen(rows), device=DEV) * scale + centre
+    z[:, 5::11] = -math.inf
+    z[:, 3::13] *= 0.0
+    z[1::2, 0::17] = torch.finfo(torch.bfloat16).min
+    z = z.to(torch.bfloat16)
+    u = unit(rows + 1, rows)
+    zero = torch.exp(-z.float().amax(1) / heat)  # as much as a logit of zero, relative to the largest
+    share = torch.tensor([0.02, 0.3, 0.6, 0.9, 0.999, 0.5], device=DEV).repeat(rows // 6 + 1)[:rows]
+    check(z, u, temperature=heat, top_p=share)
+    check(z, u, temperature=heat, top_p=share, min_p=0.02)
+    check(z, u, temperature=heat, top_p=share, min_p=torch.where(zero < 1, zero, 0.5))
+
+
+def test_nucleus_border_among_equal_logits_is_an_index():
+    # BF16, 40001 tokens of seven logits: whichever CTA holds the border's last token, also at its ends
+    level = torch.tensor([2.0, 1.0, 0.5, 0.0, -0.5, -1.0, -3.0], device=DEV)
+    z = level[torch.randint(0, 7, (1, 40001), generator=gen(4), device=DEV)].to(torch.bfloat16).expand(64, -1)
+    share = torch.linspace(0.01, 0.999, 64, device=DEV)
+    check(z, unit(5, 64), top_p=share)
+    check(z[:8], torch.ones(8, device=DEV) - 2.0 ** -24, top_p=share[::8].contiguous())  # the last kept token
+    # (0.01 in FP32 is 2.2e-10 short of 400 tokens of 40000, which is nearer than MARGIN: one row of the four is not sure)
+    check(torch.zeros((4, 40000), device=DEV, dtype=torch.bfloat16), unit(6, 4), least_sure=0.75, top_p=share[::16].contiguous())

@@ -13,7 +13,9 @@
 //     from the largest logit that as many tokens lie within as are wanted, or a few
 //     more; those are gathered, sorted and drawn from by the first CTA, up to 64
 //     of them by one warp without a barrier;
-//   * many: a histogram of the distances says where the border lies, a pass sums
+//   * many, in BF16: each logit has a bin of its own, so that the bins' weights say where the
+//     border lies and which CTA the draw falls in;
+//   * many else: a histogram of the distances says where the border lies, a pass sums
 //     the weights above it, and the tokens next to it are sorted; too many of
 //     them are narrowed by quarters of their bits, and of equal logits the first by
 //     index are counted off;
@@ -27,7 +29,7 @@
 // many the instructions of the passes, 45 of them an FP64 weight.  Measured on one
 // B200: one row of 32000 BF16 logits, top-k 40 and top-p, 6.4 us; one of
 // 128256 FP32 logits with 98000 tokens in the nucleus 40 us; 77 rows of 32003,
-// each with its own settings, 42 us; 256 rows of 128256 so 167 us (a read of the
+// each with its own settings, 41 us; 256 rows of 128256 so 140 us (a read of the
 // logits: 10 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -53,14 +55,16 @@ constexpr uint32_t kEvery = 8;            // a vector in so many is sampled
 constexpr int kGuessBins = 256;           // bins of the groups' largest logits
 constexpr float kGuessPerUnit = 8.f;
 constexpr int CAP = 2048;                 // candidates that are sorted
+constexpr uint32_t kSide = 2048;          // BF16 magnitudes with a bin of their own: 16 binades
+constexpr uint32_t kLeast = 0x3a80;       // from 2^-10, or higher ones
 constexpr double kTiny = -700.0;          // weights below exp(kTiny) count as zero
 
 struct Shared {
   alignas(16) uint32_t hist[NB];
-  float group[kGroups];
-  uint32_t guess[kGuessBins];
   uint64_t list[CAP];  // this CTA's candidates: ~key, index
-  uint64_t all[CAP];   // of the first CTA: all of them
+  float group[kGroups];
+  uint32_t guess[1024];  // (kGuessBins of them)
+  uint64_t all[CAP];  // of the first CTA: all of them
   double part_w[2][2][kParts];  // of the row's warps, in turn
   uint32_t part_c[2][2][kParts];
   double quarter_w[2][4][kParts];
@@ -71,7 +75,7 @@ struct Shared {
   float best[kParts];
   double pow[16];  // 2^(i / 16)
   double guessed;
-  float spread;
+  float spread[NW];
   uint32_t listed, low, first, found;
   uint32_t ctl[2];
 };
@@ -180,6 +184,11 @@ __device__ __forceinline__ uint4 pull4(const uint32_t* p, uint32_t rank) {
 __device__ __forceinline__ uint64_t pull(const uint64_t* p, uint32_t rank) {
   uint64_t v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];\n" : "=l"(v) : "r"(at_rank(p, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t pull(const uint32_t* p, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(at_rank(p, rank)) : "memory");
   return v;
 }
 __device__ __forceinline__ void min_at(uint32_t* p, uint32_t rank, uint32_t n) {
@@ -608,6 +617,71 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   auto in = [&](uint32_t k, uint32_t i) { return k > bkey || (k == bkey && int32_t(i) <= bidx); };
   double whole = -1.0;  // all tokens' weight, when known
 
+  // Of this warp's tokens that `has` picks, the one that is number `left` by index.
+  auto nth_of = [&](uint32_t left, auto has) {
+    uint32_t got = 0;
+    for (uint32_t v = wv0 + lane; v - lane < wv1; v += 32) {
+      float z[EPV];
+      uint32_t mask = 0;
+      if (v < wv1) {
+        fetch(v, z);
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) mask |= uint32_t(has(z[i], v * EPV + i - skew)) << i;
+      }
+      const uint32_t inc = warp_scan(uint32_t(__popc(mask)), lane), ex = inc - __popc(mask);
+      const bool here = left > ex && left <= inc;
+      if (here) got = v * EPV + __fns(mask, 0, int(left - ex)) - skew;
+      const uint32_t who = __ballot_sync(0xffffffffu, here);
+      if (who) {
+        got = __shfl_sync(0xffffffffu, got, __ffs(who) - 1);
+        break;
+      }
+      left -= __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return got;
+  };
+  // The kept tokens, once the border is known; and the draw by the warp whose
+  // tokens pass the target, `before` being the weight of the warps before it.
+  float border = -INFINITY;
+  auto kept = [&](float z, uint32_t i) { return z >= floor_z && (z > border || (z == border && int32_t(i) <= bidx)); };
+  auto draw_in = [&](double before, double target, double total, uint32_t many) {
+    int32_t token = -1;
+    float z_token = 0.f;
+    for (uint32_t v = wv0 + lane; v - lane < wv1; v += 32) {
+      float z[EPV];
+      double e[EPV], t = 0.0;
+      if (v < wv1) fetch(v, z);
+  #pragma unroll
+      for (int i = 0; i < EPV; ++i) {
+        e[i] = weight(v < wv1 && kept(z[i], v * EPV + i - skew) ? z[i] : -INFINITY);
+        t += e[i];
+      }
+      const double inc = warp_scan(t, lane);
+      // the first lane that passes the target, else the last that keeps any
+      const uint32_t some = __ballot_sync(0xffffffffu, t > 0.0);
+      const uint32_t past = __ballot_sync(0xffffffffu, t > 0.0 && before + inc > target);
+      if (some) {
+        const int who = past ? __ffs(past) - 1 : 31 - __clz(some);
+        int32_t got = -1;
+        float zg = 0.f;
+        if (lane == who) {
+          double c = before + (inc - t);
+          bool done = false;
+  #pragma unroll
+          for (int i = 0; i < EPV; ++i) {
+            c += e[i];
+            if (e[i] > 0.0 && !done) got = int32_t(v * EPV + i - skew), zg = z[i], done = c > target;
+          }
+        }
+        token = __shfl_sync(0xffffffffu, got, who);
+        z_token = __shfl_sync(0xffffffffu, zg, who);
+      }
+      if (past) break;
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) answer(token, int32_t(many), float((widened(z_token) - zm) * cool - log(total)));
+  };
+
   // Every warp finds the first of the 256 or 2048 bins up to which `want` lie;
   // with none, their number.
   auto bin_with = [&](const uint32_t* bins, uint32_t want) {
@@ -650,6 +724,255 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     atomicAdd(&s.hist[rounded(d > beyond ? x : NB - 1.f)], 1);  // (without a branch: the last bin takes what does not count)
   };
 
+  // A distance from the largest logit that as many groups' largest lie within as are
+  // wanted, or a few more; -1 with none.
+  auto near_groups = [&](uint32_t want) {
+    if (tid < kGuessBins) s.guess[tid] = 0;
+    __syncthreads();
+    for (uint32_t i = tid; i < groups; i += NT) {
+      const float x = (zmax - s.group[i]) * kGuessPerUnit;
+      if (x < float(kGuessBins) - 1.5f) atomicAdd(&s.guess[rounded(x)], 1);
+    }
+    __syncthreads();
+    const uint32_t bin = bin_with(s.guess, want);
+    return bin < kGuessBins ? (bin + 0.5f) / kGuessPerUnit : -1.f;  // (a distance of at most that has no later bin)
+  };
+
+  // ---- BF16, top-p without top-k: few distinct logits.  Each has a bin that counts its tokens,
+  // so that a weight is formed once a bin, not once a token; tokens outside the
+  // bins (magnitudes below 16 binades, or above) are weighed one by one.  The bins
+  // tell the whole, the border (all tokens above its logit, and of its own the
+  // first by index) and each CTA's kept weight; the CTA that the draw falls in
+  // weighs its tokens.  Where the border or min-p's bound lies among the tokens
+  // outside the bins, the general form below goes on.  One row of 128256, 99000 tokens
+  // in the nucleus: 23.6 us, the general form 41; 256 such rows 207 and 448.  (Without top-p one pass
+  // weighs all: 14.7 us, and 19.3 by bins.)
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    if (by_p && !by_k) {
+      static_assert(sizeof(s.all) == 2 * kSide * sizeof(uint32_t), "the bins lie where candidates are gathered later");
+      uint32_t* const bins = reinterpret_cast<uint32_t*>(s.all);  // [sign, magnitude]
+      // magnitudes [least, least + kSide): up to 2^6, or to the power of two above the largest logit's
+      const uint32_t end = (__float_as_uint(zmax) >> 16 & 0x7f80u) + 0x80u, least = max(kLeast, end - min(end, kSide));
+      auto bin_z = [&](uint32_t b) { return __uint_as_float(((b / kSide << 15) | (least + b % kSide)) << 16); };
+      const float middle = __uint_as_float(least << 16);  // outside: |z| < middle, and far ones
+      const float weighed = __double2float_ru(double(zmax) + kTiny * double(heat)), reach = near_groups(groups / 4);
+      for (uint32_t i = tid; i < 2 * kSide; i += NT) bins[i] = 0;
+      __syncthreads();
+      double w_mid = 0.0, w_far = 0.0, w_near = 0.0;
+      uint32_t n_mid = 0, n_far = 0, n_near = 0;
+      for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+        const uint4 raw = HELD ? held[v - v0] : read(v);
+        const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+        uint32_t outside = 0;
+#pragma unroll
+        for (int i = 0; i < EPV; ++i) {
+          const uint32_t b = i & 1 ? word[i / 2] >> 16 : word[i / 2] & 0xffffu, m = (b & 0x7fffu) - least;
+          if (m < kSide)
+            atomicAdd(&bins[m + (b >> 15) * kSide], 1);
+          else
+            outside |= 1u << i;
+        }
+        auto z_of = [&](uint32_t i) {
+          const uint32_t x = i < 4 ? (i < 2 ? raw.x : raw.y) : i < 6 ? raw.z : raw.w;
+          return __uint_as_float(i & 1 ? x & 0xffff0000u : x << 16) + 0.f;
+        };
+        for (; outside; outside &= outside - 1) {
+          const float z = z_of(__ffs(outside) - 1);
+          if (z < weighed) continue;
+          const double e = weight(z);
+          if (fabsf(z) < middle)
+            w_mid += e, ++n_mid;
+          else
+            w_far += e, ++n_far;
+        }
+        if (zmax - E::most(raw) <= reach)
+          for (uint32_t i = 0; i < EPV; ++i) {
+            const float z = z_of(i);
+            if (zmax - z > reach) continue;
+            w_near += weight(z), ++n_near;
+            list_it(z, v * EPV + i - skew);
+          }
+      }
+      auto share_q = [&](int i, double x) {
+        x = warp_sum(x);
+        if (lane < C) push(&s.quarter_w[turn][i][me], lane, x);
+      };
+      share_q(0, w_mid), share_q(1, w_far), share_q(2, w_near);
+      share_c(0, n_near), share_c(1, n_far);
+      cluster_sync();
+      const double mid = sum_of(s.quarter_w[turn][0]), far = sum_of(s.quarter_w[turn][1]);
+      const uint32_t near = count_of(s.part_c[turn][0]), fars = count_of(s.part_c[turn][1]);
+      const uint32_t listed = turn;
+      turn ^= 1;
+      // a thread's bins, from the largest logit down: the positive ones, then
+      // the negative ones; each counts in all CTAs
+      const uint32_t some = 2 * kSide / (C * NT), p0 = (rank * NT + tid) * some;
+      auto at = [](uint32_t p) { return p < kSide ? kSide - 1 - p : p; };
+      auto all_of = [&](uint32_t b) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int r = 0; r < kMaxCluster; ++r)
+          if (r < C) n += pull(&bins[b], r);
+        return n;
+      };
+      double t = 0.0;
+      for (uint32_t e = 0; e < some; ++e) {
+        const uint32_t b = at(p0 + e), n = all_of(b);
+        if (n) t += n * weight(bin_z(b));
+      }
+      share_w(0, t);
+      cluster_sync();
+      // every warp finds the row's warp whose bins hold the border
+      constexpr int PER = kParts / 32;
+      double x[PER], sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) sum += x[i] = lane * PER + i < parts ? s.part_w[turn][0][lane * PER + i] : 0.0;
+      const double inc = warp_scan(sum, lane);
+      whole = __shfl_sync(0xffffffffu, inc, 31) + mid + far;
+      turn ^= 1;
+      const double target = double(top_p) * whole;
+      weight_near = sum_of(s.quarter_w[listed][2]);
+      if (near && near <= CAP && weight_near >= target * (1.0 + 1e-12)) {  // all that is kept is among the nearest
+        if (rank == 0 && near <= 64) {
+          if (warp == 0)
+            draw_few(s.part_c[listed][0], near, whole);
+          else
+            cluster_sync();
+        } else if (rank == 0) {
+          gather(s.part_c[listed][0]);
+          draw_sorted(near, whole);
+        } else {
+          cluster_sync();
+        }
+        return;
+      }
+      // (up to the middle as the bins' sums were added: the negative ones' warps are
+      // the upper half)
+      uint32_t owner = ~0u;
+      double run = inc - sum, before = 0.0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t part = lane * PER + i;
+        const double from = run + (part >= parts / 2 ? mid : 0.0);
+        run += x[i];
+        if (owner == ~0u && part < parts && x[i] > 0.0 && from + x[i] >= target) owner = part, before = from;
+      }
+      const uint32_t who = __ballot_sync(0xffffffffu, owner != ~0u);
+      // (in vain where the border or min-p's bound lies among the tokens outside the bins)
+      bool exact = who != 0 && !(min_p > 0.f && ((mid > 0.0 && fabsf(floor_z) < 2 * middle) || (fars && floor_z <= bin_z(2 * kSide - 1))));
+      if (who) {
+        owner = __shfl_sync(0xffffffffu, owner, __ffs(who) - 1);
+        before = __shfl_sync(0xffffffffu, before, __ffs(who) - 1);
+        exact = exact && before < target;
+      }
+      if (exact) {
+        // each CTA finds the border's bin among that warp's, and how many of the
+        // border's own tokens, the first by index, are kept of its own
+        if (warp == 0) {
+          const uint32_t q0 = (owner * 32 + lane) * some;
+          t = 0.0;
+          for (uint32_t e = 0; e < some; ++e) {
+            const uint32_t b = at(q0 + e), n = all_of(b);
+            if (n) t += n * weight(bin_z(b));
+          }
+          const double up = warp_scan(t, lane);
+          const uint32_t first = __ballot_sync(0xffffffffu, t > 0.0 && before + up >= target);
+          const uint32_t last = __ballot_sync(0xffffffffu, t > 0.0);
+          // (by rounding none: the last that has any)
+          if (lane == (first ? __ffs(first) - 1 : 31 - __clz(last))) {
+            double c = before + (up - t), above = c;
+            uint32_t got = 0, ties = 0;
+            for (uint32_t e = 0; e < some; ++e) {
+              const uint32_t b = at(q0 + e), n = all_of(b);
+              if (!n) continue;
+              got = b, ties = n, above = c;
+              c += n * weight(bin_z(b));
+              if (c >= target) break;
+            }
+            const double need = ceil((target - above) / weight(bin_z(got)));
+            uint32_t m = need < 1.0 ? 1u : need > double(ties) ? ties : uint32_t(need);
+            for (uint32_t r = 0; r < rank; ++r) m -= min(m, pull(&bins[got], r));
+            s.found = got, s.ctl[0] = min(m, bins[got]), s.ctl[1] = bins[got];
+          }
+        }
+        __syncthreads();
+        const uint32_t border_bin = s.found, mine = s.ctl[0], ours = s.ctl[1];
+        border = bin_z(border_bin);
+        bidx = mine == ours ? INT32_MAX : -1;
+        const float from = fmaxf(floor_z, border);
+        double w = 0.0;
+        uint32_t n = 0;
+        static_assert(offsetof(Shared, all) == 2 * kSide * sizeof(double), "all that lies ahead of the bins is free by now");
+        double* const weights = reinterpret_cast<double*>(s.hist);  // of the bins' tokens that are kept
+        for (uint32_t b = tid; b < 2 * kSide; b += NT) {
+          const float z = bin_z(b);
+          const uint32_t c = z < from ? 0 : b == border_bin ? mine : bins[b];
+          const double e = c ? weight(z) : 0.0;
+          weights[b] = e;
+          n += c, w += c * e;
+        }
+        if (border < 0.f && floor_z < 0.f) w += w_mid, n += n_mid;  // (those farther away are not kept)
+        share_w(0, w);
+        share_c(0, n);
+        cluster_sync();
+        const uint32_t many = count_of(s.part_c[turn][0]);
+        // the CTA whose weights pass the draw's target, else the last that keeps any
+        double x = 0.0;
+        if (lane < C)
+          for (int y = 0; y < NW; ++y) x += s.part_w[turn][0][lane * NW + y];
+        const double inc = warp_scan(x, lane), total = __shfl_sync(0xffffffffu, inc, 31), goal = fmax(double(u), 0.0) * total;
+        const uint32_t past = __ballot_sync(0xffffffffu, x > 0.0 && inc > goal), any = __ballot_sync(0xffffffffu, x > 0.0);
+        const uint32_t cta = past ? __ffs(past) - 1 : 31 - __clz(any);
+        if (rank != cta) return;
+        double before = __shfl_sync(0xffffffffu, inc - x, cta);
+        if (mine != ours && mine) {  // the index of the last of the border's
+          uint32_t c = 0;
+          for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+            float z[EPV];
+            fetch(v, z);
+#pragma unroll
+            for (int i = 0; i < EPV; ++i) c += z[i] == border;
+          }
+          c = __reduce_add_sync(0xffffffffu, c);
+          if (lane == 0) s.scan_c[warp] = c;
+          __syncthreads();
+          uint32_t run = 0;
+          for (uint32_t y = 0; y < warp; ++y) run += s.scan_c[y];
+          if (mine > run && mine - run <= c) {
+            const uint32_t i = nth_of(mine - run, [&](float z, uint32_t) { return z == border; });
+            if (lane == 0) s.found = i;
+          }
+          __syncthreads();
+          bidx = int32_t(s.found);
+        }
+        w = 0.0;
+        for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+          float z[EPV];
+          fetch(v, z);
+#pragma unroll
+          for (int i = 0; i < EPV; ++i) {
+            const uint32_t b = __float_as_uint(z[i]) >> 16, m = (b & 0x7fffu) - least;
+            if (m < kSide) {
+              if (z[i] != border || int32_t(v * EPV + i - skew) <= bidx) w += weights[m + (b >> 15) * kSide];
+            } else if (kept(z[i], 0)) {
+              w += weight(z[i]);
+            }
+          }
+        }
+        w = warp_sum(w);
+        if (lane == 0) s.scan_w[warp] = w;
+        __syncthreads();
+        const double part = lane < NW ? s.scan_w[lane] : 0.0, to = before + warp_scan(part, lane);
+        const uint32_t over = __ballot_sync(0xffffffffu, part > 0.0 && to > goal), some = __ballot_sync(0xffffffffu, part > 0.0);
+        const uint32_t owner = over ? __ffs(over) - 1 : 31 - __clz(some);
+        before = over ? __shfl_sync(0xffffffffu, to - part, owner) : -INFINITY;  // (no token passes: the last one)
+        if (warp == owner) draw_in(before, goal, total, many);
+        return;
+      }
+      border = -INFINITY, bidx = -1;
+      if (tid == 0) s.listed = 0;
+    }
+
   // ---- few candidates: all tokens within `reach` of the largest logit, guessed so
   // that they are as many as are kept or a few more.  Up to three quarters of
   // the groups: `want` groups have a token as near as the farthest of
@@ -658,15 +981,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     float reach = -1.f;
     const uint32_t want = by_k ? uint32_t(top_k) : groups / 4;
     if (want <= 3 * groups / 4) {
-      if (tid < kGuessBins) s.guess[tid] = 0;
-      __syncthreads();
-      for (uint32_t i = tid; i < groups; i += NT) {
-        const float x = (zmax - s.group[i]) * kGuessPerUnit;
-        if (x < float(kGuessBins) - 1.5f) atomicAdd(&s.guess[rounded(x)], 1);
-      }
-      __syncthreads();
-      const uint32_t bin = bin_with(s.guess, want);
-      if (bin < kGuessBins) reach = (bin + 0.5f) / kGuessPerUnit;  // (a distance of at most that has no later bin)
+      reach = near_groups(want);
     } else {
       for (uint32_t i = tid; i < NB; i += NT) s.hist[i] = 0;
       __syncthreads();
@@ -812,16 +1127,17 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         if (tid == 0) s.low = NB, s.found = NB;
         if (by_weight) {
           double x[4], t = 0.0;
-          if (tid == 0) s.spread = 0.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) t += x[i] = h[i] ? h[i] * weight(zmax - start - (tid * 4 + i) / per_unit) : 0.0;
           double run = known + (cta_scan(t, s.scan_w) - t);
           // four standard deviations, were the bins' weights off by even chances
           // of up to half a bin
           const float squares = warp_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-          if (lane == 0) atomicAdd(&s.spread, squares);
+          if (lane == 0) s.spread[warp] = squares;
           __syncthreads();
-          const double slack = 4 * 0.2887 * cool / per_unit * sqrtf(s.spread) + 1e-7 * target, goal = target + astray;
+          float spread = 0.f;
+          for (int y = 0; y < NW; ++y) spread += s.spread[y];
+          const double slack = 4 * 0.2887 * cool / per_unit * sqrtf(spread) + 1e-7 * target, goal = target + astray;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             run += x[i];
@@ -1012,25 +1328,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
             owner = __shfl_sync(0xffffffffu, owner, __ffs(who) - 1);
             before = __shfl_sync(0xffffffffu, before, __ffs(who) - 1);
             if (me == owner) {
-              uint32_t left = m - before;
-              for (uint32_t v = wv0 + lane; v - lane < wv1; v += 32) {
-                float z[EPV];
-                uint32_t mask = 0;
-                if (v < wv1) {
-                  fetch(v, z);
-#pragma unroll
-                  for (int i = 0; i < EPV; ++i)
-                    mask |= uint32_t(key_of(z[i]) == khi && in(khi, v * EPV + i - skew)) << i;
-                }
-                const uint32_t inc = warp_scan(uint32_t(__popc(mask)), lane), ex = inc - __popc(mask);
-                if (left > ex && left <= inc) {
-                  const uint32_t at = v * EPV + __fns(mask, 0, int(left - ex)) - skew;
-                  for (uint32_t r = 0; r < C; ++r) push(&s.found, r, at);
-                }
-                const uint32_t got = __shfl_sync(0xffffffffu, inc, 31);
-                if (left <= got) break;
-                left -= got;
-              }
+              const uint32_t at = nth_of(m - before, [&](float z, uint32_t i) { return key_of(z) == khi && in(khi, i); });
+              if (lane < C) push(&s.found, lane, at);
             }
           }
           cluster_sync();
@@ -1074,8 +1373,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   // ---- the kept tokens' weights, and the draw by index.  Where top-p was the
   // last cut and min-p leaves all of them, the weights above its candidates
   // have been summed already.
-  const float border = value_of(bkey);
-  auto kept = [&](float z, uint32_t i) { return z >= floor_z && (z > border || (z == border && int32_t(i) <= bidx)); };
+  border = value_of(bkey);
   const bool summed = by_p && floor_z <= value_of(klo);
   const float upto = summed ? value_of(khi) : INFINITY, from = fmaxf(floor_z, border);
   double w = summed ? passed : 0.0;
@@ -1147,41 +1445,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     before = -INFINITY;  // (no token of it passes: its last one)
   }
   if (me != owner) return;
-  int32_t token = -1;
-  float z_token = 0.f;
-  for (uint32_t v = wv0 + lane; v - lane < wv1; v += 32) {
-    float z[EPV];
-    double e[EPV], t = 0.0;
-    if (v < wv1) fetch(v, z);
-#pragma unroll
-    for (int i = 0; i < EPV; ++i) {
-      e[i] = weight(v < wv1 && kept(z[i], v * EPV + i - skew) ? z[i] : -INFINITY);
-      t += e[i];
-    }
-    const double inc = warp_scan(t, lane);
-    // the first lane that passes the target, else the last that keeps any
-    const uint32_t some = __ballot_sync(0xffffffffu, t > 0.0);
-    const uint32_t past = __ballot_sync(0xffffffffu, t > 0.0 && before + inc > target);
-    if (some) {
-      const int who = past ? __ffs(past) - 1 : 31 - __clz(some);
-      int32_t got = -1;
-      float zg = 0.f;
-      if (lane == who) {
-        double c = before + (inc - t);
-        bool done = false;
-#pragma unroll
-        for (int i = 0; i < EPV; ++i) {
-          c += e[i];
-          if (e[i] > 0.0 && !done) got = int32_t(v * EPV + i - skew), zg = z[i], done = c > target;
-        }
-      }
-      token = __shfl_sync(0xffffffffu, got, who);
-      z_token = __shfl_sync(0xffffffffu, zg, who);
-    }
-    if (past) break;
-    before += __shfl_sync(0xffffffffu, inc, 31);
-  }
-  if (lane == 0) answer(token, int32_t(many), float((widened(z_token) - zm) * cool - log(total)));
+  draw_in(before, target, total, many);
 }
 
 template <class T>
