@@ -29,7 +29,7 @@
 // many the instructions of the passes, 45 of them an FP64 weight.  Measured on one
 // B200: one row of 32000 BF16 logits, top-k 40 and top-p, 6.4 us; one of
 // 128256 FP32 logits with 98000 tokens in the nucleus 40 us; 77 rows of 32003,
-// each with its own settings, 41 us; 256 rows of 128256 so 140 us (a read of the
+// each with its own settings, 41 us; 256 rows of 128256 so 128 us (a read of the
 // logits: 10 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -239,8 +239,6 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   const float min_p = p.a.min_p ? p.a.min_p[row] : p.a.min_p_all;
   const float u = p.a.u[row];
   const bool sane = (heat == 0.f || (heat >= kSampleColdest && heat <= kSampleHottest)) && top_p == top_p && min_p == min_p && u == u;
-  if (tid < 16) s.pow[tid] = exp2(tid / 16.0);
-  if (tid == 0) s.listed = 0, s.first = ~0u;
 
   // ---- the row's 16-byte vectors; its first element is element `skew` of
   // the first vector; this warp's vectors [wv0, wv1)
@@ -251,8 +249,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   const uint32_t per = (nv + C - 1) / C, v0 = min(nv, rank * per), v1 = min(nv, v0 + per);
   const uint32_t wper = (v1 - v0 + NW - 1) / NW, wv0 = min(v1, v0 + warp * wper), wv1 = min(v1, wv0 + wper);
   // vector v from HBM; elements outside the row are -infinity
-  auto read = [&](uint32_t v) {
-    if (v != 0 && v + 1 != nv) return __ldg(vecs + v);
+  auto at_end = [&](uint32_t v) { return v == 0 || v + 1 == nv; };
+  auto read_end = [&](uint32_t v) {
     uint4 w;
     T* e = reinterpret_cast<T*>(&w);
     for (int i = 0; i < EPV; ++i) {
@@ -261,6 +259,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     }
     return w;
   };
+  auto read = [&](uint32_t v) { return at_end(v) ? read_end(v) : __ldg(vecs + v); };
   auto fetch = [&](uint32_t v, float* z) {
     E::get(HELD ? held[v - v0] : read(v), z);
 #pragma unroll
@@ -269,12 +268,30 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
 
   // ---- the largest logit, of the row and of the groups of lanes ----
   float mine = -INFINITY;
-#pragma unroll 4
-  for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
-    const uint4 w = read(v);
-    if (HELD) held[v - v0] = w;
-    mine = max_nan(mine, E::most(w));
+  if (nv < 3)  // all are ends
+    for (uint32_t v = wv0 + lane; v < wv1; v += 32) {
+      const uint4 w = read_end(v);
+      if (HELD) held[v - v0] = w;
+      mine = max_nan(mine, E::most(w));
+    }
+  else for (uint32_t v = wv0 + lane; v < wv1; v += 128) {
+    // four loads in flight, without a branch ahead of them: an end's is
+    // another vector's at first
+    uint4 w[4];
+    const uint32_t last = wv1 - 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(vecs + max(1u, min(min(v + 32 * i, last), nv - 2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = v + 32 * i;
+      if (at >= wv1) break;
+      if (at_end(at)) w[i] = read_end(at);
+      if (HELD) held[at - v0] = w[i];
+      mine = max_nan(mine, E::most(w[i]));
+    }
   }
+  if (tid < 16) s.pow[tid] = exp2(tid / 16.0);
+  if (tid == 0) s.listed = 0, s.first = ~0u;
   // groups: a lane, or two or four; every CTA gets all of them
   const uint32_t groups = min(uint32_t(kGroups), C * NT), wide = C * NT / groups;
   cluster_wait();
@@ -745,8 +762,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   // first by index) and each CTA's kept weight; the CTA that the draw falls in
   // weighs its tokens.  Where the border or min-p's bound lies among the tokens
   // outside the bins, the general form below goes on.  One row of 128256, 99000 tokens
-  // in the nucleus: 23.6 us, the general form 41; 256 such rows 207 and 448.  (Without top-p one pass
-  // weighs all: 14.7 us, and 19.3 by bins.)
+  // in the nucleus: 23 us, the general form 41; 256 such rows 197 and 448.  (Without top-p one pass
+  // weighs all: 14 us, and 19 by bins.)
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
     if (by_p && !by_k) {
       static_assert(sizeof(s.all) == 2 * kSide * sizeof(uint32_t), "the bins lie where candidates are gathered later");
