@@ -29,7 +29,7 @@
 // many the instructions of the passes, 45 of them an FP64 weight.  Measured on one
 // B200: one row of 32000 BF16 logits, top-k 40 and top-p, 6.4 us; one of
 // 128256 FP32 logits with 98000 tokens in the nucleus 40 us; 77 rows of 32003,
-// each with its own settings, 41 us; 256 rows of 128256 so 128 us (a read of the
+// each with its own settings, 41 us; 256 rows of 128256 so 123 us (a read of the
 // logits: 10 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -48,10 +48,11 @@ constexpr int NT = 512;  // threads of a CTA
 constexpr int NW = NT / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kParts = kMaxCluster * NW;  // warps of a row
-constexpr int kGroups = 1024;             // groups of lanes whose largest logits guess the border
+constexpr int kGroups = 2048;             // groups of lanes whose largest logits guess the border
 constexpr int NB = 2048;                  // bins of the histogram of logits
 constexpr float kPerUnit = 128.f;         // of them, a unit of distance from the largest
 constexpr uint32_t kEvery = 8;            // a vector in so many is sampled
+constexpr uint32_t kGuessMost = 1200;     // tokens that are looked for so, at most: of more CAP would not hold all
 constexpr int kGuessBins = 256;           // bins of the groups' largest logits
 constexpr float kGuessPerUnit = 8.f;
 constexpr int CAP = 2048;                 // candidates that are sorted
@@ -63,7 +64,6 @@ struct Shared {
   alignas(16) uint32_t hist[NB];
   uint64_t list[CAP];  // this CTA's candidates: ~key, index
   float group[kGroups];
-  uint32_t guess[1024];  // (kGuessBins of them)
   uint64_t all[CAP];  // of the first CTA: all of them
   double part_w[2][2][kParts];  // of the row's warps, in turn
   uint32_t part_c[2][2][kParts];
@@ -292,8 +292,9 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   }
   if (tid < 16) s.pow[tid] = exp2(tid / 16.0);
   if (tid == 0) s.listed = 0, s.first = ~0u;
-  // groups: a lane, or two or four; every CTA gets all of them
-  const uint32_t groups = min(uint32_t(kGroups), C * NT), wide = C * NT / groups;
+  // groups: a lane, or two or four; every CTA gets all of them.  Twice as many for
+  // a large top-k (256 rows of 128256 BF16, top-k 1000, 224 and 197 us).
+  const uint32_t groups = min(C * NT, uint32_t(top_k > kGroups * 3 / 8 && top_k <= int(kGuessMost) ? kGroups : kGroups / 2)), wide = C * NT / groups;
   cluster_wait();
   {
     float g = mine;
@@ -744,14 +745,14 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   // A distance from the largest logit that as many groups' largest lie within as are
   // wanted, or a few more; -1 with none.
   auto near_groups = [&](uint32_t want) {
-    if (tid < kGuessBins) s.guess[tid] = 0;
+    if (tid < kGuessBins) s.hist[tid] = 0;
     __syncthreads();
     for (uint32_t i = tid; i < groups; i += NT) {
       const float x = (zmax - s.group[i]) * kGuessPerUnit;
-      if (x < float(kGuessBins) - 1.5f) atomicAdd(&s.guess[rounded(x)], 1);
+      if (x < float(kGuessBins) - 1.5f) atomicAdd(&s.hist[rounded(x)], 1);
     }
     __syncthreads();
-    const uint32_t bin = bin_with(s.guess, want);
+    const uint32_t bin = bin_with(s.hist, want);
     return bin < kGuessBins ? (bin + 0.5f) / kGuessPerUnit : -1.f;  // (a distance of at most that has no later bin)
   };
 
@@ -992,12 +993,12 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
 
   // ---- few candidates: all tokens within `reach` of the largest logit, guessed so
   // that they are as many as are kept or a few more.  Up to three quarters of
-  // the groups: `want` groups have a token as near as the farthest of
+  // the groups, and 1200: `want` groups have a token as near as the farthest of
   // their largest ones.  Above that, from a sample.
   if (by_k ? uint32_t(top_k) <= CAP * 3 / 4 : by_p) {
     float reach = -1.f;
     const uint32_t want = by_k ? uint32_t(top_k) : groups / 4;
-    if (want <= 3 * groups / 4) {
+    if (want <= min(3 * groups / 4, kGuessMost)) {
       reach = near_groups(want);
     } else {
       for (uint32_t i = tid; i < NB; i += NT) s.hist[i] = 0;
