@@ -26,11 +26,11 @@
 //   * the CTAs of a row tell each other their numbers by stores into all the
 //     others' shared memory ahead of a cluster barrier, so that each has all of them after it.
 // Bound: for one row the chain of passes and cluster barriers (1 us each); for
-// many the instructions of the passes, 45 of them an FP64 weight.  Measured on one
-// B200: one row of 32000 BF16 logits, top-k 40 and top-p, 6.4 us; one of
-// 128256 FP32 logits with 98000 tokens in the nucleus 40 us; 77 rows of 32003,
-// each with its own settings, 41 us; 256 rows of 128256 so 123 us (a read of the
-// logits: 10 us).
+// many such chains, with two CTAs an SM to hide them, and the passes' instructions,
+// 45 of them an FP64 weight.  Measured on one B200: one row of 32000 BF16 logits,
+// top-k 40 and top-p, 6.4 us; one of 128256 FP32 logits with 98000 tokens in the
+// nucleus 40 us; 77 rows of 32003 FP16, each with its own settings, 41 us; 256 rows of
+// 128256 BF16 so 123 us (a read of the logits: 10 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -700,8 +700,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     if (lane == 0) answer(token, int32_t(many), float((widened(z_token) - zm) * cool - log(total)));
   };
 
-  // Every warp finds the first of the 256 or 2048 bins up to which `want` lie;
-  // with none, their number.
+  // Every warp finds the first of the 256 bins up to which `want` lie; with
+  // none, their number.
   auto bin_with = [&](const uint32_t* bins, uint32_t want) {
     uint32_t t = 0, bin = kGuessBins;
     constexpr int PER = kGuessBins / 32;
