@@ -286,3 +286,11 @@ def test_nucleus_border_among_equal_logits_is_an_index():
     check(z[:8], torch.ones(8, device=DEV) - 2.0 ** -24, top_p=share[::8].contiguous())  # the last kept token
     # (0.01 in FP32 is 2.2e-10 short of 400 tokens of 40000, which is nearer than MARGIN: one row of the four is not sure)
     check(torch.zeros((4, 40000), device=DEV, dtype=torch.bfloat16), unit(6, 4), least_sure=0.75, top_p=share[::16].contiguous())
+
+
+@pytest.mark.parametrize("bad", [dict(temperature=1e300), dict(top_k=2.5), dict(top_p="0.9"), dict(min_p=None), dict(top_k=None)], ids=str)
+def test_settings_that_are_no_numbers_of_their_type(bad):
+    # (1e300 is FP32's infinity, which the library refuses; the others are refused ahead of it)
+    with pytest.raises(RuntimeError if bad.get("temperature") else ValueError):
+        xg.sample(logits_of(1, 4, 100, "fp32"), unit(1, 4), **bad)
+    assert (xg.sample(logits_of(1, 4, 100, "fp32"), unit(1, 4), top_k=10 ** 12) >= 0).all()

@@ -701,8 +701,11 @@ def sample(logits, u, tokens=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     kp, k = _setting(top_k, rows, (_i32,), "top_k", dev)
     pp, p = _setting(top_p, rows, f32, "top_p", dev)
     mp, m = _setting(min_p, rows, f32, "min_p", dev)
-    a = SAMPLE_ARGS.pack(logits.data_ptr(), rows, vocab, logits.stride(0), *addr, hp, kp, pp, mp, heat, max(0, min(k, 2 ** 31 - 1)), p, m,
-                         code, dev, 0)
+    try:
+        a = SAMPLE_ARGS.pack(logits.data_ptr(), rows, vocab, logits.stride(0), *addr, hp, kp, pp, mp, heat,
+                             max(0, min(k, 2 ** 31 - 1)), p, m, code, dev, 0)
+    except (TypeError, struct.error) as e:
+        raise ValueError("sample: temperature, top_p and min_p are numbers, top_k a whole one") from e
     if (lib or load()).xksv_sample(a, stream):
         raise RuntimeError("xksv_sample refused the call or failed to launch")
     return tokens
