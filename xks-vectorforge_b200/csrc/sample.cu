@@ -598,6 +598,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
     n = keep;
     for (uint32_t i = tid; i < n; i += NT) s.all[i] = s.all[i] << 32 | s.all[i] >> 32;
     if (tid == 0) s.low = ~0u;
+    __syncthreads();  // (of more than NT entries the sort gives a thread others than these)
     sort_all(n);
     // (sort_all's padding is no token)
     double x[EACH], t = 0.0;
