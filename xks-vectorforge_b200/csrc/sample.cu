@@ -1096,7 +1096,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   double passed = 0.0;
   uint32_t klo = 0, khi = 0, passed_n = 0;
   bool whole_list = false;  // this CTA's list still holds its candidates
-  bool ties_in = false;     // `passed` has what is kept of a border of one logit already
+  bool all_in = false;      // `passed` has all that is kept: what lies in [klo, khi] too
   auto select = [&](bool by_weight) {
     const uint32_t k = uint32_t(top_k);
     // The weight of the tokens nearer than `start` is known to fall short where
@@ -1341,7 +1341,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
             run += c[i];
           }
           if (by_weight && mine) passed += mine * weight(value_of(khi)), passed_n += mine;
-          ties_in = by_weight;
+          all_in = by_weight;
           const uint32_t who = __ballot_sync(0xffffffffu, owner != ~0u);
           if (who) {
             owner = __shfl_sync(0xffffffffu, owner, __ffs(who) - 1);
@@ -1356,7 +1356,8 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
         } else {
           double run = above;
           uint32_t count = ahead;
-          // (should the quarters together fall short: all of them)
+          // (should the quarters together fall short, by the order of their sums: all
+          // of them, and `passed` takes them all)
           for (uint32_t j = 0; j < 4; ++j) {
             const uint32_t c = count_of(s.quarter_c[now][j]);
             const double t = sum_of(s.quarter_w[now][j]);
@@ -1372,6 +1373,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
             passed += j == 0 ? wq[0] : j == 1 ? wq[1] : j == 2 ? wq[2] : wq[3];
             passed_n += j == 0 ? cq[0] : j == 1 ? cq[1] : j == 2 ? cq[2] : cq[3];
           }
+          all_in = by_weight && found;
         }
       }
       if (found) {
@@ -1397,7 +1399,7 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   const float upto = summed ? value_of(khi) : INFINITY, from = fmaxf(floor_z, border);
   double w = summed ? passed : 0.0;
   uint32_t n = summed ? passed_n : 0;
-  if (summed && ties_in) {
+  if (summed && all_in) {
   } else if (summed && whole_list) {
     // each warp takes its own of them; their order is not fixed, so they are
     // added as integers
