@@ -498,8 +498,11 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* str
  * `type`, strides in elements ([0] sequence, [1] head), the last dimension
  * contiguous; type is the cache's, or BF16 or FP16 over an 8-bit cache. lse is
  * FP32 [seqs, q_heads] contiguous, or NULL. Scores, softmax statistics and
- * sums are FP32, a weight enters its product within 2^-17 (8-bit and FP16 caches:
- * 2^-23, and what is below 2^-40 of the largest weight as zero). A length that is negative or above table_cols * page_size
+ * sums are FP32, a weight enters its product within 2^-17 of itself (8-bit and FP16
+ * caches: 2^-23, or 2^-40 of the largest weight where that is more; with block scales
+ * its product with its value's scale within 2^-23, or 2^-40 of the largest weight
+ * times the largest scale among the sixteen tokens of the same j / 16; scales below
+ * 2^-125 of the sequence's largest may count as zero). A length that is negative or above table_cols * page_size
  * gives zeros and -infinity, a page outside the cache counts as masked; both
  * are reported by xksv_kv_status. d_workspace: as for xksv_plan_linear, of at
  * least xksv_kv_attend_workspace(kv, seqs, q_heads, table_cols) bytes (0 for

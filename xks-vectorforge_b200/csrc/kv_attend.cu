@@ -38,7 +38,8 @@ AttendPlan kv_attend_plan(const xksv_kv_desc& c, const xksv_kv_blocks& b, uint64
   const uint64_t blocks = seqs * c.kv_heads * pl.chunks;
   const uint64_t most = uint64_t(sms) * per_sm * kWarps;
   pl.warps = uint32_t(blocks >= most || longest >= most ? most : std::min<uint64_t>(most, blocks * longest));
-  pl.slot_floats = (uint64_t(pl.heads) * (pl.pad_dim + 2) + 31) / 32 * 32;
+  // sums, maximum and weight of each head; with block scales its sums' unit
+  pl.slot_floats = (uint64_t(pl.heads) * (pl.pad_dim + (b.block ? 3 : 2)) + 31) / 32 * 32;
   pl.joins_off = 2 * pl.warps * pl.slot_floats * sizeof(float);
   pl.bytes = pl.joins_off + pl.warps * sizeof(int4);
   if (blocks * kCluster <= uint64_t(sms) * per_sm && table_cols * c.page_size <= kShort) {

@@ -30,7 +30,8 @@
 //   * Block scales: a token's scales travel with its rows through the ring. A
 //     score is multiplied by its key's; a weight enters its product as its
 //     value's part of the sixteen tokens' largest scale, which the FP32 sums take
-//     in as they add the product.  Integers become FP16 exactly, as low bits of 1024.
+//     in as they add the product, in units of the largest scale so far.  Integers become
+//     FP16 exactly, as low bits of 1024.
 //   * A unit that one warp holds alone is written at once; the others leave
 //     their pieces (sums, maximum, weight) in slots, which the second kernel
 //     joins in a fixed order: results do not depend on timing.
@@ -82,12 +83,22 @@ struct Shape {
   static constexpr bool QS = DP * NG > 256;       // query fragments in shared memory, not registers
   static constexpr int QB = QS ? DP / 16 * 32 * 8 * NG : 0;
   static constexpr int SB = BS ? kStages * 2 * BT * 4 : 0;      // the stages' scales
+  static constexpr int ST = BS ? 3 : 2;                         // a head's statistics in a piece: maximum, weight, the sums' unit
   static constexpr int WARP = kStages * 2 * KV + QB + SB + 16;  // + the stages' token masks
   static constexpr int CTA = kWarps * WARP;
   // CTAs an SM holds.  Three of two stages against two of three stages: 64
   // uneven sequences 399 us against 409, E4M3 85 against 92
   static constexpr int PER_SM = 3 * CTA <= 225 * 1024 ? 3 : 2 * CTA <= 225 * 1024 ? 2 : 1;
 };
+
+// The units of the sums with block scales: the least power of two that holds a
+// scale, of [2^-64, 2^126]: the inverses are normal numbers too, and so is a unit
+// divided by a sum of 2^31 weights of 2^15; the smallest scale is 2^-85 units.
+constexpr float kLeastUnit = 0x1p-64f, kMostUnit = 0x1p126f;
+__device__ __forceinline__ float unit_of(float scale) {
+  return __uint_as_float(min((__float_as_uint(fmaxf(scale, kLeastUnit)) + 0x7fffffu) & 0x7f800000u, __float_as_uint(kMostUnit)));
+}
+__device__ __forceinline__ float inverse_of(float unit) { return __uint_as_float(0x7f000000u - __float_as_uint(unit)); }
 
 // 16-byte piece c of row r: eight rows' pieces lie in eight bank groups.
 template <int CH>
@@ -357,7 +368,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
   // this lane's token of the next block to copy: its rows' offsets in bytes
   bool ld_ok = false;
   uint64_t ld_k = 0, ld_v = 0;
-  const float *ld_ks = p.b.k_scale, *ld_vs = p.b.v_scale;
+  uint32_t ld_page = 0, ld_place = 0;  // block scales: where it is, for `issue` (offsets take registers that they lack)
   const uint32_t psize = uint32_t(p.c.page_size);
   auto look_up = [&]() {
     const uint32_t j = (uint32_t(ld.first) / BT + ld.block) * BT + lane;
@@ -367,14 +378,13 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
       const uint32_t col = pl.page_shift >= 0 ? j >> pl.page_shift : j / psize, place = j - col * psize;
       const int32_t page = p.a.table[ld.seq * p.a.table_stride + col];  // kv_span keeps the length inside the table
       if (uint32_t(page) < p.c.pages) {
-        const uint32_t g = ld.unit / pl.chunks;
         ld_ok = true;
-        ld_k = (uint32_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2]) * Sh::ES;
-        ld_v = (uint32_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2]) * Sh::ES;
         if (BS) {
-          const uint32_t block = pl.block_shift >= 0 ? place >> pl.block_shift : place / uint32_t(p.b.block);
-          ld_ks = p.b.k_scale + uint32_t(page) * p.b.k_stride[0] + block * p.b.k_stride[1] + g * p.b.k_stride[2];
-          ld_vs = p.b.v_scale + uint32_t(page) * p.b.v_stride[0] + block * p.b.v_stride[1] + g * p.b.v_stride[2];
+          ld_page = uint32_t(page), ld_place = place;
+        } else {
+          const uint32_t g = ld.unit / pl.chunks;
+          ld_k = (uint32_t(page) * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2]) * Sh::ES;
+          ld_v = (uint32_t(page) * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2]) * Sh::ES;
         }
       } else {
         atomicOr(p.status, kStatusHeader);  // a page outside the cache
@@ -390,10 +400,16 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
     const uint32_t mask = __ballot_sync(0xffffffffu, ld_ok);
     if (lane == 0) masks[stage] = mask;
     const uint32_t kd = ring + stage * 2 * Sh::KV, vd = kd + Sh::KV;
-    if (BS && lane < BT) {
-      const uint32_t sd = qsm + Sh::QB + (stage * 2 * BT + lane) * 4;
-      copy4(sd, ld_ks, ld_ok ? 4 : 0);
-      copy4(sd + BT * 4, ld_vs, ld_ok ? 4 : 0);
+    if (BS) {
+      const uint32_t g = ld.unit / pl.chunks, page = ld_ok ? ld_page : 0, place = ld_ok ? ld_place : 0;
+      ld_k = page * p.c.k_stride[0] + place * p.c.k_stride[1] + g * p.c.k_stride[2];
+      ld_v = page * p.c.v_stride[0] + place * p.c.v_stride[1] + g * p.c.v_stride[2];
+      if (lane < BT) {
+        const uint32_t block = pl.block_shift >= 0 ? place >> pl.block_shift : place / uint32_t(p.b.block);
+        const uint32_t sd = qsm + Sh::QB + (stage * 2 * BT + lane) * 4;
+        copy4(sd, p.b.k_scale + page * p.b.k_stride[0] + block * p.b.k_stride[1] + g * p.b.k_stride[2], ld_ok ? 4 : 0);
+        copy4(sd + BT * 4, p.b.v_scale + page * p.b.v_stride[0] + block * p.b.v_stride[1] + g * p.b.v_stride[2], ld_ok ? 4 : 0);
+      }
     }
     if (FULL && run && mask == (BT == 32 ? 0xffffffffu : 0xffffu)) {
       // sixteen tokens of a page lie one token's stride apart
@@ -434,9 +450,11 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
   const int hr = lane >> 2, qc = lane & 3;
   uint32_t qf[Sh::QS ? 1 : KS][NG][2];
   float o[NG][KS][4], m[NG][2], l[NG][2], qs[NG][2];
+  float unit = 1.f;  // block scales: what the sums are in units of
   uint32_t head0 = 0, heads = 0;  // the unit's query heads
   const bool q_pairs = ((reinterpret_cast<uintptr_t>(p.a.q) / 2 | p.a.q_stride[0] | p.a.q_stride[1]) & 1) == 0;
   auto begin = [&]() {
+    unit = kLeastUnit;
     const uint32_t group = p.a.q_heads / p.c.kv_heads, g = cu.unit / pl.chunks, ch = cu.unit % pl.chunks;
     head0 = g * group + ch * pl.heads;
     heads = min(pl.heads, group - ch * pl.heads);
@@ -514,7 +532,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
     const uint64_t u0 = t - cu.block, u1 = u0 + cu.blocks;
     const KvPiece piece = CL ? KvPiece{0, 0} : kv_piece(share, me, a, b, u0, u1);
     if (piece.slot < 0) {
-      const float vs = E8 && p.c.v_scale ? p.c.v_scale[cu.unit / pl.chunks] : 1.f;
+      const float vs = BS ? unit : E8 && p.c.v_scale ? p.c.v_scale[cu.unit / pl.chunks] : 1.f;
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
@@ -549,8 +567,9 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
             for (int y = 0; y < 2; ++y)
               if (FULL || dim_of(i, y) < D) slot[head * DP + dim_of(i, y)] = o[n][i][2 * y + h];
           if (hr == 0) {
-            slot[pl.heads * DP + 2 * head] = m[n][h];
-            slot[pl.heads * DP + 2 * head + 1] = l[n][h];
+            float* const stat = slot + pl.heads * DP + Sh::ST * head;
+            stat[0] = m[n][h], stat[1] = l[n][h];
+            if (BS) stat[2] = unit;
           }
         }
       if (!CL && piece.parts && lane == 0) p.joins[me] = make_int4(int(cu.seq), int(cu.unit), int(piece.parts), 0);
@@ -576,15 +595,13 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
     __syncwarp();
     const uint32_t kd = ring + stage * 2 * Sh::KV, vd = kd + Sh::KV;
     const uint32_t mask = masks[stage];
-    float ks[TB][2], vs[TB][2];  // of this lane's tokens
+    float ks[TB][2];  // of this lane's tokens
+    const volatile float* const vscale = scales + stage * 2 * BT + BT;  // of the block's tokens
     if (BS) {
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          ks[tb][y] = scales[stage * 2 * BT + tb * 16 + hr + 8 * y];
-          vs[tb][y] = scales[stage * 2 * BT + BT + tb * 16 + hr + 8 * y];
-        }
+        for (int y = 0; y < 2; ++y) ks[tb][y] = scales[stage * 2 * BT + tb * 16 + hr + 8 * y];
     }
     // the stage before this one is free: every lane has passed the barrier
     if (t + kStages - 1 < b) {
@@ -687,17 +704,31 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
         base[n][h] = v == -INFINITY ? 0.f : v - kUp;
         grew |= v != m[n][h];
       }
+    // Block scales: the sums are in units of the least power of two that holds the
+    // largest scale so far, since weights of 2^15 times a scale overflow where the result
+    // does not.  It rises with the maximum's step (with a check at each product the
+    // kernel took 7 to 17 % longer).
+    const float own_vs = BS ? vscale[lane % BT] : 0.f;
+    if (BS) grew |= own_vs > unit;
     if (__any_sync(0xffffffffu, grew)) {
+      float down = 1.f;
+      if (BS) {
+        // (scales are ordered as their bits)
+        const float most = unit_of(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(own_vs, unit)))));
+        down = unit * inverse_of(most);
+        unit = most;
+      }
 #pragma unroll
       for (int n = 0; n < NG; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float f = exp2_fast(m[n][h] - (mx[n][h] == -INFINITY ? 0.f : mx[n][h]));
+          const float fo = BS ? f * down : f;
           l[n][h] *= f;
 #pragma unroll
           for (int i = 0; i < KS; ++i) {
-            o[n][i][h] *= f;
-            o[n][i][2 + h] *= f;
+            o[n][i][h] *= fo;
+            o[n][i][2 + h] *= fo;
           }
           m[n][h] = mx[n][h];
         }
@@ -711,28 +742,36 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
           sc[tb][n][x] = exp2_fast(sc[tb][n][x] - base[n][x & 1]);
           l[n][x & 1] += sc[tb][n][x];
         }
-    // ---- O^T += V^T P^T ----
+    const bool same = BS && pl.even && mask == (BT == 32 ? 0xffffffffu : 0xffffu);  // (no masked token's zero)
+    // Block scales: a weight enters with its token's scale as a part of the
+    // sixteen tokens' largest, which the FP32 sums take in.  Where they share
+    // one there is nothing to do for it.
+    float high[TB];
+    if (BS) {
+      if (same) {
 #pragma unroll
-    for (int tb = 0; tb < TB; ++tb) {
-      // Block scales: a weight enters with its token's scale as a part of the
-      // sixteen tokens' largest, which the FP32 sums take in.  Where they share
-      // one there is nothing to do for it.
-      float high = 1.f;
-      if (BS) {
-        high = vs[tb][0];
-        if (!pl.even || ((mask >> (16 * tb)) & 0xffffu) != 0xffffu) {
-          high = fmaxf(high, vs[tb][1]);
+        for (int tb = 0; tb < TB; ++tb) high[tb] = vscale[tb * 16];
+      } else {
 #pragma unroll
-          for (int d = 4; d < 32; d <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+        for (int tb = 0; tb < TB; ++tb) {
+          const float vs[2] = {vscale[tb * 16 + hr], vscale[tb * 16 + hr + 8]};
+          high[tb] = fmaxf(vs[0], vs[1]);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) high[tb] = fmaxf(high[tb], __shfl_xor_sync(0xffffffffu, high[tb], d));
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             // (NaN scales stay NaN)
-            const float part = vs[tb][y] == high ? 1.f : vs[tb][y] / high;
+            const float part = vs[y] == high[tb] ? 1.f : vs[y] / high[tb];
 #pragma unroll
             for (int n = 0; n < NG; ++n) sc[tb][n][2 * y] *= part, sc[tb][n][2 * y + 1] *= part;
           }
         }
       }
+    }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int tb = 0; tb < TB; ++tb) {
+      const float part = BS ? high[tb] * inverse_of(unit) : 1.f;
       uint32_t hi[NG][2], lo[NG][2];
 #pragma unroll
       for (int n = 0; n < NG; ++n)
@@ -769,7 +808,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
                 mma<false>(some, va, hi[n][0], hi[n][1]);
                 mma<false>(some, va, lo[n][0], lo[n][1]);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) o[n][i + y][x] += some[x] * high;
+                for (int x = 0; x < 4; ++x) o[n][i + y][x] += some[x] * part;
               } else {
                 mma<false>(o[n][i + y], va, hi[n][0], hi[n][1]);
                 mma<false>(o[n][i + y], va, lo[n][0], lo[n][1]);
@@ -802,10 +841,12 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
     const uint32_t runs = 32 / cl_heads, head = me % cl_heads, run0 = me / cl_heads;
     if (run0 < runs) {
       auto piece = [&](uint32_t k) { return smem_addr(smem) + (k % kWarps) * Sh::WARP; };
-      float m1 = -INFINITY, l1 = 0.f;
+      float m1 = -INFINITY, l1 = 0.f, u1 = kLeastUnit;
       if (uint32_t(lane) < share.workers) {
-        m1 = ld_cluster(piece(lane) + (pl.heads * DP + 2 * head) * 4, lane / kWarps);
-        l1 = ld_cluster(piece(lane) + (pl.heads * DP + 2 * head + 1) * 4, lane / kWarps);
+        const uint32_t stat = piece(lane) + (pl.heads * DP + Sh::ST * head) * 4;
+        m1 = ld_cluster(stat, lane / kWarps);
+        l1 = ld_cluster(stat + 4, lane / kWarps);
+        if (BS) u1 = ld_cluster(stat + 8, lane / kWarps);
       }
       float base = m1;
 #pragma unroll
@@ -815,8 +856,15 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
       float lt = l1 * w;
 #pragma unroll
       for (int d = 16; d >= 1; d >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, d);
+      float u = 1.f, wo = w;  // of block scales' sums: the largest unit, and the weight in units of it
+      if (BS) {
+        u = u1;
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) u = fmaxf(u, __shfl_xor_sync(0xffffffffu, u, d));
+        wo *= u1 * inverse_of(u);
+      }
       const bool some = lt > 0.f || lt != lt;
-      const float f = some ? (E8 && p.c.v_scale ? p.c.v_scale[cl_unit / pl.chunks] : 1.f) / lt : 0.f;
+      const float f = some ? (BS ? u : E8 && p.c.v_scale ? p.c.v_scale[cl_unit / pl.chunks] : 1.f) / lt : 0.f;
       uint16_t* out = static_cast<uint16_t*>(p.a.out) + cl_seq * p.a.out_stride[0] + (cl_head0 + head) * p.a.out_stride[1];
       for (uint32_t d0 = run0 * 32; d0 < D; d0 += runs * 32) {
         const uint32_t d = d0 + lane;
@@ -827,7 +875,7 @@ __global__ void __launch_bounds__(kWarps * 32, Shape<EL, DP, NG>::PER_SM) kv_att
         float acc = 0.f;
 #pragma unroll
         for (uint32_t k = 0; k < 32; ++k) {
-          const float wk = __shfl_sync(0xffffffffu, w, k);
+          const float wk = __shfl_sync(0xffffffffu, wo, k);
           acc += k < share.workers ? v[k] * wk : 0.f;
         }
         if (d < D) store16(bf, out + d, some ? acc * f : 0.f);
@@ -848,17 +896,18 @@ constexpr uint32_t kJoin = JT / 32;    // workers whose units a CTA joins, and p
 // successive workers), and that one takes the whole CTA: the parts' weights
 // once in shared memory, then each warp every eighth part, lanes the dims;
 // last the warps' sums in order.
-__global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const AttendPlan pl, float up) {
+template <bool BS>
+__global__ void __launch_bounds__(JT, 3) kv_join_kernel(const AttendArgs p, const AttendPlan pl, float up) {
   extern __shared__ float weight[];  // [workers]
   __shared__ __align__(16) float so[JT / 32][256];
-  __shared__ float red[2][JT / 32];
+  __shared__ float red[3][JT / 32];
   __shared__ int4 big;
   __shared__ uint32_t big_at;
   constexpr float kLn2 = 0.69314718055994531f;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t head = blockIdx.y, DP = pl.pad_dim, D = p.c.head_dim;
   const bool bf = p.a.type == XKSV_BF16;
-  const uint32_t group = p.a.q_heads / p.c.kv_heads, st = pl.heads * DP + 2 * head;
+  const uint32_t group = p.a.q_heads / p.c.kv_heads, st = pl.heads * DP + (BS ? 3 : 2) * head;
   if (threadIdx.x == 0) big_at = ~0u;
   __syncthreads();
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
@@ -874,8 +923,8 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
   auto out_of = [&](int4 j, const Unit& u) {
     return static_cast<uint16_t*>(p.a.out) + uint64_t(j.x) * p.a.out_stride[0] + u.head * p.a.out_stride[1];
   };
-  auto scale_of = [&](const Unit& u, float l) {  // no weight at all: zeros
-    return l > 0.f || l != l ? (p.c.v_scale ? p.c.v_scale[u.kv_head] : 1.f) / l : 0.f;
+  auto scale_of = [&](const Unit& u, float l, float unit) {  // no weight at all: zeros
+    return l > 0.f || l != l ? (!BS && p.c.v_scale ? p.c.v_scale[u.kv_head] : unit) / l : 0.f;
   };
   auto put_lse = [&](int4 j, const Unit& u, float base, float l) {
     if (p.a.lse)
@@ -891,11 +940,12 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
   } else if (j.z) {
     const Unit u = unit_of(j);
     if (u.mine) {
-      float m[kJoin], w[kJoin], l = 0.f, base = -INFINITY;
+      float m[kJoin], w[kJoin], in[kJoin], l = 0.f, base = -INFINITY;
 #pragma unroll
       for (uint32_t k = 0; k < kJoin; ++k) {
         m[k] = k < uint32_t(j.z) ? slot(i, k)[st] : -INFINITY;
         w[k] = k < uint32_t(j.z) ? slot(i, k)[st + 1] : 0.f;
+        in[k] = BS && k < uint32_t(j.z) ? slot(i, k)[st + 2] : kLeastUnit;
       }
       float acc[8] = {};
       float v[kJoin][4];  // 128 dims of every part at a time
@@ -917,6 +967,14 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
         m[k] = k < uint32_t(j.z) ? exp2f(m[k] - base) : 0.f;
         l += w[k] * m[k];
       }
+      float most = 1.f;
+      if (BS) {
+        most = kLeastUnit;
+#pragma unroll
+        for (uint32_t k = 0; k < kJoin; ++k) most = fmaxf(most, in[k]);
+#pragma unroll
+        for (uint32_t k = 0; k < kJoin; ++k) m[k] *= in[k] * inverse_of(most);
+      }
 #pragma unroll
       for (uint32_t k = 0; k < kJoin; ++k)
 #pragma unroll
@@ -928,7 +986,7 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
 #pragma unroll
           for (uint32_t x = 0; x < 4; ++x) acc[4 + x] += k < uint32_t(j.z) ? v[k][x] * m[k] : 0.f;
       }
-      const float f = scale_of(u, l);
+      const float f = scale_of(u, l, most);
       const bool some = l > 0.f || l != l;
       uint16_t* out = out_of(j, u);
 #pragma unroll
@@ -944,21 +1002,32 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
   const Unit u = unit_of(jm);
   if (!u.mine) return;
   const uint32_t parts = uint32_t(jm.z);
-  float mt = -INFINITY;
+  float mt = -INFINITY, most = BS ? kLeastUnit : 1.f;
   for (uint32_t k = threadIdx.x; k < parts; k += JT) {
     weight[k] = slot(many, k)[st];
     mt = fmaxf(mt, weight[k]);
+    if (BS) most = fmaxf(most, slot(many, k)[st + 2]);
   }
 #pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
-  if (lane == 0) red[0][warp] = mt;
+  for (int d = 16; d >= 1; d >>= 1) {
+    mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
+    if (BS) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  }
+  if (lane == 0) {
+    red[0][warp] = mt;
+    if (BS) red[2][warp] = most;
+  }
   __syncthreads();
-  for (int w = 0; w < JT / 32; ++w) mt = fmaxf(mt, red[0][w]);
+  for (int w = 0; w < JT / 32; ++w) {
+    mt = fmaxf(mt, red[0][w]);
+    if (BS) most = fmaxf(most, red[2][w]);
+  }
   const float base = mt == -INFINITY ? 0.f : mt;
   float l = 0.f;
   for (uint32_t k = threadIdx.x; k < parts; k += JT) {
     weight[k] = exp2f(weight[k] - base);
     l += slot(many, k)[st + 1] * weight[k];
+    if (BS) weight[k] *= slot(many, k)[st + 2] * inverse_of(most);
   }
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
@@ -984,7 +1053,7 @@ __global__ void __launch_bounds__(JT) kv_join_kernel(const AttendArgs p, const A
     *reinterpret_cast<float4*>(&so[warp][d]) = acc;
   }
   __syncthreads();
-  const float f = scale_of(u, l);
+  const float f = scale_of(u, l, most);
   const bool some = l > 0.f || l != l;
   uint16_t* out = out_of(jm, u);
   for (uint32_t d = threadIdx.x; d < D; d += JT) {
@@ -1000,7 +1069,7 @@ int pad_dim(uint32_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 template <bool MB, int EL, int DP, int NG, bool FULL, bool CL>
 cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_t st) {
   using Sh = Shape<EL, DP, NG>;
-  static_assert(8 * NG * (DP + 2) * 4 <= Sh::WARP, "a piece fits the warp's shared memory");
+  static_assert(8 * NG * (DP + Sh::ST) * 4 <= Sh::WARP, "a piece fits the warp's shared memory");
   auto kernel = kv_attend_kernel<MB, EL, DP, NG, FULL, CL>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = opt_in_smem(kernel, Sh::CTA, done);
@@ -1023,7 +1092,7 @@ cudaError_t launch_attend(const AttendArgs& p, const AttendPlan& pl, cudaStream_
   cfg.gridDim = dim3((pl.warps + kJoin - 1) / kJoin, pl.heads);
   cfg.blockDim = dim3(JT);
   cfg.dynamicSmemBytes = pl.warps * sizeof(float);
-  return cudaLaunchKernelEx(&cfg, kv_join_kernel, p, pl, MB ? 0.f : 15.f);
+  return cudaLaunchKernelEx(&cfg, kv_join_kernel<Sh::BS>, p, pl, MB ? 0.f : 15.f);
 }
 
 template <bool MB, int EL, int DP, int NG>
