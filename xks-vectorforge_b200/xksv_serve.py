@@ -163,7 +163,7 @@ class PagedSession:
 
     def _check(self):
         stream = self._stream()
-        if any(c.status(stream) for c in self.caches):
+        if any([c.status(stream) for c in self.caches]):  # (all of them: reading one clears it)
             fail("paged cache: a page or place outside the cache")
 
     def _stream(self):
