@@ -445,7 +445,8 @@ int xksv_kv_create_blocks(const xksv_kv_desc* desc, const xksv_kv_blocks* blocks
 void xksv_kv_destroy(xksv_kv* kv);
 /* Synchronises `stream`; 0 when no call reported an error since the last one
  * (then clears the word), else 1: a page outside the cache, a sequence or a
- * place outside the page table, a length above the table's. */
+ * place outside the page table, a length above the table's; with block scales
+ * also a sequence's tokens out of order, and NaN for an integer. */
 int xksv_kv_status(const xksv_kv* kv, void* stream);
 
 /* New tokens into the cache.  Token t is token index[t] of sequence seq[t]

@@ -23,3 +23,35 @@ def test_an_error_is_reported_once(tmp_path):
     assert s.generate([[1, 2, 3]], 4) == good
     assert len(s.free_pages) == 8 and len(s.free_seqs) == 2
     s.close()
+
+
+@pytest.mark.parametrize("kv,said", [("int8-blocks", "NaN"), ("e4m3-blocks", None), ("bf16", None)])
+def test_a_nan_key_is_named(tmp_path, kv, said):
+    """Integers hold no NaN: the append reports it, and the session says so.  The other
+    caches keep it, and the logits are NaN."""
+    s = serve.load_session(archive(tmp_path, "llama"), DEV, pages=8, page_size=8, max_seqs=2, kv_dtype=kv)
+    good = s.generate([[1, 2, 3]], 4)
+    with torch.no_grad():
+        s.core.embed_tokens.weight[5] = float("nan")
+    if said:
+        with pytest.raises(rt.ArchiveError, match=said):
+            s.prefill([[1, 5, 3]])
+    else:
+        seqs, logits = s.prefill([[1, 5, 3]])
+        assert logits.isnan().all()
+        s.release(seqs)
+    # it is reported once, and others go on
+    assert s.generate([[1, 2, 3]], 4) == good
+    assert len(s.free_pages) == 8 and len(s.free_seqs) == 2
+    s.close()
+
+
+@pytest.mark.parametrize("kv,said", [("int8-blocks", "NaN .*, or a page or place outside"), ("e4m3-blocks", "^paged cache: a page or place outside"),
+                                     ("bf16", "^paged cache: a page or place outside")])
+def test_an_error_names_its_possible_causes(tmp_path, kv, said):
+    s = serve.load_session(archive(tmp_path, "llama"), DEV, pages=8, page_size=8, max_seqs=2, kv_dtype=kv)
+    s.caches[1].status = lambda stream=0: 1  # (as after an error)
+    with pytest.raises(rt.ArchiveError, match=said):
+        s.prefill([[1, 2, 3]])
+    assert len(s.free_pages) == 8 and len(s.free_seqs) == 2
+    s.close()

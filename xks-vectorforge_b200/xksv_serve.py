@@ -162,9 +162,11 @@ class PagedSession:
         return layer.mlp(x, residual=h) if hasattr(layer.mlp, "xksv_fused_mlp") else h + layer.mlp(x)
 
     def _check(self):
+        import torch
         stream = self._stream()
         if any([c.status(stream) for c in self.caches]):  # (all of them: reading one clears it)
-            fail("paged cache: a page or place outside the cache")
+            nan = "a key or value that is NaN (integers hold none: stored as zero), or " if self.kv.dtype == torch.int8 else ""
+            fail(f"paged cache: {nan}a page or place outside the cache, in this call or a step before it")
 
     def _stream(self):
         import torch
