@@ -55,3 +55,21 @@ def test_an_error_names_its_possible_causes(tmp_path, kv, said):
         s.prefill([[1, 2, 3]])
     assert len(s.free_pages) == 8 and len(s.free_seqs) == 2
     s.close()
+
+
+def test_settings_of_one_value_are_numbers(tmp_path):
+    """A tensor or an array without dimensions is a number; of more than one dimension it
+    is refused."""
+    import numpy as np
+    s = serve.load_session(archive(tmp_path, "llama"), DEV, pages=40, page_size=8, max_seqs=4)
+    gen = lambda: torch.Generator(device=DEV).manual_seed(3)
+    prompts = [[1, 2, 3], [4] * 9]
+    want = s.generate(prompts, 6, temperature=0.75, top_k=20, top_p=0.5, min_p=0.25, generator=gen())
+    for one in (torch.tensor, np.array, lambda v: torch.tensor(v, device=DEV)):
+        assert s.generate(prompts, 6, temperature=one(0.75), top_k=one(20), top_p=one(0.5), min_p=one(0.25), generator=gen()) == want
+    assert s.generate(prompts, 6, temperature=torch.tensor(0.0)) == s.generate(prompts, 6)
+    for bad in (dict(temperature=torch.ones(2, 1)), dict(top_p=[[0.5], [0.5]]), dict(temperature="warm"), dict(top_k=[1.5, "a"])):
+        with pytest.raises((rt.ArchiveError, ValueError)):
+            s.generate(prompts, 2, **{"temperature": 1.0, **bad})
+    assert len(s.free_pages) == 40 and len(s.free_seqs) == 4
+    s.close()

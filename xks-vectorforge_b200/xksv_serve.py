@@ -300,10 +300,15 @@ class PagedSession:
         import torch
         how = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         for name, v in how.items():
-            if hasattr(v, "__len__"):
+            if getattr(v, "ndim", None) == 0:
+                how[name] = v.item()
+            elif hasattr(v, "__len__"):
                 if len(v) != len(prompts):
                     fail(f"generate: {len(v)} values of {name} for {len(prompts)} prompts")
-                how[name] = torch.as_tensor(v, dtype=torch.int32 if name == "top_k" else torch.float32).to(self.device)
+                try:
+                    how[name] = torch.as_tensor(v, dtype=torch.int32 if name == "top_k" else torch.float32).to(self.device)
+                except (TypeError, ValueError):
+                    fail(f"generate: {name} is no number and not one for each prompt")
         greedy = not torch.is_tensor(how["temperature"]) and how["temperature"] == 0
         seqs, logits = self.prefill(prompts)
         out = [[] for _ in seqs]
