@@ -73,3 +73,22 @@ def test_settings_of_one_value_are_numbers(tmp_path):
             s.generate(prompts, 2, **{"temperature": 1.0, **bad})
     assert len(s.free_pages) == 40 and len(s.free_seqs) == 4
     s.close()
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_torchs_default_dtype_does_not_matter(tmp_path, default):
+    path = archive(tmp_path, "llama")
+    how = dict(temperature=1.5, top_p=0.9)
+
+    def run():
+        s = serve.load_session(path, DEV, pages=40, page_size=8, max_seqs=4, kv_dtype="int8-blocks")
+        out = s.generate([[1, 2, 3], [4] * 9], 6, **how, generator=torch.Generator(device=DEV).manual_seed(3))
+        s.close()
+        return out
+
+    want, before = run(), torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        assert run() == want
+    finally:
+        torch.set_default_dtype(before)

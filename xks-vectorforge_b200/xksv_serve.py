@@ -81,7 +81,8 @@ class PagedSession:
         scales = [(None, None)] * len(self.layers)
         self.kv_block = (kv_block or page_size) if blocked else 0
         if blocked:
-            scales = torch.zeros((len(self.layers), 2, pages, page_size // self.kv_block, self.kv_heads), device=self.device)
+            scales = torch.zeros((len(self.layers), 2, pages, page_size // self.kv_block, self.kv_heads),
+                                 dtype=torch.float32, device=self.device)
         if kv_dtype == "e4m3":
             scale = torch.as_tensor(kv_scale, dtype=torch.float32, device=self.device)
             shape = (len(self.layers), 2, self.kv_heads)
@@ -289,7 +290,7 @@ class PagedSession:
         numbers or tensors [rows]), drawn with `generator`'s numbers; token -1
         for a row without a distribution (NaN)."""
         import torch
-        u = torch.rand(logits.shape[0], generator=generator, device=logits.device)
+        u = torch.rand(logits.shape[0], generator=generator, dtype=torch.float32, device=logits.device)
         return xksv_gpu.sample(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, stream=self._stream())
 
     def generate(self, prompts, max_new_tokens, eos=None, temperature=0.0, top_k=0, top_p=1.0, min_p=0.0, generator=None):
