@@ -9,6 +9,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 import xksv_gpu as xg  # noqa: E402
+from test_gpu_sample import DT, check, gen, unit  # noqa: E402
 
 DEV = "cuda:0"
 
@@ -55,3 +56,22 @@ def test_nucleus_whose_parts_fall_short_of_their_whole():
         assert len(at) == first
         token = int(tokens[r])
         assert abs(int(np.searchsorted(at, token)) - float(u[r]) * first) <= 3, r
+
+
+@pytest.mark.parametrize("kind", ["fp16", "fp32"])
+@pytest.mark.parametrize("values", [1, 2, 5, 300])
+@pytest.mark.parametrize("rows,vocab", [(3, 40001), (300, 9001), (2, 128256)])
+def test_more_tokens_near_the_largest_than_candidates(rows, vocab, values, kind):
+    """Flat and heavily tied rows: thousands of tokens lie as near as the guess of few, so
+    that the border is found among all of them, by index where it is one logit's."""
+    level = torch.cat([torch.zeros(1, device=DEV), -torch.rand(values - 1, generator=gen(values), device=DEV) * 2])
+    z = level[torch.randint(0, values, (rows, vocab), generator=gen(rows), device=DEV)].to(DT[kind])
+    for how in (dict(top_p=0.9), dict(top_p=0.31), dict(top_p=0.0625, temperature=0.5), dict(top_p=0.97, min_p=0.3)):
+        # (equal logits weigh 1 each, and 0.0625 of 128256 tokens is 8016: the border lies on
+        # a sum, which no row of them is sure of; those sums are exact on both sides)
+        border = values == 1 and (how["top_p"] * vocab).is_integer()
+        check(z, unit(rows + 1, rows), least_sure=0.0 if border else 0.9, **how)
+        if border:
+            kept = torch.empty(rows, dtype=torch.int32, device=DEV)
+            xg.sample(z, unit(rows + 1, rows), kept=kept, **how)
+            assert (kept == int(how["top_p"] * vocab)).all()

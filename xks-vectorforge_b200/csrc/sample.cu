@@ -1099,10 +1099,10 @@ __global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleArgs p) {
   bool all_in = false;      // `passed` has all that is kept: what lies in [klo, khi] too
   auto select = [&](bool by_weight) {
     const uint32_t k = uint32_t(top_k);
-    // The weight of the tokens nearer than `start` is known to fall short where
-    // the guess above was tried; behind `end` all V tokens weigh less
-    // than the whole leaves.
-    const bool tried = by_weight && !cut && whole >= 0.0 && nearest >= 0.f;
+    // Where the guess above was tried the weight of the tokens nearer than `start` is
+    // known, and falls short unless they were only too many; behind `end` all V
+    // tokens weigh less than the whole leaves.
+    const bool tried = by_weight && !cut && whole >= 0.0 && nearest >= 0.f && weight_near < double(top_p) * whole;
     start = 0.f, beyond = -1.f, per_unit = kPerUnit;
     if (tried) {
       const float end = float(log(V / ((1.0 - double(top_p)) * whole)) * double(heat));
