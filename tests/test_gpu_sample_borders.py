@@ -75,3 +75,14 @@ def test_more_tokens_near_the_largest_than_candidates(rows, vocab, values, kind)
             kept = torch.empty(rows, dtype=torch.int32, device=DEV)
             xg.sample(z, unit(rows + 1, rows), kept=kept, **how)
             assert (kept == int(how["top_p"] * vocab)).all()
+
+
+@pytest.mark.parametrize("kind,rows,vocab", [("fp32", 600, 128256), ("bf16", 600, 256000)])
+def test_many_rows_that_their_ctas_do_not_hold(kind, rows, vocab):
+    z = torch.rand((rows, vocab), generator=gen(rows), device=DEV).clamp_(min=1e-12).log_().mul_(-0.9).to(DT[kind])
+    u, some = unit(1, rows), slice(0, rows, 67)
+    for how in (dict(), dict(top_k=40, top_p=0.9), dict(top_p=0.95), dict(top_k=20000)):
+        kept = torch.empty(rows, dtype=torch.int32, device=DEV)
+        tokens = xg.sample(z, u, kept=kept, **how)
+        assert torch.equal(check(z[some].contiguous(), u[some].contiguous(), **how), tokens[some])
+        assert ((tokens >= 0) & (tokens < vocab)).all() and (kept > 0).all()

@@ -7,8 +7,9 @@
 // through the kept tokens by index, so nothing is sorted but the few
 // candidates next to the border:
 //   * a cluster of CTAs takes a row and holds it in shared memory: the logits
-//     are read from HBM once (a row larger than eight CTAs hold is read again by
-//     every pass);
+//     are read from HBM once (a row larger than its CTAs hold is read again by
+//     every pass: more than eight hold, or, of rows that do not fit an SM twice, so many that
+//     fewer CTAs a row are faster all the same, as in `launch`);
 //   * few kept tokens: the largest logits of groups of lanes guess a distance
 //     from the largest logit that as many tokens lie within as are wanted, or a few
 //     more; those are gathered, sorted and drawn from by the first CTA, up to 64
@@ -1476,15 +1477,17 @@ cudaError_t launch(const SampleArgs& given, int sms, cudaStream_t st) {
   const uint64_t row = (p.a.vocab + 16 / sizeof(T)) * sizeof(T);  // and its skew
   auto bytes = [&](uint32_t c) { return kOver + (row / 16 / c + 2) * 16; };
   // Where a row, in eight pieces or fewer, leaves an SM room for two CTAs, no
-  // fewer pieces than that and up to four CTAs an SM; else up to eight.  Clusters of
+  // fewer pieces than that and up to four CTAs an SM; else two or more, up to eight CTAs an
+  // SM, held or not.  Clusters of
   // 1, 2, 4 and 8 CTAs, rows with settings of their own, us: of 32003 BF16 40 rows 60,
   // 42, 37 and 37; 77 59, 42, 42 and 52; 150 70, 58, 63 and 79; 500 99, 92, 118 and
   // 185; of 128256 BF16 77 rows 269, 126, 80 and 72; 300 718, 404, 316 and 259; of
   // 128256 FP32, which do not fit twice, 77 rows 325, 192, 83 and 79; 150 216, 129, 117
-  // and 147; 500 311, 220, 303 and 438.
+  // and 147; 500 311, 220, 303 and 438; 1000 656, 446, 572 and 808; 2000 1011, 771,
+  // 1122 and 1621; of 256000 BF16 600 1239, 716, 617 and 767; 2000 1935, 1342, 1760 and 2335.
   const bool twice = bytes(kMaxCluster) <= kMost / 2;
   const uint64_t most = uint64_t(sms) * (twice ? 4 : 8);
-  uint32_t c = 1;
+  uint32_t c = twice ? 1 : 2;
   while (c < kMaxCluster && (p.a.rows * c * 2 <= most || (twice && bytes(c) > kMost / 2))) c *= 2;
   p.cluster = c;
   const bool holds = bytes(c) <= kMost;
