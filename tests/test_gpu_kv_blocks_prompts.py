@@ -345,3 +345,27 @@ def test_prompts_in_a_graph():
         other.c.close()
     assert c.c.status() == 0
     c.c.close()
+
+
+@pytest.mark.parametrize("block", [4, 16])
+def test_more_sequences_without_seq_than_the_first_kernel_takes(block):
+    g = gen(block)
+    S = 2500
+    lens = torch.randint(1, 20, (S,), generator=torch.Generator().manual_seed(1)).tolist()
+    table, pages = table_of(g, lens, 16)
+    k, v = (torch.randn(S, 2, 64, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(S, 4, 64, generator=g, device=DEV).to(torch.bfloat16)
+    inv = (10000.0 ** (-torch.arange(32, device=DEV) / 32)).float()
+    c = Cache(g, "int8", pages, 16, block, 2, 64)
+    before, had, q0 = [raw(t).clone().view(t.dtype) for t in (c.k, c.v)], [c.ks.clone(), c.vs.clone()], q.clone()
+    index = ints([x - 1 for x in lens])
+    c.c.append(k, v, table, index, inv_freq=inv, q=q)
+    assert c.c.status() == 0
+    at = torch.arange(S, device=DEV)
+    page, place = table[at, index.long() // 16].long(), index.long() % 16
+    keys, mag = rope64(k, index, inv, False)
+    check_half(c, "k", before[0], had[0], keys, 2.0 ** -20 * mag, page, place)
+    check_half(c, "v", before[1], had[1], v.double(), torch.zeros_like(mag), page, place)
+    want, mag = rope64(q0, index, inv, False)
+    assert ((q.double() - want).abs() <= half_step("bf16", want) + 2.0 ** -20 * mag).all()
+    c.c.close()

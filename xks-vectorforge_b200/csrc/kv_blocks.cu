@@ -33,7 +33,6 @@ namespace {
 constexpr int BTH = 128;        // threads of a CTA
 constexpr uint32_t kTile = 16;  // tokens whose angles lie in shared memory at a time
 constexpr uint32_t kHeads = 64; // KV heads of a CTA at most
-constexpr uint64_t kFew = 512;  // tokens, up to which one kernel does all
 
 struct I8 {
   int8_t b;
@@ -727,7 +726,19 @@ cudaError_t append_launch(const AppendBlocksArgs& given, int sms, cudaStream_t s
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   const uint64_t room = 6 * uint64_t(sms);
-  if (pieces && p.a.tokens > kFew) {
+  // Tokens up to which one kernel does all: it gives a run a CTA that goes over it
+  // token by token; the other has a fixed price of two launches and its tiles.  First
+  // kernel and runs, us, 32 + 8 heads of 128 E4M3: one-token sequences without `seq` 512
+  // 11.1 and 17.1, 2048 20.3 and 21.9, 4096 36.5 and 33.5; blocks of one token (16 heads
+  // of 64) 512 9.5 and 13.7, 4096 31 and 35.  With `seq` what a call holds is not known
+  // here but for its tokens a row of the table at least.  A row, blocks of 16: 8
+  // tokens 19 and 10, 64 35 and 14, 512 41 and 16; 64 rows, one token each 8.8 and 36, two
+  // 11.6 and 17.5, four 16.0 and 17.7, eight 27 and 19; 20 + 20 heads of 80, blocks of 24,
+  // four 24 and 16; one row of 64 tokens in a block of 64 (64 + 8 heads) 134 and 43, in
+  // blocks of 4 13 and 15; 1024 of one token 44 and 47.
+  const bool single = !p.a.seq || p.b.block == 1;
+  const uint64_t few = single ? 2048 : p.a.tokens >= 8 * p.a.table_rows && p.b.block >= 8 ? 0 : 512;
+  if (pieces && p.a.tokens > few) {
     if (p.a.q) {
       AppendArgs q{p.a, p.c, p.status};
       q.c.kv_heads = 0;
@@ -745,11 +756,12 @@ cudaError_t append_launch(const AppendBlocksArgs& given, int sms, cudaStream_t s
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kv_append_runs_kernel<TI, TC>, p);
   }
-  // few tokens: each its own CTA (a run's first one works); else as many as a
-  // block has, up to a tile.  The heads are split where there are fewer runs
-  // than the GPU holds CTAs.
-  p.chunk = p.a.tokens <= kFew ? 1 : uint32_t(std::min<uint64_t>(kTile, p.b.block));
-  const uint64_t runs = (p.a.tokens + p.b.block - 1) / p.b.block;
+  // few tokens, or runs of one: each its own CTA (a run's first one works); else as
+  // many as a block has, up to a tile.  The heads are split where there are fewer runs
+  // than the GPU holds CTAs (one-token sequences without `seq` taken for runs of a
+  // block's tokens: 512 22 us, not 11).
+  p.chunk = single || p.a.tokens <= 512 ? 1 : uint32_t(std::min<uint64_t>(kTile, p.b.block));
+  const uint64_t runs = single ? p.a.tokens : (p.a.tokens + p.b.block - 1) / p.b.block;
   uint64_t splits = std::max<uint64_t>((p.c.kv_heads + kHeads - 1) / kHeads, std::min<uint64_t>(p.c.kv_heads, room / runs));
   splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, 65535));
   cudaLaunchConfig_t cfg = {};
