@@ -369,3 +369,27 @@ def test_more_sequences_without_seq_than_the_first_kernel_takes(block):
     want, mag = rope64(q0, index, inv, False)
     assert ((q.double() - want).abs() <= half_step("bf16", want) + 2.0 ** -20 * mag).all()
     c.c.close()
+
+
+def test_a_sequence_that_comes_again_is_found_wherever_it_was():
+    """Among one-token sequences in any order: next but one, in the same tile, in the same CTA's
+    tokens, and far behind; padding of the same number does not count."""
+    g = gen(8)
+    n, page = 2100, 16
+    table, pages = table_of(g, [16] * (n + 3), page)
+    c = Cache(g, "int8", pages, page, 8, 1, 16)
+    k, v = (torch.randn(n, 1, 16, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    for order in (torch.arange(n), torch.randperm(n, generator=torch.Generator().manual_seed(2)), torch.arange(n).flip(0)):
+        seq, index = order.to(torch.int32).to(DEV), torch.full((n,), 8, dtype=torch.int32, device=DEV)
+        c.c.append(k, v, table, index, seq=seq)
+        assert c.c.status() == 0
+        for first, then in ((0, 2), (5, 7), (15, 17), (16, 31), (0, n - 1), (700, 1801), (n - 3, n - 1), (31, 33), (1023, 2047)):
+            again, places = seq.clone(), index.clone()
+            again[then] = again[first]
+            places[then] = 0  # (another block: what is stored is defined)
+            c.c.append(k, v, table, places, seq=again)
+            assert c.c.status() == 1, (first, then)
+            places[first] = -1
+            c.c.append(k, v, table, places, seq=again)
+            assert c.c.status() == 0, (first, then)
+    c.c.close()
