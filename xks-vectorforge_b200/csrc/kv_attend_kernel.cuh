@@ -43,8 +43,9 @@
 // 28 and 4 heads, 130 uneven sequences to 6000: 88 us, 4250 GB/s, the
 // conversion's instructions besides the reads.  Block scales (of 16 tokens):
 // 131071 tokens 65 us, 4130 GB/s (E4M3 with a scale per head 62); 64 uneven
-// sequences to 16384 of integers 210 us, 5130 GB/s (E4M3 per head 204-212); the
-// 130 with a scale for each token 97 us against 85.
+// sequences to 16384 of integers 235 to 245 us, 4570 GB/s, under the power cap that they
+// reach (217 in the first milliseconds; E4M3 per head 216); the 130 with a scale for
+// each token 101 us against 88.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

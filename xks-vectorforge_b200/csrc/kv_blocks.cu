@@ -6,11 +6,11 @@
 // largest of them is known.  Scales are powers of two: a raised scale costs an
 // earlier element at most the bits that fall below its new least one, and an
 // E4M3 element none but near zero.
-//   * Up to 512 tokens, and any strides and alignment: a CTA takes runs, whole
+//   * Runs of a token or few, and any strides and alignment: a CTA takes runs, whole
 //     (and a share of the heads, where there are few runs), and goes over their
 //     keys and values twice, the second time from L1.  Bound by the chain of
 //     loads: place, page, rows, scale.
-//   * More: the queries go through the 16-bit caches' append kernel, keys and
+//   * Prompts (the rule stands in `append_launch`): the queries go through the 16-bit caches' append kernel, keys and
 //     values by runs, a warp a head, which holds its rows in registers between
 //     the two passes.  Bound by instructions (1.8 a cycle, 24 warps an SM), about twice those
 //     of the 16-bit append's keys and values.
@@ -18,7 +18,12 @@
 // tokens of 28 + 4 heads 8.1, 3001 of 20 + 20 heads of 80 41, 16384 of 32 + 8
 // heads 112 (3290 GB/s; the 16-bit append 71).  All by the first kernel: 16384
 // tokens 159 us; the second with four heads' keys and values a CTA 126, which computes the
-// angles twice; queries in it too 146 (registers spill).
+// angles twice; queries in it too 146 (registers spill).  Longer blocks, of which a CTA
+// takes those that begin among its 16 tokens, leave others idle and are read tile by
+// tile, twice: of 16, 64, 128 and 256 tokens, a prompt of 1000 17, 44, 75 and 135 us, 16384
+// 108, 118, 155 and 238.  Inputs off 16-byte pieces, or rotated halves that fill none, go
+// element by element through the first kernel: 1000 tokens 83 us, 3001 101, 16384 307
+// (17, 24 and 112 by pieces; the 16-bit append so 25, 40 and 227).
 #include <algorithm>
 
 #include "kernels.h"
