@@ -503,7 +503,8 @@ int xksv_kv_append(const xksv_kv* kv, const xksv_kv_append_args* args, void* str
  * caches: 2^-23, or 2^-40 of the largest weight where that is more; with block scales
  * its product with its value's scale within 2^-23, or 2^-40 of the largest weight
  * times the largest scale among the sixteen tokens of the same j / 16; scales below
- * 2^-125 of the sequence's largest may count as zero). A length that is negative or above table_cols * page_size
+ * 2^-125 of the sequence's largest may count as zero; scale * q . k without the key's
+ * scale is an FP32 number too, infinite beyond those). A length that is negative or above table_cols * page_size
  * gives zeros and -infinity, a page outside the cache counts as masked; both
  * are reported by xksv_kv_status. d_workspace: as for xksv_plan_linear, of at
  * least xksv_kv_attend_workspace(kv, seqs, q_heads, table_cols) bytes (0 for
